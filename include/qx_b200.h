@@ -84,7 +84,8 @@ QX_API qx_status qx_device_query(qx_device_info* info);
 QX_API const char* qx_last_error_string(void);
 /* Reports and clears the current device's pipeline error word: QX_STATUS_DEVICE_ERROR (and
  * a message naming the role code) if a kernel enqueued through a `_dev` entry point gave up
- * one of its bounded waits since the last report, else QX_STATUS_OK. It does not wait for
+ * one of its bounded waits, or met a key-value batch that contradicts itself, since the last
+ * report, else QX_STATUS_OK. It does not wait for
  * the GPU: synchronise the stream first. The host-pointer entry points make the same check
  * before they return. No counterpart in the reference (its kernels cannot stall). */
 QX_API qx_status qx_check_device_errors(void);
@@ -572,6 +573,149 @@ typedef struct qx_gptq_u4_source {
 } qx_gptq_u4_source;
 QX_API qx_status qx_import_gptq_u4(const qx_gptq_u4_source* source, qx_canonical_tensor* tensor,
                                    uint8_t* data_out, float* scales_out, float* zero_points_out);
+
+/* ---- between the qkv projection and the output projection of a decoder layer -----------------
+ * Rotary positions, a paged key-value cache held in 8 bits, and attention over it: what a decode or
+ * prompt step does with the outputs of qx_qgemv_qkv / qx_qgemm_fused_dev / the typed projections
+ * before qx_qgemm_prepacked runs the output projection. HOST-pointer forms take every array (cache,
+ * batch, tensors) from host memory, check all that the arrays say and return when done; `_dev` forms
+ * take device arrays and only enqueue.
+ *
+ * A view of `heads` vectors of head_dim elements for every token: element d of head h of token t is at
+ * data[t * token_stride + h * head_stride + d]. Strides count elements, so slices of a packed
+ * [token][q, k and v heads][head_dim] projection are views like any other. `type` is QX_STORAGE_*.
+ * Views that are read may have strides of zero; written ones may not overlap themselves. */
+typedef struct qx_heads {
+  void* data;
+  int type;
+  int heads;
+  long long token_stride;
+  long long head_stride;
+} qx_heads;
+
+/* Rotary positions. Pair i of a head (of rotary_dim / 2) turns by position * frequency[i] radians:
+ *   (a, b) -> amplitude * (a cos - b sin, a sin + b cos)
+ * with pairs (i, i + rotary_dim / 2) for QX_ROPE_HALVES and (2i, 2i + 1) for QX_ROPE_INTERLEAVED.
+ * Elements from rotary_dim on are passed through. The struct is plain data (no handle): fill it with
+ * qx_rope_init or by hand. */
+enum { QX_ROPE_HALVES = 0, QX_ROPE_INTERLEAVED = 1 };
+typedef struct qx_rope {
+  int rotary_dim;          /* even, 2 .. 256 */
+  int style;               /* QX_ROPE_HALVES or QX_ROPE_INTERLEAVED */
+  double amplitude;        /* 1 unless the scaling for long contexts changes it */
+  double frequency[128];   /* radians per position, one per pair */
+} qx_rope;
+/* frequency[i] = base ^ (-2 i / rotary_dim), scaled for contexts longer than the trained length:
+ *   QX_ROPE_LINEAR  every frequency / factor;
+ *   QX_ROPE_BANDS   by the turns r = trained_length * frequency / (2 pi) of a pair: r <= slow is divided by
+ *                   factor, r >= fast is kept, between them (1 - w) * frequency / factor + w * frequency with
+ *                   w = (r - slow) / (fast - slow);
+ *   QX_ROPE_RAMP    the same blend, but linear in the pair's index between the pairs that turn `fast` times
+ *                   (rounded down) and `slow` times (rounded up) over the trained length (the published YaRN
+ *                   rule), amplitude = 0.1 ln(factor) + 1 for factors above 1.
+ * `scaling` NULL or kind QX_ROPE_PLAIN: as they are. */
+enum { QX_ROPE_PLAIN = 0, QX_ROPE_LINEAR = 1, QX_ROPE_BANDS = 2, QX_ROPE_RAMP = 3 };
+typedef struct qx_rope_scaling {
+  int kind;
+  double factor;           /* > 0 */
+  double trained_length;   /* BANDS, RAMP: > 0 */
+  double slow, fast;       /* BANDS, RAMP: turns, 0 < slow < fast */
+} qx_rope_scaling;
+QX_API qx_status qx_rope_init(qx_rope* rope, int rotary_dim, int style, double base,
+                              const qx_rope_scaling* scaling);
+/* y = x rotated, for `tokens` tokens at positions[token] (any order, far ones included: angles are
+ * reduced in 64 bits, products are f32, one rounding to y's type). x and y have the same type and head
+ * count and are the same view (in place) or do not overlap. `inverse` non-zero turns the other way,
+ * which with the same amplitude is also the gradient: given dL/dy it gives dL/dx. */
+QX_API qx_status qx_rope_apply(const qx_rope* rope, const qx_heads* x, const qx_heads* y,
+                               const int64_t* positions, long long tokens, int head_dim, int inverse);
+QX_API qx_status qx_rope_apply_dev(const qx_rope* rope, const qx_heads* x, const qx_heads* y,
+                                   const int64_t* positions_dev, long long tokens, int head_dim,
+                                   int inverse, void* stream);
+
+/* The cache: blocks of block_tokens tokens; per (block, kv head) the codes of its tokens and one f32
+ * scale for the keys and one for the values, value = code * scale. Memory is the caller's. A block
+ * holds [kv_heads][block_tokens][head_dim] codes. block_tokens is 16, 32, 64 or 128; head_dim a
+ * multiple of 16, 16 .. 256; the code arrays start on 16-byte boundaries. Blocks need no initial
+ * contents: nothing behind a sequence's length is used. */
+typedef struct qx_kv_cache {
+  int8_t* k_codes;         /* [blocks][kv_heads][block_tokens][head_dim] */
+  int8_t* v_codes;
+  float* k_scales;         /* [blocks][kv_heads] */
+  float* v_scales;
+  long long blocks;
+  int kv_heads;
+  int block_tokens;
+  int head_dim;
+} qx_kv_cache;
+
+/* The sequences of one call, their tokens packed one behind the other: rows token_begin[s] ..
+ * token_begin[s+1] - 1 of q, k, v and the output are the LAST tokens of sequence s, which has
+ * lengths[s] tokens with them. Rows behind token_begin[sequences] belong to no sequence and are left
+ * as they are. token_begin NULL: every sequence has max_tokens rows. Token p of sequence s lives in
+ * cache block block_table[s * table_stride + p / block_tokens], slot p % block_tokens; sequences may
+ * share blocks that are only read. `tokens` is the number of rows of the views; max_tokens and
+ * max_length are bounds on the device arrays' contents, which size the launch: rows of one sequence,
+ * and lengths. Device arrays that contradict the bounds or the cache are never followed out of it: a
+ * sequence whose numbers do not fit is not served (its outputs are not written), the tokens of a block
+ * that the cache does not have are neither written nor seen, and qx_check_device_errors() reports
+ * QX_STATUS_DEVICE_ERROR afterwards. The host-pointer forms return QX_STATUS_INVALID_ARGUMENT. */
+typedef struct qx_kv_batch {
+  int sequences;
+  const int32_t* token_begin;   /* [sequences + 1] or NULL */
+  const int32_t* lengths;       /* [sequences] */
+  const int32_t* block_table;   /* [sequences][table_stride] */
+  long long table_stride;
+  long long tokens;
+  int max_tokens;
+  int max_length;
+} qx_kv_batch;
+
+/* Quantises the batch's keys and values into the cache. Per (block, kv head) the scale becomes
+ * s' = max(s, largest magnitude of the new elements / 127), s being the scale of the tokens that the
+ * block already holds for the sequence (nothing for a block that the call begins); if it grew, the older
+ * codes become round(code * s / s'). New codes are round(x / s'), limited to +-127. Scales are f32; both
+ * rounds are half to even of the exact quotient. A block whose s' would be below 2^-100 holds zeros. A NaN or an
+ * infinity among the new elements makes the block's scale of that head NaN, and with it all of its values.
+ * Blocks that are written belong to one sequence only.
+ *
+ * `rope` (optional, rotary_dim a multiple of 16) rotates the keys on the way, in f32 and without a
+ * rounding in between, by positions[row] or, with positions NULL, by the token's place in its sequence;
+ * `q` / `q_out` (both or neither, only with rope) rotates the queries into q_out in the same launch, as
+ * qx_rope_apply does. k and v have the cache's kv_heads; all views may have types of their own, q_out
+ * has q's type. */
+QX_API qx_status qx_kv_append(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k,
+                              const qx_heads* v, const qx_rope* rope, const int64_t* positions,
+                              const qx_heads* q, const qx_heads* q_out);
+QX_API qx_status qx_kv_append_dev(const qx_kv_cache* cache, const qx_kv_batch* batch,
+                                  const qx_heads* k, const qx_heads* v, const qx_rope* rope,
+                                  const int64_t* positions_dev, const qx_heads* q,
+                                  const qx_heads* q_out, void* stream);
+/* The values of the batch's tokens back out of the cache (the rows that qx_kv_append of the same batch
+ * wrote): code * scale, rounded once to the view's type. Either view may be NULL. */
+QX_API qx_status qx_kv_read(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k,
+                            const qx_heads* v);
+QX_API qx_status qx_kv_read_dev(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k,
+                                const qx_heads* v, void* stream);
+
+/* out = softmax(scale * q . K^T) V for every row of the batch, over the cached tokens of its sequence
+ * (append first, then attend). q and out have the same head count, a multiple of kv_heads: query head h
+ * reads kv head h / (heads / kv_heads). The query of row i of a sequence with n rows stands at position
+ * p = length - n + i: `causal` hides keys behind p, `window` > 0 hides keys at p - window and before
+ * (0: none). A row that sees no key gives zeros (and -infinity in `lse`); here, other than for append, a
+ * sequence may have more rows than tokens. `lse` (optional, f32 [tokens][heads]): ln of the sum of
+ * exp(scale * q . k) over the keys seen.
+ * Products are taken to at least the precision of q's type, sums and softmax statistics are f32; f32
+ * queries are multiplied with f32 precision. Partial results of splits over the keys live in
+ * `workspace` (NULL: the library's default one). The result bits do not depend on when CTAs run; they may on
+ * max_tokens, max_length and the number of sequences, which choose the splits. */
+QX_API qx_status qx_kv_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q,
+                                 const qx_heads* out, float* lse, float scale, int causal,
+                                 long long window);
+QX_API qx_status qx_kv_attention_dev(const qx_kv_cache* cache, const qx_kv_batch* batch,
+                                     const qx_heads* q, const qx_heads* out, float* lse_dev,
+                                     float scale, int causal, long long window,
+                                     qx_workspace* workspace, void* stream);
 
 /* ---- threading: set_num_threads / num_threads, include/quixicore_cpu/threading.h:11-12.
  * The fork-join pool is replaced by CUDA streams; these are kept so callers link. The

@@ -93,6 +93,34 @@ class DeviceInfo(C.Structure):
                 ("nvlink_uniform", C.c_int), ("peer_performance_rank", C.c_byte * 16)]
 
 
+class HeadsView(C.Structure):
+    """qx_heads of include/qx_b200.h."""
+    _fields_ = [("data", _vp), ("type", C.c_int), ("heads", C.c_int), ("token_stride", _ll), ("head_stride", _ll)]
+
+
+class RopeView(C.Structure):
+    """qx_rope of include/qx_b200.h."""
+    _fields_ = [("rotary_dim", C.c_int), ("style", C.c_int), ("amplitude", C.c_double), ("frequency", C.c_double * 128)]
+
+
+class RopeScaling(C.Structure):
+    """qx_rope_scaling of include/qx_b200.h."""
+    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("trained_length", C.c_double), ("slow", C.c_double),
+                ("fast", C.c_double)]
+
+
+class KVCacheView(C.Structure):
+    """qx_kv_cache of include/qx_b200.h."""
+    _fields_ = [("k_codes", _vp), ("v_codes", _vp), ("k_scales", _vp), ("v_scales", _vp), ("blocks", _ll),
+                ("kv_heads", C.c_int), ("block_tokens", C.c_int), ("head_dim", C.c_int)]
+
+
+class KVBatchView(C.Structure):
+    """qx_kv_batch of include/qx_b200.h."""
+    _fields_ = [("sequences", C.c_int), ("token_begin", _vp), ("lengths", _vp), ("block_table", _vp),
+                ("table_stride", _ll), ("tokens", _ll), ("max_tokens", C.c_int), ("max_length", C.c_int)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -150,6 +178,22 @@ def _load():
                                        C.POINTER(CanonicalTensorView), _vp],
         "qx_import_awq_u4": [C.POINTER(AwqU4Source), C.POINTER(CanonicalTensorView), _vp, _vp, _vp],
         "qx_import_gptq_u4": [C.POINTER(GptqU4Source), C.POINTER(CanonicalTensorView), _vp, _vp, _vp],
+        "qx_rope_init": [C.POINTER(RopeView), C.c_int, C.c_int, C.c_double, C.POINTER(RopeScaling)],
+        "qx_rope_apply": [C.POINTER(RopeView), C.POINTER(HeadsView), C.POINTER(HeadsView), _vp, _ll, C.c_int, C.c_int],
+        "qx_rope_apply_dev": [C.POINTER(RopeView), C.POINTER(HeadsView), C.POINTER(HeadsView), _vp, _ll, C.c_int,
+                              C.c_int, _vp],
+        "qx_kv_append": [C.POINTER(KVCacheView), C.POINTER(KVBatchView), C.POINTER(HeadsView), C.POINTER(HeadsView),
+                         C.POINTER(RopeView), _vp, C.POINTER(HeadsView), C.POINTER(HeadsView)],
+        "qx_kv_append_dev": [C.POINTER(KVCacheView), C.POINTER(KVBatchView), C.POINTER(HeadsView),
+                             C.POINTER(HeadsView), C.POINTER(RopeView), _vp, C.POINTER(HeadsView),
+                             C.POINTER(HeadsView), _vp],
+        "qx_kv_read": [C.POINTER(KVCacheView), C.POINTER(KVBatchView), C.POINTER(HeadsView), C.POINTER(HeadsView)],
+        "qx_kv_read_dev": [C.POINTER(KVCacheView), C.POINTER(KVBatchView), C.POINTER(HeadsView),
+                           C.POINTER(HeadsView), _vp],
+        "qx_kv_attention": [C.POINTER(KVCacheView), C.POINTER(KVBatchView), C.POINTER(HeadsView),
+                            C.POINTER(HeadsView), _vp, C.c_float, C.c_int, _ll],
+        "qx_kv_attention_dev": [C.POINTER(KVCacheView), C.POINTER(KVBatchView), C.POINTER(HeadsView),
+                                C.POINTER(HeadsView), _vp, C.c_float, C.c_int, _ll, _vp, _vp],
         "qx_peer_alloc": [_sz, C.POINTER(_vp), _vp],
         "qx_peer_open": [_vp, C.POINTER(_vp)],
         "qx_peer_close": [_vp],
@@ -606,3 +650,121 @@ def qgemm_w8a32_dev(w, ws, x, y, m, n, k, ldy=None, check_scales=False) -> int:
     ldy = n if ldy is None else ldy
     return lib.qx_qgemm_w8a32_dev(_dev(w), _dev(ws), _dev(x), y.data_ptr(), m, n, k, ldy,
                                   1 if check_scales else 0, None, _stream())
+
+
+# ---- between the qkv projection and the output projection: rotary positions, the paged 8-bit key-value
+# cache, attention over it ----
+ROPE_HALVES, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS, ROPE_RAMP = range(4)
+
+_torch_types: dict = {}
+
+
+def _storage_type(dtype) -> int:
+    if not _torch_types:
+        import torch
+        _torch_types.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    return _torch_types[dtype]
+
+
+def heads_view(t, kind=None, heads=None, token_stride=None, head_stride=None) -> HeadsView:
+    """A qx_heads over a [tokens, heads, head_dim] tensor or numpy array (uint16 bits need `kind`); the
+    elements of a head lie side by side. The arguments behind `kind` replace what the array says."""
+    if t is None:
+        return None
+    if isinstance(t, np.ndarray):
+        kind = {2: F16, 4: F32}[t.itemsize] if kind is None else kind
+        data, (st, sh, sd) = t.ctypes.data, (s // t.itemsize for s in t.strides)
+    else:
+        kind = _storage_type(t.dtype) if kind is None else kind
+        data, (st, sh, sd) = t.data_ptr(), t.stride()
+    assert sd == 1 or t.shape[2] == 1, "the elements of a head lie side by side"
+    return HeadsView(data, kind, t.shape[1] if heads is None else heads, st if token_stride is None else token_stride,
+                     sh if head_stride is None else head_stride)
+
+
+def _pointer(a):
+    if a is None:
+        return None
+    return _np(a) if isinstance(a, np.ndarray) else _dev(a)
+
+
+class Rope:
+    """Rotary positions (qx_rope): frequencies by base and an optional scaling for long contexts, a dict of
+    kind (ROPE_LINEAR, ROPE_BANDS, ROPE_RAMP), factor and, for the last two, trained, slow and fast."""
+
+    def __init__(self, rotary_dim, style=ROPE_HALVES, base=10000.0, scaling=None):
+        self.view = RopeView()
+        view = None
+        if scaling is not None:
+            view = C.byref(RopeScaling(scaling["kind"], scaling.get("factor", 1.0), scaling.get("trained", 0.0),
+                                       scaling.get("slow", 0.0), scaling.get("fast", 0.0)))
+        check(lib.qx_rope_init(C.byref(self.view), rotary_dim, style, base, view), "qx_rope_init")
+
+    # numpy arrays
+    def apply(self, x, y, positions, inverse=False, kind=None) -> int:
+        return lib.qx_rope_apply(self.view, heads_view(x, kind), heads_view(y, kind), _np(positions), x.shape[0],
+                                 x.shape[2], 1 if inverse else 0)
+
+    # device tensors, torch's current stream
+    def apply_dev(self, x, y, positions, inverse=False) -> int:
+        return lib.qx_rope_apply_dev(self.view, heads_view(x), heads_view(y), _dev(positions), x.shape[0],
+                                     x.shape[2], 1 if inverse else 0, _stream())
+
+
+class KVBatch:
+    """The sequences of a call (qx_kv_batch) over int32 arrays: lengths [sequences], block_table
+    [sequences, width], token_begin [sequences + 1] or None (max_tokens rows each). All of them tensors on the
+    device for the `_dev` calls, numpy arrays for the others; they are kept alive."""
+
+    def __init__(self, lengths, block_table, max_length, token_begin=None, tokens=None, max_tokens=1):
+        self.arrays = (lengths, block_table, token_begin)
+        sequences = lengths.shape[0]
+        self.view = KVBatchView(sequences, _pointer(token_begin), _pointer(lengths), _pointer(block_table),
+                                block_table.shape[1], sequences * max_tokens if tokens is None else tokens,
+                                max_tokens, max_length)
+
+
+class KVCache:
+    """The paged key-value cache in 8 bits (qx_kv_cache): codes [blocks, kv_heads, block_tokens, head_dim] int8
+    and scales [blocks, kv_heads] f32 of keys and values, tensors on the device or numpy arrays."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales):
+        self.arrays = (k_codes, v_codes, k_scales, v_scales)
+        blocks, heads, tokens, dim = k_codes.shape
+        self.view = KVCacheView(_pointer(k_codes), _pointer(v_codes), _pointer(k_scales), _pointer(v_scales), blocks,
+                                heads, tokens, dim)
+
+    @classmethod
+    def empty(cls, blocks, kv_heads, block_tokens, head_dim, device="cuda"):
+        import torch
+        codes = [torch.zeros(blocks, kv_heads, block_tokens, head_dim, dtype=torch.int8, device=device) for _ in "kv"]
+        return cls(*codes, *[torch.zeros(blocks, kv_heads, device=device) for _ in "kv"])
+
+    # numpy arrays
+    def append(self, batch, k, v, rope=None, q=None, q_out=None, positions=None, kind=None) -> int:
+        return lib.qx_kv_append(self.view, batch.view, heads_view(k, kind), heads_view(v, kind),
+                                None if rope is None else rope.view, _np(positions), heads_view(q, kind),
+                                heads_view(q_out, kind))
+
+    def read(self, batch, k, v, kind=None) -> int:
+        return lib.qx_kv_read(self.view, batch.view, heads_view(k, kind), heads_view(v, kind))
+
+    def attention(self, batch, q, out, scale=None, causal=True, window=0, lse=None, kind=None) -> int:
+        scale = self.view.head_dim ** -0.5 if scale is None else scale
+        return lib.qx_kv_attention(self.view, batch.view, heads_view(q, kind), heads_view(out, kind), _np(lse), scale,
+                                   1 if causal else 0, window)
+
+    # device tensors, torch's current stream
+    def append_dev(self, batch, k, v, rope=None, q=None, q_out=None, positions=None) -> int:
+        return lib.qx_kv_append_dev(self.view, batch.view, heads_view(k), heads_view(v),
+                                    None if rope is None else rope.view, _dev(positions), heads_view(q),
+                                    heads_view(q_out), _stream())
+
+    def read_dev(self, batch, k, v) -> int:
+        return lib.qx_kv_read_dev(self.view, batch.view, heads_view(k), heads_view(v), _stream())
+
+    def attention_dev(self, batch, q, out, scale=None, causal=True, window=0, lse=None, workspace=None) -> int:
+        scale = self.view.head_dim ** -0.5 if scale is None else scale
+        return lib.qx_kv_attention_dev(self.view, batch.view, heads_view(q), heads_view(out), _dev(lse), scale,
+                                       1 if causal else 0, window, workspace, _stream())

@@ -11,6 +11,7 @@
 
 #include "qx_gemv_tc.cuh"
 #include "qx_int8_gemm.cuh"
+#include "qx_kv.cuh"
 #include "qx_weights.cuh"
 
 namespace qx {
@@ -133,9 +134,14 @@ qx_status take_device_error(DeviceContext* ctx) {
   if (ctx->workspace.base != nullptr) {
     (void)cudaMemset(ctx->workspace.base, 0, kWorkspaceCounterBytes);
   }
-  char text[96];
-  std::snprintf(text, sizeof text,
-                "a kernel gave up a bounded wait (pipeline stalled, role code %d)", code);
+  char text[128];
+  if (code == kv::kErrorSequence) {
+    std::snprintf(text, sizeof text, "a batch held a sequence whose rows or length do not fit the call's bounds");
+  } else if (code == kv::kErrorBlock) {
+    std::snprintf(text, sizeof text, "a batch named a cache block that does not exist");
+  } else {
+    std::snprintf(text, sizeof text, "a kernel gave up a bounded wait (pipeline stalled, role code %d)", code);
+  }
   set_last_error_text(text);
   return QX_STATUS_DEVICE_ERROR;
 }
@@ -148,6 +154,9 @@ bool all_finite_host(const float* v, long long count) {
 }
 
 }  // namespace
+
+qx_status finish_host_call(DeviceContext* ctx) { return sync_and_check(ctx, ctx->stream); }
+
 }  // namespace qx
 
 using namespace qx;

@@ -1,0 +1,223 @@
+// Shared by the kernels between the qkv projection and the output projection: views of heads, the
+// batch of packed sequences, typed loads and stores, rotation constants.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "qx_common.cuh"
+#include "qx_sm100.cuh"
+
+namespace qx {
+namespace kv {
+
+// Codes of the error word (qx_check_device_errors) for device arrays that contradict the call.
+constexpr int kErrorFirstBatch = 64;  // from here on: the batch, not a stalled pipeline
+constexpr int kErrorSequence = 64;    // a sequence's rows or length do not fit the bounds
+constexpr int kErrorBlock = 65;       // a block id outside the cache
+
+struct Heads {
+  uint8_t* data;
+  int type;
+  int heads;
+  long long token_stride, head_stride;
+  int vector;  // 1: data and strides keep every 8th element on a 16-byte boundary
+};
+
+struct Batch {
+  const int32_t* begin;
+  const int32_t* lengths;
+  const int32_t* table;
+  long long table_stride, tokens, blocks;
+  int sequences, max_tokens, max_length;
+  int* error;
+};
+
+// Turns per position (frequency / 2 pi) instead of radians: the angle modulo a turn is then one
+// rounding away, and the half-turn functions take it from there.
+struct Rotation {
+  int rotary, interleaved;
+  float amplitude, sign;  // sign -1: the other way
+  double turns[128];
+};
+
+struct Sequence {
+  long long row;  // first row in the packed views
+  int n, length;
+};
+
+// False (and a report) where the sequence's numbers do not fit: nothing of it is touched then.
+__device__ __forceinline__ bool sequence_of(const Batch& b, int s, bool rows_are_cached, Sequence* out) {
+  const long long row = b.begin != nullptr ? b.begin[s] : static_cast<long long>(s) * b.max_tokens;
+  const long long n = b.begin != nullptr ? b.begin[s + 1] - row : b.max_tokens;
+  const int length = b.lengths[s];
+  out->row = row;
+  out->n = static_cast<int>(n);
+  out->length = length;
+  const bool fits = row >= 0 && n >= 0 && n <= b.max_tokens && row + n <= b.tokens && length >= 0 &&
+                    length <= b.max_length && (!rows_are_cached || n <= length);
+  if (!fits && threadIdx.x == 0) sm100::report_error(b.error, kErrorSequence);
+  return fits;
+}
+
+__device__ __forceinline__ float bf16_low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_high(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+__device__ __forceinline__ size_t storage_size(int type) { return type == QX_STORAGE_F32 ? 4 : 2; }
+
+__device__ __forceinline__ float load_one(const uint8_t* data, int type, long long index) {
+  if (type == QX_STORAGE_F32) return reinterpret_cast<const float*>(data)[index];
+  const uint16_t bits = reinterpret_cast<const uint16_t*>(data)[index];
+  if (type == QX_STORAGE_F16) return __half2float(__ushort_as_half(bits));
+  return __uint_as_float(static_cast<uint32_t>(bits) << 16);
+}
+__device__ __forceinline__ void store_one(uint8_t* data, int type, long long index, float v) {
+  if (type == QX_STORAGE_F32) {
+    reinterpret_cast<float*>(data)[index] = v;
+  } else if (type == QX_STORAGE_F16) {
+    reinterpret_cast<__half*>(data)[index] = __float2half_rn(v);
+  } else {
+    reinterpret_cast<__nv_bfloat16*>(data)[index] = __float2bfloat16_rn(v);
+  }
+}
+
+// Eight neighbouring elements. `vector`: the first of them is on a 16-byte boundary.
+__device__ __forceinline__ void load8(const uint8_t* data, int type, int vector, long long index, float (&v)[8]) {
+  if (!vector) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = load_one(data, type, index + i);
+    return;
+  }
+  if (type == QX_STORAGE_F32) {
+    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(data) + index);
+    const float4 a = p[0], b = p[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    return;
+  }
+  const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(data) + index);
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (type == QX_STORAGE_F16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    } else {
+      v[2 * i] = bf16_low(w[i]);
+      v[2 * i + 1] = bf16_high(w[i]);
+    }
+  }
+}
+__device__ __forceinline__ void store8(uint8_t* data, int type, int vector, long long index, const float (&v)[8]) {
+  if (!vector) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) store_one(data, type, index + i, v[i]);
+    return;
+  }
+  if (type == QX_STORAGE_F32) {
+    float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(data) + index);
+    p[0] = make_float4(v[0], v[1], v[2], v[3]);
+    p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    return;
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (type == QX_STORAGE_F16) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(data) + index) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A head is cut into units of 16 elements: two runs of eight, at first(u) and second(u), that hold eight
+// whole pairs where the unit is rotated.
+struct Unit {
+  int first, second, pair;  // pair: index of the first of the eight pairs, -1: not rotated
+};
+__device__ __forceinline__ Unit unit_of(int u, int rotary, int interleaved) {
+  if (16 * u >= rotary) return {16 * u, 16 * u + 8, -1};
+  if (interleaved) return {16 * u, 16 * u + 8, 8 * u};
+  return {8 * u, 8 * u + rotary / 2, 8 * u};
+}
+// `table`: {cos, sin} of the token's pairs, times the amplitude.
+__device__ __forceinline__ void rotate_unit(const Unit& u, int interleaved, const float2* table, float (&a)[8],
+                                            float (&b)[8]) {
+  if (u.pair < 0) return;
+  if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 s = table[u.pair + i], t = table[u.pair + 4 + i];
+      const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
+      a[2 * i] = x * s.x - y * s.y;
+      a[2 * i + 1] = x * s.y + y * s.x;
+      b[2 * i] = z * t.x - w * t.y;
+      b[2 * i + 1] = z * t.y + w * t.x;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 s = table[u.pair + i];
+      const float x = a[i], y = b[i];
+      a[i] = x * s.x - y * s.y;
+      b[i] = x * s.y + y * s.x;
+    }
+  }
+}
+// {cos, sin} of position * turns[pair], times the amplitude. The product is taken in 64 bits and brought to
+// within half a turn there: in 32 bits a position of a million has lost the angle.
+__device__ __forceinline__ float2 turn(const Rotation& r, long long position, int pair) {
+  const double t = static_cast<double>(position) * r.turns[pair];
+  float s, c;
+  sincospif(2.0f * static_cast<float>(t - rint(t)), &s, &c);
+  return make_float2(c * r.amplitude, s * r.amplitude * r.sign);
+}
+
+// ---- host side -----------------------------------------------------------------------------
+inline bool known_type(int type) { return type >= QX_STORAGE_F32 && type <= QX_STORAGE_BF16; }
+inline size_t type_bytes(int type) { return type == QX_STORAGE_F32 ? 4 : 2; }
+// Shape, type and pointer of a view; `rows` tokens of `dim` elements, written to or only read.
+qx_status check_heads(const qx_heads* view, long long rows, int dim, bool written);
+qx_status check_cache(const qx_kv_cache* cache);
+qx_status check_batch(const qx_kv_cache* cache, const qx_kv_batch* batch);
+qx_status check_rope(const qx_rope* rope, int dim);
+qx_status check_rope_call(const qx_rope* rope, const qx_heads* x, const qx_heads* y, const int64_t* positions,
+                          long long tokens, int dim);
+Heads device_heads(const qx_heads* view);
+Batch device_batch(const qx_kv_cache* cache, const qx_kv_batch* batch, int* error);
+Rotation device_rotation(const qx_rope* rope, bool inverse);
+
+// A launch that may start while the kernel in front of it on the stream still runs: the kernel waits for it
+// itself (griddepcontrol.wait) before it touches memory.
+template <class Kernel, class Params>
+qx_status launch_behind(Kernel kernel, long long grid, int threads, size_t smem, cudaStream_t stream, const Params& p) {
+  if (grid > 0x7FFFFFFFLL) {
+    set_last_error_text("the call needs more thread blocks than one launch has");
+    return QX_STATUS_INVALID_SHAPE;
+  }
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(grid));
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  QX_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p));
+  count_launch();
+  return QX_STATUS_OK;
+}
+
+}  // namespace kv
+
+// Waits for the context's stream and reports what its kernels reported (qx_api.cu).
+qx_status finish_host_call(DeviceContext* ctx);
+
+}  // namespace qx
