@@ -33,7 +33,14 @@ namespace kv {
 
 namespace {
 
+// P is held times 2^12 where it is rounded to 16 bits, so that weights down to 2^-26 keep all their bits;
+// sums of P carry the same factor.
+constexpr float kShift = 12.0f;
+
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 3, kTile = 32, kRows = 16;
+
+// Rows per sequence from which 16-bit queries take the prompt kernel.
+constexpr long long kPromptFrom = 64;
 
 template <int DP>
 struct Shape {
@@ -115,9 +122,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) attention_kernel(c
   const int head = static_cast<int>(index % p.kv_heads), s = static_cast<int>(index / p.kv_heads);
   Rows rows;
   if (!rows_of(p, s, row_tile * kRows, kRows, &rows)) return;
-  const int begin = rows.low + split * p.chunk;
-  if (split > 0 && begin >= rows.high) return;
-  const int end = min(rows.high, begin + p.chunk);
+  int begin, end;
+  if (!chunk_of(p, rows, split, &begin, &end)) return;
   const int32_t* const table = p.batch.table + s * p.batch.table_stride;
   const int tiles = (end - begin + kTile - 1) / kTile;  // (zero or less: the rows see nothing)
 
@@ -528,25 +534,25 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   __shared__ float4 shared[kThreads];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  const int r = static_cast<int>(blockIdx.x % kRows);
-  const long long tile_index = blockIdx.x / kRows;
+  const int r = static_cast<int>(blockIdx.x % p.tile_rows);
+  const long long tile_index = blockIdx.x / p.tile_rows;
   const int row_tile = static_cast<int>(tile_index % p.row_tiles);
   const int head = static_cast<int>(tile_index / p.row_tiles % p.kv_heads);
   const int s = static_cast<int>(tile_index / p.row_tiles / p.kv_heads);
   Rows rows;
-  if (!rows_of(p, s, row_tile * kRows, kRows, &rows) || r >= rows.count) return;
+  if (!rows_of(p, s, row_tile * p.tile_rows, p.tile_rows, &rows) || r >= rows.count) return;
   const int used = splits_used(p, rows);
   if (used == 1) return;
-  const long long first = tile_index * p.splits * kRows + r;  // chunk c: + c * kRows
+  const long long first = tile_index * p.splits * p.tile_rows + r;  // chunk c: + c * tile_rows
   const float2* const stats = reinterpret_cast<const float2*>(p.statistics) + first;
   const int lane = threadIdx.x & 31;
   float top = -INFINITY, sum = 0.0f;
-  for (int c = lane; c < used; c += 32) top = fmaxf(top, stats[static_cast<long long>(c) * kRows].x);
+  for (int c = lane; c < used; c += 32) top = fmaxf(top, stats[static_cast<long long>(c) * p.tile_rows].x);
 #pragma unroll
   for (int h = 16; h >= 1; h >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, h));
   const float base = top == -INFINITY ? 0.0f : top;
   for (int c = lane; c < used; c += 32) {
-    const float2 v = stats[static_cast<long long>(c) * kRows];
+    const float2 v = stats[static_cast<long long>(c) * p.tile_rows];
     sum += v.y * exp2_fast(v.x - base);
   }
 #pragma unroll
@@ -556,8 +562,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (part < parts) {
     for (int c = part; c < used; c += parts) {
-      const float weight = exp2_fast(stats[static_cast<long long>(c) * kRows].x - base);
-      const float4 x = reinterpret_cast<const float4*>(p.partial + (first + static_cast<long long>(c) * kRows) * p.dim)[at];
+      const float weight = exp2_fast(stats[static_cast<long long>(c) * p.tile_rows].x - base);
+      const float4 x = reinterpret_cast<const float4*>(p.partial + (first + static_cast<long long>(c) * p.tile_rows) * p.dim)[at];
       v.x = fmaf(x.x, weight, v.x);
       v.y = fmaf(x.y, weight, v.y);
       v.z = fmaf(x.z, weight, v.z);
@@ -585,7 +591,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   }
   if (threadIdx.x == 0 && p.lse != nullptr) {
     p.lse[(rows.row + token) * p.out.heads + out_head] =
-        sum == 0.0f ? -INFINITY : (top + log2f(sum) - kShift) * 0.69314718055994531f;
+        sum == 0.0f ? -INFINITY : (top + log2f(sum) - p.shift) * 0.69314718055994531f;
   }
 }
 
@@ -634,25 +640,29 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   p.window = static_cast<int>(std::min<long long>(window, 0x7FFFFFFF));
   p.group = q->heads / cache->kv_heads;
   const long long most_rows = static_cast<long long>(batch->max_tokens) * p.group;
-  p.row_tiles = static_cast<int>((most_rows + kRows - 1) / kRows);
+  const bool prompt = q->type != QX_STORAGE_F32 && cache->head_dim <= 128 && most_rows >= kPromptFrom;
+  p.tile_rows = prompt ? kPromptRows : kRows;
+  p.shift = prompt ? kPromptShift : kShift;
+  p.row_tiles = static_cast<int>((most_rows + p.tile_rows - 1) / p.tile_rows);
   const long long items = static_cast<long long>(batch->sequences) * cache->kv_heads * p.row_tiles;
   // Most keys that a tile can see.
   long long range = batch->max_length;
-  if (p.window > 0 && p.causal) range = std::min<long long>(range, static_cast<long long>(p.window) + kRows + 32);
-  range = (range + kTile - 1) / kTile * kTile;
+  if (p.window > 0 && p.causal) range = std::min<long long>(range, static_cast<long long>(p.window) + p.tile_rows);
+  range += 31;  // (from a multiple of 32 on)
   // Chunks: one sequence fills the card with one round of equal chunks; several, of lengths that only the
   // device knows, get four rounds of smaller ones, so that the SMs which end early take the next. No chunk is
-  // below a tile per warp: then the joining would cost more than the keys.
+  // below a tile per warp (in the prompt kernel, four tiles): then the joining would cost more than the keys.
   const int dp = cache->head_dim <= 64 ? 64 : cache->head_dim <= 128 ? 128 : 256;
-  const long long slots = static_cast<long long>(ctx->prop.multiProcessorCount) * (dp == 64 ? 4 : dp == 128 ? 2 : 1);
-  const long long wanted = batch->sequences == 1 ? std::max(1LL, slots / items) : (4 * slots + items - 1) / items;
-  const long long least = kTile * kWarps * (batch->sequences == 1 ? 1 : 2);
-  long long chunk = std::max((range + wanted - 1) / wanted, least);
-  chunk = (chunk + kTile - 1) / kTile * kTile;
+  const long long slots = static_cast<long long>(ctx->prop.multiProcessorCount) * (prompt ? 1 : dp == 64 ? 4 : dp == 128 ? 2 : 1);
+  const bool one_round = batch->sequences == 1 || prompt;
+  const long long wanted = one_round ? std::max(1LL, slots / items) : (4 * slots + items - 1) / items;
+  const long long unit = prompt ? 128 : kTile;
+  const long long least = prompt ? 512 : kTile * kWarps * (batch->sequences == 1 ? 1 : 2);
+  const long long chunk = (std::max((range + wanted - 1) / wanted, least) + unit - 1) / unit * unit;
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>(std::max(1LL, (range + chunk - 1) / chunk));
   if (p.splits > 1) {
-    const size_t rows = static_cast<size_t>(items) * p.splits * kRows;
+    const size_t rows = static_cast<size_t>(items) * p.splits * p.tile_rows;
     const size_t sums = align_up(rows * cache->head_dim * sizeof(float), 256);
     // (behind the arrival counters that other kernels keep at the workspace's start)
     QX_TRY(workspace->reserve(kWorkspaceCounterBytes + sums + rows * 2 * sizeof(float)));
@@ -662,11 +672,12 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   const long long grid = items * p.splits;
   const bool wide = q->type == QX_STORAGE_F32;
   qx_status status;
-  if (dp == 64) status = wide ? launch_streamed<64, true>(p, grid, stream) : launch_streamed<64, false>(p, grid, stream);
+  if (prompt) status = launch_prompt(p, grid, stream);
+  else if (dp == 64) status = wide ? launch_streamed<64, true>(p, grid, stream) : launch_streamed<64, false>(p, grid, stream);
   else if (dp == 128) status = wide ? launch_streamed<128, true>(p, grid, stream) : launch_streamed<128, false>(p, grid, stream);
   else status = wide ? launch_streamed<256, true>(p, grid, stream) : launch_streamed<256, false>(p, grid, stream);
   QX_TRY(status);
-  return p.splits > 1 ? launch_behind(join_kernel, items * kRows, kThreads, 0, stream, p) : QX_STATUS_OK;
+  return p.splits > 1 ? launch_behind(join_kernel, items * p.tile_rows, kThreads, 0, stream, p) : QX_STATUS_OK;
 }
 
 }  // namespace kv

@@ -19,7 +19,9 @@ struct AttentionParams {
   float scale_log2;  // scale * log2(e)
   int causal, window;
   int group;         // query heads per kv head
+  int tile_rows;     // rows of a tile
   int row_tiles, splits, chunk;
+  float shift;       // log2 of what sums of weights carry
   float* partial;    // [tile][split][rows][dim] sums, then [tile][split][rows] {maximum, sum}
   float* statistics;
 };
@@ -50,7 +52,15 @@ __device__ __forceinline__ bool rows_of(const AttentionParams& p, int s, int fir
   return true;
 }
 __device__ __forceinline__ int splits_used(const AttentionParams& p, const Rows& r) {
-  return max(1, (r.high - r.low + p.chunk - 1) / p.chunk);
+  return max(1, static_cast<int>((static_cast<long long>(r.high) - r.low + p.chunk - 1) / p.chunk));
+}
+// Keys [begin, end) of a chunk; false where there is nothing to do (chunk 0 always has: rows that see nothing).
+__device__ __forceinline__ bool chunk_of(const AttentionParams& p, const Rows& r, int split, int* begin, int* end) {
+  const long long at = r.low + static_cast<long long>(split) * p.chunk;
+  if (split > 0 && at >= r.high) return false;
+  *begin = static_cast<int>(at);
+  *end = static_cast<int>(min(static_cast<long long>(r.high), at + p.chunk));
+  return true;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -59,9 +69,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// P is held times 2^12 where it is rounded to 16 bits, so that weights down to 2^-26 keep all their bits;
-// sums of P carry the same factor.
-constexpr float kShift = 12.0f;
+// Rows per CTA of the prompt kernel (qx_attention_tc.cu), and its shift: P is held times 2^11 .. 2^15 there.
+constexpr int kPromptRows = 256;
+constexpr float kPromptShift = 11.0f;
+qx_status launch_prompt(const AttentionParams& p, long long grid, cudaStream_t stream);
 
 }  // namespace kv
 }  // namespace qx

@@ -1,0 +1,626 @@
+// Attention over the paged 8-bit cache for prompts: 16-bit queries, head sizes up to 128, many rows per
+// sequence. The tensor-core form of qx_attention.cu.
+//
+// A CTA takes 256 rows (tokens x query heads of one kv head) as two tiles of 128 and walks the keys in tiles
+// of 128. S = Q K^T and O += P V run on tcgen05.mma kind::f16 (M = 128, f32 accumulators in TMEM: S and O of
+// both row tiles, 512 columns; P takes the place of its S). Roles:
+//   warps 0-3, 4-7  softmax of row tile 0, 1: a thread owns a row, so maximum and sum need no shuffles
+//   warps 8-11      codes -> f16: global memory to registers (a tile ahead) to shared memory, in the 128-byte
+//                   swizzle; keys become a K-major operand and values an N-major one of the same layout, so
+//                   nothing is transposed
+//   warp 12         issues the MMAs: while one row tile's softmax runs, the other's products do
+//
+// The codes are exact in f16 and so are the queries, times a power of two per row (f16 loses the bits of
+// elements below 2^-32 of the row's largest). The scale of a key block multiplies the scores. The scale of a
+// value block goes into the exponent of the weights: P = 2^(s + log2 vs - m), m following the largest s +
+// log2 vs, so one f16 rounding (2^-12) holds for every mixture of scales; the sums of weights divide it out
+// again, once per 16 keys, relative to the largest scale that the row has seen. (A scale more than 2^60 below
+// that one counts as 2^-60 of it, so that no weight leaves f32's range on the way; that moves an output by 2^-53
+// of the largest value.) m only follows when it has fallen 4 behind (a factor of 16): then the row's sum and O
+// are scaled, in TMEM, by the row's own warp, which is rare after the first tiles.
+//
+// Every wait is bounded; one that runs out raises the CTA's abort flag, all roles leave their loops, MMAs
+// in flight are waited for (bounded) and TMEM is freed.
+
+#include <algorithm>
+#include <cmath>
+
+#include "qx_attention.cuh"
+#include "qx_tile_pipe.cuh"
+
+namespace qx {
+namespace kv {
+namespace {
+
+using namespace sm100;
+
+constexpr int kRowTile = 128, kKeys = 128, kGroups = kKeys / 16;
+constexpr int kSoftmaxThreads = 256, kConvertWarps = 4, kTcThreads = kSoftmaxThreads + 32 * kConvertWarps + 32;
+constexpr int kMetaStages = 4;
+static_assert(kPromptRows == 2 * kRowTile, "two tiles per CTA");
+constexpr float kBehind = 4.0f;
+constexpr float kLeastLog = -100.0f;  // of a value scale: append makes no smaller one but zero
+
+constexpr float kSpan = 60.0f;  // log2 of the largest ratio of value scales that is kept
+
+struct Group {
+  float key_scale, value_log, value_inverse;  // (2^-value_log)
+  int present;
+};
+
+struct Barriers {
+  uint64_t queries[2], key_full[2], key_empty[2], value_full[2], value_empty[2];
+  uint64_t scores[2], weights[2], sums[2], meta[kMetaStages], drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <int DP>
+struct TcShape {
+  static constexpr int kOperand = kKeys * DP * 2;  // bytes of a tile of queries, keys or values
+  static constexpr int kQueries = 0;
+  static constexpr int kKeyRing = kQueries + 2 * kOperand;
+  static constexpr int kValueRing = kKeyRing + 2 * kOperand;
+  static constexpr int kMeta = kValueRing + 2 * kOperand;
+  static constexpr int kBars = kMeta + kMetaStages * kGroups * static_cast<int>(sizeof(Group));
+  static constexpr int kBytes = kBars + static_cast<int>(sizeof(Barriers)) + 1024;  // (the operands start on 1024)
+};
+
+// D[tmem] (+)= A[tmem] * B[smem], f16 operands, f32 accumulate.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// Waits for the loads in flight and names the registers that they fill, so that nothing computed from those can
+// be moved in front of the wait.
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+// N-major operand in the 128-byte swizzle: rows (of K) of 128 bytes = 64 elements of N, groups of eight rows
+// 1024 bytes apart (stride offset), the next 64 elements of N `next` bytes on (leading offset).
+__device__ __forceinline__ uint64_t make_sw128_nmajor_desc(uint32_t smem_addr, uint32_t next) {
+  uint64_t desc = 0;
+  desc |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  desc |= static_cast<uint64_t>(next >> 4) << 16;
+  desc |= static_cast<uint64_t>(1024 >> 4) << 32;
+  desc |= static_cast<uint64_t>(1) << 46;
+  desc |= static_cast<uint64_t>(2) << 61;
+  return desc;
+}
+
+// Sixteen codes to two 16-byte pieces of f16.
+__device__ __forceinline__ void convert16(const uint4& codes, uint4* a, uint4* b) {
+  a->x = tile::convert_bytes2<false>(codes.x, 0x4140);
+  a->y = tile::convert_bytes2<false>(codes.x, 0x4342);
+  a->z = tile::convert_bytes2<false>(codes.y, 0x4140);
+  a->w = tile::convert_bytes2<false>(codes.y, 0x4342);
+  b->x = tile::convert_bytes2<false>(codes.z, 0x4140);
+  b->y = tile::convert_bytes2<false>(codes.z, 0x4342);
+  b->z = tile::convert_bytes2<false>(codes.w, 0x4140);
+  b->w = tile::convert_bytes2<false>(codes.w, 0x4342);
+}
+
+// What a softmax thread knows about its row.
+struct RowState {
+  float factor;       // of the raw scores, log2(e) in it
+  int low, high;      // keys that the row sees
+  float maximum, sum;
+  float largest_log, largest;  // value scale that it has seen, and its log2
+};
+__device__ __forceinline__ float value_log_of(const Group& g, const RowState& row) {
+  const float least = row.largest_log - kSpan;
+  return g.value_log < least ? least : g.value_log;  // (no number stays none)
+}
+
+// Takes the tile's value scales into row.largest.
+template <bool kMasked>
+__device__ __forceinline__ void see_scales(const Group* groups, RowState& row, int key0) {
+  float top = row.largest_log;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const int key = key0 + 16 * g;
+    const bool seen = !kMasked || (groups[g].present != 0 && key < row.high && key + 16 > row.low);
+    if (seen) top = fmaxf(top, groups[g].value_log);
+  }
+  if (top > row.largest_log) {
+    if (row.sum != 0.0f) row.sum *= exp2_fast(top - row.largest_log);
+    row.largest_log = top;
+    row.largest = exp2f(top);
+  }
+}
+// Largest s + log2 vs of 32 scores (two groups).
+template <bool kMasked>
+__device__ __forceinline__ float top_of(const uint32_t (&raw)[32], const Group* groups, const RowState& row, int key0) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const Group g = groups[h];
+    const float f = row.factor * g.key_scale, log = value_log_of(g, row);
+    if (!kMasked) {
+      float m = __uint_as_float(raw[16 * h]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) m = fmaxf(m, __uint_as_float(raw[16 * h + i]));
+      top = fmaxf(top, fmaf(m, f, log));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = key0 + 16 * h + i;
+        const bool seen = g.present != 0 && key >= row.low && key < row.high;
+        const float t = fmaf(__uint_as_float(raw[16 * h + i]), f, log);
+        top = fmaxf(top, seen ? t : -INFINITY);
+      }
+    }
+  }
+  return top;
+}
+// 32 scores to f16 weights, and their sum without the value scales.
+template <bool kMasked>
+__device__ __forceinline__ void weights_of(const uint32_t (&raw)[32], const Group* groups, RowState& row, float base,
+                                           int key0, uint32_t (&out)[16]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const Group g = groups[h];
+    const float f = row.factor * g.key_scale, log = value_log_of(g, row), c = log - base;
+    const unsigned long long f2 = tile::pack2(__float_as_uint(f), __float_as_uint(f));
+    const unsigned long long c2 = tile::pack2(__float_as_uint(c), __float_as_uint(c));
+    unsigned long long sum2 = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      unsigned long long t2 = c2;
+      tile::fma2(t2, tile::pack2(raw[16 * h + 2 * i], raw[16 * h + 2 * i + 1]), f2);
+      uint32_t lo, hi;
+      tile::unpack2(t2, lo, hi);
+      float a = exp2_fast(__uint_as_float(lo)), b = exp2_fast(__uint_as_float(hi));
+      if (kMasked) {  // (behind exp2: also where the arguments are no numbers)
+        const int key = key0 + 16 * h + 2 * i;
+        a = g.present != 0 && key >= row.low && key < row.high ? a : 0.0f;
+        b = g.present != 0 && key + 1 >= row.low && key + 1 < row.high ? b : 0.0f;
+      }
+      const __half2 p = __floats2half2_rn(a, b);
+      out[8 * h + i] = *reinterpret_cast<const uint32_t*>(&p);
+      sum2 = tile::addf2(sum2, tile::pack2(__float_as_uint(a), __float_as_uint(b)));
+    }
+    uint32_t lo, hi;
+    tile::unpack2(sum2, lo, hi);
+    const float sum = __uint_as_float(lo) + __uint_as_float(hi);
+    // (a group that is hidden as a whole may have a scale that is no number)
+    const float relative = log > g.value_log ? 1.1529215046068470e18f : g.value_inverse * row.largest;  // (2^60)
+    if (!kMasked || sum != 0.0f) row.sum = fmaf(sum, relative, row.sum);
+  }
+}
+
+// One tile of scores to weights, in TMEM. `scores`: this warp's lanes of S, which P replaces; `sums`: of O.
+template <int DP, bool kMasked>
+__device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, const Group* groups, RowState& row, int key0,
+                                             bool first) {
+  uint32_t a[32], b[32], p[16];
+  float top;
+  tmem_ld_32x32(scores, a);
+  see_scales<kMasked>(groups, row, key0);
+  tmem_ld_wait_for(a);
+  tmem_ld_32x32(scores + 32, b);
+  top = top_of<kMasked>(a, groups, row, key0);
+  tmem_ld_wait_for(b);
+  tmem_ld_32x32(scores + 64, a);
+  top = fmaxf(top, top_of<kMasked>(b, groups + 2, row, key0 + 32));
+  tmem_ld_wait_for(a);
+  tmem_ld_32x32(scores + 96, b);
+  top = fmaxf(top, top_of<kMasked>(a, groups + 4, row, key0 + 64));
+  tmem_ld_wait_for(b);
+  tmem_ld_32x32(scores, a);
+  top = fmaxf(top, top_of<kMasked>(b, groups + 6, row, key0 + 96));
+
+  const bool behind = top > row.maximum + kBehind;  // (from -infinity on, any score is)
+  if (__any_sync(0xFFFFFFFFu, behind)) {
+    const float before = row.maximum;
+    if (behind) row.maximum = top;
+    const float keep = before == row.maximum ? 1.0f : exp2_fast(before - row.maximum);
+    row.sum *= keep;
+    if (!first) {
+      tmem_ld_wait_for(a);
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        tmem_ld_32x32(sums + c, o);
+        tmem_ld_wait_for(o);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t half[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(__uint_as_float(o[16 * h + i]) * keep);
+          tmem_st_32x16(sums + c + 16 * h, half);
+        }
+      }
+    }
+  }
+  const float base = (row.maximum == -INFINITY ? 0.0f : row.maximum) - kPromptShift;
+  tmem_ld_wait_for(a);
+  tmem_ld_32x32(scores + 32, b);
+  weights_of<kMasked>(a, groups, row, base, key0, p);
+  tmem_ld_wait_for(b);
+  tmem_st_32x16(scores, p);
+  tmem_ld_32x32(scores + 64, a);
+  weights_of<kMasked>(b, groups + 2, row, base, key0 + 32, p);
+  tmem_ld_wait_for(a);
+  tmem_st_32x16(scores + 16, p);
+  tmem_ld_32x32(scores + 96, b);
+  weights_of<kMasked>(a, groups + 4, row, base, key0 + 64, p);
+  tmem_ld_wait_for(b);
+  tmem_st_32x16(scores + 32, p);
+  weights_of<kMasked>(b, groups + 6, row, base, key0 + 96, p);
+  tmem_st_32x16(scores + 48, p);
+  tmem_st_wait();
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_constant__ AttentionParams p) {
+  using S = TcShape<DP>;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* const smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
+  Group* const meta = reinterpret_cast<Group*>(smem + S::kMeta);
+  Barriers* const bars = reinterpret_cast<Barriers*>(smem + S::kBars);
+  volatile int* const abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  long long index = blockIdx.x;
+  const int split = static_cast<int>(index % p.splits);
+  index /= p.splits;
+  // the last rows first: with a causal mask they see the most keys
+  const int row_tile = p.row_tiles - 1 - static_cast<int>(index % p.row_tiles);
+  index /= p.row_tiles;
+  const long long tile_index = index * p.row_tiles + row_tile;
+  const int head = static_cast<int>(index % p.kv_heads), s = static_cast<int>(index / p.kv_heads);
+  Rows rows;
+  if (!rows_of(p, s, row_tile * 2 * kRowTile, 2 * kRowTile, &rows)) return;
+  int begin, end;
+  if (!chunk_of(p, rows, split, &begin, &end)) return;
+  const int tiles = max(0, (end - begin + kKeys - 1) / kKeys);
+  const int row_tiles = rows.count > kRowTile ? 2 : 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->queries[i], kRowTile);
+      mbar_init(&bars->key_full[i], kConvertWarps);
+      mbar_init(&bars->key_empty[i], 1);
+      mbar_init(&bars->value_full[i], kConvertWarps);
+      mbar_init(&bars->value_empty[i], 1);
+      mbar_init(&bars->scores[i], 1);
+      mbar_init(&bars->weights[i], 4);
+      mbar_init(&bars->sums[i], 1);
+    }
+    for (int i = 0; i < kMetaStages; ++i) mbar_init(&bars->meta[i], kConvertWarps);
+    mbar_init(&bars->drain, 1);
+    bars->abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = bars->tmem_base;
+  bool ok = true;
+
+  if (warp < 8) {
+    // ---- softmax --------------------------------------------------------------------------
+    const int which = warp >> 2;
+    if (which < row_tiles) {
+      const int r = threadIdx.x & 127, in_tile = which * kRowTile + r;
+      const bool real = in_tile < rows.count;
+      const int start = rows.length - rows.n;
+      const int token = (rows.first + in_tile) / p.group, member = (rows.first + in_tile) % p.group;
+      const long long row_at = rows.row + token, out_head = static_cast<long long>(head) * p.group + member;
+      RowState row;
+      row.low = row.high = 0;
+      row.maximum = -INFINITY;
+      row.sum = 0.0f;
+      row.largest_log = -INFINITY;
+      row.largest = 0.0f;
+      if (real) {
+        row.high = p.causal ? min(rows.length, start + token + 1) : rows.length;
+        row.low = p.window > 0 ? max(0, start + token - p.window + 1) : 0;
+      }
+      // the queries: f16 times a power of two that brings the row's largest magnitude to 2^7 .. 2^8
+      {
+        const long long from = row_at * p.q.token_stride + out_head * p.q.head_stride;
+        uint32_t top = 0;
+        float v[8];
+        if (real) {
+          for (int d = 0; d < p.dim; d += 8) {
+            load8(p.q.data, p.q.type, p.q.vector, from + d, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+          }
+        }
+        top >>= 23;
+        const int shift = top >= 255 ? 0 : min(120, max(-120, 134 - static_cast<int>(top)));
+        // (a negative scale turns the query's sign, so that larger raw scores are larger scores)
+        const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
+        row.factor = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * fabsf(p.scale_log2);
+        uint8_t* const to = smem + S::kQueries + which * S::kOperand + r * 128;
+#pragma unroll 4
+        for (int d = 0; d < DP; d += 8) {
+          uint32_t w[4] = {0, 0, 0, 0};
+          if (real && d < p.dim) {
+            load8(p.q.data, p.q.type, p.q.vector, from + d, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const __half2 h = __floats2half2_rn(v[2 * i] * up, v[2 * i + 1] * up);
+              w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+          }
+          *reinterpret_cast<uint4*>(to + d / 64 * (kRowTile * 128) + ((d / 8 & 7) ^ (r & 7)) * 16) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&bars->queries[which]);
+      }
+      // below open_high and from open_low on no row of the tile has a hidden key
+      const int last = min(rows.count, (which + 1) * kRowTile) - 1;
+      const int position0 = start + (rows.first + which * kRowTile) / p.group, position1 = start + (rows.first + last) / p.group;
+      const int open_high = p.causal ? min(rows.length, position0 + 1) : rows.length;
+      const int open_low = p.window > 0 ? max(0, position1 - p.window + 1) : 0;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t scores = tmem + lanes + which * 128, sums = tmem + lanes + 256 + which * 128;
+      for (int j = 0; ok && j < tiles; ++j) {
+        ok = mbar_wait_warp(&bars->scores[which], j & 1, abort_flag) &&
+             mbar_wait_warp(&bars->meta[j % kMetaStages], j / kMetaStages & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after_sync();
+        const Group* const groups = meta + j % kMetaStages * kGroups;
+        const int key0 = begin + j * kKeys;
+        bool open = key0 + kKeys <= open_high && key0 >= open_low;
+        if (open) {
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) open = open && groups[g].present != 0;
+        }
+        if (open) softmax_tile<DP, false>(scores, sums, groups, row, key0, j == 0);
+        else softmax_tile<DP, true>(scores, sums, groups, row, key0, j == 0);
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->weights[which]);
+      }
+      if (ok && tiles > 0) ok = mbar_wait_warp(&bars->sums[which], 0, abort_flag);
+      if (ok) {
+        tc_fence_after_sync();
+        const bool whole = splits_used(p, rows) == 1;
+        // O stands against the maximum alone, the sum against that and the largest scale
+        const float gain = row.sum == 0.0f ? 0.0f : whole ? row.largest / row.sum : row.largest;
+        const float maximum = row.sum == 0.0f ? -INFINITY : row.maximum - row.largest_log;
+        const long long at = ((tile_index * p.splits + split) * 2 * kRowTile + in_tile);
+        const long long to = row_at * p.out.token_stride + out_head * p.out.head_stride;
+#pragma unroll 1
+        for (int c = 0; c < DP && c < p.dim; c += 32) {
+          uint32_t o[32];
+          if (tiles > 0) {
+            tmem_ld_32x32(sums + c, o);
+            tmem_ld_wait_for(o);
+          }
+          if (!real) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (c + 8 * i >= p.dim) break;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = row.sum == 0.0f ? 0.0f : __uint_as_float(o[8 * i + e]) * gain;
+            if (whole) {
+              store8(p.out.data, p.out.type, p.out.vector, to + c + 8 * i, v);
+            } else {
+              float4* const partial = reinterpret_cast<float4*>(p.partial + at * p.dim + c + 8 * i);
+              partial[0] = make_float4(v[0], v[1], v[2], v[3]);
+              partial[1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
+          }
+        }
+        if (real && !whole) *reinterpret_cast<float2*>(p.statistics + 2 * at) = make_float2(maximum, row.sum);
+        if (real && whole && p.lse != nullptr) {
+          p.lse[row_at * p.out.heads + out_head] =
+              row.sum == 0.0f ? -INFINITY : (maximum + log2f(row.sum) - kPromptShift) * 0.69314718055994531f;
+        }
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        report_error(p.batch.error, 41);
+      }
+    }
+  } else if (warp < 8 + kConvertWarps) {
+    // ---- codes to operands ------------------------------------------------------------------
+    const int w = warp - 8;
+    const int32_t* const table = p.batch.table + s * p.batch.table_stride;
+    constexpr int kHalves = DP / 64;     // 64 codes of a row: one swizzled row of f16
+    constexpr int kLoads = 4 * kHalves;  // per thread and tile: 32 keys per warp, eight at a time
+    uint4 k[kLoads], v[kLoads];
+    // ids of the blocks of this warp's two groups of 16 keys; -1: nothing there
+    const auto ids_of = [&](int j, int (&id)[2]) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int key = begin + j * kKeys + 32 * w + 16 * g;
+        id[g] = -1;
+        if (j < tiles && key < end) {
+          const int block = table[key / p.block_tokens];
+          if (block >= 0 && block < p.batch.blocks) id[g] = block;
+          else if (lane == 0) report_error(p.batch.error, kErrorBlock);
+        }
+      }
+    };
+    const auto load = [&](int j, const int (&id)[2], const int8_t* codes, uint4 (&to)[kLoads]) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int slot = (begin + j * kKeys + 32 * w + 16 * g) % p.block_tokens;
+        const int8_t* const from =
+            codes + ((static_cast<long long>(max(id[g], 0)) * p.kv_heads + head) * p.block_tokens + slot) * p.dim;
+#pragma unroll
+        for (int i = 0; i < kLoads / 2; ++i) {
+          const int r = i / kHalves * 8 + (lane >> 2), d = i % kHalves * 64 + (lane & 3) * 16;
+          uint4 c = make_uint4(0, 0, 0, 0);  // (nothing there, or past the head: zeros)
+          if (id[g] >= 0 && (DP == p.dim || d < p.dim)) c = __ldg(reinterpret_cast<const uint4*>(from + r * p.dim + d));
+          to[g * kLoads / 2 + i] = c;
+        }
+      }
+    };
+    const auto store = [&](uint8_t* operand, const uint4 (&from)[kLoads]) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int i = 0; i < kLoads / 2; ++i) {
+          const int r = 32 * w + 16 * g + i / kHalves * 8 + (lane >> 2), c = (lane & 3) * 2;
+          uint8_t* const row = operand + i % kHalves * (kKeys * 128) + r * 128;
+          uint4 a, b;
+          convert16(from[g * kLoads / 2 + i], &a, &b);
+          *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = a;
+          *reinterpret_cast<uint4*>(row + (((c + 1) ^ (r & 7)) << 4)) = b;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    };
+    float scales[2] = {0.0f, 0.0f};  // of lane 0, 1: its group's
+    const auto load_scales = [&](const int (&id)[2]) {
+      const int own = lane == 1 ? id[1] : id[0];
+      if (lane < 2 && own >= 0) {
+        const long long slice = static_cast<long long>(own) * p.kv_heads + head;
+        scales[0] = p.k_scales[slice];
+        scales[1] = p.v_scales[slice];
+      }
+    };
+    int id[2], next[2];
+    ids_of(0, id);
+    load(0, id, p.k_codes, k);
+    load_scales(id);
+    load(0, id, p.v_codes, v);
+    ids_of(1, next);
+    for (int j = 0; ok && j < tiles; ++j) {
+      const int stage = j & 1;
+      if (j >= 2) ok = mbar_wait_warp(&bars->key_empty[stage], ((j >> 1) - 1) & 1, abort_flag);
+      if (!ok) break;
+      if (lane < 2) {
+        const float vs = scales[1];
+        const float log = vs < 7.8886090522101181e-31f ? kLeastLog : log2f(vs);  // (2^-100; no number stays none)
+        meta[j % kMetaStages * kGroups + 2 * w + lane] =
+            Group{scales[0], log, exp2f(-log), (lane == 1 ? id[1] : id[0]) >= 0};
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->meta[j % kMetaStages]);
+      store(smem + S::kKeyRing + stage * S::kOperand, k);
+      if (lane == 0) mbar_arrive(&bars->key_full[stage]);
+      if (j + 1 < tiles) {
+        load(j + 1, next, p.k_codes, k);
+        load_scales(next);
+      }
+      if (j >= 2) ok = mbar_wait_warp(&bars->value_empty[stage], ((j >> 1) - 1) & 1, abort_flag);
+      if (!ok) break;
+      store(smem + S::kValueRing + stage * S::kOperand, v);
+      if (lane == 0) mbar_arrive(&bars->value_full[stage]);
+      if (j + 1 < tiles) load(j + 1, next, p.v_codes, v);
+      id[0] = next[0];
+      id[1] = next[1];
+      ids_of(j + 2, next);
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      report_error(p.batch.error, 42);
+    }
+  } else if (elect_one()) {
+    // ---- MMAs -------------------------------------------------------------------------------
+    const uint32_t shape = (1u << 4) | (static_cast<uint32_t>(kRowTile >> 4) << 24);
+    const uint32_t scores_desc = shape | (static_cast<uint32_t>(kKeys >> 3) << 17);
+    const uint32_t sums_desc = shape | (static_cast<uint32_t>(DP >> 3) << 17) | (1u << 16);  // (B is N-major)
+    const uint32_t base = smem_u32(smem);
+    const auto scores_of = [&](int which, int stage) {
+#pragma unroll
+      for (int d = 0; d < DP; d += 16) {
+        const uint32_t at = d / 64 * (kRowTile * 128) + d % 64 * 2;
+        mma_f16_ss(tmem + which * 128, make_sw128_kmajor_desc(base + S::kQueries + which * S::kOperand + at),
+                   make_sw128_kmajor_desc(base + S::kKeyRing + stage * S::kOperand + at), scores_desc, d > 0);
+      }
+      tc_commit(&bars->scores[which]);
+    };
+    for (int i = 0; ok && i < row_tiles; ++i) ok = mbar_wait(&bars->queries[i], 0, abort_flag);
+    if (ok && tiles > 0) ok = mbar_wait(&bars->key_full[0], 0, abort_flag);
+    tc_fence_after_sync();
+    if (ok && tiles > 0) {
+      for (int i = 0; i < row_tiles; ++i) scores_of(i, 0);
+      tc_commit(&bars->key_empty[0]);
+    }
+    for (int j = 0; ok && j < tiles; ++j) {
+      const int stage = j & 1, after = (j + 1) & 1;
+      for (int i = 0; ok && i < row_tiles; ++i) {
+        if (i == 0) ok = mbar_wait(&bars->value_full[stage], j >> 1 & 1, abort_flag);
+        ok = ok && mbar_wait(&bars->weights[i], j & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after_sync();
+#pragma unroll
+        for (int t = 0; t < kKeys; t += 16) {
+          mma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + t / 2,
+                     make_sw128_nmajor_desc(base + S::kValueRing + stage * S::kOperand + t * 128, kKeys * 128), sums_desc,
+                     j > 0 || t > 0);
+        }
+        if (j + 1 == tiles) {
+          tc_commit(&bars->sums[i]);
+          continue;
+        }
+        if (i == 0) ok = mbar_wait(&bars->key_full[after], (j + 1) >> 1 & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after_sync();
+        scores_of(i, after);
+      }
+      if (!ok) break;
+      tc_commit(&bars->value_empty[stage]);
+      if (j + 1 < tiles) tc_commit(&bars->key_empty[after]);
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      report_error(p.batch.error, 43);
+      tc_commit(&bars->drain);  // what is in flight ends before TMEM is freed
+      const unsigned long long started = global_timer_ns();
+      while (!mbar_try_wait(&bars->drain, 0) && global_timer_ns() - started < kWaitLimitNs) {
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int DP>
+qx_status launch_prompt_of(const AttentionParams& p, long long grid, cudaStream_t stream) {
+  static SmemOptIn opt_in;
+  QX_TRY(opt_in.ensure(prompt_kernel<DP>, TcShape<DP>::kBytes));
+  return launch_behind(prompt_kernel<DP>, grid, kTcThreads, TcShape<DP>::kBytes, stream, p);
+}
+
+}  // namespace
+
+qx_status launch_prompt(const AttentionParams& p, long long grid, cudaStream_t stream) {
+  return p.dim <= 64 ? launch_prompt_of<64>(p, grid, stream) : launch_prompt_of<128>(p, grid, stream);
+}
+
+}  // namespace kv
+}  // namespace qx

@@ -109,7 +109,10 @@ def attention_tolerance(out, lse, magnitude, spread, dtype, dim, length):
       a score that is off by d takes d of its weight with it, and d of the sum: 2 d;
       weights are rounded to f16 (2^-12 of each, the values are exact) or, for f32, to 22 bits, and to no less than
                the smallest step of f16, 2^-24, held times 2^12 against the row's largest weight: half of that,
-               2^-37, of every value seen, however small its weight (the sum of weights is the largest one or more);
+               2^-37, of every value seen, however small its weight (the sum of weights is the largest one or more).
+               Long prompts of 16-bit queries hold weight times value scale times 2^11, against the largest such
+               product: 2^-36 of every code under the largest scale seen, with value scales that are within a
+               factor of eight of each other (as they are where this is called) 2^-33 of every value;
       sums of at most `length` weights and of the tiles, each addition u: (length / 32 + 64) u of the magnitudes;
       one rounding to the output's type."""
     u = 2.0 ** -23
@@ -117,5 +120,6 @@ def attention_tolerance(out, lse, magnitude, spread, dtype, dim, length):
     rounded = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -12
     sums = (length / 32 + 64) * u
     weighted, plain = magnitude
-    return (HALF_STEP[dtype] * out.abs() + (2 * score + rounded + sums)[..., None] * weighted + 2.0 ** -37 * plain + 1e-37,
+    smallest = 2.0 ** -37 if dtype == torch.float32 else 2.0 ** -33
+    return (HALF_STEP[dtype] * out.abs() + (2 * score + rounded + sums)[..., None] * weighted + smallest * plain + 1e-37,
             score + sums + 2 * u * lse.abs())

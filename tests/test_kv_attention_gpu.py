@@ -104,6 +104,53 @@ def test_prompts(qx, dtype, dim, group):
     check(qx, cache, on_device(qx, cache), table, lengths, new, typed((sum(new) + 1, 2 * group, dim), dtype, 5), behind=1)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,size,group,new", [(128, 16, 8, 100), (64, 128, 2, 300), (16, 32, 1, 70), (112, 64, 3, 257)])
+@pytest.mark.parametrize("window", [0, 900])
+def test_chunks_of_a_prompt_behind_a_long_prefix(qx, dtype, dim, size, group, new, window):
+    """Few row tiles and many keys: the keys are split among CTAs and joined."""
+    width = -(-6100 // size)
+    cache, table = filled(width, 1, size, dim), table_of(1, width, width)
+    dev = on_device(qx, cache)
+    for length in (6100, 2049, 513 + new):
+        check(qx, cache, dev, table, [length], [new], typed((new, group, dim), dtype, length), True, window)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [63, 64, 65, 127, 128, 129, 255, 256, 257, 513])
+def test_tiles_of_rows(qx, dtype, rows):
+    """Row counts at and around the tiles, one query head per kv head, prompts of exactly that length and longer."""
+    cache, table = filled(30, 2, 64, 64), table_of(2, 15, 30)
+    check(qx, cache, on_device(qx, cache), table, [rows, rows + 130], [rows, rows - 60], typed((2 * rows - 60, 2, 64), dtype, rows))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, 2.0])
+def test_scales_of_a_prompts_scores(qx, scale):
+    cache, table = filled(10, 2, 32, 64), table_of(1, 10, 10)
+    check(qx, cache, on_device(qx, cache), table, [310], [310], typed((310, 2, 64), BF16, 9), scale=scale)
+
+
+def test_value_scales_far_apart_in_a_prompt(qx):
+    """Blocks whose value scales differ by 2^40, are zero or lie under the smallest that append makes: the weights
+    carry them, so the tolerance goes by the largest scale of the keys that a row sees."""
+    size, n = 16, 150
+    cache, table = filled(10, 1, size, 64), table_of(1, 10, 10)
+    for block, factor in ((0, 2.0 ** -40), (2, 0.0), (3, 2.0 ** 20), (5, 2.0 ** -110), (7, 2.0 ** 45)):
+        cache.scales[1][table[0, block]] *= np.float32(factor)
+    cache.scales[0][table[0, 4]] = 0.0
+    dev, q = on_device(qx, cache), typed((n, 2, 64), BF16, 4)
+    batch, _, _ = batch_of(qx, table, [n], [n])
+    out = torch.empty(n, 2, 64, dtype=BF16, device="cuda")
+    assert dev.attention_dev(batch, q.cuda(), out) == qx.OK
+    k, v = (torch.from_numpy(cache.values(i, table[0], n)) for i in range(2))
+    want, sums, magnitude, spread = attention(q.double(), k, v, 0.125, True, 0)
+    limit, _ = attention_tolerance(want, sums, magnitude, spread, BF16, 64, n)
+    scales = torch.from_numpy(cache.scales[1][table[0, np.arange(n) // size], 0].astype(np.float64))
+    largest = torch.cummax(scales, 0).values  # of the keys up to each row
+    limit = limit + ((2.0 ** -36 + 2.0 ** -60) * 127 * n * largest)[:, None, None]
+    assert float(((out.cpu().double() - want).abs() / limit).max()) <= 1
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_scales_of_scores(qx, dtype):
     """Peaked, flat, negative and zero scores' scales."""
