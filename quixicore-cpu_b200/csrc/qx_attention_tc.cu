@@ -9,6 +9,8 @@
 //                   swizzle; keys become a K-major operand and values an N-major one of the same layout, so
 //                   nothing is transposed
 //   warp 12         issues the MMAs: while one row tile's softmax runs, the other's products do
+// (warps 13-15 fill up the last warpgroup: registers move by warpgroups, 192 to a softmax thread, which holds a
+// whole row of S, and 64 to the others.)
 //
 // The codes are exact in f16 and so are the queries, times a power of two per row (f16 loses the bits of
 // elements below 2^-32 of the row's largest). The scale of a key block multiplies the scores. The scale of a
@@ -35,7 +37,8 @@ namespace {
 using namespace sm100;
 
 constexpr int kRowTile = 128, kKeys = 128, kGroups = kKeys / 16;
-constexpr int kSoftmaxThreads = 256, kConvertWarps = 4, kTcThreads = kSoftmaxThreads + 32 * kConvertWarps + 32;
+constexpr int kConvertWarps = 4, kTcThreads = 512;
+constexpr int kSoftmaxRegisters = 192, kOtherRegisters = 64;  // of 128 at launch: 256 * 192 + 256 * 64 = 512 * 128
 constexpr int kMetaStages = 4;
 static_assert(kPromptRows == 2 * kRowTile, "two tiles per CTA");
 constexpr float kBehind = 4.0f;
@@ -95,6 +98,13 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
                :
                : "memory");
 }
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
 // N-major operand in the 128-byte swizzle: rows (of K) of 128 bytes = 64 elements of N, groups of eight rows
 // 1024 bytes apart (stride offset), the next 64 elements of N `next` bytes on (leading offset).
 __device__ __forceinline__ uint64_t make_sw128_nmajor_desc(uint32_t smem_addr, uint32_t next) {
@@ -105,6 +115,17 @@ __device__ __forceinline__ uint64_t make_sw128_nmajor_desc(uint32_t smem_addr, u
   desc |= static_cast<uint64_t>(1) << 46;
   desc |= static_cast<uint64_t>(2) << 61;
   return desc;
+}
+
+__device__ __forceinline__ unsigned long long fmaf2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float v;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
 }
 
 // Sixteen codes to two 16-byte pieces of f16.
@@ -119,6 +140,13 @@ __device__ __forceinline__ void convert16(const uint4& codes, uint4* a, uint4* b
   b->w = tile::convert_bytes2<false>(codes.w, 0x4342);
 }
 
+// Eight neighbouring 16-bit elements as they are.
+__device__ __forceinline__ uint4 load8_raw(const uint8_t* data, int vector, long long index) {
+  const uint16_t* const from = reinterpret_cast<const uint16_t*>(data) + index;
+  if (vector) return *reinterpret_cast<const uint4*>(from);
+  return make_uint4(from[0] | from[1] << 16, from[2] | from[3] << 16, from[4] | from[5] << 16, from[6] | from[7] << 16);
+}
+
 // What a softmax thread knows about its row.
 struct RowState {
   float factor;       // of the raw scores, log2(e) in it
@@ -126,108 +154,59 @@ struct RowState {
   float maximum, sum;
   float largest_log, largest;  // value scale that it has seen, and its log2
 };
-__device__ __forceinline__ float value_log_of(const Group& g, const RowState& row) {
-  const float least = row.largest_log - kSpan;
-  return g.value_log < least ? least : g.value_log;  // (no number stays none)
-}
 
-// Takes the tile's value scales into row.largest.
-template <bool kMasked>
-__device__ __forceinline__ void see_scales(const Group* groups, RowState& row, int key0) {
-  float top = row.largest_log;
-#pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    const int key = key0 + 16 * g;
-    const bool seen = !kMasked || (groups[g].present != 0 && key < row.high && key + 16 > row.low);
-    if (seen) top = fmaxf(top, groups[g].value_log);
-  }
-  if (top > row.largest_log) {
-    if (row.sum != 0.0f) row.sum *= exp2_fast(top - row.largest_log);
-    row.largest_log = top;
-    row.largest = exp2f(top);
-  }
-}
-// Largest s + log2 vs of 32 scores (two groups).
-template <bool kMasked>
-__device__ __forceinline__ float top_of(const uint32_t (&raw)[32], const Group* groups, const RowState& row, int key0) {
-  float top = -INFINITY;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const Group g = groups[h];
-    const float f = row.factor * g.key_scale, log = value_log_of(g, row);
-    if (!kMasked) {
-      float m = __uint_as_float(raw[16 * h]);
-#pragma unroll
-      for (int i = 1; i < 16; ++i) m = fmaxf(m, __uint_as_float(raw[16 * h + i]));
-      top = fmaxf(top, fmaf(m, f, log));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = key0 + 16 * h + i;
-        const bool seen = g.present != 0 && key >= row.low && key < row.high;
-        const float t = fmaf(__uint_as_float(raw[16 * h + i]), f, log);
-        top = fmaxf(top, seen ? t : -INFINITY);
-      }
-    }
-  }
-  return top;
-}
-// 32 scores to f16 weights, and their sum without the value scales.
-template <bool kMasked>
-__device__ __forceinline__ void weights_of(const uint32_t (&raw)[32], const Group* groups, RowState& row, float base,
-                                           int key0, uint32_t (&out)[16]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const Group g = groups[h];
-    const float f = row.factor * g.key_scale, log = value_log_of(g, row), c = log - base;
-    const unsigned long long f2 = tile::pack2(__float_as_uint(f), __float_as_uint(f));
-    const unsigned long long c2 = tile::pack2(__float_as_uint(c), __float_as_uint(c));
-    unsigned long long sum2 = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      unsigned long long t2 = c2;
-      tile::fma2(t2, tile::pack2(raw[16 * h + 2 * i], raw[16 * h + 2 * i + 1]), f2);
-      uint32_t lo, hi;
-      tile::unpack2(t2, lo, hi);
-      float a = exp2_fast(__uint_as_float(lo)), b = exp2_fast(__uint_as_float(hi));
-      if (kMasked) {  // (behind exp2: also where the arguments are no numbers)
-        const int key = key0 + 16 * h + 2 * i;
-        a = g.present != 0 && key >= row.low && key < row.high ? a : 0.0f;
-        b = g.present != 0 && key + 1 >= row.low && key + 1 < row.high ? b : 0.0f;
-      }
-      const __half2 p = __floats2half2_rn(a, b);
-      out[8 * h + i] = *reinterpret_cast<const uint32_t*>(&p);
-      sum2 = tile::addf2(sum2, tile::pack2(__float_as_uint(a), __float_as_uint(b)));
-    }
-    uint32_t lo, hi;
-    tile::unpack2(sum2, lo, hi);
-    const float sum = __uint_as_float(lo) + __uint_as_float(hi);
-    // (a group that is hidden as a whole may have a scale that is no number)
-    const float relative = log > g.value_log ? 1.1529215046068470e18f : g.value_inverse * row.largest;  // (2^60)
-    if (!kMasked || sum != 0.0f) row.sum = fmaf(sum, relative, row.sum);
-  }
-}
-
-// One tile of scores to weights, in TMEM. `scores`: this warp's lanes of S, which P replaces; `sums`: of O.
-template <int DP, bool kMasked>
+// One tile of scores to weights, in TMEM. `scores`: this warp's lanes of S, which P replaces; `sums`: of O. Keys
+// share scales by `kUnit`s of 16 or 32.
+template <int DP, int kUnit, bool kMasked>
 __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, const Group* groups, RowState& row, int key0,
                                              bool first) {
-  uint32_t a[32], b[32], p[16];
-  float top;
-  tmem_ld_32x32(scores, a);
-  see_scales<kMasked>(groups, row, key0);
-  tmem_ld_wait_for(a);
-  tmem_ld_32x32(scores + 32, b);
-  top = top_of<kMasked>(a, groups, row, key0);
-  tmem_ld_wait_for(b);
-  tmem_ld_32x32(scores + 64, a);
-  top = fmaxf(top, top_of<kMasked>(b, groups + 2, row, key0 + 32));
-  tmem_ld_wait_for(a);
-  tmem_ld_32x32(scores + 96, b);
-  top = fmaxf(top, top_of<kMasked>(a, groups + 4, row, key0 + 64));
-  tmem_ld_wait_for(b);
-  tmem_ld_32x32(scores, a);
-  top = fmaxf(top, top_of<kMasked>(b, groups + 6, row, key0 + 96));
+  constexpr int kUnits = kKeys / kUnit;
+  uint32_t s[4][32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld_32x32(scores + 32 * c, s[c]);
+
+  float factor[kUnits], log[kUnits];
+  float largest = row.largest_log;
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const Group g = groups[u * (kUnit / 16)];
+    factor[u] = row.factor * g.key_scale;
+    log[u] = g.value_log;
+    const int key = key0 + kUnit * u;
+    const bool seen = !kMasked || (g.present != 0 && key < row.high && key + kUnit > row.low);
+    largest = fmaxf(largest, seen ? log[u] : -INFINITY);
+  }
+  if (largest > row.largest_log) {
+    if (row.sum != 0.0f) row.sum *= exp2_fast(largest - row.largest_log);
+    row.largest_log = largest;
+    row.largest = exp2f(largest);
+  }
+  const float least = largest - kSpan;
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) log[u] = log[u] < least ? least : log[u];  // (no number stays none)
+
+  const auto hidden = [&](int key) { return key < row.low || key >= row.high; };
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld_wait_for(s[c]);
+  float top = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const bool present = !kMasked || groups[u * (kUnit / 16)].present != 0;
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kUnit; i += 2) {
+      const int at = kUnit * u + i;
+      const float a = __uint_as_float(s[at / 32][at % 32]), b = __uint_as_float(s[at / 32][at % 32 + 1]);
+      if (!kMasked) {
+        m = max3(m, a, b);
+      } else {
+        if (present && !hidden(key0 + at)) m = fmaxf(m, a);
+        if (present && !hidden(key0 + at + 1)) m = fmaxf(m, b);
+      }
+    }
+    // (nothing seen: -infinity times a factor that may be zero or no number)
+    top = fmaxf(top, kMasked && m == -INFINITY ? -INFINITY : fmaf(m, factor[u], log[u]));
+  }
 
   const bool behind = top > row.maximum + kBehind;  // (from -infinity on, any score is)
   if (__any_sync(0xFFFFFFFFu, behind)) {
@@ -236,42 +215,57 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
     const float keep = before == row.maximum ? 1.0f : exp2_fast(before - row.maximum);
     row.sum *= keep;
     if (!first) {
-      tmem_ld_wait_for(a);
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        tmem_ld_32x32(sums + c, o);
+      for (int c = 0; c < DP; c += 16) {
+        uint32_t o[16];
+        tmem_ld_32x16(sums + c, o);
         tmem_ld_wait_for(o);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t half[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(__uint_as_float(o[16 * h + i]) * keep);
-          tmem_st_32x16(sums + c + 16 * h, half);
-        }
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+        tmem_st_32x16(sums + c, o);
       }
     }
   }
   const float base = (row.maximum == -INFINITY ? 0.0f : row.maximum) - kPromptShift;
-  tmem_ld_wait_for(a);
-  tmem_ld_32x32(scores + 32, b);
-  weights_of<kMasked>(a, groups, row, base, key0, p);
-  tmem_ld_wait_for(b);
-  tmem_st_32x16(scores, p);
-  tmem_ld_32x32(scores + 64, a);
-  weights_of<kMasked>(b, groups + 2, row, base, key0 + 32, p);
-  tmem_ld_wait_for(a);
-  tmem_st_32x16(scores + 16, p);
-  tmem_ld_32x32(scores + 96, b);
-  weights_of<kMasked>(a, groups + 4, row, base, key0 + 64, p);
-  tmem_ld_wait_for(b);
-  tmem_st_32x16(scores + 32, p);
-  weights_of<kMasked>(b, groups + 6, row, base, key0 + 96, p);
-  tmem_st_32x16(scores + 48, p);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t p[16];
+#pragma unroll
+    for (int h = 0; h < 32 / kUnit; ++h) {
+      const int u = c * (32 / kUnit) + h;
+      const float add = log[u] - base;
+      const unsigned long long f2 = tile::pack2(__float_as_uint(factor[u]), __float_as_uint(factor[u]));
+      const unsigned long long c2 = tile::pack2(__float_as_uint(add), __float_as_uint(add));
+      const Group g = groups[u * (kUnit / 16)];
+      unsigned long long sum2 = 0;
+#pragma unroll
+      for (int i = 0; i < kUnit; i += 2) {
+        const int at = kUnit * h + i;
+        const unsigned long long t2 = fmaf2(tile::pack2(s[c][at], s[c][at + 1]), f2, c2);
+        uint32_t lo, hi;
+        tile::unpack2(t2, lo, hi);
+        float a = exp2_fast(__uint_as_float(lo)), b = exp2_fast(__uint_as_float(hi));
+        if (kMasked) {  // (behind exp2: also where the arguments are no numbers)
+          a = g.present == 0 || hidden(key0 + 32 * c + at) ? 0.0f : a;
+          b = g.present == 0 || hidden(key0 + 32 * c + at + 1) ? 0.0f : b;
+        }
+        const __half2 w = __floats2half2_rn(a, b);
+        p[at / 2] = *reinterpret_cast<const uint32_t*>(&w);
+        sum2 = tile::addf2(sum2, tile::pack2(__float_as_uint(a), __float_as_uint(b)));
+      }
+      uint32_t lo, hi;
+      tile::unpack2(sum2, lo, hi);
+      const float sum = __uint_as_float(lo) + __uint_as_float(hi);
+      const float relative = log[u] > g.value_log ? 1.1529215046068470e18f : g.value_inverse * row.largest;  // (2^60)
+      // (a unit that is hidden as a whole may have a scale that is no number)
+      if (!kMasked || sum != 0.0f) row.sum = fmaf(sum, relative, row.sum);
+    }
+    tmem_st_32x16(scores + 16 * c, p);
+  }
   tmem_st_wait();
 }
 
-template <int DP>
+template <int DP, int kUnit>
 __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_constant__ AttentionParams p) {
   using S = TcShape<DP>;
   extern __shared__ uint8_t raw_smem[];
@@ -326,6 +320,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
 
   if (warp < 8) {
     // ---- softmax --------------------------------------------------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
     const int which = warp >> 2;
     if (which < row_tiles) {
       const int r = threadIdx.x & 127, in_tile = which * kRowTile + r;
@@ -346,33 +341,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       // the queries: f16 times a power of two that brings the row's largest magnitude to 2^7 .. 2^8
       {
         const long long from = row_at * p.q.token_stride + out_head * p.q.head_stride;
-        uint32_t top = 0;
-        float v[8];
-        if (real) {
-          for (int d = 0; d < p.dim; d += 8) {
-            load8(p.q.data, p.q.type, p.q.vector, from + d, v);
+        // the whole row in registers: all of its loads are in flight at once
+        uint4 raw[DP / 8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-          }
+        for (int c = 0; c < DP / 8; ++c) {
+          raw[c] = make_uint4(0, 0, 0, 0);
+          if (real && 8 * c < p.dim) raw[c] = load8_raw(p.q.data, p.q.vector, from + 8 * c);
         }
-        top >>= 23;
+        const bool f16 = p.q.type == QX_STORAGE_F16;
+        const auto pair = [&](uint32_t w) {
+          return f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w)) : make_float2(bf16_low(w), bf16_high(w));
+        };
+        uint32_t top = 0;  // of the bit patterns without sign: they grow with the magnitude
+#pragma unroll
+        for (int c = 0; c < DP / 8; ++c) {
+          const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7FFFu, w[i] >> 16 & 0x7FFFu));
+        }
+        top = __float_as_uint(pair(top).x) >> 23;
         const int shift = top >= 255 ? 0 : min(120, max(-120, 134 - static_cast<int>(top)));
         // (a negative scale turns the query's sign, so that larger raw scores are larger scores)
         const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
         row.factor = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * fabsf(p.scale_log2);
         uint8_t* const to = smem + S::kQueries + which * S::kOperand + r * 128;
-#pragma unroll 4
-        for (int d = 0; d < DP; d += 8) {
-          uint32_t w[4] = {0, 0, 0, 0};
-          if (real && d < p.dim) {
-            load8(p.q.data, p.q.type, p.q.vector, from + d, v);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const __half2 h = __floats2half2_rn(v[2 * i] * up, v[2 * i + 1] * up);
-              w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
+        for (int c = 0; c < DP / 8; ++c) {
+          uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = pair(w[i]);
+            const __half2 h = __floats2half2_rn(v.x * up, v.y * up);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
           }
-          *reinterpret_cast<uint4*>(to + d / 64 * (kRowTile * 128) + ((d / 8 & 7) ^ (r & 7)) * 16) =
+          *reinterpret_cast<uint4*>(to + c / 8 * (kRowTile * 128) + ((c & 7) ^ (r & 7)) * 16) =
               make_uint4(w[0], w[1], w[2], w[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -389,6 +391,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         ok = mbar_wait_warp(&bars->scores[which], j & 1, abort_flag) &&
              mbar_wait_warp(&bars->meta[j % kMetaStages], j / kMetaStages & 1, abort_flag);
         if (!ok) break;
+        __syncwarp();
         tc_fence_after_sync();
         const Group* const groups = meta + j % kMetaStages * kGroups;
         const int key0 = begin + j * kKeys;
@@ -397,8 +400,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
 #pragma unroll
           for (int g = 0; g < kGroups; ++g) open = open && groups[g].present != 0;
         }
-        if (open) softmax_tile<DP, false>(scores, sums, groups, row, key0, j == 0);
-        else softmax_tile<DP, true>(scores, sums, groups, row, key0, j == 0);
+        if (__all_sync(0xFFFFFFFFu, open)) softmax_tile<DP, kUnit, false>(scores, sums, groups, row, key0, j == 0);
+        else softmax_tile<DP, kUnit, true>(scores, sums, groups, row, key0, j == 0);
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->weights[which]);
@@ -448,11 +451,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
     }
   } else if (warp < 8 + kConvertWarps) {
     // ---- codes to operands ------------------------------------------------------------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     const int w = warp - 8;
     const int32_t* const table = p.batch.table + s * p.batch.table_stride;
     constexpr int kHalves = DP / 64;     // 64 codes of a row: one swizzled row of f16
     constexpr int kLoads = 4 * kHalves;  // per thread and tile: 32 keys per warp, eight at a time
-    uint4 k[kLoads], v[kLoads];
+    uint4 codes[kLoads];  // of one operand: the next to be stored
     // ids of the blocks of this warp's two groups of 16 keys; -1: nothing there
     const auto ids_of = [&](int j, int (&id)[2]) {
 #pragma unroll
@@ -466,22 +470,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         }
       }
     };
-    const auto load = [&](int j, const int (&id)[2], const int8_t* codes, uint4 (&to)[kLoads]) {
+    const auto load = [&](int j, const int (&id)[2], const int8_t* plane) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const int slot = (begin + j * kKeys + 32 * w + 16 * g) % p.block_tokens;
         const int8_t* const from =
-            codes + ((static_cast<long long>(max(id[g], 0)) * p.kv_heads + head) * p.block_tokens + slot) * p.dim;
+            plane + ((static_cast<long long>(max(id[g], 0)) * p.kv_heads + head) * p.block_tokens + slot) * p.dim;
 #pragma unroll
         for (int i = 0; i < kLoads / 2; ++i) {
           const int r = i / kHalves * 8 + (lane >> 2), d = i % kHalves * 64 + (lane & 3) * 16;
           uint4 c = make_uint4(0, 0, 0, 0);  // (nothing there, or past the head: zeros)
           if (id[g] >= 0 && (DP == p.dim || d < p.dim)) c = __ldg(reinterpret_cast<const uint4*>(from + r * p.dim + d));
-          to[g * kLoads / 2 + i] = c;
+          codes[g * kLoads / 2 + i] = c;
         }
       }
     };
-    const auto store = [&](uint8_t* operand, const uint4 (&from)[kLoads]) {
+    const auto store = [&](uint8_t* operand) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
 #pragma unroll
@@ -489,7 +493,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
           const int r = 32 * w + 16 * g + i / kHalves * 8 + (lane >> 2), c = (lane & 3) * 2;
           uint8_t* const row = operand + i % kHalves * (kKeys * 128) + r * 128;
           uint4 a, b;
-          convert16(from[g * kLoads / 2 + i], &a, &b);
+          convert16(codes[g * kLoads / 2 + i], &a, &b);
           *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = a;
           *reinterpret_cast<uint4*>(row + (((c + 1) ^ (r & 7)) << 4)) = b;
         }
@@ -508,9 +512,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
     };
     int id[2], next[2];
     ids_of(0, id);
-    load(0, id, p.k_codes, k);
+    load(0, id, p.k_codes);
     load_scales(id);
-    load(0, id, p.v_codes, v);
     ids_of(1, next);
     for (int j = 0; ok && j < tiles; ++j) {
       const int stage = j & 1;
@@ -524,17 +527,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->meta[j % kMetaStages]);
-      store(smem + S::kKeyRing + stage * S::kOperand, k);
+      store(smem + S::kKeyRing + stage * S::kOperand);
       if (lane == 0) mbar_arrive(&bars->key_full[stage]);
-      if (j + 1 < tiles) {
-        load(j + 1, next, p.k_codes, k);
-        load_scales(next);
-      }
+      load(j, id, p.v_codes);
+      if (j + 1 < tiles) load_scales(next);
       if (j >= 2) ok = mbar_wait_warp(&bars->value_empty[stage], ((j >> 1) - 1) & 1, abort_flag);
       if (!ok) break;
-      store(smem + S::kValueRing + stage * S::kOperand, v);
+      store(smem + S::kValueRing + stage * S::kOperand);
       if (lane == 0) mbar_arrive(&bars->value_full[stage]);
-      if (j + 1 < tiles) load(j + 1, next, p.v_codes, v);
+      if (j + 1 < tiles) load(j + 1, next, p.k_codes);
       id[0] = next[0];
       id[1] = next[1];
       ids_of(j + 2, next);
@@ -543,7 +544,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       *abort_flag = 1;
       report_error(p.batch.error, 42);
     }
-  } else if (elect_one()) {
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+    if (warp == 12 && elect_one()) {
     // ---- MMAs -------------------------------------------------------------------------------
     const uint32_t shape = (1u << 4) | (static_cast<uint32_t>(kRowTile >> 4) << 24);
     const uint32_t scores_desc = shape | (static_cast<uint32_t>(kKeys >> 3) << 17);
@@ -599,6 +602,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       while (!mbar_try_wait(&bars->drain, 0) && global_timer_ns() - started < kWaitLimitNs) {
       }
     }
+    }
   }
 
   tc_fence_before_sync();
@@ -609,17 +613,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   }
 }
 
-template <int DP>
+template <int DP, int kUnit>
 qx_status launch_prompt_of(const AttentionParams& p, long long grid, cudaStream_t stream) {
   static SmemOptIn opt_in;
-  QX_TRY(opt_in.ensure(prompt_kernel<DP>, TcShape<DP>::kBytes));
-  return launch_behind(prompt_kernel<DP>, grid, kTcThreads, TcShape<DP>::kBytes, stream, p);
+  QX_TRY(opt_in.ensure(prompt_kernel<DP, kUnit>, TcShape<DP>::kBytes));
+  return launch_behind(prompt_kernel<DP, kUnit>, grid, kTcThreads, TcShape<DP>::kBytes, stream, p);
 }
 
 }  // namespace
 
 qx_status launch_prompt(const AttentionParams& p, long long grid, cudaStream_t stream) {
-  return p.dim <= 64 ? launch_prompt_of<64>(p, grid, stream) : launch_prompt_of<128>(p, grid, stream);
+  if (p.block_tokens < 32) {
+    return p.dim <= 64 ? launch_prompt_of<64, 16>(p, grid, stream) : launch_prompt_of<128, 16>(p, grid, stream);
+  }
+  return p.dim <= 64 ? launch_prompt_of<64, 32>(p, grid, stream) : launch_prompt_of<128, 32>(p, grid, stream);
 }
 
 }  // namespace kv
