@@ -46,14 +46,16 @@ constexpr float kLeastLog = -100.0f;  // of a value scale: append makes no small
 
 constexpr float kSpan = 60.0f;  // log2 of the largest ratio of value scales that is kept
 
-struct Group {
-  float key_scale, value_log, value_inverse;  // (2^-value_log)
-  int present;
+// What the softmax needs to know about a tile of keys, by groups of 16.
+struct Meta {
+  float2 scales[kGroups];        // of the keys, and log2 of the values'
+  float value_inverse[kGroups];  // 2^-log2
+  int present[kGroups];
 };
 
 struct Barriers {
   uint64_t queries[2], key_full[2], key_empty[2], value_full[2], value_empty[2];
-  uint64_t scores[2], weights[2], sums[2], meta[kMetaStages], drain;
+  uint64_t scores[2], halves[2], weights[2], sums[2], meta[kMetaStages], drain;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -65,7 +67,7 @@ struct TcShape {
   static constexpr int kKeyRing = kQueries + 2 * kOperand;
   static constexpr int kValueRing = kKeyRing + 2 * kOperand;
   static constexpr int kMeta = kValueRing + 2 * kOperand;
-  static constexpr int kBars = kMeta + kMetaStages * kGroups * static_cast<int>(sizeof(Group));
+  static constexpr int kBars = kMeta + kMetaStages * static_cast<int>(sizeof(Meta));
   static constexpr int kBytes = kBars + static_cast<int>(sizeof(Barriers)) + 1024;  // (the operands start on 1024)
 };
 
@@ -158,22 +160,23 @@ struct RowState {
 // One tile of scores to weights, in TMEM. `scores`: this warp's lanes of S, which P replaces; `sums`: of O. Keys
 // share scales by `kUnit`s of 16 or 32.
 template <int DP, int kUnit, bool kMasked>
-__device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, const Group* groups, RowState& row, int key0,
-                                             bool first) {
-  constexpr int kUnits = kKeys / kUnit;
+__device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, const Meta& meta, RowState& row, int key0,
+                                             bool first, uint64_t* first_half) {
+  constexpr int kUnits = kKeys / kUnit, kPerUnit = kUnit / 16;
   uint32_t s[4][32];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_ld_32x32(scores + 32 * c, s[c]);
+  tmem_ld_32x32(scores, s[0]);
+  tmem_ld_32x32(scores + 32, s[1]);
 
-  float factor[kUnits], log[kUnits];
+  float factor[kUnits], log[kUnits], relative[kUnits];
   float largest = row.largest_log;
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    const Group g = groups[u * (kUnit / 16)];
-    factor[u] = row.factor * g.key_scale;
-    log[u] = g.value_log;
+    const float2 scales = meta.scales[u * kPerUnit];
+    factor[u] = row.factor * scales.x;
+    log[u] = scales.y;
+    relative[u] = meta.value_inverse[u * kPerUnit];
     const int key = key0 + kUnit * u;
-    const bool seen = !kMasked || (g.present != 0 && key < row.high && key + kUnit > row.low);
+    const bool seen = !kMasked || (meta.present[u * kPerUnit] != 0 && key < row.high && key + kUnit > row.low);
     largest = fmaxf(largest, seen ? log[u] : -INFINITY);
   }
   if (largest > row.largest_log) {
@@ -183,30 +186,42 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   }
   const float least = largest - kSpan;
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u) log[u] = log[u] < least ? least : log[u];  // (no number stays none)
+  for (int u = 0; u < kUnits; ++u) {
+    relative[u] = log[u] < least ? 1.1529215046068470e18f : relative[u] * row.largest;  // (2^60)
+    log[u] = log[u] < least ? least : log[u];  // (no number stays none)
+  }
 
   const auto hidden = [&](int key) { return key < row.low || key >= row.high; };
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_ld_wait_for(s[c]);
   float top = -INFINITY;
-#pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
-    const bool present = !kMasked || groups[u * (kUnit / 16)].present != 0;
-    float m = -INFINITY;
+  const auto top_of = [&](int u) {
+    const bool present = !kMasked || meta.present[u * kPerUnit] != 0;
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (four chains: one would wait for itself)
 #pragma unroll
     for (int i = 0; i < kUnit; i += 2) {
       const int at = kUnit * u + i;
       const float a = __uint_as_float(s[at / 32][at % 32]), b = __uint_as_float(s[at / 32][at % 32 + 1]);
+      float& chain = m[i / 2 % 4];
       if (!kMasked) {
-        m = max3(m, a, b);
+        chain = max3(chain, a, b);
       } else {
-        if (present && !hidden(key0 + at)) m = fmaxf(m, a);
-        if (present && !hidden(key0 + at + 1)) m = fmaxf(m, b);
+        if (present && !hidden(key0 + at)) chain = fmaxf(chain, a);
+        if (present && !hidden(key0 + at + 1)) chain = fmaxf(chain, b);
       }
     }
+    const float most = fmaxf(max3(m[0], m[1], m[2]), m[3]);
     // (nothing seen: -infinity times a factor that may be zero or no number)
-    top = fmaxf(top, kMasked && m == -INFINITY ? -INFINITY : fmaf(m, factor[u], log[u]));
-  }
+    top = fmaxf(top, kMasked && most == -INFINITY ? -INFINITY : fmaf(most, factor[u], log[u]));
+  };
+  tmem_ld_wait_for(s[0]);
+  tmem_ld_wait_for(s[1]);
+  tmem_ld_32x32(scores + 64, s[2]);
+  tmem_ld_32x32(scores + 96, s[3]);
+#pragma unroll
+  for (int u = 0; u < kUnits / 2; ++u) top_of(u);
+  tmem_ld_wait_for(s[2]);
+  tmem_ld_wait_for(s[3]);
+#pragma unroll
+  for (int u = kUnits / 2; u < kUnits; ++u) top_of(u);
 
   const bool behind = top > row.maximum + kBehind;  // (from -infinity on, any score is)
   if (__any_sync(0xFFFFFFFFu, behind)) {
@@ -236,7 +251,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
       const float add = log[u] - base;
       const unsigned long long f2 = tile::pack2(__float_as_uint(factor[u]), __float_as_uint(factor[u]));
       const unsigned long long c2 = tile::pack2(__float_as_uint(add), __float_as_uint(add));
-      const Group g = groups[u * (kUnit / 16)];
+      const bool present = !kMasked || meta.present[u * kPerUnit] != 0;
       unsigned long long sum2 = 0;
 #pragma unroll
       for (int i = 0; i < kUnit; i += 2) {
@@ -246,8 +261,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
         tile::unpack2(t2, lo, hi);
         float a = exp2_fast(__uint_as_float(lo)), b = exp2_fast(__uint_as_float(hi));
         if (kMasked) {  // (behind exp2: also where the arguments are no numbers)
-          a = g.present == 0 || hidden(key0 + 32 * c + at) ? 0.0f : a;
-          b = g.present == 0 || hidden(key0 + 32 * c + at + 1) ? 0.0f : b;
+          a = !present || hidden(key0 + 32 * c + at) ? 0.0f : a;
+          b = !present || hidden(key0 + 32 * c + at + 1) ? 0.0f : b;
         }
         const __half2 w = __floats2half2_rn(a, b);
         p[at / 2] = *reinterpret_cast<const uint32_t*>(&w);
@@ -256,11 +271,16 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
       uint32_t lo, hi;
       tile::unpack2(sum2, lo, hi);
       const float sum = __uint_as_float(lo) + __uint_as_float(hi);
-      const float relative = log[u] > g.value_log ? 1.1529215046068470e18f : g.value_inverse * row.largest;  // (2^60)
       // (a unit that is hidden as a whole may have a scale that is no number)
-      if (!kMasked || sum != 0.0f) row.sum = fmaf(sum, relative, row.sum);
+      if (!kMasked || sum != 0.0f) row.sum = fmaf(sum, relative[u], row.sum);
     }
     tmem_st_32x16(scores + 16 * c, p);
+    if (c == 1) {  // the product with the first half of the keys' values may begin
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(first_half);
+    }
   }
   tmem_st_wait();
 }
@@ -270,7 +290,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   using S = TcShape<DP>;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
-  Group* const meta = reinterpret_cast<Group*>(smem + S::kMeta);
+  Meta* const meta = reinterpret_cast<Meta*>(smem + S::kMeta);
   Barriers* const bars = reinterpret_cast<Barriers*>(smem + S::kBars);
   volatile int* const abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -300,6 +320,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       mbar_init(&bars->value_full[i], kConvertWarps);
       mbar_init(&bars->value_empty[i], 1);
       mbar_init(&bars->scores[i], 1);
+      mbar_init(&bars->halves[i], 4);
       mbar_init(&bars->weights[i], 4);
       mbar_init(&bars->sums[i], 1);
     }
@@ -393,15 +414,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         if (!ok) break;
         __syncwarp();
         tc_fence_after_sync();
-        const Group* const groups = meta + j % kMetaStages * kGroups;
+        const Meta& tile_meta = meta[j % kMetaStages];
         const int key0 = begin + j * kKeys;
         bool open = key0 + kKeys <= open_high && key0 >= open_low;
         if (open) {
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g) open = open && groups[g].present != 0;
+          for (int g = 0; g < kGroups; ++g) open = open && tile_meta.present[g] != 0;
         }
-        if (__all_sync(0xFFFFFFFFu, open)) softmax_tile<DP, kUnit, false>(scores, sums, groups, row, key0, j == 0);
-        else softmax_tile<DP, kUnit, true>(scores, sums, groups, row, key0, j == 0);
+        if (__all_sync(0xFFFFFFFFu, open)) softmax_tile<DP, kUnit, false>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which]);
+        else softmax_tile<DP, kUnit, true>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which]);
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->weights[which]);
@@ -522,8 +543,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       if (lane < 2) {
         const float vs = scales[1];
         const float log = vs < 7.8886090522101181e-31f ? kLeastLog : log2f(vs);  // (2^-100; no number stays none)
-        meta[j % kMetaStages * kGroups + 2 * w + lane] =
-            Group{scales[0], log, exp2f(-log), (lane == 1 ? id[1] : id[0]) >= 0};
+        Meta& m = meta[j % kMetaStages];
+        m.scales[2 * w + lane] = make_float2(scales[0], log);
+        m.value_inverse[2 * w + lane] = exp2f(-log);
+        m.present[2 * w + lane] = (lane == 1 ? id[1] : id[0]) >= 0;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->meta[j % kMetaStages]);
@@ -572,15 +595,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       const int stage = j & 1, after = (j + 1) & 1;
       for (int i = 0; ok && i < row_tiles; ++i) {
         if (i == 0) ok = mbar_wait(&bars->value_full[stage], j >> 1 & 1, abort_flag);
-        ok = ok && mbar_wait(&bars->weights[i], j & 1, abort_flag);
+        ok = ok && mbar_wait(&bars->halves[i], j & 1, abort_flag);
         if (!ok) break;
         tc_fence_after_sync();
 #pragma unroll
         for (int t = 0; t < kKeys; t += 16) {
+          if (t == kKeys / 2) {
+            ok = mbar_wait(&bars->weights[i], j & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after_sync();
+          }
           mma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + t / 2,
                      make_sw128_nmajor_desc(base + S::kValueRing + stage * S::kOperand + t * 128, kKeys * 128), sums_desc,
                      j > 0 || t > 0);
         }
+        if (!ok) break;
         if (j + 1 == tiles) {
           tc_commit(&bars->sums[i]);
           continue;
