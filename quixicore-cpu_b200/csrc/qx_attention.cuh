@@ -13,7 +13,7 @@ struct AttentionParams {
   const int8_t* v_codes;
   const float* k_scales;
   const float* v_scales;
-  int kv_heads, block_tokens, dim;
+  int kv_heads, block_tokens, block_shift, dim;  // (block_tokens = 1 << block_shift)
   Heads q, out;
   float* lse;
   float scale_log2;  // scale * log2(e)

@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         const int key = begin + j * kKeys + 32 * w + 16 * g;
         id[g] = -1;
         if (j < tiles && key < end) {
-          const int block = table[key / p.block_tokens];
+          const int block = table[key >> p.block_shift];
           if (block >= 0 && block < p.batch.blocks) id[g] = block;
           else if (lane == 0) report_error(p.batch.error, kErrorBlock);
         }
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
     const auto load = [&](int j, const int (&id)[2], const int8_t* plane) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const int slot = (begin + j * kKeys + 32 * w + 16 * g) % p.block_tokens;
+        const int slot = (begin + j * kKeys + 32 * w + 16 * g) & (p.block_tokens - 1);
         const int8_t* const from =
             plane + ((static_cast<long long>(max(id[g], 0)) * p.kv_heads + head) * p.block_tokens + slot) * p.dim;
 #pragma unroll

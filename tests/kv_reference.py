@@ -96,14 +96,17 @@ def attention(q, k, v, scale, causal, window, missing=()):
     lse = torch.logsumexp(s, -1) if length else torch.full((heads, n), -math.inf, dtype=torch.float64)
     p = torch.where(seen, torch.exp(s - torch.where(lse == -math.inf, 0.0, lse)[..., None]), 0.0)
     spread = (abs(scale) * (qq.abs() @ kk.abs().transpose(1, 2))).amax(-1) if length else torch.zeros(heads, n)
+    if length:  # (2^-22 of the row's largest query element, in units of the tolerances' 2^-23)
+        spread = spread + abs(scale) * qq.abs().amax(-1) * kk.abs().sum(-1).amax(-1)[:, None] * 2 / (dim / 16 + 22)
     magnitude = (p @ vv.abs()).transpose(0, 1), (seen.double() @ vv.abs()).transpose(0, 1)
     return (p @ vv).transpose(0, 1), lse.T, magnitude, spread.T
 
 
 def attention_tolerance(out, lse, magnitude, spread, dtype, dim, length):
     """Bounds on |kernel - exact|, per output element and per entry of lse. With u = 2^-23:
-      scores   products of up to 22-bit queries and exact codes, summed in f32 (each of the dim / 16 MMAs may
-               truncate), three multiplications: (dim / 16 + 22) u of the sum of magnitudes, at most;
+      scores   products of queries, rounded to 2^-22 of their row's largest magnitude (the second term of `spread`),
+               and exact codes, summed in f32 (each of the dim / 16 MMAs may truncate), three multiplications:
+               (dim / 16 + 22) u of the sum of magnitudes, at most;
       weights  exp2 to 2 u, its argument (up to `spread` * 1.44 away from the maximum) to one rounding: inside
                the next term;
       a score that is off by d takes d of its weight with it, and d of the sum: 2 d;
