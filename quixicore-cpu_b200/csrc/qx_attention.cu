@@ -159,13 +159,12 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
   float* const row_factor = reinterpret_cast<float*>(queries + S::kQueries);
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  long long index = blockIdx.x;
-  const int split = static_cast<int>(index % p.splits);
-  index /= p.splits;
-  const long long tile_index = index;
-  const int row_tile = static_cast<int>(index % p.row_tiles);
-  index /= p.row_tiles;
-  const int head = static_cast<int>(index % p.kv_heads), s = static_cast<int>(index / p.kv_heads);
+  uint32_t index = blockIdx.x;
+  const uint32_t tile_index = index / p.splits;
+  const int split = static_cast<int>(index - tile_index * p.splits);
+  index = tile_index / p.row_tiles;
+  const int row_tile = static_cast<int>(tile_index - index * p.row_tiles);
+  const int s = static_cast<int>(index / p.kv_heads), head = static_cast<int>(index - s * p.kv_heads);
   Rows rows;
   if (!rows_of(p, s, row_tile * kRows, kRows, &rows)) return;
   int begin, end;
@@ -240,19 +239,29 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
   ids_of(warp + (kStages - 1) * kWarps, next_ids);
 
   // ---- queries: whole numbers below 2^23 times a power of two per row, as three digits -----------------------
-  for (int r = warp; r < kRows; r += kWarps) {
-    float v[DP / 32];
-    uint32_t top = 0;
-    long long base = 0;
-    if (r < rows.count) {
-      const int token = (rows.first + r) / p.group, member = (rows.first + r) % p.group;
-      base = (rows.row + token) * p.q.token_stride + (static_cast<long long>(head) * p.group + member) * p.q.head_stride;
-    }
+  // A lane takes four neighbouring elements (of 128 at a time), all of the warp's rows before any is used.
+  constexpr int kOwnRows = kRows / kWarps, kOwnRuns = (DP + 127) / 128;
+  float v[kOwnRows][kOwnRuns][4];
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-      const int d = i * 32 + lane;
-      v[i] = r < rows.count && d < p.dim ? load_one(p.q.data, p.q.type, base + d) : 0.0f;
-      top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  for (int own = 0; own < kOwnRows; ++own) {
+    const int r = own * kWarps + warp, token = (rows.first + r) / p.group;
+    const long long base = (rows.row + token) * p.q.token_stride +
+                           (static_cast<long long>(head) * p.group + (rows.first + r - token * p.group)) * p.q.head_stride;
+#pragma unroll
+    for (int i = 0; i < kOwnRuns; ++i) {
+      const int d = i * 128 + lane * 4;
+      v[own][i][0] = v[own][i][1] = v[own][i][2] = v[own][i][3] = 0.0f;
+      if (r < rows.count && d < p.dim) load4(p.q.data, p.q.type, p.q.vector, base + d, v[own][i]);
+    }
+  }
+#pragma unroll
+  for (int own = 0; own < kOwnRows; ++own) {
+    const int r = own * kWarps + warp;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kOwnRuns; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v[own][i][e]) & 0x7FFFFFFFu);
     }
     top = __reduce_max_sync(0xFFFFFFFFu, top) >> 23;
     // the row's largest magnitude becomes 2^21 .. 2^22: three balanced digits reach 127 * (1 + 2^8 + 2^16)
@@ -264,22 +273,31 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
                                  : __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * p.scale_log2;
     }
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-      const int d = i * 32 + lane, own_t = d / (DP / 4), rest = d % (DP / 4);
-      int x = top >= 255 ? 0 : __float2int_rn(v[i] * factor);
-      // operand of step j: lane (row, t) holds elements 8 j .. 8 j + 7 of its share
-      const int at = ((r >> 3) * kSteps + rest / 8) * 256 + ((r & 7) * 4 + own_t) * 8 + rest % 8;
+    for (int i = 0; i < kOwnRuns; ++i) {
+      const int d = i * 128 + lane * 4;
+      uint32_t x[4];
 #pragma unroll
-      for (int digit = 0; digit < 3; ++digit) {
-        const int low = static_cast<int8_t>(x & 255);
-        reinterpret_cast<int8_t*>(queries)[digit * kRows * DP + at] = static_cast<int8_t>(low);
-        x = (x - low) >> 8;
+      for (int e = 0; e < 4; ++e) {
+        // digits + 128 are the bytes of x + 128 (1 + 2^8 + 2^16)
+        const int whole = top >= 255 ? 0 : __float2int_rn(v[own][i][e] * factor);
+        x[e] = static_cast<uint32_t>(whole + 0x808080) ^ 0x808080u;
+      }
+      // operand of step j: lane (row, t) holds elements 8 j .. 8 j + 7 of its share
+      const int own_t = d / (DP / 4), rest = d % (DP / 4);
+      const int at = ((r >> 3) * kSteps + rest / 8) * 256 + ((r & 7) * 4 + own_t) * 8 + rest % 8;
+      if (d < DP) {
+#pragma unroll
+        for (int digit = 0; digit < 3; ++digit) {
+          const uint32_t select = digit | (4 + digit) << 4;
+          *reinterpret_cast<uint32_t*>(queries + digit * kRows * DP + at) =
+              __byte_perm(__byte_perm(x[0], x[1], select), __byte_perm(x[2], x[3], select), 0x5410);
+        }
       }
     }
   }
   __syncthreads();
-  // (in registers for one tile of rows, else read as they are needed)
-  constexpr bool kResident = kRowTiles == 1 && DP <= 128;
+  // (in registers where there is room for them, else read as they are needed)
+  constexpr bool kResident = kRowTiles == 1 && DP <= 64;
   uint2 resident[kResident ? 3 * kSteps : 1];
   if (kResident) {
 #pragma unroll
@@ -426,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
         for (int h = 4; h <= 16; h <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, h));
         top = fmaxf(top, most[n][e]);
         // (a row that has seen nothing yet: weights exp2(-inf) = 0 against any finite maximum)
-        const float base = top == -INFINITY ? 0.0f : top;
+        const float base = top == -INFINITY ? 0.0f : top, less = base - kShift;
         keep[n][e] = exp2_fast(most[n][e] - base);
         moved = moved || top != most[n][e];
         most[n][e] = top;
@@ -436,13 +454,23 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float& v = score[n][k][2 * h + e];
-            const bool hidden = !open && v == -INFINITY;
-            v = exp2_fast(v - base + kShift);
+            v = exp2_fast(v - less);
             total += v;
-            if (p.block_tokens < kTile) v = hidden ? 0.0f : v * ratio[k];
           }
         }
         sum[n][e] = fmaf(sum[n][e], keep[n][e], total);
+      }
+      if (ratio[0] != ratio[1]) {  // (also where one is no number)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int key = token0 + 16 * k + 8 * (h >> 1) + g;
+            const bool hidden = !open && (!(present >> k & 1) || key < low[n][h & 1] || key >= high[n][h & 1]);
+            score[n][k][h] = hidden ? 0.0f : score[n][k][h] * ratio[k];
+          }
+        }
+        __syncwarp();
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -568,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
       v[7] = fmaf(b.w, weight[w], v[7]);
     }
     if (!whole) {
-      const long long at = (tile_index * p.splits + split) * kRows + r;
+      const long long at = (static_cast<long long>(tile_index) * p.splits + split) * kRows + r;
       float4* const to = reinterpret_cast<float4*>(p.partial + at * p.dim + d);
       to[0] = make_float4(v[0], v[1], v[2], v[3]);
       to[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -727,12 +755,13 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   if (p.window > 0 && p.causal) range = std::min<long long>(range, static_cast<long long>(p.window) + p.tile_rows);
   range += 31;  // (from a multiple of 32 on)
   // Chunks: one sequence fills the card with one round of equal chunks; several, of lengths that only the
-  // device knows, get four rounds of smaller ones, so that the SMs which end early take the next. No chunk is
+  // device knows, get half as many again (measured with 1 | 1.5 | 3 | 6 rounds, us: 32 sessions of 1200 to 8192
+  // 87 | 84 | 85 | 85, of up to 2000 31 | 34 | 38 | 38, 8 sessions of up to 20000 64 | 58 | 57 | 67). No chunk is
   // below a tile per warp (in the prompt kernel, four tiles): then the joining would cost more than the keys.
   const int dp = cache->head_dim <= 64 ? 64 : cache->head_dim <= 128 ? 128 : 256;
   const long long slots = static_cast<long long>(ctx->prop.multiProcessorCount) * (prompt ? 1 : streamed_ctas(dp, p.tile_rows / 8));
   const bool one_round = batch->sequences == 1 || prompt;
-  const long long wanted = one_round ? std::max(1LL, slots / items) : (4 * slots + items - 1) / items;
+  const long long wanted = one_round ? std::max(1LL, slots / items) : (3 * slots / 2 + items - 1) / items;
   const long long unit = prompt ? 128 : kTile;
   const long long least = prompt ? 512 : kTile * kWarps * (batch->sequences == 1 ? 1 : 2);
   const long long chunk = (std::max((range + wanted - 1) / wanted, least) + unit - 1) / unit * unit;

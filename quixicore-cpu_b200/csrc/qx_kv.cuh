@@ -81,6 +81,25 @@ __device__ __forceinline__ void store_one(uint8_t* data, int type, long long ind
   }
 }
 
+// Four neighbouring elements, as below.
+__device__ __forceinline__ void load4(const uint8_t* data, int type, int vector, long long index, float (&v)[4]) {
+  if (!vector) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = load_one(data, type, index + i);
+  } else if (type == QX_STORAGE_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(data) + index);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else {
+    const uint2 a = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(data) + index);
+    if (type == QX_STORAGE_F16) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a.x));
+      const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&a.y));
+      v[0] = x.x; v[1] = x.y; v[2] = y.x; v[3] = y.y;
+    } else {
+      v[0] = bf16_low(a.x); v[1] = bf16_high(a.x); v[2] = bf16_low(a.y); v[3] = bf16_high(a.y);
+    }
+  }
+}
 // Eight neighbouring elements. `vector`: the first of them is on a 16-byte boundary.
 __device__ __forceinline__ void load8(const uint8_t* data, int type, int vector, long long index, float (&v)[8]) {
   if (!vector) {
