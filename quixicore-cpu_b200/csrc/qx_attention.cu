@@ -10,10 +10,13 @@
 //           relative, no further than the 16-bit outputs' own), as hi + lo pairs for f32 queries; f32 sums.
 // The scales are applied to the sums: one multiplication per score (ks), one per 32 keys and output element (vs).
 //
-// Split. A CTA takes 8 rows (16 or 32 where there are that many) and a chunk of the keys; its four warps
-// take tiles of 32 keys in turn, each with a running maximum and sum of its own, and are joined at the end
-// through shared memory. So one pass over the codes serves all heads of a group, and the card is filled by
-// chunks where there are few rows; chunks are joined by a second, small kernel in a fixed order.
+// Split. A CTA takes 8 rows (16 where there are more) and a run of the keys; its four warps take tiles of 32
+// keys in turn, each with a running maximum and sum of its own, and are joined at the end through shared
+// memory. So one pass over the codes serves all heads of a group. Where every sequence is one tile of rows (tokens
+// being decoded) the launch is balanced: the tiles of all sequences and kv heads form one line, which the resident
+// CTAs cut into equal pieces, whatever the lengths; a CTA's first and last piece may be parts of an item (sequence,
+// kv head), and the last CTA to finish a part of an item joins its parts, in their order. Otherwise keys are cut
+// into chunks where there are few rows, joined by a second, small kernel.
 //
 // Data movement. Each warp has a ring of stages of its own (codes of 32 keys and values, their scales),
 // filled by 16-byte asynchronous copies: tiles in flight while one is computed, nothing to wait for but the
@@ -147,7 +150,61 @@ __device__ __forceinline__ uint32_t rest_f16(float a, float b, uint32_t rounded)
   return pair_f16(a - f.x, b - f.y);
 }
 
-template <int DP, bool kWide, int kRowTiles>
+// A balanced launch's line: per item, kItemCost units for what a CTA does before its first tile, and one per tile.
+constexpr int kItemCost = 4, kLeastPiece = 8, kBalancedSequences = 128;
+struct Line {
+  uint32_t begin[kBalancedSequences / 32];  // of sequence lane + 32 i
+  uint32_t item[kBalancedSequences / 32];   // units per kv head
+  uint32_t total, piece;                    // (the host has made sure that they fit)
+};
+template <int kRows>
+__device__ __forceinline__ Line line_of(const AttentionParams& p) {
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  Line line;
+#pragma unroll
+  for (int i = 0; i < kBalancedSequences / 32; ++i) {
+    Rows rows;
+    line.item[i] = 0;
+    if (lane + 32 * i < p.batch.sequences && rows_of(p, lane + 32 * i, 0, kRows, &rows, true)) {
+      line.item[i] = kItemCost + (rows.high - rows.low + kTile - 1) / kTile;
+    }
+  }
+  line.total = 0;
+#pragma unroll
+  for (int i = 0; i < kBalancedSequences / 32; ++i) {
+    line.begin[i] = line.total;
+    if (32 * i >= p.batch.sequences) continue;
+    const uint32_t cost = line.item[i] * p.kv_heads;
+    uint32_t through = cost;
+#pragma unroll
+    for (int h = 1; h < 32; h <<= 1) {
+      const uint32_t below = __shfl_up_sync(0xFFFFFFFFu, through, h);
+      if (lane >= h) through += below;
+    }
+    line.begin[i] += through - cost;
+    line.total += __shfl_sync(0xFFFFFFFFu, through, 31);
+  }
+  line.piece = max(static_cast<uint32_t>(kLeastPiece), (line.total + gridDim.x - 1) / gridDim.x);
+  return line;
+}
+// The sequence at a place of the line, where it begins and its units per kv head.
+__device__ __forceinline__ int sequence_at(const AttentionParams& p, const Line& line, uint32_t at, uint32_t* begin, uint32_t* item) {
+  int found = 0;
+#pragma unroll
+  for (int i = 0; i < kBalancedSequences / 32; ++i) {
+    if (32 * i >= p.batch.sequences) continue;
+    const uint32_t lanes = __ballot_sync(0xFFFFFFFFu, at >= line.begin[i] && at - line.begin[i] < line.item[i] * p.kv_heads);
+    if (lanes != 0) {
+      const int lane = __ffs(lanes) - 1;
+      found = lane + 32 * i;
+      *begin = __shfl_sync(0xFFFFFFFFu, line.begin[i], lane);
+      *item = __shfl_sync(0xFFFFFFFFu, line.item[i], lane);
+    }
+  }
+  return found;
+}
+
+template <int DP, bool kWide, int kRowTiles, bool kBalanced>
 __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
     attention_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<DP, kWide, kRowTiles>;
@@ -159,16 +216,46 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
   float* const row_factor = reinterpret_cast<float*>(queries + S::kQueries);
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  uint32_t index = blockIdx.x;
-  const uint32_t tile_index = index / p.splits;
-  const int split = static_cast<int>(index - tile_index * p.splits);
-  index = tile_index / p.row_tiles;
-  const int row_tile = static_cast<int>(tile_index - index * p.row_tiles);
-  const int s = static_cast<int>(index / p.kv_heads), head = static_cast<int>(index - s * p.kv_heads);
+  __shared__ int last_part;
+  Line line;
+  uint32_t place = 0, place_end = 0;
+  if (kBalanced) {
+    line = line_of<kRows>(p);
+    place_end = min((blockIdx.x + 1) * line.piece, line.total);
+    place = min(blockIdx.x * line.piece, place_end);
+  }
+  for (bool once = true;; once = false) {
+  int s, head, row_tile = 0, begin, end;
+  long long part;           // where partial results go
+  uint32_t first_part = 0;  // balanced: the first CTA that holds a part of the item
+  int parts = 1;
   Rows rows;
-  if (!rows_of(p, s, row_tile * kRows, kRows, &rows)) return;
-  int begin, end;
-  if (!chunk_of(p, rows, split, &begin, &end)) return;
+  if (kBalanced) {
+    if (place >= place_end) return;
+    uint32_t sequence_begin = 0, item = 1;
+    s = sequence_at(p, line, place, &sequence_begin, &item);
+    head = static_cast<int>((place - sequence_begin) / item);
+    const uint32_t item_begin = sequence_begin + head * item, item_end = item_begin + item, stop = min(place_end, item_end);
+    first_part = item_begin / line.piece;
+    parts = static_cast<int>((item_end - 1) / line.piece - first_part) + 1;
+    part = 2LL * blockIdx.x + (first_part == blockIdx.x ? 1 : 0);
+    (void)rows_of(p, s, 0, kRows, &rows);
+    const int unit0 = max(0, static_cast<int>(place - item_begin) - kItemCost), unit1 = max(0, static_cast<int>(stop - item_begin) - kItemCost);
+    begin = rows.low + unit0 * kTile;
+    end = min(rows.high, rows.low + unit1 * kTile);
+    place = stop;
+  } else {
+    if (!once) return;
+    const uint32_t tile_index = blockIdx.x / p.splits, split = blockIdx.x - tile_index * p.splits;
+    const uint32_t index = tile_index / p.row_tiles;
+    row_tile = static_cast<int>(tile_index - index * p.row_tiles);
+    s = static_cast<int>(index / p.kv_heads);
+    head = static_cast<int>(index - s * p.kv_heads);
+    if (!rows_of(p, s, row_tile * kRows, kRows, &rows)) return;
+    if (!chunk_of(p, rows, split, &begin, &end)) return;
+    part = static_cast<long long>(blockIdx.x);
+    parts = splits_used(p, rows);
+  }
   const int32_t* const table = p.batch.table + s * p.batch.table_stride;
   const int tiles = (end - begin + kTile - 1) / kTile;  // (zero or less: the rows see nothing)
 
@@ -567,8 +654,13 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
     }
   }
   __syncthreads();
-  const bool whole = splits_used(p, rows) == 1;
+  const bool whole = parts == 1;
   const int per_row = p.dim / 8;
+  const auto place_of = [&](int r, long long* out_row, long long* out_head) {
+    const int token = (rows.first + r) / p.group;
+    *out_row = rows.row + token;
+    *out_head = static_cast<long long>(head) * p.group + (rows.first + r - token * p.group);
+  };
   for (int i = threadIdx.x; i < rows.count * per_row; i += kThreads) {
     const int r = i / per_row, d = (i - r * per_row) * 8;
     float top = -INFINITY, total = 0.0f, v[8], weight[kWarps];
@@ -596,23 +688,86 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
       v[7] = fmaf(b.w, weight[w], v[7]);
     }
     if (!whole) {
-      const long long at = (static_cast<long long>(tile_index) * p.splits + split) * kRows + r;
+      const long long at = part * kRows + r;
       float4* const to = reinterpret_cast<float4*>(p.partial + at * p.dim + d);
       to[0] = make_float4(v[0], v[1], v[2], v[3]);
       to[1] = make_float4(v[4], v[5], v[6], v[7]);
       if (d == 0) *reinterpret_cast<float2*>(p.statistics + 2 * at) = make_float2(top, total);
       continue;
     }
-    const int token = (rows.first + r) / p.group, member = (rows.first + r) % p.group;
-    const long long out_head = static_cast<long long>(head) * p.group + member;
+    long long out_row, out_head;
+    place_of(r, &out_row, &out_head);
     const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] *= inverse;
-    store8(p.out.data, p.out.type, p.out.vector, (rows.row + token) * p.out.token_stride + out_head * p.out.head_stride + d, v);
+    store8(p.out.data, p.out.type, p.out.vector, out_row * p.out.token_stride + out_head * p.out.head_stride + d, v);
     if (p.lse != nullptr && d == 0) {
-      p.lse[(rows.row + token) * p.out.heads + out_head] =
+      p.lse[out_row * p.out.heads + out_head] =
           total == 0.0f ? -INFINITY : (top + log2f(total) - kShift) * 0.69314718055994531f;
     }
+  }
+  if (kBalanced) {
+    if (!whole) {
+      // The CTA that arrives last at the item's counter joins its parts, all of them from memory and in their order.
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        int* const counter = p.counters + s * p.kv_heads + head;
+        last_part = atomicAdd(counter, 1) == parts - 1;
+        if (last_part) *counter = 0;
+      }
+      __syncthreads();
+      if (last_part) {
+        __threadfence();
+        const int vectors = p.dim / 4;
+        for (int i = threadIdx.x; i < rows.count * vectors; i += kThreads) {
+          const int r = i / vectors, at = i - r * vectors;
+          float top = -INFINITY, total = 0.0f;
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          constexpr int kBatch = 8;  // loads under way
+          for (int q0 = 0; q0 < parts; q0 += kBatch) {
+            float2 stat[kBatch];
+            float4 x[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+              // (the item begins behind others in its first CTA, and at the start of the following ones)
+              const long long from = (2LL * (first_part + q0 + b) + (q0 + b == 0 ? 1 : 0)) * kRows + r;
+              stat[b] = make_float2(-INFINITY, 0.0f);
+              x[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (q0 + b < parts) {
+                stat[b] = __ldcg(reinterpret_cast<const float2*>(p.statistics) + from);
+                x[b] = __ldcg(reinterpret_cast<const float4*>(p.partial + from * p.dim) + at);
+              }
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+              const float most = fmaxf(top, stat[b].x), base = most == -INFINITY ? 0.0f : most;
+              const float keep = exp2_fast(top - base), weight = exp2_fast(stat[b].x - base);
+              top = most;
+              total = fmaf(total, keep, stat[b].y * weight);
+              v.x = fmaf(v.x, keep, x[b].x * weight);
+              v.y = fmaf(v.y, keep, x[b].y * weight);
+              v.z = fmaf(v.z, keep, x[b].z * weight);
+              v.w = fmaf(v.w, keep, x[b].w * weight);
+            }
+          }
+          const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+          long long out_row, out_head;
+          place_of(r, &out_row, &out_head);
+          const long long to = out_row * p.out.token_stride + out_head * p.out.head_stride + 4 * at;
+          store_one(p.out.data, p.out.type, to, v.x * inverse);
+          store_one(p.out.data, p.out.type, to + 1, v.y * inverse);
+          store_one(p.out.data, p.out.type, to + 2, v.z * inverse);
+          store_one(p.out.data, p.out.type, to + 3, v.w * inverse);
+          if (at == 0 && p.lse != nullptr) {
+            p.lse[out_row * p.out.heads + out_head] =
+                total == 0.0f ? -INFINITY : (top + log2f(total) - kShift) * 0.69314718055994531f;
+          }
+        }
+      }
+    }
+    __syncthreads();  // shared memory is the next piece's
+  }
   }
 }
 
@@ -694,17 +849,24 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   }
 }
 
-template <int DP, bool kWide, int kRowTiles>
+template <int DP, bool kWide, int kRowTiles, bool kBalanced>
 qx_status launch_streamed(const AttentionParams& p, long long grid, cudaStream_t stream) {
   static SmemOptIn opt_in;
   constexpr int bytes = Shape<DP, kWide, kRowTiles>::kBytes;
-  QX_TRY(opt_in.ensure(attention_kernel<DP, kWide, kRowTiles>, bytes));
-  return launch_behind(attention_kernel<DP, kWide, kRowTiles>, grid, kThreads, bytes, stream, p);
+  QX_TRY(opt_in.ensure(attention_kernel<DP, kWide, kRowTiles, kBalanced>, bytes));
+  return launch_behind(attention_kernel<DP, kWide, kRowTiles, kBalanced>, grid, kThreads, bytes, stream, p);
 }
 template <int DP, bool kWide>
-qx_status launch_rows(const AttentionParams& p, long long grid, cudaStream_t stream) {
-  if (p.tile_rows == 8) return launch_streamed<DP, kWide, 1>(p, grid, stream);
-  return launch_streamed<DP, kWide, 2>(p, grid, stream);
+qx_status launch_rows(const AttentionParams& p, bool balanced, long long grid, cudaStream_t stream) {
+  if (p.tile_rows == 8) {
+    return balanced ? launch_streamed<DP, kWide, 1, true>(p, grid, stream) : launch_streamed<DP, kWide, 1, false>(p, grid, stream);
+  }
+  return balanced ? launch_streamed<DP, kWide, 2, true>(p, grid, stream) : launch_streamed<DP, kWide, 2, false>(p, grid, stream);
+}
+qx_status launch_sized(const AttentionParams& p, int dp, bool wide, bool balanced, long long grid, cudaStream_t stream) {
+  if (dp == 64) return wide ? launch_rows<64, true>(p, balanced, grid, stream) : launch_rows<64, false>(p, balanced, grid, stream);
+  if (dp == 128) return wide ? launch_rows<128, true>(p, balanced, grid, stream) : launch_rows<128, false>(p, balanced, grid, stream);
+  return wide ? launch_rows<256, true>(p, balanced, grid, stream) : launch_rows<256, false>(p, balanced, grid, stream);
 }
 
 }  // namespace
@@ -760,6 +922,22 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   // below a tile per warp (in the prompt kernel, four tiles): then the joining would cost more than the keys.
   const int dp = cache->head_dim <= 64 ? 64 : cache->head_dim <= 128 ? 128 : 256;
   const long long slots = static_cast<long long>(ctx->prop.multiProcessorCount) * (prompt ? 1 : streamed_ctas(dp, p.tile_rows / 8));
+  const bool wide = q->type == QX_STORAGE_F32;
+  // Balanced: several sequences, and items enough that each has few parts to join (by one CTA, at about 0.15 us a part).
+  const long long counters = static_cast<long long>(batch->sequences) * cache->kv_heads;
+  const long long units = counters * ((range + kTile - 1) / kTile + kItemCost);
+  if (!prompt && p.row_tiles == 1 && batch->sequences > 1 && batch->sequences <= kBalancedSequences && counters >= slots / 16 &&
+      counters <= static_cast<long long>(kWorkspaceCounterBytes / sizeof(int)) && units < (1LL << 31)) {
+    // Two parts per CTA; behind the arrival counters, which the kernel leaves at zero.
+    const long long grid = std::min(slots, (units + kLeastPiece - 1) / kLeastPiece);
+    const size_t rows = 2 * static_cast<size_t>(grid) * p.tile_rows;
+    const size_t sums = align_up(rows * cache->head_dim * sizeof(float), 256);
+    QX_TRY(workspace->reserve(kWorkspaceCounterBytes + sums + rows * 2 * sizeof(float)));
+    p.counters = static_cast<int*>(workspace->base);
+    p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace->base) + kWorkspaceCounterBytes);
+    p.statistics = p.partial + sums / sizeof(float);
+    return launch_sized(p, dp, wide, true, grid, stream);
+  }
   const bool one_round = batch->sequences == 1 || prompt;
   const long long wanted = one_round ? std::max(1LL, slots / items) : (3 * slots / 2 + items - 1) / items;
   const long long unit = prompt ? 128 : kTile;
@@ -776,13 +954,7 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
     p.statistics = p.partial + sums / sizeof(float);
   }
   const long long grid = items * p.splits;
-  const bool wide = q->type == QX_STORAGE_F32;
-  qx_status status;
-  if (prompt) status = launch_prompt(p, grid, stream);
-  else if (dp == 64) status = wide ? launch_rows<64, true>(p, grid, stream) : launch_rows<64, false>(p, grid, stream);
-  else if (dp == 128) status = wide ? launch_rows<128, true>(p, grid, stream) : launch_rows<128, false>(p, grid, stream);
-  else status = wide ? launch_rows<256, true>(p, grid, stream) : launch_rows<256, false>(p, grid, stream);
-  QX_TRY(status);
+  QX_TRY(prompt ? launch_prompt(p, grid, stream) : launch_sized(p, dp, wide, false, grid, stream));
   return p.splits > 1 ? launch_behind(join_kernel, items * p.tile_rows, p.splits <= 16 ? 128 : kJoinThreads, 0, stream, p) : QX_STATUS_OK;
 }
 

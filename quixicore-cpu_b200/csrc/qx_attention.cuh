@@ -24,6 +24,7 @@ struct AttentionParams {
   float shift;       // log2 of what sums of weights carry
   float* partial;    // [tile][split][rows][dim] sums, then [tile][split][rows] {maximum, sum}
   float* statistics;
+  int* counters;     // [sequence][kv head] arrivals of a balanced launch, zero between calls
 };
 
 // A tile's rows are (token, query head of the group) pairs of one sequence and kv head, token major.
@@ -34,9 +35,9 @@ struct Rows {
   int low, high;       // keys [low, high) that any of them sees, low on a multiple of 32
 };
 
-__device__ __forceinline__ bool rows_of(const AttentionParams& p, int s, int first, int most, Rows* r) {
+__device__ __forceinline__ bool rows_of(const AttentionParams& p, int s, int first, int most, Rows* r, bool each = false) {
   Sequence q;
-  if (!sequence_of(p.batch, s, false, &q)) return false;
+  if (!sequence_of(p.batch, s, false, &q, each)) return false;
   const long long total = static_cast<long long>(q.n) * p.group;
   if (first >= total) return false;
   r->row = q.row;

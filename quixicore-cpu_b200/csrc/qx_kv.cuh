@@ -46,8 +46,9 @@ struct Sequence {
   int n, length;
 };
 
-// False (and a report) where the sequence's numbers do not fit: nothing of it is touched then.
-__device__ __forceinline__ bool sequence_of(const Batch& b, int s, bool rows_are_cached, Sequence* out) {
+// False (and a report) where the sequence's numbers do not fit: nothing of it is touched then. `each`: every thread
+// asks for a sequence of its own.
+__device__ __forceinline__ bool sequence_of(const Batch& b, int s, bool rows_are_cached, Sequence* out, bool each = false) {
   const long long row = b.begin != nullptr ? b.begin[s] : static_cast<long long>(s) * b.max_tokens;
   const long long n = b.begin != nullptr ? b.begin[s + 1] - row : b.max_tokens;
   const int length = b.lengths[s];
@@ -56,7 +57,7 @@ __device__ __forceinline__ bool sequence_of(const Batch& b, int s, bool rows_are
   out->length = length;
   const bool fits = row >= 0 && n >= 0 && n <= b.max_tokens && row + n <= b.tokens && length >= 0 &&
                     length <= b.max_length && (!rows_are_cached || n <= length);
-  if (!fits && threadIdx.x == 0) sm100::report_error(b.error, kErrorSequence);
+  if (!fits && (each || threadIdx.x == 0)) sm100::report_error(b.error, kErrorSequence);
   return fits;
 }
 
