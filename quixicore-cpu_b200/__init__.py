@@ -660,11 +660,10 @@ ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS, ROPE_RAMP = range(4)
 _torch_types: dict = {}
 
 
-def _storage_type(dtype) -> int:
-    if not _torch_types:
-        import torch
-        _torch_types.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
-    return _torch_types[dtype]
+def _fill_torch_types() -> dict:
+    import torch
+    _torch_types.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    return _torch_types
 
 
 def heads_view(t, kind=None, heads=None, token_stride=None, head_stride=None) -> HeadsView:
@@ -672,14 +671,15 @@ def heads_view(t, kind=None, heads=None, token_stride=None, head_stride=None) ->
     elements of a head lie side by side. The arguments behind `kind` replace what the array says."""
     if t is None:
         return None
+    shape = t.shape
     if isinstance(t, np.ndarray):
         kind = {2: F16, 4: F32}[t.itemsize] if kind is None else kind
         data, (st, sh, sd) = t.ctypes.data, (s // t.itemsize for s in t.strides)
     else:
-        kind = _storage_type(t.dtype) if kind is None else kind
+        kind = (_torch_types or _fill_torch_types())[t.dtype] if kind is None else kind
         data, (st, sh, sd) = t.data_ptr(), t.stride()
-    assert sd == 1 or t.shape[2] == 1, "the elements of a head lie side by side"
-    return HeadsView(data, kind, t.shape[1] if heads is None else heads, st if token_stride is None else token_stride,
+    assert sd == 1 or shape[2] == 1, "the elements of a head lie side by side"
+    return HeadsView(data, kind, shape[1] if heads is None else heads, st if token_stride is None else token_stride,
                      sh if head_stride is None else head_stride)
 
 

@@ -101,94 +101,169 @@ __device__ __forceinline__ void load4(const uint8_t* data, int type, int vector,
     }
   }
 }
-// Eight neighbouring elements. `vector`: the first of them is on a 16-byte boundary.
+// Eight neighbouring elements as they lie in memory (one 16-byte word of 16-bit ones, two of f32), and as f32.
+template <int kType>
+__device__ __forceinline__ void load8_words(const uint8_t* data, long long index, uint4 (&w)[kType == QX_STORAGE_F32 ? 2 : 1]) {
+  const uint4* const from = reinterpret_cast<const uint4*>(data + index * (kType == QX_STORAGE_F32 ? 4 : 2));
+  w[0] = from[0];
+  if (kType == QX_STORAGE_F32) w[kType == QX_STORAGE_F32 ? 1 : 0] = from[1];
+}
+template <int kType>
+__device__ __forceinline__ void store8_words(uint8_t* data, long long index, const uint4 (&w)[kType == QX_STORAGE_F32 ? 2 : 1]) {
+  uint4* const to = reinterpret_cast<uint4*>(data + index * (kType == QX_STORAGE_F32 ? 4 : 2));
+  to[0] = w[0];
+  if (kType == QX_STORAGE_F32) to[1] = w[kType == QX_STORAGE_F32 ? 1 : 0];
+}
+template <int kType>
+__device__ __forceinline__ void from_words(const uint4 (&words)[kType == QX_STORAGE_F32 ? 2 : 1], float (&v)[8]) {
+  const uint32_t w[4] = {words[0].x, words[0].y, words[0].z, words[0].w};
+  if constexpr (kType == QX_STORAGE_F32) {
+    const uint4& high = words[kType == QX_STORAGE_F32 ? 1 : 0];
+    const uint32_t h[4] = {high.x, high.y, high.z, high.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = __uint_as_float(w[i]);
+      v[4 + i] = __uint_as_float(h[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (kType == QX_STORAGE_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = bf16_low(w[i]);
+        v[2 * i + 1] = bf16_high(w[i]);
+      }
+    }
+  }
+}
+template <int kType>
+__device__ __forceinline__ void to_words(const float (&v)[8], uint4 (&words)[kType == QX_STORAGE_F32 ? 2 : 1]) {
+  if constexpr (kType == QX_STORAGE_F32) {
+    words[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    words[kType == QX_STORAGE_F32 ? 1 : 0] =
+        make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (kType == QX_STORAGE_F16) {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    words[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+// The same for a type that only the launch knows. `vector`: the first of them is on a 16-byte boundary.
+template <int kType>
+__device__ __forceinline__ void load8_typed(const uint8_t* data, long long index, float (&v)[8]) {
+  uint4 w[kType == QX_STORAGE_F32 ? 2 : 1];
+  load8_words<kType>(data, index, w);
+  from_words<kType>(w, v);
+}
 __device__ __forceinline__ void load8(const uint8_t* data, int type, int vector, long long index, float (&v)[8]) {
   if (!vector) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = load_one(data, type, index + i);
-    return;
+  } else if (type == QX_STORAGE_F32) {
+    load8_typed<QX_STORAGE_F32>(data, index, v);
+  } else if (type == QX_STORAGE_F16) {
+    load8_typed<QX_STORAGE_F16>(data, index, v);
+  } else {
+    load8_typed<QX_STORAGE_BF16>(data, index, v);
   }
-  if (type == QX_STORAGE_F32) {
-    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(data) + index);
-    const float4 a = p[0], b = p[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    return;
-  }
-  const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(data) + index);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (type == QX_STORAGE_F16) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    } else {
-      v[2 * i] = bf16_low(w[i]);
-      v[2 * i + 1] = bf16_high(w[i]);
-    }
-  }
+}
+template <int kType>
+__device__ __forceinline__ void store8_typed(uint8_t* data, long long index, const float (&v)[8]) {
+  uint4 w[kType == QX_STORAGE_F32 ? 2 : 1];
+  to_words<kType>(v, w);
+  store8_words<kType>(data, index, w);
 }
 __device__ __forceinline__ void store8(uint8_t* data, int type, int vector, long long index, const float (&v)[8]) {
   if (!vector) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) store_one(data, type, index + i, v[i]);
-    return;
+  } else if (type == QX_STORAGE_F32) {
+    store8_typed<QX_STORAGE_F32>(data, index, v);
+  } else if (type == QX_STORAGE_F16) {
+    store8_typed<QX_STORAGE_F16>(data, index, v);
+  } else {
+    store8_typed<QX_STORAGE_BF16>(data, index, v);
   }
-  if (type == QX_STORAGE_F32) {
-    float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(data) + index);
-    p[0] = make_float4(v[0], v[1], v[2], v[3]);
-    p[1] = make_float4(v[4], v[5], v[6], v[7]);
-    return;
-  }
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (type == QX_STORAGE_F16) {
-      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-  }
-  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(data) + index) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A head is cut into units of 16 elements: two runs of eight, at first(u) and second(u), that hold eight
-// whole pairs where the unit is rotated.
+// A head is cut into units of 16 elements, two runs of eight that lie half of the rotated (or of the other) part
+// apart, so that the runs of neighbouring units, neighbouring threads, lie side by side. The runs hold eight whole
+// pairs where the unit is rotated.
 struct Unit {
-  int first, second, pair;  // pair: index of the first of the eight pairs, -1: not rotated
+  int first, second;
+  int pair, second_pair;  // of the first pairs of the runs (QX_ROPE_HALVES: of both), -1: not rotated
 };
-__device__ __forceinline__ Unit unit_of(int u, int rotary, int interleaved) {
-  if (16 * u >= rotary) return {16 * u, 16 * u + 8, -1};
-  if (interleaved) return {16 * u, 16 * u + 8, 8 * u};
-  return {8 * u, 8 * u + rotary / 2, 8 * u};
+__device__ __forceinline__ Unit unit_of(int u, int rotary, int interleaved, int dim) {
+  if (16 * u >= rotary) {
+    const int first = rotary + 8 * (u - rotary / 16);
+    return {first, first + (dim - rotary) / 2, -1, -1};
+  }
+  if (interleaved) return {8 * u, 8 * u + rotary / 2, 4 * u, 4 * u + rotary / 4};
+  return {8 * u, 8 * u + rotary / 2, 8 * u, 8 * u + 4};
 }
-// `table`: {cos, sin} of the token's pairs, times the amplitude.
+// `table`: {cos, sin} of the token's pairs, times the amplitude; two of them are read at a time.
 __device__ __forceinline__ void rotate_unit(const Unit& u, int interleaved, const float2* table, float (&a)[8],
                                             float (&b)[8]) {
   if (u.pair < 0) return;
+  float4 s[2], t[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    s[i] = reinterpret_cast<const float4*>(table + u.pair)[i];
+    t[i] = reinterpret_cast<const float4*>(table + u.second_pair)[i];
+  }
+  const auto turn_pair = [](float& x, float& y, float c, float s) {
+    const float p = x, q = y;
+    x = p * c - q * s;
+    y = p * s + q * c;
+  };
   if (interleaved) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 s = table[u.pair + i], t = table[u.pair + 4 + i];
-      const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
-      a[2 * i] = x * s.x - y * s.y;
-      a[2 * i + 1] = x * s.y + y * s.x;
-      b[2 * i] = z * t.x - w * t.y;
-      b[2 * i + 1] = z * t.y + w * t.x;
+    for (int i = 0; i < 2; ++i) {
+      turn_pair(a[4 * i], a[4 * i + 1], s[i].x, s[i].y);
+      turn_pair(a[4 * i + 2], a[4 * i + 3], s[i].z, s[i].w);
+      turn_pair(b[4 * i], b[4 * i + 1], t[i].x, t[i].y);
+      turn_pair(b[4 * i + 2], b[4 * i + 3], t[i].z, t[i].w);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 s = table[u.pair + i];
-      const float x = a[i], y = b[i];
-      a[i] = x * s.x - y * s.y;
-      b[i] = x * s.y + y * s.x;
+    for (int i = 0; i < 2; ++i) {
+      turn_pair(a[2 * i], b[2 * i], s[i].x, s[i].y);
+      turn_pair(a[2 * i + 1], b[2 * i + 1], s[i].z, s[i].w);
+      turn_pair(a[4 + 2 * i], b[4 + 2 * i], t[i].x, t[i].y);
+      turn_pair(a[5 + 2 * i], b[5 + 2 * i], t[i].z, t[i].w);
     }
   }
 }
+// A thread's way through the (token, head) pairs of a few tokens, `step` pairs at a time, without divisions.
+struct Walk {
+  int token, head, tokens_on, heads_on, heads;
+  __device__ __forceinline__ Walk(int at, int step, int heads_) : heads(heads_) {
+    token = at / heads;
+    head = at - token * heads;
+    tokens_on = step / heads;
+    heads_on = step - tokens_on * heads;
+  }
+  __device__ __forceinline__ void advance() {
+    token += tokens_on;
+    head += heads_on;
+    if (head >= heads) {
+      head -= heads;
+      ++token;
+    }
+  }
+};
 // {cos, sin} of position * turns[pair], times the amplitude. The product is taken in 64 bits and brought to
 // within half a turn there: in 32 bits a position of a million has lost the angle.
 __device__ __forceinline__ float2 turn(const Rotation& r, long long position, int pair) {
@@ -206,6 +281,9 @@ qx_status check_heads(const qx_heads* view, long long rows, int dim, bool writte
 qx_status check_cache(const qx_kv_cache* cache);
 qx_status check_batch(const qx_kv_cache* cache, const qx_kv_batch* batch);
 qx_status check_rope(const qx_rope* rope, int dim);
+// The queries of a batch, at positions[row] or, with positions NULL, at their places in their sequences.
+qx_status launch_rope_batch(const qx_rope* rope, const qx_heads* x, const qx_heads* y, const int64_t* positions,
+                            const Batch& batch, int most, int dim, DeviceContext* ctx, cudaStream_t stream);
 qx_status check_rope_call(const qx_rope* rope, const qx_heads* x, const qx_heads* y, const int64_t* positions,
                           long long tokens, int dim);
 Heads device_heads(const qx_heads* view);

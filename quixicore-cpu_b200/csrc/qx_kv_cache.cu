@@ -2,9 +2,9 @@
 //
 // The unit of work is a (sequence, block that its new tokens reach, kv head) of the keys or of the values:
 // one CTA owns the block's scale and codes, so nothing is atomic and the result does not depend on order.
-// It reads the new elements twice, the second time out of the caches: once for their largest
-// magnitude, once for the codes, because a code needs the block's final scale. Bound by HBM for prompts
-// (element in, code out) and by the chain scale -> codes for single tokens.
+// A code needs the block's final scale, so the new elements wait in registers for it (two units of 16 per thread
+// at most; larger blocks are read twice, the second time out of the caches). Bound by HBM for prompts (element
+// in, code out) and by the chain of loads length -> block -> scale for single tokens.
 
 #include <algorithm>
 #include <limits>
@@ -33,15 +33,31 @@ struct AppendParams {
   int tokens_per_cta, query_ctas;  // of the queries: per CTA, CTAs per sequence
 };
 
-// Code of x: the exact quotient x / scale rounded half to even, whatever the rounding of the product with
-// the inverse did: that is off by one at most, and the remainder x - r * scale is exact in f32 (a
-// multiple of half an ulp of the scale, no larger than the scale).
-__device__ __forceinline__ int code_of(float x, float scale, float inverse) {
-  float r = rintf(x * inverse);
-  const float rest = fmaf(-r, scale, x), half = 0.5f * scale;
-  const bool tie_to_odd = fabsf(rest) == half && (static_cast<int>(r) & 1);
-  if (fabsf(rest) > half || tie_to_odd) r += copysignf(1.0f, rest);
-  return static_cast<int>(fminf(127.0f, fmaxf(-127.0f, r)));
+// Codes of x: the exact quotients x / scale rounded half to even. Added to 1.5 * 2^23 a quotient is rounded to a whole
+// number, whose low byte is the code. That is off by one at most, and only where the remainder x - r * scale, exact in
+// f32 (a multiple of half an ulp of the scale, no larger than the scale), reaches half a scale.
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float scale, float inverse) {
+  constexpr float kZero = 12582912.0f;
+  const float half = 0.5f * scale;
+  float m[8], furthest = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    m[i] = fmaf(x[i], inverse, kZero);
+    furthest = fmaxf(furthest, fabsf(fmaf(-(m[i] - kZero), scale, x[i])));
+  }
+  if (furthest >= half) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float rest = fmaf(-(m[i] - kZero), scale, x[i]);
+      const bool tie_to_odd = fabsf(rest) == half && (__float_as_uint(m[i]) & 1);
+      if (fabsf(rest) > half || tie_to_odd) m[i] += copysignf(1.0f, rest);
+    }
+  }
+  const auto word = [&](int i) {
+    return __byte_perm(__byte_perm(__float_as_uint(m[i]), __float_as_uint(m[i + 1]), 0x40),
+                       __byte_perm(__float_as_uint(m[i + 2]), __float_as_uint(m[i + 3]), 0x40), 0x5410);
+  };
+  return make_uint2(word(0), word(4));
 }
 // An older code on the grown scale: round half to even of code * before / scale. The products have at most
 // 32 bits, so in 64-bit floats they and their difference are exact.
@@ -55,56 +71,54 @@ __device__ __forceinline__ int regrown(int code, double before, double scale, fl
 __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
   return (a & 255) | (b & 255) << 8 | (c & 255) << 16 | static_cast<uint32_t>(d) << 24;
 }
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float scale, float inverse) {
-  int c[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = code_of(v[i], scale, inverse);
-  return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
-}
-
 __device__ __forceinline__ void rotate_queries(const AppendParams& p, long long item, float2* table) {
   const int s = static_cast<int>(item / p.query_ctas), chunk = static_cast<int>(item % p.query_ctas);
   Sequence q;
   if (!sequence_of(p.batch, s, true, &q)) return;
   const int token0 = chunk * p.tokens_per_cta, count = min(p.tokens_per_cta, q.n - token0);
   if (count <= 0) return;
-  const int pairs = p.rotation.rotary / 2, units = p.dim / 16, per_token = p.q.heads * units;
+  const int pairs = p.rotation.rotary / 2, units = p.dim / 16;
   for (int i = threadIdx.x; i < count * pairs; i += kThreads) {
     const int token = token0 + i / pairs;
     const long long position = p.positions != nullptr ? p.positions[q.row + token] : q.length - q.n + token;
     table[i] = turn(p.rotation, position, i % pairs);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < count * per_token; i += kThreads) {
-    const int token = i / per_token, rest = i - token * per_token, head = rest / units;
-    const Unit u = unit_of(rest - head * units, p.rotation.rotary, p.rotation.interleaved);
-    const long long from = (q.row + token0 + token) * p.q.token_stride + head * p.q.head_stride;
-    const long long to = (q.row + token0 + token) * p.q_out.token_stride + head * p.q_out.head_stride;
+  const int at_once = kThreads / units, first = threadIdx.x / units;
+  if (first >= at_once) return;
+  const Unit u = unit_of(static_cast<int>(threadIdx.x) - first * units, p.rotation.rotary, p.rotation.interleaved, p.dim);
+  for (Walk walk(first, at_once, p.q.heads); walk.token < count; walk.advance()) {
+    const long long from = (q.row + token0 + walk.token) * p.q.token_stride + walk.head * p.q.head_stride;
+    const long long to = (q.row + token0 + walk.token) * p.q_out.token_stride + walk.head * p.q_out.head_stride;
     float a[8], b[8];
     load8(p.q.data, p.q.type, p.q.vector, from + u.first, a);
     load8(p.q.data, p.q.type, p.q.vector, from + u.second, b);
-    rotate_unit(u, p.rotation.interleaved, table + token * pairs, a, b);
+    rotate_unit(u, p.rotation.interleaved, table + walk.token * pairs, a, b);
     store8(p.q_out.data, p.q_out.type, p.q_out.vector, to + u.first, a);
     store8(p.q_out.data, p.q_out.type, p.q_out.vector, to + u.second, b);
   }
 }
 
+// kHeld: units of 16 elements that a thread holds in registers as they came, where the block has no more than that
+// many per thread; the next head's are loaded while this one's are written. kType: their type, of keys and values.
+// kHeld 0: any size, types and alignment, each element read twice.
+template <int kHeld, int kType>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendParams p) {
-  extern __shared__ float2 table[];
-  __shared__ uint32_t warp_max[kThreads / 32];
+  extern __shared__ __align__(16) float2 table[];
+  __shared__ uint32_t warp_max[2][kThreads / 32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  const long long per_kind = static_cast<long long>(p.batch.sequences) * p.blocks_per_sequence * p.head_groups;
-  long long item = blockIdx.x;
+  const uint32_t per_kind = static_cast<uint32_t>(p.batch.sequences) * p.blocks_per_sequence * p.head_groups;
+  uint32_t item = blockIdx.x;
   if (item >= 2 * per_kind) {
     rotate_queries(p, item - 2 * per_kind, table);
     return;
   }
   const int kind = item >= per_kind ? 1 : 0;
   item -= kind * per_kind;
-  const int group = static_cast<int>(item % p.head_groups);
-  const long long at = item / p.head_groups;
-  const int s = static_cast<int>(at / p.blocks_per_sequence), reached = static_cast<int>(at % p.blocks_per_sequence);
+  const uint32_t at = item / p.head_groups;
+  const int group = static_cast<int>(item - at * p.head_groups);
+  const int s = static_cast<int>(at / p.blocks_per_sequence), reached = static_cast<int>(at - s * p.blocks_per_sequence);
   Sequence q;
   if (!sequence_of(p.batch, s, true, &q) || q.n == 0) return;
   const int first = q.length - q.n;
@@ -114,52 +128,119 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   const int from = max(first, begin), to = min(q.length, begin + p.block_tokens);
   const int kept = from - begin, count = to - from;  // older tokens of the block, new ones
   const long long row = q.row + (from - first);
+  const Heads& x = p.x[kind];
+  const bool rotated = kind == 0 && p.rotation.rotary > 0;
+  const int pairs = p.rotation.rotary / 2, units = p.dim / 16, total = count * units;
+  const int head0 = group * p.heads_per_cta, head1 = min(p.kv_heads, head0 + p.heads_per_cta);
+
+  constexpr int kUnits = kHeld > 0 ? kHeld : 1, kWords = kType == QX_STORAGE_F32 ? 2 : 1;
+  Unit unit[kUnits];
+  int token[kUnits];
+  long long source[kUnits];
+  uint4 held[kUnits][2][kWords], next[kUnits][2][kWords];
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    const int i = threadIdx.x + k * kThreads;
+    token[k] = i / units;
+    unit[k] = unit_of(i - token[k] * units, rotated ? p.rotation.rotary : 0, p.rotation.interleaved, p.dim);
+    source[k] = (row + token[k]) * x.token_stride + head0 * x.head_stride;
+  }
+  const auto load_held = [&]() {
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      if (threadIdx.x + k * kThreads < total) {
+        load8_words<kType>(x.data, source[k] + unit[k].first, next[k][0]);
+        load8_words<kType>(x.data, source[k] + unit[k].second, next[k][1]);
+        source[k] += x.head_stride;
+      }
+    }
+  };
+  if (kHeld > 0) load_held();  // (needs no block)
+
   const long long block = p.batch.table[s * p.batch.table_stride + block_index];
   if (block < 0 || block >= p.batch.blocks) {
     if (threadIdx.x == 0) sm100::report_error(p.batch.error, kErrorBlock);
     return;
   }
-  const Heads& x = p.x[kind];
-  const bool rotated = kind == 0 && p.rotation.rotary > 0;
-  const int pairs = p.rotation.rotary / 2, units = p.dim / 16;
   if (rotated) {
     for (int i = threadIdx.x; i < count * pairs; i += kThreads) {
-      const int token = i / pairs;
-      const long long position = p.positions != nullptr ? p.positions[row + token] : from + token;
-      table[i] = turn(p.rotation, position, i % pairs);
+      const int t = i / pairs;
+      const long long position = p.positions != nullptr ? p.positions[row + t] : from + t;
+      table[i] = turn(p.rotation, position, i - t * pairs);
     }
+    __syncthreads();
   }
-  const int total = count * units;
-  const int head0 = group * p.heads_per_cta, head1 = min(p.kv_heads, head0 + p.heads_per_cta);
   for (int head = head0; head < head1; ++head) {
-    const auto load_unit = [&](int i, Unit* u, float (&a)[8], float (&b)[8]) {
-      const int token = i / units;
-      *u = unit_of(i - token * units, rotated ? p.rotation.rotary : 0, p.rotation.interleaved);
-      const long long base = (row + token) * x.token_stride + head * x.head_stride;
-      load8(x.data, x.type, x.vector, base + u->first, a);
-      load8(x.data, x.type, x.vector, base + u->second, b);
-      if (rotated) rotate_unit(*u, p.rotation.interleaved, table + token * pairs, a, b);
-      return token;
-    };
     // Magnitudes are compared as bit patterns: above those of all numbers come infinity and NaN.
     uint32_t top = 0;
-    __syncthreads();  // the table is written; warp_max of the head before is read
-    for (int i = threadIdx.x; i < total; i += kThreads) {
-      Unit u;
-      float a[8], b[8];
-      load_unit(i, &u, a, b);
+    const auto measure = [&](const float (&a)[8], const float (&b)[8]) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        top = max(top, max(__float_as_uint(a[k]) & 0x7FFFFFFFu, __float_as_uint(b[k]) & 0x7FFFFFFFu));
+      for (int e = 0; e < 8; ++e) {
+        top = max(top, max(__float_as_uint(a[e]) & 0x7FFFFFFFu, __float_as_uint(b[e]) & 0x7FFFFFFFu));
+      }
+    };
+    const auto held_unit = [&](int k, float (&a)[8], float (&b)[8]) {
+      from_words<kType>(held[k][0], a);
+      from_words<kType>(held[k][1], b);
+      if (rotated) rotate_unit(unit[k], p.rotation.interleaved, table + token[k] * pairs, a, b);
+    };
+    const auto loaded_unit = [&](int i, Unit* u, float (&a)[8], float (&b)[8]) {
+      const int t = i / units;
+      *u = unit_of(i - t * units, rotated ? p.rotation.rotary : 0, p.rotation.interleaved, p.dim);
+      const long long base = (row + t) * x.token_stride + head * x.head_stride;
+      load8(x.data, x.type, x.vector, base + u->first, a);
+      load8(x.data, x.type, x.vector, base + u->second, b);
+      if (rotated) rotate_unit(*u, p.rotation.interleaved, table + t * pairs, a, b);
+      return t;
+    };
+    float* const scale_at = p.scales[kind] + block * p.kv_heads + head;
+    const float before = kept > 0 ? *scale_at : 0.0f;
+    if (kHeld > 0) {
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) {
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+          held[k][0][w] = next[k][0][w];
+          held[k][1][w] = next[k][1][w];
+        }
+      }
+      if (head + 1 < head1) load_held();
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) {
+        if (threadIdx.x + k * kThreads >= total) continue;
+        if (kType != QX_STORAGE_F32 && !rotated) {
+          // two 16-bit patterns at a time; the largest stands for its f32 value
+          uint32_t pair = 0;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint4& w = held[k][r][0];
+            pair = __vimax3_u16x2(pair, w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu);
+            pair = __vimax3_u16x2(pair, w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu);
+          }
+          const uint32_t most = max(pair & 0xFFFFu, pair >> 16);
+          const float value = kType == QX_STORAGE_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(most)))
+                                                      : __uint_as_float(most << 16);
+          top = max(top, __float_as_uint(value));
+        } else {
+          float a[8], b[8];
+          held_unit(k, a, b);
+          measure(a, b);
+        }
+      }
+    } else {
+      for (int i = threadIdx.x; i < total; i += kThreads) {
+        Unit u;
+        float a[8], b[8];
+        loaded_unit(i, &u, a, b);
+        measure(a, b);
       }
     }
     top = __reduce_max_sync(0xFFFFFFFFu, top);
-    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = top;
-    float* const scale_at = p.scales[kind] + block * p.kv_heads + head;
-    const float before = kept > 0 ? *scale_at : 0.0f;
+    // (two sets in turn: the one before is read until the next barrier)
+    if ((threadIdx.x & 31) == 0) warp_max[head & 1][threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) top = max(top, warp_max[w]);
+    for (int w = 0; w < kThreads / 32; ++w) top = max(top, warp_max[head & 1][w]);
     const bool number = top < 0x7F800000u && (__float_as_uint(before) & 0x7FFFFFFFu) < 0x7F800000u;
     float scale = fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), before);
     if (scale < kSmallestScale) scale = 0.0f;
@@ -184,11 +265,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
         *words = v;
       }
     }
-    for (int i = threadIdx.x; i < total; i += kThreads) {
-      Unit u;
-      float a[8], b[8];
-      const int token = load_unit(i, &u, a, b);
-      int8_t* const out = codes + (kept + token) * p.dim;
+    const auto write = [&](const Unit& u, int t, const float (&a)[8], const float (&b)[8]) {
+      int8_t* const out = codes + (kept + t) * p.dim;
       uint2 first8 = make_uint2(0, 0), second8 = make_uint2(0, 0);
       if (number && scale > 0.0f) {
         first8 = codes8(a, scale, inverse);
@@ -196,6 +274,22 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
       }
       *reinterpret_cast<uint2*>(out + u.first) = first8;
       *reinterpret_cast<uint2*>(out + u.second) = second8;
+    };
+    if (kHeld > 0) {
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) {
+        if (threadIdx.x + k * kThreads >= total) continue;
+        float a[8], b[8];
+        held_unit(k, a, b);
+        write(unit[k], token[k], a, b);
+      }
+    } else {
+      for (int i = threadIdx.x; i < total; i += kThreads) {
+        Unit u;
+        float a[8], b[8];
+        const int t = loaded_unit(i, &u, a, b);
+        write(u, t, a, b);
+      }
     }
   }
 }
@@ -206,49 +300,104 @@ struct ReadParams {
   const float* scales[2];
   Heads x[2];  // data NULL: not wanted
   int kv_heads, block_tokens, dim;
-  int tokens_per_cta, chunks;  // chunks of tokens per sequence
+  int blocks_per_sequence, heads_per_cta, head_groups;
 };
 
-// A CTA takes a few tokens with all of their heads: 16 codes in, 16 values out per thread at a time.
+// A CTA takes the tokens that a sequence has in one block, of a few heads: their codes lie together. A thread takes
+// as many codes as give 16 bytes of values (4 of f32, 8 of 16-bit ones), so that a warp's stores lie side by side, and
+// four tokens' at a time.
+template <bool kWide>
+__device__ __forceinline__ void read_plane(const ReadParams& p, int kind, long long block, long long row, int slot, int count,
+                                           int head0, int head1) {
+  const Heads& x = p.x[kind];
+  constexpr int kUnit = kWide ? 4 : 8, kBatch = 4;
+  const int units = p.dim / kUnit, at_once = kThreads / units, first = threadIdx.x / units;
+  if (first >= at_once) return;
+  const int d = (static_cast<int>(threadIdx.x) - first * units) * kUnit;
+  for (int head = head0; head < head1; ++head) {
+    const long long slice = block * p.kv_heads + head;
+    const float scale = __ldg(p.scales[kind] + slice);
+    const int8_t* const codes = p.codes[kind] + (slice * p.block_tokens + slot) * p.dim + d;
+    const long long to = row * x.token_stride + head * x.head_stride + d;
+    for (int t0 = first; t0 < count; t0 += kBatch * at_once) {
+      uint2 words[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int t = t0 + k * at_once;
+        if (t >= count) continue;
+        if (kWide) words[k].x = __ldg(reinterpret_cast<const uint32_t*>(codes + t * p.dim));
+        else words[k] = __ldg(reinterpret_cast<const uint2*>(codes + t * p.dim));
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int t = t0 + k * at_once;
+        if (t >= count) continue;
+        const auto value = [&](uint32_t biased, int byte) {  // 2^23 + (code + 128) as f32 bits
+          return (__uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7440 + byte)) - 8388736.0f) * scale;
+        };
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = value(words[k].x ^ 0x80808080u, e);
+        const long long out = to + t * x.token_stride;
+        if (kWide) {
+          float* const data = reinterpret_cast<float*>(x.data) + out;
+          if (x.vector) {
+            *reinterpret_cast<float4*>(data) = make_float4(v[0], v[1], v[2], v[3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) data[e] = v[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 + e] = value(words[k].y ^ 0x80808080u, e);
+          store8(x.data, x.type, x.vector, out, v);
+        }
+      }
+    }
+  }
+}
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  const int s = static_cast<int>(blockIdx.x / p.chunks), chunk = static_cast<int>(blockIdx.x % p.chunks);
+  const uint32_t at = blockIdx.x / p.head_groups;
+  const int group = static_cast<int>(blockIdx.x - at * p.head_groups);
+  const int s = static_cast<int>(at / p.blocks_per_sequence), reached = static_cast<int>(at - s * p.blocks_per_sequence);
   Sequence q;
-  if (!sequence_of(p.batch, s, true, &q)) return;
-  const int token0 = chunk * p.tokens_per_cta, count = min(p.tokens_per_cta, q.n - token0);
-  if (count <= 0) return;
-  const int units = p.dim / 16, per_token = p.kv_heads * units;
-  for (int i = threadIdx.x; i < 2 * count * per_token; i += kThreads) {
-    const int kind = i >= count * per_token ? 1 : 0;
-    const Heads& x = p.x[kind];
-    if (x.data == nullptr) continue;
-    const int rest0 = i - kind * count * per_token, token = rest0 / per_token, rest = rest0 - token * per_token;
-    const int head = rest / units, unit = rest - head * units;
-    const int position = q.length - q.n + token0 + token;
-    const long long block = p.batch.table[s * p.batch.table_stride + position / p.block_tokens];
-    if (block < 0 || block >= p.batch.blocks) {
-      sm100::report_error(p.batch.error, kErrorBlock);
-      continue;
-    }
-    const long long slice = block * p.kv_heads + head;
-    const float scale = p.scales[kind][slice];
-    const uint4 v = *reinterpret_cast<const uint4*>(
-        p.codes[kind] + (slice * p.block_tokens + position % p.block_tokens) * p.dim + 16 * unit);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    float a[8], b[8];
+  if (!sequence_of(p.batch, s, true, &q) || q.n == 0) return;
+  const int first = q.length - q.n, block_index = first / p.block_tokens + reached, begin = block_index * p.block_tokens;
+  if (begin >= q.length) return;
+  const int from = max(first, begin), count = min(q.length, begin + p.block_tokens) - from;
+  const long long block = p.batch.table[s * p.batch.table_stride + block_index];
+  if (block < 0 || block >= p.batch.blocks) {
+    if (threadIdx.x == 0) sm100::report_error(p.batch.error, kErrorBlock);
+    return;
+  }
+  const long long row = q.row + (from - first);
+  const int head0 = group * p.heads_per_cta, head1 = min(p.kv_heads, head0 + p.heads_per_cta);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      a[e] = static_cast<float>(static_cast<int8_t>(w[e >> 2] >> (8 * (e & 3)))) * scale;
-      b[e] = static_cast<float>(static_cast<int8_t>(w[2 + (e >> 2)] >> (8 * (e & 3)))) * scale;
-    }
-    const long long to = (q.row + token0 + token) * x.token_stride + head * x.head_stride + 16 * unit;
-    store8(x.data, x.type, x.vector, to, a);
-    store8(x.data, x.type, x.vector, to + 8, b);
+  for (int kind = 0; kind < 2; ++kind) {
+    if (p.x[kind].data == nullptr) continue;
+    if (p.x[kind].type == QX_STORAGE_F32) read_plane<true>(p, kind, block, row, from - begin, count, head0, head1);
+    else read_plane<false>(p, kind, block, row, from - begin, count, head0, head1);
   }
 }
 
 int sm_count(DeviceContext* ctx) { return ctx->prop.multiProcessorCount; }
+
+template <int kHeld, int kType>
+qx_status launch_append_of(const AppendParams& p, long long grid, size_t smem, cudaStream_t stream) {
+  static SmemOptIn opt_in;
+  QX_TRY(opt_in.ensure(append_kernel<kHeld, kType>, 128 * 128 * sizeof(float2)));
+  return launch_behind(append_kernel<kHeld, kType>, grid, kThreads, smem, stream, p);
+}
+template <int kType>
+qx_status launch_append_held(const AppendParams& p, int units, long long grid, size_t smem, cudaStream_t stream) {
+  if (units <= kThreads) return launch_append_of<1, kType>(p, grid, smem, stream);
+  return launch_append_of<2, kType>(p, grid, smem, stream);
+}
+
+// Blocks that `most` tokens of one sequence can reach.
+int blocks_reached(int most, int block_tokens) { return most <= 1 ? 1 : 1 + (most - 1 + block_tokens - 1) / block_tokens; }
 
 }  // namespace
 
@@ -391,29 +540,34 @@ qx_status launch_append(const qx_kv_cache* cache, const qx_kv_batch* batch, cons
   p.block_tokens = cache->block_tokens;
   p.dim = cache->head_dim;
   const int most = static_cast<int>(std::min<long long>(batch->max_tokens, batch->max_length));
-  if (most == 0) p.blocks_per_sequence = 1;
-  else p.blocks_per_sequence = 1 + (most - 1 + cache->block_tokens - 1) / cache->block_tokens;
-  // The angles of a block's tokens are shared by the heads that a CTA takes: as many as leave a few CTAs for
-  // every SM. Without a rotation there is nothing to share.
+  p.blocks_per_sequence = blocks_reached(most, cache->block_tokens);
+  // The angles of a block's tokens are shared by the heads that a CTA takes, and the loads of one head run beside
+  // the work on the one before: as many as leave a few CTAs for every SM.
   const long long blocks = static_cast<long long>(batch->sequences) * p.blocks_per_sequence;
   const long long spread = 4LL * sm_count(ctx);
-  long long heads = rope == nullptr ? 1 : blocks * cache->kv_heads / spread;
+  const long long heads = 2 * blocks * cache->kv_heads / (rope != nullptr ? spread : 3 * spread);
   p.heads_per_cta = static_cast<int>(std::min<long long>(std::max<long long>(heads, 1), cache->kv_heads));
   p.head_groups = (cache->kv_heads + p.heads_per_cta - 1) / p.heads_per_cta;
   long long grid = 2 * blocks * p.head_groups;
   const int pairs = p.rotation.rotary / 2;
   size_t smem = static_cast<size_t>(std::min(most, cache->block_tokens)) * pairs * sizeof(float2);
-  if (q != nullptr) {
-    const long long tokens = static_cast<long long>(batch->sequences) * most;
-    p.tokens_per_cta = static_cast<int>(std::min<long long>(
-        std::min<long long>(4, std::max<long long>(1, tokens / spread)), std::max(1, most)));
-    p.query_ctas = (std::max(1, most) + p.tokens_per_cta - 1) / p.tokens_per_cta;
+  const long long tokens = static_cast<long long>(batch->sequences) * most;
+  if (q != nullptr && tokens > spread) {
+    // many queries: a launch of their own, with the registers and shared memory that they need
+    QX_TRY(launch_rope_batch(rope, q, q_out, positions, p.batch, most, cache->head_dim, ctx, stream));
+  } else if (q != nullptr) {
+    p.tokens_per_cta = 1;
+    p.query_ctas = std::max(1, most);
     grid += static_cast<long long>(batch->sequences) * p.query_ctas;
     smem = std::max(smem, static_cast<size_t>(p.tokens_per_cta) * pairs * sizeof(float2));
   }
-  static SmemOptIn opt_in;
-  QX_TRY(opt_in.ensure(append_kernel, 128 * 128 * sizeof(float2)));
-  return launch_behind(append_kernel, grid, kThreads, smem, stream, p);
+  const int units = std::min(most, cache->block_tokens) * (cache->head_dim / 16);
+  if (k->type != v->type || !p.x[0].vector || !p.x[1].vector || units > 2 * kThreads) {
+    return launch_append_of<0, QX_STORAGE_F32>(p, grid, smem, stream);
+  }
+  if (k->type == QX_STORAGE_F32) return launch_append_held<QX_STORAGE_F32>(p, units, grid, smem, stream);
+  if (k->type == QX_STORAGE_F16) return launch_append_held<QX_STORAGE_F16>(p, units, grid, smem, stream);
+  return launch_append_held<QX_STORAGE_BF16>(p, units, grid, smem, stream);
 }
 
 qx_status launch_read(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k, const qx_heads* v,
@@ -432,14 +586,13 @@ qx_status launch_read(const qx_kv_cache* cache, const qx_kv_batch* batch, const 
   p.kv_heads = cache->kv_heads;
   p.block_tokens = cache->block_tokens;
   p.dim = cache->head_dim;
-  // four rounds of the CTA's threads where that leaves a few CTAs for every SM
-  const long long per_token = 2LL * cache->kv_heads * (cache->head_dim / 16);
-  const long long tokens = static_cast<long long>(batch->sequences) * batch->max_tokens;
-  long long t = std::min((4 * kThreads + per_token - 1) / per_token, tokens / (4 * sm_count(ctx)));
-  p.tokens_per_cta = static_cast<int>(std::min<long long>(std::max<long long>(t, 1), batch->max_tokens));
-  if (per_token * p.tokens_per_cta > (1 << 30)) return QX_STATUS_INVALID_SHAPE;
-  p.chunks = (batch->max_tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
-  return launch_behind(read_kernel, static_cast<long long>(batch->sequences) * p.chunks, kThreads, 0, stream, p);
+  p.blocks_per_sequence = blocks_reached(static_cast<int>(std::min<long long>(batch->max_tokens, batch->max_length)), cache->block_tokens);
+  // as many heads per CTA as leave a few CTAs for every SM
+  const long long blocks = static_cast<long long>(batch->sequences) * p.blocks_per_sequence;
+  const long long heads = blocks * cache->kv_heads / (12LL * sm_count(ctx));
+  p.heads_per_cta = static_cast<int>(std::min<long long>(std::max<long long>(heads, 1), cache->kv_heads));
+  p.head_groups = (cache->kv_heads + p.heads_per_cta - 1) / p.heads_per_cta;
+  return launch_behind(read_kernel, blocks * p.head_groups, kThreads, 0, stream, p);
 }
 
 }  // namespace kv

@@ -20,75 +20,113 @@ struct RopeParams {
   const int64_t* positions;
   long long tokens;
   int dim, tokens_per_cta, in_place;
+  int chunks;  // of tokens per sequence of `batch`; 0: the tokens are no batch
+  Batch batch;
   Rotation rotation;
 };
 
+// The rows of a CTA, and the position of the first where positions are places in a sequence.
+struct Span {
+  long long row;
+  int count;
+  long long position;
+};
+template <bool kBatch>
+__device__ __forceinline__ Span span_of(const RopeParams& p) {
+  if (!kBatch) {
+    const long long row = static_cast<long long>(blockIdx.x) * p.tokens_per_cta;
+    return {row, static_cast<int>(min(static_cast<long long>(p.tokens_per_cta), p.tokens - row)), 0};
+  }
+  const int s = static_cast<int>(blockIdx.x / p.chunks), first = static_cast<int>(blockIdx.x % p.chunks) * p.tokens_per_cta;
+  Sequence q;
+  if (!sequence_of(p.batch, s, true, &q)) return {0, 0, 0};
+  return {q.row + first, min(p.tokens_per_cta, q.n - first), q.length - q.n + first};
+}
+template <bool kBatch>
+__device__ __forceinline__ float2 turn_of(const RopeParams& p, const Span& span, int token, int pair) {
+  return turn(p.rotation, !kBatch || p.positions != nullptr ? p.positions[span.row + token] : span.position + token, pair);
+}
+
 constexpr int kRopeThreads = 256;
 
-// Whole units of 16 elements (head size and rotary part are multiples of 16), any alignment.
-template <int kType>
-__global__ void __launch_bounds__(kRopeThreads) rope_units_kernel(const __grid_constant__ RopeParams p) {
-  extern __shared__ float2 table[];
+// Whole units of 16 elements: head size and rotary part are multiples of 16, runs start on 16-byte boundaries.
+template <int kType, bool kBatch>
+__global__ void __launch_bounds__(kRopeThreads, 3) rope_units_kernel(const __grid_constant__ RopeParams p) {
+  extern __shared__ __align__(16) float2 table[];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const int pairs = p.rotation.rotary / 2;
-  const long long token0 = static_cast<long long>(blockIdx.x) * p.tokens_per_cta;
-  const int count = static_cast<int>(min(static_cast<long long>(p.tokens_per_cta), p.tokens - token0));
-  const int per_head = p.dim / 16;
-  const int units = p.in_place ? p.rotation.rotary / 16 : per_head;  // (in place the rest is where it belongs)
-  const int per_token = p.x.heads * units;
+  const Span span = span_of<kBatch>(p);
+  const int count = span.count;
+  if (count <= 0) return;
+  const int units = p.in_place ? p.rotation.rotary / 16 : p.dim / 16;  // (in place the rest is where it belongs)
+  // a thread keeps its unit of the head and walks the (token, head) pairs; the first elements are under way while
+  // the angles are taken
+  const int at_once = kRopeThreads / units, first = threadIdx.x / units;
+  const Unit unit = unit_of(static_cast<int>(threadIdx.x) - first * units, p.rotation.rotary, p.rotation.interleaved, p.dim);
+  Walk walk(first, at_once, p.x.heads);
+  if (first >= at_once) walk.token = count;  // (threads that are no whole row of units)
+  constexpr int kWords = kType == QX_STORAGE_F32 ? 2 : 1;
+  constexpr int kUnits = kType == QX_STORAGE_F32 ? 2 : 4;  // eight 16-byte loads in flight per thread
+  uint4 a[kUnits][kWords], b[kUnits][kWords];
+  int token[kUnits], head[kUnits];
+  const auto load = [&]() {
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      token[k] = walk.token;
+      head[k] = walk.head;
+      walk.advance();
+      if (token[k] >= count) continue;
+      const long long from = (span.row + token[k]) * p.x.token_stride + head[k] * p.x.head_stride;
+      load8_words<kType>(p.x.data, from + unit.first, a[k]);
+      load8_words<kType>(p.x.data, from + unit.second, b[k]);
+    }
+  };
+  load();
   for (int i = threadIdx.x; i < count * pairs; i += kRopeThreads) {
-    table[i] = turn(p.rotation, p.positions[token0 + i / pairs], i % pairs);
+    table[i] = turn_of<kBatch>(p, span, i / pairs, i % pairs);
   }
   __syncthreads();
-  // two units at a time: four 16-byte loads in flight per thread
-  constexpr int kBatch = 2;
-  const int total = count * per_token;
-  for (int i = threadIdx.x; i < total; i += kBatch * kRopeThreads) {
-    float a[kBatch][8], b[kBatch][8];
-    Unit unit[kBatch];
-    long long to[kBatch];
-    int token[kBatch];
+  while (token[0] < count) {
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int j = i + k * kRopeThreads;
-      if (j >= total) break;
-      token[k] = j / per_token;
-      const int rest = j - token[k] * per_token, head = rest / units;
-      unit[k] = unit_of(rest - head * units, p.rotation.rotary, p.rotation.interleaved);
-      const long long from = (token0 + token[k]) * p.x.token_stride + head * p.x.head_stride;
-      to[k] = (token0 + token[k]) * p.y.token_stride + head * p.y.head_stride;
-      load8(p.x.data, kType, p.x.vector, from + unit[k].first, a[k]);
-      load8(p.x.data, kType, p.x.vector, from + unit[k].second, b[k]);
+    for (int k = 0; k < kUnits; ++k) {
+      if (token[k] >= count) continue;
+      if (unit.pair >= 0) {
+        float x[8], y[8];
+        from_words<kType>(a[k], x);
+        from_words<kType>(b[k], y);
+        rotate_unit(unit, p.rotation.interleaved, table + token[k] * pairs, x, y);
+        to_words<kType>(x, a[k]);
+        to_words<kType>(y, b[k]);
+      }
+      const long long to = (span.row + token[k]) * p.y.token_stride + head[k] * p.y.head_stride;
+      store8_words<kType>(p.y.data, to + unit.first, a[k]);
+      store8_words<kType>(p.y.data, to + unit.second, b[k]);
     }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (i + k * kRopeThreads >= total) break;
-      rotate_unit(unit[k], p.rotation.interleaved, table + token[k] * pairs, a[k], b[k]);
-      store8(p.y.data, kType, p.y.vector, to[k] + unit[k].first, a[k]);
-      store8(p.y.data, kType, p.y.vector, to[k] + unit[k].second, b[k]);
-    }
+    load();
   }
 }
 
 // Any head size and any even rotary part: one pair, or one element behind them, at a time.
+template <bool kBatch>
 __global__ void __launch_bounds__(kRopeThreads) rope_pairs_kernel(const __grid_constant__ RopeParams p) {
-  extern __shared__ float2 table[];
+  extern __shared__ __align__(16) float2 table[];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const int rotary = p.rotation.rotary, pairs = rotary / 2;
-  const long long token0 = static_cast<long long>(blockIdx.x) * p.tokens_per_cta;
-  const int count = static_cast<int>(min(static_cast<long long>(p.tokens_per_cta), p.tokens - token0));
+  const Span span = span_of<kBatch>(p);
+  const int count = span.count;
+  if (count <= 0) return;
   const int per_head = pairs + (p.in_place ? 0 : p.dim - rotary);
   const int per_token = p.x.heads * per_head;
   for (int i = threadIdx.x; i < count * pairs; i += kRopeThreads) {
-    table[i] = turn(p.rotation, p.positions[token0 + i / pairs], i % pairs);
+    table[i] = turn_of<kBatch>(p, span, i / pairs, i % pairs);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < count * per_token; i += kRopeThreads) {
     const int token = i / per_token, rest = i - token * per_token, head = rest / per_head, e = rest - head * per_head;
-    const long long from = (token0 + token) * p.x.token_stride + head * p.x.head_stride;
-    const long long to = (token0 + token) * p.y.token_stride + head * p.y.head_stride;
+    const long long from = (span.row + token) * p.x.token_stride + head * p.x.head_stride;
+    const long long to = (span.row + token) * p.y.token_stride + head * p.y.head_stride;
     if (e >= pairs) {
       store_one(p.y.data, p.y.type, to + rotary + (e - pairs), load_one(p.x.data, p.x.type, from + rotary + (e - pairs)));
       continue;
@@ -144,9 +182,18 @@ qx_status check_rope_call(const qx_rope* rope, const qx_heads* x, const qx_heads
 
 namespace {
 
-qx_status launch_rope(const qx_rope* rope, const qx_heads* x, const qx_heads* y, const int64_t* positions,
+template <bool kBatch>
+qx_status launch_sized(const RopeParams& p, bool whole, int type, long long grid, size_t smem, cudaStream_t stream) {
+  if (!whole) return launch_behind(rope_pairs_kernel<kBatch>, grid, kRopeThreads, smem, stream, p);
+  switch (type) {
+    case QX_STORAGE_F32: return launch_behind(rope_units_kernel<QX_STORAGE_F32, kBatch>, grid, kRopeThreads, smem, stream, p);
+    case QX_STORAGE_F16: return launch_behind(rope_units_kernel<QX_STORAGE_F16, kBatch>, grid, kRopeThreads, smem, stream, p);
+    default: return launch_behind(rope_units_kernel<QX_STORAGE_BF16, kBatch>, grid, kRopeThreads, smem, stream, p);
+  }
+}
+
+qx_status launch_rope(RopeParams& p, const qx_rope* rope, const qx_heads* x, const qx_heads* y, const int64_t* positions,
                       long long tokens, int dim, bool inverse, DeviceContext* ctx, cudaStream_t stream) {
-  RopeParams p{};
   p.x = device_heads(x);
   p.y = device_heads(y);
   p.positions = positions;
@@ -154,7 +201,7 @@ qx_status launch_rope(const qx_rope* rope, const qx_heads* x, const qx_heads* y,
   p.dim = dim;
   p.in_place = x->data == y->data;
   p.rotation = device_rotation(rope, inverse);
-  const bool whole = dim % 16 == 0 && rope->rotary_dim % 16 == 0;
+  const bool whole = dim % 16 == 0 && rope->rotary_dim % 16 == 0 && p.x.vector && p.y.vector;
   // Tokens per CTA: enough for four rounds of its threads where there are CTAs for every SM all the same,
   // and no more than 16 KB of {cos, sin}.
   const long long per_token = static_cast<long long>(x->heads) * (whole ? dim / 16 : dim);
@@ -164,17 +211,26 @@ qx_status launch_rope(const qx_rope* rope, const qx_heads* x, const qx_heads* y,
   t = std::min<long long>(t, (tokens + 4 * ctx->prop.multiProcessorCount - 1) / (4 * ctx->prop.multiProcessorCount));
   p.tokens_per_cta = static_cast<int>(std::max<long long>(t, 1));
   if (per_token * p.tokens_per_cta > (1 << 28)) return QX_STATUS_INVALID_SHAPE;
-  const long long grid = (tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
-  const size_t smem = static_cast<size_t>(p.tokens_per_cta) * pairs * sizeof(float2);
-  if (!whole) return launch_behind(rope_pairs_kernel, grid, kRopeThreads, smem, stream, p);
-  switch (x->type) {
-    case QX_STORAGE_F32: return launch_behind(rope_units_kernel<QX_STORAGE_F32>, grid, kRopeThreads, smem, stream, p);
-    case QX_STORAGE_F16: return launch_behind(rope_units_kernel<QX_STORAGE_F16>, grid, kRopeThreads, smem, stream, p);
-    default: return launch_behind(rope_units_kernel<QX_STORAGE_BF16>, grid, kRopeThreads, smem, stream, p);
+  long long grid = (tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
+  if (p.chunks > 0) {  // (so far: the most tokens of a sequence)
+    p.chunks = (p.chunks + p.tokens_per_cta - 1) / p.tokens_per_cta;
+    grid = static_cast<long long>(p.batch.sequences) * p.chunks;
   }
+  const size_t smem = static_cast<size_t>(p.tokens_per_cta) * pairs * sizeof(float2);
+  if (p.chunks > 0) return launch_sized<true>(p, whole, x->type, grid, smem, stream);
+  return launch_sized<false>(p, whole, x->type, grid, smem, stream);
 }
 
 }  // namespace
+
+qx_status launch_rope_batch(const qx_rope* rope, const qx_heads* x, const qx_heads* y, const int64_t* positions,
+                            const Batch& batch, int most, int dim, DeviceContext* ctx, cudaStream_t stream) {
+  RopeParams p{};
+  p.batch = batch;
+  p.chunks = std::max(1, most);
+  return launch_rope(p, rope, x, y, positions, static_cast<long long>(batch.sequences) * most, dim, false, ctx, stream);
+}
+
 }  // namespace kv
 }  // namespace qx
 
@@ -231,7 +287,8 @@ qx_status qx_rope_apply_dev(const qx_rope* rope, const qx_heads* x, const qx_hea
   DeviceContext* ctx = nullptr;
   QX_TRY(current_context(&ctx));
   if (tokens == 0) return QX_STATUS_OK;
-  return kv::launch_rope(rope, x, y, positions_dev, tokens, head_dim, inverse != 0, ctx, static_cast<cudaStream_t>(stream));
+  kv::RopeParams p{};
+  return kv::launch_rope(p, rope, x, y, positions_dev, tokens, head_dim, inverse != 0, ctx, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
