@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
   int s, head, row_tile = 0, begin, end;
   long long part;           // where partial results go
   uint32_t first_part = 0;  // balanced: the first CTA that holds a part of the item
+  uint32_t tile_index = 0;  // the item's number
   int parts = 1;
   Rows rows;
   if (kBalanced) {
@@ -240,13 +241,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
     parts = static_cast<int>((item_end - 1) / line.piece - first_part) + 1;
     part = 2LL * blockIdx.x + (first_part == blockIdx.x ? 1 : 0);
     (void)rows_of(p, s, 0, kRows, &rows);
+    tile_index = s * p.kv_heads + head;
     const int unit0 = max(0, static_cast<int>(place - item_begin) - kItemCost), unit1 = max(0, static_cast<int>(stop - item_begin) - kItemCost);
     begin = rows.low + unit0 * kTile;
     end = min(rows.high, rows.low + unit1 * kTile);
     place = stop;
   } else {
     if (!once) return;
-    const uint32_t tile_index = blockIdx.x / p.splits, split = blockIdx.x - tile_index * p.splits;
+    const uint32_t split = blockIdx.x % p.splits;
+    tile_index = blockIdx.x / p.splits;
     const uint32_t index = tile_index / p.row_tiles;
     row_tile = static_cast<int>(tile_index - index * p.row_tiles);
     s = static_cast<int>(index / p.kv_heads);
@@ -706,13 +709,13 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
           total == 0.0f ? -INFINITY : (top + log2f(total) - kShift) * 0.69314718055994531f;
     }
   }
-  if (kBalanced) {
+  if (kBalanced || p.counters != nullptr) {
     if (!whole) {
       // The CTA that arrives last at the item's counter joins its parts, all of them from memory and in their order.
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
-        int* const counter = p.counters + s * p.kv_heads + head;
+        int* const counter = p.counters + tile_index;
         last_part = atomicAdd(counter, 1) == parts - 1;
         if (last_part) *counter = 0;
       }
@@ -731,7 +734,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
               // (the item begins behind others in its first CTA, and at the start of the following ones)
-              const long long from = (2LL * (first_part + q0 + b) + (q0 + b == 0 ? 1 : 0)) * kRows + r;
+              const long long from = (kBalanced ? 2LL * (first_part + q0 + b) + (q0 + b == 0 ? 1 : 0)
+                                                : static_cast<long long>(tile_index) * p.splits + q0 + b) * kRows + r;
               stat[b] = make_float2(-INFINITY, 0.0f);
               x[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
               if (q0 + b < parts) {
@@ -952,10 +956,14 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
     QX_TRY(workspace->reserve(kWorkspaceCounterBytes + sums + rows * 2 * sizeof(float)));
     p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace->base) + kWorkspaceCounterBytes);
     p.statistics = p.partial + sums / sizeof(float);
+    // few parts are joined by the last CTA to arrive, which saves a launch; many by a kernel that spreads them out
+    if (!prompt && p.splits <= 16 && items <= static_cast<long long>(kWorkspaceCounterBytes / sizeof(int))) {
+      p.counters = static_cast<int*>(workspace->base);
+    }
   }
   const long long grid = items * p.splits;
   QX_TRY(prompt ? launch_prompt(p, grid, stream) : launch_sized(p, dp, wide, false, grid, stream));
-  return p.splits > 1 ? launch_behind(join_kernel, items * p.tile_rows, p.splits <= 16 ? 128 : kJoinThreads, 0, stream, p) : QX_STATUS_OK;
+  return p.splits > 1 && p.counters == nullptr ? launch_behind(join_kernel, items * p.tile_rows, p.splits <= 16 ? 128 : kJoinThreads, 0, stream, p) : QX_STATUS_OK;
 }
 
 }  // namespace kv

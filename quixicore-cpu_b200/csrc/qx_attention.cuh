@@ -24,7 +24,7 @@ struct AttentionParams {
   float shift;       // log2 of what sums of weights carry
   float* partial;    // [tile][split][rows][dim] sums, then [tile][split][rows] {maximum, sum}
   float* statistics;
-  int* counters;     // [sequence][kv head] arrivals of a balanced launch, zero between calls
+  int* counters;     // [item] CTAs that have written a part, zero between calls; NULL: another kernel joins
 };
 
 // A tile's rows are (token, query head of the group) pairs of one sequence and kv head, token major.
