@@ -46,7 +46,7 @@ constexpr float kShift = 12.0f;
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 32;
 constexpr uint32_t kZeroSum = 0x4B400000u;  // 1.5 * 2^23: whole numbers below 2^22 added to the bits are exact
 
-// Rows per sequence from which 16-bit queries take the prompt kernel.
+// Rows per sequence from which queries take the prompt kernel.
 constexpr long long kPromptFrom = 64;
 
 // CTAs per SM, as many as shared memory and 65536 registers hold.
@@ -911,8 +911,9 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   p.window = static_cast<int>(std::min<long long>(window, 0x7FFFFFFF));
   p.group = q->heads / cache->kv_heads;
   const long long most_rows = static_cast<long long>(batch->max_tokens) * p.group;
-  const bool prompt = q->type != QX_STORAGE_F32 && cache->head_dim <= 128 && most_rows >= kPromptFrom;
-  p.tile_rows = prompt ? kPromptRows : most_rows <= 8 ? 8 : 16;
+  const bool wide = q->type == QX_STORAGE_F32;
+  const bool prompt = cache->head_dim <= 128 && most_rows >= kPromptFrom;
+  p.tile_rows = prompt ? (wide ? kPromptRowsWide : kPromptRows) : most_rows <= 8 ? 8 : 16;
   p.shift = prompt ? kPromptShift : kShift;
   p.row_tiles = static_cast<int>((most_rows + p.tile_rows - 1) / p.tile_rows);
   const long long items = static_cast<long long>(batch->sequences) * cache->kv_heads * p.row_tiles;
@@ -926,7 +927,6 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   // below a tile per warp (in the prompt kernel, four tiles): then the joining would cost more than the keys.
   const int dp = cache->head_dim <= 64 ? 64 : cache->head_dim <= 128 ? 128 : 256;
   const long long slots = static_cast<long long>(ctx->prop.multiProcessorCount) * (prompt ? 1 : streamed_ctas(dp, p.tile_rows / 8));
-  const bool wide = q->type == QX_STORAGE_F32;
   // Balanced: several sequences, and items enough that each has few parts to join (by one CTA, at about 0.15 us a part).
   const long long counters = static_cast<long long>(batch->sequences) * cache->kv_heads;
   const long long units = counters * ((range + kTile - 1) / kTile + kItemCost);
@@ -962,7 +962,7 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
     }
   }
   const long long grid = items * p.splits;
-  QX_TRY(prompt ? launch_prompt(p, grid, stream) : launch_sized(p, dp, wide, false, grid, stream));
+  QX_TRY(prompt ? launch_prompt(p, wide, grid, stream) : launch_sized(p, dp, wide, false, grid, stream));
   return p.splits > 1 && p.counters == nullptr ? launch_behind(join_kernel, items * p.tile_rows, p.splits <= 16 ? 128 : kJoinThreads, 0, stream, p) : QX_STATUS_OK;
 }
 

@@ -70,10 +70,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Rows per CTA of the prompt kernel (qx_attention_tc.cu), and its shift: P is held times 2^11 .. 2^15 there.
-constexpr int kPromptRows = 256;
+// Rows per CTA of the prompt kernel (qx_attention_tc.cu; f32 queries), and its shift: P is held times 2^11 .. 2^15
+// there.
+constexpr int kPromptRows = 256, kPromptRowsWide = 128;
 constexpr float kPromptShift = 11.0f;
-qx_status launch_prompt(const AttentionParams& p, long long grid, cudaStream_t stream);
+qx_status launch_prompt(const AttentionParams& p, bool wide, long long grid, cudaStream_t stream);
 
 }  // namespace kv
 }  // namespace qx

@@ -21,6 +21,12 @@
 // of the largest value.) m only follows when it has fallen 4 behind (a factor of 16): then the row's sum and O
 // are scaled, in TMEM, by the row's own warp, which is rare after the first tiles.
 //
+// f32 queries (kWide) take one tile of 128 rows per CTA, whose queries and weights are f16 pairs, hi + lo, of 22 bits:
+// the second tile's place in shared memory holds the low halves of the queries, the second half of S the low halves
+// of the weights, and every product is two. A sum over all keys would lose f32's last bits to the MMA's own
+// additions, so each tile's product goes to one of two buffers of O, and warps 4-7 add those up in registers, in
+// f32, with the maxima's changes in between.
+//
 // Every wait is bounded; one that runs out raises the CTA's abort flag, all roles leave their loops, MMAs
 // in flight are waited for (bounded) and TMEM is freed.
 
@@ -40,7 +46,8 @@ constexpr int kRowTile = 128, kKeys = 128, kGroups = kKeys / 16;
 constexpr int kConvertWarps = 4, kTcThreads = 512;
 constexpr int kSoftmaxRegisters = 192, kOtherRegisters = 64;  // of 128 at launch: 256 * 192 + 256 * 64 = 512 * 128
 constexpr int kMetaStages = 4;
-static_assert(kPromptRows == 2 * kRowTile, "two tiles per CTA");
+static_assert(kPromptRows == 2 * kRowTile && kPromptRowsWide == kRowTile, "two tiles per CTA, f32: one");
+constexpr int kKeepStages = 4;
 constexpr float kBehind = 4.0f;
 constexpr float kLeastLog = -100.0f;  // of a value scale: append makes no smaller one but zero
 
@@ -56,6 +63,7 @@ struct Meta {
 struct Barriers {
   uint64_t queries[2], key_full[2], key_empty[2], value_full[2], value_empty[2];
   uint64_t scores[2], halves[2], weights[2], sums[2], meta[kMetaStages], drain;
+  uint64_t kept[kKeepStages], taken[2], gain;  // kWide: factors written, buffers of O read, last factors written
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -67,7 +75,8 @@ struct TcShape {
   static constexpr int kKeyRing = kQueries + 2 * kOperand;
   static constexpr int kValueRing = kKeyRing + 2 * kOperand;
   static constexpr int kMeta = kValueRing + 2 * kOperand;
-  static constexpr int kBars = kMeta + kMetaStages * static_cast<int>(sizeof(Meta));
+  static constexpr int kKeep = kMeta + kMetaStages * static_cast<int>(sizeof(Meta));  // kWide: [stage][row], [row]
+  static constexpr int kBars = kKeep + (kKeepStages + 1) * kRowTile * 4;
   static constexpr int kBytes = kBars + static_cast<int>(sizeof(Barriers)) + 1024;  // (the operands start on 1024)
 };
 
@@ -149,6 +158,12 @@ __device__ __forceinline__ uint4 load8_raw(const uint8_t* data, int vector, long
   return make_uint4(from[0] | from[1] << 16, from[2] | from[3] << 16, from[4] | from[5] << 16, from[6] | from[7] << 16);
 }
 
+__device__ __forceinline__ uint4 load4_raw(const uint8_t* data, int vector, long long index) {
+  const uint32_t* const from = reinterpret_cast<const uint32_t*>(data) + index;
+  if (vector) return *reinterpret_cast<const uint4*>(from);
+  return make_uint4(from[0], from[1], from[2], from[3]);
+}
+
 // What a softmax thread knows about its row.
 struct RowState {
   float factor;       // of the raw scores, log2(e) in it
@@ -159,9 +174,10 @@ struct RowState {
 
 // One tile of scores to weights, in TMEM. `scores`: this warp's lanes of S, which P replaces; `sums`: of O. Keys
 // share scales by `kUnit`s of 16 or 32.
-template <int DP, int kUnit, bool kMasked>
+// kWide: the row's factor for what O holds so far goes to *keep_to instead.
+template <int DP, int kUnit, bool kMasked, bool kWide>
 __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, const Meta& meta, RowState& row, int key0,
-                                             bool first, uint64_t* first_half) {
+                                             bool first, uint64_t* first_half, float* keep_to) {
   constexpr int kUnits = kKeys / kUnit, kPerUnit = kUnit / 16;
   uint32_t s[4][32];
   tmem_ld_32x32(scores, s[0]);
@@ -224,7 +240,13 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   for (int u = kUnits / 2; u < kUnits; ++u) top_of(u);
 
   const bool behind = top > row.maximum + kBehind;  // (from -infinity on, any score is)
-  if (__any_sync(0xFFFFFFFFu, behind)) {
+  if (kWide) {
+    const float before = row.maximum;
+    if (behind) row.maximum = top;
+    const float keep = before == row.maximum ? 1.0f : exp2_fast(before - row.maximum);
+    row.sum *= keep;
+    *keep_to = keep;
+  } else if (__any_sync(0xFFFFFFFFu, behind)) {
     const float before = row.maximum;
     if (behind) row.maximum = top;
     const float keep = before == row.maximum ? 1.0f : exp2_fast(before - row.maximum);
@@ -244,7 +266,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   const float base = (row.maximum == -INFINITY ? 0.0f : row.maximum) - kPromptShift;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    uint32_t p[16];
+    uint32_t p[16], low[16];
 #pragma unroll
     for (int h = 0; h < 32 / kUnit; ++h) {
       const int u = c * (32 / kUnit) + h;
@@ -266,6 +288,11 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
         }
         const __half2 w = __floats2half2_rn(a, b);
         p[at / 2] = *reinterpret_cast<const uint32_t*>(&w);
+        if (kWide) {
+          const float2 rounded = __half22float2(w);
+          const __half2 rest = __floats2half2_rn(a - rounded.x, b - rounded.y);
+          low[at / 2] = *reinterpret_cast<const uint32_t*>(&rest);
+        }
         sum2 = tile::addf2(sum2, tile::pack2(__float_as_uint(a), __float_as_uint(b)));
       }
       uint32_t lo, hi;
@@ -275,7 +302,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
       if (!kMasked || sum != 0.0f) row.sum = fmaf(sum, relative[u], row.sum);
     }
     tmem_st_32x16(scores + 16 * c, p);
-    if (c == 1) {  // the product with the first half of the keys' values may begin
+    if (kWide) tmem_st_32x16(scores + kKeys / 2 + 16 * c, low);
+    if (!kWide && c == 1) {  // the product with the first half of the keys' values may begin
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
@@ -285,12 +313,33 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   tmem_st_wait();
 }
 
-template <int DP, int kUnit>
+// 32 elements of a row of O, from element c of the head on, times `gain`, to the output or the partial results.
+__device__ __forceinline__ void write_row(const AttentionParams& p, const uint32_t (&o)[32], float gain, bool whole, long long at,
+                                          long long row, long long head, int c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (c + 8 * i >= p.dim) break;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = gain == 0.0f ? 0.0f : __uint_as_float(o[8 * i + e]) * gain;  // (O may be unset)
+    if (whole) {
+      store8(p.out.data, p.out.type, p.out.vector, row * p.out.token_stride + head * p.out.head_stride + c + 8 * i, v);
+    } else {
+      float4* const partial = reinterpret_cast<float4*>(p.partial + at * p.dim + c + 8 * i);
+      partial[0] = make_float4(v[0], v[1], v[2], v[3]);
+      partial[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  }
+}
+
+template <int DP, int kUnit, bool kWide>
 __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_constant__ AttentionParams p) {
   using S = TcShape<DP>;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
   Meta* const meta = reinterpret_cast<Meta*>(smem + S::kMeta);
+  float* const keep = reinterpret_cast<float*>(smem + S::kKeep);
+  float* const gains = keep + kKeepStages * kRowTile;
   Barriers* const bars = reinterpret_cast<Barriers*>(smem + S::kBars);
   volatile int* const abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -306,11 +355,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   const long long tile_index = index * p.row_tiles + row_tile;
   const int head = static_cast<int>(index % p.kv_heads), s = static_cast<int>(index / p.kv_heads);
   Rows rows;
-  if (!rows_of(p, s, row_tile * 2 * kRowTile, 2 * kRowTile, &rows)) return;
+  constexpr int kCtaRows = kWide ? kRowTile : 2 * kRowTile;
+  if (!rows_of(p, s, row_tile * kCtaRows, kCtaRows, &rows)) return;
   int begin, end;
   if (!chunk_of(p, rows, split, &begin, &end)) return;
   const int tiles = max(0, (end - begin + kKeys - 1) / kKeys);
-  const int row_tiles = rows.count > kRowTile ? 2 : 1;
+  const int row_tiles = !kWide && rows.count > kRowTile ? 2 : 1;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -325,6 +375,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       mbar_init(&bars->sums[i], 1);
     }
     for (int i = 0; i < kMetaStages; ++i) mbar_init(&bars->meta[i], kConvertWarps);
+    for (int i = 0; i < kKeepStages; ++i) mbar_init(&bars->kept[i], 4);
+    mbar_init(&bars->taken[0], 4);
+    mbar_init(&bars->taken[1], 4);
+    mbar_init(&bars->gain, 4);
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
     mbar_fence_init();
@@ -343,7 +397,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
     // ---- softmax --------------------------------------------------------------------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
     const int which = warp >> 2;
-    if (which < row_tiles) {
+    if (kWide && which == 1) {
+      // ---- the tiles' products added up, f32 -------------------------------------------------
+      const int r = threadIdx.x & 127;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      uint32_t total[DP / 32][32];
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) total[c][i] = 0;
+      }
+      for (int j = 0; ok && j < tiles; ++j) {
+        ok = mbar_wait_warp(&bars->kept[j % kKeepStages], j / kKeepStages & 1, abort_flag) &&
+             mbar_wait_warp(&bars->sums[j & 1], j >> 1 & 1, abort_flag);
+        if (!ok) break;
+        __syncwarp();
+        tc_fence_after_sync();
+        const float factor = keep[j % kKeepStages * kRowTile + r];
+        const uint32_t product = tmem + lanes + 256 + (j & 1) * 128;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32(product + 32 * c, o);
+          tmem_ld_wait_for(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            total[c][i] = __float_as_uint(fmaf(__uint_as_float(total[c][i]), factor, __uint_as_float(o[i])));
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->taken[j & 1]);
+      }
+      if (ok) ok = mbar_wait_warp(&bars->gain, 0, abort_flag);
+      if (ok && r < rows.count) {
+        const int token = (rows.first + r) / p.group, member = (rows.first + r) % p.group;
+        const bool whole = splits_used(p, rows) == 1;
+        const long long at = (tile_index * p.splits + split) * kCtaRows + r;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+          write_row(p, total[c], gains[r], whole, at, rows.row + token, static_cast<long long>(head) * p.group + member, 32 * c);
+        }
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        report_error(p.batch.error, 44);
+      }
+    } else if (which < row_tiles) {
       const int r = threadIdx.x & 127, in_tile = which * kRowTile + r;
       const bool real = in_tile < rows.count;
       const int start = rows.length - rows.n;
@@ -363,11 +463,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       {
         const long long from = row_at * p.q.token_stride + out_head * p.q.head_stride;
         // the whole row in registers: all of its loads are in flight at once
-        uint4 raw[DP / 8];
+        constexpr int kWords = kWide ? 2 : 1;
+        uint4 raw[DP / 8][kWords];
 #pragma unroll
         for (int c = 0; c < DP / 8; ++c) {
-          raw[c] = make_uint4(0, 0, 0, 0);
-          if (real && 8 * c < p.dim) raw[c] = load8_raw(p.q.data, p.q.vector, from + 8 * c);
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) {
+            raw[c][w] = make_uint4(0, 0, 0, 0);
+            if (real && 8 * c < p.dim) raw[c][w] = kWide ? load4_raw(p.q.data, p.q.vector, from + 8 * c + 4 * w) : load8_raw(p.q.data, p.q.vector, from + 8 * c);
+          }
         }
         const bool f16 = p.q.type == QX_STORAGE_F16;
         const auto pair = [&](uint32_t w) {
@@ -376,11 +480,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         uint32_t top = 0;  // of the bit patterns without sign: they grow with the magnitude
 #pragma unroll
         for (int c = 0; c < DP / 8; ++c) {
-          const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7FFFu, w[i] >> 16 & 0x7FFFu));
+          for (int k = 0; k < kWords; ++k) {
+            const uint32_t w[4] = {raw[c][k].x, raw[c][k].y, raw[c][k].z, raw[c][k].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = kWide ? max(top, w[i] & 0x7FFFFFFFu) : max(top, max(w[i] & 0x7FFFu, w[i] >> 16 & 0x7FFFu));
+          }
         }
-        top = __float_as_uint(pair(top).x) >> 23;
+        top = (kWide ? top : __float_as_uint(pair(top).x)) >> 23;
         const int shift = top >= 255 ? 0 : min(120, max(-120, 134 - static_cast<int>(top)));
         // (a negative scale turns the query's sign, so that larger raw scores are larger scores)
         const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
@@ -388,15 +495,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         uint8_t* const to = smem + S::kQueries + which * S::kOperand + r * 128;
 #pragma unroll
         for (int c = 0; c < DP / 8; ++c) {
-          uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+          const uint4 &first = raw[c][0], &second = raw[c][kWords - 1];
+          const uint32_t in[8] = {first.x, first.y, first.z, first.w, second.x, second.y, second.z, second.w};
+          uint32_t w[4], low[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = pair(w[i]);
+            const float2 v = kWide ? make_float2(__uint_as_float(in[2 * i]), __uint_as_float(in[2 * i + 1])) : pair(in[i]);
             const __half2 h = __floats2half2_rn(v.x * up, v.y * up);
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            if (kWide) {
+              const float2 rounded = __half22float2(h);
+              const __half2 rest = __floats2half2_rn(v.x * up - rounded.x, v.y * up - rounded.y);
+              low[i] = *reinterpret_cast<const uint32_t*>(&rest);
+            }
           }
-          *reinterpret_cast<uint4*>(to + c / 8 * (kRowTile * 128) + ((c & 7) ^ (r & 7)) * 16) =
-              make_uint4(w[0], w[1], w[2], w[3]);
+          uint8_t* const piece = to + c / 8 * (kRowTile * 128) + ((c & 7) ^ (r & 7)) * 16;
+          *reinterpret_cast<uint4*>(piece) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (kWide) *reinterpret_cast<uint4*>(piece + S::kOperand) = make_uint4(low[0], low[1], low[2], low[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(&bars->queries[which]);
@@ -421,42 +536,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
 #pragma unroll
           for (int g = 0; g < kGroups; ++g) open = open && tile_meta.present[g] != 0;
         }
-        if (__all_sync(0xFFFFFFFFu, open)) softmax_tile<DP, kUnit, false>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which]);
-        else softmax_tile<DP, kUnit, true>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which]);
+        float* const keep_to = keep + j % kKeepStages * kRowTile + r;
+        if (__all_sync(0xFFFFFFFFu, open)) {
+          softmax_tile<DP, kUnit, false, kWide>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+        } else {
+          softmax_tile<DP, kUnit, true, kWide>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+        }
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->weights[which]);
+        if (kWide && lane == 0) mbar_arrive(&bars->kept[j % kKeepStages]);
       }
-      if (ok && tiles > 0) ok = mbar_wait_warp(&bars->sums[which], 0, abort_flag);
+      if (!kWide && ok && tiles > 0) ok = mbar_wait_warp(&bars->sums[which], 0, abort_flag);
       if (ok) {
         tc_fence_after_sync();
         const bool whole = splits_used(p, rows) == 1;
         // O stands against the maximum alone, the sum against that and the largest scale
         const float gain = row.sum == 0.0f ? 0.0f : whole ? row.largest / row.sum : row.largest;
         const float maximum = row.sum == 0.0f ? -INFINITY : row.maximum - row.largest_log;
-        const long long at = ((tile_index * p.splits + split) * 2 * kRowTile + in_tile);
-        const long long to = row_at * p.out.token_stride + out_head * p.out.head_stride;
+        const long long at = ((tile_index * p.splits + split) * kCtaRows + in_tile);
+        if (kWide) {
+          gains[r] = gain;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->gain);
+        } else {
 #pragma unroll 1
-        for (int c = 0; c < DP && c < p.dim; c += 32) {
-          uint32_t o[32];
-          if (tiles > 0) {
-            tmem_ld_32x32(sums + c, o);
-            tmem_ld_wait_for(o);
-          }
-          if (!real) continue;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (c + 8 * i >= p.dim) break;
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = row.sum == 0.0f ? 0.0f : __uint_as_float(o[8 * i + e]) * gain;
-            if (whole) {
-              store8(p.out.data, p.out.type, p.out.vector, to + c + 8 * i, v);
-            } else {
-              float4* const partial = reinterpret_cast<float4*>(p.partial + at * p.dim + c + 8 * i);
-              partial[0] = make_float4(v[0], v[1], v[2], v[3]);
-              partial[1] = make_float4(v[4], v[5], v[6], v[7]);
+          for (int c = 0; c < DP && c < p.dim; c += 32) {
+            uint32_t o[32];
+            if (tiles > 0) {
+              tmem_ld_32x32(sums + c, o);
+              tmem_ld_wait_for(o);
             }
+            if (real) write_row(p, o, gain, whole, at, row_at, out_head, c);
           }
         }
         if (real && !whole) *reinterpret_cast<float2*>(p.statistics + 2 * at) = make_float2(maximum, row.sum);
@@ -577,10 +688,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
     const uint32_t base = smem_u32(smem);
     const auto scores_of = [&](int which, int stage) {
 #pragma unroll
-      for (int d = 0; d < DP; d += 16) {
-        const uint32_t at = d / 64 * (kRowTile * 128) + d % 64 * 2;
-        mma_f16_ss(tmem + which * 128, make_sw128_kmajor_desc(base + S::kQueries + which * S::kOperand + at),
-                   make_sw128_kmajor_desc(base + S::kKeyRing + stage * S::kOperand + at), scores_desc, d > 0);
+      for (int half = kWide ? 1 : 0; half >= 0; --half) {  // (the low halves first: what sums of theirs lose is nothing)
+#pragma unroll
+        for (int d = 0; d < DP; d += 16) {
+          const uint32_t at = d / 64 * (kRowTile * 128) + d % 64 * 2;
+          mma_f16_ss(tmem + which * 128, make_sw128_kmajor_desc(base + S::kQueries + (which + half) * S::kOperand + at),
+                     make_sw128_kmajor_desc(base + S::kKeyRing + stage * S::kOperand + at), scores_desc, d > 0 || (kWide && half == 0));
+        }
       }
       tc_commit(&bars->scores[which]);
     };
@@ -595,23 +709,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       const int stage = j & 1, after = (j + 1) & 1;
       for (int i = 0; ok && i < row_tiles; ++i) {
         if (i == 0) ok = mbar_wait(&bars->value_full[stage], j >> 1 & 1, abort_flag);
-        ok = ok && mbar_wait(&bars->halves[i], j & 1, abort_flag);
+        if (kWide) {
+          if (ok && j >= 2) ok = mbar_wait(&bars->taken[j & 1], (j >> 1) - 1 & 1, abort_flag);
+          ok = ok && mbar_wait(&bars->weights[i], j & 1, abort_flag);
+        } else {
+          ok = ok && mbar_wait(&bars->halves[i], j & 1, abort_flag);
+        }
         if (!ok) break;
         tc_fence_after_sync();
 #pragma unroll
-        for (int t = 0; t < kKeys; t += 16) {
-          if (t == kKeys / 2) {
-            ok = mbar_wait(&bars->weights[i], j & 1, abort_flag);
-            if (!ok) break;
-            tc_fence_after_sync();
+        for (int half = kWide ? 1 : 0; half >= 0; --half) {
+#pragma unroll
+          for (int t = 0; t < kKeys; t += 16) {
+            if (!kWide && t == kKeys / 2) {
+              ok = mbar_wait(&bars->weights[i], j & 1, abort_flag);
+              if (!ok) break;
+              tc_fence_after_sync();
+            }
+            mma_f16_ts(tmem + 256 + (kWide ? j & 1 : i) * 128, tmem + i * 128 + half * (kKeys / 2) + t / 2,
+                       make_sw128_nmajor_desc(base + S::kValueRing + stage * S::kOperand + t * 128, kKeys * 128), sums_desc,
+                       t > 0 || (kWide ? half == 0 : j > 0));
           }
-          mma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + t / 2,
-                     make_sw128_nmajor_desc(base + S::kValueRing + stage * S::kOperand + t * 128, kKeys * 128), sums_desc,
-                     j > 0 || t > 0);
         }
         if (!ok) break;
+        if (kWide) tc_commit(&bars->sums[j & 1]);
         if (j + 1 == tiles) {
-          tc_commit(&bars->sums[i]);
+          if (!kWide) tc_commit(&bars->sums[i]);
           continue;
         }
         if (i == 0) ok = mbar_wait(&bars->key_full[after], (j + 1) >> 1 & 1, abort_flag);
@@ -642,20 +765,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   }
 }
 
-template <int DP, int kUnit>
+template <int DP, int kUnit, bool kWide>
 qx_status launch_prompt_of(const AttentionParams& p, long long grid, cudaStream_t stream) {
   static SmemOptIn opt_in;
-  QX_TRY(opt_in.ensure(prompt_kernel<DP, kUnit>, TcShape<DP>::kBytes));
-  return launch_behind(prompt_kernel<DP, kUnit>, grid, kTcThreads, TcShape<DP>::kBytes, stream, p);
+  QX_TRY(opt_in.ensure(prompt_kernel<DP, kUnit, kWide>, TcShape<DP>::kBytes));
+  return launch_behind(prompt_kernel<DP, kUnit, kWide>, grid, kTcThreads, TcShape<DP>::kBytes, stream, p);
+}
+template <bool kWide>
+qx_status launch_prompt_sized(const AttentionParams& p, long long grid, cudaStream_t stream) {
+  if (p.block_tokens < 32) {
+    return p.dim <= 64 ? launch_prompt_of<64, 16, kWide>(p, grid, stream) : launch_prompt_of<128, 16, kWide>(p, grid, stream);
+  }
+  return p.dim <= 64 ? launch_prompt_of<64, 32, kWide>(p, grid, stream) : launch_prompt_of<128, 32, kWide>(p, grid, stream);
 }
 
 }  // namespace
 
-qx_status launch_prompt(const AttentionParams& p, long long grid, cudaStream_t stream) {
-  if (p.block_tokens < 32) {
-    return p.dim <= 64 ? launch_prompt_of<64, 16>(p, grid, stream) : launch_prompt_of<128, 16>(p, grid, stream);
-  }
-  return p.dim <= 64 ? launch_prompt_of<64, 32>(p, grid, stream) : launch_prompt_of<128, 32>(p, grid, stream);
+qx_status launch_prompt(const AttentionParams& p, bool wide, long long grid, cudaStream_t stream) {
+  return wide ? launch_prompt_sized<true>(p, grid, stream) : launch_prompt_sized<false>(p, grid, stream);
 }
 
 }  // namespace kv
