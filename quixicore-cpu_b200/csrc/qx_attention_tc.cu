@@ -151,19 +151,6 @@ __device__ __forceinline__ void convert16(const uint4& codes, uint4* a, uint4* b
   b->w = tile::convert_bytes2<false>(codes.w, 0x4342);
 }
 
-// Eight neighbouring 16-bit elements as they are.
-__device__ __forceinline__ uint4 load8_raw(const uint8_t* data, int vector, long long index) {
-  const uint16_t* const from = reinterpret_cast<const uint16_t*>(data) + index;
-  if (vector) return *reinterpret_cast<const uint4*>(from);
-  return make_uint4(from[0] | from[1] << 16, from[2] | from[3] << 16, from[4] | from[5] << 16, from[6] | from[7] << 16);
-}
-
-__device__ __forceinline__ uint4 load4_raw(const uint8_t* data, int vector, long long index) {
-  const uint32_t* const from = reinterpret_cast<const uint32_t*>(data) + index;
-  if (vector) return *reinterpret_cast<const uint4*>(from);
-  return make_uint4(from[0], from[1], from[2], from[3]);
-}
-
 // What a softmax thread knows about its row.
 struct RowState {
   float factor;       // of the raw scores, log2(e) in it
@@ -314,20 +301,19 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
 }
 
 // 32 elements of a row of O, from element c of the head on, times `gain`, to the output or the partial results.
-__device__ __forceinline__ void write_row(const AttentionParams& p, const uint32_t (&o)[32], float gain, bool whole, long long at,
-                                          long long row, long long head, int c) {
+// (Passed through shared memory, so that a warp writes runs of a row, this took twice the time.)
+__device__ __forceinline__ void write_row(const AttentionParams& p, const uint32_t (&o)[32], float gain, float* partial,
+                                          long long to, int c) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (c + 8 * i >= p.dim) break;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = gain == 0.0f ? 0.0f : __uint_as_float(o[8 * i + e]) * gain;  // (O may be unset)
-    if (whole) {
-      store8(p.out.data, p.out.type, p.out.vector, row * p.out.token_stride + head * p.out.head_stride + c + 8 * i, v);
+    if (partial == nullptr) {
+      store8(p.out.data, p.out.type, p.out.vector, to + c + 8 * i, v);
     } else {
-      float4* const partial = reinterpret_cast<float4*>(p.partial + at * p.dim + c + 8 * i);
-      partial[0] = make_float4(v[0], v[1], v[2], v[3]);
-      partial[1] = make_float4(v[4], v[5], v[6], v[7]);
+      store8_typed<QX_STORAGE_F32>(reinterpret_cast<uint8_t*>(partial), to + c + 8 * i, v);
     }
   }
 }
@@ -346,14 +332,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
 
-  long long index = blockIdx.x;
-  const int split = static_cast<int>(index % p.splits);
-  index /= p.splits;
+  const uint32_t index = blockIdx.x / p.splits;
+  const int split = static_cast<int>(blockIdx.x - index * p.splits);
+  const uint32_t by_head = index / p.row_tiles;
   // the last rows first: with a causal mask they see the most keys
-  const int row_tile = p.row_tiles - 1 - static_cast<int>(index % p.row_tiles);
-  index /= p.row_tiles;
-  const long long tile_index = index * p.row_tiles + row_tile;
-  const int head = static_cast<int>(index % p.kv_heads), s = static_cast<int>(index / p.kv_heads);
+  const int row_tile = p.row_tiles - 1 - static_cast<int>(index - by_head * p.row_tiles);
+  const long long tile_index = static_cast<long long>(by_head) * p.row_tiles + row_tile;
+  const int s = static_cast<int>(by_head / p.kv_heads), head = static_cast<int>(by_head - s * p.kv_heads);
   Rows rows;
   constexpr int kCtaRows = kWide ? kRowTile : 2 * kRowTile;
   if (!rows_of(p, s, row_tile * kCtaRows, kCtaRows, &rows)) return;
@@ -434,9 +419,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         const int token = (rows.first + r) / p.group, member = (rows.first + r) % p.group;
         const bool whole = splits_used(p, rows) == 1;
         const long long at = (tile_index * p.splits + split) * kCtaRows + r;
+        const long long out_head = static_cast<long long>(head) * p.group + member;
+        const long long to = whole ? (rows.row + token) * p.out.token_stride + out_head * p.out.head_stride : at * p.dim;
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
-          write_row(p, total[c], gains[r], whole, at, rows.row + token, static_cast<long long>(head) * p.group + member, 32 * c);
+          if (32 * c < p.dim) write_row(p, total[c], gains[r], whole ? nullptr : p.partial, to, 32 * c);
         }
       }
       if (!ok) {
@@ -459,59 +446,86 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         row.high = p.causal ? min(rows.length, start + token + 1) : rows.length;
         row.low = p.window > 0 ? max(0, start + token - p.window + 1) : 0;
       }
-      // the queries: f16 times a power of two that brings the row's largest magnitude to 2^7 .. 2^8
+      // The queries: f16 times a power of two that brings the row's largest magnitude to 2^7 .. 2^8. A warp copies its
+      // rows as they are to where their operands go, runs of lanes to a row; then each thread converts its own row in
+      // place (f32: the 16-byte pieces 2c and 2c + 1 lie where the high and the low halves of elements 8c .. 8c + 7
+      // go). Loops, not straight code: what runs once per CTA waits for its instructions at every line.
       {
-        const long long from = row_at * p.q.token_stride + out_head * p.q.head_stride;
-        // the whole row in registers: all of its loads are in flight at once
-        constexpr int kWords = kWide ? 2 : 1;
-        uint4 raw[DP / 8][kWords];
-#pragma unroll
-        for (int c = 0; c < DP / 8; ++c) {
-#pragma unroll
-          for (int w = 0; w < kWords; ++w) {
-            raw[c][w] = make_uint4(0, 0, 0, 0);
-            if (real && 8 * c < p.dim) raw[c][w] = kWide ? load4_raw(p.q.data, p.q.vector, from + 8 * c + 4 * w) : load8_raw(p.q.data, p.q.vector, from + 8 * c);
+        constexpr int kElements = kWide ? 4 : 8, kLanes = DP / kElements, kAtOnce = 32 / kLanes, kTurns = 32 / kAtOnce;
+        const int piece = lane % kLanes, d = piece * kElements, warp_row = which * kRowTile + (warp & 3) * 32;
+        uint8_t* const tile = smem + S::kQueries + which * S::kOperand;
+        const auto place = [&](int r, int c) { return tile + c / 8 * (kRowTile * 128) + r * 128 + ((c & 7) ^ (r & 7)) * 16; };
+        int q_token = (rows.first + warp_row + lane / kLanes) / p.group;
+        int q_member = rows.first + warp_row + lane / kLanes - q_token * p.group;
+#pragma unroll 2
+        for (int i = 0; i < kTurns; ++i) {
+          const int r_of = i * kAtOnce + lane / kLanes, r_to = (warp & 3) * 32 + r_of;
+          uint8_t* const to = kWide ? place(r_to, piece / 2) + piece % 2 * S::kOperand : place(r_to, piece);
+          if (warp_row + r_of >= rows.count || d >= p.dim) {
+            *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+          } else {
+            const long long from = (rows.row + q_token) * p.q.token_stride +
+                                   (static_cast<long long>(head) * p.group + q_member) * p.q.head_stride + d;
+            if (p.q.vector) {
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)),
+                           "l"(p.q.data + from * (kWide ? 4 : 2))
+                           : "memory");
+            } else if (kWide) {
+#pragma unroll 1
+              for (int e = 0; e < 4; ++e) reinterpret_cast<uint32_t*>(to)[e] = reinterpret_cast<const uint32_t*>(p.q.data)[from + e];
+            } else {
+#pragma unroll 1
+              for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(p.q.data)[from + e];
+            }
           }
+          for (q_member += kAtOnce; q_member >= p.group; q_member -= p.group) ++q_token;
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
         const bool f16 = p.q.type == QX_STORAGE_F16;
         const auto pair = [&](uint32_t w) {
           return f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w)) : make_float2(bf16_low(w), bf16_high(w));
         };
         uint32_t top = 0;  // of the bit patterns without sign: they grow with the magnitude
-#pragma unroll
+#pragma unroll 4
         for (int c = 0; c < DP / 8; ++c) {
+          const uint4 a = *reinterpret_cast<const uint4*>(place(r, c));
+          if (kWide) {
+            const uint4 b = *reinterpret_cast<const uint4*>(place(r, c) + S::kOperand);
+            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-          for (int k = 0; k < kWords; ++k) {
-            const uint32_t w[4] = {raw[c][k].x, raw[c][k].y, raw[c][k].z, raw[c][k].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = kWide ? max(top, w[i] & 0x7FFFFFFFu) : max(top, max(w[i] & 0x7FFFu, w[i] >> 16 & 0x7FFFu));
+            for (int e = 0; e < 8; ++e) top = max(top, w[e] & 0x7FFFFFFFu);
+          } else {
+            top = __vimax3_u16x2(top, a.x & 0x7FFF7FFFu, a.y & 0x7FFF7FFFu);
+            top = __vimax3_u16x2(top, a.z & 0x7FFF7FFFu, a.w & 0x7FFF7FFFu);
           }
         }
-        top = (kWide ? top : __float_as_uint(pair(top).x)) >> 23;
+        if (!kWide) top = __float_as_uint(pair(max(top & 0xFFFFu, top >> 16)).x);
+        top >>= 23;
         const int shift = top >= 255 ? 0 : min(120, max(-120, 134 - static_cast<int>(top)));
         // (a negative scale turns the query's sign, so that larger raw scores are larger scores)
         const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
         row.factor = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * fabsf(p.scale_log2);
-        uint8_t* const to = smem + S::kQueries + which * S::kOperand + r * 128;
-#pragma unroll
+#pragma unroll 2
         for (int c = 0; c < DP / 8; ++c) {
-          const uint4 &first = raw[c][0], &second = raw[c][kWords - 1];
+          uint4* const at = reinterpret_cast<uint4*>(place(r, c));
+          uint4* const low_at = reinterpret_cast<uint4*>(place(r, c) + S::kOperand);
+          const uint4 first = *at, second = kWide ? *low_at : first;
           const uint32_t in[8] = {first.x, first.y, first.z, first.w, second.x, second.y, second.z, second.w};
-          uint32_t w[4], low[4];
+          uint32_t high[4], low[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 v = kWide ? make_float2(__uint_as_float(in[2 * i]), __uint_as_float(in[2 * i + 1])) : pair(in[i]);
             const __half2 h = __floats2half2_rn(v.x * up, v.y * up);
-            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            high[i] = *reinterpret_cast<const uint32_t*>(&h);
             if (kWide) {
               const float2 rounded = __half22float2(h);
               const __half2 rest = __floats2half2_rn(v.x * up - rounded.x, v.y * up - rounded.y);
               low[i] = *reinterpret_cast<const uint32_t*>(&rest);
             }
           }
-          uint8_t* const piece = to + c / 8 * (kRowTile * 128) + ((c & 7) ^ (r & 7)) * 16;
-          *reinterpret_cast<uint4*>(piece) = make_uint4(w[0], w[1], w[2], w[3]);
-          if (kWide) *reinterpret_cast<uint4*>(piece + S::kOperand) = make_uint4(low[0], low[1], low[2], low[3]);
+          *at = make_uint4(high[0], high[1], high[2], high[3]);
+          if (kWide) *low_at = make_uint4(low[0], low[1], low[2], low[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(&bars->queries[which]);
@@ -560,6 +574,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->gain);
         } else {
+          const long long to = whole ? row_at * p.out.token_stride + out_head * p.out.head_stride : at * p.dim;
 #pragma unroll 1
           for (int c = 0; c < DP && c < p.dim; c += 32) {
             uint32_t o[32];
@@ -567,7 +582,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
               tmem_ld_32x32(sums + c, o);
               tmem_ld_wait_for(o);
             }
-            if (real) write_row(p, o, gain, whole, at, row_at, out_head, c);
+            if (real) write_row(p, o, gain, whole ? nullptr : p.partial, to, c);
           }
         }
         if (real && !whole) *reinterpret_cast<float2*>(p.statistics + 2 * at) = make_float2(maximum, row.sum);
