@@ -300,8 +300,77 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   tmem_st_wait();
 }
 
-// 32 elements of a row of O, from element c of the head on, times `gain`, to the output or the partial results.
-// (Passed through shared memory, so that a warp writes runs of a row, this took twice the time.)
+// A lane's way over rows of a view, from `row` of the sequence's on: where its row begins, in elements.
+struct RowWalk {
+  long long at, step, wrap;
+  int member, by, group;
+  __device__ __forceinline__ RowWalk(const Heads& view, const Rows& rows, int head, int group_, int row, int at_once)
+      : group(group_) {
+    const int token = row / group;
+    member = row - token * group;
+    at = (rows.row + token) * view.token_stride + (static_cast<long long>(head) * group + member) * view.head_stride;
+    by = at_once % group;
+    step = at_once / group * view.token_stride + by * view.head_stride;
+    wrap = view.token_stride - group * view.head_stride;
+  }
+  __device__ __forceinline__ void next() {
+    at += step;
+    member += by;
+    if (member >= group) {
+      member -= group;
+      at += wrap;
+    }
+  }
+};
+
+// 16 bytes of a row of an operand: c counts them. And of a row of f32 elements that lies where a pair's halves go: their
+// pieces 2c and 2c + 1 where elements 8c .. 8c + 7 of the high and of the low halves do.
+template <int DP, bool kWide>
+__device__ __forceinline__ uint8_t* piece_at(uint8_t* tile, int r, int c) {
+  const int chunk = kWide ? c >> 1 : c;
+  return tile + (kWide ? (c & 1) * (kRowTile * DP * 2) : 0) + (chunk >> 3) * (kRowTile * 128) + r * 128 +
+         (((chunk ^ r) & 7) << 4);
+}
+
+// 32 elements of a row of O, from element c of the head on, times `gain`, into the operand's place of that row ...
+template <int DP, bool kWide>
+__device__ __forceinline__ void stage_row(uint8_t* tile, int type, const uint32_t (&o)[32], float gain, int r, int c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = gain == 0.0f ? 0.0f : __uint_as_float(o[8 * i + e]) * gain;  // (O may be unset)
+    if constexpr (kWide) {
+      uint4 w[2];
+      to_words<QX_STORAGE_F32>(v, w);
+      *reinterpret_cast<uint4*>(piece_at<DP, true>(tile, r, c / 4 + 2 * i)) = w[0];
+      *reinterpret_cast<uint4*>(piece_at<DP, true>(tile, r, c / 4 + 2 * i + 1)) = w[1];
+    } else {
+      uint4 w[1];
+      if (type == QX_STORAGE_F16) to_words<QX_STORAGE_F16>(v, w);
+      else to_words<QX_STORAGE_BF16>(v, w);
+      *reinterpret_cast<uint4*>(piece_at<DP, false>(tile, r, c / 8 + i)) = w[0];
+    }
+  }
+}
+// ... from where the warp writes its 32 rows, runs of lanes to a row.
+template <int DP, bool kWide>
+__device__ __forceinline__ void write_rows(const AttentionParams& p, uint8_t* tile, const Rows& rows, int head, int warp_row) {
+  constexpr int kElements = kWide ? 4 : 8, kLanes = DP / kElements, kAtOnce = 32 / kLanes;
+  const int lane = threadIdx.x & 31, piece = lane % kLanes, first = lane / kLanes;
+  __syncwarp();
+  if (piece * kElements >= p.dim) return;
+  RowWalk to(p.out, rows, head, p.group, rows.first + warp_row + first, kAtOnce);
+#pragma unroll 4
+  for (int r = first; r < 32; r += kAtOnce) {
+    if (warp_row + r < rows.count) {
+      *reinterpret_cast<uint4*>(p.out.data + (to.at + piece * kElements) * (kWide ? 4 : 2)) =
+          *reinterpret_cast<const uint4*>(piece_at<DP, kWide>(tile, (warp_row & (kRowTile - 1)) + r, piece));
+    }
+    to.next();
+  }
+}
+// The same elements by the row's own thread, to the partial results or to a view that is not as the above needs it.
 __device__ __forceinline__ void write_row(const AttentionParams& p, const uint32_t (&o)[32], float gain, float* partial,
                                           long long to, int c) {
 #pragma unroll
@@ -309,7 +378,7 @@ __device__ __forceinline__ void write_row(const AttentionParams& p, const uint32
     if (c + 8 * i >= p.dim) break;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = gain == 0.0f ? 0.0f : __uint_as_float(o[8 * i + e]) * gain;  // (O may be unset)
+    for (int e = 0; e < 8; ++e) v[e] = gain == 0.0f ? 0.0f : __uint_as_float(o[8 * i + e]) * gain;
     if (partial == nullptr) {
       store8(p.out.data, p.out.type, p.out.vector, to + c + 8 * i, v);
     } else {
@@ -415,16 +484,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         if (lane == 0) mbar_arrive(&bars->taken[j & 1]);
       }
       if (ok) ok = mbar_wait_warp(&bars->gain, 0, abort_flag);
-      if (ok && r < rows.count) {
+      if (ok) {
         const int token = (rows.first + r) / p.group, member = (rows.first + r) % p.group;
         const bool whole = splits_used(p, rows) == 1;
         const long long at = (tile_index * p.splits + split) * kCtaRows + r;
         const long long out_head = static_cast<long long>(head) * p.group + member;
         const long long to = whole ? (rows.row + token) * p.out.token_stride + out_head * p.out.head_stride : at * p.dim;
+        const bool staged = whole && p.out.type == QX_STORAGE_F32 && p.out.vector;  // (every product is done: so are the queries)
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
-          if (32 * c < p.dim) write_row(p, total[c], gains[r], whole ? nullptr : p.partial, to, 32 * c);
+          if (staged) stage_row<DP, true>(smem + S::kQueries, QX_STORAGE_F32, total[c], gains[r], r, 32 * c);
+          else if (r < rows.count && 32 * c < p.dim) write_row(p, total[c], gains[r], whole ? nullptr : p.partial, to, 32 * c);
         }
+        if (staged) write_rows<DP, true>(p, smem + S::kQueries, rows, head, (warp & 3) * 32);
       }
       if (!ok) {
         *abort_flag = 1;
@@ -451,34 +523,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       // place (f32: the 16-byte pieces 2c and 2c + 1 lie where the high and the low halves of elements 8c .. 8c + 7
       // go). Loops, not straight code: what runs once per CTA waits for its instructions at every line.
       {
-        constexpr int kElements = kWide ? 4 : 8, kLanes = DP / kElements, kAtOnce = 32 / kLanes, kTurns = 32 / kAtOnce;
+        constexpr int kElements = kWide ? 4 : 8, kBytes = kWide ? 4 : 2, kLanes = DP / kElements, kAtOnce = 32 / kLanes;
         const int piece = lane % kLanes, d = piece * kElements, warp_row = which * kRowTile + (warp & 3) * 32;
         uint8_t* const tile = smem + S::kQueries + which * S::kOperand;
-        const auto place = [&](int r, int c) { return tile + c / 8 * (kRowTile * 128) + r * 128 + ((c & 7) ^ (r & 7)) * 16; };
-        int q_token = (rows.first + warp_row + lane / kLanes) / p.group;
-        int q_member = rows.first + warp_row + lane / kLanes - q_token * p.group;
-#pragma unroll 2
-        for (int i = 0; i < kTurns; ++i) {
-          const int r_of = i * kAtOnce + lane / kLanes, r_to = (warp & 3) * 32 + r_of;
-          uint8_t* const to = kWide ? place(r_to, piece / 2) + piece % 2 * S::kOperand : place(r_to, piece);
-          if (warp_row + r_of >= rows.count || d >= p.dim) {
-            *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+        RowWalk from(p.q, rows, head, p.group, rows.first + warp_row + lane / kLanes, kAtOnce);
+        const bool vector = p.q.vector;
+#pragma unroll 4
+        for (int i = lane / kLanes; i < 32; i += kAtOnce) {
+          uint8_t* const to = piece_at<DP, kWide>(tile, (warp & 3) * 32 + i, piece);
+          const bool there = warp_row + i < rows.count && d < p.dim;
+          const uint8_t* const at = p.q.data + (there ? from.at + d : 0) * kBytes;
+          if (vector || !there) {  // (of no bytes: zeros)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                         ::"r"(smem_u32(to)), "l"(vector ? at : reinterpret_cast<const uint8_t*>(p.k_codes)), "r"(there ? 16 : 0)
+                         : "memory");
           } else {
-            const long long from = (rows.row + q_token) * p.q.token_stride +
-                                   (static_cast<long long>(head) * p.group + q_member) * p.q.head_stride + d;
-            if (p.q.vector) {
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)),
-                           "l"(p.q.data + from * (kWide ? 4 : 2))
-                           : "memory");
-            } else if (kWide) {
 #pragma unroll 1
-              for (int e = 0; e < 4; ++e) reinterpret_cast<uint32_t*>(to)[e] = reinterpret_cast<const uint32_t*>(p.q.data)[from + e];
-            } else {
-#pragma unroll 1
-              for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(p.q.data)[from + e];
+            for (int e = 0; e < 16; e += kBytes) {
+              if (kWide) *reinterpret_cast<uint32_t*>(to + e) = *reinterpret_cast<const uint32_t*>(at + e);
+              else *reinterpret_cast<uint16_t*>(to + e) = *reinterpret_cast<const uint16_t*>(at + e);
             }
           }
-          for (q_member += kAtOnce; q_member >= p.group; q_member -= p.group) ++q_token;
+          from.next();
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncwarp();
@@ -489,9 +555,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         uint32_t top = 0;  // of the bit patterns without sign: they grow with the magnitude
 #pragma unroll 4
         for (int c = 0; c < DP / 8; ++c) {
-          const uint4 a = *reinterpret_cast<const uint4*>(place(r, c));
+          const uint4 a = *reinterpret_cast<const uint4*>(piece_at<DP, false>(tile, r, c));
           if (kWide) {
-            const uint4 b = *reinterpret_cast<const uint4*>(place(r, c) + S::kOperand);
+            const uint4 b = *reinterpret_cast<const uint4*>(piece_at<DP, false>(tile, r, c) + S::kOperand);
             const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = max(top, w[e] & 0x7FFFFFFFu);
@@ -508,8 +574,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         row.factor = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * fabsf(p.scale_log2);
 #pragma unroll 2
         for (int c = 0; c < DP / 8; ++c) {
-          uint4* const at = reinterpret_cast<uint4*>(place(r, c));
-          uint4* const low_at = reinterpret_cast<uint4*>(place(r, c) + S::kOperand);
+          uint4* const at = reinterpret_cast<uint4*>(piece_at<DP, false>(tile, r, c));
+          uint4* const low_at = reinterpret_cast<uint4*>(piece_at<DP, false>(tile, r, c) + S::kOperand);
           const uint4 first = *at, second = kWide ? *low_at : first;
           const uint32_t in[8] = {first.x, first.y, first.z, first.w, second.x, second.y, second.z, second.w};
           uint32_t high[4], low[4];
@@ -575,6 +641,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
           if (lane == 0) mbar_arrive(&bars->gain);
         } else {
           const long long to = whole ? row_at * p.out.token_stride + out_head * p.out.head_stride : at * p.dim;
+          const bool staged = whole && p.out.type != QX_STORAGE_F32 && p.out.vector;  // (every product is done: so are the queries)
+          uint8_t* const tile = smem + S::kQueries + which * S::kOperand;
 #pragma unroll 1
           for (int c = 0; c < DP && c < p.dim; c += 32) {
             uint32_t o[32];
@@ -582,8 +650,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
               tmem_ld_32x32(sums + c, o);
               tmem_ld_wait_for(o);
             }
-            if (real) write_row(p, o, gain, whole ? nullptr : p.partial, to, c);
+            if (staged) stage_row<DP, false>(tile, p.out.type, o, gain, r, c);
+            else if (real) write_row(p, o, gain, whole ? nullptr : p.partial, to, c);
           }
+          if (staged) write_rows<DP, false>(p, tile, rows, head, which * kRowTile + (warp & 3) * 32);
         }
         if (real && !whole) *reinterpret_cast<float2*>(p.statistics + 2 * at) = make_float2(maximum, row.sum);
         if (real && whole && p.lse != nullptr) {
