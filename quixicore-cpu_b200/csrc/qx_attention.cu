@@ -46,8 +46,11 @@ constexpr float kShift = 12.0f;
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 32;
 constexpr uint32_t kZeroSum = 0x4B400000u;  // 1.5 * 2^23: whole numbers below 2^22 added to the bits are exact
 
-// Rows per sequence from which queries take the prompt kernel.
-constexpr long long kPromptFrom = 64;
+// Rows per sequence from which queries take the prompt kernel (f32 ones, of half as many rows per CTA and twice the
+// products: later). Streamed | prompt kernel, us: f16, 4 sequences of 4096 keys, 32 rows 37 | 40, 48 rows 48 | 41, 192
+// rows 101 | 54; one of 16384 keys, 48 rows 42 | 41; f32, 4 of 4096 keys, 64 rows 84 | 87, 100 rows 96 | 90; 16 whole
+// texts of 64 tokens 25 | 29, of 100 tokens 40 | 32.
+constexpr long long kPromptFrom = 48, kPromptFromWide = 96;
 
 // CTAs per SM, as many as shared memory and 65536 registers hold.
 constexpr int streamed_ctas(int dp, int row_tiles) { return dp == 64 ? (row_tiles == 1 ? 4 : 3) : dp == 128 ? (row_tiles == 1 ? 3 : 2) : 1; }
@@ -150,8 +153,10 @@ __device__ __forceinline__ uint32_t rest_f16(float a, float b, uint32_t rounded)
   return pair_f16(a - f.x, b - f.y);
 }
 
-// A balanced launch's line: per item, kItemCost units for what a CTA does before its first tile, and one per tile.
-constexpr int kItemCost = 4, kLeastPiece = 8, kBalancedSequences = 128;
+// A balanced launch's line: per item, kItemCost units for what a CTA does before its first tile and behind its last, and
+// one per tile (4 | 8 | 12 | 16 | 24 units, us: 32 sessions of up to 8192 66.4 | 65.0 | 64.5 | 64.7 | 67.2, 8 of five
+// tokens in windows of 4096 29.0 | 26.7 | 26.2 | 26.2 | 27.0).
+constexpr int kItemCost = 12, kLeastPiece = 8, kBalancedSequences = 128;
 struct Line {
   uint32_t begin[kBalancedSequences / 32];  // of sequence lane + 32 i
   uint32_t item[kBalancedSequences / 32];   // units per kv head
@@ -237,7 +242,9 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
     s = sequence_at(p, line, place, &sequence_begin, &item);
     head = static_cast<int>((place - sequence_begin) / item);
     const uint32_t item_begin = sequence_begin + head * item, item_end = item_begin + item, stop = min(place_end, item_end);
-    first_part = item_begin / line.piece;
+    // (the item's first part is where its first tile is: a piece that ends before that leaves it to the next CTA)
+    if (stop < item_end && stop - item_begin <= kItemCost) return;
+    first_part = min(item_begin + kItemCost, item_end - 1) / line.piece;
     parts = static_cast<int>((item_end - 1) / line.piece - first_part) + 1;
     part = 2LL * blockIdx.x + (first_part == blockIdx.x ? 1 : 0);
     (void)rows_of(p, s, 0, kRows, &rows);
@@ -912,7 +919,7 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   p.group = q->heads / cache->kv_heads;
   const long long most_rows = static_cast<long long>(batch->max_tokens) * p.group;
   const bool wide = q->type == QX_STORAGE_F32;
-  const bool prompt = cache->head_dim <= 128 && most_rows >= kPromptFrom;
+  const bool prompt = cache->head_dim <= 128 && most_rows >= (wide ? kPromptFromWide : kPromptFrom);
   p.tile_rows = prompt ? (wide ? kPromptRowsWide : kPromptRows) : most_rows <= 8 ? 8 : 16;
   p.shift = prompt ? kPromptShift : kShift;
   p.row_tiles = static_cast<int>((most_rows + p.tile_rows - 1) / p.tile_rows);
@@ -927,11 +934,14 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   // below a tile per warp (in the prompt kernel, four tiles): then the joining would cost more than the keys.
   const int dp = cache->head_dim <= 64 ? 64 : cache->head_dim <= 128 ? 128 : 256;
   const long long slots = static_cast<long long>(ctx->prop.multiProcessorCount) * (prompt ? 1 : streamed_ctas(dp, p.tile_rows / 8));
-  // Balanced: several sequences, and items enough that each has few parts to join (by one CTA, at about 0.15 us a part).
+  // Balanced: several sequences; items enough that each has few parts to join (by one CTA, at about 0.15 us a part), and
+  // not so many that whole ones even out by themselves; tiles enough per CTA that finding its piece pays. Balanced |
+  // chunks, us, 128 elements, 8 kv heads: 32 sessions of up to 8192 64.5 | 76.5, 2048 26.6 | 29.4, 1024 20.0 | 20.8, 700
+  // 18.8 | 18.3, 512 15.9 | 12.5; 12 of up to 2000 16.2 | 15.3; 64 of up to 8192 116 | 129, 100 175 | 161.
   const long long counters = static_cast<long long>(batch->sequences) * cache->kv_heads;
-  const long long units = counters * ((range + kTile - 1) / kTile + kItemCost);
+  const long long item_tiles = (range + kTile - 1) / kTile, units = counters * (item_tiles + kItemCost);
   if (!prompt && p.row_tiles == 1 && batch->sequences > 1 && batch->sequences <= kBalancedSequences && counters >= slots / 16 &&
-      counters <= static_cast<long long>(kWorkspaceCounterBytes / sizeof(int)) && units < (1LL << 31)) {
+      counters <= slots + slots / 2 && counters * item_tiles >= 16 * slots && units < (1LL << 31)) {
     // Two parts per CTA; behind the arrival counters, which the kernel leaves at zero.
     const long long grid = std::min(slots, (units + kLeastPiece - 1) / kLeastPiece);
     const size_t rows = 2 * static_cast<size_t>(grid) * p.tile_rows;
