@@ -6,7 +6,7 @@
 //   scores  [keys x rows]: the codes as they are (s8) against three balanced base-256 digits of the queries
 //           (s8, 23 bits against the row's largest magnitude): exact whole-number sums. Those start at
 //           1.5 * 2^23 as f32 bits, so that a subtraction makes f32 numbers of them;
-//   output  [head elements x rows]: the codes as f16 (exact) against the weights as f16 (a rounding of 2^-12
+//   output  [head elements x rows]: the codes as f16 (exact) against the weights as f16 (a rounding of 2^-11
 //           relative, no further than the 16-bit outputs' own), as hi + lo pairs for f32 queries; f32 sums.
 // The scales are applied to the sums: one multiplication per score (ks), one per 32 keys and output element (vs).
 //
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
   const int start = rows.length - rows.n, position0 = start + rows.first / p.group;
   const int position1 = start + (rows.first + rows.count - 1) / p.group;
   const int open_high = p.causal ? min(rows.length, position0 + 1) : rows.length;  // below: no key is hidden
-  const int open_low = p.window > 0 ? max(0, position1 - p.window + 1) : 0;
+  const int open_low = first_seen(p, position1);
   float factor[kRowTiles][2];
   int low[kRowTiles][2], high[kRowTiles][2];  // keys [low, high) of the row
 #pragma unroll
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
       if (r < rows.count) {
         const int position = start + (rows.first + r) / p.group;
         high[n][e] = p.causal ? min(rows.length, position + 1) : rows.length;
-        low[n][e] = p.window > 0 ? max(0, position - p.window + 1) : 0;
+        low[n][e] = first_seen(p, position);
       }
     }
   }

@@ -35,6 +35,12 @@ struct Rows {
   int low, high;       // keys [low, high) that any of them sees, low on a multiple of 32
 };
 
+// The first key that a row at `position` sees. (No difference with more than 31 bits: positions of rows that a sequence
+// has beyond its tokens are negative, a window may be as wide as whole numbers go.)
+__device__ __forceinline__ int first_seen(const AttentionParams& p, int position) {
+  return p.window > 0 && position >= p.window ? position - p.window + 1 : 0;
+}
+
 __device__ __forceinline__ bool rows_of(const AttentionParams& p, int s, int first, int most, Rows* r, bool each = false) {
   Sequence q;
   if (!sequence_of(p.batch, s, false, &q, each)) return false;
@@ -48,7 +54,7 @@ __device__ __forceinline__ bool rows_of(const AttentionParams& p, int s, int fir
   const int start = q.length - q.n;  // (negative where the sequence has more rows than tokens)
   const int position0 = start + first / p.group, position1 = start + (first + r->count - 1) / p.group;
   r->high = max(0, p.causal ? min(q.length, position1 + 1) : q.length);
-  r->low = p.window > 0 ? max(0, position0 - p.window + 1) & ~31 : 0;
+  r->low = first_seen(p, position0) & ~31;
   r->low = min(r->low, r->high);
   return true;
 }

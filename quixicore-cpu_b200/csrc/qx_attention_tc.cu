@@ -15,7 +15,7 @@
 // The codes are exact in f16 and so are the queries, times a power of two per row (f16 loses the bits of
 // elements below 2^-32 of the row's largest). The scale of a key block multiplies the scores. The scale of a
 // value block goes into the exponent of the weights: P = 2^(s + log2 vs - m), m following the largest s +
-// log2 vs, so one f16 rounding (2^-12) holds for every mixture of scales; the sums of weights divide it out
+// log2 vs, so one f16 rounding (2^-11) holds for every mixture of scales; the sums of weights divide it out
 // again, once per 16 keys, relative to the largest scale that the row has seen. (A scale more than 2^60 below
 // that one counts as 2^-60 of it, so that no weight leaves f32's range on the way; that moves an output by 2^-53
 // of the largest value.) m only follows when it has fallen 4 behind (a factor of 16): then the row's sum and O
@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       row.largest = 0.0f;
       if (real) {
         row.high = p.causal ? min(rows.length, start + token + 1) : rows.length;
-        row.low = p.window > 0 ? max(0, start + token - p.window + 1) : 0;
+        row.low = first_seen(p, start + token);
       }
       // The queries: f16 times a power of two that brings the row's largest magnitude to 2^7 .. 2^8. A warp copies its
       // rows as they are to where their operands go, runs of lanes to a row; then each thread converts its own row in
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       const int last = min(rows.count, (which + 1) * kRowTile) - 1;
       const int position0 = start + (rows.first + which * kRowTile) / p.group, position1 = start + (rows.first + last) / p.group;
       const int open_high = p.causal ? min(rows.length, position0 + 1) : rows.length;
-      const int open_low = p.window > 0 ? max(0, position1 - p.window + 1) : 0;
+      const int open_low = first_seen(p, position1);
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t scores = tmem + lanes + which * 128, sums = tmem + lanes + 256 + which * 128;
       for (int j = 0; ok && j < tiles; ++j) {

@@ -110,7 +110,9 @@ def attention_tolerance(out, lse, magnitude, spread, dtype, dim, length):
       weights  exp2 to 2 u, its argument (up to `spread` * 1.44 away from the maximum) to one rounding: inside
                the next term;
       a score that is off by d takes d of its weight with it, and d of the sum: 2 d;
-      weights are rounded to f16 (2^-12 of each, the values are exact) or, for f32, to 22 bits, and to no less than
+      weights are rounded to f16 (11 significant bits: a weight in [2^e, 2^(e+1)) is off by half of 2^(e-10) at
+               most, so 2^-11 of each where it stands at 2^e; the values are exact) or, for f32, to a pair of which
+               the second takes what the first leaves, 2^-11 of it, again to 2^-11: 2^-22, and to no less than
                the smallest step of f16, 2^-24, held times 2^12 against the row's largest weight: half of that,
                2^-37, of every value seen, however small its weight (the sum of weights is the largest one or more).
                Long prompts of 16-bit queries hold weight times value scale times 2^11, against the largest such
@@ -120,7 +122,7 @@ def attention_tolerance(out, lse, magnitude, spread, dtype, dim, length):
       one rounding to the output's type."""
     u = 2.0 ** -23
     score = (dim / 16 + 22) * u * spread + 4 * u
-    rounded = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -12
+    rounded = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -11
     sums = (length / 32 + 64) * u
     weighted, plain = magnitude
     smallest = 2.0 ** -37 if dtype == torch.float32 else 2.0 ** -33
