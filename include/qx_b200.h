@@ -637,7 +637,8 @@ QX_API qx_status qx_rope_apply_dev(const qx_rope* rope, const qx_heads* x, const
  * scale for the keys and one for the values, value = code * scale. Memory is the caller's. A block
  * holds [kv_heads][block_tokens][head_dim] codes. block_tokens is 16, 32, 64 or 128; head_dim a
  * multiple of 16, 16 .. 256; the code arrays start on 16-byte boundaries. Blocks need no initial
- * contents: nothing behind a sequence's length is used. */
+ * contents: nothing behind a sequence's length is used. Scales are zero or more, or NaN (append makes
+ * no others). */
 typedef struct qx_kv_cache {
   int8_t* k_codes;         /* [blocks][kv_heads][block_tokens][head_dim] */
   int8_t* v_codes;
@@ -681,7 +682,7 @@ typedef struct qx_kv_batch {
  *
  * `rope` (optional, rotary_dim a multiple of 16) rotates the keys on the way, in f32 and without a
  * rounding in between, by positions[row] or, with positions NULL, by the token's place in its sequence;
- * `q` / `q_out` (both or neither, only with rope) rotates the queries into q_out in the same launch, as
+ * `q` / `q_out` (both or neither, only with rope) rotates the queries into q_out (which may be q) in the same call, as
  * qx_rope_apply does. k and v have the cache's kv_heads; all views may have types of their own, q_out
  * has q's type. */
 QX_API qx_status qx_kv_append(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k,
@@ -706,8 +707,9 @@ QX_API qx_status qx_kv_read_dev(const qx_kv_cache* cache, const qx_kv_batch* bat
  * sequence may have more rows than tokens. `lse` (optional, f32 [tokens][heads]): ln of the sum of
  * exp(scale * q . k) over the keys seen.
  * Products are taken to at least the precision of q's type, sums and softmax statistics are f32; f32
- * queries are multiplied with f32 precision. Partial results of splits over the keys live in
- * `workspace` (NULL: the library's default one). The result bits do not depend on when CTAs run; they may on
+ * queries are multiplied with f32 precision. `out` may be q itself, the same view of it. Partial
+ * results of splits over the keys live in `workspace` (NULL: the library's default one); calls that may
+ * run at the same time need one each. The result bits do not depend on when CTAs run; they may on
  * max_tokens, max_length and the number of sequences, which choose the splits. */
 QX_API qx_status qx_kv_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q,
                                  const qx_heads* out, float* lse, float scale, int causal,

@@ -35,8 +35,6 @@
 
 namespace qx {
 namespace kv {
-
-
 namespace {
 
 // P is held times 2^12 where it is rounded to 16 bits, so that weights down to 2^-26 keep all their bits;
@@ -883,7 +881,7 @@ qx_status launch_sized(const AttentionParams& p, int dp, bool wide, bool balance
 }  // namespace
 
 qx_status check_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q, const qx_heads* out,
-                          float scale, long long window) {
+                          const float* lse, float scale, long long window) {
   QX_TRY(check_cache(cache));
   QX_TRY(check_batch(cache, batch));
   QX_TRY(check_heads(q, batch->tokens, cache->head_dim, false));
@@ -892,7 +890,11 @@ qx_status check_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, co
   if (static_cast<__int128>(batch->max_tokens) * (q->heads / cache->kv_heads) > 0x7FFFFFFF - 4096) {
     return QX_STATUS_INVALID_SHAPE;
   }
-  if (!std::isfinite(scale) || window < 0) return QX_STATUS_INVALID_ARGUMENT;
+  if (!std::isfinite(scale) || window < 0 || !on_boundary(lse)) return QX_STATUS_INVALID_ARGUMENT;
+  if (q->data == out->data && batch->tokens > 0 &&
+      (q->type != out->type || q->token_stride != out->token_stride || q->head_stride != out->head_stride)) {
+    return QX_STATUS_INVALID_ARGUMENT;  // (the queries' place, but another view)
+  }
   return QX_STATUS_OK;
 }
 
@@ -984,7 +986,7 @@ using namespace qx;
 extern "C" qx_status qx_kv_attention_dev(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q,
                                          const qx_heads* out, float* lse_dev, float scale, int causal, long long window,
                                          qx_workspace* workspace, void* stream) {
-  QX_TRY(kv::check_attention(cache, batch, q, out, scale, window));
+  QX_TRY(kv::check_attention(cache, batch, q, out, lse_dev, scale, window));
   DeviceContext* ctx = nullptr;
   QX_TRY(current_context(&ctx));
   return kv::launch_attention(cache, batch, q, out, lse_dev, scale, causal, window, ctx,

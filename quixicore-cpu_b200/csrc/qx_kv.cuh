@@ -16,6 +16,12 @@ constexpr int kErrorFirstBatch = 64;  // from here on: the batch, not a stalled 
 constexpr int kErrorSequence = 64;    // a sequence's rows or length do not fit the bounds
 constexpr int kErrorBlock = 65;       // a block id outside the cache
 
+// On a boundary of its elements; NULL is.
+template <class T>
+bool on_boundary(const T* data) {
+  return reinterpret_cast<uintptr_t>(data) % sizeof(T) == 0;
+}
+
 struct Heads {
   uint8_t* data;
   int type;
@@ -63,8 +69,6 @@ __device__ __forceinline__ bool sequence_of(const Batch& b, int s, bool rows_are
 
 __device__ __forceinline__ float bf16_low(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-
-__device__ __forceinline__ size_t storage_size(int type) { return type == QX_STORAGE_F32 ? 4 : 2; }
 
 __device__ __forceinline__ float load_one(const uint8_t* data, int type, long long index) {
   if (type == QX_STORAGE_F32) return reinterpret_cast<const float*>(data)[index];

@@ -13,10 +13,10 @@ namespace qx {
 namespace kv {
 
 qx_status check_append(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k, const qx_heads* v,
-                       const qx_rope* rope, const qx_heads* q, const qx_heads* q_out);
+                       const qx_rope* rope, const int64_t* positions, const qx_heads* q, const qx_heads* q_out);
 qx_status check_read(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k, const qx_heads* v);
 qx_status check_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q, const qx_heads* out,
-                          float scale, long long window);
+                          const float* lse, float scale, long long window);
 qx_status launch_append(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k, const qx_heads* v,
                         const qx_rope* rope, const int64_t* positions, const qx_heads* q, const qx_heads* q_out,
                         DeviceContext* ctx, cudaStream_t stream);
@@ -243,7 +243,7 @@ qx_status qx_rope_apply(const qx_rope* rope, const qx_heads* x, const qx_heads* 
 
 qx_status qx_kv_append(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k, const qx_heads* v,
                        const qx_rope* rope, const int64_t* positions, const qx_heads* q, const qx_heads* q_out) {
-  QX_TRY(check_append(cache, batch, k, v, rope, q, q_out));
+  QX_TRY(check_append(cache, batch, k, v, rope, positions, q, q_out));
   return guarded([&]() -> qx_status {
     Packed p;
     QX_TRY(pack(cache, batch, true, true, &p));
@@ -304,7 +304,7 @@ qx_status qx_kv_read(const qx_kv_cache* cache, const qx_kv_batch* batch, const q
 
 qx_status qx_kv_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q, const qx_heads* out,
                           float* lse, float scale, int causal, long long window) {
-  QX_TRY(check_attention(cache, batch, q, out, scale, window));
+  QX_TRY(check_attention(cache, batch, q, out, lse, scale, window));
   return guarded([&]() -> qx_status {
     Packed p;
     QX_TRY(pack(cache, batch, false, false, &p));

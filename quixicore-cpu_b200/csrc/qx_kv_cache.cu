@@ -461,6 +461,9 @@ qx_status check_batch(const qx_kv_cache* cache, const qx_kv_batch* batch) {
   if (batch->sequences > 0 && (batch->lengths == nullptr || (batch->max_length > 0 && batch->block_table == nullptr))) {
     return QX_STATUS_INVALID_ARGUMENT;
   }
+  if (!on_boundary(batch->token_begin) || !on_boundary(batch->lengths) || !on_boundary(batch->block_table)) {
+    return QX_STATUS_INVALID_ARGUMENT;
+  }
   return QX_STATUS_OK;
 }
 
@@ -484,7 +487,7 @@ Batch device_batch(const qx_kv_cache* cache, const qx_kv_batch* batch, int* erro
 }
 
 qx_status check_append(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k, const qx_heads* v,
-                       const qx_rope* rope, const qx_heads* q, const qx_heads* q_out) {
+                       const qx_rope* rope, const int64_t* positions, const qx_heads* q, const qx_heads* q_out) {
   QX_TRY(check_cache(cache));
   QX_TRY(check_batch(cache, batch));
   QX_TRY(check_heads(k, batch->tokens, cache->head_dim, false));
@@ -495,6 +498,7 @@ qx_status check_append(const qx_kv_cache* cache, const qx_kv_batch* batch, const
     if (rope->rotary_dim % 16 != 0) return QX_STATUS_INVALID_SHAPE;
   }
   if ((q == nullptr) != (q_out == nullptr) || (q != nullptr && rope == nullptr)) return QX_STATUS_INVALID_ARGUMENT;
+  if (!on_boundary(positions)) return QX_STATUS_INVALID_ARGUMENT;
   if (q != nullptr) {
     QX_TRY(check_heads(q, batch->tokens, cache->head_dim, false));
     QX_TRY(check_heads(q_out, batch->tokens, cache->head_dim, true));
@@ -605,7 +609,7 @@ extern "C" {
 qx_status qx_kv_append_dev(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k, const qx_heads* v,
                            const qx_rope* rope, const int64_t* positions_dev, const qx_heads* q, const qx_heads* q_out,
                            void* stream) {
-  QX_TRY(kv::check_append(cache, batch, k, v, rope, q, q_out));
+  QX_TRY(kv::check_append(cache, batch, k, v, rope, positions_dev, q, q_out));
   DeviceContext* ctx = nullptr;
   QX_TRY(current_context(&ctx));
   return kv::launch_append(cache, batch, k, v, rope, positions_dev, q, q_out, ctx, static_cast<cudaStream_t>(stream));

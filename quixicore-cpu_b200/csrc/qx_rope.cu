@@ -173,7 +173,7 @@ qx_status check_rope_call(const qx_rope* rope, const qx_heads* x, const qx_heads
   QX_TRY(check_heads(y, tokens, dim, true));
   if (x->heads != y->heads) return QX_STATUS_INVALID_SHAPE;
   if (x->type != y->type) return QX_STATUS_UNSUPPORTED_FORMAT;
-  if (tokens > 0 && positions == nullptr) return QX_STATUS_INVALID_ARGUMENT;
+  if ((tokens > 0 && positions == nullptr) || !on_boundary(positions)) return QX_STATUS_INVALID_ARGUMENT;
   if (x->data == y->data && (x->token_stride != y->token_stride || x->head_stride != y->head_stride)) {
     return QX_STATUS_INVALID_ARGUMENT;
   }

@@ -272,3 +272,35 @@ def test_device_forms_check_the_same_shapes(qx, parts):
     assert qx.lib.qx_kv_read_dev(bad, batch.view, H(x), H(x), None) == qx.INVALID_SHAPE
     assert qx.lib.qx_kv_attention_dev(bad, batch.view, H(q), H(q), None, 1.0, 1, 0, None, None) == qx.INVALID_SHAPE
     assert qx.lib.qx_rope_apply_dev(qx.Rope(32).view, H(x), H(x), None, 3, 32, 0, None) == qx.INVALID_ARGUMENT
+
+
+def test_arrays_off_their_boundaries_are_refused(qx, parts):
+    """Positions, batch arrays and lse that start inside an element, by both forms."""
+    cache, batch, x, q = parts
+    H, rope, room = qx.heads_view, qx.Rope(32), np.zeros(64, np.uint8)
+    odd = room.ctypes.data + 4
+    odd += 8 - odd % 8 + 2
+    for field in ("token_begin", "lengths", "block_table"):
+        bad = qx.KVBatchView.from_buffer_copy(batch.view)
+        setattr(bad, field, odd)
+        for name, call in each_call(qx, cache.view, batch.view, x, q):
+            assert call(b=bad) == qx.INVALID_ARGUMENT, (name, field)
+        assert qx.lib.qx_kv_append_dev(cache.view, bad, H(x), H(x), None, None, None, None, None) == qx.INVALID_ARGUMENT
+        assert qx.lib.qx_kv_read_dev(cache.view, bad, H(x), H(x), None) == qx.INVALID_ARGUMENT
+        assert qx.lib.qx_kv_attention_dev(cache.view, bad, H(q), H(q), None, 1.0, 1, 0, None, None) == qx.INVALID_ARGUMENT
+    for at in (odd, odd + 2):
+        assert qx.lib.qx_kv_append(cache.view, batch.view, H(x), H(x), rope.view, at, None, None) == qx.INVALID_ARGUMENT
+        assert qx.lib.qx_kv_append_dev(cache.view, batch.view, H(x), H(x), rope.view, at, None, None, None) == qx.INVALID_ARGUMENT
+        assert qx.lib.qx_rope_apply(rope.view, H(x), H(x), at, 3, 32, 0) == qx.INVALID_ARGUMENT
+        assert qx.lib.qx_rope_apply_dev(rope.view, H(x), H(x), at, 3, 32, 0, None) == qx.INVALID_ARGUMENT
+    assert qx.lib.qx_kv_attention(cache.view, batch.view, H(q), H(q), odd, 1.0, 1, 0) == qx.INVALID_ARGUMENT
+    assert qx.lib.qx_kv_attention_dev(cache.view, batch.view, H(q), H(q), odd, 1.0, 1, 0, None, None) == qx.INVALID_ARGUMENT
+
+
+def test_an_output_that_begins_where_the_queries_do_is_the_same_view(qx, parts):
+    cache, batch, x, q = parts
+    H = qx.heads_view
+    call = lambda b: qx.lib.qx_kv_attention(cache.view, batch.view, H(q), b, None, 1.0, 1, 0)  # noqa: E731
+    assert served(qx, call(H(q)))
+    assert call(H(q, kind=qx.BF16)) == qx.INVALID_ARGUMENT
+    assert call(H(q, token_stride=2 * q.shape[1] * q.shape[2])) == qx.INVALID_ARGUMENT
