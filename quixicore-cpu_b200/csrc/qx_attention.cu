@@ -153,7 +153,7 @@ __device__ __forceinline__ uint32_t rest_f16(float a, float b, uint32_t rounded)
 
 // A balanced launch's line: per item, kItemCost units for what a CTA does before its first tile and behind its last, and
 // one per tile (4 | 8 | 12 | 16 | 24 units, us: 32 sessions of up to 8192 66.4 | 65.0 | 64.5 | 64.7 | 67.2, 8 of five
-// tokens in windows of 4096 29.0 | 26.7 | 26.2 | 26.2 | 27.0).
+// tokens in windows of 4096 29.0 | 26.7 | 26.2 | 26.2 | 27.0; later steps changed all alike).
 constexpr int kItemCost = 12, kLeastPiece = 8, kBalancedSequences = 128;
 struct Line {
   uint32_t begin[kBalancedSequences / 32];  // of sequence lane + 32 i
@@ -324,13 +324,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
   // Two bits for every tile in flight: which of its halves are there.
   uint32_t there = 0;
   const auto note = [&](const int (&id)[2]) { there = there << 2 | (id[0] >= 0 ? 1u : 0u) | (id[1] >= 0 ? 2u : 0u); };
-  int next_ids[2];
+  // (all loads that need no other's result before the first that does)
+  int first_ids[kStages - 1][2], next_ids[2];
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    ids_of(warp + i * kWarps, next_ids);
-    note(next_ids);
-    issue(warp + i * kWarps, i, next_ids);
-  }
+  for (int i = 0; i < kStages - 1; ++i) ids_of(warp + i * kWarps, first_ids[i]);
   ids_of(warp + (kStages - 1) * kWarps, next_ids);
 
   // ---- queries: whole numbers below 2^23 times a power of two per row, as three digits -----------------------
@@ -348,6 +345,11 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
       v[own][i][0] = v[own][i][1] = v[own][i][2] = v[own][i][3] = 0.0f;
       if (r < rows.count && d < p.dim) load4(p.q.data, p.q.type, p.q.vector, base + d, v[own][i]);
     }
+  }
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    note(first_ids[i]);
+    issue(warp + i * kWarps, i, first_ids[i]);
   }
 #pragma unroll
   for (int own = 0; own < kOwnRows; ++own) {
@@ -392,14 +394,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
   }
   __syncthreads();
   // (in registers where there is room for them, else read as they are needed)
-  constexpr bool kResident = kRowTiles == 1 && DP <= 64;
-  uint2 resident[kResident ? 3 * kSteps : 1];
+  constexpr bool kResident = DP <= 64 && (kRowTiles == 1 || !kWide);
+  constexpr int kOperands = 3 * kSteps * kRowTiles;
+  uint2 resident[kResident ? kOperands : 1];
   if (kResident) {
 #pragma unroll
-    for (int i = 0; i < 3 * kSteps; ++i) resident[i] = reinterpret_cast<const uint2*>(queries)[i * 32 + lane];
+    for (int i = 0; i < kOperands; ++i) resident[i] = reinterpret_cast<const uint2*>(queries)[i * 32 + lane];
   }
   const auto query = [&](int digit, int n, int j) {
-    if (kResident) return resident[(digit * kSteps + j) % (3 * kSteps)];
+    if (kResident) return resident[((digit * kRowTiles + n) * kSteps + j) % kOperands];
     return reinterpret_cast<const uint2*>(queries + digit * kRows * DP)[(n * kSteps + j) * 32 + lane];
   };
 
@@ -558,11 +561,16 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
       if (ratio[0] != ratio[1]) {  // (also where one is no number)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
+          if (ratio[k] < INFINITY) {
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const int key = token0 + 16 * k + 8 * (h >> 1) + g;
-            const bool hidden = !open && (!(present >> k & 1) || key < low[n][h & 1] || key >= high[n][h & 1]);
-            score[n][k][h] = hidden ? 0.0f : score[n][k][h] * ratio[k];
+            for (int h = 0; h < 4; ++h) score[n][k][h] *= ratio[k];
+          } else {  // (hidden weights stay zero)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const int key = token0 + 16 * k + 8 * (h >> 1) + g;
+              const bool hidden = !open && (!(present >> k & 1) || key < low[n][h & 1] || key >= high[n][h & 1]);
+              score[n][k][h] = hidden ? 0.0f : score[n][k][h] * ratio[k];
+            }
           }
         }
         __syncwarp();
