@@ -5,6 +5,10 @@
 // A code needs the block's final scale, so the new elements wait in registers for it (two units of 16 per thread
 // at most; larger blocks are read twice, the second time out of the caches). Bound by HBM for prompts (element
 // in, code out) and by the chain of loads length -> block -> scale for single tokens.
+//
+// Measured with the read behind it: 6570 f32 tokens of 8 heads of 128 elements, 49 us together (184 MB, 3.7 TB/s; the
+// append 28 us by itself, under a profiler: waiting for its loads, issue slots half taken); 64 single bf16 tokens with
+// 32 rotated query heads each, 14.7 us.
 
 #include <algorithm>
 #include <limits>
@@ -546,7 +550,8 @@ qx_status launch_append(const qx_kv_cache* cache, const qx_kv_batch* batch, cons
   const int most = static_cast<int>(std::min<long long>(batch->max_tokens, batch->max_length));
   p.blocks_per_sequence = blocks_reached(most, cache->block_tokens);
   // The angles of a block's tokens are shared by the heads that a CTA takes, and the loads of one head run beside
-  // the work on the one before: as many as leave a few CTAs for every SM.
+  // the work on the one before: as many as leave a few CTAs for every SM (at least 4 | 12 | 36 CTAs, append and read of
+  // 6570 f32 tokens, 8 heads, us: rotated with 32 query heads 108 | 116 | 144, not rotated 50 | 49 | 57).
   const long long blocks = static_cast<long long>(batch->sequences) * p.blocks_per_sequence;
   const long long spread = 4LL * sm_count(ctx);
   const long long heads = 2 * blocks * cache->kv_heads / (rope != nullptr ? spread : 3 * spread);
@@ -556,8 +561,9 @@ qx_status launch_append(const qx_kv_cache* cache, const qx_kv_batch* batch, cons
   const int pairs = p.rotation.rotary / 2;
   size_t smem = static_cast<size_t>(std::min(most, cache->block_tokens)) * pairs * sizeof(float2);
   const long long tokens = static_cast<long long>(batch->sequences) * most;
-  if (q != nullptr && tokens > spread) {
-    // many queries: a launch of their own, with the registers and shared memory that they need
+  if (q != nullptr && tokens > 3 * spread) {
+    // many queries: a launch of their own, with the registers and shared memory that they need (beside the append | by
+    // itself, append and read of bf16, 32 query heads, us: 1000 tokens 20.7 | 23.9, 2000 36.9 | 33.5, 6570 120 | 84)
     QX_TRY(launch_rope_batch(rope, q, q_out, positions, p.batch, most, cache->head_dim, ctx, stream));
   } else if (q != nullptr) {
     p.tokens_per_cta = 1;
@@ -565,6 +571,8 @@ qx_status launch_append(const qx_kv_cache* cache, const qx_kv_batch* batch, cons
     grid += static_cast<long long>(batch->sequences) * p.query_ctas;
     smem = std::max(smem, static_cast<size_t>(p.tokens_per_cta) * pairs * sizeof(float2));
   }
+  // Elements held in registers | read twice, append and read, us: 6570 f32 tokens 49 | 57, bf16 42 | 60, 64 single
+  // tokens 14.7 | 15.8.
   const int units = std::min(most, cache->block_tokens) * (cache->head_dim / 16);
   if (k->type != v->type || !p.x[0].vector || !p.x[1].vector || units > 2 * kThreads) {
     return launch_append_of<0, QX_STORAGE_F32>(p, grid, smem, stream);
