@@ -533,24 +533,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         const int piece = lane % kLanes, d = piece * kElements, warp_row = which * kRowTile + (warp & 3) * 32;
         uint8_t* const tile = smem + S::kQueries + which * S::kOperand;
         RowWalk from(p.q, rows, head, p.group, rows.first + warp_row + lane / kLanes, kAtOnce);
-        const bool vector = p.q.vector;
-#pragma unroll 4
-        for (int i = lane / kLanes; i < 32; i += kAtOnce) {
-          uint8_t* const to = piece_at<DP, kWide>(tile, (warp & 3) * 32 + i, piece);
-          const bool there = warp_row + i < rows.count && d < p.dim;
-          const uint8_t* const at = p.q.data + (there ? from.at + d : 0) * kBytes;
-          if (vector || !there) {  // (of no bytes: zeros)
+        if (p.q.vector) {
+#pragma unroll 8
+          for (int i = lane / kLanes; i < 32; i += kAtOnce) {
+            const bool there = warp_row + i < rows.count && d < p.dim;  // (or no bytes: zeros)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                         ::"r"(smem_u32(to)), "l"(vector ? at : reinterpret_cast<const uint8_t*>(p.k_codes)), "r"(there ? 16 : 0)
+                         ::"r"(smem_u32(piece_at<DP, kWide>(tile, (warp & 3) * 32 + i, piece))),
+                         "l"(p.q.data + (there ? from.at + d : 0) * kBytes), "r"(there ? 16 : 0)
                          : "memory");
-          } else {
-#pragma unroll 1
-            for (int e = 0; e < 16; e += kBytes) {
-              if (kWide) *reinterpret_cast<uint32_t*>(to + e) = *reinterpret_cast<const uint32_t*>(at + e);
-              else *reinterpret_cast<uint16_t*>(to + e) = *reinterpret_cast<const uint16_t*>(at + e);
-            }
+            from.next();
           }
-          from.next();
+        } else {
+#pragma unroll 1
+          for (int i = lane / kLanes; i < 32; i += kAtOnce) {
+            uint8_t* const to = piece_at<DP, kWide>(tile, (warp & 3) * 32 + i, piece);
+            const bool there = warp_row + i < rows.count && d < p.dim;
+#pragma unroll 1
+            for (int e = 0; e < kElements; ++e) {
+              if (kWide) reinterpret_cast<uint32_t*>(to)[e] = there ? reinterpret_cast<const uint32_t*>(p.q.data)[from.at + d + e] : 0;
+              else reinterpret_cast<uint16_t*>(to)[e] = there ? reinterpret_cast<const uint16_t*>(p.q.data)[from.at + d + e] : 0;
+            }
+            from.next();
+          }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncwarp();
