@@ -193,3 +193,53 @@ def test_rows_of_nobody_beside_many_queries(qx, dtype):
     assert rope.apply_dev(q, want, positions) == qx.OK
     assert on_device(qx, cache).append_dev(batch, k, k, rope, q, out) == qx.OK
     assert torch.equal(out[:-3], want[:-3]) and bool((out[-3:] == 7).all())
+
+
+@pytest.mark.parametrize("lengths,new", [([900, 70, 300], [1, 1, 1]), ([900], [1]), ([900, 200], [60, 200])])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_blocks_past_two_gigabytes(qx, lengths, new, dtype):
+    """Few blocks of a cache of 2.4 GB of codes each for keys and values, the last ones: the same as in a small cache."""
+    size, dim, heads, count = 128, 128, 2, 74000  # 32 KB of codes a block
+    small, table = filled(16, heads, size, dim), table_of(len(lengths), 8 if len(lengths) < 3 else 5, 16)
+    width = -(-max(lengths) // size)
+    table = np.resize(table, (len(lengths), width)).astype(np.int32)
+    near = on_device(qx, small)
+    far = qx.KVCache.empty(count, heads, size, dim)
+    for to, come in zip(far.arrays, near.arrays):
+        to[count - 16:] = come
+    batch, _, rows = batch_of(qx, table, lengths, new)
+    moved, _, _ = batch_of(qx, table + (count - 16), lengths, new)
+    q = typed((rows, 4, dim), dtype, 3).cuda()
+    want, got = torch.zeros_like(q), torch.zeros_like(q)
+    assert near.attention_dev(batch, q, want) == qx.OK and far.attention_dev(moved, q, got) == qx.OK
+    torch.cuda.synchronize()
+    assert qx.lib.qx_check_device_errors() == qx.OK and bool((want != 0).any())
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("new", [3, 60])
+def test_views_past_two_gigabytes(qx, new):
+    """Heads whose rows lie so far apart that their offsets pass 32 bits, in every operator."""
+    heads, dim, size = 2, 64, 32
+    stride = ((1 << 31) // (new - 1) + 4096) // 64 * 64  # elements: the last row lies behind 2^31
+    room = torch.zeros((new - 1) * stride + heads * dim, dtype=BF16, device="cuda")
+    wide = room.as_strided((new, heads, dim), (stride, dim, 1))
+    x = typed((new, heads, dim), BF16, 1).cuda()
+    wide.copy_(x)
+    cache, table = filled(8, heads, size, dim), table_of(1, 4, 8)
+    batch, _, _ = batch_of(qx, table, [100], [new])
+    rope, positions = qx.Rope(dim), torch.arange(new, device="cuda")
+    for turned in (lambda src, dst: rope.apply_dev(src, dst, positions),
+                   lambda src, dst: on_device(qx, cache).append_dev(batch, x, x, rope, src, dst),
+                   lambda src, dst: on_device(qx, cache).attention_dev(batch, src, dst),
+                   lambda src, dst: on_device(qx, cache).read_dev(batch, dst, None)):
+        want, got = torch.zeros_like(x), torch.zeros_like(x)
+        assert turned(x, want) == qx.OK and turned(wide, got) == qx.OK, qx.last_error()
+        assert torch.equal(got, want) and bool((want != 0).any())
+        assert turned(x, wide) == qx.OK, qx.last_error()
+        assert torch.equal(wide, want)
+        wide.copy_(x)
+    near, far = (on_device(qx, cache) for _ in range(2))
+    assert near.append_dev(batch, x, x) == qx.OK and far.append_dev(batch, wide, wide) == qx.OK
+    for a, b in zip(near.arrays, far.arrays):
+        assert torch.equal(a, b)
