@@ -336,17 +336,20 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
   ids_of(warp + (kStages - 1) * kWarps, next_ids);
 
   // ---- queries: whole numbers below 2^23 times a power of two per row, as three digits -----------------------
-  // A lane takes four neighbouring elements (of 128 at a time), all of the warp's rows before any is used.
-  constexpr int kOwnRows = kRows / kWarps, kOwnRuns = (DP + 127) / 128;
+  // A lane takes four neighbouring elements (of 128 at a time; of two rows of 64), all of the warp's rows before any is
+  // used.
+  constexpr int kAtOnce = DP < 128 ? 128 / DP : 1, kRowLanes = 32 / kAtOnce;
+  constexpr int kOwnRows = kRows / kWarps / kAtOnce, kOwnRuns = (DP + 127) / 128;
+  const int own_lane = lane % kRowLanes;
   float v[kOwnRows][kOwnRuns][4];
 #pragma unroll
   for (int own = 0; own < kOwnRows; ++own) {
-    const int r = own * kWarps + warp, token = (rows.first + r) / p.group;
+    const int r = (own * kWarps + warp) * kAtOnce + lane / kRowLanes, token = (rows.first + r) / p.group;
     const long long base = (rows.row + token) * p.q.token_stride +
                            (static_cast<long long>(head) * p.group + (rows.first + r - token * p.group)) * p.q.head_stride;
 #pragma unroll
     for (int i = 0; i < kOwnRuns; ++i) {
-      const int d = i * 128 + lane * 4;
+      const int d = i * 128 + own_lane * 4;
       v[own][i][0] = v[own][i][1] = v[own][i][2] = v[own][i][3] = 0.0f;
       if (r < rows.count && d < p.dim) load4(p.q.data, p.q.type, p.q.vector, base + d, v[own][i]);
     }
@@ -358,25 +361,25 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
   }
 #pragma unroll
   for (int own = 0; own < kOwnRows; ++own) {
-    const int r = own * kWarps + warp;
+    const int r = (own * kWarps + warp) * kAtOnce + lane / kRowLanes;
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < kOwnRuns; ++i) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v[own][i][e]) & 0x7FFFFFFFu);
     }
-    top = __reduce_max_sync(0xFFFFFFFFu, top) >> 23;
+    top = __reduce_max_sync(kAtOnce == 1 ? 0xFFFFFFFFu : lane < 16 ? 0xFFFFu : 0xFFFF0000u, top) >> 23;
     // the row's largest magnitude becomes 2^21 .. 2^22: three balanced digits reach 127 * (1 + 2^8 + 2^16)
     const int shift = min(126, max(-126, 148 - static_cast<int>(top)));
     const float factor = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-    if (lane == 0) {
+    if (own_lane == 0) {
       // (a row that holds a NaN or an infinity gives NaN)
       row_factor[r] = top >= 255 ? __uint_as_float(0x7FC00000u)
                                  : __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * p.scale_log2;
     }
 #pragma unroll
     for (int i = 0; i < kOwnRuns; ++i) {
-      const int d = i * 128 + lane * 4;
+      const int d = i * 128 + own_lane * 4;
       uint32_t x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
