@@ -27,9 +27,9 @@
 // additions, so each tile's product goes to one of two buffers of O, and warps 4-7 add those up in registers, in
 // f32, with the maxima's changes in between.
 //
-// Measured: two prompts of up to 4096 bf16 tokens, 32 query heads on 8, 128 elements, causal: 310 us (208 GFLOP, 670
+// Measured: two prompts of up to 4096 bf16 tokens, 32 query heads on 8, 128 elements, causal: 309 us (208 GFLOP, 670
 // TFLOP/s); 1024 f16 tokens behind 15360: 321 us (830 TFLOP/s); 4 texts of up to 500 f32 tokens, 16 heads of 96
-// elements: 51 us. A tile of 128 keys takes 4600 cycles for both row tiles, where the MMAs alone take 2050 and the
+// elements: 50 us. A tile of 128 keys takes 4600 cycles for both row tiles, where the MMAs alone take 2050 and the
 // exponentials 2050: a row tile's S, softmax and P V follow one another, and only the other row tile runs beside them.
 // A CTA's way in (11000 cycles: table, queries to operands, first keys) and out (6000) comes on top.
 //
