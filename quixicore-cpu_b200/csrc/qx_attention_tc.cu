@@ -27,9 +27,9 @@
 // additions, so each tile's product goes to one of two buffers of O, and warps 4-7 add those up in registers, in
 // f32, with the maxima's changes in between.
 //
-// Measured: two prompts of up to 4096 bf16 tokens, 32 query heads on 8, 128 elements, causal: 309 us (208 GFLOP, 670
+// Measured: two prompts of up to 4096 bf16 tokens, 32 query heads on 8, 128 elements, causal: 305 us (208 GFLOP, 680
 // TFLOP/s); 1024 f16 tokens behind 15360: 321 us (830 TFLOP/s); 4 texts of up to 500 f32 tokens, 16 heads of 96
-// elements: 50 us. A tile of 128 keys takes 4600 cycles for both row tiles, where the MMAs alone take 2050 and the
+// elements: 46.5 us. A tile of 128 keys takes 4600 cycles for both row tiles, where the MMAs alone take 2050 and the
 // exponentials 2050: a row tile's S, softmax and P V follow one another, and only the other row tile runs beside them.
 // A CTA's way in (11000 cycles: table, queries to operands, first keys) and out (6000) comes on top.
 //
@@ -167,8 +167,14 @@ struct RowState {
 
 // One tile of scores to weights, in TMEM. `scores`: this warp's lanes of S, which P replaces; `sums`: of O. Keys
 // share scales by `kUnit`s of 16 or 32.
+// kOpen: no row of the warp has a hidden key. kHidden: some have; those scores become -infinity before anything else
+// is done with them. kSpecial: besides, a scale is no plain number (zero, infinite, NaN), which would take -infinity
+// to NaN: hidden keys are told apart at every step. (Two prompts of up to 4096, one of 1024 behind 15360, f32 texts
+// of up to 500, us: kOpen and kSpecial alone 308, 321, 49.5; one form for the first two 327, 360, 46.7; these three 305, 322,
+// 46.5.)
 // kWide: the row's factor for what O holds so far goes to *keep_to instead.
-template <int DP, int kUnit, bool kMasked, bool kWide>
+enum Mask { kOpen, kHidden, kSpecial };
+template <int DP, int kUnit, Mask kMask, bool kWide>
 __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, const Meta& meta, RowState& row, int key0,
                                              bool first, uint64_t* first_half, float* keep_to) {
   constexpr int kUnits = kKeys / kUnit, kPerUnit = kUnit / 16;
@@ -185,7 +191,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
     log[u] = scales.y;
     relative[u] = meta.value_inverse[u * kPerUnit];
     const int key = key0 + kUnit * u;
-    const bool seen = !kMasked || (meta.present[u * kPerUnit] != 0 && key < row.high && key + kUnit > row.low);
+    const bool seen = kMask == kOpen || (meta.present[u * kPerUnit] != 0 && key < row.high && key + kUnit > row.low);
     largest = fmaxf(largest, seen ? log[u] : -INFINITY);
   }
   if (largest > row.largest_log) {
@@ -201,16 +207,25 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   }
 
   const auto hidden = [&](int key) { return key < row.low || key >= row.high; };
+  const auto hide = [&](int c) {  // of 32 keys
+    const int low = min(max(row.low - key0 - 32 * c, 0), 32), high = min(max(row.high - key0 - 32 * c, 0), 32);
+    uint32_t seen = static_cast<uint32_t>((1ull << high) - 1) & ~static_cast<uint32_t>((1ull << low) - 1);
+    if (meta.present[2 * c] == 0) seen &= 0xFFFF0000u;
+    if (meta.present[2 * c + 1] == 0) seen &= 0xFFFFu;
+    if (__all_sync(0xFFFFFFFFu, seen == 0xFFFFFFFFu)) return;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s[c][i] = (seen >> i & 1) != 0 ? s[c][i] : 0xFF800000u;
+  };
   float top = -INFINITY;
   const auto top_of = [&](int u) {
-    const bool present = !kMasked || meta.present[u * kPerUnit] != 0;
+    const bool present = kMask != kSpecial || meta.present[u * kPerUnit] != 0;
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (four chains: one would wait for itself)
 #pragma unroll
     for (int i = 0; i < kUnit; i += 2) {
       const int at = kUnit * u + i;
       const float a = __uint_as_float(s[at / 32][at % 32]), b = __uint_as_float(s[at / 32][at % 32 + 1]);
       float& chain = m[i / 2 % 4];
-      if (!kMasked) {
+      if (kMask != kSpecial) {
         chain = max3(chain, a, b);
       } else {
         if (present && !hidden(key0 + at)) chain = fmaxf(chain, a);
@@ -219,16 +234,24 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
     }
     const float most = fmaxf(max3(m[0], m[1], m[2]), m[3]);
     // (nothing seen: -infinity times a factor that may be zero or no number)
-    top = fmaxf(top, kMasked && most == -INFINITY ? -INFINITY : fmaf(most, factor[u], log[u]));
+    top = fmaxf(top, kMask == kSpecial && most == -INFINITY ? -INFINITY : fmaf(most, factor[u], log[u]));
   };
   tmem_ld_wait_for(s[0]);
   tmem_ld_wait_for(s[1]);
   tmem_ld_32x32(scores + 64, s[2]);
   tmem_ld_32x32(scores + 96, s[3]);
+  if (kMask == kHidden) {
+    hide(0);
+    hide(1);
+  }
 #pragma unroll
   for (int u = 0; u < kUnits / 2; ++u) top_of(u);
   tmem_ld_wait_for(s[2]);
   tmem_ld_wait_for(s[3]);
+  if (kMask == kHidden) {
+    hide(2);
+    hide(3);
+  }
 #pragma unroll
   for (int u = kUnits / 2; u < kUnits; ++u) top_of(u);
 
@@ -266,7 +289,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
       const float add = log[u] - base;
       const unsigned long long f2 = tile::pack2(__float_as_uint(factor[u]), __float_as_uint(factor[u]));
       const unsigned long long c2 = tile::pack2(__float_as_uint(add), __float_as_uint(add));
-      const bool present = !kMasked || meta.present[u * kPerUnit] != 0;
+      const bool present = kMask != kSpecial || meta.present[u * kPerUnit] != 0;
       unsigned long long sum2 = 0;
 #pragma unroll
       for (int i = 0; i < kUnit; i += 2) {
@@ -275,7 +298,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
         uint32_t lo, hi;
         tile::unpack2(t2, lo, hi);
         float a = exp2_fast(__uint_as_float(lo)), b = exp2_fast(__uint_as_float(hi));
-        if (kMasked) {  // (behind exp2: also where the arguments are no numbers)
+        if (kMask == kSpecial) {  // (behind exp2: also where the arguments are no numbers)
           a = !present || hidden(key0 + 32 * c + at) ? 0.0f : a;
           b = !present || hidden(key0 + 32 * c + at + 1) ? 0.0f : b;
         }
@@ -292,7 +315,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
       tile::unpack2(sum2, lo, hi);
       const float sum = __uint_as_float(lo) + __uint_as_float(hi);
       // (a unit that is hidden as a whole may have a scale that is no number)
-      if (!kMasked || sum != 0.0f) row.sum = fmaf(sum, relative[u], row.sum);
+      if (kMask != kSpecial || sum != 0.0f) row.sum = fmaf(sum, relative[u], row.sum);
     }
     tmem_st_32x16(scores + 16 * c, p);
     if (kWide) tmem_st_32x16(scores + kKeys / 2 + 16 * c, low);
@@ -628,9 +651,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         }
         float* const keep_to = keep + j % kKeepStages * kRowTile + r;
         if (__all_sync(0xFFFFFFFFu, open)) {
-          softmax_tile<DP, kUnit, false, kWide>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+          softmax_tile<DP, kUnit, kOpen, kWide>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
         } else {
-          softmax_tile<DP, kUnit, true, kWide>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+          bool plain = true;
+#pragma unroll 1
+          for (int g = 0; g < kGroups; ++g) {
+            const float2 scales = tile_meta.scales[g];
+            const float factor = row.factor * scales.x;
+            plain = plain && factor > 0.0f && factor < INFINITY && fabsf(scales.y) < INFINITY;
+          }
+          if (__all_sync(0xFFFFFFFFu, plain)) {
+            softmax_tile<DP, kUnit, kHidden, kWide>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+          } else {
+            softmax_tile<DP, kUnit, kSpecial, kWide>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+          }
         }
         tc_fence_before_sync();
         __syncwarp();
