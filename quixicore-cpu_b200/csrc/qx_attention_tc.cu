@@ -390,13 +390,20 @@ __device__ __forceinline__ void write_rows(const AttentionParams& p, uint8_t* ti
   __syncwarp();
   if (piece * kElements >= p.dim) return;
   RowWalk to(p.out, rows, head, p.group, rows.first + warp_row + first, kAtOnce);
-#pragma unroll 4
-  for (int r = first; r < 32; r += kAtOnce) {
-    if (warp_row + r < rows.count) {
-      *reinterpret_cast<uint4*>(p.out.data + (to.at + piece * kElements) * (kWide ? 4 : 2)) =
-          *reinterpret_cast<const uint4*>(piece_at<DP, kWide>(tile, (warp_row & (kRowTile - 1)) + r, piece));
+#pragma unroll 1
+  for (int r = first; r < 32; r += 8 * kAtOnce) {
+    uint4 w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = *reinterpret_cast<const uint4*>(piece_at<DP, kWide>(tile, (warp_row & (kRowTile - 1)) + r + i * kAtOnce, piece));
     }
-    to.next();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (warp_row + r + i * kAtOnce < rows.count) {
+        *reinterpret_cast<uint4*>(p.out.data + (to.at + piece * kElements) * (kWide ? 4 : 2)) = w[i];
+      }
+      to.next();
+    }
   }
 }
 // The same elements by the row's own thread, to the partial results or to a view that is not as the above needs it.
