@@ -25,11 +25,12 @@
 // the second tile's place in shared memory holds the low halves of the queries, the second half of S the low halves
 // of the weights, and every product is two. A sum over all keys would lose f32's last bits to the MMA's own
 // additions, so each tile's product goes to one of two buffers of O, and warps 4-7 add those up in registers, in
-// f32, with the maxima's changes in between.
+// f32, with the maxima's changes in between. S has the second row tile's place for the next tile of keys, so that it is
+// ready when a softmax ends (2 x 1000 tokens, 4000 keys, 16 heads of 96 elements: 190 us without, 166 with).
 //
-// Measured: two prompts of up to 4096 bf16 tokens, 32 query heads on 8, 128 elements, causal: 305 us (208 GFLOP, 680
+// Measured: two prompts of up to 4096 bf16 tokens, 32 query heads on 8, 128 elements, causal: 303 us (208 GFLOP, 680
 // TFLOP/s); 1024 f16 tokens behind 15360: 321 us (830 TFLOP/s); 4 texts of up to 500 f32 tokens, 16 heads of 96
-// elements: 46.5 us. A tile of 128 keys takes 4600 cycles for both row tiles, where the MMAs alone take 2050 and the
+// elements: 40.5 us. A tile of 128 keys takes 4600 cycles for both row tiles, where the MMAs alone take 2050 and the
 // exponentials 2050: a row tile's S, softmax and P V follow one another, and only the other row tile runs beside them.
 // A CTA's way in (11000 cycles: table, queries to operands, first keys) and out (6000) comes on top.
 //
@@ -642,9 +643,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       const int open_high = p.causal ? min(rows.length, position0 + 1) : rows.length;
       const int open_low = first_seen(p, position1);
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t scores = tmem + lanes + which * 128, sums = tmem + lanes + 256 + which * 128;
+      const uint32_t sums = tmem + lanes + 256 + which * 128;
       for (int j = 0; ok && j < tiles; ++j) {
-        ok = mbar_wait_warp(&bars->scores[which], j & 1, abort_flag) &&
+        const int own = kWide ? j & 1 : which;  // S, its barriers
+        const uint32_t scores = tmem + lanes + own * 128;
+        ok = mbar_wait_warp(&bars->scores[own], kWide ? j >> 1 & 1 : j & 1, abort_flag) &&
              mbar_wait_warp(&bars->meta[j % kMetaStages], j / kMetaStages & 1, abort_flag);
         if (!ok) break;
         __syncwarp();
@@ -675,7 +678,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->weights[which]);
+        if (lane == 0) mbar_arrive(&bars->weights[own]);
         if (kWide && lane == 0) mbar_arrive(&bars->kept[j % kKeepStages]);
       }
       if (!kWide && ok && tiles > 0) ok = mbar_wait_warp(&bars->sums[which], 0, abort_flag);
@@ -828,11 +831,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
 #pragma unroll
         for (int d = 0; d < DP; d += 16) {
           const uint32_t at = d / 64 * (kRowTile * 128) + d % 64 * 2;
-          mma_f16_ss(tmem + which * 128, make_sw128_kmajor_desc(base + S::kQueries + (which + half) * S::kOperand + at),
+          mma_f16_ss(tmem + (kWide ? stage : which) * 128, make_sw128_kmajor_desc(base + S::kQueries + (which + half) * S::kOperand + at),
                      make_sw128_kmajor_desc(base + S::kKeyRing + stage * S::kOperand + at), scores_desc, d > 0 || (kWide && half == 0));
         }
       }
-      tc_commit(&bars->scores[which]);
+      tc_commit(&bars->scores[kWide ? stage : which]);
     };
     for (int i = 0; ok && i < row_tiles; ++i) ok = mbar_wait(&bars->queries[i], 0, abort_flag);
     if (ok && tiles > 0) ok = mbar_wait(&bars->key_full[0], 0, abort_flag);
@@ -841,13 +844,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       for (int i = 0; i < row_tiles; ++i) scores_of(i, 0);
       tc_commit(&bars->key_empty[0]);
     }
+    if (kWide && ok && tiles > 1) {  // S of a tile ahead
+      ok = mbar_wait(&bars->key_full[1], 0, abort_flag);
+      if (ok) {
+        tc_fence_after_sync();
+        scores_of(0, 1);
+        tc_commit(&bars->key_empty[1]);
+      }
+    }
     for (int j = 0; ok && j < tiles; ++j) {
       const int stage = j & 1, after = (j + 1) & 1;
       for (int i = 0; ok && i < row_tiles; ++i) {
         if (i == 0) ok = mbar_wait(&bars->value_full[stage], j >> 1 & 1, abort_flag);
         if (kWide) {
           if (ok && j >= 2) ok = mbar_wait(&bars->taken[j & 1], (j >> 1) - 1 & 1, abort_flag);
-          ok = ok && mbar_wait(&bars->weights[i], j & 1, abort_flag);
+          ok = ok && mbar_wait(&bars->weights[j & 1], j >> 1 & 1, abort_flag);
         } else {
           ok = ok && mbar_wait(&bars->halves[i], j & 1, abort_flag);
         }
@@ -862,15 +873,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
               if (!ok) break;
               tc_fence_after_sync();
             }
-            mma_f16_ts(tmem + 256 + (kWide ? j & 1 : i) * 128, tmem + i * 128 + half * (kKeys / 2) + t / 2,
+            mma_f16_ts(tmem + 256 + (kWide ? j & 1 : i) * 128, tmem + (kWide ? j & 1 : i) * 128 + half * (kKeys / 2) + t / 2,
                        make_sw128_nmajor_desc(base + S::kValueRing + stage * S::kOperand + t * 128, kKeys * 128), sums_desc,
                        t > 0 || (kWide ? half == 0 : j > 0));
           }
         }
         if (!ok) break;
-        if (kWide) tc_commit(&bars->sums[j & 1]);
+        if (kWide) {
+          tc_commit(&bars->sums[j & 1]);
+          continue;
+        }
         if (j + 1 == tiles) {
-          if (!kWide) tc_commit(&bars->sums[i]);
+          tc_commit(&bars->sums[i]);
           continue;
         }
         if (i == 0) ok = mbar_wait(&bars->key_full[after], (j + 1) >> 1 & 1, abort_flag);
@@ -880,7 +894,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       }
       if (!ok) break;
       tc_commit(&bars->value_empty[stage]);
-      if (j + 1 < tiles) tc_commit(&bars->key_empty[after]);
+      if (kWide) {
+        if (j + 2 >= tiles) continue;
+        ok = mbar_wait(&bars->key_full[stage], (j + 2) >> 1 & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after_sync();
+        scores_of(0, stage);
+        tc_commit(&bars->key_empty[stage]);
+      } else if (j + 1 < tiles) {
+        tc_commit(&bars->key_empty[after]);
+      }
     }
     if (!ok) {
       *abort_flag = 1;
