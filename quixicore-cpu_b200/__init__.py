@@ -689,6 +689,20 @@ def _pointer(a):
     return _np(a) if isinstance(a, np.ndarray) else _dev(a)
 
 
+_element_types = {name: {np.dtype(name)} for name in ("int8", "int32", "int64", "float32")}
+
+
+def _is(a, name):
+    """a, None or an array of that element type: the library sees only where it lies."""
+    if a is not None and a.dtype not in _element_types[name]:
+        if not isinstance(a, np.ndarray):
+            import torch
+            for each, types in _element_types.items():
+                types.add(getattr(torch, each))
+        assert a.dtype in _element_types[name], f"need {name}, not {a.dtype}"
+    return a
+
+
 class Rope:
     """Rotary positions (qx_rope): frequencies by base and an optional scaling for long contexts, a dict of
     kind (ROPE_LINEAR, ROPE_BANDS, ROPE_RAMP), factor and, for the last two, trained, slow and fast."""
@@ -703,12 +717,13 @@ class Rope:
 
     # numpy arrays
     def apply(self, x, y, positions, inverse=False, kind=None) -> int:
-        return lib.qx_rope_apply(self.view, heads_view(x, kind), heads_view(y, kind), _np(positions), x.shape[0],
+        return lib.qx_rope_apply(self.view, heads_view(x, kind), heads_view(y, kind),
+                                 _np(_is(positions, "int64")), x.shape[0],
                                  x.shape[2], 1 if inverse else 0)
 
     # device tensors, torch's current stream
     def apply_dev(self, x, y, positions, inverse=False) -> int:
-        return lib.qx_rope_apply_dev(self.view, heads_view(x), heads_view(y), _dev(positions), x.shape[0],
+        return lib.qx_rope_apply_dev(self.view, heads_view(x), heads_view(y), _dev(_is(positions, "int64")), x.shape[0],
                                      x.shape[2], 1 if inverse else 0, _stream())
 
 
@@ -720,6 +735,8 @@ class KVBatch:
     def __init__(self, lengths, block_table, max_length, token_begin=None, tokens=None, max_tokens=1):
         self.arrays = (lengths, block_table, token_begin)
         sequences = lengths.shape[0]
+        for array in self.arrays:
+            _is(array, "int32")
         self.view = KVBatchView(sequences, _pointer(token_begin), _pointer(lengths), _pointer(block_table),
                                 block_table.shape[1], sequences * max_tokens if tokens is None else tokens,
                                 max_tokens, max_length)
@@ -731,7 +748,9 @@ class KVCache:
 
     def __init__(self, k_codes, v_codes, k_scales, v_scales):
         self.arrays = (k_codes, v_codes, k_scales, v_scales)
-        blocks, heads, tokens, dim = k_codes.shape
+        blocks, heads, tokens, dim = shape = k_codes.shape
+        assert v_codes.shape == shape and k_scales.shape == v_scales.shape == shape[:2], "shapes differ"
+        assert v_codes.dtype == _is(k_codes, "int8").dtype and v_scales.dtype == _is(k_scales, "float32").dtype, "types differ"
         self.view = KVCacheView(_pointer(k_codes), _pointer(v_codes), _pointer(k_scales), _pointer(v_scales), blocks,
                                 heads, tokens, dim)
 
@@ -744,7 +763,7 @@ class KVCache:
     # numpy arrays
     def append(self, batch, k, v, rope=None, q=None, q_out=None, positions=None, kind=None) -> int:
         return lib.qx_kv_append(self.view, batch.view, heads_view(k, kind), heads_view(v, kind),
-                                None if rope is None else rope.view, _np(positions), heads_view(q, kind),
+                                None if rope is None else rope.view, _np(_is(positions, "int64")), heads_view(q, kind),
                                 heads_view(q_out, kind))
 
     def read(self, batch, k, v, kind=None) -> int:
@@ -752,13 +771,13 @@ class KVCache:
 
     def attention(self, batch, q, out, scale=None, causal=True, window=0, lse=None, kind=None) -> int:
         scale = self.view.head_dim ** -0.5 if scale is None else scale
-        return lib.qx_kv_attention(self.view, batch.view, heads_view(q, kind), heads_view(out, kind), _np(lse), scale,
+        return lib.qx_kv_attention(self.view, batch.view, heads_view(q, kind), heads_view(out, kind), _np(_is(lse, "float32")), scale,
                                    1 if causal else 0, window)
 
     # device tensors, torch's current stream
     def append_dev(self, batch, k, v, rope=None, q=None, q_out=None, positions=None) -> int:
         return lib.qx_kv_append_dev(self.view, batch.view, heads_view(k), heads_view(v),
-                                    None if rope is None else rope.view, _dev(positions), heads_view(q),
+                                    None if rope is None else rope.view, _dev(_is(positions, "int64")), heads_view(q),
                                     heads_view(q_out), _stream())
 
     def read_dev(self, batch, k, v) -> int:
@@ -766,5 +785,5 @@ class KVCache:
 
     def attention_dev(self, batch, q, out, scale=None, causal=True, window=0, lse=None, workspace=None) -> int:
         scale = self.view.head_dim ** -0.5 if scale is None else scale
-        return lib.qx_kv_attention_dev(self.view, batch.view, heads_view(q), heads_view(out), _dev(lse), scale,
+        return lib.qx_kv_attention_dev(self.view, batch.view, heads_view(q), heads_view(out), _dev(_is(lse, "float32")), scale,
                                        1 if causal else 0, window, workspace, _stream())

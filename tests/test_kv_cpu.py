@@ -304,3 +304,25 @@ def test_an_output_that_begins_where_the_queries_do_is_the_same_view(qx, parts):
     assert served(qx, call(H(q)))
     assert call(H(q, kind=qx.BF16)) == qx.INVALID_ARGUMENT
     assert call(H(q, token_stride=2 * q.shape[1] * q.shape[2])) == qx.INVALID_ARGUMENT
+
+
+def test_arrays_of_another_element_type_are_refused(qx, parts):
+    """The library sees addresses only; the Python calls look at what lies there."""
+    cache, batch, x, q = parts
+    lengths, table, begin = batch.arrays
+    for wrong in ((lengths.astype(np.int64), table, begin), (lengths, table.astype(np.int64), begin),
+                  (lengths, table, begin.astype(np.uint32))):
+        with pytest.raises(AssertionError):
+            qx.KVBatch(wrong[0], wrong[1], 32, wrong[2], 3, 2)
+    k_codes, v_codes, k_scales, v_scales = cache.arrays
+    for wrong in ((k_codes.view(np.uint8), v_codes, k_scales, v_scales), (k_codes, v_codes, k_scales, v_scales.astype(np.float64)),
+                  (k_codes, v_codes[:2], k_scales, v_scales), (k_codes, v_codes, k_scales, v_scales[:, :1])):
+        with pytest.raises(AssertionError):
+            qx.KVCache(*wrong)
+    rope, at = qx.Rope(32), np.arange(3, dtype=np.int32)
+    with pytest.raises(AssertionError):
+        rope.apply(x, x, at)
+    with pytest.raises(AssertionError):
+        cache.append(batch, x, x, rope, positions=at)
+    with pytest.raises(AssertionError):
+        cache.attention(batch, q, q, lse=np.zeros((3, q.shape[1])))
