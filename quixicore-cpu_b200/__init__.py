@@ -666,16 +666,19 @@ def _fill_torch_types() -> dict:
     return _torch_types
 
 
-def heads_view(t, kind=None, heads=None, token_stride=None, head_stride=None) -> HeadsView:
+def heads_view(t, kind=None, heads=None, token_stride=None, head_stride=None, device=None) -> HeadsView:
     """A qx_heads over a [tokens, heads, head_dim] tensor or numpy array (uint16 bits need `kind`); the
-    elements of a head lie side by side. The arguments behind `kind` replace what the array says."""
+    elements of a head lie side by side. The arguments behind `kind` replace what the array says; `device`: it has
+    to be a tensor there."""
     if t is None:
         return None
     shape = t.shape
     if isinstance(t, np.ndarray):
+        assert device is None, "need a tensor on the device"
         kind = {2: F16, 4: F32}[t.itemsize] if kind is None else kind
         data, (st, sh, sd) = t.ctypes.data, (s // t.itemsize for s in t.strides)
     else:
+        assert device is None or t.get_device() == device, "need a tensor on the current device"
         kind = (_torch_types or _fill_torch_types())[t.dtype] if kind is None else kind
         data, (st, sh, sd) = t.data_ptr(), t.stride()
     assert sd == 1 or shape[2] == 1, "the elements of a head lie side by side"
@@ -683,24 +686,40 @@ def heads_view(t, kind=None, heads=None, token_stride=None, head_stride=None) ->
                      sh if head_stride is None else head_stride)
 
 
-def _pointer(a):
+_element_types: dict = {}
+
+
+def _fill_element_types() -> dict:
+    import torch
+    _element_types.update({name: getattr(torch, name) for name in ("int8", "int32", "int64", "float32")})
+    return _element_types
+
+
+def _array(a, name, device):
+    """The address of an array of that element type (the library sees nothing else of it): a contiguous tensor on
+    `device`, or a numpy array where that is None."""
     if a is None:
         return None
-    return _np(a) if isinstance(a, np.ndarray) else _dev(a)
+    if device is None:
+        assert isinstance(a, np.ndarray) and a.dtype == name, f"need a numpy array of {name}"
+        return _np(a)
+    # (numpy's element types are none of torch's)
+    assert (a.dtype is (_element_types or _fill_element_types())[name] and a.get_device() == device >= 0 and
+            a.is_contiguous()), f"need a contiguous tensor of {name} on the device"
+    return a.data_ptr()
 
 
-_element_types = {name: {np.dtype(name)} for name in ("int8", "int32", "int64", "float32")}
+def _device() -> int:
+    """The current device: a call's kernels run there, on its current stream."""
+    global _raw_device
+    if _raw_device is None:
+        import torch
+        torch.cuda.current_device()  # (initialises CUDA)
+        _raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    return _raw_device()
 
 
-def _is(a, name):
-    """a, None or an array of that element type: the library sees only where it lies."""
-    if a is not None and a.dtype not in _element_types[name]:
-        if not isinstance(a, np.ndarray):
-            import torch
-            for each, types in _element_types.items():
-                types.add(getattr(torch, each))
-        assert a.dtype in _element_types[name], f"need {name}, not {a.dtype}"
-    return a
+_raw_device = None
 
 
 class Rope:
@@ -718,13 +737,15 @@ class Rope:
     # numpy arrays
     def apply(self, x, y, positions, inverse=False, kind=None) -> int:
         return lib.qx_rope_apply(self.view, heads_view(x, kind), heads_view(y, kind),
-                                 _np(_is(positions, "int64")), x.shape[0],
+                                 _array(positions, "int64", None), x.shape[0],
                                  x.shape[2], 1 if inverse else 0)
 
     # device tensors, torch's current stream
     def apply_dev(self, x, y, positions, inverse=False) -> int:
-        return lib.qx_rope_apply_dev(self.view, heads_view(x), heads_view(y), _dev(_is(positions, "int64")), x.shape[0],
-                                     x.shape[2], 1 if inverse else 0, _stream())
+        device = _device()
+        return lib.qx_rope_apply_dev(self.view, heads_view(x, device=device), heads_view(y, device=device),
+                                     _array(positions, "int64", device), x.shape[0], x.shape[2],
+                                     1 if inverse else 0, _stream())
 
 
 class KVBatch:
@@ -735,9 +756,9 @@ class KVBatch:
     def __init__(self, lengths, block_table, max_length, token_begin=None, tokens=None, max_tokens=1):
         self.arrays = (lengths, block_table, token_begin)
         sequences = lengths.shape[0]
-        for array in self.arrays:
-            _is(array, "int32")
-        self.view = KVBatchView(sequences, _pointer(token_begin), _pointer(lengths), _pointer(block_table),
+        self.device = device = None if isinstance(lengths, np.ndarray) else lengths.get_device()
+        self.view = KVBatchView(sequences, _array(token_begin, "int32", device), _array(lengths, "int32", device),
+                                _array(block_table, "int32", device),
                                 block_table.shape[1], sequences * max_tokens if tokens is None else tokens,
                                 max_tokens, max_length)
 
@@ -749,10 +770,11 @@ class KVCache:
     def __init__(self, k_codes, v_codes, k_scales, v_scales):
         self.arrays = (k_codes, v_codes, k_scales, v_scales)
         blocks, heads, tokens, dim = shape = k_codes.shape
-        assert v_codes.shape == shape and k_scales.shape == v_scales.shape == shape[:2], "shapes differ"
-        assert v_codes.dtype == _is(k_codes, "int8").dtype and v_scales.dtype == _is(k_scales, "float32").dtype, "types differ"
-        self.view = KVCacheView(_pointer(k_codes), _pointer(v_codes), _pointer(k_scales), _pointer(v_scales), blocks,
-                                heads, tokens, dim)
+        assert v_codes.shape == shape and k_scales.shape == v_scales.shape == (blocks, heads), "shapes differ"
+        self.device = device = None if isinstance(k_codes, np.ndarray) else k_codes.get_device()
+        self.view = KVCacheView(_array(k_codes, "int8", device), _array(v_codes, "int8", device),
+                                _array(k_scales, "float32", device), _array(v_scales, "float32", device), blocks, heads,
+                                tokens, dim)
 
     @classmethod
     def empty(cls, blocks, kv_heads, block_tokens, head_dim, device="cuda"):
@@ -762,28 +784,39 @@ class KVCache:
 
     # numpy arrays
     def append(self, batch, k, v, rope=None, q=None, q_out=None, positions=None, kind=None) -> int:
+        assert self.device is None and batch.device is None, "need numpy arrays"
         return lib.qx_kv_append(self.view, batch.view, heads_view(k, kind), heads_view(v, kind),
-                                None if rope is None else rope.view, _np(_is(positions, "int64")), heads_view(q, kind),
+                                None if rope is None else rope.view, _array(positions, "int64", None), heads_view(q, kind),
                                 heads_view(q_out, kind))
 
     def read(self, batch, k, v, kind=None) -> int:
+        assert self.device is None and batch.device is None, "need numpy arrays"
         return lib.qx_kv_read(self.view, batch.view, heads_view(k, kind), heads_view(v, kind))
 
     def attention(self, batch, q, out, scale=None, causal=True, window=0, lse=None, kind=None) -> int:
         scale = self.view.head_dim ** -0.5 if scale is None else scale
-        return lib.qx_kv_attention(self.view, batch.view, heads_view(q, kind), heads_view(out, kind), _np(_is(lse, "float32")), scale,
-                                   1 if causal else 0, window)
+        assert self.device is None and batch.device is None, "need numpy arrays"
+        return lib.qx_kv_attention(self.view, batch.view, heads_view(q, kind), heads_view(out, kind),
+                                   _array(lse, "float32", None), scale, 1 if causal else 0, window)
 
     # device tensors, torch's current stream
     def append_dev(self, batch, k, v, rope=None, q=None, q_out=None, positions=None) -> int:
-        return lib.qx_kv_append_dev(self.view, batch.view, heads_view(k), heads_view(v),
-                                    None if rope is None else rope.view, _dev(_is(positions, "int64")), heads_view(q),
-                                    heads_view(q_out), _stream())
+        device = _device()
+        assert self.device == device == batch.device, "need tensors on the current device"
+        return lib.qx_kv_append_dev(self.view, batch.view, heads_view(k, device=device), heads_view(v, device=device),
+                                    None if rope is None else rope.view, _array(positions, "int64", device),
+                                    heads_view(q, device=device), heads_view(q_out, device=device), _stream())
 
     def read_dev(self, batch, k, v) -> int:
-        return lib.qx_kv_read_dev(self.view, batch.view, heads_view(k), heads_view(v), _stream())
+        device = _device()
+        assert self.device == device == batch.device, "need tensors on the current device"
+        return lib.qx_kv_read_dev(self.view, batch.view, heads_view(k, device=device), heads_view(v, device=device),
+                                  _stream())
 
     def attention_dev(self, batch, q, out, scale=None, causal=True, window=0, lse=None, workspace=None) -> int:
         scale = self.view.head_dim ** -0.5 if scale is None else scale
-        return lib.qx_kv_attention_dev(self.view, batch.view, heads_view(q), heads_view(out), _dev(_is(lse, "float32")), scale,
-                                       1 if causal else 0, window, workspace, _stream())
+        device = _device()
+        assert self.device == device == batch.device, "need tensors on the current device"
+        return lib.qx_kv_attention_dev(self.view, batch.view, heads_view(q, device=device), heads_view(out, device=device),
+                                       _array(lse, "float32", device), scale, 1 if causal else 0, window, workspace,
+                                       _stream())

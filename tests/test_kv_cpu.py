@@ -6,6 +6,7 @@ import math
 
 import numpy as np
 import pytest
+import torch
 
 
 def cache_arrays(blocks=4, heads=2, size=16, dim=32):
@@ -326,3 +327,24 @@ def test_arrays_of_another_element_type_are_refused(qx, parts):
         cache.append(batch, x, x, rope, positions=at)
     with pytest.raises(AssertionError):
         cache.attention(batch, q, q, lse=np.zeros((3, q.shape[1])))
+
+
+def test_arrays_in_another_place_are_refused(qx, parts, monkeypatch):
+    """Host arrays never reach a `_dev` call, nor tensors of another device: the kernel would follow their addresses."""
+    cache, batch, x, q = parts
+    at = np.arange(3)
+    monkeypatch.setattr(qx, "_device", lambda: 0)
+    for call in (lambda: qx.Rope(32).apply_dev(x, x, at), lambda: cache.append_dev(batch, x, x),
+                 lambda: cache.read_dev(batch, x, x), lambda: cache.attention_dev(batch, q, q)):
+        with pytest.raises(AssertionError):
+            call()
+    elsewhere = qx.KVBatch(*batch.arrays[:2], 32, batch.arrays[2], 3, 2)
+    elsewhere.device = 1  # (as if its tensors lay there)
+    for call in (lambda: cache.append(elsewhere, x, x), lambda: cache.read(elsewhere, x, x),
+                 lambda: cache.attention(elsewhere, q, q)):
+        with pytest.raises(AssertionError):
+            call()
+    with pytest.raises(AssertionError):
+        qx.heads_view(torch.zeros(3, 2, 32), device=0)  # (a tensor of the host)
+    with pytest.raises(AssertionError):
+        qx.KVBatch(batch.arrays[0], torch.from_numpy(batch.arrays[1]), 32, batch.arrays[2], 3, 2)
