@@ -584,7 +584,8 @@ QX_API qx_status qx_import_gptq_u4(const qx_gptq_u4_source* source, qx_canonical
  * A view of `heads` vectors of head_dim elements for every token: element d of head h of token t is at
  * data[t * token_stride + h * head_stride + d]. Strides count elements, so slices of a packed
  * [token][q, k and v heads][head_dim] projection are views like any other. `type` is QX_STORAGE_*.
- * Views that are read may have strides of zero; written ones may not overlap themselves. */
+ * Views that are read may have strides of zero; written ones may not overlap themselves. What lies between
+ * the elements of a written view stays as it is, other written views of the same call among it. */
 typedef struct qx_heads {
   void* data;
   int type;

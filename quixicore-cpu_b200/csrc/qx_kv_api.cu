@@ -3,6 +3,7 @@
 // names travel to the device packed together, the kernels are those of the device forms.
 
 #include <algorithm>
+#include <cstring>
 #include <new>
 #include <stdexcept>
 #include <vector>
@@ -28,13 +29,30 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
 
 namespace {
 
-// Host arrays that a call uses, laid out one behind the other in the context's staging memory.
+// Where the elements of a view lie in memory: `rows` x `heads` runs of `bytes`, strides in bytes.
+struct Runs {
+  long long rows, heads;
+  size_t row_stride, head_stride, bytes;
+  size_t extent() const {
+    return rows <= 0 ? 0 : (rows - 1) * row_stride + (heads - 1) * head_stride + bytes;
+  }
+  bool gapless() const { return extent() == static_cast<size_t>(rows) * heads * bytes; }
+};
+Runs runs_of(const qx_heads* view, long long rows, int dim) {
+  const size_t size = type_bytes(view->type);
+  return {rows, view->heads, view->token_stride * size, view->head_stride * size, dim * size};
+}
+
+// Host arrays that a call uses, laid out one behind the other in the context's staging memory. What comes back is
+// the elements of the views that are written, run by run: between them may lie another view's, or what is none of
+// the call's business.
 class Arrays {
  public:
   // Returns the array's number. `out`: it is copied back.
-  int add(const void* host, size_t bytes, bool out) {
-    items_.push_back({const_cast<void*>(host), bytes, total_, out});
-    total_ += align_up(std::max<size_t>(bytes, 1), 256);
+  int add(const void* host, size_t bytes, bool out) { return add(host, Runs{1, 1, 0, 0, bytes}, out); }
+  int add(const void* host, const Runs& runs, bool out) {
+    items_.push_back({const_cast<void*>(host), runs, runs.extent(), total_, out, {}});
+    total_ += align_up(std::max<size_t>(items_.back().bytes, 1), 256);
     return static_cast<int>(items_.size()) - 1;
   }
   qx_status to_device(DeviceContext* ctx) {
@@ -46,10 +64,26 @@ class Arrays {
     }
     return QX_STATUS_OK;
   }
-  qx_status from_device() const {
-    for (const Item& i : items_) {
+  // Waits for the stream, and for what the kernels reported.
+  qx_status from_device() {
+    for (Item& i : items_) {
       if (!i.out || i.bytes == 0) continue;
-      QX_CUDA_TRY(cudaMemcpyAsync(i.host, at(i), i.bytes, cudaMemcpyDeviceToHost, ctx_->stream));
+      void* to = i.host;
+      if (!i.runs.gapless()) {
+        i.back.resize(i.bytes);
+        to = i.back.data();
+      }
+      QX_CUDA_TRY(cudaMemcpyAsync(to, at(i), i.bytes, cudaMemcpyDeviceToHost, ctx_->stream));
+    }
+    QX_TRY(finish_host_call(ctx_));
+    for (const Item& i : items_) {
+      if (i.back.empty()) continue;
+      for (long long r = 0; r < i.runs.rows; ++r) {
+        for (long long h = 0; h < i.runs.heads; ++h) {
+          const size_t offset = r * i.runs.row_stride + h * i.runs.head_stride;
+          std::memcpy(static_cast<uint8_t*>(i.host) + offset, i.back.data() + offset, i.runs.bytes);
+        }
+      }
     }
     return QX_STATUS_OK;
   }
@@ -61,8 +95,10 @@ class Arrays {
  private:
   struct Item {
     void* host;
+    Runs runs;
     size_t bytes, offset;
     bool out;
+    std::vector<uint8_t> back;
   };
   uint8_t* at(const Item& i) const { return static_cast<uint8_t*>(ctx_->staging) + i.offset; }
   std::vector<Item> items_;
@@ -70,14 +106,8 @@ class Arrays {
   DeviceContext* ctx_ = nullptr;
 };
 
-// The extent of a view in memory. What lies between its elements travels both ways and stays as it is.
-size_t extent(const qx_heads* view, long long rows, int dim) {
-  if (view == nullptr || rows <= 0) return 0;
-  return static_cast<size_t>((rows - 1) * view->token_stride + (view->heads - 1) * view->head_stride + dim) *
-         type_bytes(view->type);
-}
 int add_view(Arrays* a, const qx_heads* view, long long rows, int dim, bool out) {
-  return view == nullptr ? -1 : a->add(view->data, extent(view, rows, dim), out);
+  return view == nullptr ? -1 : a->add(view->data, runs_of(view, rows, dim), out);
 }
 qx_heads on_device(const Arrays& a, const qx_heads* view, int number) {
   qx_heads v = *view;
@@ -236,8 +266,7 @@ qx_status qx_rope_apply(const qx_rope* rope, const qx_heads* x, const qx_heads* 
     QX_TRY(a.to_device(ctx));
     const qx_heads dx = on_device(a, x, from), dy = on_device(a, y, to);
     QX_TRY(qx_rope_apply_dev(rope, &dx, &dy, a.device<int64_t>(at), tokens, head_dim, inverse, ctx->stream));
-    QX_TRY(a.from_device());
-    return finish_host_call(ctx);
+    return a.from_device();
   });
 }
 
@@ -271,7 +300,6 @@ qx_status qx_kv_append(const qx_kv_cache* cache, const qx_kv_batch* batch, const
     QX_TRY(launch_append(&dc, &db, &dk, &dv, rope, a.device<int64_t>(at), q == nullptr ? nullptr : &dq,
                          q == nullptr ? nullptr : &dout, ctx, ctx->stream));
     QX_TRY(a.from_device());
-    QX_TRY(finish_host_call(ctx));
     unpack(cache, p);
     return QX_STATUS_OK;
   });
@@ -297,8 +325,7 @@ qx_status qx_kv_read(const qx_kv_cache* cache, const qx_kv_batch* batch, const q
     if (k != nullptr) dk = on_device(a, k, ak);
     if (v != nullptr) dv = on_device(a, v, av);
     QX_TRY(launch_read(&dc, &db, k == nullptr ? nullptr : &dk, v == nullptr ? nullptr : &dv, ctx, ctx->stream));
-    QX_TRY(a.from_device());
-    return finish_host_call(ctx);
+    return a.from_device();
   });
 }
 
@@ -323,8 +350,7 @@ qx_status qx_kv_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, co
     const qx_heads dq = on_device(a, q, aq), dout = on_device(a, out, ao);
     QX_TRY(launch_attention(&dc, &db, &dq, &dout, a.device<float>(al), scale, causal, window, ctx, &ctx->workspace,
                             ctx->stream));
-    QX_TRY(a.from_device());
-    return finish_host_call(ctx);
+    return a.from_device();
   });
 }
 
