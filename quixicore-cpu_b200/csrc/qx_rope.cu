@@ -50,7 +50,8 @@ __device__ __forceinline__ float2 turn_of(const RopeParams& p, const Span& span,
 
 constexpr int kRopeThreads = 256;
 
-// Whole units of 16 elements: head size and rotary part are multiples of 16, runs start on 16-byte boundaries.
+// Whole units of 16 elements: head size and rotary part are multiples of 16, runs start on 16-byte boundaries, a head
+// has no more units than the CTA threads.
 template <int kType, bool kBatch>
 __global__ void __launch_bounds__(kRopeThreads, 3) rope_units_kernel(const __grid_constant__ RopeParams p) {
   extern __shared__ __align__(16) float2 table[];
@@ -108,7 +109,8 @@ __global__ void __launch_bounds__(kRopeThreads, 3) rope_units_kernel(const __gri
   }
 }
 
-// Any head size and any even rotary part: one pair, or one element behind them, at a time.
+// Any head size and any even rotary part (heads of more than 4096 elements among them): one pair, or one element
+// behind them, at a time.
 template <bool kBatch>
 __global__ void __launch_bounds__(kRopeThreads) rope_pairs_kernel(const __grid_constant__ RopeParams p) {
   extern __shared__ __align__(16) float2 table[];
@@ -202,7 +204,9 @@ qx_status launch_rope(RopeParams& p, const qx_rope* rope, const qx_heads* x, con
   p.dim = dim;
   p.in_place = x->data == y->data;
   p.rotation = device_rotation(rope, inverse);
-  const bool whole = dim % 16 == 0 && rope->rotary_dim % 16 == 0 && p.x.vector && p.y.vector;
+  // (a row of units takes a thread each; in place only the rotated ones, which are 16 at most)
+  const bool whole = dim % 16 == 0 && rope->rotary_dim % 16 == 0 && p.x.vector && p.y.vector &&
+                     (p.in_place || dim / 16 <= kRopeThreads);
   // Tokens per CTA: enough for four rounds of its threads where there are CTAs for every SM all the same,
   // and no more than 16 KB of {cos, sin}.
   const long long per_token = static_cast<long long>(x->heads) * (whole ? dim / 16 : dim);
