@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     const float inverse = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
     if (threadIdx.x == 0) *scale_at = number ? scale : __uint_as_float(0x7FC00000u);
     int8_t* const codes = p.codes[kind] + (block * p.kv_heads + head) * p.block_tokens * p.dim;
-    if (number && scale > before && before > 0.0f) {
+    if (number && scale > before) {  // (beside a scale of zero all codes stand for zeros, whatever they are)
       const float ratio = before * inverse;
       for (int i = threadIdx.x; i < kept * units; i += kThreads) {
         uint4* const words = reinterpret_cast<uint4*>(codes) + i;
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
           int c[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            c[e] = regrown(static_cast<int8_t>(w[k] >> (8 * e)), before, scale, ratio);
+            c[e] = before > 0.0f ? regrown(static_cast<int8_t>(w[k] >> (8 * e)), before, scale, ratio) : 0;
           }
           w[k] = pack4(c[0], c[1], c[2], c[3]);
         }
