@@ -8,7 +8,10 @@
 //           1.5 * 2^23 as f32 bits, so that a subtraction makes f32 numbers of them;
 //   output  [head elements x rows]: the codes as f16 (exact) against the weights as f16 (a rounding of 2^-11
 //           relative, no further than the 16-bit outputs' own), as hi + lo pairs for f32 queries; f32 sums.
-// The scales are applied to the sums: one multiplication per score (ks), one per 32 keys and output element (vs).
+// The scales are applied to the sums: one multiplication per score (ks), one per 16 keys and output element (vs): a
+// block of 16 keeps its own, however much larger its neighbour's is (blocks of 64 | 16 tokens, 32 sessions of up to 8192
+// 64.6 | 67.2 us; one multiplication per 32 keys and the ratio of two blocks' scales in their weights, which loses those
+// below 2^-26: 63.7 | 69.9, drafts 23.6 against 22.5).
 //
 // Split. A CTA takes 8 rows (16 where there are more) and a run of the keys; its four warps take tiles of 32
 // keys in turn, each with a running maximum and sum of its own, and are joined at the end through shared
@@ -27,10 +30,10 @@
 // groups so that these reads meet no conflicts for head sizes up to 128.
 //
 // Bound by HBM for long contexts: 2 * head_dim bytes per key and kv head, whatever the group. Measured (128 elements, 8
-// kv heads): 32 sessions of up to 8192 tokens, 32 query heads, 64 us (314 MB, 4.9 TB/s, 0.75 of the copy bandwidth);
+// kv heads): 32 sessions of up to 8192 tokens, 32 query heads, 64.6 us (314 MB, 4.9 TB/s, 0.75 of the copy bandwidth);
 // one of 131072 tokens, 64 query heads, 54 us (5.0 TB/s); one of 1000 tokens, f32, 7.7 us. What is above the bytes' time
 // is a CTA's way in and out: about 9000 cycles before its first tile (cold instructions, length, table, queries) and
-// 4000 behind its last. With 64 elements and 15 rows (drafts) the instructions bind: 32 sessions, windows of 4096, 59 us
+// 4000 behind its last. With 64 elements and 15 rows (drafts) the instructions bind: 32 sessions, windows of 4096, 55 us
 // for 134 MB, issue slots 54 % taken.
 
 #include <algorithm>
@@ -504,36 +507,30 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
     }
 
     // ---- softmax --------------------------------------------------------------------------
-    // One scale for the tile's values: the larger of its two blocks', the weights take the ratio. (Beside a scale
-    // that is no number the larger is the other; with that at zero, any does.) A weight of zero that a mask has
-    // made stays zero beside a scale that is no number.
-    float scale = vs[0], ratio[2] = {1.0f, 1.0f};
-    if (p.block_tokens < kTile) {
-      scale = fmaxf(vs[0], vs[1]);
-      if (!(scale > 0.0f)) scale = 1.0f;
-      ratio[0] = vs[0] / scale;
-      ratio[1] = vs[1] / scale;
-    }
-    float gain[kRowTiles][2];
+    // The scale of a half's values for a row: zero where the row sees none of them, so that a scale that is no number
+    // meets weights of zero nowhere.
+    float gain[kRowTiles][2][2];
 #pragma unroll
-    for (int n = 0; n < kRowTiles; ++n) gain[n][0] = gain[n][1] = scale;
+    for (int n = 0; n < kRowTiles; ++n) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) gain[n][k][0] = gain[n][k][1] = vs[k];
+    }
     if (!open) {
 #pragma unroll
       for (int n = 0; n < kRowTiles; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          bool sees = false;  // whether the row sees any key of the tile
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const int first = token0 + 16 * k;
-            if ((present >> k & 1) && low[n][e] < first + 16 && high[n][e] > max(first, low[n][e])) sees = true;
+            const bool sees = (present >> k & 1) && low[n][e] < first + 16 && high[n][e] > max(first, low[n][e]);
+            if (!sees) gain[n][k][e] = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int key = first + 8 * h + g;
               if (!(present >> k & 1) || key < low[n][e] || key >= high[n][e]) score[n][k][2 * h + e] = -INFINITY;
             }
           }
-          if (!sees) gain[n][e] = 0.0f;
         }
       }
       __syncwarp();  // (a branch, not predicates: most tiles skip this)
@@ -565,23 +562,6 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
           }
         }
         sum[n][e] = fmaf(sum[n][e], keep[n][e], total);
-      }
-      if (ratio[0] != ratio[1]) {  // (also where one is no number)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (ratio[k] < INFINITY) {
-#pragma unroll
-            for (int h = 0; h < 4; ++h) score[n][k][h] *= ratio[k];
-          } else {  // (hidden weights stay zero)
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              const int key = token0 + 16 * k + 8 * (h >> 1) + g;
-              const bool hidden = !open && (!(present >> k & 1) || key < low[n][h & 1] || key >= high[n][h & 1]);
-              score[n][k][h] = hidden ? 0.0f : score[n][k][h] * ratio[k];
-            }
-          }
-        }
-        __syncwarp();
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -637,18 +617,17 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
           }
 #pragma unroll
           for (int n = 0; n < kRowTiles; ++n) {
-            float acc[4];
-            mma_f16_first(acc, a[0], weight[n][0], weight[n][1]);
-            mma_f16(acc, a[1], weight[n][2], weight[n][3]);
-            if (kWide) {
-              mma_f16(acc, a[0], low_weight[n][0], low_weight[n][1]);
-              mma_f16(acc, a[1], low_weight[n][2], low_weight[n][3]);
-            }
             float (&out)[4] = o[n][4 * i + 2 * word + h];
-            out[0] = fmaf(acc[0], gain[n][0], out[0]);
-            out[1] = fmaf(acc[1], gain[n][1], out[1]);
-            out[2] = fmaf(acc[2], gain[n][0], out[2]);
-            out[3] = fmaf(acc[3], gain[n][1], out[3]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float acc[4];
+              mma_f16_first(acc, a[k], weight[n][2 * k], weight[n][2 * k + 1]);
+              if (kWide) mma_f16(acc, a[k], low_weight[n][2 * k], low_weight[n][2 * k + 1]);
+              out[0] = fmaf(acc[0], gain[n][k][0], out[0]);
+              out[1] = fmaf(acc[1], gain[n][k][1], out[1]);
+              out[2] = fmaf(acc[2], gain[n][k][0], out[2]);
+              out[3] = fmaf(acc[3], gain[n][k][1], out[3]);
+            }
           }
         }
       }

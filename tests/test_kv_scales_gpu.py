@@ -1,13 +1,13 @@
 """Block scales at the ends of their range, in a cache that somebody else filled too: zero and tiny ones beside codes
-that are not zero."""
+that are not zero, neighbours far apart, masks that hide the larger one."""
 
 import numpy as np
 import pytest
 import torch
 
-from kv_reference import Cache
-from test_kv_attention_gpu import BF16, F32
-from test_kv_cache_gpu import append_both, on_device, table_of, typed
+from kv_reference import Cache, attention, attention_tolerance
+from test_kv_attention_gpu import BF16, F16, F32, filled
+from test_kv_cache_gpu import append_both, batch_of, on_device, table_of, typed
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,76 @@ def test_append_beside_codes_without_a_scale(qx, dtype, size, before, spread):
         block, kept = table[s, (t - 1) // size], (t - 1) % size + 1
         for got, want in same_codes:
             assert np.array_equal(got[block, :, :kept], want[block, :, :kept])
+
+
+def compare(qx, cache, table, lengths, new, q, window=0, missing=None):
+    """Causal attention with an f32 output (values of any magnitude fit) and its lse, row by row; `missing`: keys without
+    a weight in any precision."""
+    heads, dim = q.shape[1:]
+    batch, begin, rows = batch_of(qx, table, lengths, new)
+    out, lse = torch.full((rows, heads, dim), 3.0, device="cuda"), torch.full((rows, heads), 3.0, device="cuda")
+    assert on_device(qx, cache).attention_dev(batch, q.cuda(), out, window=window, lse=lse) == qx.OK, qx.last_error()
+    for s, (t, n) in enumerate(zip(lengths, new)):
+        at = slice(int(begin[s]), int(begin[s]) + n)
+        k, v = (torch.from_numpy(cache.values(i, table[s], t)) for i in range(2))
+        want, sums, magnitude, _ = attention(q[at].double(), k, v, dim ** -0.5, True, window, missing or ())
+        if missing:
+            k[list(missing)] = 0  # (their products are no part of the others' scores)
+        *_, spread = attention(q[at].double(), k, v, dim ** -0.5, True, window)
+        limit, lse_limit = attention_tolerance(want, sums, magnitude, spread, q.dtype, dim, t)
+        off, lse_off = (out[at].cpu().double() - want).abs() / limit, (lse[at].cpu().double() - sums).abs() / lse_limit
+        assert float(off.max()) <= 1 and float(lse_off.max()) <= 1, (s, float(off.max()), float(lse_off.max()))
+
+
+SHAPES = pytest.mark.parametrize("dim,group,new", [(64, 1, 1), (128, 4, 1), (64, 3, 5), (256, 2, 3), (96, 5, 2)])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@SHAPES
+@pytest.mark.parametrize("factor", [2.0 ** 20, 2.0 ** 45])
+@pytest.mark.parametrize("where", ["in front of the window", "behind the mask"])
+def test_a_hidden_block_leaves_its_neighbour_its_bits(qx, dtype, dim, group, new, factor, where):
+    """Two blocks of 16 share a tile of keys, and a mask hides the one with the larger scale: the tolerance goes by what
+    a row sees."""
+    size = 16
+    cache, table = filled(30, 2, size, dim), table_of(3, 10, 30)
+    if where == "in front of the window":  # the rows stand at the ends of blocks 3, 5 and 7
+        lengths, window = [6 * size, 4 * size, 8 * size], 8
+        for row in table:
+            cache.scales[1][row[0::2]] *= np.float32(factor)
+    else:  # only the last row sees the first token of the last block
+        lengths, window = [5 * size + 1, 3 * size + 1, 7 * size + 1], 0
+        for row, t in zip(table, lengths):
+            cache.scales[1][row[t // size]] *= np.float32(factor)
+    q = typed((3 * new, 2 * group, dim), dtype, 4)
+    compare(qx, cache, table, lengths, [new] * 3, q, window)
+    compare(qx, cache, table[:1], lengths[:1], [new], q[:new], window)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@SHAPES
+def test_a_block_that_weighs_nothing_leaves_its_neighbour_its_bits(qx, dtype, dim, group, new):
+    """The louder of two blocks of 16 in a tile is seen, with scores so far below the others' that its weights are zero in
+    any precision: what is left is attention without it."""
+    size, n = 16, 90
+    cache, table = filled(6, 1, size, dim), table_of(1, 6, 6)
+    q = typed((new, group, dim), dtype, 4).abs() + 1
+    quiet = table[0, 2]
+    cache.codes[0][quiet], cache.scales[0][quiet] = -127, 2000.0 / dim / dim ** -0.5 / 127  # scores of -2000 and below
+    cache.scales[1][quiet] *= np.float32(2.0 ** 40)
+    k = torch.from_numpy(cache.values(0, table[0], n))
+    scores = dim ** -0.5 * (q.double().transpose(0, 1) @ k[:, 0].T)
+    assert float((scores[..., 2 * size:3 * size].amax(-1) - scores[..., :2 * size].amax(-1)).max()) < -700  # (of e)
+    compare(qx, cache, table, [n], [new], q, missing=range(2 * size, 3 * size))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@SHAPES
+@pytest.mark.parametrize("length", [16, 17, 90])
+def test_values_of_two_blocks_without_a_scale_are_zeros(qx, dtype, dim, group, new, length):
+    cache, table = filled(6, 1, 16, dim), table_of(1, 6, 6)
+    cache.scales[1][:] = 0.0
+    batch, _, _ = batch_of(qx, table, [length], [new])
+    out = torch.full((new, group, dim), 3.0, device="cuda")
+    assert on_device(qx, cache).attention_dev(batch, typed((new, group, dim), dtype, 3).cuda(), out) == qx.OK
+    assert bool((out == 0).all())
