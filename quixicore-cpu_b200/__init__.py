@@ -686,6 +686,28 @@ def heads_view(t, kind=None, heads=None, token_stride=None, head_stride=None, de
                      sh if head_stride is None else head_stride)
 
 
+def _rows(t, tokens, dim, kind) -> HeadsView:
+    """heads_view of a numpy operand of a call over `tokens` rows of heads of `dim` elements: the library gets no sizes
+    and would follow a smaller array past its end."""
+    if t is None:
+        return None
+    rows, _, elements = t.shape
+    assert rows >= tokens and elements == dim, "need [tokens, heads, head_dim] of the call's tokens and head size"
+    assert kind is None or t.itemsize == (4 if kind == F32 else 2), "elements of another size than their type's"
+    return heads_view(t, kind)
+
+
+def _device_rows(t, tokens, dim, device) -> HeadsView:
+    """The same of a tensor on `device`, all at once: a call of few tokens takes the host longer than the GPU."""
+    if t is None:
+        return None
+    assert not isinstance(t, np.ndarray), "need a tensor on the device"
+    (rows, heads, elements), (token_stride, head_stride, stride) = t.shape, t.stride()
+    assert (rows >= tokens and elements == dim and stride == 1 and t.get_device() == device
+            ), "need [tokens, heads, head_dim] of the call's tokens and head size, on the current device"
+    return HeadsView(t.data_ptr(), (_torch_types or _fill_torch_types())[t.dtype], heads, token_stride, head_stride)
+
+
 _element_types: dict = {}
 
 
@@ -695,11 +717,15 @@ def _fill_element_types() -> dict:
     return _element_types
 
 
-def _array(a, name, device):
+def _array(a, name, device, least=0, width=None):
     """The address of an array of that element type (the library sees nothing else of it): a contiguous tensor on
-    `device`, or a numpy array where that is None."""
+    `device`, or a numpy array where that is None. `least`: of so many rows, one behind the other, or more; `width`: of
+    their elements, where there are several."""
     if a is None:
         return None
+    if least:
+        shape = a.shape
+        assert shape[0] >= least and shape[1:] == (() if width is None else (width,)), "an array of another shape than the call's"
     if device is None:
         assert isinstance(a, np.ndarray) and a.dtype == name, f"need a numpy array of {name}"
         return _np(a)
@@ -736,16 +762,18 @@ class Rope:
 
     # numpy arrays
     def apply(self, x, y, positions, inverse=False, kind=None) -> int:
-        return lib.qx_rope_apply(self.view, heads_view(x, kind), heads_view(y, kind),
-                                 _array(positions, "int64", None), x.shape[0],
-                                 x.shape[2], 1 if inverse else 0)
+        tokens, _, dim = x.shape
+        assert x.shape == y.shape, "x and y differ in shape"
+        return lib.qx_rope_apply(self.view, _rows(x, tokens, dim, kind), _rows(y, tokens, dim, kind),
+                                 _array(positions, "int64", None, tokens), tokens, dim, 1 if inverse else 0)
 
     # device tensors, torch's current stream
     def apply_dev(self, x, y, positions, inverse=False) -> int:
         device = _device()
-        return lib.qx_rope_apply_dev(self.view, heads_view(x, device=device), heads_view(y, device=device),
-                                     _array(positions, "int64", device), x.shape[0], x.shape[2],
-                                     1 if inverse else 0, _stream())
+        tokens, _, dim = x.shape
+        assert x.shape == y.shape, "x and y differ in shape"
+        return lib.qx_rope_apply_dev(self.view, _device_rows(x, tokens, dim, device), _device_rows(y, tokens, dim, device),
+                                     _array(positions, "int64", device, tokens), tokens, dim, 1 if inverse else 0, _stream())
 
 
 class KVBatch:
@@ -755,11 +783,14 @@ class KVBatch:
 
     def __init__(self, lengths, block_table, max_length, token_begin=None, tokens=None, max_tokens=1):
         self.arrays = (lengths, block_table, token_begin)
-        sequences = lengths.shape[0]
+        shape, table = lengths.shape, block_table.shape
+        sequences = shape[0]
+        assert len(shape) == 1 and len(table) == 2 and table[0] >= sequences, "need lengths [sequences], block_table [sequences, width]"
+        assert token_begin is None or token_begin.shape[0] > sequences, "need token_begin [sequences + 1]"
         self.device = device = None if isinstance(lengths, np.ndarray) else lengths.get_device()
         self.view = KVBatchView(sequences, _array(token_begin, "int32", device), _array(lengths, "int32", device),
                                 _array(block_table, "int32", device),
-                                block_table.shape[1], sequences * max_tokens if tokens is None else tokens,
+                                table[1], sequences * max_tokens if tokens is None else tokens,
                                 max_tokens, max_length)
 
 
@@ -785,38 +816,45 @@ class KVCache:
     # numpy arrays
     def append(self, batch, k, v, rope=None, q=None, q_out=None, positions=None, kind=None) -> int:
         assert self.device is None and batch.device is None, "need numpy arrays"
-        return lib.qx_kv_append(self.view, batch.view, heads_view(k, kind), heads_view(v, kind),
-                                None if rope is None else rope.view, _array(positions, "int64", None), heads_view(q, kind),
-                                heads_view(q_out, kind))
+        tokens, dim = batch.view.tokens, self.view.head_dim
+        return lib.qx_kv_append(self.view, batch.view, _rows(k, tokens, dim, kind), _rows(v, tokens, dim, kind),
+                                None if rope is None else rope.view, _array(positions, "int64", None, tokens),
+                                _rows(q, tokens, dim, kind), _rows(q_out, tokens, dim, kind))
 
     def read(self, batch, k, v, kind=None) -> int:
         assert self.device is None and batch.device is None, "need numpy arrays"
-        return lib.qx_kv_read(self.view, batch.view, heads_view(k, kind), heads_view(v, kind))
+        tokens, dim = batch.view.tokens, self.view.head_dim
+        return lib.qx_kv_read(self.view, batch.view, _rows(k, tokens, dim, kind), _rows(v, tokens, dim, kind))
 
     def attention(self, batch, q, out, scale=None, causal=True, window=0, lse=None, kind=None) -> int:
-        scale = self.view.head_dim ** -0.5 if scale is None else scale
         assert self.device is None and batch.device is None, "need numpy arrays"
-        return lib.qx_kv_attention(self.view, batch.view, heads_view(q, kind), heads_view(out, kind),
-                                   _array(lse, "float32", None), scale, 1 if causal else 0, window)
+        tokens, dim = batch.view.tokens, self.view.head_dim
+        scale = dim ** -0.5 if scale is None else scale
+        return lib.qx_kv_attention(self.view, batch.view, _rows(q, tokens, dim, kind), _rows(out, tokens, dim, kind),
+                                   _array(lse, "float32", None, tokens, q.shape[1]), scale, 1 if causal else 0, window)
 
     # device tensors, torch's current stream
     def append_dev(self, batch, k, v, rope=None, q=None, q_out=None, positions=None) -> int:
         device = _device()
         assert self.device == device == batch.device, "need tensors on the current device"
-        return lib.qx_kv_append_dev(self.view, batch.view, heads_view(k, device=device), heads_view(v, device=device),
-                                    None if rope is None else rope.view, _array(positions, "int64", device),
-                                    heads_view(q, device=device), heads_view(q_out, device=device), _stream())
+        tokens, dim = batch.view.tokens, self.view.head_dim
+        return lib.qx_kv_append_dev(self.view, batch.view, _device_rows(k, tokens, dim, device), _device_rows(v, tokens, dim, device),
+                                    None if rope is None else rope.view, _array(positions, "int64", device, tokens),
+                                    _device_rows(q, tokens, dim, device), _device_rows(q_out, tokens, dim, device), _stream())
 
     def read_dev(self, batch, k, v) -> int:
         device = _device()
         assert self.device == device == batch.device, "need tensors on the current device"
-        return lib.qx_kv_read_dev(self.view, batch.view, heads_view(k, device=device), heads_view(v, device=device),
+        tokens, dim = batch.view.tokens, self.view.head_dim
+        return lib.qx_kv_read_dev(self.view, batch.view, _device_rows(k, tokens, dim, device), _device_rows(v, tokens, dim, device),
                                   _stream())
 
     def attention_dev(self, batch, q, out, scale=None, causal=True, window=0, lse=None, workspace=None) -> int:
-        scale = self.view.head_dim ** -0.5 if scale is None else scale
         device = _device()
         assert self.device == device == batch.device, "need tensors on the current device"
-        return lib.qx_kv_attention_dev(self.view, batch.view, heads_view(q, device=device), heads_view(out, device=device),
-                                       _array(lse, "float32", device), scale, 1 if causal else 0, window, workspace,
-                                       _stream())
+        tokens, dim = batch.view.tokens, self.view.head_dim
+        scale = dim ** -0.5 if scale is None else scale
+        return lib.qx_kv_attention_dev(self.view, batch.view, _device_rows(q, tokens, dim, device),
+                                       _device_rows(out, tokens, dim, device),
+                                       _array(lse, "float32", device, tokens, q.shape[1]), scale, 1 if causal else 0, window,
+                                       workspace, _stream())
