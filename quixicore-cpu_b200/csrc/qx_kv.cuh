@@ -12,9 +12,8 @@ namespace qx {
 namespace kv {
 
 // Codes of the error word (qx_check_device_errors) for device arrays that contradict the call.
-constexpr int kErrorFirstBatch = 64;  // from here on: the batch, not a stalled pipeline
-constexpr int kErrorSequence = 64;    // a sequence's rows or length do not fit the bounds
-constexpr int kErrorBlock = 65;       // a block id outside the cache
+constexpr int kErrorSequence = sm100::kErrorFirstBatch;   // a sequence's rows or length do not fit the bounds
+constexpr int kErrorBlock = sm100::kErrorFirstBatch + 1;  // a block id outside the cache
 
 // On a boundary of its elements; NULL is.
 template <class T>

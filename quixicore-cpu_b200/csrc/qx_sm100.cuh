@@ -85,7 +85,9 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
 
 // Records why a kernel gives up (role / barrier code) in the caller's error word, which may
 // be host memory mapped into the device's address space: plain accesses only, first code
-// wins (approximately: concurrent reporters may overwrite each other, any of them will do).
+// wins (approximately: concurrent reporters may overwrite each other, any of them will do). Codes
+// from kErrorFirstBatch on say that a batch contradicts itself, all below that a wait gave up.
+constexpr int kErrorFirstBatch = 128;
 __device__ __forceinline__ void report_error(int* word, int code) {
   volatile int* w = word;
   if (*w == 0) *w = code;
