@@ -126,12 +126,13 @@ qx_status sync_and_check(DeviceContext* ctx, cudaStream_t s) {
 }
 
 // Reads and clears the error word of `ctx`; an aborted kernel may leave arrival counters
-// behind, so the default workspace's counter area is cleared with it.
+// behind, so the default workspace's counter area is cleared with it. (Not for a batch that
+// contradicts itself: nothing was aborted, and other streams' kernels may be counting.)
 qx_status take_device_error(DeviceContext* ctx) {
   const int code = *static_cast<volatile int*>(ctx->error_host);
   if (code == 0) return QX_STATUS_OK;
   *static_cast<volatile int*>(ctx->error_host) = 0;
-  if (ctx->workspace.base != nullptr) {
+  if (code < sm100::kErrorFirstBatch && ctx->workspace.base != nullptr) {
     (void)cudaMemset(ctx->workspace.base, 0, kWorkspaceCounterBytes);
   }
   char text[128];

@@ -86,11 +86,13 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
 // Records why a kernel gives up (role / barrier code) in the caller's error word, which may
 // be host memory mapped into the device's address space: plain accesses only, first code
 // wins (approximately: concurrent reporters may overwrite each other, any of them will do). Codes
-// from kErrorFirstBatch on say that a batch contradicts itself, all below that a wait gave up.
+// from kErrorFirstBatch on say that a batch contradicts itself, no kernel was stopped: a stall, which
+// may leave arrival counters behind, takes their place.
 constexpr int kErrorFirstBatch = 128;
 __device__ __forceinline__ void report_error(int* word, int code) {
   volatile int* w = word;
-  if (*w == 0) *w = code;
+  const int before = *w;
+  if (before == 0 || (before >= kErrorFirstBatch && code < kErrorFirstBatch)) *w = code;
 }
 
 // ---- TMA ---------------------------------------------------------------------------
