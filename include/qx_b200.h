@@ -705,8 +705,8 @@ QX_API qx_status qx_kv_read_dev(const qx_kv_cache* cache, const qx_kv_batch* bat
  * reads kv head h / (heads / kv_heads). The query of row i of a sequence with n rows stands at position
  * p = length - n + i: `causal` hides keys behind p, `window` > 0 hides keys at p - window and before
  * (0: none). A row that sees no key gives zeros (and -infinity in `lse`); here, other than for append, a
- * sequence may have more rows than tokens. `lse` (optional, f32 [tokens][heads]): ln of the sum of
- * exp(scale * q . k) over the keys seen.
+ * sequence may have more rows than tokens. A row that sees a key and whose query holds a NaN or an infinity gives
+ * NaN. `lse` (optional, f32 [tokens][heads]): ln of the sum of exp(scale * q . k) over the keys seen.
  * Products are taken to at least the precision of q's type, sums and softmax statistics are f32; f32
  * queries are multiplied with f32 precision. `out` may be q itself, the same view of it. Partial
  * results of splits over the keys live in `workspace` (NULL: the library's default one); calls that may

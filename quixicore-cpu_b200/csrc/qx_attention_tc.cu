@@ -612,7 +612,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         const int shift = top >= 255 ? 0 : min(120, max(-120, 134 - static_cast<int>(top)));
         // (a negative scale turns the query's sign, so that larger raw scores are larger scores)
         const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
-        row.factor = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * fabsf(p.scale_log2);
+        // (a row that holds a NaN or an infinity gives NaN: its products may all be -infinity, which reads as no key)
+        row.factor = top >= 255 ? __uint_as_float(0x7FC00000u)
+                                : __uint_as_float(static_cast<uint32_t>(127 - shift) << 23) * fabsf(p.scale_log2);
 #pragma unroll 2
         for (int c = 0; c < DP / 8; ++c) {
           uint4* const at = reinterpret_cast<uint4*>(piece_at<DP, false>(tile, r, c));
