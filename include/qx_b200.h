@@ -638,8 +638,8 @@ QX_API qx_status qx_rope_apply_dev(const qx_rope* rope, const qx_heads* x, const
  * scale for the keys and one for the values, value = code * scale. Memory is the caller's. A block
  * holds [kv_heads][block_tokens][head_dim] codes. block_tokens is 16, 32, 64 or 128; head_dim a
  * multiple of 16, 16 .. 256; the code arrays start on 16-byte boundaries. Blocks need no initial
- * contents: nothing behind a sequence's length is used. Scales are zero or more, or NaN (append makes
- * no others). */
+ * contents: nothing behind a sequence's length is used. Scales are zero or more, or NaN; append makes
+ * no others, and none between zero and 2^-100 (attention may take such a scale of values for zero). */
 typedef struct qx_kv_cache {
   int8_t* k_codes;         /* [blocks][kv_heads][block_tokens][head_dim] */
   int8_t* v_codes;

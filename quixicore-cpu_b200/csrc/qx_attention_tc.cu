@@ -56,7 +56,8 @@ constexpr int kMetaStages = 4;
 static_assert(kPromptRows == 2 * kRowTile && kPromptRowsWide == kRowTile, "two tiles per CTA, f32: one");
 constexpr int kKeepStages = 4;
 constexpr float kBehind = 4.0f;
-constexpr float kLeastLog = -100.0f;  // of a value scale: append makes no smaller one but zero
+constexpr float kLeastLog = -100.0f;  // of a value scale: append makes no smaller one but zero, and smaller ones count as that
+constexpr float kLeastScale = 7.8886090522101181e-31f;  // 2^-100
 
 constexpr float kSpan = 60.0f;  // log2 of the largest ratio of value scales that is kept
 
@@ -794,7 +795,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       if (!ok) break;
       if (lane < 2) {
         const float vs = scales[1];
-        const float log = vs < 7.8886090522101181e-31f ? kLeastLog : log2f(vs);  // (2^-100; no number stays none)
+        const float log = vs < kLeastScale ? kLeastLog : log2f(vs);  // (no number stays none)
         Meta& m = meta[j % kMetaStages];
         m.scales[2 * w + lane] = make_float2(scales[0], log);
         m.value_inverse[2 * w + lane] = exp2f(-log);
@@ -804,7 +805,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       if (lane == 0) mbar_arrive(&bars->meta[j % kMetaStages]);
       store(smem + S::kKeyRing + stage * S::kOperand);
       if (lane == 0) mbar_arrive(&bars->key_full[stage]);
-      load(j, id, p.v_codes);
+      // (a scale of zero makes zeros of any codes; it has no logarithm, so the codes stand for it)
+      const int value_id[2] = {__shfl_sync(0xFFFFFFFFu, scales[1], 0) < kLeastScale ? -1 : id[0],
+                               __shfl_sync(0xFFFFFFFFu, scales[1], 1) < kLeastScale ? -1 : id[1]};
+      load(j, value_id, p.v_codes);
       if (j + 1 < tiles) load_scales(next);
       if (j >= 2) ok = mbar_wait_warp(&bars->value_empty[stage], ((j >> 1) - 1) & 1, abort_flag);
       if (!ok) break;

@@ -114,3 +114,24 @@ def test_values_of_two_blocks_without_a_scale_are_zeros(qx, dtype, dim, group, n
     out = torch.full((new, group, dim), 3.0, device="cuda")
     assert on_device(qx, cache).attention_dev(batch, typed((new, group, dim), dtype, 3).cuda(), out) == qx.OK
     assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("size", [16, 64])
+@pytest.mark.parametrize("scale", [0.0, -0.0])
+@pytest.mark.parametrize("length,new", [(200, 130), (3000, 130)])
+def test_values_of_a_prompt_without_a_scale_are_zeros(qx, dtype, size, scale, length, new):
+    """Beside blocks that have one, too: rows that see none of those give zeros, the others what those give."""
+    width = -(-length // size)
+    cache, table = filled(width, 1, size, 64), table_of(1, width, width)
+    cache.scales[1][:] = scale
+    q = typed((new, 2, 64), dtype, 3)
+    out = torch.full((new, 2, 64), 3.0, device="cuda")
+    batch, _, _ = batch_of(qx, table, [length], [new])
+    assert on_device(qx, cache).attention_dev(batch, q.cuda(), out) == qx.OK
+    assert bool((out == 0).all())
+    cache.scales[1][table[0, (length - 20) // size]] = 0.01
+    compare(qx, cache, table, [length], [new], q)
+    first = (length - 20) // size * size - (length - new)
+    assert on_device(qx, cache).attention_dev(batch, q.cuda(), out) == qx.OK
+    assert bool((out[:max(0, first)] == 0).all()) and bool((out[max(0, first) + 1:] != 0).any())
