@@ -196,8 +196,11 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
     const bool seen = kMask == kOpen || (meta.present[u * kPerUnit] != 0 && key < row.high && key + kUnit > row.low);
     largest = fmaxf(largest, seen ? log[u] : -INFINITY);
   }
+  // The sum stands against the largest scale and the maximum. It follows both in one step: alone, a rise of the scale by
+  // more than about 2^100 would take it past f32's range, where the maximum rises as far.
+  float rise = 0.0f;
   if (largest > row.largest_log) {
-    if (row.sum != 0.0f) row.sum *= exp2_fast(largest - row.largest_log);
+    if (row.sum != 0.0f) rise = largest - row.largest_log;
     row.largest_log = largest;
     row.largest = exp2f(largest);
   }
@@ -261,14 +264,15 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   if (kWide) {
     const float before = row.maximum;
     if (behind) row.maximum = top;
-    const float keep = before == row.maximum ? 1.0f : exp2_fast(before - row.maximum);
-    row.sum *= keep;
-    *keep_to = keep;
+    const float moved = before == row.maximum ? 0.0f : before - row.maximum;
+    *keep_to = exp2_fast(moved);
+    rise += moved;
   } else if (__any_sync(0xFFFFFFFFu, behind)) {
     const float before = row.maximum;
     if (behind) row.maximum = top;
-    const float keep = before == row.maximum ? 1.0f : exp2_fast(before - row.maximum);
-    row.sum *= keep;
+    const float moved = before == row.maximum ? 0.0f : before - row.maximum;
+    const float keep = exp2_fast(moved);
+    rise += moved;
     if (!first) {
 #pragma unroll 1
       for (int c = 0; c < DP; c += 16) {
@@ -281,6 +285,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
       }
     }
   }
+  if (rise != 0.0f) row.sum *= exp2_fast(rise);
   const float base = (row.maximum == -INFINITY ? 0.0f : row.maximum) - kPromptShift;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {

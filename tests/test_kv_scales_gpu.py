@@ -135,3 +135,16 @@ def test_values_of_a_prompt_without_a_scale_are_zeros(qx, dtype, size, scale, le
     first = (length - 20) // size * size - (length - new)
     assert on_device(qx, cache).attention_dev(batch, q.cuda(), out) == qx.OK
     assert bool((out[:max(0, first)] == 0).all()) and bool((out[max(0, first) + 1:] != 0).any())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("size", [16, 64, 128])
+@pytest.mark.parametrize("first,then", [(0.0, 2.0 ** 14), (0.0, 2.0 ** 40), (2.0 ** -90, 2.0 ** 40), (2.0 ** -60, 2.0 ** 60)])
+@pytest.mark.parametrize("length,new", [(400, 400), (700, 130)])
+def test_quiet_values_in_front_of_loud_ones(qx, dtype, size, first, then, length, new):
+    """The first 128 keys' values are zero or tiny against all others: their weights count like any."""
+    width = -(-length // size)
+    cache, table = filled(width, 1, size, 64), table_of(1, width, width)
+    cache.scales[1][:] *= np.float32(then)
+    cache.scales[1][table[0, :128 // size]] = first
+    compare(qx, cache, table, [length], [new], typed((new, 2, 64), dtype, 3))
