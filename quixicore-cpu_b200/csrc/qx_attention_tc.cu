@@ -60,11 +60,12 @@ constexpr float kLeastLog = -100.0f;  // of a value scale: append makes no small
 constexpr float kLeastScale = 7.8886090522101181e-31f;  // 2^-100
 
 constexpr float kSpan = 60.0f;  // log2 of the largest ratio of value scales that is kept
+constexpr float kSpanInverse = 1.1529215046068470e18f;  // 2^kSpan
 
 // What the softmax needs to know about a tile of keys, by groups of 16.
 struct Meta {
   float2 scales[kGroups];        // of the keys, and log2 of the values'
-  float value_inverse[kGroups];  // 2^-log2
+  float value_inverse[kGroups];  // of the values' scale
   int present[kGroups];
 };
 
@@ -207,7 +208,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   const float least = largest - kSpan;
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    relative[u] = log[u] < least ? 1.1529215046068470e18f : relative[u] * row.largest;  // (2^60)
+    relative[u] = log[u] < least ? kSpanInverse : relative[u] * row.largest;
     log[u] = log[u] < least ? least : log[u];  // (no number stays none)
   }
 
@@ -803,7 +804,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         const float log = vs < kLeastScale ? kLeastLog : log2f(vs);  // (no number stays none)
         Meta& m = meta[j % kMetaStages];
         m.scales[2 * w + lane] = make_float2(scales[0], log);
-        m.value_inverse[2 * w + lane] = exp2f(-log);
+        // (of the scale itself: so the rounding of its logarithm, 2^-19 of a scale of 2^-64, is the weight's as much as
+        // the value's, and divided out; a whole number and the rest apart would keep it from the weights too, but take the
+        // f32 kernel 41.6 in place of 40.8 us, two f32 prompts of up to 4096 760 in place of 737)
+        m.value_inverse[2 * w + lane] = vs < kLeastScale ? exp2f(-kLeastLog) : 1.0f / vs;
         m.present[2 * w + lane] = (lane == 1 ? id[1] : id[0]) >= 0;
       }
       __syncwarp();

@@ -148,3 +148,29 @@ def test_quiet_values_in_front_of_loud_ones(qx, dtype, size, first, then, length
     cache.scales[1][:] *= np.float32(then)
     cache.scales[1][table[0, :128 // size]] = first
     compare(qx, cache, table, [length], [new], typed((new, 2, 64), dtype, 3))
+
+
+def rounded_logarithms(around, sign):
+    """A scale whose logarithm f32 rounds up (1) or down (-1) the most."""
+    mantissas = np.float32(2.0) ** around * np.linspace(1, 1.999, 100001).astype(np.float32)
+    exact = np.log2(mantissas.astype(np.float64))
+    return mantissas[np.argmax(sign * (exact.astype(np.float32).astype(np.float64) - exact))]
+
+
+U = 2.0 ** -23
+
+
+@pytest.mark.parametrize("dim,size", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("around", [-90, -66, -40, 40, 66])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_f32_prompts_keep_the_bits_of_value_scales(qx, dim, size, around, sign):
+    """Every row sees its own key alone. Its weight is held as two f16 halves, 2 u, and meets the code in two products,
+    1 u; the inverse of the scale, its product with the weight, the quotient of the largest scale and the sum, and the
+    product with that are rounded, 0.5 u each."""
+    cache, table = filled(-(-300 // size), 1, size, dim), table_of(1, -(-300 // size), -(-300 // size))
+    cache.scales[1][:] = rounded_logarithms(around, sign)
+    batch, _, _ = batch_of(qx, table, [300], [200])
+    out = torch.zeros(200, 2, dim, device="cuda")
+    assert on_device(qx, cache).attention_dev(batch, typed((200, 2, dim), F32, 3).cuda(), out, window=1) == qx.OK
+    want = torch.from_numpy(cache.values(1, table[0], 300)[100:])
+    assert float(((out.cpu().double() - want).abs() / want.abs().clamp_min(2.0 ** -120)).max()) <= 5 * U
