@@ -707,11 +707,15 @@ QX_API qx_status qx_kv_read_dev(const qx_kv_cache* cache, const qx_kv_batch* bat
  * (0: none). A row that sees no key gives zeros (and -infinity in `lse`); here, other than for append, a
  * sequence may have more rows than tokens. A row that sees a key and whose query holds a NaN or an infinity gives
  * NaN. `lse` (optional, f32 [tokens][heads]): ln of the sum of exp(scale * q . k) over the keys seen.
- * Products are taken to at least the precision of q's type, sums and softmax statistics are f32; f32
- * queries are multiplied with f32 precision. `out` may be q itself, the same view of it. Partial
- * results of splits over the keys live in `workspace` (NULL: the library's default one); calls that may
- * run at the same time need one each. The result bits do not depend on when CTAs run; they may on
- * max_tokens, max_length and the number of sequences, which choose the splits. */
+ * Precision. A query element is rounded to no more than 2^-22 of the largest of its row (one head of one token):
+ * an element far below that loses bits, whatever the keys hold there. Codes and scales are used as they are; sums
+ * and softmax statistics are f32. Weights are rounded to 2^-11 for 16-bit queries, to 2^-22 for f32 ones, and
+ * to no less than 2^-37 of the row's largest (2^-36 of its largest product with a block's scale of values in calls of
+ * many rows; a scale more than 2^60 below the largest that a row sees counts as 2^-60 of it there).
+ * `out` may be q itself, the same view of it. Partial results of splits over the keys live in `workspace` (NULL: the
+ * library's default one); calls that may run at the same time need one each. The result bits do not depend on
+ * when CTAs run; they may on max_tokens, max_length, the number of sequences and the lengths of all of them, which
+ * choose the splits. */
 QX_API qx_status qx_kv_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q,
                                  const qx_heads* out, float* lse, float scale, int causal,
                                  long long window);

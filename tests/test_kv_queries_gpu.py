@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_kv_attention_gpu import BF16, F16, F32, filled
+from test_kv_attention_gpu import BF16, F16, F32, check, filled
 from test_kv_cache_gpu import batch_of, on_device, table_of, typed
 
 pytestmark = pytest.mark.gpu
@@ -45,3 +45,28 @@ def test_a_query_that_is_no_number_and_sees_no_key(qx, dtype, new):
     out, lse = torch.full((new, 2, 64), 3.0, dtype=dtype, device="cuda"), torch.zeros(new, 2, device="cuda")
     assert on_device(qx, cache).attention_dev(batch, q.cuda(), out, lse=lse) == qx.OK
     assert bool((out[:2] == 0).all()) and bool((lse[:2] == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype,above", [(F32, 2.0 ** 12), (F32, 2.0 ** 30), (F16, 2.0 ** 12), (BF16, 2.0 ** 12), (BF16, 2.0 ** 30)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 5, 200])
+def test_one_element_far_above_its_row(qx, dtype, above, dim, new):
+    """... where the keys hold zeros, so that the small elements make the scores: they are rounded to 2^-22 of the large
+    one (the tolerance counts that), and to nothing else."""
+    cache, table = filled(20, 2, 32, dim), table_of(1, 20, 20)
+    cache.codes[0][:, :, :, 5] = 0
+    q = typed((new, 4, dim), dtype, 11).double()
+    q[:, :, 5] = above
+    check(qx, cache, on_device(qx, cache), table, [600], [new], q.to(dtype))
+
+
+@pytest.mark.parametrize("new", [1, 3, 200])
+def test_bits_of_a_session_may_follow_its_neighbours(qx, new):
+    """What stays: the tolerance, and the bits of the same call made again."""
+    cache, table = filled(600, 8, 32, 64), table_of(12, 50, 600)
+    dev, q = on_device(qx, cache), typed((12 * new, 32, 64), BF16, 2)
+    for others in (1600, 700, new):
+        lengths = [1500] + [others] * 11
+        first, lse = check(qx, cache, dev, table, lengths, [new] * 12, q)
+        again, lse_again = check(qx, cache, dev, table, lengths, [new] * 12, q)
+        assert torch.equal(first, again) and torch.equal(lse, lse_again)
