@@ -661,7 +661,8 @@ typedef struct qx_kv_cache {
  * and lengths. Device arrays that contradict the bounds or the cache are never followed out of it: a
  * sequence whose numbers do not fit is not served (its outputs are not written), the tokens of a block
  * that the cache does not have are neither written nor seen, and qx_check_device_errors() reports
- * QX_STATUS_DEVICE_ERROR afterwards. The host-pointer forms return QX_STATUS_INVALID_ARGUMENT. */
+ * QX_STATUS_DEVICE_ERROR afterwards. The host-pointer forms return QX_STATUS_INVALID_ARGUMENT, and
+ * QX_STATUS_INVALID_SHAPE for sequences that reach 2^31 rows. */
 typedef struct qx_kv_batch {
   int sequences;
   const int32_t* token_begin;   /* [sequences + 1] or NULL */

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <limits>
 #include <new>
 #include <stdexcept>
 #include <vector>
@@ -146,6 +147,7 @@ qx_status pack(const qx_kv_cache* cache, const qx_kv_batch* batch, bool rows_are
     if (row < before || n < 0 || n > batch->max_tokens || next > batch->tokens || (rows_are_cached && n > length)) {
       return QX_STATUS_INVALID_ARGUMENT;
     }
+    if (next > std::numeric_limits<int32_t>::max()) return QX_STATUS_INVALID_SHAPE;  // (the packed batch counts in 32 bits)
     before = next;
     out->begin.push_back(static_cast<int32_t>(row));
     out->lengths.push_back(length);

@@ -143,3 +143,12 @@ def test_device_calls(qx, monkeypatch):
     refused(lambda: cache.append_dev(batch, x, x, rope, positions=E(2, dtype=i64)))
     refused(lambda: rope.apply_dev(x, x, E(2, dtype=i64)))
     assert len(called) == 4
+
+
+def test_more_rows_than_32_bits_count_on_the_host(qx):
+    """Sequences of max_tokens rows each, without token_begin: their first rows would wrap."""
+    cache = qx.KVCache(*arrays())
+    batch = qx.KVBatch(np.zeros(3, np.int32), np.zeros((3, 2), np.int32), 32, None, 3 << 30, 1 << 30)
+    q, out = np.zeros((1, 2, 32), np.float32), np.zeros((1, 2, 32), np.float32)
+    views = qx.heads_view(q, token_stride=0), qx.heads_view(out, token_stride=64)
+    assert qx.lib.qx_kv_attention(cache.view, batch.view, *views, None, 1.0, 1, 0) == qx.INVALID_SHAPE
