@@ -30,11 +30,11 @@
 // groups so that these reads meet no conflicts for head sizes up to 128.
 //
 // Bound by HBM for long contexts: 2 * head_dim bytes per key and kv head, whatever the group. Measured (128 elements, 8
-// kv heads): 32 sessions of up to 8192 tokens, 32 query heads, 64.6 us (314 MB, 4.9 TB/s, 0.75 of the copy bandwidth);
-// one of 131072 tokens, 64 query heads, 54 us (5.0 TB/s); one of 1000 tokens, f32, 7.7 us. What is above the bytes' time
-// is a CTA's way in and out: about 9000 cycles before its first tile (cold instructions, length, table, queries) and
-// 4000 behind its last. With 64 elements and 15 rows (drafts) the instructions bind: 32 sessions, windows of 4096, 55 us
-// for 134 MB, issue slots 54 % taken.
+// kv heads): 32 sessions of up to 8192 tokens, 32 query heads, 64.5 us (314 MB, 4.9 TB/s, 0.74 of the copy bandwidth; 72
+// where other calls' inputs have taken its own out of L2); one of 131072 tokens, 64 query heads, 54 us (5.0 TB/s; 61); one
+// of 1000 tokens, f32, 7.5 us. What is above the bytes' time is a CTA's way in and out: about 9000 cycles before its first
+// tile (cold instructions, length, table, queries) and 4000 behind its last. With 64 elements and 15 rows (drafts) the
+// instructions bind: 32 sessions, windows of 4096, 55 us for 134 MB, issue slots 55 % taken.
 
 #include <algorithm>
 #include <cmath>

@@ -18,8 +18,8 @@
 // log2 vs, so one f16 rounding (2^-11) holds for every mixture of scales; the sums of weights divide it out
 // again, once per 16 keys, relative to the largest scale that the row has seen. (A scale more than 2^60 below
 // that one counts as 2^-60 of it, so that no weight leaves f32's range on the way; that moves an output by 2^-53
-// of the largest value.) m only follows when it has fallen 4 behind (a factor of 16): then the row's sum and O
-// are scaled, in TMEM, by the row's own warp, which is rare after the first tiles.
+// of the largest value.) A scale of zero takes its block's codes for zeros. m only follows when it has fallen 4 behind (a
+// factor of 16): then the row's sum and O are scaled, in TMEM, by the row's own warp, which is rare after the first tiles.
 //
 // f32 queries (kWide) take one tile of 128 rows per CTA, whose queries and weights are f16 pairs, hi + lo, of 22 bits:
 // the second tile's place in shared memory holds the low halves of the queries, the second half of S the low halves
@@ -29,8 +29,8 @@
 // ready when a softmax ends (2 x 1000 tokens, 4000 keys, 16 heads of 96 elements: 190 us without, 166 with).
 //
 // Measured: two prompts of up to 4096 bf16 tokens, 32 query heads on 8, 128 elements, causal: 303 us (208 GFLOP, 680
-// TFLOP/s); 1024 f16 tokens behind 15360: 321 us (830 TFLOP/s); 4 texts of up to 500 f32 tokens, 16 heads of 96
-// elements: 40.5 us. A tile of 128 keys takes 4600 cycles for both row tiles, where the MMAs alone take 2050 and the
+// TFLOP/s); 1024 f16 tokens behind 15360: 322 us (825 TFLOP/s); 4 texts of up to 500 f32 tokens, 16 heads of 96
+// elements: 41.0 us. A tile of 128 keys takes 4600 cycles for both row tiles, where the MMAs alone take 2050 and the
 // exponentials 2050: a row tile's S, softmax and P V follow one another, and only the other row tile runs beside them.
 // A CTA's way in (11000 cycles: table, queries to operands, first keys) and out (6000) comes on top.
 //
