@@ -46,8 +46,9 @@ namespace kv {
 namespace {
 
 // P is held times 2^12 where it is rounded to 16 bits, so that weights down to 2^-26 keep all their bits;
-// sums of P carry the same factor.
+// sums of P carry the same factor, sums of P V do not (values near the end of f32's range stay in it).
 constexpr float kShift = 12.0f;
+constexpr float kCarried = 4096.0f, kCarriedInverse = 1.0f / kCarried;  // 2^kShift
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 32;
 constexpr uint32_t kZeroSum = 0x4B400000u;  // 1.5 * 2^23: whole numbers below 2^22 added to the bits are exact
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
     const float4 scales = *reinterpret_cast<const float4*>(meta);
     // (of a half that is not there the stage holds anything)
     const float ks[2] = {scales.x, scales.y};
-    const float vs[2] = {present & 1 ? scales.z : 0.0f, present & 2 ? scales.w : 0.0f};
+    const float vs[2] = {present & 1 ? scales.z * kCarriedInverse : 0.0f, present & 2 ? scales.w * kCarriedInverse : 0.0f};
     const bool open = token0 + kTile <= open_high && token0 >= open_low && present == 3;
 
     // ---- scores of 16 keys at a time: lane (g, t) gets keys g, g + 8 and rows 2 t, 2 t + 1 ----------------------
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
     }
     long long out_row, out_head;
     place_of(r, &out_row, &out_head);
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inverse = total == 0.0f ? 0.0f : kCarried / total;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] *= inverse;
     store8(p.out.data, p.out.type, p.out.vector, out_row * p.out.token_stride + out_head * p.out.head_stride + d, v);
@@ -755,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, kWide, kRowTiles>::kCtas)
               v.w = fmaf(v.w, keep, x[b].w * weight);
             }
           }
-          const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+          const float inverse = total == 0.0f ? 0.0f : kCarried / total;
           long long out_row, out_head;
           place_of(r, &out_row, &out_head);
           const long long to = out_row * p.out.token_stride + out_head * p.out.head_stride + 4 * at;
@@ -841,7 +842,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     v.z = fmaf(x.z, weight, v.z);
     v.w = fmaf(x.w, weight, v.w);
   }
-  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inverse = sum == 0.0f ? 0.0f : exp2f(p.shift) / sum;
   const long long to = (rows.row + token) * p.out.token_stride + out_head * p.out.head_stride + 4 * threadIdx.x;
   store_one(p.out.data, p.out.type, to, v.x * inverse);
   store_one(p.out.data, p.out.type, to + 1, v.y * inverse);

@@ -21,7 +21,7 @@ struct AttentionParams {
   int group;         // query heads per kv head
   int tile_rows;     // rows of a tile
   int row_tiles, splits, chunk;
-  float shift;       // log2 of what sums of weights carry
+  float shift;       // log2 of what sums of weights carry (and those of weights times values do not)
   float* partial;    // [tile][split][rows][dim] sums, then [tile][split][rows] {maximum, sum}
   float* statistics;
   int* counters;     // [item] CTAs that have written a part, zero between calls; NULL: another kernel joins

@@ -59,6 +59,7 @@ constexpr float kBehind = 4.0f;
 constexpr float kLeastLog = -100.0f;  // of a value scale: append makes no smaller one but zero, and smaller ones count as that
 constexpr float kLeastScale = 7.8886090522101181e-31f;  // 2^-100
 
+constexpr float kCarriedInverse = 1.0f / 2048.0f;  // 2^-kPromptShift
 constexpr float kSpan = 60.0f;  // log2 of the largest ratio of value scales that is kept
 constexpr float kSpanInverse = 1.1529215046068470e18f;  // 2^kSpan
 
@@ -694,8 +695,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       if (ok) {
         tc_fence_after_sync();
         const bool whole = splits_used(p, rows) == 1;
-        // O stands against the maximum alone, the sum against that and the largest scale
-        const float gain = row.sum == 0.0f ? 0.0f : whole ? row.largest / row.sum : row.largest;
+        // O stands against the maximum alone, the sum against that and the largest scale; what the sum carries is taken
+        // from the partial results of O, as the kernel that joins them has it
+        const float gain = row.sum == 0.0f ? 0.0f : whole ? row.largest / row.sum : row.largest * kCarriedInverse;
         const float maximum = row.sum == 0.0f ? -INFINITY : row.maximum - row.largest_log;
         const long long at = ((tile_index * p.splits + split) * kCtaRows + in_tile);
         if (kWide) {

@@ -174,3 +174,16 @@ def test_f32_prompts_keep_the_bits_of_value_scales(qx, dim, size, around, sign):
     assert on_device(qx, cache).attention_dev(batch, typed((200, 2, dim), F32, 3).cuda(), out, window=1) == qx.OK
     want = torch.from_numpy(cache.values(1, table[0], 300)[100:])
     assert float(((out.cpu().double() - want).abs() / want.abs().clamp_min(2.0 ** -120)).max()) <= 5 * U
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("by", [2.0 ** -90, 2.0 ** 112])
+@pytest.mark.parametrize("sequences,length,new", [(1, 90, 1), (1, 6000, 2), (1, 20000, 1), (40, 900, 1), (2, 300, 150), (1, 6000, 100)])
+def test_values_of_any_magnitude(qx, dtype, by, sequences, length, new):
+    """Whole rows, rows in parts joined by either kernel, the balanced line: no sum leaves f32's range before the output
+    does."""
+    size, dim = 32, 64
+    width = -(-length // size)
+    cache, table = filled(width, 2, size, dim), table_of(1, width, width).repeat(sequences, 0)  # (all the same blocks)
+    cache.scales[1][:] *= np.float32(by)
+    compare(qx, cache, table, [length] * sequences, [new] * sequences, typed((sequences * new, 4, dim), dtype, 3))
