@@ -680,7 +680,7 @@ typedef struct qx_kv_batch {
  * codes become round(code * s / s'). New codes are round(x / s'), limited to +-127. Scales are f32; both
  * rounds are half to even of the exact quotient. A block whose s' would be below 2^-100 holds zeros. A NaN or an
  * infinity among the new elements makes the block's scale of that head NaN, and with it all of its values.
- * Blocks that are written belong to one sequence only.
+ * Blocks that are written belong to one sequence only, and to one place of it.
  *
  * `rope` (optional, rotary_dim a multiple of 16) rotates the keys on the way, in f32 and without a
  * rounding in between, by positions[row] or, with positions NULL, by the token's place in its sequence;
@@ -713,10 +713,10 @@ QX_API qx_status qx_kv_read_dev(const qx_kv_cache* cache, const qx_kv_batch* bat
  * and softmax statistics are f32. Weights are rounded to 2^-11 for 16-bit queries, to 2^-22 for f32 ones, and
  * to no less than 2^-37 of the row's largest (2^-36 of its largest product with a block's scale of values in calls of
  * many rows; a scale more than 2^60 below the largest that a row sees counts as 2^-60 of it there).
- * `out` may be q itself, the same view of it. Partial results of splits over the keys live in `workspace` (NULL: the
- * library's default one); calls that may run at the same time need one each. The result bits do not depend on
- * when CTAs run; they may on max_tokens, max_length, the number of sequences and the lengths of all of them, which
- * choose the splits. */
+ * `out` may be q itself, the same view of it. Partial results of splits over the keys live in `workspace`, one of the
+ * current device (NULL: the library's default one); calls that may run at the same time need one each. The result
+ * bits do not depend on when CTAs run; they may on max_tokens, max_length, the number of sequences and the lengths of
+ * all of them, which choose the splits. */
 QX_API qx_status qx_kv_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q,
                                  const qx_heads* out, float* lse, float scale, int causal,
                                  long long window);

@@ -987,6 +987,8 @@ extern "C" qx_status qx_kv_attention_dev(const qx_kv_cache* cache, const qx_kv_b
   QX_TRY(kv::check_attention(cache, batch, q, out, lse_dev, scale, window));
   DeviceContext* ctx = nullptr;
   QX_TRY(current_context(&ctx));
-  return kv::launch_attention(cache, batch, q, out, lse_dev, scale, causal, window, ctx,
-                              workspace != nullptr ? workspace : &ctx->workspace, static_cast<cudaStream_t>(stream));
+  if (workspace == nullptr) workspace = &ctx->workspace;
+  if (workspace->device != ctx->device) return QX_STATUS_INVALID_ARGUMENT;
+  return kv::launch_attention(cache, batch, q, out, lse_dev, scale, causal, window, ctx, workspace,
+                              static_cast<cudaStream_t>(stream));
 }

@@ -1,6 +1,8 @@
 """A batch that contradicts itself is reported without touching what other calls are at: no kernel was stopped, so the
 arrival counters that calls share with their workspace stay as they are."""
 
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -65,3 +67,22 @@ def test_reports_beside_attention_on_another_stream(qx, lengths):
     assert dev.attention_dev(batch, q, after) == qx.OK
     torch.cuda.synchronize()
     assert torch.equal(after, want) and qx.lib.qx_check_device_errors() == qx.OK
+
+
+def test_a_workspace_of_another_device_is_refused(qx):
+    """Its memory lies where the kernels of this device must not follow it. (There is one device here: the workspace says
+    that it belongs to another.)"""
+    cache, table = filled(60, 2, 64, 128), table_of(1, 60, 60)
+    dev, batch = on_device(qx, cache), batch_of(qx, table, [3800], [1])[0]
+    q, out = typed((1, 8, 128), BF16, 1).cuda(), torch.full((1, 8, 128), 5.0, dtype=BF16, device="cuda")
+    workspace = C.c_void_p()
+    assert qx.lib.qx_workspace_create(64 << 20, C.byref(workspace)) == qx.OK
+    device = C.c_int.from_address(workspace.value)
+    assert device.value == torch.cuda.current_device()
+    device.value += 1
+    assert dev.attention_dev(batch, q, out, workspace=workspace) == qx.INVALID_ARGUMENT
+    torch.cuda.synchronize()
+    assert bool((out == 5).all())
+    device.value -= 1
+    assert dev.attention_dev(batch, q, out, workspace=workspace) == qx.OK
+    qx.lib.qx_workspace_destroy(workspace)
