@@ -725,6 +725,39 @@ QX_API qx_status qx_kv_attention_dev(const qx_kv_cache* cache, const qx_kv_batch
                                      float scale, int causal, long long window,
                                      qx_workspace* workspace, void* stream);
 
+/* ---- between the blocks of a layer --------------------------------------------------------
+ * The norm behind a block, its gate and residual scale, the sum with the residual stream and the norm in
+ * front of the next block, in one pass over the rows:
+ *   joined = residual + scale * gate * post(block),   normed = pre(joined)
+ * A view of one row of `dim` elements for every token: element d of token t is at data[t * stride + d]. A view that
+ * is read may have a stride of zero (a gate of one row for all tokens); rows of a written one do not overlap. */
+typedef struct qx_rows {
+  void* data;
+  int type;                /* QX_STORAGE_* */
+  long long stride;        /* in elements */
+} qx_rows;
+/* QX_NORM_RMS: v / sqrt(mean(v^2) + eps) * (weight + offset) + bias; QX_NORM_LAYER: the same of v - mean(v). */
+enum { QX_NORM_RMS = 0, QX_NORM_LAYER = 1 };
+typedef struct qx_norm {
+  int kind;
+  int type;                /* of weight and bias */
+  const void* weight;      /* [dim]; NULL: no factor (and no offset) */
+  const void* bias;        /* [dim]; NULL: none */
+  float eps;               /* zero or more */
+  float offset;            /* 1 where the weights are stored as differences from 1 */
+} qx_norm;
+/* Any of these may be NULL: residual (zeros) or block (then joined = residual, without post and gate), not both;
+ * post, gate; joined (not stored), or pre and normed together (not computed), not all. Every view and norm may have a
+ * type of its own. joined and normed may each be residual, block or gate itself, the same view of it; otherwise written
+ * views overlap no other view. dim is 1 .. 32768. Sums and statistics are f32, each output is rounded once; normed is
+ * that of joined before its rounding. A row has the same bits in every batch. */
+QX_API qx_status qx_residual_norm(const qx_rows* residual, const qx_rows* block, const qx_norm* post,
+                                  const qx_rows* gate, float scale, const qx_rows* joined, const qx_norm* pre,
+                                  const qx_rows* normed, long long tokens, long long dim);
+QX_API qx_status qx_residual_norm_dev(const qx_rows* residual, const qx_rows* block, const qx_norm* post,
+                                      const qx_rows* gate, float scale, const qx_rows* joined, const qx_norm* pre,
+                                      const qx_rows* normed, long long tokens, long long dim, void* stream);
+
 /* ---- threading: set_num_threads / num_threads, include/quixicore_cpu/threading.h:11-12.
  * The fork-join pool is replaced by CUDA streams; these are kept so callers link. The
  * value is stored and returned, results never depend on it. */

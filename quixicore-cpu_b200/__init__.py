@@ -121,6 +121,17 @@ class KVBatchView(C.Structure):
                 ("table_stride", _ll), ("tokens", _ll), ("max_tokens", C.c_int), ("max_length", C.c_int)]
 
 
+class RowsView(C.Structure):
+    """qx_rows of include/qx_b200.h."""
+    _fields_ = [("data", _vp), ("type", C.c_int), ("stride", _ll)]
+
+
+class NormView(C.Structure):
+    """qx_norm of include/qx_b200.h."""
+    _fields_ = [("kind", C.c_int), ("type", C.c_int), ("weight", _vp), ("bias", _vp), ("eps", C.c_float),
+                ("offset", C.c_float)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -194,6 +205,10 @@ def _load():
                             C.POINTER(HeadsView), _vp, C.c_float, C.c_int, _ll],
         "qx_kv_attention_dev": [C.POINTER(KVCacheView), C.POINTER(KVBatchView), C.POINTER(HeadsView),
                                 C.POINTER(HeadsView), _vp, C.c_float, C.c_int, _ll, _vp, _vp],
+        "qx_residual_norm": [C.POINTER(RowsView), C.POINTER(RowsView), C.POINTER(NormView), C.POINTER(RowsView), C.c_float,
+                             C.POINTER(RowsView), C.POINTER(NormView), C.POINTER(RowsView), _ll, _ll],
+        "qx_residual_norm_dev": [C.POINTER(RowsView), C.POINTER(RowsView), C.POINTER(NormView), C.POINTER(RowsView),
+                                 C.c_float, C.POINTER(RowsView), C.POINTER(NormView), C.POINTER(RowsView), _ll, _ll, _vp],
         "qx_peer_alloc": [_sz, C.POINTER(_vp), _vp],
         "qx_peer_open": [_vp, C.POINTER(_vp)],
         "qx_peer_close": [_vp],
@@ -858,3 +873,77 @@ class KVCache:
                                        _device_rows(out, tokens, dim, device),
                                        _array(lse, "float32", device, tokens, q.shape[1]), scale, 1 if causal else 0, window,
                                        workspace, _stream())
+
+
+# ---- between the blocks of a layer: norms, gate, residual sum ----
+NORM_RMS, NORM_LAYER = 0, 1
+
+
+class Norm:
+    """A norm (qx_norm) of rows of as many elements as its weight and bias have, tensors on the device or numpy arrays of
+    one type (uint16 bits need `storage`), either or both None; they are kept alive."""
+
+    def __init__(self, weight=None, bias=None, kind=NORM_RMS, eps=1e-6, offset=0.0, storage=None):
+        self.arrays = (weight, bias)
+        self.dim = self.device = None
+        addresses, kinds = [], set()
+        for a in self.arrays:
+            if a is None:
+                addresses.append(None)
+                continue
+            host = isinstance(a, np.ndarray)
+            device = -1 if host else a.get_device()
+            assert len(a.shape) == 1 and self.dim in (None, a.shape[0]) and self.device in (None, device), "need weight [dim], bias [dim]"
+            assert (a.flags["C_CONTIGUOUS"] if host else device >= 0 and a.is_contiguous()), "need contiguous arrays"
+            self.dim, self.device = a.shape[0], device
+            addresses.append(a.ctypes.data if host else a.data_ptr())
+            kinds.add(_numpy_kind(a, storage) if host else (_torch_types or _fill_torch_types())[a.dtype])
+        assert len(kinds) < 2, "weight and bias have the same type"
+        self.view = NormView(kind, kinds.pop() if kinds else F32, *addresses, eps, offset)
+
+
+def _numpy_kind(a, storage) -> int:
+    """The storage type of a numpy operand: f32, or 16-bit elements of the type that is named (f16 where none is)."""
+    kind = {2: F16, 4: F32}[a.itemsize] if storage is None else storage
+    assert a.itemsize == (4 if kind == F32 else 2), "elements of another size than their type's"
+    return kind
+
+
+def _row_view(t, tokens, dim, device, storage=None, one=False) -> RowsView:
+    """A qx_rows over a [tokens, dim] operand (`one`: or over [1, dim], for all tokens), on `device` or, where that is
+    -1, a numpy array. The library gets no sizes and would follow a smaller one past its end."""
+    if t is None:
+        return None
+    rows, elements = t.shape
+    if isinstance(t, np.ndarray):
+        assert device == -1, "need a tensor on the current device"
+        kind, data, (stride, step) = _numpy_kind(t, storage), t.ctypes.data, (s // t.itemsize for s in t.strides)
+    else:
+        assert t.get_device() == device >= 0, "need tensors on the current device, or numpy arrays"
+        kind, data, (stride, step) = (_torch_types or _fill_torch_types())[t.dtype], t.data_ptr(), t.stride()
+    assert elements == dim and (step == 1 or dim == 1), "need [tokens, dim] with the elements of a row side by side"
+    if one and rows == 1:
+        return RowsView(data, kind, 0)
+    assert rows >= tokens, "need a row for every token"
+    return RowsView(data, kind, stride)
+
+
+def _residual_norm(device, residual, block, joined, normed, pre, post, gate, scale, storage=None):
+    tokens, dim = (block if residual is None else residual).shape
+    for norm in (pre, post):
+        assert norm is None or (norm.dim in (None, dim) and norm.device in (None, device)), "norms of another size or device"
+    return (_row_view(residual, tokens, dim, device, storage), _row_view(block, tokens, dim, device, storage),
+            None if post is None else post.view, _row_view(gate, tokens, dim, device, storage, True), scale,
+            _row_view(joined, tokens, dim, device, storage), None if pre is None else pre.view,
+            _row_view(normed, tokens, dim, device, storage), tokens, dim)
+
+
+def residual_norm(residual, block, joined, normed=None, pre=None, post=None, gate=None, scale=1.0, storage=None) -> int:
+    """joined = residual + scale * gate * post(block), normed = pre(joined) over numpy arrays [tokens, dim]."""
+    return lib.qx_residual_norm(*_residual_norm(-1, residual, block, joined, normed, pre, post, gate, scale, storage))
+
+
+def residual_norm_dev(residual, block, joined, normed=None, pre=None, post=None, gate=None, scale=1.0) -> int:
+    """The same over tensors on the current device, on torch's current stream."""
+    return lib.qx_residual_norm_dev(*_residual_norm(_device(), residual, block, joined, normed, pre, post, gate, scale),
+                                    _stream())

@@ -296,14 +296,14 @@ Rotation device_rotation(const qx_rope* rope, bool inverse);
 // A launch that may start while the kernel in front of it on the stream still runs: the kernel waits for it
 // itself (griddepcontrol.wait) before it touches memory.
 template <class Kernel, class Params>
-qx_status launch_behind(Kernel kernel, long long grid, int threads, size_t smem, cudaStream_t stream, const Params& p) {
+qx_status launch_behind(Kernel kernel, long long grid, dim3 threads, size_t smem, cudaStream_t stream, const Params& p) {
   if (grid > 0x7FFFFFFFLL) {
     set_last_error_text("the call needs more thread blocks than one launch has");
     return QX_STATUS_INVALID_SHAPE;
   }
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(grid));
-  config.blockDim = dim3(threads);
+  config.blockDim = threads;
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attribute{};
