@@ -750,7 +750,7 @@ typedef struct qx_norm {
  * post, gate; joined (not stored), or pre and normed together (not computed), not all. Every view and norm may have a
  * type of its own. joined and normed may each be residual, block or gate itself, the same view of it; otherwise written
  * views overlap no other view. dim is 1 .. 32768. Sums and statistics are f32, each output is rounded once; normed is
- * that of joined before its rounding. A row has the same bits in every batch. */
+ * that of joined before its rounding. A row has the same bits in every batch of views of its types and alignment. */
 QX_API qx_status qx_residual_norm(const qx_rows* residual, const qx_rows* block, const qx_norm* post,
                                   const qx_rows* gate, float scale, const qx_rows* joined, const qx_norm* pre,
                                   const qx_rows* normed, long long tokens, long long dim);

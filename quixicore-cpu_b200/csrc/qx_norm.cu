@@ -8,9 +8,11 @@
 // the number of norms; statistics are f32 (a layer norm's variance is that of the differences from the mean, taken
 // in a second sum over the registers: no cancellation), and normed is taken from joined before its rounding. A row
 // takes one CTA of up to 512 threads, or a part of one, each with vectors of eight elements; which depends on the
-// row's length alone, so that a row has the same bits in every batch. Up to 8192 elements all loads of a row are under way
-// before the first is used; longer rows hold registers enough for one operand at a time.
+// row's length, types and alignment alone, so that a row has the same bits in every batch. Up to 16384 elements all loads of a row are under way
+// before the first is used. Bound by HBM for many rows: 8192 of 4096 bf16 elements 46.9 us for 268 MB (5.7 TB/s, 0.87 of the
+// copy bandwidth); by the launch and one way to memory for few (one row 2.3 us, 64 of 5120 with both norms 3.8).
 #include <cmath>
+#include <initializer_list>
 #include <limits>
 
 #include "qx_host_arrays.cuh"
@@ -21,6 +23,7 @@ namespace {
 
 constexpr int kNormThreads = 512, kMostVectors = 8;
 constexpr int kMostDim = 8 * kNormThreads * kMostVectors;
+constexpr int kSums = 4, kRowWarps = kNormThreads / 32;
 
 struct View {
   uint8_t* data;  // NULL: there is none
@@ -40,45 +43,53 @@ struct JoinParams {
   int dim;
 };
 
-// Eight neighbouring elements as they lie in memory; where they are no whole vector, each on its own as f32 bits.
-struct Words {
-  uint4 a[2];
-  int type;
-};
-__device__ __forceinline__ Words load_words(const View& x, long long row, int d, int count) {
-  Words w;
-  const long long index = row * x.stride + d;
-  w.type = x.type;
-  w.a[1] = make_uint4(0, 0, 0, 0);
-  if (x.vector && count == 8) {
-    const uint4* const from = reinterpret_cast<const uint4*>(x.data + index * (x.type == QX_STORAGE_F32 ? 4 : 2));
-    w.a[0] = from[0];
-    if (x.type == QX_STORAGE_F32) w.a[1] = from[1];
-  } else {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < count ? load_one(x.data, x.type, index + i) : 0.0f;
-    to_words<QX_STORAGE_F32>(v, w.a);
-    w.type = QX_STORAGE_F32;
+// How a thread's 8 * kVectors elements of a row lie, and how they are read and written. Vectors: runs of eight, whose
+// type the kernel knows. Elements: each on its own, neighbouring threads side by side, of types that the launch knows;
+// for rows that are no whole number of vectors or start off a 16-byte boundary, and rare mixtures of types.
+template <int kType>
+struct InVectors {
+  static constexpr bool kEach = false;
+  uint4 w[kType == QX_STORAGE_F32 ? 2 : 1];
+  static __device__ __forceinline__ int place(int i, int) { return (static_cast<int>(threadIdx.x) + i * static_cast<int>(blockDim.x)) * 8; }
+  __device__ __forceinline__ void load(const View& x, long long row, int dim, int i) {
+    const int d = place(i, 0);
+    if (d < dim) load8_words<kType>(x.data, row * x.stride + d, w);
   }
-  return w;
-}
-__device__ __forceinline__ void values_of(const Words& w, float (&v)[8]) {
-  const uint4 narrow[1] = {w.a[0]};
-  if (w.type == QX_STORAGE_F32) from_words<QX_STORAGE_F32>(w.a, v);
-  else if (w.type == QX_STORAGE_F16) from_words<QX_STORAGE_F16>(narrow, v);
-  else from_words<QX_STORAGE_BF16>(narrow, v);
-}
-__device__ __forceinline__ void store_values(const View& y, long long row, int d, int count, const float (&v)[8]) {
-  const long long index = row * y.stride + d;
-  if (count == 8) {
-    store8(y.data, y.type, y.vector, index, v);
-  } else {
-    for (int i = 0; i < 8; ++i) {
-      if (i < count) store_one(y.data, y.type, index + i, v[i]);
+  __device__ __forceinline__ void values(const View&, float (&v)[8]) const { from_words<kType>(w, v); }
+  static __device__ __forceinline__ void store(const View& y, long long row, int dim, int i, const float (&v)[8]) {
+    const int d = place(i, 0);
+    if (d < dim) store8_typed<kType>(y.data, row * y.stride + d, v);
+  }
+};
+struct InElements {
+  static constexpr bool kEach = true;
+  uint32_t w[8];
+  static __device__ __forceinline__ int place(int i, int e) { return static_cast<int>(threadIdx.x) + (8 * i + e) * static_cast<int>(blockDim.x); }
+  __device__ __forceinline__ void load(const View& x, long long row, int dim, int i) {
+    const long long at = row * x.stride;
+    if (x.type == QX_STORAGE_F32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = place(i, e) < dim ? reinterpret_cast<const uint32_t*>(x.data)[at + place(i, e)] : 0;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = place(i, e) < dim ? reinterpret_cast<const uint16_t*>(x.data)[at + place(i, e)] : 0;
     }
   }
-}
+  __device__ __forceinline__ void values(const View& x, float (&v)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = x.type == QX_STORAGE_F32   ? __uint_as_float(w[e])
+             : x.type == QX_STORAGE_F16 ? __half2float(__ushort_as_half(static_cast<uint16_t>(w[e])))
+                                        : __uint_as_float(w[e] << 16);
+    }
+  }
+  static __device__ __forceinline__ void store(const View& y, long long row, int dim, int i, const float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (place(i, e) < dim) store_one(y.data, y.type, row * y.stride + place(i, e), v[e]);
+    }
+  }
+};
 
 // The sum over the threads of a row, the same for each of them; `shared` is this sum's own.
 __device__ __forceinline__ float row_sum(float v, float* shared) {
@@ -92,43 +103,36 @@ __device__ __forceinline__ float row_sum(float v, float* shared) {
   const int lane = threadIdx.x & 31;
   v = lane < warps ? own[lane] : 0.0f;
 #pragma unroll
-  for (int h = 8; h > 0; h >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, h);
+  for (int h = kRowWarps / 2; h > 0; h >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, h);
   return __shfl_sync(0xFFFFFFFFu, v, 0);
 }
 
-constexpr int kSums = 4, kRowWarps = kNormThreads / 32;
-constexpr int kEarly = 2;  // vectors a thread, up to which every operand is loaded ahead
-
-// A thread's vectors lie blockDim.x vectors apart.
-template <int kVectors>
+// `Weight`: how weight and bias are read.
+template <int kVectors, class Weight>
 __device__ __forceinline__ void normalise(const NormParams& n, float inverse_dim, int dim, float (&v)[kVectors][8],
                                           float (*shared)[kRowWarps]) {
-  constexpr int kHeld = kVectors <= kEarly ? kVectors : 1;
-  Words weight[kHeld], bias[kHeld];
-  const auto place = [](int i) { return (static_cast<int>(threadIdx.x) + i * static_cast<int>(blockDim.x)) * 8; };
-  const auto load = [&](int i, int held) {
-    const int d = place(i), count = min(8, dim - d);
-    if (n.weight.data != nullptr && count > 0) weight[held] = load_words(n.weight, 0, d, count);
-    if (n.bias.data != nullptr && count > 0) bias[held] = load_words(n.bias, 0, d, count);
+  constexpr bool kHeld = kVectors <= 4;  // (ahead of the sums, where there are registers for them)
+  Weight weight[kVectors], bias[kVectors];
+  const auto load = [&](int i) {
+    if (n.weight.data != nullptr) weight[i].load(n.weight, 0, dim, i);
+    if (n.bias.data != nullptr) bias[i].load(n.bias, 0, dim, i);
   };
-  if (kVectors <= kEarly) {
+  if (kHeld) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) load(i, i);
+    for (int i = 0; i < kVectors; ++i) load(i);
   }
-  float mean = 0.0f;
   if (n.layer) {
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
       sum += ((v[i][0] + v[i][1]) + (v[i][2] + v[i][3])) + ((v[i][4] + v[i][5]) + (v[i][6] + v[i][7]));
     }
-    mean = row_sum(sum, shared[0]) * inverse_dim;
+    const float mean = row_sum(sum, shared[0]) * inverse_dim;
     // (places behind the row's end stay zeros, here and in the next norm)
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
-      const int count = dim - place(i);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] -= e < count ? mean : 0.0f;
+      for (int e = 0; e < 8; ++e) v[i][e] -= Weight::place(i, e) < dim ? mean : 0.0f;
     }
   }
   float squares = 0.0f;
@@ -142,81 +146,73 @@ __device__ __forceinline__ void normalise(const NormParams& n, float inverse_dim
   const float factor = 1.0f / sqrtf(row_sum(squares, shared[1]) * inverse_dim + n.eps);
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    if (place(i) >= dim) continue;
-    const int held = kVectors <= kEarly ? i : 0;
-    if (kVectors > kEarly) load(i, held);
+    if (!kHeld) load(i);
     float w[8], b[8];
-    if (n.weight.data != nullptr) values_of(weight[held % kHeld], w);
-    if (n.bias.data != nullptr) values_of(bias[held % kHeld], b);
+    if (n.weight.data != nullptr) weight[i].values(n.weight, w);
+    if (n.bias.data != nullptr) bias[i].values(n.bias, b);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = v[i][e] * factor;
-      v[i][e] = n.weight.data != nullptr ? x * (w[e] + n.offset) : x;
-      if (n.bias.data != nullptr) v[i][e] += b[e];
+      float x = v[i][e] * factor;
+      if (n.weight.data != nullptr) x *= w[e] + n.offset;
+      if (n.bias.data != nullptr) x += b[e];
+      v[i][e] = Weight::place(i, e) < dim ? x : 0.0f;
     }
   }
 }
 
-template <int kVectors>
-__global__ void __launch_bounds__(kNormThreads) residual_norm_kernel(const __grid_constant__ JoinParams p) {
+// `Stream`: how residual and joined are read and written; `Block`: block, gate and normed.
+template <int kVectors, class Stream, class Block, class Weight>
+__global__ void __launch_bounds__(kNormThreads, kVectors == 2 && !Stream::kEach ? 2 : 1) residual_norm_kernel(const __grid_constant__ JoinParams p) {
   __shared__ float sums[kSums][kRowWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const long long row = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
-  const bool there = row < p.tokens;  // (all threads reach the barriers)
-  const auto place = [](int i) { return (static_cast<int>(threadIdx.x) + i * static_cast<int>(blockDim.x)) * 8; };
-  constexpr int kHeld = kVectors <= kEarly ? kVectors : 1;
-  Words block[kVectors], residual[kHeld], gate[kHeld];
-  const auto load = [&](int i, int held) {
-    const int d = place(i), count = min(8, p.dim - d);
-    if (!there || count <= 0) return;
-    if (p.residual.data != nullptr) residual[held] = load_words(p.residual, row, d, count);
-    if (p.gate.data != nullptr) gate[held] = load_words(p.gate, row, d, count);
+  const int dim = row < p.tokens ? p.dim : 0;  // (all threads reach the barriers)
+  constexpr bool kHeld = kVectors <= 4;        // (else there are registers for one operand at a time)
+  Block block[kVectors], gate[kVectors];
+  Stream residual[kVectors];
+  const auto load = [&](int i) {
+    if (p.residual.data != nullptr) residual[i].load(p.residual, row, dim, i);
+    if (p.gate.data != nullptr) gate[i].load(p.gate, row, dim, i);
   };
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    const int d = place(i), count = min(8, p.dim - d);
-    if (there && count > 0 && p.block.data != nullptr) block[i] = load_words(p.block, row, d, count);
-    if (kVectors <= kEarly) load(i, i % kHeld);
+    if (p.block.data != nullptr) block[i].load(p.block, row, dim, i);
+    if (kHeld) load(i);
   }
   float v[kVectors][8];
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
-    if (p.block.data != nullptr && there && place(i) < p.dim) values_of(block[i], v[i]);
+    if (p.block.data != nullptr && Block::place(i, 0) < dim) block[i].values(p.block, v[i]);
   }
-  if (p.post.on) normalise<kVectors>(p.post, p.inverse_dim, p.dim, v, sums);
+  if (p.post.on) normalise<kVectors, Weight>(p.post, p.inverse_dim, p.dim, v, sums);
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    const int d = place(i);
-    if (!there || d >= p.dim) continue;
-    const int held = kVectors <= kEarly ? i % kHeld : 0;
-    if (kVectors > kEarly) load(i, held);
+    if (Block::place(i, 0) >= dim) continue;
+    if (!kHeld) load(i);
     if (p.gate.data != nullptr) {
       float g[8];
-      values_of(gate[held], g);
+      gate[i].values(p.gate, g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] *= g[e];
     }
     if (p.residual.data != nullptr) {
       float r[8];
-      values_of(residual[held], r);
+      residual[i].values(p.residual, r);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = p.block.data != nullptr ? fmaf(p.scale, v[i][e], r[e]) : r[e];
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] *= p.scale;
     }
-    if (p.joined.data != nullptr) store_values(p.joined, row, d, min(8, p.dim - d), v[i]);
+    if (p.joined.data != nullptr) Stream::store(p.joined, row, dim, i, v[i]);
   }
   if (!p.pre.on) return;
-  normalise<kVectors>(p.pre, p.inverse_dim, p.dim, v, sums + 2);
+  normalise<kVectors, Weight>(p.pre, p.inverse_dim, p.dim, v, sums + 2);
 #pragma unroll
-  for (int i = 0; i < kVectors; ++i) {
-    const int d = place(i);
-    if (there && d < p.dim) store_values(p.normed, row, d, min(8, p.dim - d), v[i]);
-  }
+  for (int i = 0; i < kVectors; ++i) Block::store(p.normed, row, dim, i, v[i]);
 }
 
 bool aligned(const void* data, int type) { return reinterpret_cast<uintptr_t>(data) % type_bytes(type) == 0; }
@@ -292,10 +288,42 @@ NormParams device_norm(const qx_norm* norm) {
           norm->eps, norm->offset};
 }
 
-template <int kVectors>
-qx_status launch(const JoinParams& p, int threads, int rows, cudaStream_t stream) {
+// The type of those operands that there are; -1: they differ, or are no whole vectors.
+int common_type(const JoinParams& p, std::initializer_list<const View*> views) {
+  int type = -2;
+  for (const View* view : views) {
+    if (view->data == nullptr) continue;
+    if (!view->vector || p.dim % 8 != 0 || (type >= 0 && view->type != type)) return -1;
+    type = view->type;
+  }
+  return type;
+}
+
+template <class Stream, class Block, class Weight>
+qx_status launch(const JoinParams& p, cudaStream_t stream) {
+  // Two vectors a thread: on 64 registers they keep more bytes under way than one or four do (8192 rows of 4096 bf16
+  // elements with 1 | 2 | 4 | 8: 52.4 | 46.9 | 56.1 | 87.8 us; one row 2.1 | 2.3 | 3.2 | 8.1). Single elements take eight
+  // a thread as long as they can (1500 f32 rows of 1153, with 1 | 2 | 4 times eight: 15.5 | 25.4 | 44.1).
+  const int vectors = (p.dim + 7) / 8;
+  int each = vectors <= 32 || Stream::kEach ? 1 : 2;
+  while (each * kNormThreads < vectors) each *= 2;
+  const int threads = ((vectors + each - 1) / each + 31) / 32 * 32;
+  const int rows = std::max(1, 128 / threads);
   const long long grid = (p.tokens + rows - 1) / rows;
-  return launch_behind(residual_norm_kernel<kVectors>, grid, dim3(threads, rows), 0, stream, p);
+  const dim3 block(threads, rows);
+  switch (each) {
+    case 1: return launch_behind(residual_norm_kernel<1, Stream, Block, Weight>, grid, block, 0, stream, p);
+    case 2: return launch_behind(residual_norm_kernel<2, Stream, Block, Weight>, grid, block, 0, stream, p);
+    case 4: return launch_behind(residual_norm_kernel<4, Stream, Block, Weight>, grid, block, 0, stream, p);
+    default: return launch_behind(residual_norm_kernel<8, Stream, Block, Weight>, grid, block, 0, stream, p);
+  }
+}
+template <int kStream, int kBlock>
+qx_status launch_typed(const JoinParams& p, int weight, cudaStream_t stream) {
+  if (weight == QX_STORAGE_F32) {
+    return launch<InVectors<kStream>, InVectors<kBlock>, InVectors<QX_STORAGE_F32>>(p, stream);
+  }
+  return launch<InVectors<kStream>, InVectors<kBlock>, InVectors<kBlock>>(p, stream);
 }
 
 qx_status launch_residual_norm(const qx_rows* residual, const qx_rows* block, const qx_norm* post, const qx_rows* gate,
@@ -314,17 +342,23 @@ qx_status launch_residual_norm(const qx_rows* residual, const qx_rows* block, co
   p.inverse_dim = 1.0f / dim;
   p.tokens = tokens;
   p.dim = dim;
-  const int vectors = (dim + 7) / 8;
-  int each = 1;
-  while (each * kNormThreads < vectors) each *= 2;
-  const int threads = ((vectors + each - 1) / each + 31) / 32 * 32;
-  const int rows = std::max(1, 256 / threads);
-  switch (each) {
-    case 1: return launch<1>(p, threads, rows, stream);
-    case 2: return launch<2>(p, threads, rows, stream);
-    case 4: return launch<4>(p, threads, rows, stream);
-    default: return launch<8>(p, threads, rows, stream);
+  // Types that go together: the stream's own or f32, the blocks' own, weights of the blocks' type or f32.
+  int s = common_type(p, {&p.residual, &p.joined}), b = common_type(p, {&p.block, &p.gate, &p.normed});
+  int w = common_type(p, {&p.post.weight, &p.post.bias, &p.pre.weight, &p.pre.bias});
+  if (b == -2) b = s;
+  if (s == -2) s = b;
+  if (w == -2) w = b;
+  if (s >= 0 && b >= 0 && (s == b || s == QX_STORAGE_F32) && (w == b || w == QX_STORAGE_F32)) {
+    constexpr int kF32 = QX_STORAGE_F32, kF16 = QX_STORAGE_F16, kBf16 = QX_STORAGE_BF16;
+    if (b == kF32) return launch_typed<kF32, kF32>(p, w, stream);
+    if (b == kF16) {
+      return s == kF16 ? launch_typed<kF16, kF16>(p, w, stream)
+                       : launch_typed<kF32, kF16>(p, w, stream);
+    }
+    return s == kBf16 ? launch_typed<kBf16, kBf16>(p, w, stream)
+                      : launch_typed<kF32, kBf16>(p, w, stream);
   }
+  return launch<InElements, InElements, InElements>(p, stream);
 }
 
 Runs runs_of(const qx_rows* view, long long tokens, long long dim) {
