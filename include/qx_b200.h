@@ -758,6 +758,48 @@ QX_API qx_status qx_residual_norm_dev(const qx_rows* residual, const qx_rows* bl
                                       const qx_rows* gate, float scale, const qx_rows* joined, const qx_norm* pre,
                                       const qx_rows* normed, long long tokens, long long dim, void* stream);
 
+/* ---- a mixture-of-experts feed-forward layer, for few tokens -----------------------------------
+ *   l = x W^T,  s = softmax(l) over all experts or sigmoid(l)
+ *   chosen: the `top` experts of the largest l, or of the largest s + bias where there is one; of equal ones the lower
+ *   w = scale * s (/ the sum of the chosen ones' s),   out = sum of w_e y_e over the chosen + sum of y_e over the shared
+ *   y_e = down_e (activation(gate_e x) * (up_e x))
+ * with GGUF q8_0 or q4_0 blocks for gate, up and down: [experts + shared][inner][dim], the same, and
+ * [experts + shared][dim][inner], the shared experts behind the others. dim and inner are multiples of 32 up to 65536,
+ * experts 1 .. 512, shared 0 .. 32. The weights are copied to the device (or, `_dev`, taken from there) and laid out
+ * for the kernels, as many bytes as they come in; the sources are not used afterwards (`_dev`: once `stream` has come that far). */
+typedef struct qx_moe qx_moe;
+QX_API qx_status qx_moe_prepare(int format, const void* gate, const void* up, const void* down, int experts, int shared,
+                                long long dim, long long inner, qx_moe** out);
+QX_API qx_status qx_moe_prepare_dev(int format, const void* gate_dev, const void* up_dev, const void* down_dev, int experts,
+                                    int shared, long long dim, long long inner, void* stream, qx_moe** out);
+QX_API void qx_moe_destroy(qx_moe* moe);
+enum { QX_MOE_SOFTMAX = 0, QX_MOE_SIGMOID = 1 };
+typedef struct qx_moe_router {
+  const void* weights;     /* [experts][dim], one row behind the other */
+  int type;                /* of weights: QX_STORAGE_* */
+  int top;                 /* 1 .. 32 */
+  const float* bias;       /* [experts], for the choice only; NULL: none */
+  int score;               /* QX_MOE_SOFTMAX or QX_MOE_SIGMOID */
+  int normalise;           /* non-zero: the chosen weights sum up to `scale` */
+  float scale;
+} qx_moe_router;
+/* x and out: [tokens][dim], each with a type of its own; out is x itself, the same view of it, or lies elsewhere.
+ * `chosen` and `weights` (either may be NULL) receive the experts and their w, [tokens][top], largest first. `activation`
+ * is QX_ACTIVATION_*. Any number of tokens is served, in passes of 128; the kernels are made for few, whose experts' weights
+ * are read once per 16 tokens (8 of f32).
+ * Precision. Logits are summed up in 64 bits from sums of eight f32 products, scores and weights of the router are taken in
+ * 64 bits. Codes are used as they are; activations as f16 under a power of two per 32 elements: 16-bit ones exactly (an
+ * element below 2^-37 of its block's largest loses bits), f32 ones to 2^-22, the products of gate and up to 2^-11 of themselves for
+ * 16-bit x and 2^-22 for f32 x (no finer than 2^-38 of their block's largest, nor than 2^-135). Sums are f32, out is rounded once. A token's bits
+ * do not depend on the other tokens. A token that holds a NaN or an infinity spoils its own output only.
+ * What lies between the kernels is in `workspace`, one of the current device (NULL: the library's default one); calls
+ * that may run at the same time need one each. */
+QX_API qx_status qx_moe_apply(const qx_moe* moe, const qx_moe_router* router, const qx_rows* x, const qx_rows* out,
+                              long long tokens, int activation, int32_t* chosen, float* weights);
+QX_API qx_status qx_moe_apply_dev(const qx_moe* moe, const qx_moe_router* router, const qx_rows* x, const qx_rows* out,
+                                  long long tokens, int activation, int32_t* chosen_dev, float* weights_dev,
+                                  qx_workspace* workspace, void* stream);
+
 /* ---- threading: set_num_threads / num_threads, include/quixicore_cpu/threading.h:11-12.
  * The fork-join pool is replaced by CUDA streams; these are kept so callers link. The
  * value is stored and returned, results never depend on it. */

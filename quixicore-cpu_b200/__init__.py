@@ -132,6 +132,12 @@ class NormView(C.Structure):
                 ("offset", C.c_float)]
 
 
+class MoeRouterView(C.Structure):
+    """qx_moe_router of include/qx_b200.h."""
+    _fields_ = [("weights", _vp), ("type", C.c_int), ("top", C.c_int), ("bias", _vp), ("score", C.c_int),
+                ("normalise", C.c_int), ("scale", C.c_float)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -209,6 +215,11 @@ def _load():
                              C.POINTER(RowsView), C.POINTER(NormView), C.POINTER(RowsView), _ll, _ll],
         "qx_residual_norm_dev": [C.POINTER(RowsView), C.POINTER(RowsView), C.POINTER(NormView), C.POINTER(RowsView),
                                  C.c_float, C.POINTER(RowsView), C.POINTER(NormView), C.POINTER(RowsView), _ll, _ll, _vp],
+        "qx_moe_prepare": [C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, _ll, _ll, C.POINTER(_vp)],
+        "qx_moe_prepare_dev": [C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, _ll, _ll, _vp, C.POINTER(_vp)],
+        "qx_moe_apply": [_vp, C.POINTER(MoeRouterView), C.POINTER(RowsView), C.POINTER(RowsView), _ll, C.c_int, _vp, _vp],
+        "qx_moe_apply_dev": [_vp, C.POINTER(MoeRouterView), C.POINTER(RowsView), C.POINTER(RowsView), _ll, C.c_int, _vp, _vp,
+                             _vp, _vp],
         "qx_peer_alloc": [_sz, C.POINTER(_vp), _vp],
         "qx_peer_open": [_vp, C.POINTER(_vp)],
         "qx_peer_close": [_vp],
@@ -233,6 +244,8 @@ def _load():
     lib.qx_weights_destroy.restype = None
     lib.qx_canonical_destroy.argtypes = [_vp]
     lib.qx_canonical_destroy.restype = None
+    lib.qx_moe_destroy.argtypes = [_vp]
+    lib.qx_moe_destroy.restype = None
     lib.qx_workspace_destroy.argtypes = [_vp]
     lib.qx_workspace_destroy.restype = None
     lib.qx_workspace_capacity.argtypes = [_vp]
@@ -947,3 +960,83 @@ def residual_norm_dev(residual, block, joined, normed=None, pre=None, post=None,
     """The same over tensors on the current device, on torch's current stream."""
     return lib.qx_residual_norm_dev(*_residual_norm(_device(), residual, block, joined, normed, pre, post, gate, scale),
                                     _stream())
+
+
+# ---- mixture-of-experts layers ----
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+
+
+class Router:
+    """A layer's router (qx_moe_router) over weights [experts, dim] and bias [experts] f32 or None, tensors on the device
+    or numpy arrays (uint16 bits need `storage`); they are kept alive."""
+
+    def __init__(self, weights, top, score=SCORE_SOFTMAX, bias=None, normalise=True, scale=1.0, storage=None):
+        self.arrays = (weights, bias)
+        host = isinstance(weights, np.ndarray)
+        self.experts, self.dim = weights.shape
+        self.device = -1 if host else weights.get_device()
+        assert (weights.flags["C_CONTIGUOUS"] if host else weights.is_contiguous() and self.device >= 0), "need contiguous weights"
+        kind = _numpy_kind(weights, storage) if host else (_torch_types or _fill_torch_types())[weights.dtype]
+        assert bias is None or bias.shape == (self.experts,), "need a bias for every expert"
+        self.view = MoeRouterView(weights.ctypes.data if host else weights.data_ptr(), kind, top,
+                                  _array(bias, "float32", None if host else self.device), score, 1 if normalise else 0, scale)
+
+
+class Experts:
+    """The prepared experts of a layer (qx_moe), their weights laid out on the device."""
+
+    def __init__(self):
+        self.handle = None
+
+    def _prepare(self, call, address, fmt, gate, up, down, experts, dim, inner, shared, *stream):
+        self.reset()
+        count, block = experts + shared, BLOCK_BYTES.get(fmt, 1)
+        for a, rows, columns in ((gate, inner, dim), (up, inner, dim), (down, dim, inner)):
+            size = a.size if isinstance(a, np.ndarray) else a.numel()
+            assert a.itemsize == 1 and size == count * rows * (columns // 32) * block, "need the blocks of every expert, as bytes"
+        handle = _vp()
+        status = call(fmt, address(gate), address(up), address(down), experts, shared, dim, inner, *stream, C.byref(handle))
+        if status == OK:
+            self.handle, self.experts, self.dim = handle.value, experts, dim
+        return status
+
+    def prepare(self, fmt, gate, up, down, experts, dim, inner, shared=0) -> int:
+        """GGUF blocks [experts + shared, inner, dim] (gate, up) and [experts + shared, dim, inner] (down) as bytes."""
+        return self._prepare(lib.qx_moe_prepare, _np, fmt, gate, up, down, experts, dim, inner, shared)
+
+    def prepare_dev(self, fmt, gate, up, down, experts, dim, inner, shared=0) -> int:
+        device = _device()
+        assert all(t.get_device() == device for t in (gate, up, down)), "need tensors on the current device"
+        return self._prepare(lib.qx_moe_prepare_dev, _dev, fmt, gate, up, down, experts, dim, inner, shared, _stream())
+
+    @property
+    def ready(self) -> bool:
+        return self.handle is not None
+
+    def reset(self) -> None:
+        if self.handle is not None:
+            lib.qx_moe_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        if getattr(self, "handle", None) is not None and lib is not None:
+            self.reset()
+
+    def _operands(self, device, router, x, out, chosen, weights, storage=None):
+        tokens = x.shape[0]
+        assert router.device == device and (not self.ready or (router.experts, router.dim) == (self.experts, self.dim)
+                                            ), "a router of another size or device"
+        where = None if device < 0 else device
+        return (self.handle, router.view, _row_view(x, tokens, router.dim, device, storage),
+                _row_view(out, tokens, router.dim, device, storage), tokens), (
+                    _array(chosen, "int32", where, tokens, router.view.top), _array(weights, "float32", where, tokens, router.view.top))
+
+    def apply(self, router, x, out, activation=ACT_SILU, chosen=None, weights=None, storage=None) -> int:
+        """numpy arrays [tokens, dim]; chosen int32 and weights f32 [tokens, top], or None."""
+        operands, picks = self._operands(-1, router, x, out, chosen, weights, storage)
+        return lib.qx_moe_apply(*operands, activation, *picks)
+
+    def apply_dev(self, router, x, out, activation=ACT_SILU, chosen=None, weights=None, workspace=None) -> int:
+        """Tensors on the current device, torch's current stream."""
+        operands, picks = self._operands(_device(), router, x, out, chosen, weights)
+        return lib.qx_moe_apply_dev(*operands, activation, *picks, workspace, _stream())

@@ -22,6 +22,10 @@ struct Runs {
   }
   bool gapless() const { return extent() == static_cast<size_t>(rows) * heads * bytes; }
 };
+inline Runs runs_of(const qx_rows* view, long long tokens, long long dim) {
+  const size_t size = type_bytes(view->type);
+  return {tokens, 1, view->stride * size, 0, dim * size};
+}
 // Host arrays that a call uses, laid out one behind the other in the context's staging memory. What comes back is
 // the elements of the views that are written, run by run: between them may lie another view's, or what is none of
 // the call's business.

@@ -282,6 +282,8 @@ inline size_t type_bytes(int type) { return type == QX_STORAGE_F32 ? 4 : 2; }
 // Shape, type and pointer of a view; `rows` tokens of `dim` elements, written to or only read.
 qx_status check_heads(const qx_heads* view, long long rows, int dim, bool written);
 qx_status check_cache(const qx_kv_cache* cache);
+// The same of rows of `dim` elements; NULL is fine.
+qx_status check_rows(const qx_rows* view, long long tokens, long long dim, bool written);
 qx_status check_batch(const qx_kv_cache* cache, const qx_kv_batch* batch);
 qx_status check_rope(const qx_rope* rope, int dim);
 // The queries of a batch, at positions[row] or, with positions NULL, at their places in their sequences.

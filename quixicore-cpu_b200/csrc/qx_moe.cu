@@ -1,0 +1,1100 @@
+// A mixture-of-experts layer for few tokens, in two kernels: the router, and the experts' products.
+//
+//   l = x Wr^T, s = softmax(l) or sigmoid(l); the `top` experts of the largest l (or s + bias); weights s, normalised
+//   y = sum over the chosen e of w_e down_e (act(gate_e x) * (up_e x)), and over the shared experts with weight 1
+//
+// What bounds it is the reading of the touched experts' blocks, once: 18 or 34 bytes per 32 weights. Everything else is
+// arranged around keeping those loads under way from the first to the last.
+//
+// Router (moe_router_kernel). Logits are sums of at most eight f32 products at a time, added up in 64 bits: two experts
+// on both sides of the choice are told apart as far as the inputs' own products are. A warp takes two experts and eight tokens and a
+// quarter of the columns. The last CTA to finish eight tokens chooses their experts, a warp per token; the last of those
+// sorts all (token, expert) pairs by expert. Beside them, other CTAs turn the activations into f16 terms.
+//
+// Experts (moe_experts_kernel). Work is cut into units that CTAs draw as tickets, in this order:
+//   up       64 rows (32 of gate, the same 32 of up) of one expert, for up to 16 columns: tokens of it, times terms
+//   down     64 rows of the down projection of one expert, once all of its up units are done
+//   combine  1024 elements of one token's output, once all down units are done
+// A ticket only waits for smaller ones, which their CTAs have begun: no CTA has to be resident for another to go on. A
+// warp that copies runs ahead of eight that multiply through a ring of stages, across units, and calls a unit's weights
+// into L2 before it waits for what the unit depends on.
+//
+// Products. Warp-level f16 MMAs with the weights as the operand of 16 rows: codes are exact in f16 (a nibble is ORed into
+// the mantissa of 1024, a byte permuted there), and one MMA pair takes a block of 32 columns, whose sum is multiplied by
+// the block's scale d and the activations' in f32. Activations are f16 under a power of two per 32 columns: 16-bit inputs
+// exactly (bar elements below 2^-37 of their block's largest), f32 inputs as two terms, hi + lo (22 bits). The product of
+// gate and up is rounded the same way: to 2^-11 of itself for 16-bit inputs (no further than their own rounding, and `inner` such errors of random signs are
+// summed up), 2^-22 for f32 ones. Two terms of a token are
+// two columns, so up to eight columns cost nothing: the MMA has them anyway.
+//
+// A row's bits do not depend on the other tokens: columns are independent, and every sum has a fixed order.
+//
+// Every wait is bounded (two seconds); one that runs out raises the CTA's abort flag, is reported, and the copies in flight are
+// waited for (bounded).
+
+#include <algorithm>
+#include <cmath>
+
+#include "qx_host_arrays.cuh"
+#include "qx_moe.cuh"
+#include "qx_scaled_gemm.cuh"
+#include "qx_tile_pipe.cuh"
+
+namespace qx {
+namespace moe {
+namespace {
+
+using namespace sm100;
+
+// ---- preparation -----------------------------------------------------------------------------
+// One warp per record.
+template <int kFormat>
+__global__ void __launch_bounds__(256) moe_relayout_kernel(const uint8_t* __restrict__ first, const uint8_t* __restrict__ second,
+                                                           uint8_t* __restrict__ to, long long tiles, int blocks) {
+  constexpr int kBlock = kFormat == QX_FORMAT_Q4_0 ? 18 : 34, kRecord = record_bytes(kFormat);
+  const long long record = blockIdx.x * 8LL + threadIdx.x / 32;
+  if (record >= tiles * blocks) return;
+  const long long tile = record / blocks;
+  const int block = static_cast<int>(record - tile * blocks), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* const out = to + record * kRecord;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    // interleaved: rows g of both matrices; else rows g and g + 8 of one
+    const uint8_t* const matrix = h == 0 || second == nullptr ? first : second;
+    const long long row = second == nullptr ? tile * 16 + 8 * h + g : tile * 8 + g;
+    const uint8_t* const from = matrix + (row * blocks + block) * kBlock;
+    if (kFormat == QX_FORMAT_Q4_0) {
+      uint32_t word = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // element 8 t + i: pairs 2 p, 2 p + 1 become nibbles p, p + 4
+        const int e = 8 * t + i;
+        const uint32_t byte = from[2 + (e & 15)], nibble = e < 16 ? byte & 15 : byte >> 4;
+        word |= nibble << (4 * (i >> 1) + 16 * (i & 1));
+      }
+      reinterpret_cast<uint32_t*>(out)[2 * lane + h] = word;
+    } else {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) word |= static_cast<uint32_t>(from[2 + 8 * t + 4 * w + i] ^ 0x80) << (8 * i);
+        reinterpret_cast<uint32_t*>(out)[4 * lane + 2 * h + w] = word;  // code + 128
+      }
+    }
+    if (t == 0) {
+      reinterpret_cast<uint16_t*>(out + kRecord - 32)[2 * g + h] = static_cast<uint16_t>(from[0] | from[1] << 8);
+    }
+  }
+}
+
+// ---- router ------------------------------------------------------------------------------------
+constexpr int kRouterTokens = 8, kRouterExperts = 4, kRouterSplits = 4, kRouterThreads = 256;
+
+// Eight neighbouring elements as they lie in memory; off 16-byte boundaries as f32.
+struct Words {
+  uint4 w[2];
+  __device__ __forceinline__ void load(const uint8_t* data, int type, int vector, long long index) {
+    if (!vector) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = kv::load_one(data, type, index + i);
+      kv::to_words<QX_STORAGE_F32>(v, w);
+    } else {
+      const uint4* const from = reinterpret_cast<const uint4*>(data + index * (type == QX_STORAGE_F32 ? 4 : 2));
+      w[0] = from[0];
+      if (type == QX_STORAGE_F32) w[1] = from[1];
+    }
+  }
+  __device__ __forceinline__ void values(int type, int vector, float (&v)[8]) const {
+    const uint4 narrow[1] = {w[0]};
+    if (!vector || type == QX_STORAGE_F32) kv::from_words<QX_STORAGE_F32>(w, v);
+    else if (type == QX_STORAGE_F16) kv::from_words<QX_STORAGE_F16>(narrow, v);
+    else kv::from_words<QX_STORAGE_BF16>(narrow, v);
+  }
+};
+
+__device__ __forceinline__ uint32_t pair_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+// {factor, inverse} that bring the largest magnitude of a block (as f32 bits) to 2^13 .. 2^14.
+__device__ __forceinline__ float2 block_factor(uint32_t top) {
+  const int exponent = max(30, static_cast<int>(top >> 23));
+  return make_float2(__uint_as_float(static_cast<uint32_t>(267 - exponent) << 23),
+                     __uint_as_float(static_cast<uint32_t>(exponent - 13) << 23));
+}
+
+// A warp turns 128 columns of a token into terms.
+__device__ __forceinline__ void convert_slab(const Params& p, int token, int slab) {
+  const int lane = threadIdx.x & 31, d = slab * 128 + lane * 4;
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (d < p.dim) kv::load4(p.x, p.x_type, p.x_vector, token * p.x_stride + d, v);
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int h = 1; h < 8; h <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, h));
+  const float2 factor = block_factor(top);
+  for (int term = 0; term < p.terms; ++term) {
+    uint8_t* const to = p.x_terms + (static_cast<long long>(token * p.terms + term) * slabs_of(p.dim) + slab) * kSlabBytes;
+    __half2 h[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (term == 0) {
+        v[2 * e] *= factor.x;
+        v[2 * e + 1] *= factor.x;
+      }
+      h[e] = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+      const float2 back = __half22float2(h[e]);
+      v[2 * e] -= back.x;
+      v[2 * e + 1] -= back.y;
+    }
+    *reinterpret_cast<uint2*>(to + lane * 8) = make_uint2(pair_bits(h[0]), pair_bits(h[1]));
+    if ((lane & 7) == 0) *reinterpret_cast<float*>(to + 256 + lane / 8 * 4) = factor.y;
+  }
+}
+
+// Order-preserving whole number of a double; NaN is above everything.
+__device__ __forceinline__ unsigned long long ordered(double v) {
+  const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(v));
+  if (v != v) return ~0ull;
+  return bits >> 63 ? ~bits : bits | 1ull << 63;
+}
+
+// A warp chooses a token's experts. kEach: experts per lane, expert = lane + 32 i.
+template <int kEach>
+__device__ __forceinline__ void choose(const Params& p, int token) {
+  const int lane = threadIdx.x & 31, places = p.top + p.shared;
+  const double* const logits = p.logits + static_cast<long long>(token) * p.experts;
+  double logit[kEach], largest = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = lane + 32 * i;
+    logit[i] = e < p.experts ? __ldcg(logits + e) : -INFINITY;
+    largest = fmax(largest, logit[i]);
+  }
+  double score[kEach], total = 0.0;
+  if (p.score == QX_MOE_SOFTMAX) {
+#pragma unroll
+    for (int h = 16; h > 0; h >>= 1) largest = fmax(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, h));
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      score[i] = 0.0;
+      if (lane + 32 * i < p.experts) score[i] = exp(logit[i] - largest);
+      total += score[i];
+    }
+#pragma unroll
+    for (int h = 16; h > 0; h >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, h);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) score[i] = 1.0 / (1.0 + exp(-logit[i]));
+    total = 1.0;
+  }
+  unsigned long long key[kEach];
+  uint32_t left = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = lane + 32 * i;
+    key[i] = 0;
+    if (e < p.experts) {
+      left |= 1u << i;
+      key[i] = ordered(p.bias == nullptr ? logit[i] : score[i] / total + static_cast<double>(p.bias[e]));
+    }
+  }
+  double mine = 0.0, sum = 0.0;  // of the place that is this lane's
+  int expert = 0;
+  for (int place = 0; place < p.top; ++place) {
+    // the largest key left, of the lowest expert where it is there twice
+    unsigned long long best = 0;
+    int at = -1;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if ((left >> i & 1) && (at < 0 || key[i] > best)) {
+        best = key[i];
+        at = i;
+      }
+    }
+    const uint32_t high = __reduce_max_sync(0xFFFFFFFFu, at < 0 ? 0 : static_cast<uint32_t>(best >> 32));
+    const bool still = at >= 0 && static_cast<uint32_t>(best >> 32) == high;
+    const uint32_t low = __reduce_max_sync(0xFFFFFFFFu, still ? static_cast<uint32_t>(best) : 0);
+    const bool mine_is = still && static_cast<uint32_t>(best) == low;
+    const uint32_t chosen = __reduce_min_sync(0xFFFFFFFFu, mine_is ? static_cast<uint32_t>(lane + 32 * at) : 0x7FFFFFFFu);
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (chosen == static_cast<uint32_t>(lane + 32 * i)) {
+        s = score[i];
+        left &= ~(1u << i);
+      }
+    }
+    s = __shfl_sync(0xFFFFFFFFu, s, chosen & 31);
+    sum += s;
+    if (lane == place) {
+      mine = s;
+      expert = static_cast<int>(chosen);
+    }
+  }
+  if (lane < p.top) {
+    const float weight = static_cast<float>(mine / (p.normalise ? sum : total) * static_cast<double>(p.scale));
+    p.picks[token * places + lane] = expert;
+    p.weights[token * places + lane] = weight;
+    if (p.chosen != nullptr) p.chosen[static_cast<long long>(token) * p.top + lane] = expert;
+    if (p.chosen_weights != nullptr) p.chosen_weights[static_cast<long long>(token) * p.top + lane] = weight;
+  }
+  if (lane < p.shared) {
+    p.picks[token * places + p.top + lane] = p.experts + lane;
+    p.weights[token * places + p.top + lane] = 1.0f;
+  }
+}
+
+constexpr int kAllExperts = kMostExperts + kMostShared, kMaskWords = kPassTokens / 32;
+struct SortSpace {
+  uint32_t tokens[kAllExperts][kMaskWords];  // of each expert
+  int first[kAllExperts], sums[2][kRouterThreads / 32];
+};
+// The CTA sorts (token, expert) pairs by expert and cuts each expert's into groups.
+__device__ __forceinline__ void sort_pairs(const Params& p, SortSpace& s) {
+  const int experts = p.experts + p.shared, places = p.top + p.shared, entries = p.tokens * places;
+  const int most = kColumns / p.terms, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  for (int i = threadIdx.x; i < experts * kMaskWords; i += kRouterThreads) s.tokens[i / kMaskWords][i % kMaskWords] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < entries; i += kRouterThreads) {
+    const int token = i / places;
+    atomicOr(&s.tokens[__ldcg(p.picks + i)][token / 32], 1u << (token & 31));
+  }
+  __syncthreads();
+  // Running numbers of entries and groups in front of each expert, 256 experts at a time.
+  int entries_before = 0, groups_before = 0;
+  for (int e0 = 0; e0 < experts; e0 += kRouterThreads) {
+    const int e = e0 + static_cast<int>(threadIdx.x);
+    int count = 0;
+    if (e < experts) {
+#pragma unroll
+      for (int w = 0; w < kMaskWords; ++w) count += __popc(s.tokens[e][w]);
+    }
+    const int cuts = (count + most - 1) / most;
+    int through = count, cuts_through = cuts;
+#pragma unroll
+    for (int h = 1; h < 32; h <<= 1) {
+      const int a = __shfl_up_sync(0xFFFFFFFFu, through, h), b = __shfl_up_sync(0xFFFFFFFFu, cuts_through, h);
+      if (lane >= h) {
+        through += a;
+        cuts_through += b;
+      }
+    }
+    if (lane == 31) {
+      s.sums[0][warp] = through;
+      s.sums[1][warp] = cuts_through;
+    }
+    __syncthreads();
+    int first = entries_before + through - count, group = groups_before + cuts_through - cuts;
+    for (int w = 0; w < kRouterThreads / 32; ++w) {
+      if (w < warp) {
+        first += s.sums[0][w];
+        group += s.sums[1][w];
+      }
+      entries_before += s.sums[0][w];
+      groups_before += s.sums[1][w];
+    }
+    if (e < experts) {
+      s.first[e] = first;
+      for (int i = 0; i < cuts; ++i) p.groups[group + i] = {e, first + i * most, min(most, count - i * most)};
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < entries; i += kRouterThreads) {
+    const int token = i / places, e = __ldcg(p.picks + i);
+    int rank = __popc(s.tokens[e][token / 32] & ((1u << (token & 31)) - 1));
+    for (int w = 0; w < token / 32; ++w) rank += __popc(s.tokens[e][w]);
+    p.list[s.first[e] + rank] = i;
+  }
+  if (threadIdx.x == 0) p.plan->groups = groups_before;
+}
+
+// The last thread block to arrive at a counter of `all`, which is then zero again.
+__device__ __forceinline__ bool arrives_last(int* counter, int all, int* shared) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = atomicAdd(counter, 1) == all - 1;
+    if (last) *counter = 0;
+    *shared = last;
+  }
+  __syncthreads();
+  if (*shared == 0) return false;
+  __threadfence();
+  return true;
+}
+
+// Grid: [token groups][expert groups] CTAs of the router, then those that convert activations.
+__global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid_constant__ Params p) {
+  __shared__ union {
+    double parts[kRouterSplits][kRouterExperts][kRouterTokens];
+    SortSpace sort;
+  } s;
+  __shared__ int last;
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int token_groups = (p.tokens + kRouterTokens - 1) / kRouterTokens;
+  const int expert_groups = (p.experts + kRouterExperts - 1) / kRouterExperts;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int index = static_cast<int>(blockIdx.x) - token_groups * expert_groups;
+  if (index >= 0) {
+    const int slabs = slabs_of(p.dim), item = index * 8 + warp;
+    if (item < p.tokens * slabs) convert_slab(p, item / slabs, item % slabs);
+    return;
+  }
+  if (blockIdx.x == 0) {
+    const int most = p.tokens * (p.top + p.shared);
+    for (int i = threadIdx.x; i < most; i += kRouterThreads) p.up_done[i] = 0;
+    if (threadIdx.x == 0) p.plan->ticket = p.plan->down_done = 0;
+  }
+  const int token_group = blockIdx.x / expert_groups, expert_group = blockIdx.x % expert_groups;
+  const int token0 = token_group * kRouterTokens, split = warp & (kRouterSplits - 1);
+  const int expert0 = expert_group * kRouterExperts + warp / kRouterSplits * 2;
+  double sum[16];  // [expert of two][token]
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum[i] = 0.0;
+  for (int d = (split * 32 + lane) * 8; d < p.dim; d += kRouterSplits * 256) {
+    Words w[2], x[kRouterTokens];  // (all under way before the first is used)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      w[e].load(p.router, p.router_type, p.router_vector, static_cast<long long>(min(expert0 + e, p.experts - 1)) * p.dim + d);
+    }
+#pragma unroll
+    for (int t = 0; t < kRouterTokens; ++t) {
+      if (token0 + t < p.tokens) x[t].load(p.x, p.x_type, p.x_vector, (token0 + t) * p.x_stride + d);
+    }
+    float a[2][8];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) w[e].values(p.router_type, p.router_vector, a[e]);
+#pragma unroll
+    for (int t = 0; t < kRouterTokens; ++t) {
+      if (token0 + t >= p.tokens) continue;
+      float v[8];
+      x[t].values(p.x_type, p.x_vector, v);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float part = a[e][0] * v[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) part = fmaf(a[e][i], v[i], part);
+        sum[8 * e + t] += static_cast<double>(part);
+      }
+    }
+  }
+  // sixteen sums over 32 lanes: every step halves what a lane holds; lanes 2 i and 2 i + 1 end up with sum i
+#pragma unroll
+  for (int h = 16, n = 8; h > 1; h >>= 1, n >>= 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i >= n) continue;
+      const bool upper = lane & h;
+      const double send = upper ? sum[i] : sum[i + n], keep = upper ? sum[i + n] : sum[i];
+      sum[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, h);
+    }
+  }
+  sum[0] += __shfl_xor_sync(0xFFFFFFFFu, sum[0], 1);
+  if ((lane & 1) == 0) s.parts[split][warp / kRouterSplits * 2 + (lane >> 4)][lane >> 1 & 7] = sum[0];
+  __syncthreads();
+  if (threadIdx.x < kRouterExperts * kRouterTokens) {
+    const int e = threadIdx.x / kRouterTokens, t = threadIdx.x % kRouterTokens;
+    double v = s.parts[0][e][t];
+#pragma unroll
+    for (int i = 1; i < kRouterSplits; ++i) v += s.parts[i][e][t];
+    const int expert = expert_group * kRouterExperts + e;
+    if (expert < p.experts && token0 + t < p.tokens) p.logits[static_cast<long long>(token0 + t) * p.experts + expert] = v;
+  }
+  if (!arrives_last(p.arrivals + token_group, expert_groups, &last)) return;
+  if (token0 + warp < p.tokens) {
+    if (p.experts <= 128) choose<4>(p, token0 + warp);
+    else choose<kMostExperts / 32>(p, token0 + warp);
+  }
+  if (!arrives_last(p.arrivals + kPassTokens / kRouterTokens, token_groups, &last)) return;
+  sort_pairs(p, s.sort);
+}
+
+// ---- experts -----------------------------------------------------------------------------------
+constexpr int kMathWarps = 8, kExpertThreads = 32 * (kMathWarps + 1);
+constexpr int kUnitTiles = 4, kUnitRows = kUnitTiles * kTileRows;
+constexpr int kStageBlocks = 8;                          // columns of a stage, in blocks: two slabs
+constexpr int kColumnBytes = 2 * kSlabBytes + 32;        // between columns: eight lanes of a 16-byte load meet no conflict
+constexpr int kCombineWidth = 1024;
+constexpr int kReduceStride = 2 * 128 + 4;               // floats per warp
+enum { kUp = 0, kDown = 1, kCombine = 2, kExit = 3 };
+
+struct StageInfo {
+  int kind, blocks, last, tiles;
+  int unit, group, count, expert;
+  int entries[kColumns];
+};
+
+template <int kFormat>
+struct ExpertShape {
+  static constexpr int kRecord = record_bytes(kFormat);
+  static constexpr int kStages = kFormat == QX_FORMAT_Q4_0 ? 5 : 3;
+  static constexpr int kTileBytes = kStageBlocks * kRecord;
+  static constexpr int kWeights = kUnitTiles * kTileBytes;
+  static constexpr int kStage = kWeights + kColumns * kColumnBytes;
+  static constexpr int kReduce = kStages * kStage;
+  static constexpr int kInfo = kReduce + kMathWarps * kReduceStride * 4;
+  static constexpr int kBars = kInfo + kStages * static_cast<int>(sizeof(StageInfo));
+  static constexpr int kBytes = kBars + 2 * kStages * 8 + 16;
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// The codes of a lane's columns 8 t .. 8 t + 7 of rows g and g + 8, as f16: operands of the block's two MMAs.
+template <int kFormat>
+struct Codes;
+template <>
+struct Codes<QX_FORMAT_Q4_0> {
+  static __device__ __forceinline__ void load(const uint8_t* record, int lane, uint32_t (&a)[4], uint32_t (&b)[4]) {
+    const uint2 w = *reinterpret_cast<const uint2*>(record + lane * 8);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t low = h == 0 ? w.x : w.y, high = low >> 8;
+      const auto even = [](uint32_t v) {  // 1024 + n - 1032
+        const uint32_t raw = (v & 0x000F000Fu) | 0x64006400u;
+        return pair_bits(__hsub2(*reinterpret_cast<const __half2*>(&raw), __half2half2(__ushort_as_half(0x6408))));
+      };
+      const auto odd = [](uint32_t v) {  // (1024 + 16 n) / 16 - 72
+        const uint32_t raw = (v & 0x00F000F0u) | 0x64006400u;
+        return pair_bits(__hfma2(*reinterpret_cast<const __half2*>(&raw), __half2half2(__ushort_as_half(0x2C00)),
+                                 __half2half2(__ushort_as_half(0xD480))));
+      };
+      a[h] = even(low);
+      a[2 + h] = odd(low);
+      b[h] = even(high);
+      b[2 + h] = odd(high);
+    }
+  }
+};
+template <>
+struct Codes<QX_FORMAT_Q8_0> {
+  static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t select) {  // 1024 + (code + 128) - 1152
+    const uint32_t raw = __byte_perm(w, 0x64646464u, select);
+    return pair_bits(__hsub2(*reinterpret_cast<const __half2*>(&raw), __half2half2(__ushort_as_half(0x6480))));
+  }
+  static __device__ __forceinline__ void load(const uint8_t* record, int lane, uint32_t (&a)[4], uint32_t (&b)[4]) {
+    const uint4 w = *reinterpret_cast<const uint4*>(record + lane * 16);
+    a[0] = pair(w.x, 0x4140);
+    a[1] = pair(w.z, 0x4140);
+    a[2] = pair(w.x, 0x4342);
+    a[3] = pair(w.z, 0x4342);
+    b[0] = pair(w.y, 0x4140);
+    b[1] = pair(w.w, 0x4140);
+    b[2] = pair(w.y, 0x4342);
+    b[3] = pair(w.w, 0x4342);
+  }
+};
+
+using F32x2 = unsigned long long;
+__device__ __forceinline__ F32x2 both(float v) { return tile::pack2(__float_as_uint(v), __float_as_uint(v)); }
+__device__ __forceinline__ F32x2 pair_of(float a, float b) { return tile::pack2(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ F32x2 mul2(F32x2 a, F32x2 b) {
+  F32x2 v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+
+// A warp's blocks of a stage: 16 rows x 8 kN columns, sums in `total` [column tile][row g, row g + 8].
+template <int kFormat, int kN>
+__device__ __forceinline__ void multiply(const uint8_t* records, const uint8_t* columns, int blocks, F32x2 (&total)[2][2]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float scales[kN][2][4];  // of columns 2 t, 2 t + 1 and the slab's four blocks
+#pragma unroll
+  for (int n = 0; n < kN; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float4 f = *reinterpret_cast<const float4*>(columns + (8 * n + 2 * t + e) * kColumnBytes + 256);
+      scales[n][e][0] = f.x;
+      scales[n][e][1] = f.y;
+      scales[n][e][2] = f.z;
+      scales[n][e][3] = f.w;
+    }
+  }
+  const auto block = [&](int b) {
+    const uint8_t* const record = records + b * record_bytes(kFormat);
+    uint32_t a0[4], a1[4];
+    Codes<kFormat>::load(record, lane, a0, a1);
+    const float2 d = __half22float2(reinterpret_cast<const __half2*>(record + record_bytes(kFormat) - 32)[g]);
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const uint4 x = *reinterpret_cast<const uint4*>(columns + (8 * n + g) * kColumnBytes + b * 64 + t * 16);
+      float sum[4];
+      mma_f16_first(sum, a0, x.x, x.y);
+      mma_f16(sum, a1, x.z, x.w);
+      const F32x2 s = pair_of(scales[n][0][b], scales[n][1][b]);
+      tile::fma2(total[n][0], pair_of(sum[0], sum[1]), mul2(s, both(d.x)));
+      tile::fma2(total[n][1], pair_of(sum[2], sum[3]), mul2(s, both(d.y)));
+    }
+  };
+  if (blocks == kSlabBlocks) {
+#pragma unroll
+    for (int b = 0; b < kSlabBlocks; ++b) block(b);
+  } else {
+#pragma unroll
+    for (int b = 0; b < kSlabBlocks; ++b) {
+      if (b < blocks) block(b);
+    }
+  }
+}
+
+// The math warps meet: barrier 1.
+__device__ __forceinline__ void math_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kMathWarps) : "memory"); }
+
+// What the copying warp reads of other CTAs' results goes through the asynchronous proxy.
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async;" ::: "memory"); }
+
+__device__ __forceinline__ int load_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+// Until *counter >= target; false where the time runs out or the CTA gives up.
+__device__ __forceinline__ bool wait_for_count(const int* counter, int target, volatile int* abort_flag) {
+  if (load_acquire(counter) >= target) return true;
+  const unsigned long long start = global_timer_ns();
+  for (uint32_t spin = 1;; ++spin) {
+    if (load_acquire(counter) >= target) return true;
+    __nanosleep(32);
+    if ((spin & 63u) == 0u && (*abort_flag != 0 || global_timer_ns() - start > kWaitLimitNs)) return false;
+  }
+}
+
+template <int kFormat, int kTerms>
+__global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __grid_constant__ Params p) {
+  using S = ExpertShape<kFormat>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* const reduce = reinterpret_cast<float*>(smem + S::kReduce);
+  StageInfo* const infos = reinterpret_cast<StageInfo*>(smem + S::kInfo);
+  uint64_t* const full = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* const empty = full + kStages;
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, kMathWarps);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  asm volatile("griddepcontrol.launch_dependents;");
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int up_blocks = p.dim / 32, down_blocks = p.inner / 32;
+  const int up_units = p.inner / 32, down_tiles = p.dim / kTileRows, down_units = (down_tiles + kUnitTiles - 1) / kUnitTiles;
+
+  if (warp == kMathWarps) {
+    // ---- copies ------------------------------------------------------------------------------
+    const int groups = __ldcg(&p.plan->groups);
+    const int combine_chunks = (p.dim + kCombineWidth - 1) / kCombineWidth;
+    const long long ups = static_cast<long long>(groups) * up_units, downs = static_cast<long long>(groups) * down_units;
+    const long long all = ups + downs + static_cast<long long>(p.tokens) * combine_chunks;
+    tile::Ring ring;
+    int issued = 0;  // stages, as far as the ring's size
+    bool ok = true;
+    int next = 0;
+    if (lane == 0) next = atomicAdd(&p.plan->ticket, 1);
+    for (;;) {
+      const long long ticket = __shfl_sync(0xFFFFFFFFu, next, 0);
+      if (lane == 0 && ticket < all) next = atomicAdd(&p.plan->ticket, 1);  // (needed a unit later)
+      const int kind = ticket < ups ? kUp : ticket < ups + downs ? kDown : ticket < all ? kCombine : kExit;
+      int group = 0, unit = 0, blocks = 0, tiles = 0, stages = 1;
+      Group work = {0, 0, 0};
+      const uint8_t* weights = nullptr;
+      const uint8_t* activations = nullptr;
+      int entry = 0, column_row = 0;
+      if (kind == kUp || kind == kDown) {
+        const int units = kind == kUp ? up_units : down_units;
+        const long long at = kind == kUp ? ticket : ticket - ups;
+        group = static_cast<int>(at / units);
+        unit = static_cast<int>(at - static_cast<long long>(group) * units);
+        work.expert = __ldcg(&p.groups[group].expert);
+        work.first = __ldcg(&p.groups[group].first);
+        work.count = __ldcg(&p.groups[group].count);
+        blocks = kind == kUp ? up_blocks : down_blocks;
+        stages = (blocks + kStageBlocks - 1) / kStageBlocks;
+        tiles = kind == kUp ? kUnitTiles : min(kUnitTiles, down_tiles - unit * kUnitTiles);
+        const long long tile0 = static_cast<long long>(work.expert) * (kind == kUp ? p.inner / 8 : down_tiles) + unit * kUnitTiles;
+        weights = (kind == kUp ? p.up : p.down) + tile0 * blocks * S::kRecord;
+        const int column = lane - kUnitTiles;
+        if (column >= 0 && column < work.count * kTerms) {
+          entry = __ldcg(p.list + work.first + column / kTerms);
+          column_row = kind == kUp ? entry / (p.top + p.shared) : entry;
+          activations = (kind == kUp ? p.x_terms : p.inner_terms) +
+                        static_cast<long long>(column_row * kTerms + column % kTerms) * slabs_of(blocks * 32) * kSlabBytes;
+        }
+        if (kind == kDown) {
+          // (the weights on their way to L2 while the unit's activations are waited for)
+          if (lane < tiles) {
+            const uint64_t from = reinterpret_cast<uint64_t>(weights + static_cast<long long>(lane) * blocks * S::kRecord);
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(blocks * S::kRecord));
+          }
+          ok = wait_for_count(p.up_done + group, up_units, abort_flag);
+        }
+      } else if (kind == kCombine) {
+        const int at = static_cast<int>(ticket - ups - downs);
+        group = at / combine_chunks;  // (the token)
+        unit = at - group * combine_chunks;
+        ok = wait_for_count(&p.plan->down_done, static_cast<int>(downs), abort_flag);
+      }
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) {
+        if (lane == 0) report_error(p.error, 51);
+        break;
+      }
+      proxy_fence();
+      for (int stage = 0; stage < stages; ++stage) {
+        ok = issued < kStages || mbar_wait_warp(empty + ring.slot, ring.phase ^ 1u, abort_flag);
+        if (!ok) {
+          if (lane == 0) report_error(p.error, 52);
+          break;
+        }
+        issued = min(issued + 1, kStages);
+        const int in_stage = min(kStageBlocks, blocks - stage * kStageBlocks);
+        const uint32_t column_bytes = (in_stage + kSlabBlocks - 1) / kSlabBlocks * kSlabBytes;
+        StageInfo& info = infos[ring.slot];
+        const int column = lane - kUnitTiles;
+        if (lane == 0) {
+          info.kind = kind;
+          info.blocks = in_stage;
+          info.last = stage == stages - 1;
+          info.tiles = tiles;
+          info.unit = unit;
+          info.group = group;
+          info.count = work.count;
+          info.expert = work.expert;
+        }
+        if (column >= 0 && column < work.count * kTerms && column % kTerms == 0) info.entries[column / kTerms] = entry;
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_expect_tx(full + ring.slot, kind < kCombine ? tiles * in_stage * S::kRecord + work.count * kTerms * column_bytes : 0);
+        }
+        __syncwarp();
+        uint8_t* const to = smem + ring.slot * S::kStage;
+        if (lane < tiles) {
+          tile::bulk_load(to + lane * S::kTileBytes, weights + (static_cast<long long>(lane) * blocks + stage * kStageBlocks) * S::kRecord,
+                          in_stage * S::kRecord, full + ring.slot);
+        } else if (activations != nullptr) {
+          tile::bulk_load(to + S::kWeights + column * kColumnBytes, activations + stage * 2 * kSlabBytes, column_bytes, full + ring.slot);
+        }
+        ring.advance(kStages);
+      }
+      if (!ok || kind == kExit) break;
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      // what is in flight has to land before the CTA's memory is another's: the last use of each stage
+      __syncwarp();
+      const unsigned long long start = global_timer_ns();
+      for (int slot = 0; slot < issued; ++slot) {
+        const uint32_t phase = slot < static_cast<int>(ring.slot) ? ring.phase : ring.phase ^ 1u;
+        while (!mbar_try_wait(full + slot, phase) && global_timer_ns() - start < kWaitLimitNs) {
+        }
+      }
+    }
+    return;
+  }
+
+  // ---- products ------------------------------------------------------------------------------
+  const int g = lane >> 2, t = lane & 3, tile_in_unit = warp >> 1, half = warp & 1;
+  const int inner_slabs = slabs_of(p.inner), places = p.top + p.shared;
+  tile::Ring ring;
+  F32x2 total[2][2] = {{0, 0}, {0, 0}};
+  for (;;) {
+    if (!mbar_wait_warp(full + ring.slot, ring.phase, abort_flag)) {
+      if (threadIdx.x == 0 && *abort_flag == 0) report_error(p.error, 53);
+      *abort_flag = 1;
+      return;  // (the other math warps see the flag, or run into the same wait)
+    }
+    const StageInfo& info = infos[ring.slot];
+    const int kind = info.kind, last = info.last, unit = info.unit, group = info.group, count = info.count;
+    if (kind == kExit) return;
+    const int tiles = info.tiles, entry = lane < count ? info.entries[lane] : 0;
+    if (kind != kCombine && tile_in_unit < tiles) {
+      const uint8_t* const stage = smem + ring.slot * S::kStage;
+      const uint8_t* const records = stage + tile_in_unit * S::kTileBytes + half * kSlabBlocks * S::kRecord;
+      const uint8_t* const columns = stage + S::kWeights + half * kSlabBytes;
+      const int blocks = max(0, min(kSlabBlocks, info.blocks - half * kSlabBlocks));
+      if (count * kTerms <= 8) multiply<kFormat, 1>(records, columns, blocks, total);
+      else multiply<kFormat, 2>(records, columns, blocks, total);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + ring.slot);
+    ring.advance(kStages);
+    if (kind == kCombine) {
+      const int d = unit * kCombineWidth + static_cast<int>(threadIdx.x) * 4;
+      if (d < p.dim) {
+        const float* const from = p.products + static_cast<long long>(group) * places * p.dim + d;
+        const float* const weight = p.weights + group * places;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i0 = 0; i0 < places; i0 += 8) {
+          float4 v[8];
+          float w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (i0 + i >= places) continue;
+            v[i] = __ldcg(reinterpret_cast<const float4*>(from + static_cast<long long>(i0 + i) * p.dim));
+            w[i] = __ldcg(weight + i0 + i);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (i0 + i >= places) continue;
+            sum.x = fmaf(w[i], v[i].x, sum.x);
+            sum.y = fmaf(w[i], v[i].y, sum.y);
+            sum.z = fmaf(w[i], v[i].z, sum.z);
+            sum.w = fmaf(w[i], v[i].w, sum.w);
+          }
+        }
+        const long long to = group * p.out_stride + d;
+        kv::store_one(p.out, p.out_type, to, sum.x);
+        kv::store_one(p.out, p.out_type, to + 1, sum.y);
+        kv::store_one(p.out, p.out_type, to + 2, sum.z);
+        kv::store_one(p.out, p.out_type, to + 3, sum.w);
+      }
+      continue;
+    }
+    if (!last) continue;
+
+    // ---- the unit's sums: two warps per tile -------------------------------------------------
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        uint32_t a, b;
+        tile::unpack2(total[n][r], a, b);
+        reduce[warp * kReduceStride + n * 128 + (2 * r) * 32 + lane] = __uint_as_float(a);
+        reduce[warp * kReduceStride + n * 128 + (2 * r + 1) * 32 + lane] = __uint_as_float(b);
+        total[n][r] = 0;
+      }
+    }
+    math_barrier();
+    // Row g (or g + 8) of a tile for token c: its terms, each from both warps.
+    const auto sum_of = [&](int tile_at, int row, int c) {
+      float v = 0.0f;
+#pragma unroll
+      for (int term = kTerms - 1; term >= 0; --term) {
+        const int column = c * kTerms + term;
+        const float* const at = reduce + 2 * tile_at * kReduceStride + (column >> 3) * 128 +
+                                (2 * (row >> 3) + (column & 1)) * 32 + (row & 7) * 4 + ((column & 7) >> 1);
+        v += at[0] + at[kReduceStride];
+      }
+      return v;
+    };
+    if (kind == kUp) {
+      // a warp takes a token, a lane a column of the inner activations: a block of 32
+      for (int c = warp; c < count; c += kMathWarps) {
+        const float gate = sum_of(lane >> 3, lane & 7, c), up = sum_of(lane >> 3, 8 + (lane & 7), c);
+        float a = projection_activation(gate, p.activation) * up;
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(a) & 0x7FFFFFFFu);
+        const float2 factor = block_factor(top);
+        a *= factor.x;
+        const int row = __shfl_sync(0xFFFFFFFFu, entry, c);
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {
+          uint8_t* const to = p.inner_terms + (static_cast<long long>(row * kTerms + term) * inner_slabs + (unit >> 2)) * kSlabBytes;
+          const __half h = __float2half_rn(a);
+          reinterpret_cast<__half*>(to + (unit & 3) * 64)[lane] = h;
+          a -= __half2float(h);
+          if (lane == 0) reinterpret_cast<float*>(to + 256)[unit & 3] = factor.y;
+        }
+      }
+      proxy_fence();
+    } else {
+      const int r = threadIdx.x & (kUnitRows - 1), row = unit * kUnitRows + r;
+      for (int c0 = 0; c0 < count; c0 += 256 / kUnitRows) {
+        const int c = c0 + static_cast<int>(threadIdx.x) / kUnitRows, at = __shfl_sync(0xFFFFFFFFu, entry, c & 31);
+        if (c < count && row < p.dim) p.products[static_cast<long long>(at) * p.dim + row] = sum_of(r >> 4, r & 15, c);
+      }
+    }
+    math_barrier();
+    if (threadIdx.x == 0) {
+      __threadfence();
+      atomicAdd(kind == kUp ? p.up_done + group : &p.plan->down_done, 1);
+    }
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------------
+
+qx_status check_prepare(int format, const void* gate, const void* up, const void* down, int experts, int shared, long long dim,
+                        long long inner, qx_moe** out) {
+  if (out == nullptr) return QX_STATUS_INVALID_ARGUMENT;
+  *out = nullptr;
+  if (gate == nullptr || up == nullptr || down == nullptr) return QX_STATUS_INVALID_ARGUMENT;
+  size_t block_bytes = 0;
+  if (!format_info(format, &block_bytes)) return QX_STATUS_UNSUPPORTED_FORMAT;
+  if (experts < 1 || experts > kMostExperts || shared < 0 || shared > kMostShared || dim <= 0 || inner <= 0 || dim % kBlockK != 0 ||
+      inner % kBlockK != 0 || dim > kMostWidth || inner > kMostWidth) {
+    return QX_STATUS_INVALID_SHAPE;
+  }
+  return QX_STATUS_OK;
+}
+
+qx_status relayout(int format, const uint8_t* first, const uint8_t* second, uint8_t* to, long long rows, int columns,
+                   cudaStream_t stream) {
+  const long long tiles = (second == nullptr ? rows : 2 * rows) / kTileRows, records = tiles * (columns / 32);
+  const long long grid = (records + 7) / 8;
+  if (grid > 0x7FFFFFFFLL) return QX_STATUS_INVALID_SHAPE;
+  if (format == QX_FORMAT_Q4_0) {
+    moe_relayout_kernel<QX_FORMAT_Q4_0><<<static_cast<unsigned>(grid), 256, 0, stream>>>(first, second, to, tiles, columns / 32);
+  } else {
+    moe_relayout_kernel<QX_FORMAT_Q8_0><<<static_cast<unsigned>(grid), 256, 0, stream>>>(first, second, to, tiles, columns / 32);
+  }
+  QX_CUDA_TRY(cudaGetLastError());
+  count_launch();
+  return QX_STATUS_OK;
+}
+
+qx_status prepare(int format, const uint8_t* gate, const uint8_t* up, const uint8_t* down, int experts, int shared, int dim,
+                  int inner, bool host, DeviceContext* ctx, cudaStream_t stream, qx_moe** out) {
+  auto* m = new (std::nothrow) qx_moe();
+  if (m == nullptr) return QX_STATUS_OUT_OF_MEMORY;
+  m->device = ctx->device;
+  m->format = format;
+  m->experts = experts;
+  m->shared = shared;
+  m->dim = dim;
+  m->inner = inner;
+  const int count = experts + shared;
+  const size_t matrix = static_cast<size_t>(inner) * (dim / 32);  // blocks
+  const size_t block = format == QX_FORMAT_Q4_0 ? 18 : 34, bytes = matrix * block;
+  m->up_bytes = 2 * bytes * count;
+  m->down_bytes = bytes * count;
+  void* temp = nullptr;
+  const auto fill = [&]() -> qx_status {
+    QX_CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&m->up), m->up_bytes));
+    QX_CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&m->down), m->down_bytes));
+    if (!host) {
+      QX_TRY(relayout(format, gate, up, m->up, static_cast<long long>(inner) * count, dim, stream));
+      return relayout(format, down, nullptr, m->down, static_cast<long long>(dim) * count, inner, stream);
+    }
+    QX_CUDA_TRY(cudaMalloc(&temp, 3 * bytes));  // (one expert at a time)
+    uint8_t* const to = static_cast<uint8_t*>(temp);
+    for (int e = 0; e < count; ++e) {
+      QX_CUDA_TRY(cudaMemcpyAsync(to, gate + e * bytes, bytes, cudaMemcpyHostToDevice, stream));
+      QX_CUDA_TRY(cudaMemcpyAsync(to + bytes, up + e * bytes, bytes, cudaMemcpyHostToDevice, stream));
+      QX_CUDA_TRY(cudaMemcpyAsync(to + 2 * bytes, down + e * bytes, bytes, cudaMemcpyHostToDevice, stream));
+      QX_TRY(relayout(format, to, to + bytes, m->up + 2 * bytes * e, inner, dim, stream));
+      QX_TRY(relayout(format, to + 2 * bytes, nullptr, m->down + bytes * e, dim, inner, stream));
+    }
+    QX_CUDA_TRY(cudaStreamSynchronize(stream));
+    return QX_STATUS_OK;
+  };
+  const qx_status status = fill();
+  if (temp != nullptr) (void)cudaFree(temp);
+  if (status != QX_STATUS_OK) {
+    qx_moe_destroy(m);
+    return status;
+  }
+  *out = m;
+  return QX_STATUS_OK;
+}
+
+bool on_boundary_of(const void* data, int type) { return reinterpret_cast<uintptr_t>(data) % kv::type_bytes(type) == 0; }
+
+qx_status check_apply(const qx_moe* m, const qx_moe_router* router, const qx_rows* x, const qx_rows* out, long long tokens,
+                      int activation, const int32_t* chosen, const float* weights) {
+  if (m == nullptr || router == nullptr || x == nullptr || out == nullptr || tokens < 0) return QX_STATUS_INVALID_ARGUMENT;
+  if (!kv::known_type(router->type)) return QX_STATUS_UNSUPPORTED_FORMAT;
+  if (router->top < 1 || router->top > std::min(kMostTop, m->experts)) return QX_STATUS_INVALID_SHAPE;
+  if (router->weights == nullptr || !on_boundary_of(router->weights, router->type) || !kv::on_boundary(router->bias) ||
+      (router->score != QX_MOE_SOFTMAX && router->score != QX_MOE_SIGMOID) || !std::isfinite(router->scale) ||
+      activation < QX_ACTIVATION_NONE || activation > QX_ACTIVATION_RELU2 || !kv::on_boundary(chosen) || !kv::on_boundary(weights)) {
+    return QX_STATUS_INVALID_ARGUMENT;
+  }
+  QX_TRY(kv::check_rows(x, tokens, m->dim, false));
+  QX_TRY(kv::check_rows(out, tokens, m->dim, true));
+  if (tokens > 0 && x->data == out->data && (x->type != out->type || (tokens > 1 && x->stride != out->stride))) {
+    return QX_STATUS_INVALID_ARGUMENT;  // (the inputs' place, but another view)
+  }
+  return QX_STATUS_OK;
+}
+
+// Scratch behind the workspace's arrival counters.
+struct Layout {
+  size_t total = kWorkspaceCounterBytes;
+  size_t take(size_t bytes) {
+    const size_t at = total;
+    total = align_up(total + bytes, 256);
+    return at;
+  }
+};
+
+template <int kFormat, int kTerms>
+qx_status launch_experts(const Params& p, long long grid, cudaStream_t stream) {
+  static SmemOptIn opt_in;
+  constexpr int bytes = ExpertShape<kFormat>::kBytes;
+  static_assert(2 * (bytes + 1024) <= 228 * 1024, "two CTAs share an SM");
+  QX_TRY(opt_in.ensure(moe_experts_kernel<kFormat, kTerms>, bytes));
+  return kv::launch_behind(moe_experts_kernel<kFormat, kTerms>, grid, kExpertThreads, bytes, stream, p);
+}
+
+qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_rows* x, const qx_rows* out, long long tokens,
+                       int activation, int32_t* chosen, float* weights, DeviceContext* ctx, qx_workspace* workspace,
+                       cudaStream_t stream) {
+  if (tokens == 0) return QX_STATUS_OK;
+  const size_t x_size = kv::type_bytes(x->type), out_size = kv::type_bytes(out->type);
+  const auto whole = [](const void* data, size_t row_bytes) { return reinterpret_cast<uintptr_t>(data) % 16 == 0 && row_bytes % 16 == 0; };
+  Params p{};
+  p.up = m->up;
+  p.down = m->down;
+  p.experts = m->experts;
+  p.shared = m->shared;
+  p.dim = m->dim;
+  p.inner = m->inner;
+  p.router = static_cast<const uint8_t*>(router->weights);
+  p.router_type = router->type;
+  p.router_vector = whole(router->weights, 0);
+  p.bias = router->bias;
+  p.top = router->top;
+  p.score = router->score;
+  p.normalise = router->normalise != 0;
+  p.scale = router->scale;
+  p.x_type = x->type;
+  p.x_vector = whole(x->data, x->stride * x_size);
+  p.x_stride = x->stride;
+  p.out_type = out->type;
+  p.out_vector = whole(out->data, out->stride * out_size);
+  p.out_stride = out->stride;
+  p.activation = activation;
+  p.terms = x->type == QX_STORAGE_F32 ? 2 : 1;
+  p.error = ctx->error_dev;
+
+  const long long pass = std::min<long long>(tokens, kPassTokens);
+  const size_t entries = static_cast<size_t>(pass) * (p.top + p.shared);
+  Layout l;
+  const size_t at_x = l.take(static_cast<size_t>(pass) * p.terms * slabs_of(p.dim) * kSlabBytes);
+  const size_t at_logits = l.take(static_cast<size_t>(pass) * p.experts * sizeof(double));
+  const size_t at_picks = l.take(entries * sizeof(int)), at_weights = l.take(entries * sizeof(float));
+  const size_t at_plan = l.take(sizeof(Plan)), at_done = l.take(entries * sizeof(int));
+  const size_t at_groups = l.take(entries * sizeof(Group)), at_list = l.take(entries * sizeof(int));
+  const size_t at_inner = l.take(entries * p.terms * slabs_of(p.inner) * kSlabBytes);
+  const size_t at_products = l.take(entries * p.dim * sizeof(float));
+  QX_TRY(workspace->reserve(l.total));
+  uint8_t* const base = static_cast<uint8_t*>(workspace->base);
+  p.arrivals = reinterpret_cast<int*>(base);
+  p.x_terms = base + at_x;
+  p.logits = reinterpret_cast<double*>(base + at_logits);
+  p.picks = reinterpret_cast<int*>(base + at_picks);
+  p.weights = reinterpret_cast<float*>(base + at_weights);
+  p.plan = reinterpret_cast<Plan*>(base + at_plan);
+  p.up_done = reinterpret_cast<int*>(base + at_done);
+  p.groups = reinterpret_cast<Group*>(base + at_groups);
+  p.list = reinterpret_cast<int*>(base + at_list);
+  p.inner_terms = base + at_inner;
+  p.products = reinterpret_cast<float*>(base + at_products);
+
+  for (long long t0 = 0; t0 < tokens; t0 += kPassTokens) {
+    p.tokens = static_cast<int>(std::min<long long>(kPassTokens, tokens - t0));
+    p.x = static_cast<const uint8_t*>(x->data) + t0 * x->stride * x_size;
+    p.out = static_cast<uint8_t*>(out->data) + t0 * out->stride * out_size;
+    p.chosen = chosen == nullptr ? nullptr : chosen + t0 * p.top;
+    p.chosen_weights = weights == nullptr ? nullptr : weights + t0 * p.top;
+    const int router_ctas = (p.tokens + kRouterTokens - 1) / kRouterTokens * ((p.experts + kRouterExperts - 1) / kRouterExperts);
+    const int convert_ctas = (p.tokens * slabs_of(p.dim) + 7) / 8;
+    QX_TRY(kv::launch_behind(moe_router_kernel, router_ctas + convert_ctas, kRouterThreads, 0, stream, p));
+    // (no more CTAs than there may be units)
+    const long long units = static_cast<long long>(p.tokens) * (p.top + p.shared) * (p.inner / 32);
+    const long long grid = std::min<long long>(2LL * ctx->prop.multiProcessorCount, units);
+    if (m->format == QX_FORMAT_Q4_0) {
+      QX_TRY(p.terms == 1 ? (launch_experts<QX_FORMAT_Q4_0, 1>(p, grid, stream)) : (launch_experts<QX_FORMAT_Q4_0, 2>(p, grid, stream)));
+    } else {
+      QX_TRY(p.terms == 1 ? (launch_experts<QX_FORMAT_Q8_0, 1>(p, grid, stream)) : (launch_experts<QX_FORMAT_Q8_0, 2>(p, grid, stream)));
+    }
+  }
+  return QX_STATUS_OK;
+}
+
+}  // namespace
+}  // namespace moe
+}  // namespace qx
+
+using namespace qx;
+
+extern "C" {
+
+qx_status qx_moe_prepare(int format, const void* gate, const void* up, const void* down, int experts, int shared, long long dim,
+                         long long inner, qx_moe** out) {
+  QX_TRY(moe::check_prepare(format, gate, up, down, experts, shared, dim, inner, out));
+  DeviceContext* ctx = nullptr;
+  QX_TRY(current_context(&ctx));
+  std::lock_guard<std::mutex> lock(ctx->mutex);
+  return moe::prepare(format, static_cast<const uint8_t*>(gate), static_cast<const uint8_t*>(up), static_cast<const uint8_t*>(down),
+                      experts, shared, static_cast<int>(dim), static_cast<int>(inner), true, ctx, ctx->stream, out);
+}
+
+qx_status qx_moe_prepare_dev(int format, const void* gate_dev, const void* up_dev, const void* down_dev, int experts, int shared,
+                             long long dim, long long inner, void* stream, qx_moe** out) {
+  QX_TRY(moe::check_prepare(format, gate_dev, up_dev, down_dev, experts, shared, dim, inner, out));
+  DeviceContext* ctx = nullptr;
+  QX_TRY(current_context(&ctx));
+  return moe::prepare(format, static_cast<const uint8_t*>(gate_dev), static_cast<const uint8_t*>(up_dev),
+                      static_cast<const uint8_t*>(down_dev), experts, shared, static_cast<int>(dim), static_cast<int>(inner), false,
+                      ctx, static_cast<cudaStream_t>(stream), out);
+}
+
+void qx_moe_destroy(qx_moe* moe) {
+  if (moe == nullptr) return;
+  if (moe->up != nullptr) (void)cudaFree(moe->up);
+  if (moe->down != nullptr) (void)cudaFree(moe->down);
+  delete moe;
+}
+
+qx_status qx_moe_apply_dev(const qx_moe* moe, const qx_moe_router* router, const qx_rows* x, const qx_rows* out, long long tokens,
+                           int activation, int32_t* chosen_dev, float* weights_dev, qx_workspace* workspace, void* stream) {
+  QX_TRY(moe::check_apply(moe, router, x, out, tokens, activation, chosen_dev, weights_dev));
+  DeviceContext* ctx = nullptr;
+  QX_TRY(current_context(&ctx));
+  if (workspace == nullptr) workspace = &ctx->workspace;
+  if (workspace->device != ctx->device || moe->device != ctx->device) return QX_STATUS_INVALID_ARGUMENT;
+  return moe::launch_apply(moe, router, x, out, tokens, activation, chosen_dev, weights_dev, ctx, workspace,
+                           static_cast<cudaStream_t>(stream));
+}
+
+qx_status qx_moe_apply(const qx_moe* moe, const qx_moe_router* router, const qx_rows* x, const qx_rows* out, long long tokens,
+                       int activation, int32_t* chosen, float* weights) {
+  QX_TRY(moe::check_apply(moe, router, x, out, tokens, activation, chosen, weights));
+  return kv::guarded([&]() -> qx_status {
+    DeviceContext* ctx = nullptr;
+    QX_TRY(current_context(&ctx));
+    if (moe->device != ctx->device) return QX_STATUS_INVALID_ARGUMENT;
+    if (tokens == 0) return QX_STATUS_OK;
+    std::lock_guard<std::mutex> lock(ctx->mutex);
+    kv::Arrays a;
+    const int from = a.add(x->data, kv::runs_of(x, tokens, moe->dim), x->data == out->data);
+    const int to = x->data == out->data ? from : a.add(out->data, kv::runs_of(out, tokens, moe->dim), true);
+    const int rows = a.add(router->weights, static_cast<size_t>(moe->experts) * moe->dim * kv::type_bytes(router->type), false);
+    const int bias = router->bias == nullptr ? -1 : a.add(router->bias, moe->experts * sizeof(float), false);
+    const size_t picks = static_cast<size_t>(tokens) * router->top;
+    const int ids = chosen == nullptr ? -1 : a.add(chosen, picks * sizeof(int32_t), true);
+    const int shares = weights == nullptr ? -1 : a.add(weights, picks * sizeof(float), true);
+    QX_TRY(a.to_device(ctx));
+    qx_rows dx = *x, dout = *out;
+    qx_moe_router r = *router;
+    dx.data = a.device<void>(from);
+    dout.data = a.device<void>(to);
+    r.weights = a.device<void>(rows);
+    r.bias = a.device<float>(bias);
+    QX_TRY(moe::launch_apply(moe, &r, &dx, &dout, tokens, activation, a.device<int32_t>(ids), a.device<float>(shares), ctx,
+                             &ctx->workspace, ctx->stream));
+    return a.from_device();
+  });
+}
+
+}  // extern "C"

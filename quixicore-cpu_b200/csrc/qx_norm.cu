@@ -217,16 +217,6 @@ __global__ void __launch_bounds__(kNormThreads, kVectors == 2 && !Stream::kEach 
 
 bool aligned(const void* data, int type) { return reinterpret_cast<uintptr_t>(data) % type_bytes(type) == 0; }
 
-qx_status check_rows(const qx_rows* view, long long tokens, long long dim, bool written) {
-  if (view == nullptr) return QX_STATUS_OK;
-  if (!known_type(view->type)) return QX_STATUS_UNSUPPORTED_FORMAT;
-  if (view->stride < 0 || (written && tokens > 1 && view->stride < dim)) return QX_STATUS_INVALID_SHAPE;
-  if (tokens <= 0) return QX_STATUS_OK;
-  if ((static_cast<__int128>(tokens - 1) * view->stride + dim) * 4 > std::numeric_limits<long long>::max()) {
-    return QX_STATUS_INVALID_SHAPE;
-  }
-  return view->data == nullptr || !aligned(view->data, view->type) ? QX_STATUS_INVALID_ARGUMENT : QX_STATUS_OK;
-}
 qx_status check_norm(const qx_norm* norm) {
   if (norm == nullptr) return QX_STATUS_OK;
   if (norm->kind != QX_NORM_RMS && norm->kind != QX_NORM_LAYER) return QX_STATUS_INVALID_ARGUMENT;
@@ -361,12 +351,19 @@ qx_status launch_residual_norm(const qx_rows* residual, const qx_rows* block, co
   return launch<InElements, InElements, InElements>(p, stream);
 }
 
-Runs runs_of(const qx_rows* view, long long tokens, long long dim) {
-  const size_t size = type_bytes(view->type);
-  return {tokens, 1, view->stride * size, 0, dim * size};
+}  // namespace
+
+qx_status check_rows(const qx_rows* view, long long tokens, long long dim, bool written) {
+  if (view == nullptr) return QX_STATUS_OK;
+  if (!known_type(view->type)) return QX_STATUS_UNSUPPORTED_FORMAT;
+  if (view->stride < 0 || (written && tokens > 1 && view->stride < dim)) return QX_STATUS_INVALID_SHAPE;
+  if (tokens <= 0) return QX_STATUS_OK;
+  if ((static_cast<__int128>(tokens - 1) * view->stride + dim) * 4 > std::numeric_limits<long long>::max()) {
+    return QX_STATUS_INVALID_SHAPE;
+  }
+  return view->data == nullptr || !aligned(view->data, view->type) ? QX_STATUS_INVALID_ARGUMENT : QX_STATUS_OK;
 }
 
-}  // namespace
 }  // namespace kv
 }  // namespace qx
 
