@@ -785,7 +785,7 @@ typedef struct qx_moe_router {
 } qx_moe_router;
 /* x and out: [tokens][dim], each with a type of its own; out is x itself, the same view of it, or lies elsewhere.
  * `chosen` and `weights` (either may be NULL) receive the experts and their w, [tokens][top], largest first. `activation`
- * is QX_ACTIVATION_*. Any number of tokens is served, in passes of 128; the kernels are made for few, whose experts' weights
+ * is QX_ACTIVATION_*. Any number of tokens is served, in passes of up to 128; the kernels are made for few, whose experts' weights
  * are read once per 16 tokens (8 of f32).
  * Precision. Logits are summed up in 64 bits from sums of eight f32 products, scores and weights of the router are taken in
  * 64 bits. Codes are used as they are; activations as f16 under a power of two per 32 elements: 16-bit ones exactly (an

@@ -7,17 +7,18 @@
 // arranged around keeping those loads under way from the first to the last.
 //
 // Router (moe_router_kernel). Logits are sums of at most eight f32 products at a time, added up in 64 bits: two experts
-// on both sides of the choice are told apart as far as the inputs' own products are. A warp takes two experts and eight tokens and a
-// quarter of the columns. The last CTA to finish eight tokens chooses their experts, a warp per token; the last of those
-// sorts all (token, expert) pairs by expert. Beside them, other CTAs turn the activations into f16 terms.
+// on both sides of the choice are told apart as far as the inputs' own products are. A CTA takes two experts and eight tokens, a
+// warp an eighth of the columns; the last CTA to finish eight tokens chooses their experts, a warp per token. Beside them,
+// other CTAs turn the activations into f16 terms.
 //
-// Experts (moe_experts_kernel). Work is cut into units that CTAs draw as tickets, in this order:
+// Experts (moe_experts_kernel). Every CTA sorts the (token, expert) pairs by expert, in shared memory: a microsecond, which a
+// kernel of its own or the router's last CTA would add to the launch as well. Work is cut into units that CTAs draw as tickets, in this order:
 //   up       64 rows (32 of gate, the same 32 of up) of one expert, for up to 16 columns: tokens of it, times terms
 //   down     64 rows of the down projection of one expert, once all of its up units are done
 //   combine  1024 elements of one token's output, once all down units are done
 // A ticket only waits for smaller ones, which their CTAs have begun: no CTA has to be resident for another to go on. A
-// warp that copies runs ahead of eight that multiply through a ring of stages, across units, and calls a unit's weights
-// into L2 before it waits for what the unit depends on.
+// warp that copies runs ahead of eight that multiply through a ring of stages, across units; where a unit has to wait for
+// others, its weights are on their way already.
 //
 // Products. Warp-level f16 MMAs with the weights as the operand of 16 rows: codes are exact in f16 (a nibble is ORed into
 // the mantissa of 1024, a byte permuted there), and one MMA pair takes a block of 32 columns, whose sum is multiplied by
@@ -50,12 +51,16 @@ using namespace sm100;
 // One warp per record.
 template <int kFormat>
 __global__ void __launch_bounds__(256) moe_relayout_kernel(const uint8_t* __restrict__ first, const uint8_t* __restrict__ second,
-                                                           uint8_t* __restrict__ to, long long tiles, int blocks) {
+                                                           uint8_t* __restrict__ to, long long tiles, int tiles_each, int blocks) {
   constexpr int kBlock = kFormat == QX_FORMAT_Q4_0 ? 18 : 34, kRecord = record_bytes(kFormat);
   const long long record = blockIdx.x * 8LL + threadIdx.x / 32;
   if (record >= tiles * blocks) return;
-  const long long tile = record / blocks;
-  const int block = static_cast<int>(record - tile * blocks), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long long expert = record / (static_cast<long long>(tiles_each) * blocks);
+  const long long in_expert = record - expert * tiles_each * blocks;
+  const int unit = static_cast<int>(in_expert / (kUnitTiles * blocks)), in_unit = static_cast<int>(in_expert - static_cast<long long>(unit) * kUnitTiles * blocks);
+  const int in_block = min(kUnitTiles, tiles_each - unit * kUnitTiles), block = in_unit / in_block;
+  const long long tile = expert * tiles_each + unit * kUnitTiles + in_unit % in_block;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* const out = to + record * kRecord;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -88,7 +93,7 @@ __global__ void __launch_bounds__(256) moe_relayout_kernel(const uint8_t* __rest
 }
 
 // ---- router ------------------------------------------------------------------------------------
-constexpr int kRouterTokens = 8, kRouterExperts = 4, kRouterSplits = 4, kRouterThreads = 256;
+constexpr int kRouterTokens = 8, kRouterExperts = 2, kRouterSplits = 8, kRouterThreads = 256;
 
 // Eight neighbouring elements as they lie in memory; off 16-byte boundaries as f32.
 struct Words {
@@ -123,8 +128,8 @@ __device__ __forceinline__ float2 block_factor(uint32_t top) {
 }
 
 // A warp turns 128 columns of a token into terms.
-__device__ __forceinline__ void convert_slab(const Params& p, int token, int slab) {
-  const int lane = threadIdx.x & 31, d = slab * 128 + lane * 4;
+__device__ __forceinline__ void convert_columns(const Params& p, int token, int part) {
+  const int lane = threadIdx.x & 31, d = part * 128 + lane * 4;
   float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (d < p.dim) kv::load4(p.x, p.x_type, p.x_vector, token * p.x_stride + d, v);
   uint32_t top = 0;
@@ -133,22 +138,20 @@ __device__ __forceinline__ void convert_slab(const Params& p, int token, int sla
 #pragma unroll
   for (int h = 1; h < 8; h <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, h));
   const float2 factor = block_factor(top);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] *= factor.x;
   for (int term = 0; term < p.terms; ++term) {
-    uint8_t* const to = p.x_terms + (static_cast<long long>(token * p.terms + term) * slabs_of(p.dim) + slab) * kSlabBytes;
+    const long long row = static_cast<long long>(token) * p.terms + term;
     __half2 h[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      if (term == 0) {
-        v[2 * e] *= factor.x;
-        v[2 * e + 1] *= factor.x;
-      }
       h[e] = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
       const float2 back = __half22float2(h[e]);
       v[2 * e] -= back.x;
       v[2 * e + 1] -= back.y;
     }
-    *reinterpret_cast<uint2*>(to + lane * 8) = make_uint2(pair_bits(h[0]), pair_bits(h[1]));
-    if ((lane & 7) == 0) *reinterpret_cast<float*>(to + 256 + lane / 8 * 4) = factor.y;
+    if (d < p.dim) *reinterpret_cast<uint2*>(p.x_terms + row * p.dim + d) = make_uint2(pair_bits(h[0]), pair_bits(h[1]));
+    if (d < p.dim && (lane & 7) == 0) p.x_scales[row * scales_of(p.dim) + d / 32] = factor.y;
   }
 }
 
@@ -178,14 +181,18 @@ __device__ __forceinline__ void choose(const Params& p, int token) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       score[i] = 0.0;
-      if (lane + 32 * i < p.experts) score[i] = exp(logit[i] - largest);
+      // (weights are f32; a choice by score + bias takes all bits there are)
+      const double below = logit[i] - largest;
+      if (lane + 32 * i < p.experts) score[i] = p.bias == nullptr ? static_cast<double>(expf(static_cast<float>(below))) : exp(below);
       total += score[i];
     }
 #pragma unroll
     for (int h = 16; h > 0; h >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, h);
   } else {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) score[i] = 1.0 / (1.0 + exp(-logit[i]));
+    for (int i = 0; i < kEach; ++i) {
+      score[i] = p.bias == nullptr ? static_cast<double>(1.0f / (1.0f + expf(static_cast<float>(-logit[i])))) : 1.0 / (1.0 + exp(-logit[i]));
+    }
     total = 1.0;
   }
   unsigned long long key[kEach];
@@ -245,70 +252,6 @@ __device__ __forceinline__ void choose(const Params& p, int token) {
   }
 }
 
-constexpr int kAllExperts = kMostExperts + kMostShared, kMaskWords = kPassTokens / 32;
-struct SortSpace {
-  uint32_t tokens[kAllExperts][kMaskWords];  // of each expert
-  int first[kAllExperts], sums[2][kRouterThreads / 32];
-};
-// The CTA sorts (token, expert) pairs by expert and cuts each expert's into groups.
-__device__ __forceinline__ void sort_pairs(const Params& p, SortSpace& s) {
-  const int experts = p.experts + p.shared, places = p.top + p.shared, entries = p.tokens * places;
-  const int most = kColumns / p.terms, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-  for (int i = threadIdx.x; i < experts * kMaskWords; i += kRouterThreads) s.tokens[i / kMaskWords][i % kMaskWords] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < entries; i += kRouterThreads) {
-    const int token = i / places;
-    atomicOr(&s.tokens[__ldcg(p.picks + i)][token / 32], 1u << (token & 31));
-  }
-  __syncthreads();
-  // Running numbers of entries and groups in front of each expert, 256 experts at a time.
-  int entries_before = 0, groups_before = 0;
-  for (int e0 = 0; e0 < experts; e0 += kRouterThreads) {
-    const int e = e0 + static_cast<int>(threadIdx.x);
-    int count = 0;
-    if (e < experts) {
-#pragma unroll
-      for (int w = 0; w < kMaskWords; ++w) count += __popc(s.tokens[e][w]);
-    }
-    const int cuts = (count + most - 1) / most;
-    int through = count, cuts_through = cuts;
-#pragma unroll
-    for (int h = 1; h < 32; h <<= 1) {
-      const int a = __shfl_up_sync(0xFFFFFFFFu, through, h), b = __shfl_up_sync(0xFFFFFFFFu, cuts_through, h);
-      if (lane >= h) {
-        through += a;
-        cuts_through += b;
-      }
-    }
-    if (lane == 31) {
-      s.sums[0][warp] = through;
-      s.sums[1][warp] = cuts_through;
-    }
-    __syncthreads();
-    int first = entries_before + through - count, group = groups_before + cuts_through - cuts;
-    for (int w = 0; w < kRouterThreads / 32; ++w) {
-      if (w < warp) {
-        first += s.sums[0][w];
-        group += s.sums[1][w];
-      }
-      entries_before += s.sums[0][w];
-      groups_before += s.sums[1][w];
-    }
-    if (e < experts) {
-      s.first[e] = first;
-      for (int i = 0; i < cuts; ++i) p.groups[group + i] = {e, first + i * most, min(most, count - i * most)};
-    }
-    __syncthreads();
-  }
-  for (int i = threadIdx.x; i < entries; i += kRouterThreads) {
-    const int token = i / places, e = __ldcg(p.picks + i);
-    int rank = __popc(s.tokens[e][token / 32] & ((1u << (token & 31)) - 1));
-    for (int w = 0; w < token / 32; ++w) rank += __popc(s.tokens[e][w]);
-    p.list[s.first[e] + rank] = i;
-  }
-  if (threadIdx.x == 0) p.plan->groups = groups_before;
-}
-
 // The last thread block to arrive at a counter of `all`, which is then zero again.
 __device__ __forceinline__ bool arrives_last(int* counter, int all, int* shared) {
   __threadfence();
@@ -326,10 +269,7 @@ __device__ __forceinline__ bool arrives_last(int* counter, int all, int* shared)
 
 // Grid: [token groups][expert groups] CTAs of the router, then those that convert activations.
 __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid_constant__ Params p) {
-  __shared__ union {
-    double parts[kRouterSplits][kRouterExperts][kRouterTokens];
-    SortSpace sort;
-  } s;
+  __shared__ double parts[kRouterSplits][kRouterExperts][kRouterTokens];
   __shared__ int last;
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -338,22 +278,21 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int index = static_cast<int>(blockIdx.x) - token_groups * expert_groups;
   if (index >= 0) {
-    const int slabs = slabs_of(p.dim), item = index * 8 + warp;
-    if (item < p.tokens * slabs) convert_slab(p, item / slabs, item % slabs);
+    const int each = (p.dim + 127) / 128, item = index * 8 + warp;
+    if (item < p.tokens * each) convert_columns(p, item / each, item % each);
     return;
   }
   if (blockIdx.x == 0) {
     const int most = p.tokens * (p.top + p.shared);
     for (int i = threadIdx.x; i < most; i += kRouterThreads) p.up_done[i] = 0;
-    if (threadIdx.x == 0) p.plan->ticket = p.plan->down_done = 0;
+    if (threadIdx.x == 0) *p.progress = {0, 0};
   }
   const int token_group = blockIdx.x / expert_groups, expert_group = blockIdx.x % expert_groups;
-  const int token0 = token_group * kRouterTokens, split = warp & (kRouterSplits - 1);
-  const int expert0 = expert_group * kRouterExperts + warp / kRouterSplits * 2;
+  const int token0 = token_group * kRouterTokens, expert0 = expert_group * kRouterExperts;
   double sum[16];  // [expert of two][token]
 #pragma unroll
   for (int i = 0; i < 16; ++i) sum[i] = 0.0;
-  for (int d = (split * 32 + lane) * 8; d < p.dim; d += kRouterSplits * 256) {
+  for (int d = static_cast<int>(threadIdx.x) * 8; d < p.dim; d += kRouterSplits * 256) {
     Words w[2], x[kRouterTokens];  // (all under way before the first is used)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -392,13 +331,13 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid
     }
   }
   sum[0] += __shfl_xor_sync(0xFFFFFFFFu, sum[0], 1);
-  if ((lane & 1) == 0) s.parts[split][warp / kRouterSplits * 2 + (lane >> 4)][lane >> 1 & 7] = sum[0];
+  if ((lane & 1) == 0) parts[warp][lane >> 4][lane >> 1 & 7] = sum[0];
   __syncthreads();
   if (threadIdx.x < kRouterExperts * kRouterTokens) {
     const int e = threadIdx.x / kRouterTokens, t = threadIdx.x % kRouterTokens;
-    double v = s.parts[0][e][t];
+    double v = parts[0][e][t];
 #pragma unroll
-    for (int i = 1; i < kRouterSplits; ++i) v += s.parts[i][e][t];
+    for (int i = 1; i < kRouterSplits; ++i) v += parts[i][e][t];
     const int expert = expert_group * kRouterExperts + e;
     if (expert < p.experts && token0 + t < p.tokens) p.logits[static_cast<long long>(token0 + t) * p.experts + expert] = v;
   }
@@ -407,37 +346,130 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid
     if (p.experts <= 128) choose<4>(p, token0 + warp);
     else choose<kMostExperts / 32>(p, token0 + warp);
   }
-  if (!arrives_last(p.arrivals + kPassTokens / kRouterTokens, token_groups, &last)) return;
-  sort_pairs(p, s.sort);
 }
 
 // ---- experts -----------------------------------------------------------------------------------
 constexpr int kMathWarps = 8, kExpertThreads = 32 * (kMathWarps + 1);
-constexpr int kUnitTiles = 4, kUnitRows = kUnitTiles * kTileRows;
-constexpr int kStageBlocks = 8;                          // columns of a stage, in blocks: two slabs
-constexpr int kColumnBytes = 2 * kSlabBytes + 32;        // between columns: eight lanes of a 16-byte load meet no conflict
+constexpr int kUnitRows = kUnitTiles * kTileRows;
+// A stage holds eight blocks of columns of a unit's four tiles; a warp takes two tiles and two of the blocks, so that
+// an activation operand read from shared memory serves two products.
+constexpr int kStageBlocks = 8, kWarpTiles = 2, kWarpBlocks = 2;
+constexpr int kColumnBytes = kStageBlocks * 64 + 64;  // the 64: eight lanes of a 16-byte load meet no conflict
+constexpr int kScaleBytes = kStageBlocks * 4;
 constexpr int kCombineWidth = 1024;
-constexpr int kReduceStride = 2 * 128 + 4;               // floats per warp
+constexpr int kReduceTile = 128 + 1, kReduceWarp = kWarpTiles * kReduceTile;  // floats: [row g, g + 8 x column 2 t, 2 t + 1][lane]
 enum { kUp = 0, kDown = 1, kCombine = 2, kExit = 3 };
 
 struct StageInfo {
   int kind, blocks, last, tiles;
-  int unit, group, count, expert;
-  int entries[kColumns];
+  int unit, group, count, unused;
+  uint16_t entries[kColumns];
+};
+// The pairs of a pass by expert, and how each expert's are cut into groups.
+struct Group {
+  uint16_t expert, first, count;  // entries list[first .. first + count - 1]
+};
+struct Plan {
+  int groups;
+  uint16_t list[kPassEntries];  // entries, by expert, ascending
+  Group group[kPassEntries];
+};
+constexpr int kAllExperts = kMostExperts + kMostShared, kMaskWords = kPassTokens / 32;
+struct SortSpace {
+  uint32_t tokens[kAllExperts][kMaskWords];  // of each expert
+  uint16_t first[kAllExperts];
+  int sums[2][kExpertThreads / 32];
 };
 
 template <int kFormat>
 struct ExpertShape {
   static constexpr int kRecord = record_bytes(kFormat);
   static constexpr int kStages = kFormat == QX_FORMAT_Q4_0 ? 5 : 3;
-  static constexpr int kTileBytes = kStageBlocks * kRecord;
-  static constexpr int kWeights = kUnitTiles * kTileBytes;
-  static constexpr int kStage = kWeights + kColumns * kColumnBytes;
+  static constexpr int kWeights = kStageBlocks * kUnitTiles * kRecord;
+  static constexpr int kScales = kWeights + kColumns * kColumnBytes;
+  static constexpr int kStage = kScales + kColumns * kScaleBytes;
   static constexpr int kReduce = kStages * kStage;
-  static constexpr int kInfo = kReduce + kMathWarps * kReduceStride * 4;
+  static constexpr int kInfo = kReduce + (kMathWarps * kReduceWarp * 4 + 15) / 16 * 16;
   static constexpr int kBars = kInfo + kStages * static_cast<int>(sizeof(StageInfo));
-  static constexpr int kBytes = kBars + 2 * kStages * 8 + 16;
+  static constexpr int kPlan = kBars + 2 * kStages * 8 + 16;
+  static constexpr int kBytes = kPlan + static_cast<int>(sizeof(Plan));
+  static_assert(sizeof(SortSpace) <= kStages * kStage, "sorting takes the ring's place");
 };
+
+// All threads of the CTA sort the pairs.
+__device__ __forceinline__ void sort_pairs(const Params& p, int terms, SortSpace& s, Plan& plan) {
+  const int experts = p.experts + p.shared, places = p.top + p.shared, entries = p.tokens * places;
+  const int most = kColumns / terms, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  for (int i = threadIdx.x; i < experts * kMaskWords; i += kExpertThreads) s.tokens[i / kMaskWords][i % kMaskWords] = 0;
+  __syncthreads();
+  constexpr int kEach = (kPassEntries + kExpertThreads - 1) / kExpertThreads;
+  int pick[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = threadIdx.x + j * kExpertThreads;
+    if (i < entries) pick[j] = __ldcg(p.picks + i);
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = threadIdx.x + j * kExpertThreads, token = i / places;
+    if (i < entries) atomicOr(&s.tokens[pick[j]][token / 32], 1u << (token & 31));
+  }
+  __syncthreads();
+  // Running numbers of entries and groups in front of each expert, a thread per expert at a time.
+  int entries_before = 0, groups_before = 0;
+  for (int e0 = 0; e0 < experts; e0 += kExpertThreads) {
+    const int e = e0 + static_cast<int>(threadIdx.x);
+    int count = 0;
+    if (e < experts) {
+#pragma unroll
+      for (int w = 0; w < kMaskWords; ++w) count += __popc(s.tokens[e][w]);
+    }
+    const int cuts = (count + most - 1) / most;
+    int through = count, cuts_through = cuts;
+#pragma unroll
+    for (int h = 1; h < 32; h <<= 1) {
+      const int a = __shfl_up_sync(0xFFFFFFFFu, through, h), b = __shfl_up_sync(0xFFFFFFFFu, cuts_through, h);
+      if (lane >= h) {
+        through += a;
+        cuts_through += b;
+      }
+    }
+    if (lane == 31) {
+      s.sums[0][warp] = through;
+      s.sums[1][warp] = cuts_through;
+    }
+    __syncthreads();
+    int first = entries_before + through - count, group = groups_before + cuts_through - cuts;
+#pragma unroll
+    for (int w = 0; w < kExpertThreads / 32; ++w) {
+      const int a = s.sums[0][w], b = s.sums[1][w];
+      first += w < warp ? a : 0;
+      group += w < warp ? b : 0;
+      entries_before += a;
+      groups_before += b;
+    }
+    if (e < experts) {
+      s.first[e] = static_cast<uint16_t>(first);
+      for (int i = 0; i < cuts; ++i) {
+        plan.group[group + i] = {static_cast<uint16_t>(e), static_cast<uint16_t>(first + i * most),
+                                 static_cast<uint16_t>(min(most, count - i * most))};
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = threadIdx.x + j * kExpertThreads;
+    if (i >= entries) continue;
+    const int token = i / places;
+    int rank = __popc(s.tokens[pick[j]][token / 32] & ((1u << (token & 31)) - 1));
+#pragma unroll
+    for (int w = 0; w < kMaskWords; ++w) rank += w < token / 32 ? __popc(s.tokens[pick[j]][w]) : 0;
+    plan.list[s.first[pick[j]] + rank] = static_cast<uint16_t>(i);
+  }
+  if (threadIdx.x == 0) plan.groups = groups_before;
+  __syncthreads();
+}
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -508,45 +540,43 @@ __device__ __forceinline__ F32x2 mul2(F32x2 a, F32x2 b) {
   return v;
 }
 
-// A warp's blocks of a stage: 16 rows x 8 kN columns, sums in `total` [column tile][row g, row g + 8].
+// A warp's blocks of a stage: 2 x 16 rows x 8 kN columns, sums in `total` [tile][column tile][row g, row g + 8].
 template <int kFormat, int kN>
-__device__ __forceinline__ void multiply(const uint8_t* records, const uint8_t* columns, int blocks, F32x2 (&total)[2][2]) {
+__device__ __forceinline__ void multiply(const uint8_t* records, int tiles, const uint8_t* columns, const uint8_t* scales, int blocks,
+                                         F32x2 (&total)[kWarpTiles][2][2]) {
+  constexpr int kRecord = record_bytes(kFormat);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float scales[kN][2][4];  // of columns 2 t, 2 t + 1 and the slab's four blocks
+  float2 factors[kN][2];  // of columns 2 t, 2 t + 1 and both blocks; odd columns lie behind the even ones
 #pragma unroll
   for (int n = 0; n < kN; ++n) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float4 f = *reinterpret_cast<const float4*>(columns + (8 * n + 2 * t + e) * kColumnBytes + 256);
-      scales[n][e][0] = f.x;
-      scales[n][e][1] = f.y;
-      scales[n][e][2] = f.z;
-      scales[n][e][3] = f.w;
+      factors[n][e] = *reinterpret_cast<const float2*>(scales + (4 * n + t + 8 * e) * kScaleBytes);
     }
   }
-  const auto block = [&](int b) {
-    const uint8_t* const record = records + b * record_bytes(kFormat);
-    uint32_t a0[4], a1[4];
-    Codes<kFormat>::load(record, lane, a0, a1);
-    const float2 d = __half22float2(reinterpret_cast<const __half2*>(record + record_bytes(kFormat) - 32)[g]);
+#pragma unroll
+  for (int b = 0; b < kWarpBlocks; ++b) {
+    if (b >= blocks) continue;
+    uint32_t a[kWarpTiles][2][4];
+    float2 d[kWarpTiles];
+#pragma unroll
+    for (int i = 0; i < kWarpTiles; ++i) {
+      const uint8_t* const record = records + (b * tiles + i) * kRecord;
+      Codes<kFormat>::load(record, lane, a[i][0], a[i][1]);
+      d[i] = __half22float2(reinterpret_cast<const __half2*>(record + kRecord - 32)[g]);
+    }
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       const uint4 x = *reinterpret_cast<const uint4*>(columns + (8 * n + g) * kColumnBytes + b * 64 + t * 16);
-      float sum[4];
-      mma_f16_first(sum, a0, x.x, x.y);
-      mma_f16(sum, a1, x.z, x.w);
-      const F32x2 s = pair_of(scales[n][0][b], scales[n][1][b]);
-      tile::fma2(total[n][0], pair_of(sum[0], sum[1]), mul2(s, both(d.x)));
-      tile::fma2(total[n][1], pair_of(sum[2], sum[3]), mul2(s, both(d.y)));
-    }
-  };
-  if (blocks == kSlabBlocks) {
+      const F32x2 s = b == 0 ? pair_of(factors[n][0].x, factors[n][1].x) : pair_of(factors[n][0].y, factors[n][1].y);
 #pragma unroll
-    for (int b = 0; b < kSlabBlocks; ++b) block(b);
-  } else {
-#pragma unroll
-    for (int b = 0; b < kSlabBlocks; ++b) {
-      if (b < blocks) block(b);
+      for (int i = 0; i < kWarpTiles; ++i) {
+        float sum[4];
+        mma_f16_first(sum, a[i][0], x.x, x.y);
+        mma_f16(sum, a[i][1], x.z, x.w);
+        tile::fma2(total[i][n][0], pair_of(sum[0], sum[1]), mul2(s, both(d[i].x)));
+        tile::fma2(total[i][n][1], pair_of(sum[2], sum[3]), mul2(s, both(d[i].y)));
+      }
     }
   }
 }
@@ -554,8 +584,13 @@ __device__ __forceinline__ void multiply(const uint8_t* records, const uint8_t* 
 // The math warps meet: barrier 1.
 __device__ __forceinline__ void math_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kMathWarps) : "memory"); }
 
-// What the copying warp reads of other CTAs' results goes through the asynchronous proxy.
-__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// This thread's arrival at a barrier, once its copies so far have landed.
+__device__ __forceinline__ void arrive_behind_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
 __device__ __forceinline__ int load_acquire(const int* p) {
   int v;
@@ -583,93 +618,76 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
   uint64_t* const full = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* const empty = full + kStages;
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
+  Plan& plan = *reinterpret_cast<Plan*>(smem + S::kPlan);
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(full + i, 1);
+      mbar_init(full + i, 1 + 32);  // (the weights, and each lane's copies of activations)
       mbar_init(empty + i, kMathWarps);
     }
     *abort_flag = 0;
     mbar_fence_init();
   }
   asm volatile("griddepcontrol.launch_dependents;");
-  __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  int next = 0;
+  if (threadIdx.x == 32 * kMathWarps) next = atomicAdd(&p.progress->ticket, 1);
+  sort_pairs(p, kTerms, *reinterpret_cast<SortSpace*>(smem), plan);
 
   const int up_blocks = p.dim / 32, down_blocks = p.inner / 32;
   const int up_units = p.inner / 32, down_tiles = p.dim / kTileRows, down_units = (down_tiles + kUnitTiles - 1) / kUnitTiles;
 
   if (warp == kMathWarps) {
     // ---- copies ------------------------------------------------------------------------------
-    const int groups = __ldcg(&p.plan->groups);
     const int combine_chunks = (p.dim + kCombineWidth - 1) / kCombineWidth;
-    const long long ups = static_cast<long long>(groups) * up_units, downs = static_cast<long long>(groups) * down_units;
-    const long long all = ups + downs + static_cast<long long>(p.tokens) * combine_chunks;
+    const int ups = plan.groups * up_units, downs = plan.groups * down_units, all = ups + downs + p.tokens * combine_chunks;
     tile::Ring ring;
     int issued = 0;  // stages, as far as the ring's size
     bool ok = true;
-    int next = 0;
-    if (lane == 0) next = atomicAdd(&p.plan->ticket, 1);
+    asm volatile("fence.proxy.async;" ::: "memory");  // (the ring's place was the sorting's)
     for (;;) {
-      const long long ticket = __shfl_sync(0xFFFFFFFFu, next, 0);
-      if (lane == 0 && ticket < all) next = atomicAdd(&p.plan->ticket, 1);  // (needed a unit later)
+      const int ticket = __shfl_sync(0xFFFFFFFFu, next, 0);
+      if (lane == 0 && ticket < all) next = atomicAdd(&p.progress->ticket, 1);  // (needed a unit later)
       const int kind = ticket < ups ? kUp : ticket < ups + downs ? kDown : ticket < all ? kCombine : kExit;
-      int group = 0, unit = 0, blocks = 0, tiles = 0, stages = 1;
-      Group work = {0, 0, 0};
+      int group = 0, unit = 0, blocks = 0, tiles = 0, stages = 1, count = 0, entry = 0;
       const uint8_t* weights = nullptr;
-      const uint8_t* activations = nullptr;
-      int entry = 0, column_row = 0;
+      int row = 0;  // lane < count * terms: the row of activations that is its column
+      const int* counter = nullptr;  // what the unit waits for
+      int target = 0;
       if (kind == kUp || kind == kDown) {
-        const int units = kind == kUp ? up_units : down_units;
-        const long long at = kind == kUp ? ticket : ticket - ups;
-        group = static_cast<int>(at / units);
-        unit = static_cast<int>(at - static_cast<long long>(group) * units);
-        work.expert = __ldcg(&p.groups[group].expert);
-        work.first = __ldcg(&p.groups[group].first);
-        work.count = __ldcg(&p.groups[group].count);
+        const int units = kind == kUp ? up_units : down_units, at = kind == kUp ? ticket : ticket - ups;
+        group = at / units;
+        unit = at - group * units;
+        const Group work = plan.group[group];
+        count = work.count;
         blocks = kind == kUp ? up_blocks : down_blocks;
         stages = (blocks + kStageBlocks - 1) / kStageBlocks;
         tiles = kind == kUp ? kUnitTiles : min(kUnitTiles, down_tiles - unit * kUnitTiles);
         const long long tile0 = static_cast<long long>(work.expert) * (kind == kUp ? p.inner / 8 : down_tiles) + unit * kUnitTiles;
         weights = (kind == kUp ? p.up : p.down) + tile0 * blocks * S::kRecord;
-        const int column = lane - kUnitTiles;
-        if (column >= 0 && column < work.count * kTerms) {
-          entry = __ldcg(p.list + work.first + column / kTerms);
-          column_row = kind == kUp ? entry / (p.top + p.shared) : entry;
-          activations = (kind == kUp ? p.x_terms : p.inner_terms) +
-                        static_cast<long long>(column_row * kTerms + column % kTerms) * slabs_of(blocks * 32) * kSlabBytes;
+        if (lane < count * kTerms) {
+          entry = plan.list[work.first + lane / kTerms];
+          row = (kind == kUp ? entry / (p.top + p.shared) : entry) * kTerms + lane % kTerms;
         }
         if (kind == kDown) {
-          // (the weights on their way to L2 while the unit's activations are waited for)
-          if (lane < tiles) {
-            const uint64_t from = reinterpret_cast<uint64_t>(weights + static_cast<long long>(lane) * blocks * S::kRecord);
-            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(blocks * S::kRecord));
-          }
-          ok = wait_for_count(p.up_done + group, up_units, abort_flag);
+          counter = p.up_done + group;
+          target = up_units;
         }
       } else if (kind == kCombine) {
-        const int at = static_cast<int>(ticket - ups - downs);
-        group = at / combine_chunks;  // (the token)
-        unit = at - group * combine_chunks;
-        ok = wait_for_count(&p.plan->down_done, static_cast<int>(downs), abort_flag);
+        group = (ticket - ups - downs) / combine_chunks;  // (the token)
+        unit = ticket - ups - downs - group * combine_chunks;
+        counter = &p.progress->down_done;
+        target = downs;
       }
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) {
-        if (lane == 0) report_error(p.error, 51);
-        break;
-      }
-      proxy_fence();
-      for (int stage = 0; stage < stages; ++stage) {
+      const auto begin_stage = [&](int stage) {
         ok = issued < kStages || mbar_wait_warp(empty + ring.slot, ring.phase ^ 1u, abort_flag);
         if (!ok) {
           if (lane == 0) report_error(p.error, 52);
-          break;
+          return;
         }
         issued = min(issued + 1, kStages);
         const int in_stage = min(kStageBlocks, blocks - stage * kStageBlocks);
-        const uint32_t column_bytes = (in_stage + kSlabBlocks - 1) / kSlabBlocks * kSlabBytes;
         StageInfo& info = infos[ring.slot];
-        const int column = lane - kUnitTiles;
         if (lane == 0) {
           info.kind = kind;
           info.blocks = in_stage;
@@ -677,22 +695,55 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
           info.tiles = tiles;
           info.unit = unit;
           info.group = group;
-          info.count = work.count;
-          info.expert = work.expert;
+          info.count = count;
         }
-        if (column >= 0 && column < work.count * kTerms && column % kTerms == 0) info.entries[column / kTerms] = entry;
+        if (lane < count * kTerms && lane % kTerms == 0) info.entries[lane / kTerms] = static_cast<uint16_t>(entry);
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive_expect_tx(full + ring.slot, kind < kCombine ? tiles * in_stage * S::kRecord + work.count * kTerms * column_bytes : 0);
+          const uint32_t bytes = in_stage * tiles * S::kRecord;
+          mbar_arrive_expect_tx(full + ring.slot, bytes);
+          if (bytes > 0) {
+            tile::bulk_load(smem + ring.slot * S::kStage, weights + static_cast<long long>(stage) * kStageBlocks * tiles * S::kRecord, bytes,
+                            full + ring.slot);
+          }
         }
-        __syncwarp();
-        uint8_t* const to = smem + ring.slot * S::kStage;
-        if (lane < tiles) {
-          tile::bulk_load(to + lane * S::kTileBytes, weights + (static_cast<long long>(lane) * blocks + stage * kStageBlocks) * S::kRecord,
-                          in_stage * S::kRecord, full + ring.slot);
-        } else if (activations != nullptr) {
-          tile::bulk_load(to + S::kWeights + column * kColumnBytes, activations + stage * 2 * kSlabBytes, column_bytes, full + ring.slot);
+      };
+      // A column's 256 values are one 16-byte copy of each lane, the scales of all columns another.
+      const auto bring_columns = [&](int stage, int slot) {
+        const int in_stage = min(kStageBlocks, blocks - stage * kStageBlocks), columns = count * kTerms;
+        const int width = kind == kUp ? p.dim : p.inner;
+        const __half* const values = (kind == kUp ? p.x_terms : p.inner_terms) + stage * kStageBlocks * 32 + lane * 8;
+        const float* const scales = (kind == kUp ? p.x_scales : p.inner_scales) + stage * kStageBlocks;
+        const uint32_t to = smem_u32(smem + slot * S::kStage);
+        for (int c = 0; c < columns; ++c) {
+          const long long from = __shfl_sync(0xFFFFFFFFu, row, c);
+          if (lane < in_stage * 4) copy16(to + S::kWeights + c * kColumnBytes + lane * 16, values + from * width);
         }
+        const int c = lane >> 1, part = (lane & 1) * 4;
+        const long long from = __shfl_sync(0xFFFFFFFFu, row, c);
+        if (c < columns && part < in_stage) {
+          copy16(to + S::kScales + ((c >> 1) + 8 * (c & 1)) * kScaleBytes + part * 4, scales + from * scales_of(width) + part);
+        }
+        arrive_behind_copies(full + slot);
+      };
+      // Weights first, where the activations are not there yet.
+      int stage = 0;
+      if (counter != nullptr && !__all_sync(0xFFFFFFFFu, load_acquire(counter) >= target)) {
+        const int slot0 = ring.slot;
+        const int ahead = kind == kDown ? min(stages, kStages) : 0;
+        for (; ok && stage < ahead; ++stage) {
+          begin_stage(stage);
+          ring.advance(kStages);
+        }
+        if (ok) {
+          ok = __all_sync(0xFFFFFFFFu, wait_for_count(counter, target, abort_flag));
+          if (!ok && lane == 0) report_error(p.error, 51);
+        }
+        for (int i = 0; ok && i < ahead; ++i) bring_columns(i, (slot0 + i) % kStages);
+      }
+      for (; ok && stage < stages; ++stage) {
+        begin_stage(stage);
+        if (ok) bring_columns(stage, ring.slot);
         ring.advance(kStages);
       }
       if (!ok || kind == kExit) break;
@@ -712,10 +763,9 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
   }
 
   // ---- products ------------------------------------------------------------------------------
-  const int g = lane >> 2, t = lane & 3, tile_in_unit = warp >> 1, half = warp & 1;
-  const int inner_slabs = slabs_of(p.inner), places = p.top + p.shared;
+  const int tile0 = warp / 4 * kWarpTiles, block0 = (warp & 3) * kWarpBlocks, places = p.top + p.shared;
   tile::Ring ring;
-  F32x2 total[2][2] = {{0, 0}, {0, 0}};
+  F32x2 total[kWarpTiles][2][2] = {};
   for (;;) {
     if (!mbar_wait_warp(full + ring.slot, ring.phase, abort_flag)) {
       if (threadIdx.x == 0 && *abort_flag == 0) report_error(p.error, 53);
@@ -725,14 +775,16 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
     const StageInfo& info = infos[ring.slot];
     const int kind = info.kind, last = info.last, unit = info.unit, group = info.group, count = info.count;
     if (kind == kExit) return;
-    const int tiles = info.tiles, entry = lane < count ? info.entries[lane] : 0;
-    if (kind != kCombine && tile_in_unit < tiles) {
+    const int entry = lane < count ? info.entries[lane] : 0;
+    if (kind != kCombine && tile0 < info.tiles) {
       const uint8_t* const stage = smem + ring.slot * S::kStage;
-      const uint8_t* const records = stage + tile_in_unit * S::kTileBytes + half * kSlabBlocks * S::kRecord;
-      const uint8_t* const columns = stage + S::kWeights + half * kSlabBytes;
-      const int blocks = max(0, min(kSlabBlocks, info.blocks - half * kSlabBlocks));
-      if (count * kTerms <= 8) multiply<kFormat, 1>(records, columns, blocks, total);
-      else multiply<kFormat, 2>(records, columns, blocks, total);
+      const int tiles = info.tiles;
+      const uint8_t* const records = stage + (block0 * tiles + tile0) * S::kRecord;
+      const uint8_t* const columns = stage + S::kWeights + block0 * 64;
+      const uint8_t* const scales = stage + S::kScales + block0 * 4;
+      const int blocks = info.blocks - block0;
+      if (count * kTerms <= 8) multiply<kFormat, 1>(records, tiles, columns, scales, blocks, total);
+      else multiply<kFormat, 2>(records, tiles, columns, scales, blocks, total);
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + ring.slot);
@@ -771,61 +823,69 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
     }
     if (!last) continue;
 
-    // ---- the unit's sums: two warps per tile -------------------------------------------------
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        uint32_t a, b;
-        tile::unpack2(total[n][r], a, b);
-        reduce[warp * kReduceStride + n * 128 + (2 * r) * 32 + lane] = __uint_as_float(a);
-        reduce[warp * kReduceStride + n * 128 + (2 * r + 1) * 32 + lane] = __uint_as_float(b);
-        total[n][r] = 0;
-      }
-    }
-    math_barrier();
-    // Row g (or g + 8) of a tile for token c: its terms, each from both warps.
-    const auto sum_of = [&](int tile_at, int row, int c) {
+    // ---- the unit's sums: four warps per pair of tiles, eight columns at a time -----------------
+    // Row g (or g + 8) of a tile, a token's terms, from the four warps that have a part.
+    const auto sum_of = [&](int tile_at, int row, int column0) {
       float v = 0.0f;
 #pragma unroll
       for (int term = kTerms - 1; term >= 0; --term) {
-        const int column = c * kTerms + term;
-        const float* const at = reduce + 2 * tile_at * kReduceStride + (column >> 3) * 128 +
-                                (2 * (row >> 3) + (column & 1)) * 32 + (row & 7) * 4 + ((column & 7) >> 1);
-        v += at[0] + at[kReduceStride];
+        const int c = column0 + term;
+        const float* const at = reduce + tile_at / kWarpTiles * 4 * kReduceWarp + tile_at % kWarpTiles * kReduceTile +
+                                (2 * (row >> 3) + (c & 1)) * 32 + (row & 7) * 4 + (c >> 1);
+        v += (at[0] + at[kReduceWarp]) + (at[2 * kReduceWarp] + at[3 * kReduceWarp]);
       }
       return v;
     };
-    if (kind == kUp) {
-      // a warp takes a token, a lane a column of the inner activations: a block of 32
-      for (int c = warp; c < count; c += kMathWarps) {
-        const float gate = sum_of(lane >> 3, lane & 7, c), up = sum_of(lane >> 3, 8 + (lane & 7), c);
-        float a = projection_activation(gate, p.activation) * up;
-        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(a) & 0x7FFFFFFFu);
-        const float2 factor = block_factor(top);
-        a *= factor.x;
-        const int row = __shfl_sync(0xFFFFFFFFu, entry, c);
+    constexpr int kTokens = 8 / kTerms;  // in eight columns
 #pragma unroll
-        for (int term = 0; term < kTerms; ++term) {
-          uint8_t* const to = p.inner_terms + (static_cast<long long>(row * kTerms + term) * inner_slabs + (unit >> 2)) * kSlabBytes;
-          const __half h = __float2half_rn(a);
-          reinterpret_cast<__half*>(to + (unit & 3) * 64)[lane] = h;
-          a -= __half2float(h);
-          if (lane == 0) reinterpret_cast<float*>(to + 256)[unit & 3] = factor.y;
+    for (int n = 0; n < 2; ++n) {
+      if (n * kTokens >= count) continue;
+#pragma unroll
+      for (int i = 0; i < kWarpTiles; ++i) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint32_t a, b;
+          tile::unpack2(total[i][n][r], a, b);
+          float* const to = reduce + warp * kReduceWarp + i * kReduceTile + 2 * r * 32 + lane;
+          to[0] = __uint_as_float(a);
+          to[32] = __uint_as_float(b);
+          total[i][n][r] = 0;
         }
       }
-      proxy_fence();
-    } else {
-      const int r = threadIdx.x & (kUnitRows - 1), row = unit * kUnitRows + r;
-      for (int c0 = 0; c0 < count; c0 += 256 / kUnitRows) {
-        const int c = c0 + static_cast<int>(threadIdx.x) / kUnitRows, at = __shfl_sync(0xFFFFFFFFu, entry, c & 31);
-        if (c < count && row < p.dim) p.products[static_cast<long long>(at) * p.dim + row] = sum_of(r >> 4, r & 15, c);
+      math_barrier();
+      if (kind == kUp) {
+        // a warp takes a token, a lane a column of the inner activations: a block of 32
+        const int c = n * kTokens + warp;
+        if (warp < kTokens && c < count) {
+          const float gate = sum_of(lane >> 3, lane & 7, warp * kTerms), up = sum_of(lane >> 3, 8 + (lane & 7), warp * kTerms);
+          float a = projection_activation(gate, p.activation) * up;
+          const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(a) & 0x7FFFFFFFu);
+          const float2 factor = block_factor(top);
+          a *= factor.x;
+          const long long row = static_cast<long long>(__shfl_sync(0xFFFFFFFFu, entry, c)) * kTerms;
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term) {
+            const __half h = __float2half_rn(a);
+            p.inner_terms[(row + term) * p.inner + unit * 32 + lane] = h;
+            a -= __half2float(h);
+            if (lane == 0) p.inner_scales[(row + term) * scales_of(p.inner) + unit] = factor.y;
+          }
+        }
+      } else {
+        const int r = threadIdx.x & (kUnitRows - 1), row = unit * kUnitRows + r;
+        for (int c0 = 0; c0 < kTokens; c0 += 32 * kMathWarps / kUnitRows) {
+          const int in = c0 + static_cast<int>(threadIdx.x) / kUnitRows, c = n * kTokens + in;
+          const int at = __shfl_sync(0xFFFFFFFFu, entry, c & 31);
+          if (in < kTokens && c < count && row < p.dim) {
+            p.products[static_cast<long long>(at) * p.dim + row] = sum_of(r >> 4, r & 15, in * kTerms);
+          }
+        }
       }
+      math_barrier();
     }
-    math_barrier();
     if (threadIdx.x == 0) {
       __threadfence();
-      atomicAdd(kind == kUp ? p.up_done + group : &p.plan->down_done, 1);
+      atomicAdd(kind == kUp ? p.up_done + group : &p.progress->down_done, 1);
     }
   }
 }
@@ -846,15 +906,17 @@ qx_status check_prepare(int format, const void* gate, const void* up, const void
   return QX_STATUS_OK;
 }
 
-qx_status relayout(int format, const uint8_t* first, const uint8_t* second, uint8_t* to, long long rows, int columns,
+// `count` experts of `rows` rows.
+qx_status relayout(int format, const uint8_t* first, const uint8_t* second, uint8_t* to, int count, int rows, int columns,
                    cudaStream_t stream) {
-  const long long tiles = (second == nullptr ? rows : 2 * rows) / kTileRows, records = tiles * (columns / 32);
+  const int each = (second == nullptr ? rows : 2 * rows) / kTileRows;
+  const long long tiles = static_cast<long long>(count) * each, records = tiles * (columns / 32);
   const long long grid = (records + 7) / 8;
   if (grid > 0x7FFFFFFFLL) return QX_STATUS_INVALID_SHAPE;
   if (format == QX_FORMAT_Q4_0) {
-    moe_relayout_kernel<QX_FORMAT_Q4_0><<<static_cast<unsigned>(grid), 256, 0, stream>>>(first, second, to, tiles, columns / 32);
+    moe_relayout_kernel<QX_FORMAT_Q4_0><<<static_cast<unsigned>(grid), 256, 0, stream>>>(first, second, to, tiles, each, columns / 32);
   } else {
-    moe_relayout_kernel<QX_FORMAT_Q8_0><<<static_cast<unsigned>(grid), 256, 0, stream>>>(first, second, to, tiles, columns / 32);
+    moe_relayout_kernel<QX_FORMAT_Q8_0><<<static_cast<unsigned>(grid), 256, 0, stream>>>(first, second, to, tiles, each, columns / 32);
   }
   QX_CUDA_TRY(cudaGetLastError());
   count_launch();
@@ -881,8 +943,8 @@ qx_status prepare(int format, const uint8_t* gate, const uint8_t* up, const uint
     QX_CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&m->up), m->up_bytes));
     QX_CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&m->down), m->down_bytes));
     if (!host) {
-      QX_TRY(relayout(format, gate, up, m->up, static_cast<long long>(inner) * count, dim, stream));
-      return relayout(format, down, nullptr, m->down, static_cast<long long>(dim) * count, inner, stream);
+      QX_TRY(relayout(format, gate, up, m->up, count, inner, dim, stream));
+      return relayout(format, down, nullptr, m->down, count, dim, inner, stream);
     }
     QX_CUDA_TRY(cudaMalloc(&temp, 3 * bytes));  // (one expert at a time)
     uint8_t* const to = static_cast<uint8_t*>(temp);
@@ -890,8 +952,8 @@ qx_status prepare(int format, const uint8_t* gate, const uint8_t* up, const uint
       QX_CUDA_TRY(cudaMemcpyAsync(to, gate + e * bytes, bytes, cudaMemcpyHostToDevice, stream));
       QX_CUDA_TRY(cudaMemcpyAsync(to + bytes, up + e * bytes, bytes, cudaMemcpyHostToDevice, stream));
       QX_CUDA_TRY(cudaMemcpyAsync(to + 2 * bytes, down + e * bytes, bytes, cudaMemcpyHostToDevice, stream));
-      QX_TRY(relayout(format, to, to + bytes, m->up + 2 * bytes * e, inner, dim, stream));
-      QX_TRY(relayout(format, to + 2 * bytes, nullptr, m->down + bytes * e, dim, inner, stream));
+      QX_TRY(relayout(format, to, to + bytes, m->up + 2 * bytes * e, 1, inner, dim, stream));
+      QX_TRY(relayout(format, to + 2 * bytes, nullptr, m->down + bytes * e, 1, dim, inner, stream));
     }
     QX_CUDA_TRY(cudaStreamSynchronize(stream));
     return QX_STATUS_OK;
@@ -976,38 +1038,38 @@ qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_ro
   p.terms = x->type == QX_STORAGE_F32 ? 2 : 1;
   p.error = ctx->error_dev;
 
-  const long long pass = std::min<long long>(tokens, kPassTokens);
-  const size_t entries = static_cast<size_t>(pass) * (p.top + p.shared);
+  const long long pass = std::min<long long>(tokens, std::min(kPassTokens, kPassEntries / (p.top + p.shared)));
+  const size_t entries = static_cast<size_t>(pass) * (p.top + p.shared), rows = static_cast<size_t>(pass) * p.terms;
   Layout l;
-  const size_t at_x = l.take(static_cast<size_t>(pass) * p.terms * slabs_of(p.dim) * kSlabBytes);
+  const size_t at_x = l.take(rows * p.dim * sizeof(__half)), at_x_scales = l.take(rows * scales_of(p.dim) * sizeof(float));
   const size_t at_logits = l.take(static_cast<size_t>(pass) * p.experts * sizeof(double));
   const size_t at_picks = l.take(entries * sizeof(int)), at_weights = l.take(entries * sizeof(float));
-  const size_t at_plan = l.take(sizeof(Plan)), at_done = l.take(entries * sizeof(int));
-  const size_t at_groups = l.take(entries * sizeof(Group)), at_list = l.take(entries * sizeof(int));
-  const size_t at_inner = l.take(entries * p.terms * slabs_of(p.inner) * kSlabBytes);
+  const size_t at_progress = l.take(sizeof(Progress)), at_done = l.take(entries * sizeof(int));
+  const size_t at_inner = l.take(entries * p.terms * p.inner * sizeof(__half));
+  const size_t at_inner_scales = l.take(entries * p.terms * scales_of(p.inner) * sizeof(float));
   const size_t at_products = l.take(entries * p.dim * sizeof(float));
   QX_TRY(workspace->reserve(l.total));
   uint8_t* const base = static_cast<uint8_t*>(workspace->base);
   p.arrivals = reinterpret_cast<int*>(base);
-  p.x_terms = base + at_x;
+  p.x_terms = reinterpret_cast<__half*>(base + at_x);
+  p.x_scales = reinterpret_cast<float*>(base + at_x_scales);
   p.logits = reinterpret_cast<double*>(base + at_logits);
   p.picks = reinterpret_cast<int*>(base + at_picks);
   p.weights = reinterpret_cast<float*>(base + at_weights);
-  p.plan = reinterpret_cast<Plan*>(base + at_plan);
+  p.progress = reinterpret_cast<Progress*>(base + at_progress);
   p.up_done = reinterpret_cast<int*>(base + at_done);
-  p.groups = reinterpret_cast<Group*>(base + at_groups);
-  p.list = reinterpret_cast<int*>(base + at_list);
-  p.inner_terms = base + at_inner;
+  p.inner_terms = reinterpret_cast<__half*>(base + at_inner);
+  p.inner_scales = reinterpret_cast<float*>(base + at_inner_scales);
   p.products = reinterpret_cast<float*>(base + at_products);
 
-  for (long long t0 = 0; t0 < tokens; t0 += kPassTokens) {
-    p.tokens = static_cast<int>(std::min<long long>(kPassTokens, tokens - t0));
+  for (long long t0 = 0; t0 < tokens; t0 += pass) {
+    p.tokens = static_cast<int>(std::min(pass, tokens - t0));
     p.x = static_cast<const uint8_t*>(x->data) + t0 * x->stride * x_size;
     p.out = static_cast<uint8_t*>(out->data) + t0 * out->stride * out_size;
     p.chosen = chosen == nullptr ? nullptr : chosen + t0 * p.top;
     p.chosen_weights = weights == nullptr ? nullptr : weights + t0 * p.top;
     const int router_ctas = (p.tokens + kRouterTokens - 1) / kRouterTokens * ((p.experts + kRouterExperts - 1) / kRouterExperts);
-    const int convert_ctas = (p.tokens * slabs_of(p.dim) + 7) / 8;
+    const int convert_ctas = (p.tokens * ((p.dim + 127) / 128) + 7) / 8;
     QX_TRY(kv::launch_behind(moe_router_kernel, router_ctas + convert_ctas, kRouterThreads, 0, stream, p));
     // (no more CTAs than there may be units)
     const long long units = static_cast<long long>(p.tokens) * (p.top + p.shared) * (p.inner / 32);

@@ -15,29 +15,27 @@ struct qx_moe {
 namespace qx {
 namespace moe {
 
-// Limits of a layer, and of one pass over it.
+// Limits of a layer, and of one pass over it: tokens, and (token, expert) pairs.
 constexpr int kMostExperts = 512, kMostShared = 32, kMostTop = 32, kMostWidth = 65536;
-constexpr int kPassTokens = 128;
+constexpr int kPassTokens = 128, kPassEntries = 1024;
 
-// Weights lie as tiles of 16 rows; a tile is a row of records, one per 32 columns: the codes as a warp's lanes take
-// them (lane (g, t): columns 8 t .. 8 t + 7 of rows g and g + 8), then {d of row g, d of row g + 8} as f16 pairs. A tile
-// of the first matrix is 8 rows of the gate and the same 8 of the up projection.
-constexpr int kTileRows = 16;
+// Weights lie as records of a tile of 16 rows and a block of 32 columns: the codes as a warp's lanes take them (lane
+// (g, t): columns 8 t .. 8 t + 7 of rows g and g + 8), then {d of row g, d of row g + 8} as f16 pairs. Four tiles of an expert
+// (a unit of work; the last may have two) lie together, block by block, so that a stage of any number of blocks is one
+// run of bytes. A tile of the first matrix is 8 rows of the gate and the same 8 of the up projection.
+constexpr int kTileRows = 16, kUnitTiles = 4;
 constexpr int record_bytes(int format) { return (format == QX_FORMAT_Q4_0 ? 256 : 512) + 32; }
 
-// Activations lie as slabs of four blocks of 32 columns: 4 x 32 f16 values, then their four f32 scales.
-constexpr int kSlabBlocks = 4, kSlabBytes = kSlabBlocks * (64 + 4);
-inline __host__ __device__ int slabs_of(int columns) { return (columns / 32 + kSlabBlocks - 1) / kSlabBlocks; }
+// Activations lie as rows of f16 values, a row per token and term, and beside them an f32 scale per 32 of them. Rows of
+// scales are whole 16-byte pieces.
+inline __host__ __device__ int scales_of(int columns) { return (columns / 32 + 3) / 4 * 4; }
 
 // Columns of a product (tokens of one expert, times the terms of an activation) that one unit of work takes.
 constexpr int kColumns = 16;
 
-struct Group {
-  int expert, first, count;  // entries list[first .. first + count - 1]
-};
-// What the router leaves for the experts' kernel: `groups`, and how often each place has been counted.
-struct Plan {
-  int groups, ticket, down_done, unused;
+// How far the units of a pass have come.
+struct Progress {
+  int ticket, down_done;
 };
 
 struct Params {
@@ -62,16 +60,16 @@ struct Params {
   int32_t* chosen;       // [token][top], may be NULL
   float* chosen_weights;
   // scratch
-  int* arrivals;         // zero between calls: one per eight tokens, one for all
-  uint8_t* x_terms;      // [token][term][slab]
+  int* arrivals;         // one per eight tokens, zero between calls
+  __half* x_terms;       // [token][term][dim]
+  float* x_scales;
   double* logits;        // [token][expert]
   int* picks;            // [token][top + shared] experts
   float* weights;        // [token][top + shared]
-  Plan* plan;
-  int* up_done;          // [group]
-  Group* groups;
-  int* list;             // entries (token * (top + shared) + place), by expert, ascending
-  uint8_t* inner_terms;  // [entry][term][slab]
+  Progress* progress;
+  int* up_done;          // [group] units
+  __half* inner_terms;   // [entry][term][inner], entry = token * (top + shared) + place
+  float* inner_scales;
   float* products;       // [entry][dim]
   int* error;
 };
