@@ -786,12 +786,12 @@ typedef struct qx_moe_router {
 /* x and out: [tokens][dim], each with a type of its own; out is x itself, the same view of it, or lies elsewhere.
  * `chosen` and `weights` (either may be NULL) receive the experts and their w, [tokens][top], largest first. `activation`
  * is QX_ACTIVATION_*. Any number of tokens is served, in passes of up to 128; the kernels are made for few, whose experts' weights
- * are read once per 16 tokens (8 of f32).
+ * are read once per eight tokens of theirs (f32: four).
  * Precision. Logits are summed up in 64 bits from sums of eight f32 products, scores and weights of the router are taken in
- * 64 bits. Codes are used as they are; activations as f16 under a power of two per 32 elements: 16-bit ones exactly (an
- * element below 2^-37 of its block's largest loses bits), f32 ones to 2^-22, the products of gate and up to 2^-11 of themselves for
- * 16-bit x and 2^-22 for f32 x (no finer than 2^-38 of their block's largest, nor than 2^-135). Sums are f32, out is rounded once. A token's bits
- * do not depend on the other tokens. A token that holds a NaN or an infinity spoils its own output only.
+ * 64 bits. Codes are used as they are; x and the products of gate and up are rounded to 2^-15 of the largest of their 32
+ * neighbours (a block's columns) for 16-bit x, to 2^-23 of it for f32 x, and to 2^-103 where that is more. Sums of a block are exact, sums of
+ * blocks f32, out is rounded once. A token's bits do not depend on the other tokens. A token that holds a NaN or an
+ * infinity, or whose product of gate and up overflows, spoils its own output only.
  * What lies between the kernels is in `workspace`, one of the current device (NULL: the library's default one); calls
  * that may run at the same time need one each. */
 QX_API qx_status qx_moe_apply(const qx_moe* moe, const qx_moe_router* router, const qx_rows* x, const qx_rows* out,

@@ -9,24 +9,25 @@
 // Router (moe_router_kernel). Logits are sums of at most eight f32 products at a time, added up in 64 bits: two experts
 // on both sides of the choice are told apart as far as the inputs' own products are. A CTA takes two experts and eight tokens, a
 // warp an eighth of the columns; the last CTA to finish eight tokens chooses their experts, a warp per token. Beside them,
-// other CTAs turn the activations into f16 terms.
+// other CTAs turn the activations into digits.
 //
 // Experts (moe_experts_kernel). Every CTA sorts the (token, expert) pairs by expert, in shared memory: a microsecond, which a
 // kernel of its own or the router's last CTA would add to the launch as well. Work is cut into units that CTAs draw as tickets, in this order:
-//   up       64 rows (32 of gate, the same 32 of up) of one expert, for up to 16 columns: tokens of it, times terms
+//   up       64 rows (32 of gate, the same 32 of up) of one expert, for up to eight tokens of it (f32: four)
 //   down     64 rows of the down projection of one expert, once all of its up units are done
 //   combine  1024 elements of one token's output, once all down units are done
 // A ticket only waits for smaller ones, which their CTAs have begun: no CTA has to be resident for another to go on. A
 // warp that copies runs ahead of eight that multiply through a ring of stages, across units; where a unit has to wait for
 // others, its weights are on their way already.
 //
-// Products. Warp-level f16 MMAs with the weights as the operand of 16 rows: codes are exact in f16 (a nibble is ORed into
-// the mantissa of 1024, a byte permuted there), and one MMA pair takes a block of 32 columns, whose sum is multiplied by
-// the block's scale d and the activations' in f32. Activations are f16 under a power of two per 32 columns: 16-bit inputs
-// exactly (bar elements below 2^-37 of their block's largest), f32 inputs as two terms, hi + lo (22 bits). The product of
-// gate and up is rounded the same way: to 2^-11 of itself for 16-bit inputs (no further than their own rounding, and `inner` such errors of random signs are
-// summed up), 2^-22 for f32 ones. Two terms of a token are
-// two columns, so up to eight columns cost nothing: the MMA has them anyway.
+// Products. Whole-number MMAs (16 x 8 x 32) with the weights as the operand of 16 rows: codes as they are (q8_0), or
+// nibbles as unsigned bytes (q4_0), against the activations as balanced base-256 digits under a power of two per 32
+// columns: two digits for 16-bit inputs (2^-15 of a block's largest), three for f32 ones (2^-23). An MMA takes a block; its
+// exact sum starts at 1.5 * 2^23 as f32 bits (less 8 times the digits' sum for nibbles, which stand for n - 8), so that a
+// subtraction makes an f32 number of it, and is multiplied by the block's d and the activations' scale. The digits of a token are
+// neighbouring columns, joined at a unit's end: four tokens (f32: two) cost no more than one. (As f16 pairs on f16 MMAs the
+// conversion of the codes took three quarters of the instructions, and the layer twice the time.) The products of gate and
+// up get digits in the same way.
 //
 // A row's bits do not depend on the other tokens: columns are independent, and every sum has a fixed order.
 //
@@ -35,6 +36,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "qx_host_arrays.cuh"
 #include "qx_moe.cuh"
@@ -71,10 +73,10 @@ __global__ void __launch_bounds__(256) moe_relayout_kernel(const uint8_t* __rest
     if (kFormat == QX_FORMAT_Q4_0) {
       uint32_t word = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {  // element 8 t + i: pairs 2 p, 2 p + 1 become nibbles p, p + 4
+      for (int i = 0; i < 8; ++i) {  // elements 8 t + i and 8 t + 4 + i share byte i
         const int e = 8 * t + i;
         const uint32_t byte = from[2 + (e & 15)], nibble = e < 16 ? byte & 15 : byte >> 4;
-        word |= nibble << (4 * (i >> 1) + 16 * (i & 1));
+        word |= nibble << (8 * (i & 3) + 4 * (i >> 2));
       }
       reinterpret_cast<uint32_t*>(out)[2 * lane + h] = word;
     } else {
@@ -82,8 +84,8 @@ __global__ void __launch_bounds__(256) moe_relayout_kernel(const uint8_t* __rest
       for (int w = 0; w < 2; ++w) {
         uint32_t word = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) word |= static_cast<uint32_t>(from[2 + 8 * t + 4 * w + i] ^ 0x80) << (8 * i);
-        reinterpret_cast<uint32_t*>(out)[4 * lane + 2 * h + w] = word;  // code + 128
+        for (int i = 0; i < 4; ++i) word |= static_cast<uint32_t>(from[2 + 8 * t + 4 * w + i]) << (8 * i);
+        reinterpret_cast<uint32_t*>(out)[4 * lane + 2 * w + h] = word;
       }
     }
     if (t == 0) {
@@ -118,16 +120,26 @@ struct Words {
   }
 };
 
-__device__ __forceinline__ uint32_t pair_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+constexpr int kZeroSum = 0x4B400000;  // 1.5 * 2^23: whole numbers below 2^22 added to the bits are exact
 
-// {factor, inverse} that bring the largest magnitude of a block (as f32 bits) to 2^13 .. 2^14.
-__device__ __forceinline__ float2 block_factor(uint32_t top) {
-  const int exponent = max(30, static_cast<int>(top >> 23));
-  return make_float2(__uint_as_float(static_cast<uint32_t>(267 - exponent) << 23),
-                     __uint_as_float(static_cast<uint32_t>(exponent - 13) << 23));
+// The power of two that brings a block whose largest magnitude is `top` (as f32 bits) to what two or three balanced digits
+// hold (127 * 257, 127 * 65793), and its inverse; NaN for a block that holds a NaN or an infinity.
+struct Factor {
+  float up, down;
+};
+__device__ __forceinline__ Factor block_factor(uint32_t top, int digits) {
+  const int bits = digits == 2 ? 14 : 22, exponent = max(47, static_cast<int>((top + 0x10200u) >> 23));
+  return {__uint_as_float(static_cast<uint32_t>(bits + 254 - exponent) << 23),
+          top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(exponent - bits) << 23)};
+}
+// The digits of a value under its block's factor: signed bytes, the lowest first.
+__device__ __forceinline__ uint32_t digits_of(float v, const Factor& f, int digits) {
+  const int whole = f.down != f.down ? 0 : __float2int_rn(v * f.up);
+  const uint32_t half = digits == 2 ? 0x8080u : 0x808080u;
+  return (static_cast<uint32_t>(whole) + half) ^ half;
 }
 
-// A warp turns 128 columns of a token into terms.
+// A warp turns 128 columns of a token into digits.
 __device__ __forceinline__ void convert_columns(const Params& p, int token, int part) {
   const int lane = threadIdx.x & 31, d = part * 128 + lane * 4;
   float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -137,21 +149,21 @@ __device__ __forceinline__ void convert_columns(const Params& p, int token, int 
   for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
 #pragma unroll
   for (int h = 1; h < 8; h <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, h));
-  const float2 factor = block_factor(top);
+  const Factor factor = block_factor(top, p.digits);
+  uint32_t x[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] *= factor.x;
-  for (int term = 0; term < p.terms; ++term) {
-    const long long row = static_cast<long long>(token) * p.terms + term;
-    __half2 h[2];
+  for (int e = 0; e < 4; ++e) x[e] = digits_of(v[e], factor, p.digits);
+  for (int digit = 0; digit < p.digits; ++digit) {
+    const uint32_t select = digit | (4 + digit) << 4;
+    const uint32_t word = __byte_perm(__byte_perm(x[0], x[1], select), __byte_perm(x[2], x[3], select), 0x5410);
+    int sum = __dp4a(static_cast<int>(word), 0x01010101, 0);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      h[e] = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
-      const float2 back = __half22float2(h[e]);
-      v[2 * e] -= back.x;
-      v[2 * e + 1] -= back.y;
+    for (int h = 1; h < 8; h <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, h);
+    const long long row = static_cast<long long>(token) * p.digits + digit;
+    if (d < p.dim) {
+      *reinterpret_cast<uint32_t*>(p.x_digits + row * p.dim + d) = word;
+      if ((lane & 7) == 0) p.x_blocks[row * blocks_of(p.dim) + d / 32] = {factor.down, kZeroSum - 8 * sum};
     }
-    if (d < p.dim) *reinterpret_cast<uint2*>(p.x_terms + row * p.dim + d) = make_uint2(pair_bits(h[0]), pair_bits(h[1]));
-    if (d < p.dim && (lane & 7) == 0) p.x_scales[row * scales_of(p.dim) + d / 32] = factor.y;
   }
 }
 
@@ -351,19 +363,18 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid
 // ---- experts -----------------------------------------------------------------------------------
 constexpr int kMathWarps = 8, kExpertThreads = 32 * (kMathWarps + 1);
 constexpr int kUnitRows = kUnitTiles * kTileRows;
-// A stage holds eight blocks of columns of a unit's four tiles; a warp takes two tiles and two of the blocks, so that
-// an activation operand read from shared memory serves two products.
-constexpr int kStageBlocks = 8, kWarpTiles = 2, kWarpBlocks = 2;
-constexpr int kColumnBytes = kStageBlocks * 64 + 64;  // the 64: eight lanes of a 16-byte load meet no conflict
-constexpr int kScaleBytes = kStageBlocks * 4;
 constexpr int kCombineWidth = 1024;
+// A warp takes two of a unit's four tiles, so that an activation operand read from shared memory serves two products,
+// and every fourth pair of a stage's blocks.
+constexpr int kWarpTiles = 2;
 constexpr int kReduceTile = 128 + 1, kReduceWarp = kWarpTiles * kReduceTile;  // floats: [row g, g + 8 x column 2 t, 2 t + 1][lane]
 enum { kUp = 0, kDown = 1, kCombine = 2, kExit = 3 };
 
-struct StageInfo {
-  int kind, blocks, last, tiles;
-  int unit, group, count, unused;
-  uint16_t entries[kColumns];
+// What a unit is, beside its first stage.
+struct UnitInfo {
+  int kind, blocks, tiles, unit;
+  int group, count, unused[2];
+  uint16_t entries[8];
 };
 // The pairs of a pass by expert, and how each expert's are cut into groups.
 struct Group {
@@ -384,22 +395,25 @@ struct SortSpace {
 template <int kFormat>
 struct ExpertShape {
   static constexpr int kRecord = record_bytes(kFormat);
-  static constexpr int kStages = kFormat == QX_FORMAT_Q4_0 ? 5 : 3;
-  static constexpr int kWeights = kStageBlocks * kUnitTiles * kRecord;
+  static constexpr int kBlocks = kFormat == QX_FORMAT_Q4_0 ? 16 : 8;  // of a stage
+  static constexpr int kStages = kFormat == QX_FORMAT_Q4_0 ? 3 : 4;
+  // Between columns: lanes of an 8-byte load, four columns at a time, and of a 16-byte one meet no conflicts.
+  static constexpr int kColumnBytes = kBlocks * 32 + 32, kBlockBytes = kBlocks * 8 + 16;
+  static constexpr int kWeights = kBlocks * kUnitTiles * kRecord;
   static constexpr int kScales = kWeights + kColumns * kColumnBytes;
-  static constexpr int kStage = kScales + kColumns * kScaleBytes;
+  static constexpr int kStage = kScales + kColumns * kBlockBytes;
   static constexpr int kReduce = kStages * kStage;
   static constexpr int kInfo = kReduce + (kMathWarps * kReduceWarp * 4 + 15) / 16 * 16;
-  static constexpr int kBars = kInfo + kStages * static_cast<int>(sizeof(StageInfo));
+  static constexpr int kBars = kInfo + kStages * static_cast<int>(sizeof(UnitInfo));
   static constexpr int kPlan = kBars + 2 * kStages * 8 + 16;
   static constexpr int kBytes = kPlan + static_cast<int>(sizeof(Plan));
   static_assert(sizeof(SortSpace) <= kStages * kStage, "sorting takes the ring's place");
 };
 
-// All threads of the CTA sort the pairs.
-__device__ __forceinline__ void sort_pairs(const Params& p, int terms, SortSpace& s, Plan& plan) {
+// All threads of the CTA sort the pairs, into groups of `most` tokens.
+__device__ __forceinline__ void sort_pairs(const Params& p, int most, SortSpace& s, Plan& plan) {
   const int experts = p.experts + p.shared, places = p.top + p.shared, entries = p.tokens * places;
-  const int most = kColumns / terms, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   for (int i = threadIdx.x; i < experts * kMaskWords; i += kExpertThreads) s.tokens[i / kMaskWords][i % kMaskWords] = 0;
   __syncthreads();
   constexpr int kEach = (kPassEntries + kExpertThreads - 1) / kExpertThreads;
@@ -471,111 +485,85 @@ __device__ __forceinline__ void sort_pairs(const Params& p, int terms, SortSpace
   __syncthreads();
 }
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// A block's sums: the operand's type is that of the codes.
+__device__ __forceinline__ void mma_block(uint32_t (&d)[4], const uint32_t (&a)[4], uint2 b, int c0, int c1, bool nibbles) {
+  if (nibbles) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %11, %10, %11};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(c0), "r"(c1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(kZeroSum));
+  }
 }
-__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
-}
-
-// The codes of a lane's columns 8 t .. 8 t + 7 of rows g and g + 8, as f16: operands of the block's two MMAs.
+// The codes of a lane's columns 8 t .. 8 t + 7 of rows g and g + 8: operands of the block's MMA.
 template <int kFormat>
-struct Codes;
-template <>
-struct Codes<QX_FORMAT_Q4_0> {
-  static __device__ __forceinline__ void load(const uint8_t* record, int lane, uint32_t (&a)[4], uint32_t (&b)[4]) {
+__device__ __forceinline__ void load_codes(const uint8_t* record, int lane, uint32_t (&a)[4]) {
+  if (kFormat == QX_FORMAT_Q4_0) {
     const uint2 w = *reinterpret_cast<const uint2*>(record + lane * 8);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t low = h == 0 ? w.x : w.y, high = low >> 8;
-      const auto even = [](uint32_t v) {  // 1024 + n - 1032
-        const uint32_t raw = (v & 0x000F000Fu) | 0x64006400u;
-        return pair_bits(__hsub2(*reinterpret_cast<const __half2*>(&raw), __half2half2(__ushort_as_half(0x6408))));
-      };
-      const auto odd = [](uint32_t v) {  // (1024 + 16 n) / 16 - 72
-        const uint32_t raw = (v & 0x00F000F0u) | 0x64006400u;
-        return pair_bits(__hfma2(*reinterpret_cast<const __half2*>(&raw), __half2half2(__ushort_as_half(0x2C00)),
-                                 __half2half2(__ushort_as_half(0xD480))));
-      };
-      a[h] = even(low);
-      a[2 + h] = odd(low);
-      b[h] = even(high);
-      b[2 + h] = odd(high);
-    }
-  }
-};
-template <>
-struct Codes<QX_FORMAT_Q8_0> {
-  static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t select) {  // 1024 + (code + 128) - 1152
-    const uint32_t raw = __byte_perm(w, 0x64646464u, select);
-    return pair_bits(__hsub2(*reinterpret_cast<const __half2*>(&raw), __half2half2(__ushort_as_half(0x6480))));
-  }
-  static __device__ __forceinline__ void load(const uint8_t* record, int lane, uint32_t (&a)[4], uint32_t (&b)[4]) {
+    a[0] = w.x & 0x0F0F0F0Fu;
+    a[1] = w.y & 0x0F0F0F0Fu;
+    a[2] = w.x >> 4 & 0x0F0F0F0Fu;
+    a[3] = w.y >> 4 & 0x0F0F0F0Fu;
+  } else {
     const uint4 w = *reinterpret_cast<const uint4*>(record + lane * 16);
-    a[0] = pair(w.x, 0x4140);
-    a[1] = pair(w.z, 0x4140);
-    a[2] = pair(w.x, 0x4342);
-    a[3] = pair(w.z, 0x4342);
-    b[0] = pair(w.y, 0x4140);
-    b[1] = pair(w.w, 0x4140);
-    b[2] = pair(w.y, 0x4342);
-    b[3] = pair(w.w, 0x4342);
+    a[0] = w.x;
+    a[1] = w.y;
+    a[2] = w.z;
+    a[3] = w.w;
   }
-};
+}
 
 using F32x2 = unsigned long long;
-__device__ __forceinline__ F32x2 both(float v) { return tile::pack2(__float_as_uint(v), __float_as_uint(v)); }
 __device__ __forceinline__ F32x2 pair_of(float a, float b) { return tile::pack2(__float_as_uint(a), __float_as_uint(b)); }
-__device__ __forceinline__ F32x2 mul2(F32x2 a, F32x2 b) {
-  F32x2 v;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-  return v;
-}
 
-// A warp's blocks of a stage: 2 x 16 rows x 8 kN columns, sums in `total` [tile][column tile][row g, row g + 8].
-template <int kFormat, int kN>
+// A warp's blocks of a stage: 2 x 16 rows x 8 kN columns, sums in `total` [tile][column tile][row g, row g + 8]. The
+// pointers are at the warp's first pair of blocks; `blocks` is what the stage has from there on.
+template <int kFormat, int kN, bool kWhole>
 __device__ __forceinline__ void multiply(const uint8_t* records, int tiles, const uint8_t* columns, const uint8_t* scales, int blocks,
                                          F32x2 (&total)[kWarpTiles][2][2]) {
-  constexpr int kRecord = record_bytes(kFormat);
+  using S = ExpertShape<kFormat>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float2 factors[kN][2];  // of columns 2 t, 2 t + 1 and both blocks; odd columns lie behind the even ones
+  const F32x2 zero = tile::pack2(kZeroSum, kZeroSum);
 #pragma unroll
-  for (int n = 0; n < kN; ++n) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      factors[n][e] = *reinterpret_cast<const float2*>(scales + (4 * n + t + 8 * e) * kScaleBytes);
-    }
-  }
-#pragma unroll
-  for (int b = 0; b < kWarpBlocks; ++b) {
-    if (b >= blocks) continue;
-    uint32_t a[kWarpTiles][2][4];
-    float2 d[kWarpTiles];
-#pragma unroll
-    for (int i = 0; i < kWarpTiles; ++i) {
-      const uint8_t* const record = records + (b * tiles + i) * kRecord;
-      Codes<kFormat>::load(record, lane, a[i][0], a[i][1]);
-      d[i] = __half22float2(reinterpret_cast<const __half2*>(record + kRecord - 32)[g]);
-    }
+  for (int pair = 0; pair < S::kBlocks / 8; ++pair) {
+    if (!kWhole && 8 * pair >= blocks) continue;
+    uint4 block[kN][2];  // {scale, first} of both blocks, of columns 2 t and 2 t + 1; odd columns lie behind the even ones
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      const uint4 x = *reinterpret_cast<const uint4*>(columns + (8 * n + g) * kColumnBytes + b * 64 + t * 16);
-      const F32x2 s = b == 0 ? pair_of(factors[n][0].x, factors[n][1].x) : pair_of(factors[n][0].y, factors[n][1].y);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        block[n][e] = *reinterpret_cast<const uint4*>(scales + (4 * n + t + 8 * e) * S::kBlockBytes + pair * 64);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if (!kWhole && 8 * pair + b >= blocks) continue;
+      uint32_t a[kWarpTiles][4];
+      float2 d[kWarpTiles];
 #pragma unroll
       for (int i = 0; i < kWarpTiles; ++i) {
-        float sum[4];
-        mma_f16_first(sum, a[i][0], x.x, x.y);
-        mma_f16(sum, a[i][1], x.z, x.w);
-        tile::fma2(total[i][n][0], pair_of(sum[0], sum[1]), mul2(s, both(d[i].x)));
-        tile::fma2(total[i][n][1], pair_of(sum[2], sum[3]), mul2(s, both(d[i].y)));
+        const uint8_t* const record = records + ((8 * pair + b) * tiles + i) * S::kRecord;
+        load_codes<kFormat>(record, lane, a[i]);
+        d[i] = __half22float2(reinterpret_cast<const __half2*>(record + S::kRecord - 32)[g]);
+      }
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        const uint2 x = *reinterpret_cast<const uint2*>(columns + (8 * n + g) * S::kColumnBytes + (8 * pair + b) * 32 + t * 8);
+        const float s0 = __uint_as_float(b == 0 ? block[n][0].x : block[n][0].z), s1 = __uint_as_float(b == 0 ? block[n][1].x : block[n][1].z);
+        const int c0 = static_cast<int>(b == 0 ? block[n][0].y : block[n][0].w), c1 = static_cast<int>(b == 0 ? block[n][1].y : block[n][1].w);
+#pragma unroll
+        for (int i = 0; i < kWarpTiles; ++i) {
+          uint32_t sum[4];
+          mma_block(sum, a[i], x, c0, c1, kFormat == QX_FORMAT_Q4_0);
+          tile::fma2(total[i][n][0], tile::subf2(tile::pack2(sum[0], sum[1]), zero), pair_of(s0 * d[i].x, s1 * d[i].x));
+          tile::fma2(total[i][n][1], tile::subf2(tile::pack2(sum[2], sum[3]), zero), pair_of(s0 * d[i].y, s1 * d[i].y));
+        }
       }
     }
   }
@@ -608,13 +596,13 @@ __device__ __forceinline__ bool wait_for_count(const int* counter, int target, v
   }
 }
 
-template <int kFormat, int kTerms>
+template <int kFormat, int kDigits>
 __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __grid_constant__ Params p) {
   using S = ExpertShape<kFormat>;
-  constexpr int kStages = S::kStages;
+  constexpr int kStages = S::kStages, kTokens = tokens_per_eight(kDigits);
   extern __shared__ __align__(128) uint8_t smem[];
   float* const reduce = reinterpret_cast<float*>(smem + S::kReduce);
-  StageInfo* const infos = reinterpret_cast<StageInfo*>(smem + S::kInfo);
+  UnitInfo* const infos = reinterpret_cast<UnitInfo*>(smem + S::kInfo);
   uint64_t* const full = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* const empty = full + kStages;
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
@@ -632,7 +620,7 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
   asm volatile("griddepcontrol.wait;" ::: "memory");
   int next = 0;
   if (threadIdx.x == 32 * kMathWarps) next = atomicAdd(&p.progress->ticket, 1);
-  sort_pairs(p, kTerms, *reinterpret_cast<SortSpace*>(smem), plan);
+  sort_pairs(p, 2 * kTokens, *reinterpret_cast<SortSpace*>(smem), plan);
 
   const int up_blocks = p.dim / 32, down_blocks = p.inner / 32;
   const int up_units = p.inner / 32, down_tiles = p.dim / kTileRows, down_units = (down_tiles + kUnitTiles - 1) / kUnitTiles;
@@ -651,7 +639,9 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
       const int kind = ticket < ups ? kUp : ticket < ups + downs ? kDown : ticket < all ? kCombine : kExit;
       int group = 0, unit = 0, blocks = 0, tiles = 0, stages = 1, count = 0, entry = 0;
       const uint8_t* weights = nullptr;
-      int row = 0;  // lane < count * terms: the row of activations that is its column
+      // Lane c < 16 looks after column c: a digit of a token.
+      const int place = lane / 8 * kTokens + lane % 8 / kDigits, digit = lane % 8 % kDigits;
+      int row = -1;  // of the activations
       const int* counter = nullptr;  // what the unit waits for
       int target = 0;
       if (kind == kUp || kind == kDown) {
@@ -661,13 +651,13 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
         const Group work = plan.group[group];
         count = work.count;
         blocks = kind == kUp ? up_blocks : down_blocks;
-        stages = (blocks + kStageBlocks - 1) / kStageBlocks;
+        stages = (blocks + S::kBlocks - 1) / S::kBlocks;
         tiles = kind == kUp ? kUnitTiles : min(kUnitTiles, down_tiles - unit * kUnitTiles);
         const long long tile0 = static_cast<long long>(work.expert) * (kind == kUp ? p.inner / 8 : down_tiles) + unit * kUnitTiles;
         weights = (kind == kUp ? p.up : p.down) + tile0 * blocks * S::kRecord;
-        if (lane < count * kTerms) {
-          entry = plan.list[work.first + lane / kTerms];
-          row = (kind == kUp ? entry / (p.top + p.shared) : entry) * kTerms + lane % kTerms;
+        if (lane < kColumns && lane % 8 < kTokens * kDigits && place < count) {
+          entry = plan.list[work.first + place];
+          row = (kind == kUp ? entry / (p.top + p.shared) : entry) * kDigits + digit;
         }
         if (kind == kDown) {
           counter = p.up_done + group;
@@ -686,43 +676,49 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
           return;
         }
         issued = min(issued + 1, kStages);
-        const int in_stage = min(kStageBlocks, blocks - stage * kStageBlocks);
-        StageInfo& info = infos[ring.slot];
-        if (lane == 0) {
-          info.kind = kind;
-          info.blocks = in_stage;
-          info.last = stage == stages - 1;
-          info.tiles = tiles;
-          info.unit = unit;
-          info.group = group;
-          info.count = count;
+        const int in_stage = min(S::kBlocks, blocks - stage * S::kBlocks);
+        if (stage == 0) {
+          UnitInfo& info = infos[ring.slot];
+          if (lane == 0) {
+            info.kind = kind;
+            info.blocks = blocks;
+            info.tiles = tiles;
+            info.unit = unit;
+            info.group = group;
+            info.count = count;
+          }
+          if (row >= 0 && digit == 0) info.entries[place] = static_cast<uint16_t>(entry);
+          __syncwarp();
         }
-        if (lane < count * kTerms && lane % kTerms == 0) info.entries[lane / kTerms] = static_cast<uint16_t>(entry);
-        __syncwarp();
         if (lane == 0) {
           const uint32_t bytes = in_stage * tiles * S::kRecord;
           mbar_arrive_expect_tx(full + ring.slot, bytes);
           if (bytes > 0) {
-            tile::bulk_load(smem + ring.slot * S::kStage, weights + static_cast<long long>(stage) * kStageBlocks * tiles * S::kRecord, bytes,
+            tile::bulk_load(smem + ring.slot * S::kStage, weights + static_cast<long long>(stage) * S::kBlocks * tiles * S::kRecord, bytes,
                             full + ring.slot);
           }
         }
       };
-      // A column's 256 values are one 16-byte copy of each lane, the scales of all columns another.
+      // Columns, 16 bytes a lane: a column takes 2 * kBlocks lanes, its scales kBlocks / 2.
       const auto bring_columns = [&](int stage, int slot) {
-        const int in_stage = min(kStageBlocks, blocks - stage * kStageBlocks), columns = count * kTerms;
+        const int in_stage = min(S::kBlocks, blocks - stage * S::kBlocks), columns = count == 0 ? 0 : count > kTokens ? 16 : 8;
         const int width = kind == kUp ? p.dim : p.inner;
-        const __half* const values = (kind == kUp ? p.x_terms : p.inner_terms) + stage * kStageBlocks * 32 + lane * 8;
-        const float* const scales = (kind == kUp ? p.x_scales : p.inner_scales) + stage * kStageBlocks;
+        const int8_t* const digits = (kind == kUp ? p.x_digits : p.inner_digits) + stage * S::kBlocks * 32;
+        const Block* const scales = (kind == kUp ? p.x_blocks : p.inner_blocks) + stage * S::kBlocks;
         const uint32_t to = smem_u32(smem + slot * S::kStage);
-        for (int c = 0; c < columns; ++c) {
-          const long long from = __shfl_sync(0xFFFFFFFFu, row, c);
-          if (lane < in_stage * 4) copy16(to + S::kWeights + c * kColumnBytes + lane * 16, values + from * width);
+        constexpr int kLanes = 2 * S::kBlocks, kScaleLanes = S::kBlocks / 2;
+        for (int c0 = 0; c0 < columns; c0 += 32 / kLanes) {
+          const int c = c0 + lane / kLanes, part = lane % kLanes, from = __shfl_sync(0xFFFFFFFFu, row, c);
+          if (from >= 0 && part < in_stage * 2) {
+            copy16(to + S::kWeights + c * S::kColumnBytes + part * 16, digits + static_cast<long long>(from) * width + part * 16);
+          }
         }
-        const int c = lane >> 1, part = (lane & 1) * 4;
-        const long long from = __shfl_sync(0xFFFFFFFFu, row, c);
-        if (c < columns && part < in_stage) {
-          copy16(to + S::kScales + ((c >> 1) + 8 * (c & 1)) * kScaleBytes + part * 4, scales + from * scales_of(width) + part);
+        for (int c0 = 0; c0 < columns; c0 += 32 / kScaleLanes) {
+          const int c = c0 + lane / kScaleLanes, part = lane % kScaleLanes, from = __shfl_sync(0xFFFFFFFFu, row, c & 31);
+          if (c < columns && from >= 0 && part * 2 < in_stage) {
+            copy16(to + S::kScales + ((c >> 1) + 8 * (c & 1)) * S::kBlockBytes + part * 16,
+                   scales + static_cast<long long>(from) * blocks_of(width) + part * 2);
+          }
         }
         arrive_behind_copies(full + slot);
       };
@@ -763,32 +759,27 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
   }
 
   // ---- products ------------------------------------------------------------------------------
-  const int tile0 = warp / 4 * kWarpTiles, block0 = (warp & 3) * kWarpBlocks, places = p.top + p.shared;
+  const int tile0 = warp / 4 * kWarpTiles, block0 = (warp & 3) * 2, places = p.top + p.shared;
   tile::Ring ring;
   F32x2 total[kWarpTiles][2][2] = {};
-  for (;;) {
-    if (!mbar_wait_warp(full + ring.slot, ring.phase, abort_flag)) {
-      if (threadIdx.x == 0 && *abort_flag == 0) report_error(p.error, 53);
-      *abort_flag = 1;
-      return;  // (the other math warps see the flag, or run into the same wait)
-    }
-    const StageInfo& info = infos[ring.slot];
-    const int kind = info.kind, last = info.last, unit = info.unit, group = info.group, count = info.count;
-    if (kind == kExit) return;
-    const int entry = lane < count ? info.entries[lane] : 0;
-    if (kind != kCombine && tile0 < info.tiles) {
-      const uint8_t* const stage = smem + ring.slot * S::kStage;
-      const int tiles = info.tiles;
-      const uint8_t* const records = stage + (block0 * tiles + tile0) * S::kRecord;
-      const uint8_t* const columns = stage + S::kWeights + block0 * 64;
-      const uint8_t* const scales = stage + S::kScales + block0 * 4;
-      const int blocks = info.blocks - block0;
-      if (count * kTerms <= 8) multiply<kFormat, 1>(records, tiles, columns, scales, blocks, total);
-      else multiply<kFormat, 2>(records, tiles, columns, scales, blocks, total);
-    }
+  const auto wait_for_stage = [&]() {
+    if (mbar_wait_warp(full + ring.slot, ring.phase, abort_flag)) return true;
+    if (threadIdx.x == 0 && *abort_flag == 0) report_error(p.error, 53);
+    *abort_flag = 1;
+    return false;  // (the other math warps see the flag, or run into the same wait)
+  };
+  const auto free_stage = [&]() {
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + ring.slot);
     ring.advance(kStages);
+  };
+  for (;;) {
+    if (!wait_for_stage()) return;
+    const UnitInfo& info = infos[ring.slot];
+    const int kind = info.kind, unit = info.unit, group = info.group, count = info.count, tiles = info.tiles, blocks = info.blocks;
+    if (kind == kExit) return;
+    const int entry = lane < count ? info.entries[lane] : 0;
+    if (kind == kCombine) free_stage();
     if (kind == kCombine) {
       const int d = unit * kCombineWidth + static_cast<int>(threadIdx.x) * 4;
       if (d < p.dim) {
@@ -821,22 +812,42 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
       }
       continue;
     }
-    if (!last) continue;
+    bool ok = true;
+    const auto multiply_unit = [&](auto column_tiles) {
+      constexpr int kN = decltype(column_tiles)::value;
+      for (int left = blocks;;) {
+        if (tile0 < tiles) {
+          const uint8_t* const stage = smem + ring.slot * S::kStage;
+          const uint8_t* const records = stage + (block0 * tiles + tile0) * S::kRecord;
+          const uint8_t* const columns = stage + S::kWeights + block0 * 32;
+          const uint8_t* const scales = stage + S::kScales + block0 * 8;
+          if (left >= S::kBlocks) multiply<kFormat, kN, true>(records, tiles, columns, scales, S::kBlocks, total);
+          else multiply<kFormat, kN, false>(records, tiles, columns, scales, left - block0, total);
+        }
+        free_stage();
+        left -= S::kBlocks;
+        if (left <= 0) return;
+        ok = wait_for_stage();
+        if (!ok) return;
+      }
+    };
+    if (count <= kTokens) multiply_unit(std::integral_constant<int, 1>());
+    else multiply_unit(std::integral_constant<int, 2>());
+    if (!ok) return;
 
     // ---- the unit's sums: four warps per pair of tiles, eight columns at a time -----------------
-    // Row g (or g + 8) of a tile, a token's terms, from the four warps that have a part.
-    const auto sum_of = [&](int tile_at, int row, int column0) {
+    // Row g (or g + 8) of a tile, a token's digits, from the four warps that have a part.
+    const auto sum_of = [&](int tile_at, int row, int token) {
       float v = 0.0f;
 #pragma unroll
-      for (int term = kTerms - 1; term >= 0; --term) {
-        const int c = column0 + term;
+      for (int digit = kDigits - 1; digit >= 0; --digit) {
+        const int c = token * kDigits + digit;
         const float* const at = reduce + tile_at / kWarpTiles * 4 * kReduceWarp + tile_at % kWarpTiles * kReduceTile +
                                 (2 * (row >> 3) + (c & 1)) * 32 + (row & 7) * 4 + (c >> 1);
-        v += (at[0] + at[kReduceWarp]) + (at[2 * kReduceWarp] + at[3 * kReduceWarp]);
+        v = fmaf(v, 256.0f, (at[0] + at[kReduceWarp]) + (at[2 * kReduceWarp] + at[3 * kReduceWarp]));
       }
       return v;
     };
-    constexpr int kTokens = 8 / kTerms;  // in eight columns
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       if (n * kTokens >= count) continue;
@@ -857,18 +868,17 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
         // a warp takes a token, a lane a column of the inner activations: a block of 32
         const int c = n * kTokens + warp;
         if (warp < kTokens && c < count) {
-          const float gate = sum_of(lane >> 3, lane & 7, warp * kTerms), up = sum_of(lane >> 3, 8 + (lane & 7), warp * kTerms);
-          float a = projection_activation(gate, p.activation) * up;
+          const float gate = sum_of(lane >> 3, lane & 7, warp), up = sum_of(lane >> 3, 8 + (lane & 7), warp);
+          const float a = projection_activation(gate, p.activation) * up;
           const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(a) & 0x7FFFFFFFu);
-          const float2 factor = block_factor(top);
-          a *= factor.x;
-          const long long row = static_cast<long long>(__shfl_sync(0xFFFFFFFFu, entry, c)) * kTerms;
+          const Factor factor = block_factor(top, kDigits);
+          const uint32_t x = digits_of(a, factor, kDigits);
+          const long long row = static_cast<long long>(__shfl_sync(0xFFFFFFFFu, entry, c)) * kDigits;
 #pragma unroll
-          for (int term = 0; term < kTerms; ++term) {
-            const __half h = __float2half_rn(a);
-            p.inner_terms[(row + term) * p.inner + unit * 32 + lane] = h;
-            a -= __half2float(h);
-            if (lane == 0) p.inner_scales[(row + term) * scales_of(p.inner) + unit] = factor.y;
+          for (int digit = 0; digit < kDigits; ++digit) {
+            const int v = static_cast<int8_t>(x >> (8 * digit)), sum = __reduce_add_sync(0xFFFFFFFFu, v);
+            p.inner_digits[(row + digit) * p.inner + unit * 32 + lane] = static_cast<int8_t>(v);
+            if (lane == 0) p.inner_blocks[(row + digit) * blocks_of(p.inner) + unit] = {factor.down, kZeroSum - 8 * sum};
           }
         }
       } else {
@@ -877,13 +887,13 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
           const int in = c0 + static_cast<int>(threadIdx.x) / kUnitRows, c = n * kTokens + in;
           const int at = __shfl_sync(0xFFFFFFFFu, entry, c & 31);
           if (in < kTokens && c < count && row < p.dim) {
-            p.products[static_cast<long long>(at) * p.dim + row] = sum_of(r >> 4, r & 15, in * kTerms);
+            p.products[static_cast<long long>(at) * p.dim + row] = sum_of(r >> 4, r & 15, in);
           }
         }
       }
       math_barrier();
     }
-    if (threadIdx.x == 0) {
+    if (static_cast<int>(threadIdx.x) == (unit & (kMathWarps - 1)) * 32) {  // (not always the same warp's time)
       __threadfence();
       atomicAdd(kind == kUp ? p.up_done + group : &p.progress->down_done, 1);
     }
@@ -998,13 +1008,13 @@ struct Layout {
   }
 };
 
-template <int kFormat, int kTerms>
+template <int kFormat, int kDigits>
 qx_status launch_experts(const Params& p, long long grid, cudaStream_t stream) {
   static SmemOptIn opt_in;
   constexpr int bytes = ExpertShape<kFormat>::kBytes;
   static_assert(2 * (bytes + 1024) <= 228 * 1024, "two CTAs share an SM");
-  QX_TRY(opt_in.ensure(moe_experts_kernel<kFormat, kTerms>, bytes));
-  return kv::launch_behind(moe_experts_kernel<kFormat, kTerms>, grid, kExpertThreads, bytes, stream, p);
+  QX_TRY(opt_in.ensure(moe_experts_kernel<kFormat, kDigits>, bytes));
+  return kv::launch_behind(moe_experts_kernel<kFormat, kDigits>, grid, kExpertThreads, bytes, stream, p);
 }
 
 qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_rows* x, const qx_rows* out, long long tokens,
@@ -1035,31 +1045,31 @@ qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_ro
   p.out_vector = whole(out->data, out->stride * out_size);
   p.out_stride = out->stride;
   p.activation = activation;
-  p.terms = x->type == QX_STORAGE_F32 ? 2 : 1;
+  p.digits = x->type == QX_STORAGE_F32 ? 3 : 2;
   p.error = ctx->error_dev;
 
   const long long pass = std::min<long long>(tokens, std::min(kPassTokens, kPassEntries / (p.top + p.shared)));
-  const size_t entries = static_cast<size_t>(pass) * (p.top + p.shared), rows = static_cast<size_t>(pass) * p.terms;
+  const size_t entries = static_cast<size_t>(pass) * (p.top + p.shared), rows = static_cast<size_t>(pass) * p.digits;
   Layout l;
-  const size_t at_x = l.take(rows * p.dim * sizeof(__half)), at_x_scales = l.take(rows * scales_of(p.dim) * sizeof(float));
+  const size_t at_x = l.take(rows * p.dim), at_x_blocks = l.take(rows * blocks_of(p.dim) * sizeof(Block));
   const size_t at_logits = l.take(static_cast<size_t>(pass) * p.experts * sizeof(double));
   const size_t at_picks = l.take(entries * sizeof(int)), at_weights = l.take(entries * sizeof(float));
   const size_t at_progress = l.take(sizeof(Progress)), at_done = l.take(entries * sizeof(int));
-  const size_t at_inner = l.take(entries * p.terms * p.inner * sizeof(__half));
-  const size_t at_inner_scales = l.take(entries * p.terms * scales_of(p.inner) * sizeof(float));
+  const size_t at_inner = l.take(entries * p.digits * p.inner);
+  const size_t at_inner_blocks = l.take(entries * p.digits * blocks_of(p.inner) * sizeof(Block));
   const size_t at_products = l.take(entries * p.dim * sizeof(float));
   QX_TRY(workspace->reserve(l.total));
   uint8_t* const base = static_cast<uint8_t*>(workspace->base);
   p.arrivals = reinterpret_cast<int*>(base);
-  p.x_terms = reinterpret_cast<__half*>(base + at_x);
-  p.x_scales = reinterpret_cast<float*>(base + at_x_scales);
+  p.x_digits = reinterpret_cast<int8_t*>(base + at_x);
+  p.x_blocks = reinterpret_cast<Block*>(base + at_x_blocks);
   p.logits = reinterpret_cast<double*>(base + at_logits);
   p.picks = reinterpret_cast<int*>(base + at_picks);
   p.weights = reinterpret_cast<float*>(base + at_weights);
   p.progress = reinterpret_cast<Progress*>(base + at_progress);
   p.up_done = reinterpret_cast<int*>(base + at_done);
-  p.inner_terms = reinterpret_cast<__half*>(base + at_inner);
-  p.inner_scales = reinterpret_cast<float*>(base + at_inner_scales);
+  p.inner_digits = reinterpret_cast<int8_t*>(base + at_inner);
+  p.inner_blocks = reinterpret_cast<Block*>(base + at_inner_blocks);
   p.products = reinterpret_cast<float*>(base + at_products);
 
   for (long long t0 = 0; t0 < tokens; t0 += pass) {
@@ -1075,9 +1085,9 @@ qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_ro
     const long long units = static_cast<long long>(p.tokens) * (p.top + p.shared) * (p.inner / 32);
     const long long grid = std::min<long long>(2LL * ctx->prop.multiProcessorCount, units);
     if (m->format == QX_FORMAT_Q4_0) {
-      QX_TRY(p.terms == 1 ? (launch_experts<QX_FORMAT_Q4_0, 1>(p, grid, stream)) : (launch_experts<QX_FORMAT_Q4_0, 2>(p, grid, stream)));
+      QX_TRY(p.digits == 2 ? (launch_experts<QX_FORMAT_Q4_0, 2>(p, grid, stream)) : (launch_experts<QX_FORMAT_Q4_0, 3>(p, grid, stream)));
     } else {
-      QX_TRY(p.terms == 1 ? (launch_experts<QX_FORMAT_Q8_0, 1>(p, grid, stream)) : (launch_experts<QX_FORMAT_Q8_0, 2>(p, grid, stream)));
+      QX_TRY(p.digits == 2 ? (launch_experts<QX_FORMAT_Q8_0, 2>(p, grid, stream)) : (launch_experts<QX_FORMAT_Q8_0, 3>(p, grid, stream)));
     }
   }
   return QX_STATUS_OK;

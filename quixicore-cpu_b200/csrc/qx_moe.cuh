@@ -20,18 +20,23 @@ constexpr int kMostExperts = 512, kMostShared = 32, kMostTop = 32, kMostWidth = 
 constexpr int kPassTokens = 128, kPassEntries = 1024;
 
 // Weights lie as records of a tile of 16 rows and a block of 32 columns: the codes as a warp's lanes take them (lane
-// (g, t): columns 8 t .. 8 t + 7 of rows g and g + 8), then {d of row g, d of row g + 8} as f16 pairs. Four tiles of an expert
+// (g, t): columns 8 t .. 8 t + 7 of rows g and g + 8, as they are operands of an MMA), then {d of row g, d of row g + 8} as f16 pairs. Four tiles of an expert
 // (a unit of work; the last may have two) lie together, block by block, so that a stage of any number of blocks is one
 // run of bytes. A tile of the first matrix is 8 rows of the gate and the same 8 of the up projection.
 constexpr int kTileRows = 16, kUnitTiles = 4;
 constexpr int record_bytes(int format) { return (format == QX_FORMAT_Q4_0 ? 256 : 512) + 32; }
 
-// Activations lie as rows of f16 values, a row per token and term, and beside them an f32 scale per 32 of them. Rows of
-// scales are whole 16-byte pieces.
-inline __host__ __device__ int scales_of(int columns) { return (columns / 32 + 3) / 4 * 4; }
+// Activations lie as rows of 8-bit digits, a row per token and digit, and beside them, per 32 of them, their scale and
+// what a sum of products with them starts from. Rows of those are whole 16-byte pieces.
+struct Block {
+  float scale;
+  int first;
+};
+inline __host__ __device__ int blocks_of(int columns) { return (columns / 32 + 1) / 2 * 2; }
 
-// Columns of a product (tokens of one expert, times the terms of an activation) that one unit of work takes.
+// A unit of work takes 16 columns of a product: the digits of up to eight tokens (two digits) or four (three).
 constexpr int kColumns = 16;
+constexpr int tokens_per_eight(int digits) { return 8 / digits; }
 
 // How far the units of a pass have come.
 struct Progress {
@@ -56,20 +61,20 @@ struct Params {
   uint8_t* out;
   int out_type, out_vector;
   long long out_stride;
-  int tokens, activation, terms;
+  int tokens, activation, digits;
   int32_t* chosen;       // [token][top], may be NULL
   float* chosen_weights;
   // scratch
   int* arrivals;         // one per eight tokens, zero between calls
-  __half* x_terms;       // [token][term][dim]
-  float* x_scales;
+  int8_t* x_digits;      // [token][digit][dim]
+  Block* x_blocks;
   double* logits;        // [token][expert]
   int* picks;            // [token][top + shared] experts
   float* weights;        // [token][top + shared]
   Progress* progress;
   int* up_done;          // [group] units
-  __half* inner_terms;   // [entry][term][inner], entry = token * (top + shared) + place
-  float* inner_scales;
+  int8_t* inner_digits;  // [entry][digit][inner], entry = token * (top + shared) + place
+  Block* inner_blocks;
   float* products;       // [entry][dim]
   int* error;
 };

@@ -75,22 +75,25 @@ def route(m, x, top, sigmoid=False, biased=False, normalise=True, scale=1.0, cho
 def apply(m, x, top, activation=SILU, sigmoid=False, biased=False, normalise=True, scale=1.0, out_type=None, chosen=None):
     """-> the layer's output, and the limit of |kernel - output|, both in 64 bits.
 
-    Roundings of a sum of n terms: n u of the sum of their magnitudes at most, whatever the order; a product with a block
-    is one sum of 32 products inside an MMA (rounded or cut: 2 u a step, in four steps), two multiplications with scales, and the
-    blocks are added one behind the other, in two halves. So a matrix product of k columns is off by
-    (k / 32 + 12) * 2 u of sum |w x| at most. Inputs: 16-bit ones are exact, f32 ones are taken to 2^-22 of themselves, or
-    2^-38 of their block's largest. The activation's slope is below 1.13 (its argument is off, and a few u of itself);
-    relu^2 has a slope of 2 g. The inner activations are rounded to 2^-11 (16-bit x) or 2^-22 of themselves."""
+    Inputs and inner activations are digits under a power of two: off by 2^-15 (16-bit x) or 2^-23 of the largest of their
+    block of 32, or 2^-103. The sums of a block are exact. Then, in f32, the factor of a block and its product are two
+    roundings, the blocks are added one behind the other in four parts, two additions join those, and the digits are joined:
+    a matrix product of k columns is off by (k / 32 + 12) u of the sum of its terms' magnitudes at most. Those of the digits
+    are no more than |x| and 2^-6 of the block's largest. The activation's slope is below 1.13 (its argument is off, and a few
+    u of itself); relu^2 has a slope of 2 g."""
     chosen, weights, weights_off = route(m, x, top, sigmoid, biased, normalise, scale, chosen)
-    wide = x.dtype == torch.float32
-    kept, least = (2.0 ** -22, 2.0 ** -38) if wide else (0.0, 2.0 ** -38)
-    inner_kept = 2.0 ** -22 if wide else 2.0 ** -11
+    kept = 2.0 ** -23 if x.dtype == torch.float32 else 2.0 ** -15
     x = x.double()
 
     def largest(v):  # of each block of 32, spread over it
         return v.abs().unflatten(1, (-1, 32)).amax(2, keepdim=True).expand(-1, -1, 32).flatten(1)
 
-    x_off = kept * x.abs() + least * largest(x)
+    def product(v, v_off, w):
+        """v @ w.T where v is off by v_off, and how far it is off."""
+        size = v.abs() + v_off + 2.0 ** -6 * largest(v.abs() + v_off)
+        return v @ w.T, (v_off + U * (v.shape[1] / 32 + 12) * size) @ w.abs().T
+
+    x_off = kept * largest(x) + 2.0 ** -103
     out, limit = torch.zeros_like(x), torch.zeros_like(x)
     for e in range(m.experts + m.shared):
         if e < m.experts:
@@ -101,18 +104,15 @@ def apply(m, x, top, activation=SILU, sigmoid=False, biased=False, normalise=Tru
         if not len(rows):
             continue
         v, v_off = x[rows], x_off[rows]
-        sums = 2 * U * (m.dim / 32 + 12)
-        g, u = v @ m.gate[e].T, v @ m.up[e].T
-        g_off = v.abs() @ m.gate[e].abs().T * sums + v_off @ m.gate[e].abs().T
-        u_off = v.abs() @ m.up[e].abs().T * sums + v_off @ m.up[e].abs().T
+        g, g_off = product(v, v_off, m.gate[e])
+        u, u_off = product(v, v_off, m.up[e])
         f = activate(g, activation)
         slope = 2 * (g.abs() + g_off) if activation == 4 else 1.13
         f_off = slope * g_off + 8 * U * (f.abs() + g.abs())
         a = f * u
         a_off = f_off * u.abs() + (f.abs() + f_off) * u_off + U * a.abs()
-        a_off = a_off + inner_kept * (a.abs() + a_off) + least * largest(a)
-        y = a @ m.down[e].T
-        y_off = a_off @ m.down[e].abs().T + (a.abs() + a_off) @ m.down[e].abs().T * (2 * U * (m.inner / 32 + 12))
+        a_off = a_off + kept * largest(a.abs() + a_off) + 2.0 ** -103
+        y, y_off = product(a, a_off, m.down[e])
         out[rows] += w * y
         limit[rows] += w.abs() * y_off + w_off * (y.abs() + y_off) + (top + m.shared + 1) * U * (w * y).abs()
     return out, limit + HALF_STEP[out_type] * (out.abs() + limit) + (2.0 ** -25 if out_type == torch.float16 else 2.0 ** -134)

@@ -154,7 +154,7 @@ def test_what_is_no_number_stays_in_its_row(qx):
         assert torch.equal(out[t], want[t])
 
 
-@pytest.mark.parametrize("size", [2.0 ** -40, 2.0 ** -20, 2.0 ** 40])
+@pytest.mark.parametrize("size", [2.0 ** -30, 2.0 ** -20, 2.0 ** 40])
 def test_small_and_large_activations(qx, size):
     """A bilinear layer (no activation) of x times a power of two is the square of that times the layer: to the last bit in f32."""
     m = ref.layer(0, 4, 128, 96, seed=12)
