@@ -16,9 +16,9 @@
 //   up       64 rows (32 of gate, the same 32 of up) of one expert, for up to eight tokens of it (f32: four)
 //   down     64 rows of the down projection of one expert, once all of its up units are done
 //   combine  1024 elements of one token's output, once all down units are done
-// A ticket only waits for smaller ones, which their CTAs have begun: no CTA has to be resident for another to go on. A
-// warp that copies runs ahead of eight that multiply through a ring of stages, across units; where a unit has to wait for
-// others, its weights are on their way already.
+// A ticket only waits for smaller ones, which their CTAs have begun: no CTA has to be resident for another to go on. Eight
+// warps multiply what two others bring into a ring of stages: one the weights, across units as far ahead as the ring reaches,
+// one the activations, which it waits for where a unit depends on others.
 //
 // Products. Whole-number MMAs (16 x 8 x 32) with the weights as the operand of 16 rows: codes as they are (q8_0), or
 // nibbles as unsigned bytes (q4_0), against the activations as balanced base-256 digits under a power of two per 32
@@ -361,7 +361,8 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid
 }
 
 // ---- experts -----------------------------------------------------------------------------------
-constexpr int kMathWarps = 8, kExpertThreads = 32 * (kMathWarps + 1);
+constexpr int kMathWarps = 8, kExpertThreads = 32 * (kMathWarps + 2);
+constexpr int kWeightWarp = kMathWarps, kColumnWarp = kMathWarps + 1;
 constexpr int kUnitRows = kUnitTiles * kTileRows;
 constexpr int kCombineWidth = 1024;
 // A warp takes two of a unit's four tiles, so that an activation operand read from shared memory serves two products,
@@ -378,14 +379,15 @@ struct UnitInfo {
 };
 // The pairs of a pass by expert, and how each expert's are cut into groups.
 struct Group {
-  uint16_t expert, first, count;  // entries list[first .. first + count - 1]
+  uint32_t expert : 10, first : 11, count : 4;  // entries list[first .. first + count - 1]
 };
+constexpr int kAllExperts = kMostExperts + kMostShared, kMostGroups = kAllExperts + kPassEntries / 4;
 struct Plan {
   int groups;
   uint16_t list[kPassEntries];  // entries, by expert, ascending
-  Group group[kPassEntries];
+  Group group[kMostGroups];
 };
-constexpr int kAllExperts = kMostExperts + kMostShared, kMaskWords = kPassTokens / 32;
+constexpr int kMaskWords = kPassTokens / 32;
 struct SortSpace {
   uint32_t tokens[kAllExperts][kMaskWords];  // of each expert
   uint16_t first[kAllExperts];
@@ -403,9 +405,9 @@ struct ExpertShape {
   static constexpr int kScales = kWeights + kColumns * kColumnBytes;
   static constexpr int kStage = kScales + kColumns * kBlockBytes;
   static constexpr int kReduce = kStages * kStage;
-  static constexpr int kInfo = kReduce + (kMathWarps * kReduceWarp * 4 + 15) / 16 * 16;
+  static constexpr int kInfo = kReduce + (2 * kMathWarps * kReduceWarp * 4 + 15) / 16 * 16;
   static constexpr int kBars = kInfo + kStages * static_cast<int>(sizeof(UnitInfo));
-  static constexpr int kPlan = kBars + 2 * kStages * 8 + 16;
+  static constexpr int kPlan = kBars + 3 * kStages * 8 + 16;
   static constexpr int kBytes = kPlan + static_cast<int>(sizeof(Plan));
   static_assert(sizeof(SortSpace) <= kStages * kStage, "sorting takes the ring's place");
 };
@@ -414,8 +416,6 @@ struct ExpertShape {
 __device__ __forceinline__ void sort_pairs(const Params& p, int most, SortSpace& s, Plan& plan) {
   const int experts = p.experts + p.shared, places = p.top + p.shared, entries = p.tokens * places;
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-  for (int i = threadIdx.x; i < experts * kMaskWords; i += kExpertThreads) s.tokens[i / kMaskWords][i % kMaskWords] = 0;
-  __syncthreads();
   constexpr int kEach = (kPassEntries + kExpertThreads - 1) / kExpertThreads;
   int pick[kEach];
 #pragma unroll
@@ -423,6 +423,8 @@ __device__ __forceinline__ void sort_pairs(const Params& p, int most, SortSpace&
     const int i = threadIdx.x + j * kExpertThreads;
     if (i < entries) pick[j] = __ldcg(p.picks + i);
   }
+  for (int i = threadIdx.x; i < experts * kMaskWords; i += kExpertThreads) s.tokens[i / kMaskWords][i % kMaskWords] = 0;
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     const int i = threadIdx.x + j * kExpertThreads, token = i / places;
@@ -465,8 +467,10 @@ __device__ __forceinline__ void sort_pairs(const Params& p, int most, SortSpace&
     if (e < experts) {
       s.first[e] = static_cast<uint16_t>(first);
       for (int i = 0; i < cuts; ++i) {
-        plan.group[group + i] = {static_cast<uint16_t>(e), static_cast<uint16_t>(first + i * most),
-                                 static_cast<uint16_t>(min(most, count - i * most))};
+        Group& to = plan.group[group + i];
+        to.expert = static_cast<uint32_t>(e);
+        to.first = static_cast<uint32_t>(first + i * most);
+        to.count = static_cast<uint32_t>(min(most, count - i * most));
       }
     }
     __syncthreads();
@@ -488,13 +492,13 @@ __device__ __forceinline__ void sort_pairs(const Params& p, int most, SortSpace&
 // A block's sums: the operand's type is that of the codes.
 __device__ __forceinline__ void mma_block(uint32_t (&d)[4], const uint32_t (&a)[4], uint2 b, int c0, int c1, bool nibbles) {
   if (nibbles) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%10, %11, %10, %11};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(c0), "r"(c1));
   } else {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%10, %10, %10, %10};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
@@ -523,13 +527,14 @@ using F32x2 = unsigned long long;
 __device__ __forceinline__ F32x2 pair_of(float a, float b) { return tile::pack2(__float_as_uint(a), __float_as_uint(b)); }
 
 // A warp's blocks of a stage: 2 x 16 rows x 8 kN columns, sums in `total` [tile][column tile][row g, row g + 8]. The
-// pointers are at the warp's first pair of blocks; `blocks` is what the stage has from there on.
+// pointers are at the warp's first pair of blocks; `blocks` is what the stage has from there on. kWhole: all of four tiles.
 template <int kFormat, int kN, bool kWhole>
-__device__ __forceinline__ void multiply(const uint8_t* records, int tiles, const uint8_t* columns, const uint8_t* scales, int blocks,
+__device__ __forceinline__ void multiply(const uint8_t* records, int tiles_there, const uint8_t* columns, const uint8_t* scales, int blocks,
                                          F32x2 (&total)[kWarpTiles][2][2]) {
   using S = ExpertShape<kFormat>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const F32x2 zero = tile::pack2(kZeroSum, kZeroSum);
+  const int tiles = kWhole ? kUnitTiles : tiles_there;
 #pragma unroll
   for (int pair = 0; pair < S::kBlocks / 8; ++pair) {
     if (!kWhole && 8 * pair >= blocks) continue;
@@ -605,13 +610,15 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
   UnitInfo* const infos = reinterpret_cast<UnitInfo*>(smem + S::kInfo);
   uint64_t* const full = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* const empty = full + kStages;
-  volatile int* const abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
+  uint64_t* const begun = empty + kStages;
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(begun + kStages);
   Plan& plan = *reinterpret_cast<Plan*>(smem + S::kPlan);
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(full + i, 1 + 32);  // (the weights, and each lane's copies of activations)
       mbar_init(empty + i, kMathWarps);
+      mbar_init(begun + i, 1);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -619,142 +626,160 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   int next = 0;
-  if (threadIdx.x == 32 * kMathWarps) next = atomicAdd(&p.progress->ticket, 1);
+  if (threadIdx.x == 32 * kWeightWarp) next = atomicAdd(&p.progress->ticket, 1);
   sort_pairs(p, 2 * kTokens, *reinterpret_cast<SortSpace*>(smem), plan);
 
   const int up_blocks = p.dim / 32, down_blocks = p.inner / 32;
   const int up_units = p.inner / 32, down_tiles = p.dim / kTileRows, down_units = (down_tiles + kUnitTiles - 1) / kUnitTiles;
 
-  if (warp == kMathWarps) {
-    // ---- copies ------------------------------------------------------------------------------
+  if (warp == kWeightWarp) {
+    // ---- weights, as far ahead as the ring reaches ---------------------------------------------
     const int combine_chunks = (p.dim + kCombineWidth - 1) / kCombineWidth;
     const int ups = plan.groups * up_units, downs = plan.groups * down_units, all = ups + downs + p.tokens * combine_chunks;
     tile::Ring ring;
     int issued = 0;  // stages, as far as the ring's size
     bool ok = true;
     asm volatile("fence.proxy.async;" ::: "memory");  // (the ring's place was the sorting's)
-    for (;;) {
+    for (bool more = true; ok && more;) {
       const int ticket = __shfl_sync(0xFFFFFFFFu, next, 0);
       if (lane == 0 && ticket < all) next = atomicAdd(&p.progress->ticket, 1);  // (needed a unit later)
-      const int kind = ticket < ups ? kUp : ticket < ups + downs ? kDown : ticket < all ? kCombine : kExit;
-      int group = 0, unit = 0, blocks = 0, tiles = 0, stages = 1, count = 0, entry = 0;
+      UnitInfo unit;
+      unit.kind = ticket < ups ? kUp : ticket < ups + downs ? kDown : ticket < all ? kCombine : kExit;
+      unit.blocks = unit.tiles = unit.count = unit.group = unit.unit = 0;
+      more = unit.kind != kExit;
+      int entry = 0, stages = 1;
       const uint8_t* weights = nullptr;
-      // Lane c < 16 looks after column c: a digit of a token.
-      const int place = lane / 8 * kTokens + lane % 8 / kDigits, digit = lane % 8 % kDigits;
-      int row = -1;  // of the activations
-      const int* counter = nullptr;  // what the unit waits for
-      int target = 0;
-      if (kind == kUp || kind == kDown) {
-        const int units = kind == kUp ? up_units : down_units, at = kind == kUp ? ticket : ticket - ups;
-        group = at / units;
-        unit = at - group * units;
-        const Group work = plan.group[group];
-        count = work.count;
-        blocks = kind == kUp ? up_blocks : down_blocks;
-        stages = (blocks + S::kBlocks - 1) / S::kBlocks;
-        tiles = kind == kUp ? kUnitTiles : min(kUnitTiles, down_tiles - unit * kUnitTiles);
-        const long long tile0 = static_cast<long long>(work.expert) * (kind == kUp ? p.inner / 8 : down_tiles) + unit * kUnitTiles;
-        weights = (kind == kUp ? p.up : p.down) + tile0 * blocks * S::kRecord;
-        if (lane < kColumns && lane % 8 < kTokens * kDigits && place < count) {
-          entry = plan.list[work.first + place];
-          row = (kind == kUp ? entry / (p.top + p.shared) : entry) * kDigits + digit;
-        }
-        if (kind == kDown) {
-          counter = p.up_done + group;
-          target = up_units;
-        }
-      } else if (kind == kCombine) {
-        group = (ticket - ups - downs) / combine_chunks;  // (the token)
-        unit = ticket - ups - downs - group * combine_chunks;
-        counter = &p.progress->down_done;
-        target = downs;
+      if (unit.kind == kUp || unit.kind == kDown) {
+        const bool up = unit.kind == kUp;
+        const int units = up ? up_units : down_units, at = up ? ticket : ticket - ups;
+        unit.group = at / units;
+        unit.unit = at - unit.group * units;
+        const Group work = plan.group[unit.group];
+        unit.count = work.count;
+        unit.blocks = up ? up_blocks : down_blocks;
+        unit.tiles = up ? kUnitTiles : min(kUnitTiles, down_tiles - unit.unit * kUnitTiles);
+        stages = (unit.blocks + S::kBlocks - 1) / S::kBlocks;
+        const long long tile0 = static_cast<long long>(work.expert) * (up ? p.inner / 8 : down_tiles) + unit.unit * kUnitTiles;
+        weights = (up ? p.up : p.down) + tile0 * unit.blocks * S::kRecord;
+        if (lane < unit.count) entry = plan.list[work.first + lane];
+      } else if (unit.kind == kCombine) {
+        unit.group = (ticket - ups - downs) / combine_chunks;  // (the token)
+        unit.unit = ticket - ups - downs - unit.group * combine_chunks;
       }
-      const auto begin_stage = [&](int stage) {
+      for (int stage = 0; stage < stages; ++stage) {
         ok = issued < kStages || mbar_wait_warp(empty + ring.slot, ring.phase ^ 1u, abort_flag);
-        if (!ok) {
-          if (lane == 0) report_error(p.error, 52);
-          return;
-        }
+        if (!ok) break;
         issued = min(issued + 1, kStages);
-        const int in_stage = min(S::kBlocks, blocks - stage * S::kBlocks);
         if (stage == 0) {
           UnitInfo& info = infos[ring.slot];
           if (lane == 0) {
-            info.kind = kind;
-            info.blocks = blocks;
-            info.tiles = tiles;
-            info.unit = unit;
-            info.group = group;
-            info.count = count;
+            info.kind = unit.kind;
+            info.blocks = unit.blocks;
+            info.tiles = unit.tiles;
+            info.unit = unit.unit;
+            info.group = unit.group;
+            info.count = unit.count;
           }
-          if (row >= 0 && digit == 0) info.entries[place] = static_cast<uint16_t>(entry);
+          if (lane < unit.count) info.entries[lane] = static_cast<uint16_t>(entry);
           __syncwarp();
         }
         if (lane == 0) {
-          const uint32_t bytes = in_stage * tiles * S::kRecord;
+          mbar_arrive(begun + ring.slot);
+          const uint32_t bytes = min(S::kBlocks, unit.blocks - stage * S::kBlocks) * unit.tiles * S::kRecord;
           mbar_arrive_expect_tx(full + ring.slot, bytes);
           if (bytes > 0) {
-            tile::bulk_load(smem + ring.slot * S::kStage, weights + static_cast<long long>(stage) * S::kBlocks * tiles * S::kRecord, bytes,
-                            full + ring.slot);
+            tile::bulk_load(smem + ring.slot * S::kStage, weights + static_cast<long long>(stage) * S::kBlocks * unit.tiles * S::kRecord,
+                            bytes, full + ring.slot);
           }
         }
-      };
-      // Columns, 16 bytes a lane: a column takes 2 * kBlocks lanes, its scales kBlocks / 2.
-      const auto bring_columns = [&](int stage, int slot) {
-        const int in_stage = min(S::kBlocks, blocks - stage * S::kBlocks), columns = count == 0 ? 0 : count > kTokens ? 16 : 8;
-        const int width = kind == kUp ? p.dim : p.inner;
-        const int8_t* const digits = (kind == kUp ? p.x_digits : p.inner_digits) + stage * S::kBlocks * 32;
-        const Block* const scales = (kind == kUp ? p.x_blocks : p.inner_blocks) + stage * S::kBlocks;
-        const uint32_t to = smem_u32(smem + slot * S::kStage);
-        constexpr int kLanes = 2 * S::kBlocks, kScaleLanes = S::kBlocks / 2;
-        for (int c0 = 0; c0 < columns; c0 += 32 / kLanes) {
-          const int c = c0 + lane / kLanes, part = lane % kLanes, from = __shfl_sync(0xFFFFFFFFu, row, c);
-          if (from >= 0 && part < in_stage * 2) {
-            copy16(to + S::kWeights + c * S::kColumnBytes + part * 16, digits + static_cast<long long>(from) * width + part * 16);
-          }
-        }
-        for (int c0 = 0; c0 < columns; c0 += 32 / kScaleLanes) {
-          const int c = c0 + lane / kScaleLanes, part = lane % kScaleLanes, from = __shfl_sync(0xFFFFFFFFu, row, c & 31);
-          if (c < columns && from >= 0 && part * 2 < in_stage) {
-            copy16(to + S::kScales + ((c >> 1) + 8 * (c & 1)) * S::kBlockBytes + part * 16,
-                   scales + static_cast<long long>(from) * blocks_of(width) + part * 2);
-          }
-        }
-        arrive_behind_copies(full + slot);
-      };
-      // Weights first, where the activations are not there yet.
-      int stage = 0;
-      if (counter != nullptr && !__all_sync(0xFFFFFFFFu, load_acquire(counter) >= target)) {
-        const int slot0 = ring.slot;
-        const int ahead = kind == kDown ? min(stages, kStages) : 0;
-        for (; ok && stage < ahead; ++stage) {
-          begin_stage(stage);
-          ring.advance(kStages);
-        }
-        if (ok) {
-          ok = __all_sync(0xFFFFFFFFu, wait_for_count(counter, target, abort_flag));
-          if (!ok && lane == 0) report_error(p.error, 51);
-        }
-        for (int i = 0; ok && i < ahead; ++i) bring_columns(i, (slot0 + i) % kStages);
-      }
-      for (; ok && stage < stages; ++stage) {
-        begin_stage(stage);
-        if (ok) bring_columns(stage, ring.slot);
         ring.advance(kStages);
       }
-      if (!ok || kind == kExit) break;
     }
     if (!ok) {
+      if (lane == 0 && *abort_flag == 0) report_error(p.error, 52);
       *abort_flag = 1;
-      // what is in flight has to land before the CTA's memory is another's: the last use of each stage
+      // what is in flight has to land before the CTA's memory is another's: the last use of each stage, or half a
+      // second where its activations never come
       __syncwarp();
       const unsigned long long start = global_timer_ns();
       for (int slot = 0; slot < issued; ++slot) {
         const uint32_t phase = slot < static_cast<int>(ring.slot) ? ring.phase : ring.phase ^ 1u;
-        while (!mbar_try_wait(full + slot, phase) && global_timer_ns() - start < kWaitLimitNs) {
+        while (!mbar_try_wait(full + slot, phase) && global_timer_ns() - start < kWaitLimitNs / 4) {
         }
       }
     }
+    return;
+  }
+
+  if (warp == kColumnWarp) {
+    // ---- activations, once they are there --------------------------------------------------------
+    const int downs = plan.groups * down_units;
+    tile::Ring ring;
+    bool ok = true;
+    for (;;) {
+      ok = mbar_wait_warp(begun + ring.slot, ring.phase, abort_flag);
+      if (!ok) break;
+      const UnitInfo& info = infos[ring.slot];
+      const int kind = info.kind, blocks = info.blocks, count = info.count, group = info.group;
+      const int width = kind == kUp ? p.dim : p.inner;
+      const int8_t* const digits = kind == kUp ? p.x_digits : p.inner_digits;
+      const Block* const scales = kind == kUp ? p.x_blocks : p.inner_blocks;
+      // Lane c < 16 looks after column c, a digit of a token: its row of digits.
+      const int place = lane / 8 * kTokens + lane % 8 / kDigits;
+      int row = -1;
+      if (lane < kColumns && lane % 8 < kTokens * kDigits && place < count) {
+        const int entry = info.entries[place];
+        row = (kind == kUp ? entry / (p.top + p.shared) : entry) * kDigits + lane % 8 % kDigits;
+      }
+      // 16 bytes a lane: a column takes 2 * kBlocks lanes, its scales kBlocks / 2.
+      constexpr int kLanes = 2 * S::kBlocks, kScaleLanes = S::kBlocks / 2;
+      constexpr int kTurns = kColumns * kLanes / 32, kScaleTurns = kColumns * kScaleLanes / 32;
+      int from[kTurns], scales_from[kScaleTurns];
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int r = __shfl_sync(0xFFFFFFFFu, row, i * (32 / kLanes) + lane / kLanes);
+        from[i] = r < 0 ? -1 : r * width + lane % kLanes * 16;
+      }
+#pragma unroll
+      for (int i = 0; i < kScaleTurns; ++i) {
+        const int r = __shfl_sync(0xFFFFFFFFu, row, i * (32 / kScaleLanes) + lane / kScaleLanes);
+        scales_from[i] = r < 0 ? -1 : r * blocks_of(width) + lane % kScaleLanes * 2;
+      }
+      if (kind == kDown) ok = wait_for_count(p.up_done + group, up_units, abort_flag);
+      if (kind == kCombine) ok = wait_for_count(&p.progress->down_done, downs, abort_flag);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      for (int first = 0;;) {
+        const int in_stage = min(S::kBlocks, blocks - first);
+        const uint32_t to = smem_u32(smem + ring.slot * S::kStage);
+        const bool value = lane % kLanes < in_stage * 2, scale = lane % kScaleLanes * 2 < in_stage;
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+          if (value && from[i] >= 0) {
+            copy16(to + S::kWeights + (i * (32 / kLanes) + lane / kLanes) * S::kColumnBytes + lane % kLanes * 16, digits + from[i] + first * 32);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kScaleTurns; ++i) {
+          const int c = i * (32 / kScaleLanes) + lane / kScaleLanes;
+          if (scale && scales_from[i] >= 0) {
+            copy16(to + S::kScales + ((c >> 1) + 8 * (c & 1)) * S::kBlockBytes + lane % kScaleLanes * 16, scales + scales_from[i] + first);
+          }
+        }
+        arrive_behind_copies(full + ring.slot);
+        ring.advance(kStages);
+        first += S::kBlocks;
+        if (first >= blocks) break;
+        ok = mbar_wait_warp(begun + ring.slot, ring.phase, abort_flag);
+        if (!ok) break;
+      }
+      if (!ok || kind == kExit) break;
+    }
+    if (!ok) {
+      if (lane == 0 && *abort_flag == 0) report_error(p.error, 51);
+      *abort_flag = 1;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     return;
   }
 
@@ -821,8 +846,8 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
           const uint8_t* const records = stage + (block0 * tiles + tile0) * S::kRecord;
           const uint8_t* const columns = stage + S::kWeights + block0 * 32;
           const uint8_t* const scales = stage + S::kScales + block0 * 8;
-          if (left >= S::kBlocks) multiply<kFormat, kN, true>(records, tiles, columns, scales, S::kBlocks, total);
-          else multiply<kFormat, kN, false>(records, tiles, columns, scales, left - block0, total);
+          if (left >= S::kBlocks && tiles == kUnitTiles) multiply<kFormat, kN, true>(records, tiles, columns, scales, S::kBlocks, total);
+          else multiply<kFormat, kN, false>(records, tiles, columns, scales, min(left, S::kBlocks) - block0, total);
         }
         free_stage();
         left -= S::kBlocks;
@@ -835,14 +860,14 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
     else multiply_unit(std::integral_constant<int, 2>());
     if (!ok) return;
 
-    // ---- the unit's sums: four warps per pair of tiles, eight columns at a time -----------------
+    // ---- the unit's sums: four warps per pair of tiles -------------------------------------------
     // Row g (or g + 8) of a tile, a token's digits, from the four warps that have a part.
     const auto sum_of = [&](int tile_at, int row, int token) {
       float v = 0.0f;
 #pragma unroll
       for (int digit = kDigits - 1; digit >= 0; --digit) {
-        const int c = token * kDigits + digit;
-        const float* const at = reduce + tile_at / kWarpTiles * 4 * kReduceWarp + tile_at % kWarpTiles * kReduceTile +
+        const int c = token % kTokens * kDigits + digit;
+        const float* const at = reduce + token / kTokens * kMathWarps * kReduceWarp + tile_at / kWarpTiles * 4 * kReduceWarp + tile_at % kWarpTiles * kReduceTile +
                                 (2 * (row >> 3) + (c & 1)) * 32 + (row & 7) * 4 + (c >> 1);
         v = fmaf(v, 256.0f, (at[0] + at[kReduceWarp]) + (at[2 * kReduceWarp] + at[3 * kReduceWarp]));
       }
@@ -857,42 +882,40 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
         for (int r = 0; r < 2; ++r) {
           uint32_t a, b;
           tile::unpack2(total[i][n][r], a, b);
-          float* const to = reduce + warp * kReduceWarp + i * kReduceTile + 2 * r * 32 + lane;
+          float* const to = reduce + (n * kMathWarps + warp) * kReduceWarp + i * kReduceTile + 2 * r * 32 + lane;
           to[0] = __uint_as_float(a);
           to[32] = __uint_as_float(b);
           total[i][n][r] = 0;
         }
       }
-      math_barrier();
-      if (kind == kUp) {
-        // a warp takes a token, a lane a column of the inner activations: a block of 32
-        const int c = n * kTokens + warp;
-        if (warp < kTokens && c < count) {
-          const float gate = sum_of(lane >> 3, lane & 7, warp), up = sum_of(lane >> 3, 8 + (lane & 7), warp);
-          const float a = projection_activation(gate, p.activation) * up;
-          const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(a) & 0x7FFFFFFFu);
-          const Factor factor = block_factor(top, kDigits);
-          const uint32_t x = digits_of(a, factor, kDigits);
-          const long long row = static_cast<long long>(__shfl_sync(0xFFFFFFFFu, entry, c)) * kDigits;
+    }
+    math_barrier();
+    if (kind == kUp) {
+      // a warp takes a token, a lane a column of the inner activations: a block of 32
+      static_assert(2 * kTokens <= kMathWarps, "a warp for every token");
+      if (warp < count) {
+        const float gate = sum_of(lane >> 3, lane & 7, warp), up = sum_of(lane >> 3, 8 + (lane & 7), warp);
+        const float a = projection_activation(gate, p.activation) * up;
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(a) & 0x7FFFFFFFu);
+        const Factor factor = block_factor(top, kDigits);
+        const uint32_t x = digits_of(a, factor, kDigits);
+        const long long row = static_cast<long long>(__shfl_sync(0xFFFFFFFFu, entry, warp)) * kDigits;
 #pragma unroll
-          for (int digit = 0; digit < kDigits; ++digit) {
-            const int v = static_cast<int8_t>(x >> (8 * digit)), sum = __reduce_add_sync(0xFFFFFFFFu, v);
-            p.inner_digits[(row + digit) * p.inner + unit * 32 + lane] = static_cast<int8_t>(v);
-            if (lane == 0) p.inner_blocks[(row + digit) * blocks_of(p.inner) + unit] = {factor.down, kZeroSum - 8 * sum};
-          }
-        }
-      } else {
-        const int r = threadIdx.x & (kUnitRows - 1), row = unit * kUnitRows + r;
-        for (int c0 = 0; c0 < kTokens; c0 += 32 * kMathWarps / kUnitRows) {
-          const int in = c0 + static_cast<int>(threadIdx.x) / kUnitRows, c = n * kTokens + in;
-          const int at = __shfl_sync(0xFFFFFFFFu, entry, c & 31);
-          if (in < kTokens && c < count && row < p.dim) {
-            p.products[static_cast<long long>(at) * p.dim + row] = sum_of(r >> 4, r & 15, in);
-          }
+        for (int digit = 0; digit < kDigits; ++digit) {
+          const int v = static_cast<int8_t>(x >> (8 * digit)), sum = __reduce_add_sync(0xFFFFFFFFu, v);
+          p.inner_digits[(row + digit) * p.inner + unit * 32 + lane] = static_cast<int8_t>(v);
+          if (lane == 0) p.inner_blocks[(row + digit) * blocks_of(p.inner) + unit] = {factor.down, kZeroSum - 8 * sum};
         }
       }
-      math_barrier();
+    } else {
+      const int r = threadIdx.x & (kUnitRows - 1), row = unit * kUnitRows + r;
+#pragma unroll
+      for (int c0 = 0; c0 < 2 * kTokens; c0 += 32 * kMathWarps / kUnitRows) {
+        const int c = c0 + static_cast<int>(threadIdx.x) / kUnitRows, at = __shfl_sync(0xFFFFFFFFu, entry, c);
+        if (c < count && row < p.dim) p.products[static_cast<long long>(at) * p.dim + row] = sum_of(r >> 4, r & 15, c);
+      }
     }
+    math_barrier();
     if (static_cast<int>(threadIdx.x) == (unit & (kMathWarps - 1)) * 32) {  // (not always the same warp's time)
       __threadfence();
       atomicAdd(kind == kUp ? p.up_done + group : &p.progress->down_done, 1);
