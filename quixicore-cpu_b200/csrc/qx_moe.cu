@@ -23,11 +23,11 @@
 // Products. Whole-number MMAs (16 x 8 x 32) with the weights as the operand of 16 rows: codes as they are (q8_0), or
 // nibbles as unsigned bytes (q4_0), against the activations as balanced base-256 digits under a power of two per 32
 // columns: two digits for 16-bit inputs (2^-15 of a block's largest), three for f32 ones (2^-23). An MMA takes a block; its
-// exact sum starts at 1.5 * 2^23 as f32 bits (less 8 times the digits' sum for nibbles, which stand for n - 8), so that a
-// subtraction makes an f32 number of it, and is multiplied by the block's d and the activations' scale. The digits of a token are
-// neighbouring columns, joined at a unit's end: four tokens (f32: two) cost no more than one. (As f16 pairs on f16 MMAs the
-// conversion of the codes took three quarters of the instructions, and the layer twice the time.) The products of gate and
-// up get digits in the same way.
+// exact sum starts at 1.5 * 2^23 as f32 bits, so that a subtraction (for nibbles, which stand for n - 8, of 8 times the
+// digits' sum more) makes an f32 number of it. A token's digits are neighbouring columns: a lane joins two of them and
+// multiplies with the block's d and the activations' scale. Four tokens (f32: two) cost no more than one. (As f16 pairs on f16
+// MMAs the conversion of the codes took three quarters of the instructions, and the layer twice the time.) The products of
+// gate and up get digits in the same way.
 //
 // A row's bits do not depend on the other tokens: columns are independent, and every sum has a fixed order.
 //
@@ -139,6 +139,14 @@ __device__ __forceinline__ uint32_t digits_of(float v, const Factor& f, int digi
   return (static_cast<uint32_t>(whole) + half) ^ half;
 }
 
+// What the products with a block of activations need: `sums` of its digits.
+__device__ __forceinline__ void store_blocks(const Params& p, Block* to, int row, int blocks, int block, float scale, const int (&sums)[3]) {
+  const int pairs = columns_of(p.digits) / 2, each = p.nibbles ? 8 : 0;
+  Block* const at = to + static_cast<long long>(row) * pairs * blocks + block;
+  at[0] = {{kZeroSum + each * sums[0], kZeroSum + each * sums[1]}, scale, 0};
+  if (pairs > 1) at[blocks] = {{kZeroSum + each * sums[2], kZeroSum}, scale, 0};
+}
+
 // A warp turns 128 columns of a token into digits.
 __device__ __forceinline__ void convert_columns(const Params& p, int token, int part) {
   const int lane = threadIdx.x & 31, d = part * 128 + lane * 4;
@@ -153,18 +161,18 @@ __device__ __forceinline__ void convert_columns(const Params& p, int token, int 
   uint32_t x[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = digits_of(v[e], factor, p.digits);
-  for (int digit = 0; digit < p.digits; ++digit) {
+  int sums[3] = {0, 0, 0};
+#pragma unroll
+  for (int digit = 0; digit < 3; ++digit) {
+    if (digit >= p.digits) continue;
     const uint32_t select = digit | (4 + digit) << 4;
     const uint32_t word = __byte_perm(__byte_perm(x[0], x[1], select), __byte_perm(x[2], x[3], select), 0x5410);
-    int sum = __dp4a(static_cast<int>(word), 0x01010101, 0);
+    sums[digit] = __dp4a(static_cast<int>(word), 0x01010101, 0);
 #pragma unroll
-    for (int h = 1; h < 8; h <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, h);
-    const long long row = static_cast<long long>(token) * p.digits + digit;
-    if (d < p.dim) {
-      *reinterpret_cast<uint32_t*>(p.x_digits + row * p.dim + d) = word;
-      if ((lane & 7) == 0) p.x_blocks[row * blocks_of(p.dim) + d / 32] = {factor.down, kZeroSum - 8 * sum};
-    }
+    for (int h = 1; h < 8; h <<= 1) sums[digit] += __shfl_xor_sync(0xFFFFFFFFu, sums[digit], h);
+    if (d < p.dim) *reinterpret_cast<uint32_t*>(p.x_digits + (static_cast<long long>(token) * p.digits + digit) * p.dim + d) = word;
   }
+  if (d < p.dim && (lane & 7) == 0) store_blocks(p, p.x_blocks, token, p.dim / 32, d / 32, factor.down, sums);
 }
 
 // Order-preserving whole number of a double; NaN is above everything.
@@ -365,10 +373,7 @@ constexpr int kMathWarps = 8, kExpertThreads = 32 * (kMathWarps + 2);
 constexpr int kWeightWarp = kMathWarps, kColumnWarp = kMathWarps + 1;
 constexpr int kUnitRows = kUnitTiles * kTileRows;
 constexpr int kCombineWidth = 1024;
-// A warp takes two of a unit's four tiles, so that an activation operand read from shared memory serves two products,
-// and every fourth pair of a stage's blocks.
-constexpr int kWarpTiles = 2;
-constexpr int kReduceTile = 128 + 1, kReduceWarp = kWarpTiles * kReduceTile;  // floats: [row g, g + 8 x column 2 t, 2 t + 1][lane]
+constexpr int kReduceTile = 64 + 1, kReduceWarp = kUnitTiles * kReduceTile;  // floats: [row g, g + 8][lane]
 enum { kUp = 0, kDown = 1, kCombine = 2, kExit = 3 };
 
 // What a unit is, beside its first stage.
@@ -399,11 +404,11 @@ struct ExpertShape {
   static constexpr int kRecord = record_bytes(kFormat);
   static constexpr int kBlocks = kFormat == QX_FORMAT_Q4_0 ? 16 : 8;  // of a stage
   static constexpr int kStages = kFormat == QX_FORMAT_Q4_0 ? 3 : 4;
-  // Between columns: lanes of an 8-byte load, four columns at a time, and of a 16-byte one meet no conflicts.
-  static constexpr int kColumnBytes = kBlocks * 32 + 32, kBlockBytes = kBlocks * 8 + 16;
+  // Between columns, and pairs of them: lanes of an 8-byte load, four columns at a time, and of a 16-byte one meet no conflicts.
+  static constexpr int kColumnBytes = kBlocks * 32 + 32, kPairBytes = (kBlocks + 1) * static_cast<int>(sizeof(Block));
   static constexpr int kWeights = kBlocks * kUnitTiles * kRecord;
   static constexpr int kScales = kWeights + kColumns * kColumnBytes;
-  static constexpr int kStage = kScales + kColumns * kBlockBytes;
+  static constexpr int kStage = kScales + kColumns / 2 * kPairBytes;
   static constexpr int kReduce = kStages * kStage;
   static constexpr int kInfo = kReduce + (2 * kMathWarps * kReduceWarp * 4 + 15) / 16 * 16;
   static constexpr int kBars = kInfo + kStages * static_cast<int>(sizeof(UnitInfo));
@@ -490,16 +495,14 @@ __device__ __forceinline__ void sort_pairs(const Params& p, int most, SortSpace&
 }
 
 // A block's sums: the operand's type is that of the codes.
-__device__ __forceinline__ void mma_block(uint32_t (&d)[4], const uint32_t (&a)[4], uint2 b, int c0, int c1, bool nibbles) {
+__device__ __forceinline__ void mma_block(uint32_t (&d)[4], const uint32_t (&a)[4], uint2 b, bool nibbles) {
   if (nibbles) {
-    asm(
-        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%10, %11, %10, %11};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(c0), "r"(c1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(kZeroSum));
   } else {
-    asm(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%10, %10, %10, %10};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(kZeroSum));
@@ -523,51 +526,44 @@ __device__ __forceinline__ void load_codes(const uint8_t* record, int lane, uint
   }
 }
 
-using F32x2 = unsigned long long;
-__device__ __forceinline__ F32x2 pair_of(float a, float b) { return tile::pack2(__float_as_uint(a), __float_as_uint(b)); }
-
-// A warp's blocks of a stage: 2 x 16 rows x 8 kN columns, sums in `total` [tile][column tile][row g, row g + 8]. The
-// pointers are at the warp's first pair of blocks; `blocks` is what the stage has from there on. kWhole: all of four tiles.
+// A warp's blocks of a stage, every eighth: 64 rows x 8 kN columns, sums in `total` [tile][column tile][row g, row g + 8] of
+// the lane's pair of digits; `join`: how many of the lower digit one of the higher is. The pointers are at the warp's first
+// block; `blocks` is what the stage has from there on. kWhole: all of four tiles.
 template <int kFormat, int kN, bool kWhole>
 __device__ __forceinline__ void multiply(const uint8_t* records, int tiles_there, const uint8_t* columns, const uint8_t* scales, int blocks,
-                                         F32x2 (&total)[kWarpTiles][2][2]) {
+                                         float join, float (&total)[kUnitTiles][2][2]) {
   using S = ExpertShape<kFormat>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const F32x2 zero = tile::pack2(kZeroSum, kZeroSum);
   const int tiles = kWhole ? kUnitTiles : tiles_there;
 #pragma unroll
-  for (int pair = 0; pair < S::kBlocks / 8; ++pair) {
-    if (!kWhole && 8 * pair >= blocks) continue;
-    uint4 block[kN][2];  // {scale, first} of both blocks, of columns 2 t and 2 t + 1; odd columns lie behind the even ones
+  for (int b = 0; b < S::kBlocks / kMathWarps; ++b) {
+    if (!kWhole && b * kMathWarps >= blocks) continue;
+    uint2 x[kN];
+    uint4 block[kN];  // {zeros, scale} of the lane's pair
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        block[n][e] = *reinterpret_cast<const uint4*>(scales + (4 * n + t + 8 * e) * S::kBlockBytes + pair * 64);
-      }
+      x[n] = *reinterpret_cast<const uint2*>(columns + (8 * n + g) * S::kColumnBytes + b * kMathWarps * 32 + t * 8);
+      block[n] = *reinterpret_cast<const uint4*>(scales + (4 * n + t) * S::kPairBytes + b * kMathWarps * sizeof(Block));
     }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      if (!kWhole && 8 * pair + b >= blocks) continue;
-      uint32_t a[kWarpTiles][4];
-      float2 d[kWarpTiles];
-#pragma unroll
-      for (int i = 0; i < kWarpTiles; ++i) {
-        const uint8_t* const record = records + ((8 * pair + b) * tiles + i) * S::kRecord;
-        load_codes<kFormat>(record, lane, a[i]);
-        d[i] = __half22float2(reinterpret_cast<const __half2*>(record + S::kRecord - 32)[g]);
-      }
+    for (int i = 0; i < kUnitTiles; ++i) {
+      if (!kWhole && i >= tiles) continue;
+      const uint8_t* const record = records + (b * kMathWarps * tiles + i) * S::kRecord;
+      uint32_t a[4];
+      load_codes<kFormat>(record, lane, a);
+      const float2 d = __half22float2(reinterpret_cast<const __half2*>(record + S::kRecord - 32)[g]);
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        const uint2 x = *reinterpret_cast<const uint2*>(columns + (8 * n + g) * S::kColumnBytes + (8 * pair + b) * 32 + t * 8);
-        const float s0 = __uint_as_float(b == 0 ? block[n][0].x : block[n][0].z), s1 = __uint_as_float(b == 0 ? block[n][1].x : block[n][1].z);
-        const int c0 = static_cast<int>(b == 0 ? block[n][0].y : block[n][0].w), c1 = static_cast<int>(b == 0 ? block[n][1].y : block[n][1].w);
+        uint32_t sum[4];
+        mma_block(sum, a, x[n], kFormat == QX_FORMAT_Q4_0);
+        const unsigned long long zero = tile::pack2(block[n].x, block[n].y);
+        const float scale = __uint_as_float(block[n].z);
 #pragma unroll
-        for (int i = 0; i < kWarpTiles; ++i) {
-          uint32_t sum[4];
-          mma_block(sum, a[i], x, c0, c1, kFormat == QX_FORMAT_Q4_0);
-          tile::fma2(total[i][n][0], tile::subf2(tile::pack2(sum[0], sum[1]), zero), pair_of(s0 * d[i].x, s1 * d[i].x));
-          tile::fma2(total[i][n][1], tile::subf2(tile::pack2(sum[2], sum[3]), zero), pair_of(s0 * d[i].y, s1 * d[i].y));
+        for (int r = 0; r < 2; ++r) {
+          uint32_t low, high;
+          tile::unpack2(tile::subf2(tile::pack2(sum[2 * r], sum[2 * r + 1]), zero), low, high);
+          const float both = fmaf(__uint_as_float(high), join, __uint_as_float(low));
+          total[i][n][r] = fmaf(both, scale * (r == 0 ? d.x : d.y), total[i][n][r]);
         }
       }
     }
@@ -604,7 +600,7 @@ __device__ __forceinline__ bool wait_for_count(const int* counter, int target, v
 template <int kFormat, int kDigits>
 __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __grid_constant__ Params p) {
   using S = ExpertShape<kFormat>;
-  constexpr int kStages = S::kStages, kTokens = tokens_per_eight(kDigits);
+  constexpr int kStages = S::kStages, kSpan = columns_of(kDigits), kTokens = 8 / kSpan;
   extern __shared__ __align__(128) uint8_t smem[];
   float* const reduce = reinterpret_cast<float*>(smem + S::kReduce);
   UnitInfo* const infos = reinterpret_cast<UnitInfo*>(smem + S::kInfo);
@@ -723,27 +719,29 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
       const int kind = info.kind, blocks = info.blocks, count = info.count, group = info.group;
       const int width = kind == kUp ? p.dim : p.inner;
       const int8_t* const digits = kind == kUp ? p.x_digits : p.inner_digits;
-      const Block* const scales = kind == kUp ? p.x_blocks : p.inner_blocks;
-      // Lane c < 16 looks after column c, a digit of a token: its row of digits.
-      const int place = lane / 8 * kTokens + lane % 8 / kDigits;
-      int row = -1;
-      if (lane < kColumns && lane % 8 < kTokens * kDigits && place < count) {
-        const int entry = info.entries[place];
-        row = (kind == kUp ? entry / (p.top + p.shared) : entry) * kDigits + lane % 8 % kDigits;
+      const Block* const blocks_at = kind == kUp ? p.x_blocks : p.inner_blocks;
+      // Lane c < 16 looks after column c, a digit of a token, lane p < 8 after pair p of them: their rows.
+      int row = -1, pair_row = -1;
+      const int place = lane / kSpan, pair_place = 2 * lane / kSpan;
+      if (place < count && lane % kSpan < kDigits) {
+        row = (kind == kUp ? info.entries[place] / (p.top + p.shared) : info.entries[place]) * kDigits + lane % kSpan;
       }
-      // 16 bytes a lane: a column takes 2 * kBlocks lanes, its scales kBlocks / 2.
-      constexpr int kLanes = 2 * S::kBlocks, kScaleLanes = S::kBlocks / 2;
-      constexpr int kTurns = kColumns * kLanes / 32, kScaleTurns = kColumns * kScaleLanes / 32;
-      int from[kTurns], scales_from[kScaleTurns];
+      if (pair_place < count) {
+        pair_row = (kind == kUp ? info.entries[pair_place] / (p.top + p.shared) : info.entries[pair_place]) * (kSpan / 2) + lane % (kSpan / 2);
+      }
+      // 16 bytes a lane: a column takes 2 * kBlocks lanes, a pair's blocks kBlocks.
+      constexpr int kLanes = 2 * S::kBlocks, kPairLanes = S::kBlocks;
+      constexpr int kTurns = kColumns * kLanes / 32, kPairTurns = kColumns / 2 * kPairLanes / 32;
+      int from[kTurns], pairs_from[kPairTurns];
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
         const int r = __shfl_sync(0xFFFFFFFFu, row, i * (32 / kLanes) + lane / kLanes);
         from[i] = r < 0 ? -1 : r * width + lane % kLanes * 16;
       }
 #pragma unroll
-      for (int i = 0; i < kScaleTurns; ++i) {
-        const int r = __shfl_sync(0xFFFFFFFFu, row, i * (32 / kScaleLanes) + lane / kScaleLanes);
-        scales_from[i] = r < 0 ? -1 : r * blocks_of(width) + lane % kScaleLanes * 2;
+      for (int i = 0; i < kPairTurns; ++i) {
+        const int r = __shfl_sync(0xFFFFFFFFu, pair_row, i * (32 / kPairLanes) + lane / kPairLanes);
+        pairs_from[i] = r < 0 ? -1 : r * (width / 32) + lane % kPairLanes;
       }
       if (kind == kDown) ok = wait_for_count(p.up_done + group, up_units, abort_flag);
       if (kind == kCombine) ok = wait_for_count(&p.progress->down_done, downs, abort_flag);
@@ -752,7 +750,7 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
       for (int first = 0;;) {
         const int in_stage = min(S::kBlocks, blocks - first);
         const uint32_t to = smem_u32(smem + ring.slot * S::kStage);
-        const bool value = lane % kLanes < in_stage * 2, scale = lane % kScaleLanes * 2 < in_stage;
+        const bool value = lane % kLanes < in_stage * 2, block = lane % kPairLanes < in_stage;
 #pragma unroll
         for (int i = 0; i < kTurns; ++i) {
           if (value && from[i] >= 0) {
@@ -760,10 +758,10 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
           }
         }
 #pragma unroll
-        for (int i = 0; i < kScaleTurns; ++i) {
-          const int c = i * (32 / kScaleLanes) + lane / kScaleLanes;
-          if (scale && scales_from[i] >= 0) {
-            copy16(to + S::kScales + ((c >> 1) + 8 * (c & 1)) * S::kBlockBytes + lane % kScaleLanes * 16, scales + scales_from[i] + first);
+        for (int i = 0; i < kPairTurns; ++i) {
+          if (block && pairs_from[i] >= 0) {
+            copy16(to + S::kScales + (i * (32 / kPairLanes) + lane / kPairLanes) * S::kPairBytes + lane % kPairLanes * static_cast<int>(sizeof(Block)),
+                   blocks_at + pairs_from[i] + first);
           }
         }
         arrive_behind_copies(full + ring.slot);
@@ -784,9 +782,10 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
   }
 
   // ---- products ------------------------------------------------------------------------------
-  const int tile0 = warp / 4 * kWarpTiles, block0 = (warp & 3) * 2, places = p.top + p.shared;
+  const int places = p.top + p.shared;
+  const float join = kSpan == 4 && (lane & 1) ? 0.0f : 256.0f;  // (a third digit stands alone)
   tile::Ring ring;
-  F32x2 total[kWarpTiles][2][2] = {};
+  float total[kUnitTiles][2][2] = {};
   const auto wait_for_stage = [&]() {
     if (mbar_wait_warp(full + ring.slot, ring.phase, abort_flag)) return true;
     if (threadIdx.x == 0 && *abort_flag == 0) report_error(p.error, 53);
@@ -841,14 +840,12 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
     const auto multiply_unit = [&](auto column_tiles) {
       constexpr int kN = decltype(column_tiles)::value;
       for (int left = blocks;;) {
-        if (tile0 < tiles) {
-          const uint8_t* const stage = smem + ring.slot * S::kStage;
-          const uint8_t* const records = stage + (block0 * tiles + tile0) * S::kRecord;
-          const uint8_t* const columns = stage + S::kWeights + block0 * 32;
-          const uint8_t* const scales = stage + S::kScales + block0 * 8;
-          if (left >= S::kBlocks && tiles == kUnitTiles) multiply<kFormat, kN, true>(records, tiles, columns, scales, S::kBlocks, total);
-          else multiply<kFormat, kN, false>(records, tiles, columns, scales, min(left, S::kBlocks) - block0, total);
-        }
+        const uint8_t* const stage = smem + ring.slot * S::kStage;
+        const uint8_t* const records = stage + warp * tiles * S::kRecord;
+        const uint8_t* const columns = stage + S::kWeights + warp * 32;
+        const uint8_t* const scales = stage + S::kScales + warp * sizeof(Block);
+        if (left >= S::kBlocks && tiles == kUnitTiles) multiply<kFormat, kN, true>(records, tiles, columns, scales, S::kBlocks, join, total);
+        else multiply<kFormat, kN, false>(records, tiles, columns, scales, min(left, S::kBlocks) - warp, join, total);
         free_stage();
         left -= S::kBlocks;
         if (left <= 0) return;
@@ -860,35 +857,33 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
     else multiply_unit(std::integral_constant<int, 2>());
     if (!ok) return;
 
-    // ---- the unit's sums: four warps per pair of tiles -------------------------------------------
-    // Row g (or g + 8) of a tile, a token's digits, from the four warps that have a part.
-    const auto sum_of = [&](int tile_at, int row, int token) {
-      float v = 0.0f;
-#pragma unroll
-      for (int digit = kDigits - 1; digit >= 0; --digit) {
-        const int c = token % kTokens * kDigits + digit;
-        const float* const at = reduce + token / kTokens * kMathWarps * kReduceWarp + tile_at / kWarpTiles * 4 * kReduceWarp + tile_at % kWarpTiles * kReduceTile +
-                                (2 * (row >> 3) + (c & 1)) * 32 + (row & 7) * 4 + (c >> 1);
-        v = fmaf(v, 256.0f, (at[0] + at[kReduceWarp]) + (at[2 * kReduceWarp] + at[3 * kReduceWarp]));
-      }
-      return v;
-    };
+    // ---- the unit's sums: every warp has a part of each ------------------------------------------
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       if (n * kTokens >= count) continue;
 #pragma unroll
-      for (int i = 0; i < kWarpTiles; ++i) {
+      for (int i = 0; i < kUnitTiles; ++i) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          uint32_t a, b;
-          tile::unpack2(total[i][n][r], a, b);
-          float* const to = reduce + (n * kMathWarps + warp) * kReduceWarp + i * kReduceTile + 2 * r * 32 + lane;
-          to[0] = __uint_as_float(a);
-          to[32] = __uint_as_float(b);
-          total[i][n][r] = 0;
+          reduce[(n * kMathWarps + warp) * kReduceWarp + i * kReduceTile + r * 32 + lane] = total[i][n][r];
+          total[i][n][r] = 0.0f;
         }
       }
     }
+    // Row g (or g + 8) of a tile for a token: its pairs of digits, from all warps.
+    const auto sum_of = [&](int tile_at, int row, int token) {
+      const float* const at = reduce + token / kTokens * kMathWarps * kReduceWarp + tile_at * kReduceTile + (row >> 3) * 32 + (row & 7) * 4 +
+                              token % kTokens * (kSpan / 2);
+      float v[kSpan / 2];
+#pragma unroll
+      for (int pair = 0; pair < kSpan / 2; ++pair) {
+        float part[kMathWarps];
+#pragma unroll
+        for (int w = 0; w < kMathWarps; ++w) part[w] = at[w * kReduceWarp + pair];
+        v[pair] = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+      }
+      return kSpan == 2 ? v[0] : fmaf(v[kSpan / 2 - 1], 65536.0f, v[0]);
+    };
     math_barrier();
     if (kind == kUp) {
       // a warp takes a token, a lane a column of the inner activations: a block of 32
@@ -899,13 +894,15 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
         const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(a) & 0x7FFFFFFFu);
         const Factor factor = block_factor(top, kDigits);
         const uint32_t x = digits_of(a, factor, kDigits);
-        const long long row = static_cast<long long>(__shfl_sync(0xFFFFFFFFu, entry, warp)) * kDigits;
+        const int at = __shfl_sync(0xFFFFFFFFu, entry, warp);
+        int sums[3] = {0, 0, 0};
 #pragma unroll
         for (int digit = 0; digit < kDigits; ++digit) {
-          const int v = static_cast<int8_t>(x >> (8 * digit)), sum = __reduce_add_sync(0xFFFFFFFFu, v);
-          p.inner_digits[(row + digit) * p.inner + unit * 32 + lane] = static_cast<int8_t>(v);
-          if (lane == 0) p.inner_blocks[(row + digit) * blocks_of(p.inner) + unit] = {factor.down, kZeroSum - 8 * sum};
+          const int v = static_cast<int8_t>(x >> (8 * digit));
+          sums[digit] = __reduce_add_sync(0xFFFFFFFFu, v);
+          p.inner_digits[(static_cast<long long>(at) * kDigits + digit) * p.inner + unit * 32 + lane] = static_cast<int8_t>(v);
         }
+        if (lane == 0) store_blocks(p, p.inner_blocks, at, p.inner / 32, unit, factor.down, sums);
       }
     } else {
       const int r = threadIdx.x & (kUnitRows - 1), row = unit * kUnitRows + r;
@@ -1069,17 +1066,18 @@ qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_ro
   p.out_stride = out->stride;
   p.activation = activation;
   p.digits = x->type == QX_STORAGE_F32 ? 3 : 2;
+  p.nibbles = m->format == QX_FORMAT_Q4_0;
   p.error = ctx->error_dev;
 
   const long long pass = std::min<long long>(tokens, std::min(kPassTokens, kPassEntries / (p.top + p.shared)));
-  const size_t entries = static_cast<size_t>(pass) * (p.top + p.shared), rows = static_cast<size_t>(pass) * p.digits;
+  const size_t entries = static_cast<size_t>(pass) * (p.top + p.shared), pairs = columns_of(p.digits) / 2;
   Layout l;
-  const size_t at_x = l.take(rows * p.dim), at_x_blocks = l.take(rows * blocks_of(p.dim) * sizeof(Block));
+  const size_t at_x = l.take(pass * p.digits * p.dim), at_x_blocks = l.take(pass * pairs * (p.dim / 32) * sizeof(Block));
   const size_t at_logits = l.take(static_cast<size_t>(pass) * p.experts * sizeof(double));
   const size_t at_picks = l.take(entries * sizeof(int)), at_weights = l.take(entries * sizeof(float));
   const size_t at_progress = l.take(sizeof(Progress)), at_done = l.take(entries * sizeof(int));
   const size_t at_inner = l.take(entries * p.digits * p.inner);
-  const size_t at_inner_blocks = l.take(entries * p.digits * blocks_of(p.inner) * sizeof(Block));
+  const size_t at_inner_blocks = l.take(entries * pairs * (p.inner / 32) * sizeof(Block));
   const size_t at_products = l.take(entries * p.dim * sizeof(float));
   QX_TRY(workspace->reserve(l.total));
   uint8_t* const base = static_cast<uint8_t*>(workspace->base);

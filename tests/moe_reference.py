@@ -76,11 +76,11 @@ def apply(m, x, top, activation=SILU, sigmoid=False, biased=False, normalise=Tru
     """-> the layer's output, and the limit of |kernel - output|, both in 64 bits.
 
     Inputs and inner activations are digits under a power of two: off by 2^-15 (16-bit x) or 2^-23 of the largest of their
-    block of 32, or 2^-103. The sums of a block are exact. Then, in f32, the factor of a block and its product are two
-    roundings, the blocks are added one behind the other in four parts, two additions join those, and the digits are joined:
-    a matrix product of k columns is off by (k / 32 + 12) u of the sum of its terms' magnitudes at most. Those of the digits
-    are no more than |x| and 2^-6 of the block's largest. The activation's slope is below 1.13 (its argument is off, and a few
-    u of itself); relu^2 has a slope of 2 g."""
+    block of 32, or 2^-103. The sums of a block are exact. Then, in f32: two digits are joined, the block's factors are
+    multiplied, and their product added, four roundings, one behind the other in eight parts, which three additions join:
+    a matrix product of k columns is off by (k / 32 / 8 + 12) u of the sum of its terms' magnitudes at most. Those of the
+    digits are no more than |x| and 2^-6 of the block's largest. The activation's slope is below 1.13 (its argument is off, and
+    a few u of itself); relu^2 has a slope of 2 g."""
     chosen, weights, weights_off = route(m, x, top, sigmoid, biased, normalise, scale, chosen)
     kept = 2.0 ** -23 if x.dtype == torch.float32 else 2.0 ** -15
     x = x.double()
@@ -91,7 +91,7 @@ def apply(m, x, top, activation=SILU, sigmoid=False, biased=False, normalise=Tru
     def product(v, v_off, w):
         """v @ w.T where v is off by v_off, and how far it is off."""
         size = v.abs() + v_off + 2.0 ** -6 * largest(v.abs() + v_off)
-        return v @ w.T, (v_off + U * (v.shape[1] / 32 + 12) * size) @ w.abs().T
+        return v @ w.T, (v_off + U * (v.shape[1] / 256 + 12) * size) @ w.abs().T
 
     x_off = kept * largest(x) + 2.0 ** -103
     out, limit = torch.zeros_like(x), torch.zeros_like(x)
