@@ -20,14 +20,14 @@
 // warps multiply what two others bring into a ring of stages: one the weights, across units as far ahead as the ring reaches,
 // one the activations, which it waits for where a unit depends on others.
 //
-// Products. Whole-number MMAs (16 x 8 x 32) with the weights as the operand of 16 rows: codes as they are (q8_0), or
-// nibbles as unsigned bytes (q4_0), against the activations as balanced base-256 digits under a power of two per 32
-// columns: two digits for 16-bit inputs (2^-15 of a block's largest), three for f32 ones (2^-23). An MMA takes a block; its
-// exact sum starts at 1.5 * 2^23 as f32 bits, so that a subtraction (for nibbles, which stand for n - 8, of 8 times the
-// digits' sum more) makes an f32 number of it. A token's digits are neighbouring columns: a lane joins two of them and
-// multiplies with the block's d and the activations' scale. Four tokens (f32: two) cost no more than one. (As f16 pairs on f16
-// MMAs the conversion of the codes took three quarters of the instructions, and the layer twice the time.) The products of
-// gate and up get digits in the same way.
+// Products. Whole-number MMAs (16 x 8 x 32, s8) with the weights as the operand of 16 rows: codes as they are (q8_0), or
+// nibbles, laid out as the signed n - 8, as 16 times that in the upper halves of bytes (q4_0), against the activations as
+// balanced base-256 digits under a power of two per 32 columns: two digits for 16-bit inputs (2^-15 of a block's largest), three
+// for f32 ones (2^-23). An MMA takes a block and gives exact sums. A token's digits are neighbouring columns: a lane joins two
+// of them, and multiplies with the block's d and the activations' scale. Four tokens (f32: two) cost no more than one.
+// (As f16 pairs on f16 MMAs the conversion of the codes took three quarters of the instructions, and the layer twice the
+// time; sums that start at the bits of 1.5 * 2^23, to be f32 numbers after a subtraction, cost four moves an MMA.) The
+// products of gate and up get digits in the same way.
 //
 // A row's bits do not depend on the other tokens: columns are independent, and every sum has a fixed order.
 //
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(256) moe_relayout_kernel(const uint8_t* __rest
       for (int i = 0; i < 8; ++i) {  // elements 8 t + i and 8 t + 4 + i share byte i
         const int e = 8 * t + i;
         const uint32_t byte = from[2 + (e & 15)], nibble = e < 16 ? byte & 15 : byte >> 4;
-        word |= nibble << (8 * (i & 3) + 4 * (i >> 2));
+        word |= (nibble ^ 8) << (8 * (i & 3) + 4 * (i >> 2));
       }
       reinterpret_cast<uint32_t*>(out)[2 * lane + h] = word;
     } else {
@@ -120,8 +120,6 @@ struct Words {
   }
 };
 
-constexpr int kZeroSum = 0x4B400000;  // 1.5 * 2^23: whole numbers below 2^22 added to the bits are exact
-
 // The power of two that brings a block whose largest magnitude is `top` (as f32 bits) to what two or three balanced digits
 // hold (127 * 257, 127 * 65793), and its inverse; NaN for a block that holds a NaN or an infinity.
 struct Factor {
@@ -139,14 +137,6 @@ __device__ __forceinline__ uint32_t digits_of(float v, const Factor& f, int digi
   return (static_cast<uint32_t>(whole) + half) ^ half;
 }
 
-// What the products with a block of activations need: `sums` of its digits.
-__device__ __forceinline__ void store_blocks(const Params& p, Block* to, int row, int blocks, int block, float scale, const int (&sums)[3]) {
-  const int pairs = columns_of(p.digits) / 2, each = p.nibbles ? 8 : 0;
-  Block* const at = to + static_cast<long long>(row) * pairs * blocks + block;
-  at[0] = {{kZeroSum + each * sums[0], kZeroSum + each * sums[1]}, scale, 0};
-  if (pairs > 1) at[blocks] = {{kZeroSum + each * sums[2], kZeroSum}, scale, 0};
-}
-
 // A warp turns 128 columns of a token into digits.
 __device__ __forceinline__ void convert_columns(const Params& p, int token, int part) {
   const int lane = threadIdx.x & 31, d = part * 128 + lane * 4;
@@ -161,18 +151,12 @@ __device__ __forceinline__ void convert_columns(const Params& p, int token, int 
   uint32_t x[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = digits_of(v[e], factor, p.digits);
-  int sums[3] = {0, 0, 0};
-#pragma unroll
-  for (int digit = 0; digit < 3; ++digit) {
-    if (digit >= p.digits) continue;
+  for (int digit = 0; digit < p.digits; ++digit) {
     const uint32_t select = digit | (4 + digit) << 4;
     const uint32_t word = __byte_perm(__byte_perm(x[0], x[1], select), __byte_perm(x[2], x[3], select), 0x5410);
-    sums[digit] = __dp4a(static_cast<int>(word), 0x01010101, 0);
-#pragma unroll
-    for (int h = 1; h < 8; h <<= 1) sums[digit] += __shfl_xor_sync(0xFFFFFFFFu, sums[digit], h);
     if (d < p.dim) *reinterpret_cast<uint32_t*>(p.x_digits + (static_cast<long long>(token) * p.digits + digit) * p.dim + d) = word;
   }
-  if (d < p.dim && (lane & 7) == 0) store_blocks(p, p.x_blocks, token, p.dim / 32, d / 32, factor.down, sums);
+  if (d < p.dim && (lane & 7) == 0) p.x_scales[static_cast<long long>(token) * scales_of(p.dim) + d / 32] = factor.down;
 }
 
 // Order-preserving whole number of a double; NaN is above everything.
@@ -372,7 +356,7 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid
 constexpr int kMathWarps = 8, kExpertThreads = 32 * (kMathWarps + 2);
 constexpr int kWeightWarp = kMathWarps, kColumnWarp = kMathWarps + 1;
 constexpr int kUnitRows = kUnitTiles * kTileRows;
-constexpr int kCombineWidth = 1024;
+constexpr int kCombineWidth = 1024, kMostTokens = 8;
 constexpr int kReduceTile = 64 + 1, kReduceWarp = kUnitTiles * kReduceTile;  // floats: [row g, g + 8][lane]
 enum { kUp = 0, kDown = 1, kCombine = 2, kExit = 3 };
 
@@ -404,11 +388,11 @@ struct ExpertShape {
   static constexpr int kRecord = record_bytes(kFormat);
   static constexpr int kBlocks = kFormat == QX_FORMAT_Q4_0 ? 16 : 8;  // of a stage
   static constexpr int kStages = kFormat == QX_FORMAT_Q4_0 ? 3 : 4;
-  // Between columns, and pairs of them: lanes of an 8-byte load, four columns at a time, and of a 16-byte one meet no conflicts.
-  static constexpr int kColumnBytes = kBlocks * 32 + 32, kPairBytes = (kBlocks + 1) * static_cast<int>(sizeof(Block));
+  // Between columns, and tokens' scales: lanes of an 8-byte load, four columns at a time, and of a 4-byte one meet no conflicts.
+  static constexpr int kColumnBytes = kBlocks * 32 + 32, kScaleBytes = kBlocks * 4 + 16;
   static constexpr int kWeights = kBlocks * kUnitTiles * kRecord;
   static constexpr int kScales = kWeights + kColumns * kColumnBytes;
-  static constexpr int kStage = kScales + kColumns / 2 * kPairBytes;
+  static constexpr int kStage = kScales + kMostTokens * kScaleBytes;
   static constexpr int kReduce = kStages * kStage;
   static constexpr int kInfo = kReduce + (2 * kMathWarps * kReduceWarp * 4 + 15) / 16 * 16;
   static constexpr int kBars = kInfo + kStages * static_cast<int>(sizeof(UnitInfo));
@@ -494,29 +478,22 @@ __device__ __forceinline__ void sort_pairs(const Params& p, int most, SortSpace&
   __syncthreads();
 }
 
-// A block's sums: the operand's type is that of the codes.
-__device__ __forceinline__ void mma_block(uint32_t (&d)[4], const uint32_t (&a)[4], uint2 b, bool nibbles) {
-  if (nibbles) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%10, %10, %10, %10};"
-        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(kZeroSum));
-  } else {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%10, %10, %10, %10};"
-        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(kZeroSum));
-  }
+// A block's sums.
+__device__ __forceinline__ void mma_block(int (&d)[4], const uint32_t (&a)[4], uint2 b) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(0));
 }
-// The codes of a lane's columns 8 t .. 8 t + 7 of rows g and g + 8: operands of the block's MMA.
+// The codes (q4_0: 16 times) of a lane's columns 8 t .. 8 t + 7 of rows g and g + 8: operands of the block's MMA.
 template <int kFormat>
 __device__ __forceinline__ void load_codes(const uint8_t* record, int lane, uint32_t (&a)[4]) {
   if (kFormat == QX_FORMAT_Q4_0) {
     const uint2 w = *reinterpret_cast<const uint2*>(record + lane * 8);
-    a[0] = w.x & 0x0F0F0F0Fu;
-    a[1] = w.y & 0x0F0F0F0Fu;
-    a[2] = w.x >> 4 & 0x0F0F0F0Fu;
-    a[3] = w.y >> 4 & 0x0F0F0F0Fu;
+    a[0] = w.x << 4 & 0xF0F0F0F0u;
+    a[1] = w.y << 4 & 0xF0F0F0F0u;
+    a[2] = w.x & 0xF0F0F0F0u;
+    a[3] = w.y & 0xF0F0F0F0u;
   } else {
     const uint4 w = *reinterpret_cast<const uint4*>(record + lane * 16);
     a[0] = w.x;
@@ -528,10 +505,10 @@ __device__ __forceinline__ void load_codes(const uint8_t* record, int lane, uint
 
 // A warp's blocks of a stage, every eighth: 64 rows x 8 kN columns, sums in `total` [tile][column tile][row g, row g + 8] of
 // the lane's pair of digits; `join`: how many of the lower digit one of the higher is. The pointers are at the warp's first
-// block; `blocks` is what the stage has from there on. kWhole: all of four tiles.
-template <int kFormat, int kN, bool kWhole>
+// block (scales: of the lane's token); `blocks` is what the stage has from there on. kWhole: all of four tiles.
+template <int kFormat, int kN, int kTokens, bool kWhole>
 __device__ __forceinline__ void multiply(const uint8_t* records, int tiles_there, const uint8_t* columns, const uint8_t* scales, int blocks,
-                                         float join, float (&total)[kUnitTiles][2][2]) {
+                                         int join, float (&total)[kUnitTiles][2][2]) {
   using S = ExpertShape<kFormat>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int tiles = kWhole ? kUnitTiles : tiles_there;
@@ -539,11 +516,11 @@ __device__ __forceinline__ void multiply(const uint8_t* records, int tiles_there
   for (int b = 0; b < S::kBlocks / kMathWarps; ++b) {
     if (!kWhole && b * kMathWarps >= blocks) continue;
     uint2 x[kN];
-    uint4 block[kN];  // {zeros, scale} of the lane's pair
+    float scale[kN];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       x[n] = *reinterpret_cast<const uint2*>(columns + (8 * n + g) * S::kColumnBytes + b * kMathWarps * 32 + t * 8);
-      block[n] = *reinterpret_cast<const uint4*>(scales + (4 * n + t) * S::kPairBytes + b * kMathWarps * sizeof(Block));
+      scale[n] = *reinterpret_cast<const float*>(scales + n * kTokens * S::kScaleBytes + b * kMathWarps * 4);
     }
 #pragma unroll
     for (int i = 0; i < kUnitTiles; ++i) {
@@ -554,17 +531,11 @@ __device__ __forceinline__ void multiply(const uint8_t* records, int tiles_there
       const float2 d = __half22float2(reinterpret_cast<const __half2*>(record + S::kRecord - 32)[g]);
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        uint32_t sum[4];
-        mma_block(sum, a, x[n], kFormat == QX_FORMAT_Q4_0);
-        const unsigned long long zero = tile::pack2(block[n].x, block[n].y);
-        const float scale = __uint_as_float(block[n].z);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          uint32_t low, high;
-          tile::unpack2(tile::subf2(tile::pack2(sum[2 * r], sum[2 * r + 1]), zero), low, high);
-          const float both = fmaf(__uint_as_float(high), join, __uint_as_float(low));
-          total[i][n][r] = fmaf(both, scale * (r == 0 ? d.x : d.y), total[i][n][r]);
-        }
+        int sum[4];
+        mma_block(sum, a, x[n]);
+        // (below 2^28)
+        total[i][n][0] = fmaf(static_cast<float>(sum[1] * join + sum[0]), scale[n] * d.x, total[i][n][0]);
+        total[i][n][1] = fmaf(static_cast<float>(sum[3] * join + sum[2]), scale[n] * d.y, total[i][n][1]);
       }
     }
   }
@@ -585,6 +556,19 @@ __device__ __forceinline__ int load_acquire(const int* p) {
   int v;
   asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
+}
+// The copying warps' bounded wait: they run ahead, and polls would take issue slots from the products.
+__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  bool done = mbar_try_wait(bar, parity);
+  if (!done) {
+    const unsigned long long start = global_timer_ns();
+    for (uint32_t spin = 1; !done; ++spin) {
+      __nanosleep(32);
+      done = mbar_try_wait(bar, parity);
+      if ((spin & 63u) == 0u && (*abort_flag != 0 || global_timer_ns() - start > kWaitLimitNs)) break;
+    }
+  }
+  return __all_sync(0xFFFFFFFFu, done);
 }
 // Until *counter >= target; false where the time runs out or the CTA gives up.
 __device__ __forceinline__ bool wait_for_count(const int* counter, int target, volatile int* abort_flag) {
@@ -663,7 +647,7 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
         unit.unit = ticket - ups - downs - unit.group * combine_chunks;
       }
       for (int stage = 0; stage < stages; ++stage) {
-        ok = issued < kStages || mbar_wait_warp(empty + ring.slot, ring.phase ^ 1u, abort_flag);
+        ok = issued < kStages || wait_asleep(empty + ring.slot, ring.phase ^ 1u, abort_flag);
         if (!ok) break;
         issued = min(issued + 1, kStages);
         if (stage == 0) {
@@ -713,36 +697,31 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
     tile::Ring ring;
     bool ok = true;
     for (;;) {
-      ok = mbar_wait_warp(begun + ring.slot, ring.phase, abort_flag);
+      ok = wait_asleep(begun + ring.slot, ring.phase, abort_flag);
       if (!ok) break;
       const UnitInfo& info = infos[ring.slot];
       const int kind = info.kind, blocks = info.blocks, count = info.count, group = info.group;
       const int width = kind == kUp ? p.dim : p.inner;
       const int8_t* const digits = kind == kUp ? p.x_digits : p.inner_digits;
-      const Block* const blocks_at = kind == kUp ? p.x_blocks : p.inner_blocks;
-      // Lane c < 16 looks after column c, a digit of a token, lane p < 8 after pair p of them: their rows.
-      int row = -1, pair_row = -1;
-      const int place = lane / kSpan, pair_place = 2 * lane / kSpan;
-      if (place < count && lane % kSpan < kDigits) {
-        row = (kind == kUp ? info.entries[place] / (p.top + p.shared) : info.entries[place]) * kDigits + lane % kSpan;
+      const float* const scales = kind == kUp ? p.x_scales : p.inner_scales;
+      // Lane c < 16 looks after column c, a digit of a token: its row.
+      const int place = lane / kSpan;
+      int token = -1, row = -1;
+      if (lane < kColumns && place < count) {
+        token = kind == kUp ? info.entries[place] / (p.top + p.shared) : info.entries[place];
+        if (lane % kSpan < kDigits) row = token * kDigits + lane % kSpan;
       }
-      if (pair_place < count) {
-        pair_row = (kind == kUp ? info.entries[pair_place] / (p.top + p.shared) : info.entries[pair_place]) * (kSpan / 2) + lane % (kSpan / 2);
-      }
-      // 16 bytes a lane: a column takes 2 * kBlocks lanes, a pair's blocks kBlocks.
-      constexpr int kLanes = 2 * S::kBlocks, kPairLanes = S::kBlocks;
-      constexpr int kTurns = kColumns * kLanes / 32, kPairTurns = kColumns / 2 * kPairLanes / 32;
-      int from[kTurns], pairs_from[kPairTurns];
+      // 16 bytes a lane: a column takes 2 * kBlocks lanes, a token's scales kBlocks / 4.
+      constexpr int kLanes = 2 * S::kBlocks, kScaleLanes = S::kBlocks / 4, kTurns = kColumns * kLanes / 32;
+      int from[kTurns];
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
         const int r = __shfl_sync(0xFFFFFFFFu, row, i * (32 / kLanes) + lane / kLanes);
         from[i] = r < 0 ? -1 : r * width + lane % kLanes * 16;
       }
-#pragma unroll
-      for (int i = 0; i < kPairTurns; ++i) {
-        const int r = __shfl_sync(0xFFFFFFFFu, pair_row, i * (32 / kPairLanes) + lane / kPairLanes);
-        pairs_from[i] = r < 0 ? -1 : r * (width / 32) + lane % kPairLanes;
-      }
+      static_assert(kMostTokens * kScaleLanes <= 32, "the scales of all tokens are one turn");
+      const int scale_token = __shfl_sync(0xFFFFFFFFu, token, lane / kScaleLanes * kSpan);
+      const int scales_from = scale_token < 0 || lane / kScaleLanes >= count ? -1 : scale_token * scales_of(width) + lane % kScaleLanes * 4;
       if (kind == kDown) ok = wait_for_count(p.up_done + group, up_units, abort_flag);
       if (kind == kCombine) ok = wait_for_count(&p.progress->down_done, downs, abort_flag);
       ok = __all_sync(0xFFFFFFFFu, ok);
@@ -750,25 +729,21 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
       for (int first = 0;;) {
         const int in_stage = min(S::kBlocks, blocks - first);
         const uint32_t to = smem_u32(smem + ring.slot * S::kStage);
-        const bool value = lane % kLanes < in_stage * 2, block = lane % kPairLanes < in_stage;
+        const bool value = lane % kLanes < in_stage * 2;
 #pragma unroll
         for (int i = 0; i < kTurns; ++i) {
           if (value && from[i] >= 0) {
             copy16(to + S::kWeights + (i * (32 / kLanes) + lane / kLanes) * S::kColumnBytes + lane % kLanes * 16, digits + from[i] + first * 32);
           }
         }
-#pragma unroll
-        for (int i = 0; i < kPairTurns; ++i) {
-          if (block && pairs_from[i] >= 0) {
-            copy16(to + S::kScales + (i * (32 / kPairLanes) + lane / kPairLanes) * S::kPairBytes + lane % kPairLanes * static_cast<int>(sizeof(Block)),
-                   blocks_at + pairs_from[i] + first);
-          }
+        if (scales_from >= 0 && lane % kScaleLanes * 4 < in_stage) {
+          copy16(to + S::kScales + lane / kScaleLanes * S::kScaleBytes + lane % kScaleLanes * 16, scales + scales_from + first);
         }
         arrive_behind_copies(full + ring.slot);
         ring.advance(kStages);
         first += S::kBlocks;
         if (first >= blocks) break;
-        ok = mbar_wait_warp(begun + ring.slot, ring.phase, abort_flag);
+        ok = wait_asleep(begun + ring.slot, ring.phase, abort_flag);
         if (!ok) break;
       }
       if (!ok || kind == kExit) break;
@@ -783,7 +758,7 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
 
   // ---- products ------------------------------------------------------------------------------
   const int places = p.top + p.shared;
-  const float join = kSpan == 4 && (lane & 1) ? 0.0f : 256.0f;  // (a third digit stands alone)
+  const int join = kSpan == 4 && (lane & 1) ? 0 : 256;  // (a third digit stands alone)
   tile::Ring ring;
   float total[kUnitTiles][2][2] = {};
   const auto wait_for_stage = [&]() {
@@ -843,9 +818,9 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
         const uint8_t* const stage = smem + ring.slot * S::kStage;
         const uint8_t* const records = stage + warp * tiles * S::kRecord;
         const uint8_t* const columns = stage + S::kWeights + warp * 32;
-        const uint8_t* const scales = stage + S::kScales + warp * sizeof(Block);
-        if (left >= S::kBlocks && tiles == kUnitTiles) multiply<kFormat, kN, true>(records, tiles, columns, scales, S::kBlocks, join, total);
-        else multiply<kFormat, kN, false>(records, tiles, columns, scales, min(left, S::kBlocks) - warp, join, total);
+        const uint8_t* const scales = stage + S::kScales + (lane & 3) * 2 / kSpan * S::kScaleBytes + warp * 4;
+        if (left >= S::kBlocks && tiles == kUnitTiles) multiply<kFormat, kN, kTokens, true>(records, tiles, columns, scales, S::kBlocks, join, total);
+        else multiply<kFormat, kN, kTokens, false>(records, tiles, columns, scales, min(left, S::kBlocks) - warp, join, total);
         free_stage();
         left -= S::kBlocks;
         if (left <= 0) return;
@@ -882,7 +857,8 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
         for (int w = 0; w < kMathWarps; ++w) part[w] = at[w * kReduceWarp + pair];
         v[pair] = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
       }
-      return kSpan == 2 ? v[0] : fmaf(v[kSpan / 2 - 1], 65536.0f, v[0]);
+      const float sum = kSpan == 2 ? v[0] : fmaf(v[kSpan / 2 - 1], 65536.0f, v[0]);
+      return kFormat == QX_FORMAT_Q4_0 ? sum * 0.0625f : sum;
     };
     math_barrier();
     if (kind == kUp) {
@@ -895,14 +871,11 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
         const Factor factor = block_factor(top, kDigits);
         const uint32_t x = digits_of(a, factor, kDigits);
         const int at = __shfl_sync(0xFFFFFFFFu, entry, warp);
-        int sums[3] = {0, 0, 0};
 #pragma unroll
         for (int digit = 0; digit < kDigits; ++digit) {
-          const int v = static_cast<int8_t>(x >> (8 * digit));
-          sums[digit] = __reduce_add_sync(0xFFFFFFFFu, v);
-          p.inner_digits[(static_cast<long long>(at) * kDigits + digit) * p.inner + unit * 32 + lane] = static_cast<int8_t>(v);
+          p.inner_digits[(static_cast<long long>(at) * kDigits + digit) * p.inner + unit * 32 + lane] = static_cast<int8_t>(x >> (8 * digit));
         }
-        if (lane == 0) store_blocks(p, p.inner_blocks, at, p.inner / 32, unit, factor.down, sums);
+        if (lane == 0) p.inner_scales[static_cast<long long>(at) * scales_of(p.inner) + unit] = factor.down;
       }
     } else {
       const int r = threadIdx.x & (kUnitRows - 1), row = unit * kUnitRows + r;
@@ -1066,31 +1039,30 @@ qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_ro
   p.out_stride = out->stride;
   p.activation = activation;
   p.digits = x->type == QX_STORAGE_F32 ? 3 : 2;
-  p.nibbles = m->format == QX_FORMAT_Q4_0;
   p.error = ctx->error_dev;
 
   const long long pass = std::min<long long>(tokens, std::min(kPassTokens, kPassEntries / (p.top + p.shared)));
-  const size_t entries = static_cast<size_t>(pass) * (p.top + p.shared), pairs = columns_of(p.digits) / 2;
+  const size_t entries = static_cast<size_t>(pass) * (p.top + p.shared);
   Layout l;
-  const size_t at_x = l.take(pass * p.digits * p.dim), at_x_blocks = l.take(pass * pairs * (p.dim / 32) * sizeof(Block));
+  const size_t at_x = l.take(pass * p.digits * p.dim), at_x_scales = l.take(pass * scales_of(p.dim) * sizeof(float));
   const size_t at_logits = l.take(static_cast<size_t>(pass) * p.experts * sizeof(double));
   const size_t at_picks = l.take(entries * sizeof(int)), at_weights = l.take(entries * sizeof(float));
   const size_t at_progress = l.take(sizeof(Progress)), at_done = l.take(entries * sizeof(int));
   const size_t at_inner = l.take(entries * p.digits * p.inner);
-  const size_t at_inner_blocks = l.take(entries * pairs * (p.inner / 32) * sizeof(Block));
+  const size_t at_inner_scales = l.take(entries * scales_of(p.inner) * sizeof(float));
   const size_t at_products = l.take(entries * p.dim * sizeof(float));
   QX_TRY(workspace->reserve(l.total));
   uint8_t* const base = static_cast<uint8_t*>(workspace->base);
   p.arrivals = reinterpret_cast<int*>(base);
   p.x_digits = reinterpret_cast<int8_t*>(base + at_x);
-  p.x_blocks = reinterpret_cast<Block*>(base + at_x_blocks);
+  p.x_scales = reinterpret_cast<float*>(base + at_x_scales);
   p.logits = reinterpret_cast<double*>(base + at_logits);
   p.picks = reinterpret_cast<int*>(base + at_picks);
   p.weights = reinterpret_cast<float*>(base + at_weights);
   p.progress = reinterpret_cast<Progress*>(base + at_progress);
   p.up_done = reinterpret_cast<int*>(base + at_done);
   p.inner_digits = reinterpret_cast<int8_t*>(base + at_inner);
-  p.inner_blocks = reinterpret_cast<Block*>(base + at_inner_blocks);
+  p.inner_scales = reinterpret_cast<float*>(base + at_inner_scales);
   p.products = reinterpret_cast<float*>(base + at_products);
 
   for (long long t0 = 0; t0 < tokens; t0 += pass) {

@@ -26,13 +26,9 @@ constexpr int kPassTokens = 128, kPassEntries = 1024;
 constexpr int kTileRows = 16, kUnitTiles = 4;
 constexpr int record_bytes(int format) { return (format == QX_FORMAT_Q4_0 ? 256 : 512) + 32; }
 
-// Activations lie as rows of 8-bit digits, a row per token and digit (the lowest first), and beside them a row per token and
-// pair of digits of what their products with a block of 32 columns need.
-struct Block {
-  int zero[2];  // what a sum of products counts from, of either digit, as f32 bits
-  float scale;  // of the block, whatever the digit
-  int unused;
-};
+// Activations lie as rows of 8-bit digits, a row per token and digit (the lowest first), and beside them, a row per token,
+// an f32 scale per 32 of them. Rows of scales are whole 16-byte pieces.
+inline __host__ __device__ int scales_of(int columns) { return (columns / 32 + 3) / 4 * 4; }
 // Columns of an MMA that a token takes: two digits, or three and one to spare.
 constexpr int columns_of(int digits) { return digits == 2 ? 2 : 4; }
 
@@ -62,20 +58,20 @@ struct Params {
   uint8_t* out;
   int out_type, out_vector;
   long long out_stride;
-  int tokens, activation, digits, nibbles;
+  int tokens, activation, digits;
   int32_t* chosen;       // [token][top], may be NULL
   float* chosen_weights;
   // scratch
   int* arrivals;         // one per eight tokens, zero between calls
   int8_t* x_digits;      // [token][digit][dim]
-  Block* x_blocks;       // [token][pair of digits][dim / 32]
+  float* x_scales;
   double* logits;        // [token][expert]
   int* picks;            // [token][top + shared] experts
   float* weights;        // [token][top + shared]
   Progress* progress;
   int* up_done;          // [group] units
   int8_t* inner_digits;  // [entry][digit][inner], entry = token * (top + shared) + place
-  Block* inner_blocks;   // [entry][pair of digits][inner / 32]
+  float* inner_scales;
   float* products;       // [entry][dim]
   int* error;
 };
