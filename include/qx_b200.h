@@ -787,8 +787,8 @@ typedef struct qx_moe_router {
  * `chosen` and `weights` (either may be NULL) receive the experts and their w, [tokens][top], largest first. `activation`
  * is QX_ACTIVATION_*. Any number of tokens is served, in passes of up to 128; the kernels are made for few, whose experts' weights
  * are read once per eight tokens of theirs (f32: four).
- * Precision. Logits are summed up in 64 bits from sums of eight f32 products, scores and weights of the router are taken in
- * 64 bits. Codes are used as they are; x and the products of gate and up are rounded to 2^-15 of the largest of their 32
+ * Precision. Logits are summed up in 64 bits from f32 sums of 32 exact products, scores and weights are f32 (64 bits with a
+ * bias). Codes are used as they are; x and the products of gate and up are rounded to 2^-15 of the largest of their 32
  * neighbours (a block's columns) for 16-bit x, to 2^-23 of it for f32 x, and to 2^-103 where that is more. Sums of a block are exact, sums of
  * blocks f32, out is rounded once. A token's bits do not depend on the other tokens. A token that holds a NaN or an
  * infinity, or whose product of gate and up overflows, spoils its own output only.

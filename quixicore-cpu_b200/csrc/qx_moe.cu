@@ -6,10 +6,12 @@
 // What bounds it is the reading of the touched experts' blocks, once: 18 or 34 bytes per 32 weights. Everything else is
 // arranged around keeping those loads under way from the first to the last.
 //
-// Router (moe_router_kernel). Logits are sums of at most eight f32 products at a time, added up in 64 bits: two experts
-// on both sides of the choice are told apart as far as the inputs' own products are. A CTA takes two experts and eight tokens, a
-// warp an eighth of the columns; the last CTA to finish eight tokens chooses their experts, a warp per token. Beside them,
-// other CTAs turn the activations into digits.
+// Router (moe_router_kernel). Both operands are cut into bf16 terms that add up to them (one for bf16, two for f16, three for
+// f32), so that every product on bf16 MMAs is exact; sums over 32 columns are the MMA's, those over the rest 64-bit: two experts
+// on both sides of the choice are told apart as far as the inputs' own products are. A CTA takes 16 experts and eight tokens, its
+// 16 warps 32 columns each in turn; the CTAs of eight tokens are a cluster, whose first gets all their logits in shared
+// memory and chooses the experts, a warp per token. Beside them, other CTAs turn the activations into digits. What it costs
+// is latency, a good part of it that of instructions which are fetched once, so loops stay loops here.
 //
 // Experts (moe_experts_kernel). Every CTA sorts the (token, expert) pairs by expert, in shared memory: a microsecond, which a
 // kernel of its own or the router's last CTA would add to the launch as well. Work is cut into units that CTAs draw as tickets, in this order:
@@ -95,7 +97,7 @@ __global__ void __launch_bounds__(256) moe_relayout_kernel(const uint8_t* __rest
 }
 
 // ---- router ------------------------------------------------------------------------------------
-constexpr int kRouterTokens = 8, kRouterExperts = 2, kRouterSplits = 8, kRouterThreads = 256;
+constexpr int kRouterTokens = 8, kRouterExperts = 16, kRouterWarps = 16, kRouterThreads = 32 * kRouterWarps, kRouterCluster = 8;
 
 // Eight neighbouring elements as they lie in memory; off 16-byte boundaries as f32.
 struct Words {
@@ -159,92 +161,86 @@ __device__ __forceinline__ void convert_columns(const Params& p, int token, int 
   if (d < p.dim && (lane & 7) == 0) p.x_scales[static_cast<long long>(token) * scales_of(p.dim) + d / 32] = factor.down;
 }
 
-// Order-preserving whole number of a double; NaN is above everything.
+// Order-preserving whole number of a double, and back; NaN is above everything.
 __device__ __forceinline__ unsigned long long ordered(double v) {
   const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(v));
   if (v != v) return ~0ull;
   return bits >> 63 ? ~bits : bits | 1ull << 63;
 }
-
-// A warp chooses a token's experts. kEach: experts per lane, expert = lane + 32 i.
-template <int kEach>
-__device__ __forceinline__ void choose(const Params& p, int token) {
-  const int lane = threadIdx.x & 31, places = p.top + p.shared;
-  const double* const logits = p.logits + static_cast<long long>(token) * p.experts;
-  double logit[kEach], largest = -INFINITY;
+__device__ __forceinline__ double from_ordered(unsigned long long key) {
+  return __longlong_as_double(static_cast<long long>(key >> 63 ? key & ~(1ull << 63) : ~key));
+}
+template <class T>
+__device__ __forceinline__ T warp_sum(T v) {
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int e = lane + 32 * i;
-    logit[i] = e < p.experts ? __ldcg(logits + e) : -INFINITY;
-    largest = fmax(largest, logit[i]);
-  }
-  double score[kEach], total = 0.0;
-  if (p.score == QX_MOE_SOFTMAX) {
+  for (int h = 16; h > 0; h >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, h);
+  return v;
+}
+
+// A warp chooses a token's experts by their keys: logits, or scores and biases.
+__device__ __forceinline__ void choose(const Params& p, unsigned long long* keys, int token) {
+  const int lane = threadIdx.x & 31, places = p.top + p.shared, each = (p.experts + 31) / 32;
+  if (p.bias != nullptr && p.score == QX_MOE_SOFTMAX) {  // (scores need all logits)
+    double largest = -INFINITY, total = 0.0;
+    for (int e = lane; e < p.experts; e += 32) largest = fmax(largest, from_ordered(keys[e]));
 #pragma unroll
     for (int h = 16; h > 0; h >>= 1) largest = fmax(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, h));
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      score[i] = 0.0;
-      // (weights are f32; a choice by score + bias takes all bits there are)
-      const double below = logit[i] - largest;
-      if (lane + 32 * i < p.experts) score[i] = p.bias == nullptr ? static_cast<double>(expf(static_cast<float>(below))) : exp(below);
-      total += score[i];
+    for (int pass = 0; pass < 2; ++pass) {
+      for (int e = lane; e < p.experts; e += 32) {
+        const double score = exp(from_ordered(keys[e]) - largest);
+        if (pass == 0) total += score;
+        else keys[e] = ordered(score / total + static_cast<double>(p.bias[e]));
+      }
+      if (pass == 0) total = warp_sum(total);
     }
-#pragma unroll
-    for (int h = 16; h > 0; h >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, h);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      score[i] = p.bias == nullptr ? static_cast<double>(1.0f / (1.0f + expf(static_cast<float>(-logit[i])))) : 1.0 / (1.0 + exp(-logit[i]));
-    }
-    total = 1.0;
+    __syncwarp();
   }
-  unsigned long long key[kEach];
   uint32_t left = 0;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int e = lane + 32 * i;
-    key[i] = 0;
-    if (e < p.experts) {
-      left |= 1u << i;
-      key[i] = ordered(p.bias == nullptr ? logit[i] : score[i] / total + static_cast<double>(p.bias[e]));
-    }
-  }
-  double mine = 0.0, sum = 0.0;  // of the place that is this lane's
+  for (int i = 0; i < each; ++i) left |= lane + 32 * i < p.experts ? 1u << i : 0u;
+  unsigned long long mine = 0;  // of the place that is this lane's
   int expert = 0;
   for (int place = 0; place < p.top; ++place) {
     // the largest key left, of the lowest expert where it is there twice
     unsigned long long best = 0;
     int at = -1;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      if ((left >> i & 1) && (at < 0 || key[i] > best)) {
-        best = key[i];
+    for (int i = 0; i < each; ++i) {
+      if (!(left >> i & 1)) continue;
+      const unsigned long long key = keys[lane + 32 * i];
+      if (at < 0 || key > best) {
+        best = key;
         at = i;
       }
     }
     const uint32_t high = __reduce_max_sync(0xFFFFFFFFu, at < 0 ? 0 : static_cast<uint32_t>(best >> 32));
     const bool still = at >= 0 && static_cast<uint32_t>(best >> 32) == high;
     const uint32_t low = __reduce_max_sync(0xFFFFFFFFu, still ? static_cast<uint32_t>(best) : 0);
-    const bool mine_is = still && static_cast<uint32_t>(best) == low;
-    const uint32_t chosen = __reduce_min_sync(0xFFFFFFFFu, mine_is ? static_cast<uint32_t>(lane + 32 * at) : 0x7FFFFFFFu);
-    double s = 0.0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      if (chosen == static_cast<uint32_t>(lane + 32 * i)) {
-        s = score[i];
-        left &= ~(1u << i);
-      }
-    }
-    s = __shfl_sync(0xFFFFFFFFu, s, chosen & 31);
-    sum += s;
+    const bool is = still && static_cast<uint32_t>(best) == low;
+    const uint32_t chosen = __reduce_min_sync(0xFFFFFFFFu, is ? static_cast<uint32_t>(lane + 32 * at) : 0x7FFFFFFFu);
+    if (static_cast<uint32_t>(lane) == (chosen & 31)) left &= ~(1u << (chosen >> 5));
     if (lane == place) {
-      mine = s;
+      mine = static_cast<unsigned long long>(high) << 32 | low;
       expert = static_cast<int>(chosen);
     }
   }
-  if (lane < p.top) {
-    const float weight = static_cast<float>(mine / (p.normalise ? sum : total) * static_cast<double>(p.scale));
+  // Scores: differences of logits from the largest are exact enough in 32 bits.
+  const bool takes = lane < p.top;
+  const double key = from_ordered(mine), largest = __shfl_sync(0xFFFFFFFFu, key, 0);
+  float score = 0.0f, total = 1.0f;
+  if (p.bias != nullptr) {
+    if (takes) score = static_cast<float>(key - static_cast<double>(p.bias[expert]));
+  } else if (p.score == QX_MOE_SIGMOID) {
+    if (takes) score = 1.0f / (1.0f + expf(static_cast<float>(-key)));
+  } else {
+    if (takes) score = expf(static_cast<float>(key - largest));
+    if (!p.normalise) {
+      total = 0.0f;
+      for (int e = lane; e < p.experts; e += 32) total += expf(static_cast<float>(from_ordered(keys[e]) - largest));
+      total = warp_sum(total);
+    }
+  }
+  if (p.normalise) total = warp_sum(score);
+  if (takes) {
+    const float weight = score / total * p.scale;
     p.picks[token * places + lane] = expert;
     p.weights[token * places + lane] = weight;
     if (p.chosen != nullptr) p.chosen[static_cast<long long>(token) * p.top + lane] = expert;
@@ -256,33 +252,98 @@ __device__ __forceinline__ void choose(const Params& p, int token) {
   }
 }
 
-// The last thread block to arrive at a counter of `all`, which is then zero again.
-__device__ __forceinline__ bool arrives_last(int* counter, int all, int* shared) {
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const bool last = atomicAdd(counter, 1) == all - 1;
-    if (last) *counter = 0;
-    *shared = last;
+// Eight elements as bf16 terms, pairs of them as MMA operands.
+template <int kType>
+struct Terms {
+  static constexpr int kCount = kType == QX_STORAGE_BF16 ? 1 : kType == QX_STORAGE_F16 ? 2 : 3;
+  uint32_t w[kCount][4];
+  __device__ __forceinline__ Terms(const Words& words, int vector) {
+    if (kType == QX_STORAGE_BF16 && vector) {
+      w[0][0] = words.w[0].x;
+      w[0][1] = words.w[0].y;
+      w[0][2] = words.w[0].z;
+      w[0][3] = words.w[0].w;
+      return;
+    }
+    float v[8];
+    words.values(kType, vector, v);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // (cut off, not rounded: what is left is exact and has eight bits less)
+        const uint32_t a = __float_as_uint(v[2 * j]), b = __float_as_uint(v[2 * j + 1]);
+        w[i][j] = __byte_perm(a, b, 0x7632);
+        v[2 * j] -= __uint_as_float(a & 0xFFFF0000u);
+        v[2 * j + 1] -= __uint_as_float(b & 0xFFFF0000u);
+      }
+    }
   }
-  __syncthreads();
-  if (*shared == 0) return false;
-  __threadfence();
-  return true;
+};
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// A warp's part of the logits of 16 experts and eight tokens: lane (g, t) has experts g, g + 8 and tokens 2 t, 2 t + 1. Lane
+// (g, t) reads columns 8 t .. 8 t + 7 of a run of 32: any order of columns does that is both operands'.
+template <int kX, int kW>
+__device__ __forceinline__ void sum_logits(const Params& p, int token0, int expert0, double (&sum)[4]) {
+  constexpr int kBatch = kX == QX_STORAGE_F32 || kW == QX_STORAGE_F32 ? 2 : 4;  // runs under way
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long long x_row = min(token0 + g, p.tokens - 1) * p.x_stride;
+  const long long rows[2] = {static_cast<long long>(min(expert0 + g, p.experts - 1)) * p.dim,
+                             static_cast<long long>(min(expert0 + g + 8, p.experts - 1)) * p.dim};
+  for (int k0 = static_cast<int>(threadIdx.x) / 32 * 32 + t * 8; k0 < p.dim; k0 += kBatch * kRouterWarps * 32) {
+    Words x[kBatch], w[kBatch][2];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int k = k0 + i * kRouterWarps * 32;
+      if (k >= p.dim) continue;
+      x[i].load(p.x, kX, p.x_vector, x_row + k);
+      w[i][0].load(p.router, kW, p.router_vector, rows[0] + k);
+      w[i][1].load(p.router, kW, p.router_vector, rows[1] + k);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (k0 + i * kRouterWarps * 32 >= p.dim) continue;
+      const Terms<kX> b(x[i], p.x_vector);
+      const Terms<kW> a0(w[i][0], p.router_vector), a1(w[i][1], p.router_vector);
+      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      // (the smallest products first)
+#pragma unroll
+      for (int u = Terms<kW>::kCount - 1; u >= 0; --u) {
+#pragma unroll
+        for (int v = Terms<kX>::kCount - 1; v >= 0; --v) {
+          mma_bf16(part, a0.w[u][0], a1.w[u][0], a0.w[u][1], a1.w[u][1], b.w[v][0], b.w[v][1]);
+          mma_bf16(part, a0.w[u][2], a1.w[u][2], a0.w[u][3], a1.w[u][3], b.w[v][2], b.w[v][3]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += static_cast<double>(part[e]);
+    }
+  }
+}
+// Shared memory: a cluster's first CTA holds the keys of eight tokens, behind the parts of sums.
+constexpr int kPartBytes = kRouterWarps * kRouterExperts * kRouterTokens * 8;
 
-// Grid: [token groups][expert groups] CTAs of the router, then those that convert activations.
-__global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid_constant__ Params p) {
-  __shared__ double parts[kRouterSplits][kRouterExperts][kRouterTokens];
-  __shared__ int last;
+// Grid: a cluster for every eight tokens, then those that convert activations. kX, kW: types of activations and router.
+template <int kX, int kW>
+__global__ void __launch_bounds__(kRouterThreads, 1) moe_router_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  auto& parts = *reinterpret_cast<double(*)[kRouterWarps][kRouterExperts][kRouterTokens]>(smem);
+  unsigned long long* const keys = reinterpret_cast<unsigned long long*>(smem + kPartBytes);  // [token][expert]
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  uint32_t rank, size;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
   const int token_groups = (p.tokens + kRouterTokens - 1) / kRouterTokens;
   const int expert_groups = (p.experts + kRouterExperts - 1) / kRouterExperts;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int index = static_cast<int>(blockIdx.x) - token_groups * expert_groups;
-  if (index >= 0) {
-    const int each = (p.dim + 127) / 128, item = index * 8 + warp;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, token_group = static_cast<int>(blockIdx.x / size);
+  if (token_group >= token_groups) {
+    const int each = (p.dim + 127) / 128, item = (static_cast<int>(blockIdx.x) - token_groups * static_cast<int>(size)) * kRouterWarps + warp;
     if (item < p.tokens * each) convert_columns(p, item / each, item % each);
     return;
   }
@@ -291,65 +352,30 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid
     for (int i = threadIdx.x; i < most; i += kRouterThreads) p.up_done[i] = 0;
     if (threadIdx.x == 0) *p.progress = {0, 0};
   }
-  const int token_group = blockIdx.x / expert_groups, expert_group = blockIdx.x % expert_groups;
-  const int token0 = token_group * kRouterTokens, expert0 = expert_group * kRouterExperts;
-  double sum[16];  // [expert of two][token]
+  const int token0 = token_group * kRouterTokens;
+  for (int expert_group = static_cast<int>(rank); expert_group < expert_groups; expert_group += static_cast<int>(size)) {
+    const int expert0 = expert_group * kRouterExperts;
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    sum_logits<kX, kW>(p, token0, expert0, sum);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sum[i] = 0.0;
-  for (int d = static_cast<int>(threadIdx.x) * 8; d < p.dim; d += kRouterSplits * 256) {
-    Words w[2], x[kRouterTokens];  // (all under way before the first is used)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      w[e].load(p.router, p.router_type, p.router_vector, static_cast<long long>(min(expert0 + e, p.experts - 1)) * p.dim + d);
-    }
-#pragma unroll
-    for (int t = 0; t < kRouterTokens; ++t) {
-      if (token0 + t < p.tokens) x[t].load(p.x, p.x_type, p.x_vector, (token0 + t) * p.x_stride + d);
-    }
-    float a[2][8];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) w[e].values(p.router_type, p.router_vector, a[e]);
-#pragma unroll
-    for (int t = 0; t < kRouterTokens; ++t) {
-      if (token0 + t >= p.tokens) continue;
-      float v[8];
-      x[t].values(p.x_type, p.x_vector, v);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float part = a[e][0] * v[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) part = fmaf(a[e][i], v[i], part);
-        sum[8 * e + t] += static_cast<double>(part);
-      }
-    }
-  }
-  // sixteen sums over 32 lanes: every step halves what a lane holds; lanes 2 i and 2 i + 1 end up with sum i
-#pragma unroll
-  for (int h = 16, n = 8; h > 1; h >>= 1, n >>= 1) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i >= n) continue;
-      const bool upper = lane & h;
-      const double send = upper ? sum[i] : sum[i + n], keep = upper ? sum[i + n] : sum[i];
-      sum[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, h);
-    }
-  }
-  sum[0] += __shfl_xor_sync(0xFFFFFFFFu, sum[0], 1);
-  if ((lane & 1) == 0) parts[warp][lane >> 4][lane >> 1 & 7] = sum[0];
-  __syncthreads();
-  if (threadIdx.x < kRouterExperts * kRouterTokens) {
+    for (int e = 0; e < 4; ++e) parts[warp][(lane >> 2) + 8 * (e >> 1)][2 * (lane & 3) + (e & 1)] = sum[e];
+    __syncthreads();
     const int e = threadIdx.x / kRouterTokens, t = threadIdx.x % kRouterTokens;
-    double v = parts[0][e][t];
+    if (threadIdx.x < kRouterExperts * kRouterTokens && expert0 + e < p.experts) {
+      double v[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-    for (int i = 1; i < kRouterSplits; ++i) v += parts[i][e][t];
-    const int expert = expert_group * kRouterExperts + e;
-    if (expert < p.experts && token0 + t < p.tokens) p.logits[static_cast<long long>(token0 + t) * p.experts + expert] = v;
+      for (int i = 0; i < kRouterWarps; ++i) v[i & 3] += parts[i][e][t];
+      double key = (v[0] + v[1]) + (v[2] + v[3]);
+      if (p.bias != nullptr && p.score == QX_MOE_SIGMOID) key = 1.0 / (1.0 + exp(-key)) + static_cast<double>(p.bias[expert0 + e]);
+      uint32_t to;
+      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(keys + t * p.experts + expert0 + e)));
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(ordered(key)) : "memory");
+    }
+    __syncthreads();
   }
-  if (!arrives_last(p.arrivals + token_group, expert_groups, &last)) return;
-  if (token0 + warp < p.tokens) {
-    if (p.experts <= 128) choose<4>(p, token0 + warp);
-    else choose<kMostExperts / 32>(p, token0 + warp);
-  }
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (rank == 0 && warp < kRouterTokens && token0 + warp < p.tokens) choose(p, keys + warp * p.experts, token0 + warp);
 }
 
 // ---- experts -----------------------------------------------------------------------------------
@@ -405,6 +431,18 @@ struct ExpertShape {
 __device__ __forceinline__ void sort_pairs(const Params& p, int most, SortSpace& s, Plan& plan) {
   const int experts = p.experts + p.shared, places = p.top + p.shared, entries = p.tokens * places;
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  if (p.tokens == 1) {  // a group for every pick
+    if (threadIdx.x < entries) {
+      plan.list[threadIdx.x] = static_cast<uint16_t>(threadIdx.x);
+      Group& to = plan.group[threadIdx.x];
+      to.expert = static_cast<uint32_t>(__ldcg(p.picks + threadIdx.x));
+      to.first = threadIdx.x;
+      to.count = 1;
+    }
+    if (threadIdx.x == 0) plan.groups = entries;
+    __syncthreads();
+    return;
+  }
   constexpr int kEach = (kPassEntries + kExpertThreads - 1) / kExpertThreads;
   int pick[kEach];
 #pragma unroll
@@ -1001,6 +1039,40 @@ struct Layout {
   }
 };
 
+template <int kX, int kW>
+qx_status launch_router(const Params& p, cudaStream_t stream) {
+  static SmemOptIn opt_in;
+  QX_TRY(opt_in.ensure(moe_router_kernel<kX, kW>, kPartBytes + kRouterTokens * kMostExperts * 8));
+  int size = 1;
+  while (size < kRouterCluster && size * kRouterExperts < p.experts) size *= 2;
+  const int convert = (p.tokens * ((p.dim + 127) / 128) + kRouterWarps - 1) / kRouterWarps;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(((p.tokens + kRouterTokens - 1) / kRouterTokens + (convert + size - 1) / size) * size);
+  config.blockDim = dim3(kRouterThreads);
+  config.dynamicSmemBytes = kPartBytes + static_cast<size_t>(kRouterTokens) * p.experts * 8;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = size;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  config.attrs = attributes;
+  config.numAttrs = 2;
+  QX_CUDA_TRY(cudaLaunchKernelEx(&config, moe_router_kernel<kX, kW>, p));
+  count_launch();
+  return QX_STATUS_OK;
+}
+
+template <int kX>
+qx_status launch_router(const Params& p, cudaStream_t stream) {
+  switch (p.router_type) {
+    case QX_STORAGE_F32: return launch_router<kX, QX_STORAGE_F32>(p, stream);
+    case QX_STORAGE_F16: return launch_router<kX, QX_STORAGE_F16>(p, stream);
+    default: return launch_router<kX, QX_STORAGE_BF16>(p, stream);
+  }
+}
+
 template <int kFormat, int kDigits>
 qx_status launch_experts(const Params& p, long long grid, cudaStream_t stream) {
   static SmemOptIn opt_in;
@@ -1045,7 +1117,6 @@ qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_ro
   const size_t entries = static_cast<size_t>(pass) * (p.top + p.shared);
   Layout l;
   const size_t at_x = l.take(pass * p.digits * p.dim), at_x_scales = l.take(pass * scales_of(p.dim) * sizeof(float));
-  const size_t at_logits = l.take(static_cast<size_t>(pass) * p.experts * sizeof(double));
   const size_t at_picks = l.take(entries * sizeof(int)), at_weights = l.take(entries * sizeof(float));
   const size_t at_progress = l.take(sizeof(Progress)), at_done = l.take(entries * sizeof(int));
   const size_t at_inner = l.take(entries * p.digits * p.inner);
@@ -1053,10 +1124,8 @@ qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_ro
   const size_t at_products = l.take(entries * p.dim * sizeof(float));
   QX_TRY(workspace->reserve(l.total));
   uint8_t* const base = static_cast<uint8_t*>(workspace->base);
-  p.arrivals = reinterpret_cast<int*>(base);
   p.x_digits = reinterpret_cast<int8_t*>(base + at_x);
   p.x_scales = reinterpret_cast<float*>(base + at_x_scales);
-  p.logits = reinterpret_cast<double*>(base + at_logits);
   p.picks = reinterpret_cast<int*>(base + at_picks);
   p.weights = reinterpret_cast<float*>(base + at_weights);
   p.progress = reinterpret_cast<Progress*>(base + at_progress);
@@ -1071,9 +1140,9 @@ qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_ro
     p.out = static_cast<uint8_t*>(out->data) + t0 * out->stride * out_size;
     p.chosen = chosen == nullptr ? nullptr : chosen + t0 * p.top;
     p.chosen_weights = weights == nullptr ? nullptr : weights + t0 * p.top;
-    const int router_ctas = (p.tokens + kRouterTokens - 1) / kRouterTokens * ((p.experts + kRouterExperts - 1) / kRouterExperts);
-    const int convert_ctas = (p.tokens * ((p.dim + 127) / 128) + 7) / 8;
-    QX_TRY(kv::launch_behind(moe_router_kernel, router_ctas + convert_ctas, kRouterThreads, 0, stream, p));
+    QX_TRY(p.x_type == QX_STORAGE_F32   ? launch_router<QX_STORAGE_F32>(p, stream)
+           : p.x_type == QX_STORAGE_F16 ? launch_router<QX_STORAGE_F16>(p, stream)
+                                        : launch_router<QX_STORAGE_BF16>(p, stream));
     // (no more CTAs than there may be units)
     const long long units = static_cast<long long>(p.tokens) * (p.top + p.shared) * (p.inner / 32);
     const long long grid = std::min<long long>(2LL * ctx->prop.multiProcessorCount, units);

@@ -62,10 +62,8 @@ struct Params {
   int32_t* chosen;       // [token][top], may be NULL
   float* chosen_weights;
   // scratch
-  int* arrivals;         // one per eight tokens, zero between calls
   int8_t* x_digits;      // [token][digit][dim]
   float* x_scales;
-  double* logits;        // [token][expert]
   int* picks;            // [token][top + shared] experts
   float* weights;        // [token][top + shared]
   Progress* progress;

@@ -54,8 +54,9 @@ def route(m, x, top, sigmoid=False, biased=False, normalise=True, scale=1.0, cho
     experts may lie closer together than sums in f32 tell apart) and taken."""
     x, w = x.double(), m.router.double()
     logits = x @ w.T
-    # eight products a sum in f32 (eight roundings of no more than the products' magnitudes), then 64 bits
-    off = 8 * U * (x.abs() @ w.abs().T)
+    # exact products, 32 a sum in f32 (f32 and f16 operands: their terms' products too, which are no larger) as MMAs take them, in
+    # 2 .. 18 steps that cut off, 2 u of no more than the products' magnitudes each, then 64 bits
+    off = 36 * U * (x.abs() @ w.abs().T)
     score = torch.sigmoid(logits) if sigmoid else torch.softmax(logits, 1)
     # (a logit that is off by o moves every score's share by no more than 2 o relative)
     key, key_off = (score + m.bias.double(), 2 * off.amax(1, keepdim=True) * score) if biased else (logits, off)
@@ -69,7 +70,8 @@ def route(m, x, top, sigmoid=False, biased=False, normalise=True, scale=1.0, cho
         assert bool((moved <= 2 * key_off.amax(1, keepdim=True)).all()), "another choice"
     picked = score.gather(1, chosen)
     weights = scale * (picked / picked.sum(1, keepdim=True) if normalise else picked)
-    return chosen, weights, weights.abs() * (2 * off.amax(1, keepdim=True) + 2 * U)
+    # (exponents are rounded to f32: u of their size moves a score by as much, relative; exp, sums and quotients 8 u)
+    return chosen, weights, weights.abs() * (2 * off.amax(1, keepdim=True) + (8 + 4 * logits.abs().amax(1, keepdim=True)) * U)
 
 
 def apply(m, x, top, activation=SILU, sigmoid=False, biased=False, normalise=True, scale=1.0, out_type=None, chosen=None):
