@@ -725,6 +725,20 @@ QX_API qx_status qx_kv_attention_dev(const qx_kv_cache* cache, const qx_kv_batch
                                      float scale, int causal, long long window,
                                      qx_workspace* workspace, void* stream);
 
+/* Attention for trees of drafted tokens: the rows of a sequence (64 at most) are drafts that continue its text in several
+ * ways; append them first, each with its position (that of its depth in the tree). Row i sees all tokens in front of the
+ * drafts, and draft j of its sequence (the token of row j) where bit j of seen[row i] is set: its ancestors and
+ * itself. Bits of rows that the sequence does not have count for nothing. `window` is 0 or 64 and more: a row that sees d drafts stands
+ * at position (tokens in front) + d - 1, and keys in front of the drafts at that position - window and before are hidden.
+ * `seen` has an entry for every row of the views. All else is as for qx_kv_attention. Tokens that are accepted
+ * in the end are appended again, in their order, as the last tokens of a sequence of that length. */
+QX_API qx_status qx_kv_tree_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q,
+                                      const qx_heads* out, float* lse, float scale, long long window,
+                                      const uint64_t* seen);
+QX_API qx_status qx_kv_tree_attention_dev(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q,
+                                          const qx_heads* out, float* lse_dev, float scale, long long window,
+                                          const uint64_t* seen_dev, qx_workspace* workspace, void* stream);
+
 /* ---- between the blocks of a layer --------------------------------------------------------
  * The norm behind a block, its gate and residual scale, the sum with the residual stream and the norm in
  * front of the next block, in one pass over the rows:

@@ -211,6 +211,10 @@ def _load():
                             C.POINTER(HeadsView), _vp, C.c_float, C.c_int, _ll],
         "qx_kv_attention_dev": [C.POINTER(KVCacheView), C.POINTER(KVBatchView), C.POINTER(HeadsView),
                                 C.POINTER(HeadsView), _vp, C.c_float, C.c_int, _ll, _vp, _vp],
+        "qx_kv_tree_attention": [C.POINTER(KVCacheView), C.POINTER(KVBatchView), C.POINTER(HeadsView),
+                                 C.POINTER(HeadsView), _vp, C.c_float, _ll, _vp],
+        "qx_kv_tree_attention_dev": [C.POINTER(KVCacheView), C.POINTER(KVBatchView), C.POINTER(HeadsView),
+                                     C.POINTER(HeadsView), _vp, C.c_float, _ll, _vp, _vp, _vp],
         "qx_residual_norm": [C.POINTER(RowsView), C.POINTER(RowsView), C.POINTER(NormView), C.POINTER(RowsView), C.c_float,
                              C.POINTER(RowsView), C.POINTER(NormView), C.POINTER(RowsView), _ll, _ll],
         "qx_residual_norm_dev": [C.POINTER(RowsView), C.POINTER(RowsView), C.POINTER(NormView), C.POINTER(RowsView),
@@ -861,6 +865,15 @@ class KVCache:
         return lib.qx_kv_attention(self.view, batch.view, _rows(q, tokens, dim, kind), _rows(out, tokens, dim, kind),
                                    _array(lse, "float32", None, tokens, q.shape[1]), scale, 1 if causal else 0, window)
 
+    def tree_attention(self, batch, q, out, seen, scale=None, window=0, lse=None, kind=None) -> int:
+        """seen: int64 [tokens], bit j of row i: it sees the draft of row j of its sequence."""
+        assert self.device is None and batch.device is None, "need numpy arrays"
+        tokens, dim = batch.view.tokens, self.view.head_dim
+        scale = dim ** -0.5 if scale is None else scale
+        return lib.qx_kv_tree_attention(self.view, batch.view, _rows(q, tokens, dim, kind), _rows(out, tokens, dim, kind),
+                                        _array(lse, "float32", None, tokens, q.shape[1]), scale, window,
+                                        _array(seen, "int64", None, tokens))
+
     # device tensors, torch's current stream
     def append_dev(self, batch, k, v, rope=None, q=None, q_out=None, positions=None) -> int:
         device = _device()
@@ -886,6 +899,16 @@ class KVCache:
                                        _device_rows(out, tokens, dim, device),
                                        _array(lse, "float32", device, tokens, q.shape[1]), scale, 1 if causal else 0, window,
                                        workspace, _stream())
+
+    def tree_attention_dev(self, batch, q, out, seen, scale=None, window=0, lse=None, workspace=None) -> int:
+        device = _device()
+        assert self.device == device == batch.device, "need tensors on the current device"
+        tokens, dim = batch.view.tokens, self.view.head_dim
+        scale = dim ** -0.5 if scale is None else scale
+        return lib.qx_kv_tree_attention_dev(self.view, batch.view, _device_rows(q, tokens, dim, device),
+                                            _device_rows(out, tokens, dim, device),
+                                            _array(lse, "float32", device, tokens, q.shape[1]), scale, window,
+                                            _array(seen, "int64", device, tokens), workspace, _stream())
 
 
 # ---- between the blocks of a layer: norms, gate, residual sum ----

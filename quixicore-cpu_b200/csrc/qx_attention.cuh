@@ -18,6 +18,7 @@ struct AttentionParams {
   float* lse;
   float scale_log2;  // scale * log2(e)
   int causal, window;
+  const uint64_t* tree;  // [row of the views] drafts that it sees; NULL: no trees
   int group;         // query heads per kv head
   int tile_rows;     // rows of a tile
   int row_tiles, splits, chunk;
@@ -41,6 +42,24 @@ __device__ __forceinline__ int first_seen(const AttentionParams& p, int position
   return p.window > 0 && position >= p.window ? position - p.window + 1 : 0;
 }
 
+// kTree: the sequence's rows are drafts, row i sees those in front of them and draft j where bit j of its mask says so. Its
+// position is the one behind as many drafts as it sees, itself among them.
+constexpr int kTreeRows = 64;
+__device__ __forceinline__ uint64_t drafts_of(const AttentionParams& p, const Rows& r, int token) {
+  return p.tree[r.row + token] & (r.n >= kTreeRows ? ~0ull : (1ull << r.n) - 1);
+}
+// Which of the kKeys (16 or 32) keys from `key` on a row sees: bit i, key + i. `low`: its first key; `start`: the first draft.
+template <int kKeys>
+__device__ __forceinline__ uint32_t seen_of(uint64_t drafts, int key, int start, int low) {
+  constexpr uint32_t kAll = static_cast<uint32_t>((1ull << kKeys) - 1);
+  const int in = key - start;  // (the drafts end the text: nothing is behind them)
+  uint32_t seen = in >= kTreeRows ? 0u : in >= 0 ? static_cast<uint32_t>(drafts >> in)
+                  : in > -kKeys ? static_cast<uint32_t>(drafts << -in) | ((1u << -in) - 1) : kAll;
+  const int hidden = min(max(low - key, 0), kKeys);
+  return seen & kAll & static_cast<uint32_t>(~((1ull << hidden) - 1));
+}
+
+template <bool kTree = false>
 __device__ __forceinline__ bool rows_of(const AttentionParams& p, int s, int first, int most, Rows* r, bool each = false) {
   Sequence q;
   if (!sequence_of(p.batch, s, false, &q, each)) return false;
@@ -52,8 +71,8 @@ __device__ __forceinline__ bool rows_of(const AttentionParams& p, int s, int fir
   r->first = first;
   r->count = static_cast<int>(min(static_cast<long long>(most), total - first));
   const int start = q.length - q.n;  // (negative where the sequence has more rows than tokens)
-  const int position0 = start + first / p.group, position1 = start + (first + r->count - 1) / p.group;
-  r->high = max(0, p.causal ? min(q.length, position1 + 1) : q.length);
+  const int position0 = kTree ? start - 1 : start + first / p.group, position1 = start + (first + r->count - 1) / p.group;
+  r->high = max(0, p.causal && !kTree ? min(q.length, position1 + 1) : q.length);
   r->low = first_seen(p, position0) & ~31;
   r->low = min(r->low, r->high);
   return true;
@@ -81,6 +100,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
 constexpr int kPromptRows = 256, kPromptRowsWide = 128;
 constexpr float kPromptShift = 11.0f;
 qx_status launch_prompt(const AttentionParams& p, bool wide, long long grid, cudaStream_t stream);
+// The streamed kernel for trees (qx_attention_tree.cu).
+qx_status launch_tree_streamed(const AttentionParams& p, int dp, bool wide, bool balanced, long long grid, cudaStream_t stream);
 
 }  // namespace kv
 }  // namespace qx

@@ -165,6 +165,8 @@ __device__ __forceinline__ void convert16(const uint4& codes, uint4* a, uint4* b
 struct RowState {
   float factor;       // of the raw scores, log2(e) in it
   int low, high;      // keys that the row sees
+  int start;          // kTree: of the keys from here on, those that `drafts` names
+  uint64_t drafts;
   float maximum, sum;
   float largest_log, largest;  // value scale that it has seen, and its log2
 };
@@ -178,7 +180,7 @@ struct RowState {
 // 46.5.)
 // kWide: the row's factor for what O holds so far goes to *keep_to instead.
 enum Mask { kOpen, kHidden, kSpecial };
-template <int DP, int kUnit, Mask kMask, bool kWide>
+template <int DP, int kUnit, Mask kMask, bool kWide, bool kTree>
 __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, const Meta& meta, RowState& row, int key0,
                                              bool first, uint64_t* first_half, float* keep_to) {
   constexpr int kUnits = kKeys / kUnit, kPerUnit = kUnit / 16;
@@ -195,7 +197,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
     log[u] = scales.y;
     relative[u] = meta.value_inverse[u * kPerUnit];
     const int key = key0 + kUnit * u;
-    const bool seen = kMask == kOpen || (meta.present[u * kPerUnit] != 0 && key < row.high && key + kUnit > row.low);
+    const bool seen = kMask == kOpen || (meta.present[u * kPerUnit] != 0 && key < row.high && key + kUnit > row.low &&
+                                         (!kTree || seen_of<kUnit>(row.drafts, key, row.start, row.low) != 0));
     largest = fmaxf(largest, seen ? log[u] : -INFINITY);
   }
   // The sum stands against the largest scale and the maximum. It follows both in one step: alone, a rise of the scale by
@@ -213,10 +216,13 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
     log[u] = log[u] < least ? least : log[u];  // (no number stays none)
   }
 
-  const auto hidden = [&](int key) { return key < row.low || key >= row.high; };
+  const auto hidden = [&](int key) {
+    return key < row.low || key >= row.high || (kTree && key >= row.start && !(row.drafts >> (key - row.start) & 1));
+  };
   const auto hide = [&](int c) {  // of 32 keys
     const int low = min(max(row.low - key0 - 32 * c, 0), 32), high = min(max(row.high - key0 - 32 * c, 0), 32);
     uint32_t seen = static_cast<uint32_t>((1ull << high) - 1) & ~static_cast<uint32_t>((1ull << low) - 1);
+    if (kTree) seen &= seen_of<32>(row.drafts, key0 + 32 * c, row.start, row.low);
     if (meta.present[2 * c] == 0) seen &= 0xFFFF0000u;
     if (meta.present[2 * c + 1] == 0) seen &= 0xFFFFu;
     if (__all_sync(0xFFFFFFFFu, seen == 0xFFFFFFFFu)) return;
@@ -432,7 +438,7 @@ __device__ __forceinline__ void write_row(const AttentionParams& p, const uint32
   }
 }
 
-template <int DP, int kUnit, bool kWide>
+template <int DP, int kUnit, bool kWide, bool kTree>
 __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_constant__ AttentionParams p) {
   using S = TcShape<DP>;
   extern __shared__ uint8_t raw_smem[];
@@ -455,7 +461,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   const int s = static_cast<int>(by_head / p.kv_heads), head = static_cast<int>(by_head - s * p.kv_heads);
   Rows rows;
   constexpr int kCtaRows = kWide ? kRowTile : 2 * kRowTile;
-  if (!rows_of(p, s, row_tile * kCtaRows, kCtaRows, &rows)) return;
+  if (!rows_of<kTree>(p, s, row_tile * kCtaRows, kCtaRows, &rows)) return;
   int begin, end;
   if (!chunk_of(p, rows, split, &begin, &end)) return;
   const int tiles = max(0, (end - begin + kKeys - 1) / kKeys);
@@ -555,13 +561,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       const long long row_at = rows.row + token, out_head = static_cast<long long>(head) * p.group + member;
       RowState row;
       row.low = row.high = 0;
+      row.start = start;
+      row.drafts = 0;
       row.maximum = -INFINITY;
       row.sum = 0.0f;
       row.largest_log = -INFINITY;
       row.largest = 0.0f;
       if (real) {
-        row.high = p.causal ? min(rows.length, start + token + 1) : rows.length;
-        row.low = first_seen(p, start + token);
+        row.high = p.causal && !kTree ? min(rows.length, start + token + 1) : rows.length;
+        if (kTree) row.drafts = drafts_of(p, rows, token);
+        row.low = first_seen(p, start + (kTree ? __popcll(row.drafts) - 1 : token));
       }
       // The queries: f16 times a power of two that brings the row's largest magnitude to 2^7 .. 2^8. A warp copies its
       // rows as they are to where their operands go, runs of lanes to a row; then each thread converts its own row in
@@ -650,8 +659,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       // below open_high and from open_low on no row of the tile has a hidden key
       const int last = min(rows.count, (which + 1) * kRowTile) - 1;
       const int position0 = start + (rows.first + which * kRowTile) / p.group, position1 = start + (rows.first + last) / p.group;
-      const int open_high = p.causal ? min(rows.length, position0 + 1) : rows.length;
-      const int open_low = first_seen(p, position1);
+      const int open_high = kTree ? start : p.causal ? min(rows.length, position0 + 1) : rows.length;
+      const int open_low = first_seen(p, kTree ? start + rows.n - 1 : position1);
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t sums = tmem + lanes + 256 + which * 128;
       for (int j = 0; ok && j < tiles; ++j) {
@@ -671,7 +680,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         }
         float* const keep_to = keep + j % kKeepStages * kRowTile + r;
         if (__all_sync(0xFFFFFFFFu, open)) {
-          softmax_tile<DP, kUnit, kOpen, kWide>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+          softmax_tile<DP, kUnit, kOpen, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
         } else {
           bool plain = true;
 #pragma unroll 1
@@ -681,9 +690,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
             plain = plain && factor > 0.0f && factor < INFINITY && fabsf(scales.y) < INFINITY;
           }
           if (__all_sync(0xFFFFFFFFu, plain)) {
-            softmax_tile<DP, kUnit, kHidden, kWide>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+            softmax_tile<DP, kUnit, kHidden, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
           } else {
-            softmax_tile<DP, kUnit, kSpecial, kWide>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+            softmax_tile<DP, kUnit, kSpecial, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
           }
         }
         tc_fence_before_sync();
@@ -941,24 +950,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   }
 }
 
-template <int DP, int kUnit, bool kWide>
+template <int DP, int kUnit, bool kWide, bool kTree>
 qx_status launch_prompt_of(const AttentionParams& p, long long grid, cudaStream_t stream) {
   static SmemOptIn opt_in;
-  QX_TRY(opt_in.ensure(prompt_kernel<DP, kUnit, kWide>, TcShape<DP>::kBytes));
-  return launch_behind(prompt_kernel<DP, kUnit, kWide>, grid, kTcThreads, TcShape<DP>::kBytes, stream, p);
+  QX_TRY(opt_in.ensure(prompt_kernel<DP, kUnit, kWide, kTree>, TcShape<DP>::kBytes));
+  return launch_behind(prompt_kernel<DP, kUnit, kWide, kTree>, grid, kTcThreads, TcShape<DP>::kBytes, stream, p);
 }
-template <bool kWide>
+template <bool kWide, bool kTree>
 qx_status launch_prompt_sized(const AttentionParams& p, long long grid, cudaStream_t stream) {
   if (p.block_tokens < 32) {
-    return p.dim <= 64 ? launch_prompt_of<64, 16, kWide>(p, grid, stream) : launch_prompt_of<128, 16, kWide>(p, grid, stream);
+    return p.dim <= 64 ? launch_prompt_of<64, 16, kWide, kTree>(p, grid, stream) : launch_prompt_of<128, 16, kWide, kTree>(p, grid, stream);
   }
-  return p.dim <= 64 ? launch_prompt_of<64, 32, kWide>(p, grid, stream) : launch_prompt_of<128, 32, kWide>(p, grid, stream);
+  return p.dim <= 64 ? launch_prompt_of<64, 32, kWide, kTree>(p, grid, stream) : launch_prompt_of<128, 32, kWide, kTree>(p, grid, stream);
 }
 
 }  // namespace
 
 qx_status launch_prompt(const AttentionParams& p, bool wide, long long grid, cudaStream_t stream) {
-  return wide ? launch_prompt_sized<true>(p, grid, stream) : launch_prompt_sized<false>(p, grid, stream);
+  if (p.tree != nullptr) return wide ? launch_prompt_sized<true, true>(p, grid, stream) : launch_prompt_sized<false, true>(p, grid, stream);
+  return wide ? launch_prompt_sized<true, false>(p, grid, stream) : launch_prompt_sized<false, false>(p, grid, stream);
 }
 
 }  // namespace kv

@@ -23,8 +23,10 @@ qx_status launch_append(const qx_kv_cache* cache, const qx_kv_batch* batch, cons
 qx_status launch_read(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* k, const qx_heads* v,
                       DeviceContext* ctx, cudaStream_t stream);
 qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q, const qx_heads* out,
-                           float* lse, float scale, int causal, long long window, DeviceContext* ctx,
+                           float* lse, float scale, int causal, long long window, const uint64_t* tree, DeviceContext* ctx,
                            qx_workspace* workspace, cudaStream_t stream);
+qx_status check_tree_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q, const qx_heads* out,
+                               const float* lse, float scale, long long window, const uint64_t* seen);
 
 namespace {
 
@@ -165,6 +167,32 @@ struct PackedArrays {
 using namespace qx;
 using namespace qx::kv;
 
+// `seen`: masks of drafts, or NULL.
+static qx_status attention_of(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q, const qx_heads* out, float* lse,
+                              float scale, int causal, long long window, const uint64_t* seen) {
+  return guarded([&]() -> qx_status {
+    Packed p;
+    QX_TRY(pack(cache, batch, false, false, &p));
+    DeviceContext* ctx = nullptr;
+    QX_TRY(current_context(&ctx));
+    std::lock_guard<std::mutex> lock(ctx->mutex);
+    Arrays a;
+    PackedArrays pa;
+    pa.add(&a, p, false);
+    const int aq = add_view(&a, q, batch->tokens, cache->head_dim, false);
+    const int ao = add_view(&a, out, batch->tokens, cache->head_dim, true);
+    const int al = lse == nullptr ? -1 : a.add(lse, static_cast<size_t>(batch->tokens) * q->heads * 4, true);
+    const int at = seen == nullptr ? -1 : a.add(seen, static_cast<size_t>(batch->tokens) * sizeof(uint64_t), false);
+    QX_TRY(a.to_device(ctx));
+    const qx_kv_cache dc = pa.cache(a, cache, p);
+    const qx_kv_batch db = pa.batch(a, batch, p);
+    const qx_heads dq = on_device(a, q, aq), dout = on_device(a, out, ao);
+    QX_TRY(launch_attention(&dc, &db, &dq, &dout, a.device<float>(al), scale, causal, window, a.device<uint64_t>(at), ctx,
+                            &ctx->workspace, ctx->stream));
+    return a.from_device();
+  });
+}
+
 extern "C" {
 
 qx_status qx_rope_apply(const qx_rope* rope, const qx_heads* x, const qx_heads* y, const int64_t* positions,
@@ -248,26 +276,13 @@ qx_status qx_kv_read(const qx_kv_cache* cache, const qx_kv_batch* batch, const q
 qx_status qx_kv_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q, const qx_heads* out,
                           float* lse, float scale, int causal, long long window) {
   QX_TRY(check_attention(cache, batch, q, out, lse, scale, window));
-  return guarded([&]() -> qx_status {
-    Packed p;
-    QX_TRY(pack(cache, batch, false, false, &p));
-    DeviceContext* ctx = nullptr;
-    QX_TRY(current_context(&ctx));
-    std::lock_guard<std::mutex> lock(ctx->mutex);
-    Arrays a;
-    PackedArrays pa;
-    pa.add(&a, p, false);
-    const int aq = add_view(&a, q, batch->tokens, cache->head_dim, false);
-    const int ao = add_view(&a, out, batch->tokens, cache->head_dim, true);
-    const int al = lse == nullptr ? -1 : a.add(lse, static_cast<size_t>(batch->tokens) * q->heads * 4, true);
-    QX_TRY(a.to_device(ctx));
-    const qx_kv_cache dc = pa.cache(a, cache, p);
-    const qx_kv_batch db = pa.batch(a, batch, p);
-    const qx_heads dq = on_device(a, q, aq), dout = on_device(a, out, ao);
-    QX_TRY(launch_attention(&dc, &db, &dq, &dout, a.device<float>(al), scale, causal, window, ctx, &ctx->workspace,
-                            ctx->stream));
-    return a.from_device();
-  });
+  return attention_of(cache, batch, q, out, lse, scale, causal, window, nullptr);
+}
+
+qx_status qx_kv_tree_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q, const qx_heads* out,
+                               float* lse, float scale, long long window, const uint64_t* seen) {
+  QX_TRY(check_tree_attention(cache, batch, q, out, lse, scale, window, seen));
+  return attention_of(cache, batch, q, out, lse, scale, 1, window, seen);
 }
 
 }  // extern "C"
