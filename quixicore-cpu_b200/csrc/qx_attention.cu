@@ -12,6 +12,7 @@ namespace {
 // rows 101 | 54; one of 16384 keys, 48 rows 42 | 41; f32, 4 of 4096 keys, 64 rows 84 | 87, 100 rows 96 | 90; 16 whole
 // texts of 64 tokens 25 | 29, of 100 tokens 40 | 32.
 constexpr long long kPromptFrom = 48, kPromptFromWide = 96;
+constexpr long long kSpreadUpTo = 128;
 
 // Joins the chunks of one row, in an order that their number fixes: the threads are cut into parts, a thread of part i
 // takes four head elements of chunks i, i + parts, ..., with several chunks' loads under way before it uses the first.
@@ -92,6 +93,73 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   }
 }
 
+// The same for trees and few chunks: a CTA takes every `stride`th row of a tile, dim / 4 threads to a row, each all of its chunks
+// in their order. (Six trees of 63 drafts, 189 rows, three chunks: 22 us with a thread block per row, which most of these are
+// too small for.)
+constexpr int kTreeJoinThreads = 256, kTreeJoinSplits = 32;
+struct TreeJoin {
+  AttentionParams attention;
+  int stride;
+};
+__global__ void __launch_bounds__(kTreeJoinThreads) tree_join_kernel(const __grid_constant__ TreeJoin j) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  const AttentionParams& p = j.attention;
+  const int first_row = static_cast<int>(blockIdx.x % j.stride);
+  const long long tile_index = blockIdx.x / j.stride;
+  const int row_tile = static_cast<int>(tile_index % p.row_tiles);
+  const int head = static_cast<int>(tile_index / p.row_tiles % p.kv_heads);
+  const int s = static_cast<int>(tile_index / p.row_tiles / p.kv_heads);
+  Rows rows;
+  if (!rows_of<true>(p, s, row_tile * p.tile_rows, p.tile_rows, &rows)) return;
+  const int used = splits_used(p, rows);
+  if (used == 1) return;
+  const int vectors = p.dim / 4, count = (rows.count - first_row + j.stride - 1) / j.stride * vectors;
+  for (int i = threadIdx.x; i < count; i += kTreeJoinThreads) {
+    const int r = first_row + i / vectors * j.stride, at = i % vectors;
+    const long long first = tile_index * p.splits * p.tile_rows + r;
+    float top = -INFINITY, sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int kBatch = 8;  // loads under way
+    for (int c0 = 0; c0 < used; c0 += kBatch) {
+      float2 stat[kBatch];
+      float4 x[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        stat[b] = make_float2(-INFINITY, 0.0f);
+        x[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (c0 + b < used) {
+          const long long from = first + static_cast<long long>(c0 + b) * p.tile_rows;
+          stat[b] = __ldcg(reinterpret_cast<const float2*>(p.statistics) + from);
+          x[b] = __ldcg(reinterpret_cast<const float4*>(p.partial + from * p.dim) + at);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const float most = fmaxf(top, stat[b].x), base = most == -INFINITY ? 0.0f : most;
+        const float keep = exp2_fast(top - base), weight = exp2_fast(stat[b].x - base);
+        top = most;
+        sum = fmaf(sum, keep, stat[b].y * weight);
+        v.x = fmaf(v.x, keep, x[b].x * weight);
+        v.y = fmaf(v.y, keep, x[b].y * weight);
+        v.z = fmaf(v.z, keep, x[b].z * weight);
+        v.w = fmaf(v.w, keep, x[b].w * weight);
+      }
+    }
+    const float inverse = sum == 0.0f ? 0.0f : exp2f(p.shift) / sum;
+    const int token = (rows.first + r) / p.group, member = (rows.first + r) % p.group;
+    const long long out_row = rows.row + token, out_head = static_cast<long long>(head) * p.group + member;
+    const long long to = out_row * p.out.token_stride + out_head * p.out.head_stride + 4 * at;
+    store_one(p.out.data, p.out.type, to, v.x * inverse);
+    store_one(p.out.data, p.out.type, to + 1, v.y * inverse);
+    store_one(p.out.data, p.out.type, to + 2, v.z * inverse);
+    store_one(p.out.data, p.out.type, to + 3, v.w * inverse);
+    if (at == 0 && p.lse != nullptr) {
+      p.lse[out_row * p.out.heads + out_head] = sum == 0.0f ? -INFINITY : (top + log2f(sum) - p.shift) * 0.69314718055994531f;
+    }
+  }
+}
+
 }  // namespace
 
 qx_status check_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q, const qx_heads* out,
@@ -146,7 +214,8 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   const long long most_rows = static_cast<long long>(batch->max_tokens) * p.group;
   const bool wide = q->type == QX_STORAGE_F32;
   const bool prompt = cache->head_dim <= 128 && most_rows >= (wide ? kPromptFromWide : kPromptFrom);
-  p.tile_rows = prompt ? (wide ? kPromptRowsWide : kPromptRows) : most_rows <= 8 ? 8 : 16;
+  const bool spread = prompt && tree != nullptr && !wide && most_rows <= kSpreadUpTo;
+  p.tile_rows = prompt ? (wide ? kPromptRowsWide : spread ? kPromptRowsSpread : kPromptRows) : most_rows <= 8 ? 8 : 16;
   p.shift = prompt ? kPromptShift : kShift;
   p.row_tiles = static_cast<int>((most_rows + p.tile_rows - 1) / p.tile_rows);
   const long long items = static_cast<long long>(batch->sequences) * cache->kv_heads * p.row_tiles;
@@ -204,8 +273,14 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
     }
   }
   const long long grid = items * p.splits;
-  QX_TRY(prompt ? launch_prompt(p, wide, grid, stream) : streamed(false, grid));
+  QX_TRY(prompt ? launch_prompt(p, wide, spread, grid, stream) : streamed(false, grid));
   if (p.splits <= 1 || p.counters != nullptr) return QX_STATUS_OK;
+  if (tree != nullptr && p.splits <= kTreeJoinSplits) {
+    // two CTAs per SM, of a thread's worth of rows at least
+    const int most = std::max(1, p.tile_rows * (p.dim / 4) / kTreeJoinThreads);
+    const int stride = static_cast<int>(std::min<long long>(most, std::max(1LL, 2LL * ctx->prop.multiProcessorCount / items)));
+    return launch_behind(tree_join_kernel, items * stride, kTreeJoinThreads, 0, stream, TreeJoin{p, stride});
+  }
   return launch_behind(tree == nullptr ? join_kernel<false> : join_kernel<true>, items * p.tile_rows, p.splits <= 16 ? 128 : kJoinThreads, 0, stream, p);
 }
 

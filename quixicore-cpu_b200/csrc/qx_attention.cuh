@@ -97,9 +97,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 // Rows per CTA of the prompt kernel (qx_attention_tc.cu; f32 queries), and its shift: P is held times 2^11 .. 2^15
 // there.
-constexpr int kPromptRows = 256, kPromptRowsWide = 128;
+constexpr int kPromptRows = 256, kPromptRowsWide = 128, kPromptRowsSpread = 128;
 constexpr float kPromptShift = 11.0f;
-qx_status launch_prompt(const AttentionParams& p, bool wide, long long grid, cudaStream_t stream);
+// `spread`: of trees, 16-bit queries, in tiles of 128 rows.
+qx_status launch_prompt(const AttentionParams& p, bool wide, bool spread, long long grid, cudaStream_t stream);
 // The streamed kernel for trees (qx_attention_tree.cu).
 qx_status launch_tree_streamed(const AttentionParams& p, int dp, bool wide, bool balanced, long long grid, cudaStream_t stream);
 

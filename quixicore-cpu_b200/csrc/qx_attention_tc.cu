@@ -180,9 +180,10 @@ struct RowState {
 // 46.5.)
 // kWide: the row's factor for what O holds so far goes to *keep_to instead.
 enum Mask { kOpen, kHidden, kSpecial };
-template <int DP, int kUnit, Mask kMask, bool kWide, bool kTree>
+// `before`: kSpread, waits until the products that O holds so far are done (else they are, when S is there).
+template <int DP, int kUnit, Mask kMask, bool kWide, bool kTree, class Before>
 __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, const Meta& meta, RowState& row, int key0,
-                                             bool first, uint64_t* first_half, float* keep_to) {
+                                             bool first, uint64_t* first_half, float* keep_to, const Before& before_o) {
   constexpr int kUnits = kKeys / kUnit, kPerUnit = kUnit / 16;
   uint32_t s[4][32];
   tmem_ld_32x32(scores, s[0]);
@@ -282,6 +283,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
     const float keep = exp2_fast(moved);
     rise += moved;
     if (!first) {
+      before_o();
 #pragma unroll 1
       for (int c = 0; c < DP; c += 16) {
         uint32_t o[16];
@@ -438,7 +440,9 @@ __device__ __forceinline__ void write_row(const AttentionParams& p, const uint32
   }
 }
 
-template <int DP, int kUnit, bool kWide, bool kTree>
+// kSpread: one tile of 128 rows; warps 4-7 take the conversion of the values from warps 8-11, and S of the next tile of keys
+// is computed during a softmax, in the second row tile's place.
+template <int DP, int kUnit, bool kWide, bool kTree, bool kSpread>
 __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_constant__ AttentionParams p) {
   using S = TcShape<DP>;
   extern __shared__ uint8_t raw_smem[];
@@ -460,12 +464,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   const long long tile_index = static_cast<long long>(by_head) * p.row_tiles + row_tile;
   const int s = static_cast<int>(by_head / p.kv_heads), head = static_cast<int>(by_head - s * p.kv_heads);
   Rows rows;
-  constexpr int kCtaRows = kWide ? kRowTile : 2 * kRowTile;
+  constexpr int kCtaRows = kWide || kSpread ? kRowTile : 2 * kRowTile;
+  static_assert(!(kWide && kSpread), "f32 queries have work for warps 4-7");
   if (!rows_of<kTree>(p, s, row_tile * kCtaRows, kCtaRows, &rows)) return;
   int begin, end;
   if (!chunk_of(p, rows, split, &begin, &end)) return;
   const int tiles = max(0, (end - begin + kKeys - 1) / kKeys);
-  const int row_tiles = !kWide && rows.count > kRowTile ? 2 : 1;
+  const int row_tiles = !kWide && !kSpread && rows.count > kRowTile ? 2 : 1;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -498,11 +503,135 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   const uint32_t tmem = bars->tmem_base;
   bool ok = true;
 
+  // ---- codes to operands, by four warps -----------------------------------------------------
+  const auto convert = [&](bool keys, bool values) {
+    const int w = warp & 3;
+    const int32_t* const table = p.batch.table + s * p.batch.table_stride;
+    constexpr int kHalves = DP / 64;     // 64 codes of a row: one swizzled row of f16
+    constexpr int kLoads = 4 * kHalves;  // per thread and tile: 32 keys per warp, eight at a time
+    uint4 codes[kLoads];  // of one operand: the next to be stored
+    // ids of the blocks of this warp's two groups of 16 keys; -1: nothing there
+    const auto ids_of = [&](int j, int (&id)[2]) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int key = begin + j * kKeys + 32 * w + 16 * g;
+        id[g] = -1;
+        if (j < tiles && key < end) {
+          const int block = table[key >> p.block_shift];
+          if (block >= 0 && block < p.batch.blocks) id[g] = block;
+          else if (lane == 0) report_error(p.batch.error, kErrorBlock);
+        }
+      }
+    };
+    const auto load = [&](int j, const int (&id)[2], const int8_t* plane) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int slot = (begin + j * kKeys + 32 * w + 16 * g) & (p.block_tokens - 1);
+        const int8_t* const from =
+            plane + ((static_cast<long long>(max(id[g], 0)) * p.kv_heads + head) * p.block_tokens + slot) * p.dim;
+#pragma unroll
+        for (int i = 0; i < kLoads / 2; ++i) {
+          const int r = i / kHalves * 8 + (lane >> 2), d = i % kHalves * 64 + (lane & 3) * 16;
+          uint4 c = make_uint4(0, 0, 0, 0);  // (nothing there, or past the head: zeros)
+          if (id[g] >= 0 && (DP == p.dim || d < p.dim)) c = __ldg(reinterpret_cast<const uint4*>(from + r * p.dim + d));
+          codes[g * kLoads / 2 + i] = c;
+        }
+      }
+    };
+    const auto store = [&](uint8_t* operand) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int i = 0; i < kLoads / 2; ++i) {
+          const int r = 32 * w + 16 * g + i / kHalves * 8 + (lane >> 2), c = (lane & 3) * 2;
+          uint8_t* const row = operand + i % kHalves * (kKeys * 128) + r * 128;
+          uint4 a, b;
+          convert16(codes[g * kLoads / 2 + i], &a, &b);
+          *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = a;
+          *reinterpret_cast<uint4*>(row + (((c + 1) ^ (r & 7)) << 4)) = b;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    };
+    float scales[2] = {0.0f, 0.0f};  // of lane 0, 1: its group's
+    const auto load_scales = [&](const int (&id)[2]) {
+      const int own = lane == 1 ? id[1] : id[0];
+      if (lane < 2 && own >= 0) {
+        const long long slice = static_cast<long long>(own) * p.kv_heads + head;
+        scales[0] = p.k_scales[slice];
+        scales[1] = p.v_scales[slice];
+      }
+    };
+    // One of them alone (kSpread), or keys and then values of each tile.
+    int id[2], next[2];
+    ids_of(0, id);
+    load(0, id, keys ? p.k_codes : p.v_codes);
+    load_scales(id);
+    ids_of(1, next);
+    for (int j = 0; ok && j < tiles; ++j) {
+      const int stage = j & 1;
+      if (keys) {
+        if (j >= 2) ok = mbar_wait_warp(&bars->key_empty[stage], ((j >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+        if (lane < 2) {
+          const float vs = scales[1];
+          const float log = vs < kLeastScale ? kLeastLog : log2f(vs);  // (no number stays none)
+          Meta& m = meta[j % kMetaStages];
+          m.scales[2 * w + lane] = make_float2(scales[0], log);
+          // (of the scale itself: so the rounding of its logarithm, 2^-19 of a scale of 2^-64, is the weight's as much as
+          // the value's, and divided out; a whole number and the rest apart would keep it from the weights too, but take the
+          // f32 kernel 41.6 in place of 40.8 us, two f32 prompts of up to 4096 760 in place of 737)
+          m.value_inverse[2 * w + lane] = vs < kLeastScale ? exp2f(-kLeastLog) : 1.0f / vs;
+          m.present[2 * w + lane] = (lane == 1 ? id[1] : id[0]) >= 0;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->meta[j % kMetaStages]);
+        store(smem + S::kKeyRing + stage * S::kOperand);
+        if (lane == 0) mbar_arrive(&bars->key_full[stage]);
+      }
+      if (values && !keys) {
+        if (j >= 2) ok = mbar_wait_warp(&bars->value_empty[stage], ((j >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {  // (as below)
+          if (__shfl_sync(0xFFFFFFFFu, scales[1], g) < kLeastScale) {
+#pragma unroll
+            for (int i = 0; i < kLoads / 2; ++i) codes[g * kLoads / 2 + i] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        store(smem + S::kValueRing + stage * S::kOperand);
+        if (lane == 0) mbar_arrive(&bars->value_full[stage]);
+      } else if (values) {
+        // (a scale of zero makes zeros of any codes; it has no logarithm, so the codes stand for it)
+        const int value_id[2] = {__shfl_sync(0xFFFFFFFFu, scales[1], 0) < kLeastScale ? -1 : id[0],
+                                 __shfl_sync(0xFFFFFFFFu, scales[1], 1) < kLeastScale ? -1 : id[1]};
+        load(j, value_id, p.v_codes);
+        if (j + 1 < tiles) load_scales(next);
+        if (j >= 2) ok = mbar_wait_warp(&bars->value_empty[stage], ((j >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+        store(smem + S::kValueRing + stage * S::kOperand);
+        if (lane == 0) mbar_arrive(&bars->value_full[stage]);
+      }
+      if (!(keys && values) && j + 1 < tiles) load_scales(next);
+      if (j + 1 < tiles) load(j + 1, next, keys ? p.k_codes : p.v_codes);
+      id[0] = next[0];
+      id[1] = next[1];
+      ids_of(j + 2, next);
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      report_error(p.batch.error, 42);
+    }
+  };
+
   if (warp < 8) {
     // ---- softmax --------------------------------------------------------------------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
     const int which = warp >> 2;
-    if (kWide && which == 1) {
+    if (kSpread && which == 1) {
+      convert(false, true);
+    } else if (kWide && which == 1) {
       // ---- the tiles' products added up, f32 -------------------------------------------------
       const int r = threadIdx.x & 127;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -664,9 +793,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t sums = tmem + lanes + 256 + which * 128;
       for (int j = 0; ok && j < tiles; ++j) {
-        const int own = kWide ? j & 1 : which;  // S, its barriers
+        const int own = kWide || kSpread ? j & 1 : which;  // S, its barriers
         const uint32_t scores = tmem + lanes + own * 128;
-        ok = mbar_wait_warp(&bars->scores[own], kWide ? j >> 1 & 1 : j & 1, abort_flag) &&
+        ok = mbar_wait_warp(&bars->scores[own], kWide || kSpread ? j >> 1 & 1 : j & 1, abort_flag) &&
              mbar_wait_warp(&bars->meta[j % kMetaStages], j / kMetaStages & 1, abort_flag);
         if (!ok) break;
         __syncwarp();
@@ -679,8 +808,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
           for (int g = 0; g < kGroups; ++g) open = open && tile_meta.present[g] != 0;
         }
         float* const keep_to = keep + j % kKeepStages * kRowTile + r;
+        // (S of this tile came after the products of the one before the last: of the last one there is this)
+        const auto before_o = [&]() {
+          if (kSpread) {
+            ok = mbar_wait_warp(&bars->sums[(j - 1) & 1], (j - 1) >> 1 & 1, abort_flag) && ok;
+            tc_fence_after_sync();
+          }
+        };
         if (__all_sync(0xFFFFFFFFu, open)) {
-          softmax_tile<DP, kUnit, kOpen, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+          softmax_tile<DP, kUnit, kOpen, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[kSpread ? own : which], keep_to, before_o);
         } else {
           bool plain = true;
 #pragma unroll 1
@@ -690,9 +826,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
             plain = plain && factor > 0.0f && factor < INFINITY && fabsf(scales.y) < INFINITY;
           }
           if (__all_sync(0xFFFFFFFFu, plain)) {
-            softmax_tile<DP, kUnit, kHidden, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+            softmax_tile<DP, kUnit, kHidden, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[kSpread ? own : which], keep_to, before_o);
           } else {
-            softmax_tile<DP, kUnit, kSpecial, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[which], keep_to);
+            softmax_tile<DP, kUnit, kSpecial, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[kSpread ? own : which], keep_to, before_o);
           }
         }
         tc_fence_before_sync();
@@ -700,7 +836,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         if (lane == 0) mbar_arrive(&bars->weights[own]);
         if (kWide && lane == 0) mbar_arrive(&bars->kept[j % kKeepStages]);
       }
-      if (!kWide && ok && tiles > 0) ok = mbar_wait_warp(&bars->sums[which], 0, abort_flag);
+      if (!kWide && ok && tiles > 0) {
+        ok = mbar_wait_warp(&bars->sums[kSpread ? (tiles - 1) & 1 : which], kSpread ? (tiles - 1) >> 1 & 1 : 0, abort_flag);
+      }
       if (ok) {
         tc_fence_after_sync();
         const bool whole = splits_used(p, rows) == 1;
@@ -741,108 +879,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       }
     }
   } else if (warp < 8 + kConvertWarps) {
-    // ---- codes to operands ------------------------------------------------------------------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-    const int w = warp - 8;
-    const int32_t* const table = p.batch.table + s * p.batch.table_stride;
-    constexpr int kHalves = DP / 64;     // 64 codes of a row: one swizzled row of f16
-    constexpr int kLoads = 4 * kHalves;  // per thread and tile: 32 keys per warp, eight at a time
-    uint4 codes[kLoads];  // of one operand: the next to be stored
-    // ids of the blocks of this warp's two groups of 16 keys; -1: nothing there
-    const auto ids_of = [&](int j, int (&id)[2]) {
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int key = begin + j * kKeys + 32 * w + 16 * g;
-        id[g] = -1;
-        if (j < tiles && key < end) {
-          const int block = table[key >> p.block_shift];
-          if (block >= 0 && block < p.batch.blocks) id[g] = block;
-          else if (lane == 0) report_error(p.batch.error, kErrorBlock);
-        }
-      }
-    };
-    const auto load = [&](int j, const int (&id)[2], const int8_t* plane) {
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int slot = (begin + j * kKeys + 32 * w + 16 * g) & (p.block_tokens - 1);
-        const int8_t* const from =
-            plane + ((static_cast<long long>(max(id[g], 0)) * p.kv_heads + head) * p.block_tokens + slot) * p.dim;
-#pragma unroll
-        for (int i = 0; i < kLoads / 2; ++i) {
-          const int r = i / kHalves * 8 + (lane >> 2), d = i % kHalves * 64 + (lane & 3) * 16;
-          uint4 c = make_uint4(0, 0, 0, 0);  // (nothing there, or past the head: zeros)
-          if (id[g] >= 0 && (DP == p.dim || d < p.dim)) c = __ldg(reinterpret_cast<const uint4*>(from + r * p.dim + d));
-          codes[g * kLoads / 2 + i] = c;
-        }
-      }
-    };
-    const auto store = [&](uint8_t* operand) {
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-#pragma unroll
-        for (int i = 0; i < kLoads / 2; ++i) {
-          const int r = 32 * w + 16 * g + i / kHalves * 8 + (lane >> 2), c = (lane & 3) * 2;
-          uint8_t* const row = operand + i % kHalves * (kKeys * 128) + r * 128;
-          uint4 a, b;
-          convert16(codes[g * kLoads / 2 + i], &a, &b);
-          *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = a;
-          *reinterpret_cast<uint4*>(row + (((c + 1) ^ (r & 7)) << 4)) = b;
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-    };
-    float scales[2] = {0.0f, 0.0f};  // of lane 0, 1: its group's
-    const auto load_scales = [&](const int (&id)[2]) {
-      const int own = lane == 1 ? id[1] : id[0];
-      if (lane < 2 && own >= 0) {
-        const long long slice = static_cast<long long>(own) * p.kv_heads + head;
-        scales[0] = p.k_scales[slice];
-        scales[1] = p.v_scales[slice];
-      }
-    };
-    int id[2], next[2];
-    ids_of(0, id);
-    load(0, id, p.k_codes);
-    load_scales(id);
-    ids_of(1, next);
-    for (int j = 0; ok && j < tiles; ++j) {
-      const int stage = j & 1;
-      if (j >= 2) ok = mbar_wait_warp(&bars->key_empty[stage], ((j >> 1) - 1) & 1, abort_flag);
-      if (!ok) break;
-      if (lane < 2) {
-        const float vs = scales[1];
-        const float log = vs < kLeastScale ? kLeastLog : log2f(vs);  // (no number stays none)
-        Meta& m = meta[j % kMetaStages];
-        m.scales[2 * w + lane] = make_float2(scales[0], log);
-        // (of the scale itself: so the rounding of its logarithm, 2^-19 of a scale of 2^-64, is the weight's as much as
-        // the value's, and divided out; a whole number and the rest apart would keep it from the weights too, but take the
-        // f32 kernel 41.6 in place of 40.8 us, two f32 prompts of up to 4096 760 in place of 737)
-        m.value_inverse[2 * w + lane] = vs < kLeastScale ? exp2f(-kLeastLog) : 1.0f / vs;
-        m.present[2 * w + lane] = (lane == 1 ? id[1] : id[0]) >= 0;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->meta[j % kMetaStages]);
-      store(smem + S::kKeyRing + stage * S::kOperand);
-      if (lane == 0) mbar_arrive(&bars->key_full[stage]);
-      // (a scale of zero makes zeros of any codes; it has no logarithm, so the codes stand for it)
-      const int value_id[2] = {__shfl_sync(0xFFFFFFFFu, scales[1], 0) < kLeastScale ? -1 : id[0],
-                               __shfl_sync(0xFFFFFFFFu, scales[1], 1) < kLeastScale ? -1 : id[1]};
-      load(j, value_id, p.v_codes);
-      if (j + 1 < tiles) load_scales(next);
-      if (j >= 2) ok = mbar_wait_warp(&bars->value_empty[stage], ((j >> 1) - 1) & 1, abort_flag);
-      if (!ok) break;
-      store(smem + S::kValueRing + stage * S::kOperand);
-      if (lane == 0) mbar_arrive(&bars->value_full[stage]);
-      if (j + 1 < tiles) load(j + 1, next, p.k_codes);
-      id[0] = next[0];
-      id[1] = next[1];
-      ids_of(j + 2, next);
-    }
-    if (!ok) {
-      *abort_flag = 1;
-      report_error(p.batch.error, 42);
-    }
+    convert(true, !kSpread);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     if (warp == 12 && elect_one()) {
@@ -857,11 +895,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
 #pragma unroll
         for (int d = 0; d < DP; d += 16) {
           const uint32_t at = d / 64 * (kRowTile * 128) + d % 64 * 2;
-          mma_f16_ss(tmem + (kWide ? stage : which) * 128, make_sw128_kmajor_desc(base + S::kQueries + (which + half) * S::kOperand + at),
+          mma_f16_ss(tmem + (kWide || kSpread ? stage : which) * 128, make_sw128_kmajor_desc(base + S::kQueries + (which + half) * S::kOperand + at),
                      make_sw128_kmajor_desc(base + S::kKeyRing + stage * S::kOperand + at), scores_desc, d > 0 || (kWide && half == 0));
         }
       }
-      tc_commit(&bars->scores[kWide ? stage : which]);
+      tc_commit(&bars->scores[kWide || kSpread ? stage : which]);
     };
     for (int i = 0; ok && i < row_tiles; ++i) ok = mbar_wait(&bars->queries[i], 0, abort_flag);
     if (ok && tiles > 0) ok = mbar_wait(&bars->key_full[0], 0, abort_flag);
@@ -870,7 +908,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       for (int i = 0; i < row_tiles; ++i) scores_of(i, 0);
       tc_commit(&bars->key_empty[0]);
     }
-    if (kWide && ok && tiles > 1) {  // S of a tile ahead
+    if ((kWide || kSpread) && ok && tiles > 1) {  // S of a tile ahead
       ok = mbar_wait(&bars->key_full[1], 0, abort_flag);
       if (ok) {
         tc_fence_after_sync();
@@ -886,7 +924,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
           if (ok && j >= 2) ok = mbar_wait(&bars->taken[j & 1], (j >> 1) - 1 & 1, abort_flag);
           ok = ok && mbar_wait(&bars->weights[j & 1], j >> 1 & 1, abort_flag);
         } else {
-          ok = ok && mbar_wait(&bars->halves[i], j & 1, abort_flag);
+          ok = ok && mbar_wait(&bars->halves[kSpread ? stage : i], kSpread ? j >> 1 & 1 : j & 1, abort_flag);
         }
         if (!ok) break;
         tc_fence_after_sync();
@@ -895,11 +933,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
 #pragma unroll
           for (int t = 0; t < kKeys; t += 16) {
             if (!kWide && t == kKeys / 2) {
-              ok = mbar_wait(&bars->weights[i], j & 1, abort_flag);
+              ok = mbar_wait(&bars->weights[kSpread ? stage : i], kSpread ? j >> 1 & 1 : j & 1, abort_flag);
               if (!ok) break;
               tc_fence_after_sync();
             }
-            mma_f16_ts(tmem + 256 + (kWide ? j & 1 : i) * 128, tmem + (kWide ? j & 1 : i) * 128 + half * (kKeys / 2) + t / 2,
+            mma_f16_ts(tmem + 256 + (kWide ? j & 1 : i) * 128, tmem + (kWide || kSpread ? j & 1 : i) * 128 + half * (kKeys / 2) + t / 2,
                        make_sw128_nmajor_desc(base + S::kValueRing + stage * S::kOperand + t * 128, kKeys * 128), sums_desc,
                        t > 0 || (kWide ? half == 0 : j > 0));
           }
@@ -907,6 +945,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         if (!ok) break;
         if (kWide) {
           tc_commit(&bars->sums[j & 1]);
+          continue;
+        }
+        if (kSpread) {
+          tc_commit(&bars->sums[stage]);
           continue;
         }
         if (j + 1 == tiles) {
@@ -920,7 +962,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       }
       if (!ok) break;
       tc_commit(&bars->value_empty[stage]);
-      if (kWide) {
+      if (kWide || kSpread) {
         if (j + 2 >= tiles) continue;
         ok = mbar_wait(&bars->key_full[stage], (j + 2) >> 1 & 1, abort_flag);
         if (!ok) break;
@@ -950,23 +992,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   }
 }
 
-template <int DP, int kUnit, bool kWide, bool kTree>
+template <int DP, int kUnit, bool kWide, bool kTree, bool kSpread>
 qx_status launch_prompt_of(const AttentionParams& p, long long grid, cudaStream_t stream) {
   static SmemOptIn opt_in;
-  QX_TRY(opt_in.ensure(prompt_kernel<DP, kUnit, kWide, kTree>, TcShape<DP>::kBytes));
-  return launch_behind(prompt_kernel<DP, kUnit, kWide, kTree>, grid, kTcThreads, TcShape<DP>::kBytes, stream, p);
+  QX_TRY(opt_in.ensure(prompt_kernel<DP, kUnit, kWide, kTree, kSpread>, TcShape<DP>::kBytes));
+  return launch_behind(prompt_kernel<DP, kUnit, kWide, kTree, kSpread>, grid, kTcThreads, TcShape<DP>::kBytes, stream, p);
 }
-template <bool kWide, bool kTree>
+template <bool kWide, bool kTree, bool kSpread = false>
 qx_status launch_prompt_sized(const AttentionParams& p, long long grid, cudaStream_t stream) {
   if (p.block_tokens < 32) {
-    return p.dim <= 64 ? launch_prompt_of<64, 16, kWide, kTree>(p, grid, stream) : launch_prompt_of<128, 16, kWide, kTree>(p, grid, stream);
+    return p.dim <= 64 ? launch_prompt_of<64, 16, kWide, kTree, kSpread>(p, grid, stream) : launch_prompt_of<128, 16, kWide, kTree, kSpread>(p, grid, stream);
   }
-  return p.dim <= 64 ? launch_prompt_of<64, 32, kWide, kTree>(p, grid, stream) : launch_prompt_of<128, 32, kWide, kTree>(p, grid, stream);
+  return p.dim <= 64 ? launch_prompt_of<64, 32, kWide, kTree, kSpread>(p, grid, stream) : launch_prompt_of<128, 32, kWide, kTree, kSpread>(p, grid, stream);
 }
 
 }  // namespace
 
-qx_status launch_prompt(const AttentionParams& p, bool wide, long long grid, cudaStream_t stream) {
+qx_status launch_prompt(const AttentionParams& p, bool wide, bool spread, long long grid, cudaStream_t stream) {
+  if (spread) return launch_prompt_sized<false, true, true>(p, grid, stream);
   if (p.tree != nullptr) return wide ? launch_prompt_sized<true, true>(p, grid, stream) : launch_prompt_sized<false, true>(p, grid, stream);
   return wide ? launch_prompt_sized<true, false>(p, grid, stream) : launch_prompt_sized<false, false>(p, grid, stream);
 }
