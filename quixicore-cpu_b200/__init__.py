@@ -921,21 +921,26 @@ class Norm:
 
     def __init__(self, weight=None, bias=None, kind=NORM_RMS, eps=1e-6, offset=0.0, storage=None):
         self.arrays = (weight, bias)
-        self.dim = self.device = None
-        addresses, kinds = [], set()
-        for a in self.arrays:
-            if a is None:
-                addresses.append(None)
-                continue
-            host = isinstance(a, np.ndarray)
-            device = -1 if host else a.get_device()
-            assert len(a.shape) == 1 and self.dim in (None, a.shape[0]) and self.device in (None, device), "need weight [dim], bias [dim]"
-            assert (a.flags["C_CONTIGUOUS"] if host else device >= 0 and a.is_contiguous()), "need contiguous arrays"
-            self.dim, self.device = a.shape[0], device
-            addresses.append(a.ctypes.data if host else a.data_ptr())
-            kinds.add(_numpy_kind(a, storage) if host else (_torch_types or _fill_torch_types())[a.dtype])
-        assert len(kinds) < 2, "weight and bias have the same type"
-        self.view = NormView(kind, kinds.pop() if kinds else F32, *addresses, eps, offset)
+        at, shift, self.dim, self.device, storage_type = None, None, None, None, F32
+        if weight is not None:
+            at, storage_type, self.dim, self.device = _norm_array(weight, storage)
+        if bias is not None:
+            shift, *same = _norm_array(bias, storage)
+            assert weight is None or same == [storage_type, self.dim, self.device], "weight and bias have one size, type and device"
+            storage_type, self.dim, self.device = same
+        self.view = NormView(kind, storage_type, at, shift, eps, offset)
+
+
+def _norm_array(a, storage):
+    """Address, storage type, length and device (-1: the host) of a norm's weight or bias."""
+    assert len(a.shape) == 1, "need weight [dim], bias [dim]"
+    dim = a.shape[0]
+    if isinstance(a, np.ndarray):
+        assert a.flags["C_CONTIGUOUS"], "need contiguous arrays"
+        return a.ctypes.data, _numpy_kind(a, storage), dim, -1
+    device = a.get_device()
+    assert device >= 0 and a.is_contiguous(), "need contiguous arrays, tensors on the device"
+    return a.data_ptr(), (_torch_types or _fill_torch_types())[a.dtype], dim, device
 
 
 def _numpy_kind(a, storage) -> int:
@@ -951,12 +956,12 @@ def _row_view(t, tokens, dim, device, storage=None, one=False) -> RowsView:
     if t is None:
         return None
     rows, elements = t.shape
-    if isinstance(t, np.ndarray):
-        assert device == -1, "need a tensor on the current device"
-        kind, data, (stride, step) = _numpy_kind(t, storage), t.ctypes.data, (s // t.itemsize for s in t.strides)
-    else:
-        assert t.get_device() == device >= 0, "need tensors on the current device, or numpy arrays"
+    if device >= 0:
+        assert not isinstance(t, np.ndarray) and t.get_device() == device, "need a tensor on the current device"
         kind, data, (stride, step) = (_torch_types or _fill_torch_types())[t.dtype], t.data_ptr(), t.stride()
+    else:
+        assert isinstance(t, np.ndarray), "need tensors on the current device, or numpy arrays"
+        kind, data, (stride, step) = _numpy_kind(t, storage), t.ctypes.data, (s // t.itemsize for s in t.strides)
     assert elements == dim and (step == 1 or dim == 1), "need [tokens, dim] with the elements of a row side by side"
     if one and rows == 1:
         return RowsView(data, kind, 0)
@@ -966,12 +971,16 @@ def _row_view(t, tokens, dim, device, storage=None, one=False) -> RowsView:
 
 def _residual_norm(device, residual, block, joined, normed, pre, post, gate, scale, storage=None):
     tokens, dim = (block if residual is None else residual).shape
-    for norm in (pre, post):
-        assert norm is None or (norm.dim in (None, dim) and norm.device in (None, device)), "norms of another size or device"
-    return (_row_view(residual, tokens, dim, device, storage), _row_view(block, tokens, dim, device, storage),
-            None if post is None else post.view, _row_view(gate, tokens, dim, device, storage, True), scale,
-            _row_view(joined, tokens, dim, device, storage), None if pre is None else pre.view,
-            _row_view(normed, tokens, dim, device, storage), tokens, dim)
+    before = after = None
+    if post is not None:
+        assert post.dim in (None, dim) and post.device in (None, device), "a norm of another size or device"
+        before = post.view
+    if pre is not None:
+        assert pre.dim in (None, dim) and pre.device in (None, device), "a norm of another size or device"
+        after = pre.view
+    return (_row_view(residual, tokens, dim, device, storage), _row_view(block, tokens, dim, device, storage), before,
+            _row_view(gate, tokens, dim, device, storage, True), scale, _row_view(joined, tokens, dim, device, storage),
+            after, _row_view(normed, tokens, dim, device, storage), tokens, dim)
 
 
 def residual_norm(residual, block, joined, normed=None, pre=None, post=None, gate=None, scale=1.0, storage=None) -> int:

@@ -61,13 +61,15 @@ struct InVectors {
     if (d < dim) store8_typed<kType>(y.data, row * y.stride + d, v);
   }
 };
+template <int kOfType>  // -1: each operand has its own
 struct InElements {
   static constexpr bool kEach = true;
   uint32_t w[8];
   static __device__ __forceinline__ int place(int i, int e) { return static_cast<int>(threadIdx.x) + (8 * i + e) * static_cast<int>(blockDim.x); }
+  static __device__ __forceinline__ int type_of(const View& x) { return kOfType < 0 ? x.type : kOfType; }
   __device__ __forceinline__ void load(const View& x, long long row, int dim, int i) {
     const long long at = row * x.stride;
-    if (x.type == QX_STORAGE_F32) {
+    if (type_of(x) == QX_STORAGE_F32) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = place(i, e) < dim ? reinterpret_cast<const uint32_t*>(x.data)[at + place(i, e)] : 0;
     } else {
@@ -78,15 +80,15 @@ struct InElements {
   __device__ __forceinline__ void values(const View& x, float (&v)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[e] = x.type == QX_STORAGE_F32   ? __uint_as_float(w[e])
-             : x.type == QX_STORAGE_F16 ? __half2float(__ushort_as_half(static_cast<uint16_t>(w[e])))
-                                        : __uint_as_float(w[e] << 16);
+      v[e] = type_of(x) == QX_STORAGE_F32   ? __uint_as_float(w[e])
+             : type_of(x) == QX_STORAGE_F16 ? __half2float(__ushort_as_half(static_cast<uint16_t>(w[e])))
+                                            : __uint_as_float(w[e] << 16);
     }
   }
   static __device__ __forceinline__ void store(const View& y, long long row, int dim, int i, const float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (place(i, e) < dim) store_one(y.data, y.type, row * y.stride + place(i, e), v[e]);
+      if (place(i, e) < dim) store_one(y.data, type_of(y), row * y.stride + place(i, e), v[e]);
     }
   }
 };
@@ -160,9 +162,11 @@ __device__ __forceinline__ void normalise(const NormParams& n, float inverse_dim
   }
 }
 
-// `Stream`: how residual and joined are read and written; `Block`: block, gate and normed.
+// `Stream`: how residual and joined are read and written; `Block`: block, gate and normed. Two CTAs of 512 threads an SM
+// where 64 registers hold a thread's operands (1500 f32 rows of 1153 in single elements: 12.9 us; a CTA less to 14.1, 42
+// registers, which spill, to 19.0).
 template <int kVectors, class Stream, class Block, class Weight>
-__global__ void __launch_bounds__(kNormThreads, kVectors == 2 && !Stream::kEach ? 2 : 1) residual_norm_kernel(const __grid_constant__ JoinParams p) {
+__global__ void __launch_bounds__(kNormThreads, kVectors == 1 || (kVectors == 2 && !Stream::kEach) ? 2 : 1) residual_norm_kernel(const __grid_constant__ JoinParams p) {
   __shared__ float sums[kSums][kRowWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
@@ -278,22 +282,28 @@ NormParams device_norm(const qx_norm* norm) {
           norm->eps, norm->offset};
 }
 
-// The type of those operands that there are; -1: they differ, or are no whole vectors.
-int common_type(const JoinParams& p, std::initializer_list<const View*> views) {
+// The type of those operands that there are; -1: they differ, -2: there is none.
+int common_type(std::initializer_list<const View*> views) {
   int type = -2;
   for (const View* view : views) {
     if (view->data == nullptr) continue;
-    if (!view->vector || p.dim % 8 != 0 || (type >= 0 && view->type != type)) return -1;
+    if (type >= 0 && view->type != type) return -1;
     type = view->type;
   }
   return type;
+}
+bool all_vectors(std::initializer_list<const View*> views) {
+  for (const View* view : views) {
+    if (view->data != nullptr && !view->vector) return false;
+  }
+  return true;
 }
 
 template <class Stream, class Block, class Weight>
 qx_status launch(const JoinParams& p, cudaStream_t stream) {
   // Two vectors a thread: on 64 registers they keep more bytes under way than one or four do (8192 rows of 4096 bf16
   // elements with 1 | 2 | 4 | 8: 52.4 | 46.9 | 56.1 | 87.8 us; one row 2.1 | 2.3 | 3.2 | 8.1). Single elements take eight
-  // a thread as long as they can (1500 f32 rows of 1153, with 1 | 2 | 4 times eight: 15.5 | 25.4 | 44.1).
+  // a thread as long as they can (1500 f32 rows of 1153, with 1 | 2 | 4 times eight: 12.9 | 17.9 | 39.0).
   const int vectors = (p.dim + 7) / 8;
   int each = vectors <= 32 || Stream::kEach ? 1 : 2;
   while (each * kNormThreads < vectors) each *= 2;
@@ -316,6 +326,11 @@ qx_status launch_typed(const JoinParams& p, int weight, cudaStream_t stream) {
   return launch<InVectors<kStream>, InVectors<kBlock>, InVectors<kBlock>>(p, stream);
 }
 
+template <int kOfType>
+qx_status launch_elements(const JoinParams& p, cudaStream_t stream) {
+  return launch<InElements<kOfType>, InElements<kOfType>, InElements<kOfType>>(p, stream);
+}
+
 qx_status launch_residual_norm(const qx_rows* residual, const qx_rows* block, const qx_norm* post, const qx_rows* gate,
                                float scale, const qx_rows* joined, const qx_norm* pre, const qx_rows* normed,
                                long long tokens, int dim, cudaStream_t stream) {
@@ -333,13 +348,15 @@ qx_status launch_residual_norm(const qx_rows* residual, const qx_rows* block, co
   p.tokens = tokens;
   p.dim = dim;
   // Types that go together: the stream's own or f32, the blocks' own, weights of the blocks' type or f32.
-  int s = common_type(p, {&p.residual, &p.joined}), b = common_type(p, {&p.block, &p.gate, &p.normed});
-  int w = common_type(p, {&p.post.weight, &p.post.bias, &p.pre.weight, &p.pre.bias});
+  constexpr int kF32 = QX_STORAGE_F32, kF16 = QX_STORAGE_F16, kBf16 = QX_STORAGE_BF16;
+  int s = common_type({&p.residual, &p.joined}), b = common_type({&p.block, &p.gate, &p.normed});
+  int w = common_type({&p.post.weight, &p.post.bias, &p.pre.weight, &p.pre.bias});
   if (b == -2) b = s;
   if (s == -2) s = b;
   if (w == -2) w = b;
-  if (s >= 0 && b >= 0 && (s == b || s == QX_STORAGE_F32) && (w == b || w == QX_STORAGE_F32)) {
-    constexpr int kF32 = QX_STORAGE_F32, kF16 = QX_STORAGE_F16, kBf16 = QX_STORAGE_BF16;
+  const bool vectors = p.dim % 8 == 0 && all_vectors({&p.residual, &p.joined, &p.block, &p.gate, &p.normed, &p.post.weight,
+                                                      &p.post.bias, &p.pre.weight, &p.pre.bias});
+  if (vectors && s >= 0 && b >= 0 && (s == b || s == kF32) && (w == b || w == kF32)) {
     if (b == kF32) return launch_typed<kF32, kF32>(p, w, stream);
     if (b == kF16) {
       return s == kF16 ? launch_typed<kF16, kF16>(p, w, stream)
@@ -348,7 +365,14 @@ qx_status launch_residual_norm(const qx_rows* residual, const qx_rows* block, co
     return s == kBf16 ? launch_typed<kBf16, kBf16>(p, w, stream)
                       : launch_typed<kF32, kBf16>(p, w, stream);
   }
-  return launch<InElements, InElements, InElements>(p, stream);
+  // One type for all saves the kernel its choices at every element (1500 f32 rows of 1153, both norms:
+  // 12.9 us, with them 17.5).
+  if (s == b && w == b) {
+    if (b == kF32) return launch_elements<kF32>(p, stream);
+    if (b == kF16) return launch_elements<kF16>(p, stream);
+    if (b == kBf16) return launch_elements<kBf16>(p, stream);
+  }
+  return launch_elements<-1>(p, stream);
 }
 
 }  // namespace
