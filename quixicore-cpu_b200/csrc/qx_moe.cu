@@ -177,8 +177,8 @@ __device__ __forceinline__ T warp_sum(T v) {
   return v;
 }
 
-// A warp chooses a token's experts by their keys: logits, or scores and biases.
-__device__ __forceinline__ void choose(const Params& p, unsigned long long* keys, int token) {
+// A warp chooses a token's experts by their keys: logits, or scores and biases (`scores`: those alone).
+__device__ __forceinline__ void choose(const Params& p, unsigned long long* keys, float* scores, int token) {
   const int lane = threadIdx.x & 31, places = p.top + p.shared, each = (p.experts + 31) / 32;
   if (p.bias != nullptr && p.score == QX_MOE_SOFTMAX) {  // (scores need all logits)
     double largest = -INFINITY, total = 0.0;
@@ -188,8 +188,12 @@ __device__ __forceinline__ void choose(const Params& p, unsigned long long* keys
     for (int pass = 0; pass < 2; ++pass) {
       for (int e = lane; e < p.experts; e += 32) {
         const double score = exp(from_ordered(keys[e]) - largest);
-        if (pass == 0) total += score;
-        else keys[e] = ordered(score / total + static_cast<double>(p.bias[e]));
+        if (pass == 0) {
+          total += score;
+        } else {
+          scores[e] = static_cast<float>(score / total);
+          keys[e] = ordered(score / total + static_cast<double>(p.bias[e]));
+        }
       }
       if (pass == 0) total = warp_sum(total);
     }
@@ -227,9 +231,11 @@ __device__ __forceinline__ void choose(const Params& p, unsigned long long* keys
   const double key = from_ordered(mine), largest = __shfl_sync(0xFFFFFFFFu, key, 0);
   float score = 0.0f, total = 1.0f;
   if (p.bias != nullptr) {
-    if (takes) score = static_cast<float>(key - static_cast<double>(p.bias[expert]));
+    if (takes) score = scores[expert];
   } else if (p.score == QX_MOE_SIGMOID) {
-    if (takes) score = 1.0f / (1.0f + expf(static_cast<float>(-key)));
+    // (far below zero sigmoid(l) is e^l, whose quotients do not run out of f32)
+    const bool far = p.normalise && largest < -80.0;
+    if (takes) score = far ? expf(static_cast<float>(key - largest)) : 1.0f / (1.0f + expf(static_cast<float>(-key)));
   } else {
     if (takes) score = expf(static_cast<float>(key - largest));
     if (!p.normalise) {
@@ -325,8 +331,8 @@ __device__ __forceinline__ void sum_logits(const Params& p, int token0, int expe
     }
   }
 }
-// Shared memory: a cluster's first CTA holds the keys of eight tokens, behind the parts of sums.
-constexpr int kPartBytes = kRouterWarps * kRouterExperts * kRouterTokens * 8;
+// Shared memory: a cluster's first CTA holds the keys and scores of eight tokens, behind the parts of sums.
+constexpr int kPartBytes = kRouterWarps * kRouterExperts * kRouterTokens * 8, kKeyBytes = 8 + 4;
 
 // Grid: a cluster for every eight tokens, then those that convert activations. kX, kW: types of activations and router.
 template <int kX, int kW>
@@ -334,8 +340,11 @@ __global__ void __launch_bounds__(kRouterThreads, 1) moe_router_kernel(const __g
   extern __shared__ __align__(128) uint8_t smem[];
   auto& parts = *reinterpret_cast<double(*)[kRouterWarps][kRouterExperts][kRouterTokens]>(smem);
   unsigned long long* const keys = reinterpret_cast<unsigned long long*>(smem + kPartBytes);  // [token][expert]
+  float* const scores = reinterpret_cast<float*>(keys + kRouterTokens * p.experts);
   asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;");  // (its CTAs run: their shared memory may be written)
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;");
   uint32_t rank, size;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
@@ -366,8 +375,13 @@ __global__ void __launch_bounds__(kRouterThreads, 1) moe_router_kernel(const __g
 #pragma unroll
       for (int i = 0; i < kRouterWarps; ++i) v[i & 3] += parts[i][e][t];
       double key = (v[0] + v[1]) + (v[2] + v[3]);
-      if (p.bias != nullptr && p.score == QX_MOE_SIGMOID) key = 1.0 / (1.0 + exp(-key)) + static_cast<double>(p.bias[expert0 + e]);
       uint32_t to;
+      if (p.bias != nullptr && p.score == QX_MOE_SIGMOID) {
+        const double score = 1.0 / (1.0 + exp(-key));
+        key = score + static_cast<double>(p.bias[expert0 + e]);
+        asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(scores + t * p.experts + expert0 + e)));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(static_cast<float>(score)) : "memory");
+      }
       asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(keys + t * p.experts + expert0 + e)));
       asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(ordered(key)) : "memory");
     }
@@ -375,7 +389,7 @@ __global__ void __launch_bounds__(kRouterThreads, 1) moe_router_kernel(const __g
   }
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (rank == 0 && warp < kRouterTokens && token0 + warp < p.tokens) choose(p, keys + warp * p.experts, token0 + warp);
+  if (rank == 0 && warp < kRouterTokens && token0 + warp < p.tokens) choose(p, keys + warp * p.experts, scores + warp * p.experts, token0 + warp);
 }
 
 // ---- experts -----------------------------------------------------------------------------------
@@ -777,7 +791,8 @@ __global__ void __launch_bounds__(kExpertThreads, 2) moe_experts_kernel(const __
         if (scales_from >= 0 && lane % kScaleLanes * 4 < in_stage) {
           copy16(to + S::kScales + lane / kScaleLanes * S::kScaleBytes + lane % kScaleLanes * 16, scales + scales_from + first);
         }
-        arrive_behind_copies(full + ring.slot);
+        if (kind == kCombine) mbar_arrive(full + ring.slot);  // (no copies: hands on what the wait has seen)
+        else arrive_behind_copies(full + ring.slot);
         ring.advance(kStages);
         first += S::kBlocks;
         if (first >= blocks) break;
@@ -1009,14 +1024,12 @@ qx_status prepare(int format, const uint8_t* gate, const uint8_t* up, const uint
   return QX_STATUS_OK;
 }
 
-bool on_boundary_of(const void* data, int type) { return reinterpret_cast<uintptr_t>(data) % kv::type_bytes(type) == 0; }
-
 qx_status check_apply(const qx_moe* m, const qx_moe_router* router, const qx_rows* x, const qx_rows* out, long long tokens,
                       int activation, const int32_t* chosen, const float* weights) {
   if (m == nullptr || router == nullptr || x == nullptr || out == nullptr || tokens < 0) return QX_STATUS_INVALID_ARGUMENT;
   if (!kv::known_type(router->type)) return QX_STATUS_UNSUPPORTED_FORMAT;
   if (router->top < 1 || router->top > std::min(kMostTop, m->experts)) return QX_STATUS_INVALID_SHAPE;
-  if (router->weights == nullptr || !on_boundary_of(router->weights, router->type) || !kv::on_boundary(router->bias) ||
+  if (router->weights == nullptr || reinterpret_cast<uintptr_t>(router->weights) % kv::type_bytes(router->type) != 0 || !kv::on_boundary(router->bias) ||
       (router->score != QX_MOE_SOFTMAX && router->score != QX_MOE_SIGMOID) || !std::isfinite(router->scale) ||
       activation < QX_ACTIVATION_NONE || activation > QX_ACTIVATION_RELU2 || !kv::on_boundary(chosen) || !kv::on_boundary(weights)) {
     return QX_STATUS_INVALID_ARGUMENT;
@@ -1042,14 +1055,14 @@ struct Layout {
 template <int kX, int kW>
 qx_status launch_router(const Params& p, cudaStream_t stream) {
   static SmemOptIn opt_in;
-  QX_TRY(opt_in.ensure(moe_router_kernel<kX, kW>, kPartBytes + kRouterTokens * kMostExperts * 8));
+  QX_TRY(opt_in.ensure(moe_router_kernel<kX, kW>, kPartBytes + kRouterTokens * kMostExperts * kKeyBytes));
   int size = 1;
   while (size < kRouterCluster && size * kRouterExperts < p.experts) size *= 2;
   const int convert = (p.tokens * ((p.dim + 127) / 128) + kRouterWarps - 1) / kRouterWarps;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(((p.tokens + kRouterTokens - 1) / kRouterTokens + (convert + size - 1) / size) * size);
   config.blockDim = dim3(kRouterThreads);
-  config.dynamicSmemBytes = kPartBytes + static_cast<size_t>(kRouterTokens) * p.experts * 8;
+  config.dynamicSmemBytes = kPartBytes + static_cast<size_t>(kRouterTokens) * p.experts * kKeyBytes;
   config.stream = stream;
   cudaLaunchAttribute attributes[2];
   attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1107,7 +1120,6 @@ qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_ro
   p.x_vector = whole(x->data, x->stride * x_size);
   p.x_stride = x->stride;
   p.out_type = out->type;
-  p.out_vector = whole(out->data, out->stride * out_size);
   p.out_stride = out->stride;
   p.activation = activation;
   p.digits = x->type == QX_STORAGE_F32 ? 3 : 2;

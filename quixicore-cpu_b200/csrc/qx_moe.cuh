@@ -56,7 +56,7 @@ struct Params {
   int x_type, x_vector;
   long long x_stride;
   uint8_t* out;
-  int out_type, out_vector;
+  int out_type;
   long long out_stride;
   int tokens, activation, digits;
   int32_t* chosen;       // [token][top], may be NULL

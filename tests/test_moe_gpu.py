@@ -260,3 +260,23 @@ def test_codes_of_every_value(qx):
             setattr(m, name, torch.from_numpy((values * d).reshape(1, 256, 256)))
         m.raw = tuple(b.reshape(-1) for b in blocks)
         check(qx, m, tokens_of(m, 3, torch.float32), 1)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_scores_far_below_their_bias(qx, sigmoid):
+    """Experts that are chosen for a large bias, with scores down to 1e-20: their weights are those of the scores."""
+    m = ref.layer(0, 12, 64, 32, seed=31)
+    m.router = m.router * 12
+    m.bias = torch.linspace(-40, 50, 12)
+    for normalise in (False, True):
+        check(qx, m, tokens_of(m, 9, torch.float32), 4, sigmoid=sigmoid, biased=True, normalise=normalise)
+
+
+def test_scores_that_all_lie_far_below_zero(qx):
+    """sigmoid(l) of about e^-150 runs out of f32; normalised weights are quotients of such."""
+    m = ref.layer(1, 6, 64, 32, seed=32)
+    x = tokens_of(m, 5, torch.float32)
+    x[:, 0] = 8.0
+    m.router[:, 0] = -20.0
+    assert float((x.double() @ m.router.double().T).max()) < -140
+    check(qx, m, x, 3, sigmoid=True)
