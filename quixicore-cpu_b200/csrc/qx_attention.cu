@@ -12,7 +12,12 @@ namespace {
 // rows 101 | 54; one of 16384 keys, 48 rows 42 | 41; f32, 4 of 4096 keys, 64 rows 84 | 87, 100 rows 96 | 90; 16 whole
 // texts of 64 tokens 25 | 29, of 100 tokens 40 | 32.
 constexpr long long kPromptFrom = 48, kPromptFromWide = 96;
-constexpr long long kSpreadUpTo = 128;
+// Trees whose rows fill one or three tiles of 128 take CTAs of one such tile, two softmax groups sharing its keys; of CTAs with
+// two tiles the last would have one to itself. One tile | two tiles a CTA, us, bf16 unless it says f16: 16 sequences of 64 rows, up
+// to 8192 keys 107 | 149; 384 rows, 131072 keys 273 | 306; 4 of 320 rows, 8192 keys 109 | 117; 8 of 384 rows, up to 4096 keys
+// 57 | 73; one of 384 f16 rows of 64 elements, 16384 keys 45 | 52. An even number: 6 of 189 f16 rows of 64 elements, 4096 keys
+// 58 | 44; 4 of 192 rows, 4096 keys 47 | 44. (Five and more tiles would convert each code five times.)
+constexpr long long kSpreadTiles = 3;
 
 // Joins the chunks of one row, in an order that their number fixes: the threads are cut into parts, a thread of part i
 // takes four head elements of chunks i, i + parts, ..., with several chunks' loads under way before it uses the first.
@@ -214,7 +219,8 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   const long long most_rows = static_cast<long long>(batch->max_tokens) * p.group;
   const bool wide = q->type == QX_STORAGE_F32;
   const bool prompt = cache->head_dim <= 128 && most_rows >= (wide ? kPromptFromWide : kPromptFrom);
-  const bool spread = prompt && tree != nullptr && !wide && most_rows <= kSpreadUpTo;
+  const long long spread_tiles = (most_rows + kPromptRowsSpread - 1) / kPromptRowsSpread;
+  const bool spread = prompt && tree != nullptr && !wide && spread_tiles <= kSpreadTiles && spread_tiles % 2 == 1;
   p.tile_rows = prompt ? (wide ? kPromptRowsWide : spread ? kPromptRowsSpread : kPromptRows) : most_rows <= 8 ? 8 : 16;
   p.shift = prompt ? kPromptShift : kShift;
   p.row_tiles = static_cast<int>((most_rows + p.tile_rows - 1) / p.tile_rows);

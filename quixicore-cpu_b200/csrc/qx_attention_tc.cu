@@ -52,6 +52,9 @@ using namespace sm100;
 constexpr int kRowTile = 128, kKeys = 128, kGroups = kKeys / 16;
 constexpr int kConvertWarps = 4, kTcThreads = 512;
 constexpr int kSoftmaxRegisters = 192, kOtherRegisters = 64;  // of 128 at launch: 256 * 192 + 256 * 64 = 512 * 128
+// (kSpread: a warpgroup more, of 96 registers at launch: 256 * 144 + 384 * 64 = 640 * 96)
+constexpr int kSpreadRegisters = 144;
+constexpr int threads_of(bool spread) { return spread ? kTcThreads + 32 * kConvertWarps : kTcThreads; }
 constexpr int kMetaStages = 4;
 static_assert(kPromptRows == 2 * kRowTile && kPromptRowsWide == kRowTile, "two tiles per CTA, f32: one");
 constexpr int kKeepStages = 4;
@@ -85,7 +88,7 @@ struct TcShape {
   static constexpr int kKeyRing = kQueries + 2 * kOperand;
   static constexpr int kValueRing = kKeyRing + 2 * kOperand;
   static constexpr int kMeta = kValueRing + 2 * kOperand;
-  static constexpr int kKeep = kMeta + kMetaStages * static_cast<int>(sizeof(Meta));  // kWide: [stage][row], [row]
+  static constexpr int kKeep = kMeta + kMetaStages * static_cast<int>(sizeof(Meta));  // kWide: [stage][row], [row]; kSpread: rows' ends, factors
   static constexpr int kBars = kKeep + (kKeepStages + 1) * kRowTile * 4;
   static constexpr int kBytes = kBars + static_cast<int>(sizeof(Barriers)) + 1024;  // (the operands start on 1024)
 };
@@ -180,12 +183,14 @@ struct RowState {
 // 46.5.)
 // kWide: the row's factor for what O holds so far goes to *keep_to instead.
 enum Mask { kOpen, kHidden, kSpecial };
-// `before`: kSpread, waits until the products that O holds so far are done (else they are, when S is there).
-template <int DP, int kUnit, Mask kMask, bool kWide, bool kTree, class Before>
-__device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, const Meta& meta, RowState& row, int key0,
+// kHalf: of a tile's keys, those from key0 on, whose groups begin with `group0`. `before_o` then waits until the products
+// that O holds so far are done (else they are, when S is there).
+template <int DP, int kUnit, Mask kMask, bool kWide, bool kTree, bool kHalf, class Before>
+__device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, const Meta& meta, int group0, RowState& row, int key0,
                                              bool first, uint64_t* first_half, float* keep_to, const Before& before_o) {
-  constexpr int kUnits = kKeys / kUnit, kPerUnit = kUnit / 16;
-  uint32_t s[4][32];
+  constexpr int kRuns = kHalf ? 2 : 4;  // of 32 keys
+  constexpr int kUnits = 32 * kRuns / kUnit, kPerUnit = kUnit / 16;
+  uint32_t s[kRuns][32];
   tmem_ld_32x32(scores, s[0]);
   tmem_ld_32x32(scores + 32, s[1]);
 
@@ -193,12 +198,12 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   float largest = row.largest_log;
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    const float2 scales = meta.scales[u * kPerUnit];
+    const float2 scales = meta.scales[group0 + u * kPerUnit];
     factor[u] = row.factor * scales.x;
     log[u] = scales.y;
-    relative[u] = meta.value_inverse[u * kPerUnit];
+    relative[u] = meta.value_inverse[group0 + u * kPerUnit];
     const int key = key0 + kUnit * u;
-    const bool seen = kMask == kOpen || (meta.present[u * kPerUnit] != 0 && key < row.high && key + kUnit > row.low &&
+    const bool seen = kMask == kOpen || (meta.present[group0 + u * kPerUnit] != 0 && key < row.high && key + kUnit > row.low &&
                                          (!kTree || seen_of<kUnit>(row.drafts, key, row.start, row.low) != 0));
     largest = fmaxf(largest, seen ? log[u] : -INFINITY);
   }
@@ -224,15 +229,15 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
     const int low = min(max(row.low - key0 - 32 * c, 0), 32), high = min(max(row.high - key0 - 32 * c, 0), 32);
     uint32_t seen = static_cast<uint32_t>((1ull << high) - 1) & ~static_cast<uint32_t>((1ull << low) - 1);
     if (kTree) seen &= seen_of<32>(row.drafts, key0 + 32 * c, row.start, row.low);
-    if (meta.present[2 * c] == 0) seen &= 0xFFFF0000u;
-    if (meta.present[2 * c + 1] == 0) seen &= 0xFFFFu;
+    if (meta.present[group0 + 2 * c] == 0) seen &= 0xFFFF0000u;
+    if (meta.present[group0 + 2 * c + 1] == 0) seen &= 0xFFFFu;
     if (__all_sync(0xFFFFFFFFu, seen == 0xFFFFFFFFu)) return;
 #pragma unroll
     for (int i = 0; i < 32; ++i) s[c][i] = (seen >> i & 1) != 0 ? s[c][i] : 0xFF800000u;
   };
   float top = -INFINITY;
   const auto top_of = [&](int u) {
-    const bool present = kMask != kSpecial || meta.present[u * kPerUnit] != 0;
+    const bool present = kMask != kSpecial || meta.present[group0 + u * kPerUnit] != 0;
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (four chains: one would wait for itself)
 #pragma unroll
     for (int i = 0; i < kUnit; i += 2) {
@@ -252,22 +257,26 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   };
   tmem_ld_wait_for(s[0]);
   tmem_ld_wait_for(s[1]);
-  tmem_ld_32x32(scores + 64, s[2]);
-  tmem_ld_32x32(scores + 96, s[3]);
+  if constexpr (!kHalf) {
+    tmem_ld_32x32(scores + 64, s[2]);
+    tmem_ld_32x32(scores + 96, s[3]);
+  }
   if (kMask == kHidden) {
     hide(0);
     hide(1);
   }
 #pragma unroll
-  for (int u = 0; u < kUnits / 2; ++u) top_of(u);
-  tmem_ld_wait_for(s[2]);
-  tmem_ld_wait_for(s[3]);
-  if (kMask == kHidden) {
-    hide(2);
-    hide(3);
-  }
+  for (int u = 0; u < 64 / kUnit; ++u) top_of(u);
+  if constexpr (!kHalf) {
+    tmem_ld_wait_for(s[2]);
+    tmem_ld_wait_for(s[3]);
+    if (kMask == kHidden) {
+      hide(2);
+      hide(3);
+    }
 #pragma unroll
-  for (int u = kUnits / 2; u < kUnits; ++u) top_of(u);
+    for (int u = 64 / kUnit; u < kUnits; ++u) top_of(u);
+  }
 
   const bool behind = top > row.maximum + kBehind;  // (from -infinity on, any score is)
   if (kWide) {
@@ -298,7 +307,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
   if (rise != 0.0f) row.sum *= exp2_fast(rise);
   const float base = (row.maximum == -INFINITY ? 0.0f : row.maximum) - kPromptShift;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < kRuns; ++c) {
     uint32_t p[16], low[16];
 #pragma unroll
     for (int h = 0; h < 32 / kUnit; ++h) {
@@ -306,7 +315,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
       const float add = log[u] - base;
       const unsigned long long f2 = tile::pack2(__float_as_uint(factor[u]), __float_as_uint(factor[u]));
       const unsigned long long c2 = tile::pack2(__float_as_uint(add), __float_as_uint(add));
-      const bool present = kMask != kSpecial || meta.present[u * kPerUnit] != 0;
+      const bool present = kMask != kSpecial || meta.present[group0 + u * kPerUnit] != 0;
       unsigned long long sum2 = 0;
 #pragma unroll
       for (int i = 0; i < kUnit; i += 2) {
@@ -336,7 +345,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t scores, uint32_t sums, con
     }
     tmem_st_32x16(scores + 16 * c, p);
     if (kWide) tmem_st_32x16(scores + kKeys / 2 + 16 * c, low);
-    if (!kWide && c == 1) {  // the product with the first half of the keys' values may begin
+    if (!kWide && !kHalf && c == 1) {  // the product with the first half of the keys' values may begin
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
@@ -440,10 +449,13 @@ __device__ __forceinline__ void write_row(const AttentionParams& p, const uint32
   }
 }
 
-// kSpread: one tile of 128 rows; warps 4-7 take the conversion of the values from warps 8-11, and S of the next tile of keys
-// is computed during a softmax, in the second row tile's place.
+// kSpread: one tile of 128 rows. Of each tile of keys warps 0-3 take the first half and warps 4-7 the second, each with a
+// maximum, a sum and an O of its own, which are joined at the end; S of the next tile is computed during a softmax, in the
+// second row tile's place. Warps 8-11 convert keys alone, warps 16-19 values. (16 trees of 64 bf16 rows over up to 8192 keys: 107
+// us, 3200 cycles a tile. One softmax group and values converted by the other: 123; the groups taking tiles by turns: 134; codes
+// two tiles ahead in registers or called into L2 ahead: 154, 123, as the warps of an SM partition then take one another's time.)
 template <int DP, int kUnit, bool kWide, bool kTree, bool kSpread>
-__global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(threads_of(kSpread), 1) prompt_kernel(const __grid_constant__ AttentionParams p) {
   using S = TcShape<DP>;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
@@ -627,11 +639,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
 
   if (warp < 8) {
     // ---- softmax --------------------------------------------------------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSpread ? kSpreadRegisters : kSoftmaxRegisters));
     const int which = warp >> 2;
-    if (kSpread && which == 1) {
-      convert(false, true);
-    } else if (kWide && which == 1) {
+    if (kWide && which == 1) {
       // ---- the tiles' products added up, f32 -------------------------------------------------
       const int r = threadIdx.x & 127;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -682,8 +692,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
         *abort_flag = 1;
         report_error(p.batch.error, 44);
       }
-    } else if (which < row_tiles) {
-      const int r = threadIdx.x & 127, in_tile = which * kRowTile + r;
+    } else if (kSpread || which < row_tiles) {
+      const int r = threadIdx.x & 127, in_tile = (kSpread ? 0 : which * kRowTile) + r;
       const bool real = in_tile < rows.count;
       const int start = rows.length - rows.n;
       const int token = (rows.first + in_tile) / p.group, member = (rows.first + in_tile) % p.group;
@@ -705,7 +715,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
       // rows as they are to where their operands go, runs of lanes to a row; then each thread converts its own row in
       // place (f32: the 16-byte pieces 2c and 2c + 1 lie where the high and the low halves of elements 8c .. 8c + 7
       // go). Loops, not straight code: what runs once per CTA waits for its instructions at every line.
-      {
+      if (kSpread && which == 1) {
+        ok = mbar_wait_warp(&bars->queries[0], 0, abort_flag);
+        row.factor = gains[r];
+      } else {
         constexpr int kElements = kWide ? 4 : 8, kBytes = kWide ? 4 : 2, kLanes = DP / kElements, kAtOnce = 32 / kLanes;
         const int piece = lane % kLanes, d = piece * kElements, warp_row = which * kRowTile + (warp & 3) * 32;
         uint8_t* const tile = smem + S::kQueries + which * S::kOperand;
@@ -782,30 +795,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
           *at = make_uint4(high[0], high[1], high[2], high[3]);
           if (kWide) *low_at = make_uint4(low[0], low[1], low[2], low[3]);
         }
+        if (kSpread) gains[r] = row.factor;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(&bars->queries[which]);
       }
       // below open_high and from open_low on no row of the tile has a hidden key
-      const int last = min(rows.count, (which + 1) * kRowTile) - 1;
-      const int position0 = start + (rows.first + which * kRowTile) / p.group, position1 = start + (rows.first + last) / p.group;
+      const int last = min(rows.count, in_tile - r + kRowTile) - 1;
+      const int position0 = start + (rows.first + in_tile - r) / p.group, position1 = start + (rows.first + last) / p.group;
       const int open_high = kTree ? start : p.causal ? min(rows.length, position0 + 1) : rows.length;
       const int open_low = first_seen(p, kTree ? start + rows.n - 1 : position1);
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t sums = tmem + lanes + 256 + which * 128;
       for (int j = 0; ok && j < tiles; ++j) {
         const int own = kWide || kSpread ? j & 1 : which;  // S, its barriers
-        const uint32_t scores = tmem + lanes + own * 128;
+        const uint32_t scores = tmem + lanes + own * 128 + (kSpread ? which * (kKeys / 2) : 0);
         ok = mbar_wait_warp(&bars->scores[own], kWide || kSpread ? j >> 1 & 1 : j & 1, abort_flag) &&
              mbar_wait_warp(&bars->meta[j % kMetaStages], j / kMetaStages & 1, abort_flag);
         if (!ok) break;
         __syncwarp();
         tc_fence_after_sync();
         const Meta& tile_meta = meta[j % kMetaStages];
-        const int key0 = begin + j * kKeys;
-        bool open = key0 + kKeys <= open_high && key0 >= open_low;
+        constexpr int kOwnGroups = kSpread ? kGroups / 2 : kGroups;
+        const int group0 = kSpread ? which * kOwnGroups : 0, key0 = begin + j * kKeys + 16 * group0;
+        bool open = key0 + 16 * kOwnGroups <= open_high && key0 >= open_low;
         if (open) {
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g) open = open && tile_meta.present[g] != 0;
+          for (int g = 0; g < kOwnGroups; ++g) open = open && tile_meta.present[group0 + g] != 0;
         }
         float* const keep_to = keep + j % kKeepStages * kRowTile + r;
         // (S of this tile came after the products of the one before the last: of the last one there is this)
@@ -816,36 +831,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
           }
         };
         if (__all_sync(0xFFFFFFFFu, open)) {
-          softmax_tile<DP, kUnit, kOpen, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[kSpread ? own : which], keep_to, before_o);
+          softmax_tile<DP, kUnit, kOpen, kWide, kTree, kSpread>(scores, sums, tile_meta, group0, row, key0, j == 0, &bars->halves[which], keep_to, before_o);
         } else {
           bool plain = true;
 #pragma unroll 1
-          for (int g = 0; g < kGroups; ++g) {
-            const float2 scales = tile_meta.scales[g];
+          for (int g = 0; g < kOwnGroups; ++g) {
+            const float2 scales = tile_meta.scales[group0 + g];
             const float factor = row.factor * scales.x;
             plain = plain && factor > 0.0f && factor < INFINITY && fabsf(scales.y) < INFINITY;
           }
           if (__all_sync(0xFFFFFFFFu, plain)) {
-            softmax_tile<DP, kUnit, kHidden, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[kSpread ? own : which], keep_to, before_o);
+            softmax_tile<DP, kUnit, kHidden, kWide, kTree, kSpread>(scores, sums, tile_meta, group0, row, key0, j == 0, &bars->halves[which], keep_to, before_o);
           } else {
-            softmax_tile<DP, kUnit, kSpecial, kWide, kTree>(scores, sums, tile_meta, row, key0, j == 0, &bars->halves[kSpread ? own : which], keep_to, before_o);
+            softmax_tile<DP, kUnit, kSpecial, kWide, kTree, kSpread>(scores, sums, tile_meta, group0, row, key0, j == 0, &bars->halves[which], keep_to, before_o);
           }
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->weights[own]);
+        if (lane == 0) mbar_arrive(kSpread && which == 0 ? &bars->halves[own] : &bars->weights[own]);
         if (kWide && lane == 0) mbar_arrive(&bars->kept[j % kKeepStages]);
       }
       if (!kWide && ok && tiles > 0) {
         ok = mbar_wait_warp(&bars->sums[kSpread ? (tiles - 1) & 1 : which], kSpread ? (tiles - 1) >> 1 & 1 : 0, abort_flag);
       }
-      if (ok) {
+      // O stands against the maximum alone, the sum against that and the largest scale; what the sum carries is taken
+      // from the partial results of O, as the kernel that joins them has it
+      float maximum = row.sum == 0.0f ? -INFINITY : row.maximum - row.largest_log;
+      float share = 1.0f, other_gain = 0.0f;  // kSpread: of the second half's keys
+      if (kSpread) {
+        float4* const ends = reinterpret_cast<float4*>(keep);
+        static_assert(kKeepStages * sizeof(float) >= sizeof(float4), "the rows' ends lie in the factors' place");
+        if (which == 1) ends[r] = make_float4(maximum, row.sum, row.largest, 0.0f);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (which == 0) {
+          const float4 other = ends[r];
+          const float most = fmaxf(maximum, other.x), base = most == -INFINITY ? 0.0f : most, other_share = exp2_fast(other.x - base);
+          share = exp2_fast(maximum - base);
+          maximum = most;
+          row.sum = fmaf(row.sum, share, other.y * other_share);
+          other_gain = other_share * other.z;
+        }
+      }
+      if (ok && (!kSpread || which == 0)) {
         tc_fence_after_sync();
         const bool whole = splits_used(p, rows) == 1;
-        // O stands against the maximum alone, the sum against that and the largest scale; what the sum carries is taken
-        // from the partial results of O, as the kernel that joins them has it
-        const float gain = row.sum == 0.0f ? 0.0f : whole ? row.largest / row.sum : row.largest * kCarriedInverse;
-        const float maximum = row.sum == 0.0f ? -INFINITY : row.maximum - row.largest_log;
+        const float by = row.sum == 0.0f ? 0.0f : whole ? 1.0f / row.sum : kCarriedInverse;
+        const float gain = kSpread ? share * row.largest * by : row.sum == 0.0f ? 0.0f : whole ? row.largest / row.sum : row.largest * kCarriedInverse;
+        other_gain *= by;
         const long long at = ((tile_index * p.splits + split) * kCtaRows + in_tile);
         if (kWide) {
           gains[r] = gain;
@@ -855,15 +887,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
           const long long to = whole ? row_at * p.out.token_stride + out_head * p.out.head_stride : at * p.dim;
           const bool staged = whole && p.out.type != QX_STORAGE_F32 && p.out.vector;  // (every product is done: so are the queries)
           uint8_t* const tile = smem + S::kQueries + which * S::kOperand;
+          const float applied = !kSpread ? gain : row.sum == 0.0f ? 0.0f : 1.0f;  // (kSpread: both gains are, below)
 #pragma unroll 1
           for (int c = 0; c < DP && c < p.dim; c += 32) {
             uint32_t o[32];
             if (tiles > 0) {
               tmem_ld_32x32(sums + c, o);
               tmem_ld_wait_for(o);
+              if (kSpread) {
+                uint32_t other[32];
+                tmem_ld_32x32(sums + 128 + c, other);
+                tmem_ld_wait_for(other);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                  const float a = gain == 0.0f ? 0.0f : __uint_as_float(o[i]) * gain;
+                  o[i] = __float_as_uint(other_gain == 0.0f ? a : fmaf(__uint_as_float(other[i]), other_gain, a));
+                }
+              }
             }
-            if (staged) stage_row<DP, false>(tile, p.out.type, o, gain, r, c);
-            else if (real) write_row(p, o, gain, whole ? nullptr : p.partial, to, c);
+            if (staged) stage_row<DP, false>(tile, p.out.type, o, applied, r, c);
+            else if (real) write_row(p, o, applied, whole ? nullptr : p.partial, to, c);
           }
           if (staged) write_rows<DP, false>(p, tile, rows, head, which * kRowTile + (warp & 3) * 32);
         }
@@ -881,6 +924,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
   } else if (warp < 8 + kConvertWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     convert(true, !kSpread);
+  } else if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+    if (kSpread) convert(false, true);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     if (warp == 12 && elect_one()) {
@@ -937,9 +983,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) prompt_kernel(const __grid_cons
               if (!ok) break;
               tc_fence_after_sync();
             }
-            mma_f16_ts(tmem + 256 + (kWide ? j & 1 : i) * 128, tmem + (kWide || kSpread ? j & 1 : i) * 128 + half * (kKeys / 2) + t / 2,
+            // (kSpread: the weights of each half of the keys lie at the start of its scores)
+            const int second = kSpread && t >= kKeys / 2 ? 1 : 0;
+            mma_f16_ts(tmem + 256 + (kWide ? j & 1 : i + second) * 128,
+                       tmem + (kWide || kSpread ? j & 1 : i) * 128 + half * (kKeys / 2) + t / 2 + second * (kKeys / 4),
                        make_sw128_nmajor_desc(base + S::kValueRing + stage * S::kOperand + t * 128, kKeys * 128), sums_desc,
-                       t > 0 || (kWide ? half == 0 : j > 0));
+                       (kSpread ? t % (kKeys / 2) : t) > 0 || (kWide ? half == 0 : j > 0));
           }
         }
         if (!ok) break;
@@ -996,7 +1045,7 @@ template <int DP, int kUnit, bool kWide, bool kTree, bool kSpread>
 qx_status launch_prompt_of(const AttentionParams& p, long long grid, cudaStream_t stream) {
   static SmemOptIn opt_in;
   QX_TRY(opt_in.ensure(prompt_kernel<DP, kUnit, kWide, kTree, kSpread>, TcShape<DP>::kBytes));
-  return launch_behind(prompt_kernel<DP, kUnit, kWide, kTree, kSpread>, grid, kTcThreads, TcShape<DP>::kBytes, stream, p);
+  return launch_behind(prompt_kernel<DP, kUnit, kWide, kTree, kSpread>, grid, threads_of(kSpread), TcShape<DP>::kBytes, stream, p);
 }
 template <bool kWide, bool kTree, bool kSpread = false>
 qx_status launch_prompt_sized(const AttentionParams& p, long long grid, cudaStream_t stream) {

@@ -298,3 +298,12 @@ def test_a_verification_step(qx):
         qx.check(cache.append_dev(batch_at(kept, [len(path) for path in paths]), k[rows], v[rows], rope), "append")
     torch.cuda.synchronize()
     qx.check(qx.lib.qx_check_device_errors(), "steps")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("group,drafts,length,dim,window", [(6, 64, 700, 128, 0), (6, 47, 129, 64, 0), (5, 63, 2600, 128, 1000), (8, 33, 50, 80, 64)])
+def test_three_tiles_of_rows(qx, dtype, group, drafts, length, dim, window):
+    rng = np.random.default_rng(group + length)
+    cache, table = filled(100, 2, 32, dim), tables(rng, 2, 90, 100)
+    trees = [tree(rng, drafts), tree(rng, drafts // 3)]
+    check(qx, cache, on_device(qx, cache), table, [length, drafts // 3 + 5], trees, typed((drafts + drafts // 3, 2 * group, dim), dtype, length), window)
