@@ -33,6 +33,11 @@
 //
 // A row's bits do not depend on the other tokens: columns are independent, and every sum has a fixed order.
 //
+// Measured, whole calls: 64 bf16 tokens, 8 of 128 q4_0 experts (4096 x 1536): 267 us, 5.0 TB/s, 0.76 of the copy bandwidth (63 % of
+// the issue slots: most of it block sums made f32 and scaled); 8 f16 tokens, 6 of 64 and 2 shared q8_0 experts (2048 x 1408): 63.5
+// us, 0.81; one bf16 token, 8 of 64 q4_0 experts (2048 x 1024): 18.6 us, of which 4.4 are its bytes: router 5.5, sorting
+// 0.5, up 6.6, down 3.5, combining 1.5, a chain; 5 f32 tokens, 2 of 8 and 1 shared q8_0 experts (1120 x 2016): 26.3.
+//
 // Every wait is bounded (two seconds); one that runs out raises the CTA's abort flag, is reported, and the copies in flight are
 // waited for (bounded).
 
