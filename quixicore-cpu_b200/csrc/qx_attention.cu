@@ -12,6 +12,10 @@ namespace {
 // rows 101 | 54; one of 16384 keys, 48 rows 42 | 41; f32, 4 of 4096 keys, 64 rows 84 | 87, 100 rows 96 | 90; 16 whole
 // texts of 64 tokens 25 | 29, of 100 tokens 40 | 32.
 constexpr long long kPromptFrom = 48, kPromptFromWide = 96;
+// Trees of 16-bit rows: as soon as the streamed kernel would read the codes more than once, over texts that are not short.
+// Streamed | prompt kernel, us, 24 (44) rows of 128 elements: 16 sequences of 8192 keys 132 | 107 (169 | 107), 4 of 4096 39 | 27 (49 |
+// 27), one of 16384 32 | 27 (40 | 27), 4 of 600 16.6 | 18.4 (17.1 | 18.6); of 64 elements, 32 rows, 4 of 4096 24.5 | 24.1.
+constexpr long long kPromptFromTree = 17, kPromptFromTreeKeys = 1024;
 // Trees whose rows fill one or three tiles of 128 take CTAs of one such tile, two softmax groups sharing its keys; of CTAs with
 // two tiles the last would have one to itself. One tile | two tiles a CTA, us, bf16 unless it says f16: 16 sequences of 64 rows, up
 // to 8192 keys 107 | 149; 384 rows, 131072 keys 273 | 306; 4 of 320 rows, 8192 keys 109 | 117; 8 of 384 rows, up to 4096 keys
@@ -218,7 +222,9 @@ qx_status launch_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, c
   p.group = q->heads / cache->kv_heads;
   const long long most_rows = static_cast<long long>(batch->max_tokens) * p.group;
   const bool wide = q->type == QX_STORAGE_F32;
-  const bool prompt = cache->head_dim <= 128 && most_rows >= (wide ? kPromptFromWide : kPromptFrom);
+  const long long tree_keys = p.window > 0 ? std::min<long long>(batch->max_length, static_cast<long long>(p.window) + kTreeRows) : batch->max_length;
+  const bool long_tree = tree != nullptr && tree_keys >= kPromptFromTreeKeys;
+  const bool prompt = cache->head_dim <= 128 && most_rows >= (wide ? kPromptFromWide : long_tree ? kPromptFromTree : kPromptFrom);
   const long long spread_tiles = (most_rows + kPromptRowsSpread - 1) / kPromptRowsSpread;
   const bool spread = prompt && tree != nullptr && !wide && spread_tiles <= kSpreadTiles && spread_tiles % 2 == 1;
   p.tile_rows = prompt ? (wide ? kPromptRowsWide : spread ? kPromptRowsSpread : kPromptRows) : most_rows <= 8 ? 8 : 16;
