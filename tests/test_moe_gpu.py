@@ -2,6 +2,7 @@
 every kind, strides, in place, host buffers, streams, graphs, workspaces; what is no number stays in its row."""
 
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -280,3 +281,47 @@ def test_scores_that_all_lie_far_below_zero(qx):
     m.router[:, 0] = -20.0
     assert float((x.double() @ m.router.double().T).max()) < -140
     check(qx, m, x, 3, sigmoid=True)
+
+
+@pytest.mark.parametrize("fmt,experts,dim,inner,shared,top,tokens", [(0, 512, 64, 32, 32, 32, 70), (1, 2, 65536, 32, 0, 1, 2), (0, 2, 32, 65536, 0, 1, 3)])
+def test_the_largest_layers(qx, fmt, experts, dim, inner, shared, top, tokens):
+    """As many experts, chosen and shared ones, and as wide rows as there may be."""
+    m = ref.layer(fmt, experts, dim, inner, shared, seed=33)
+    check(qx, m, tokens_of(m, tokens, torch.float32), top)
+
+
+def test_one_token_for_all(qx):
+    m = ref.layer(1, 6, 64, 96, seed=34)
+    check(qx, m, tokens_of(m, 1, torch.bfloat16).expand(5, 64), 2)
+    x, out = tokens_of(m, 1, torch.float32).cuda().expand(5, 64), torch.zeros(5, 64, device="cuda")
+    qx.check(prepared(qx, m).apply_dev(router(qx, m, 2), x, out), "apply")
+    assert all(torch.equal(row, out[0]) for row in out)
+
+
+def test_threads_with_a_stream_and_workspace_each(qx):
+    m = ref.layer(1, 16, 512, 256, 1, seed=35)
+    experts, r = prepared(qx, m), router(qx, m, 4)
+    x = tokens_of(m, 9, torch.bfloat16).cuda()
+    want = torch.empty_like(x)
+    qx.check(experts.apply_dev(r, x, want), "apply")
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        space, stream = workspace(qx), torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                out = torch.empty_like(x)
+                status = experts.apply_dev(r, x, out, workspace=space)
+                stream.synchronize()
+                if status != qx.OK or not torch.equal(out, want):
+                    wrong.append(status)
+        qx.lib.qx_workspace_destroy(space)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    qx.check(qx.lib.qx_check_device_errors(), "apply")
+    assert not wrong
