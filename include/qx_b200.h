@@ -763,8 +763,9 @@ typedef struct qx_norm {
 /* Any of these may be NULL: residual (zeros) or block (then joined = residual, without post and gate), not both;
  * post, gate; joined (not stored), or pre and normed together (not computed), not all. Every view and norm may have a
  * type of its own. joined and normed may each be residual, block or gate itself, the same view of it; otherwise written
- * views overlap no other view. dim is 1 .. 32768. Sums and statistics are f32 (a row's squares have to lie in its range), each output is rounded once; normed is
- * that of joined before its rounding. A row has the same bits in every batch of views of its types and alignment. */
+ * views overlap no other view. dim is 1 .. 32768. Sums and statistics are f32 (whose range a row's squares have to lie
+ * in), each output is rounded once; normed is that of joined before its rounding. A row has the same bits in every batch
+ * of views of its types and alignment. */
 QX_API qx_status qx_residual_norm(const qx_rows* residual, const qx_rows* block, const qx_norm* post,
                                   const qx_rows* gate, float scale, const qx_rows* joined, const qx_norm* pre,
                                   const qx_rows* normed, long long tokens, long long dim);
@@ -798,14 +799,14 @@ typedef struct qx_moe_router {
   float scale;
 } qx_moe_router;
 /* x and out: [tokens][dim], each with a type of its own; out is x itself, the same view of it, or lies elsewhere.
- * `chosen` and `weights` (either may be NULL) receive the experts and their w, [tokens][top], largest first. `activation`
- * is QX_ACTIVATION_*. Any number of tokens is served, in passes of up to 128; the kernels are made for few, whose experts' weights
- * are read once per eight tokens of theirs (f32: four).
+ * `chosen` and `weights` (either may be NULL) receive the experts and their w, [tokens][top], largest first.
+ * `activation` is QX_ACTIVATION_*. Any number of tokens is served, in passes of up to 128; the kernels are made for few,
+ * whose experts' weights are read once per eight tokens of theirs (f32: four).
  * Precision. Logits are summed up in 64 bits from f32 sums of 32 exact products, weights are f32 (choices by score and
- * bias: 64 bits). Codes are used as they are; x and the products of gate and up are rounded to 2^-15 of the largest of their 32
- * neighbours (a block's columns) for 16-bit x, to 2^-23 of it for f32 x, and to 2^-103 where that is more. Sums of a block are exact, sums of
- * blocks f32, out is rounded once. A token's bits do not depend on the other tokens. A token that holds a NaN or an
- * infinity, or whose product of gate and up overflows, spoils its own output only.
+ * bias: 64 bits). Codes are used as they are; x and the products of gate and up are rounded to 2^-15 of the largest of
+ * their 32 neighbours (a block's columns) for 16-bit x, to 2^-23 of it for f32 x, and to 2^-103 where that is more. Sums
+ * of a block are exact, sums of blocks f32, out is rounded once. A token's bits do not depend on the other tokens. A
+ * token that holds a NaN or an infinity, or whose product of gate and up overflows, spoils its own output only.
  * What lies between the kernels is in `workspace`, one of the current device (NULL: the library's default one); calls
  * that may run at the same time need one each. */
 QX_API qx_status qx_moe_apply(const qx_moe* moe, const qx_moe_router* router, const qx_rows* x, const qx_rows* out,
