@@ -969,29 +969,41 @@ def _row_view(t, tokens, dim, device, storage=None, one=False) -> RowsView:
     return RowsView(data, kind, stride)
 
 
-def _residual_norm(device, residual, block, joined, normed, pre, post, gate, scale, storage=None):
-    tokens, dim = (block if residual is None else residual).shape
-    before = after = None
-    if post is not None:
-        assert post.dim in (None, dim) and post.device in (None, device), "a norm of another size or device"
-        before = post.view
-    if pre is not None:
-        assert pre.dim in (None, dim) and pre.device in (None, device), "a norm of another size or device"
-        after = pre.view
-    return (_row_view(residual, tokens, dim, device, storage), _row_view(block, tokens, dim, device, storage), before,
-            _row_view(gate, tokens, dim, device, storage, True), scale, _row_view(joined, tokens, dim, device, storage),
-            after, _row_view(normed, tokens, dim, device, storage), tokens, dim)
+def _device_row(t, tokens, dim, device) -> RowsView:
+    """The same of a tensor on `device`, all at once: a call of few rows takes the host longer than the GPU."""
+    if t is None:
+        return None
+    assert not isinstance(t, np.ndarray), "need a tensor on the current device"
+    (rows, elements), (stride, step) = t.shape, t.stride()
+    assert (rows >= tokens and elements == dim and (step == 1 or dim == 1) and t.get_device() == device
+            ), "need [tokens, dim] with the elements of a row side by side, on the current device"
+    return RowsView(t.data_ptr(), (_torch_types or _fill_torch_types())[t.dtype], stride)
+
+
+def _norm_view(norm, dim, device):
+    if norm is None:
+        return None
+    assert norm.dim in (None, dim) and norm.device in (None, device), "a norm of another size or device"
+    return norm.view
 
 
 def residual_norm(residual, block, joined, normed=None, pre=None, post=None, gate=None, scale=1.0, storage=None) -> int:
     """joined = residual + scale * gate * post(block), normed = pre(joined) over numpy arrays [tokens, dim]."""
-    return lib.qx_residual_norm(*_residual_norm(-1, residual, block, joined, normed, pre, post, gate, scale, storage))
+    tokens, dim = (block if residual is None else residual).shape
+    return lib.qx_residual_norm(_row_view(residual, tokens, dim, -1, storage), _row_view(block, tokens, dim, -1, storage),
+                                _norm_view(post, dim, -1), _row_view(gate, tokens, dim, -1, storage, True), scale,
+                                _row_view(joined, tokens, dim, -1, storage), _norm_view(pre, dim, -1),
+                                _row_view(normed, tokens, dim, -1, storage), tokens, dim)
 
 
 def residual_norm_dev(residual, block, joined, normed=None, pre=None, post=None, gate=None, scale=1.0) -> int:
     """The same over tensors on the current device, on torch's current stream."""
-    return lib.qx_residual_norm_dev(*_residual_norm(_device(), residual, block, joined, normed, pre, post, gate, scale),
-                                    _stream())
+    device = _device()
+    tokens, dim = (block if residual is None else residual).shape
+    return lib.qx_residual_norm_dev(_device_row(residual, tokens, dim, device), _device_row(block, tokens, dim, device),
+                                    _norm_view(post, dim, device), None if gate is None else _row_view(gate, tokens, dim, device, None, True),
+                                    scale, _device_row(joined, tokens, dim, device), _norm_view(pre, dim, device),
+                                    _device_row(normed, tokens, dim, device), tokens, dim, _stream())
 
 
 # ---- mixture-of-experts layers ----
