@@ -166,6 +166,8 @@ __device__ __forceinline__ void convert_columns(const Params& p, int token, int 
   if (d < p.dim && (lane & 7) == 0) p.x_scales[static_cast<long long>(token) * scales_of(p.dim) + d / 32] = factor.down;
 }
 
+constexpr float kLeastScore = 7.8886090522101181e-31f;  // 2^-100: from here on f32 holds scores and their quotients
+
 // Order-preserving whole number of a double, and back; NaN is above everything.
 __device__ __forceinline__ unsigned long long ordered(double v) {
   const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(v));
@@ -182,25 +184,43 @@ __device__ __forceinline__ T warp_sum(T v) {
   return v;
 }
 
-// A warp chooses a token's experts by their keys: logits, or scores and biases (`scores`: those alone).
-__device__ __forceinline__ void choose(const Params& p, unsigned long long* keys, float* scores, int token) {
-  const int lane = threadIdx.x & 31, places = p.top + p.shared, each = (p.experts + 31) / 32;
-  if (p.bias != nullptr && p.score == QX_MOE_SOFTMAX) {  // (scores need all logits)
-    double largest = -INFINITY, total = 0.0;
-    for (int e = lane; e < p.experts; e += 32) largest = fmax(largest, from_ordered(keys[e]));
+// The weight of a lane's expert where scores run out of f32 (sigmoids, or such as a bias has lifted past far larger logits):
+// quotients by logarithms, in 64 bits, where no score is too small. `most`, `all`: of a softmax, the largest of all logits and the
+// sum of all e^(l - most). (Rare, so not inline: what every token runs stays together.)
+__device__ __noinline__ float far_weight(double logit, bool sigmoid, double most, double all, bool takes, bool normalise, float scale) {
+  double power = sigmoid ? fmin(logit, 0.0) - log1p(exp(-fabs(logit))) : logit - most - log(all), sum = 1.0;
+  if (normalise) {
+    double top = takes ? power : -INFINITY;
 #pragma unroll
-    for (int h = 16; h > 0; h >>= 1) largest = fmax(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, h));
+    for (int h = 16; h > 0; h >>= 1) top = fmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, h));
+    power -= top;
+    sum = warp_sum(takes ? exp(power) : 0.0);
+  }
+  return static_cast<float>(exp(power) / sum * scale);
+}
+
+// A warp chooses a token's experts by their keys: logits, or scores and biases (`scores`, `logits`: without the biases).
+__device__ __forceinline__ void choose(const Params& p, unsigned long long* keys, double* logits, float* scores, int token) {
+  const int lane = threadIdx.x & 31, places = p.top + p.shared, each = (p.experts + 31) / 32;
+  double most = -INFINITY, all = 0.0;  // softmax with biases: the largest of all logits, the sum of all e^(l - most)
+  if (p.bias != nullptr && p.score == QX_MOE_SOFTMAX) {  // (scores need all logits)
+    for (int e = lane; e < p.experts; e += 32) {
+      logits[e] = from_ordered(keys[e]);
+      most = fmax(most, logits[e]);
+    }
+#pragma unroll
+    for (int h = 16; h > 0; h >>= 1) most = fmax(most, __shfl_xor_sync(0xFFFFFFFFu, most, h));
     for (int pass = 0; pass < 2; ++pass) {
       for (int e = lane; e < p.experts; e += 32) {
-        const double score = exp(from_ordered(keys[e]) - largest);
+        const double score = exp(logits[e] - most);
         if (pass == 0) {
-          total += score;
+          all += score;
         } else {
-          scores[e] = static_cast<float>(score / total);
-          keys[e] = ordered(score / total + static_cast<double>(p.bias[e]));
+          scores[e] = static_cast<float>(score / all);
+          keys[e] = ordered(score / all + static_cast<double>(p.bias[e]));
         }
       }
-      if (pass == 0) total = warp_sum(total);
+      if (pass == 0) all = warp_sum(all);
     }
     __syncwarp();
   }
@@ -238,9 +258,7 @@ __device__ __forceinline__ void choose(const Params& p, unsigned long long* keys
   if (p.bias != nullptr) {
     if (takes) score = scores[expert];
   } else if (p.score == QX_MOE_SIGMOID) {
-    // (far below zero sigmoid(l) is e^l, whose quotients do not run out of f32)
-    const bool far = p.normalise && largest < -80.0;
-    if (takes) score = far ? expf(static_cast<float>(key - largest)) : 1.0f / (1.0f + expf(static_cast<float>(-key)));
+    if (takes) score = 1.0f / (1.0f + expf(static_cast<float>(-key)));
   } else {
     if (takes) score = expf(static_cast<float>(key - largest));
     if (!p.normalise) {
@@ -260,6 +278,16 @@ __device__ __forceinline__ void choose(const Params& p, unsigned long long* keys
   if (lane < p.shared) {
     p.picks[token * places + p.top + lane] = p.experts + lane;
     p.weights[token * places + p.top + lane] = 1.0f;
+  }
+  // Once more where scores ran out of f32. (A softmax without a bias stands against its largest, which is chosen. Behind all else,
+  // which costs the others 0.1 us; as a choice of the weight in front of the stores 0.3.)
+  if ((p.bias != nullptr || p.score == QX_MOE_SIGMOID) && __any_sync(0xFFFFFFFFu, takes && score < kLeastScore)) {
+    const double logit = p.bias != nullptr && takes ? logits[expert] : key;
+    const float weight = far_weight(logit, p.score == QX_MOE_SIGMOID, most, all, takes, p.normalise != 0, p.scale);
+    if (takes) {
+      p.weights[token * places + lane] = weight;
+      if (p.chosen_weights != nullptr) p.chosen_weights[static_cast<long long>(token) * p.top + lane] = weight;
+    }
   }
 }
 
@@ -336,8 +364,10 @@ __device__ __forceinline__ void sum_logits(const Params& p, int token0, int expe
     }
   }
 }
-// Shared memory: a cluster's first CTA holds the keys and scores of eight tokens, behind the parts of sums.
-constexpr int kPartBytes = kRouterWarps * kRouterExperts * kRouterTokens * 8, kKeyBytes = 8 + 4;
+// Shared memory: a cluster's first CTA holds the keys of eight tokens, with a bias their logits and scores too, behind the
+// parts of sums.
+constexpr int kPartBytes = kRouterWarps * kRouterExperts * kRouterTokens * 8;
+constexpr int key_bytes(bool biased) { return biased ? 8 + 8 + 4 : 8; }
 
 // Grid: a cluster for every eight tokens, then those that convert activations. kX, kW: types of activations and router.
 template <int kX, int kW>
@@ -345,7 +375,8 @@ __global__ void __launch_bounds__(kRouterThreads, 1) moe_router_kernel(const __g
   extern __shared__ __align__(128) uint8_t smem[];
   auto& parts = *reinterpret_cast<double(*)[kRouterWarps][kRouterExperts][kRouterTokens]>(smem);
   unsigned long long* const keys = reinterpret_cast<unsigned long long*>(smem + kPartBytes);  // [token][expert]
-  float* const scores = reinterpret_cast<float*>(keys + kRouterTokens * p.experts);
+  double* const logits = reinterpret_cast<double*>(keys + kRouterTokens * p.experts);
+  float* const scores = reinterpret_cast<float*>(logits + kRouterTokens * p.experts);
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("barrier.cluster.arrive.relaxed.aligned;");  // (its CTAs run: their shared memory may be written)
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -383,6 +414,8 @@ __global__ void __launch_bounds__(kRouterThreads, 1) moe_router_kernel(const __g
       uint32_t to;
       if (p.bias != nullptr && p.score == QX_MOE_SIGMOID) {
         const double score = 1.0 / (1.0 + exp(-key));
+        asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(logits + t * p.experts + expert0 + e)));
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(key) : "memory");
         key = score + static_cast<double>(p.bias[expert0 + e]);
         asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(scores + t * p.experts + expert0 + e)));
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(static_cast<float>(score)) : "memory");
@@ -394,7 +427,9 @@ __global__ void __launch_bounds__(kRouterThreads, 1) moe_router_kernel(const __g
   }
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (rank == 0 && warp < kRouterTokens && token0 + warp < p.tokens) choose(p, keys + warp * p.experts, scores + warp * p.experts, token0 + warp);
+  if (rank == 0 && warp < kRouterTokens && token0 + warp < p.tokens) {
+    choose(p, keys + warp * p.experts, logits + warp * p.experts, scores + warp * p.experts, token0 + warp);
+  }
 }
 
 // ---- experts -----------------------------------------------------------------------------------
@@ -1060,14 +1095,14 @@ struct Layout {
 template <int kX, int kW>
 qx_status launch_router(const Params& p, cudaStream_t stream) {
   static SmemOptIn opt_in;
-  QX_TRY(opt_in.ensure(moe_router_kernel<kX, kW>, kPartBytes + kRouterTokens * kMostExperts * kKeyBytes));
+  QX_TRY(opt_in.ensure(moe_router_kernel<kX, kW>, kPartBytes + kRouterTokens * kMostExperts * key_bytes(true)));
   int size = 1;
   while (size < kRouterCluster && size * kRouterExperts < p.experts) size *= 2;
   const int convert = (p.tokens * ((p.dim + 127) / 128) + kRouterWarps - 1) / kRouterWarps;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(((p.tokens + kRouterTokens - 1) / kRouterTokens + (convert + size - 1) / size) * size);
   config.blockDim = dim3(kRouterThreads);
-  config.dynamicSmemBytes = kPartBytes + static_cast<size_t>(kRouterTokens) * p.experts * kKeyBytes;
+  config.dynamicSmemBytes = kPartBytes + static_cast<size_t>(kRouterTokens) * p.experts * key_bytes(p.bias != nullptr);
   config.stream = stream;
   cudaLaunchAttribute attributes[2];
   attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
