@@ -128,12 +128,13 @@ struct Words {
 };
 
 // The power of two that brings a block whose largest magnitude is `top` (as f32 bits) to what two or three balanced digits
-// hold (127 * 257, 127 * 65793), and its inverse; NaN for a block that holds a NaN or an infinity.
+// hold (127 * 257, 127 * 65793), and its inverse; NaN for a block that holds a NaN or an infinity. No digit stands for less than
+// 2^-102: times the smallest d of a block that is still a normal number.
 struct Factor {
   float up, down;
 };
 __device__ __forceinline__ Factor block_factor(uint32_t top, int digits) {
-  const int bits = digits == 2 ? 14 : 22, exponent = max(47, static_cast<int>((top + 0x10200u) >> 23));
+  const int bits = digits == 2 ? 14 : 22, exponent = max(25 + bits, static_cast<int>((top + 0x10200u) >> 23));
   return {__uint_as_float(static_cast<uint32_t>(bits + 254 - exponent) << 23),
           top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(exponent - bits) << 23)};
 }
