@@ -47,6 +47,7 @@
 
 #include "qx_host_arrays.cuh"
 #include "qx_moe.cuh"
+#include "qx_moe_units.h"
 #include "qx_scaled_gemm.cuh"
 #include "qx_tile_pipe.cuh"
 
@@ -437,7 +438,8 @@ __global__ void __launch_bounds__(kRouterThreads, 1) moe_router_kernel(const __g
 constexpr int kMathWarps = 8, kExpertThreads = 32 * (kMathWarps + 2);
 constexpr int kWeightWarp = kMathWarps, kColumnWarp = kMathWarps + 1;
 constexpr int kUnitRows = kUnitTiles * kTileRows;
-constexpr int kCombineWidth = 1024, kMostTokens = 8;
+constexpr int kMostTokens = 8;
+static_assert(kUpWidth == kUnitRows / 2 && kDownWidth == kUnitRows && kCombineWidth == 4 * 32 * kMathWarps, "what the kernel cuts");
 constexpr int kReduceTile = 64 + 1, kReduceWarp = kUnitTiles * kReduceTile;  // floats: [row g, g + 8][lane]
 enum { kUp = 0, kDown = 1, kCombine = 2, kExit = 3 };
 
@@ -1196,9 +1198,7 @@ qx_status launch_apply(const qx_moe* m, const qx_moe_router* router, const qx_ro
     QX_TRY(p.x_type == QX_STORAGE_F32   ? launch_router<QX_STORAGE_F32>(p, stream)
            : p.x_type == QX_STORAGE_F16 ? launch_router<QX_STORAGE_F16>(p, stream)
                                         : launch_router<QX_STORAGE_BF16>(p, stream));
-    // (no more CTAs than there may be units)
-    const long long units = static_cast<long long>(p.tokens) * (p.top + p.shared) * (p.inner / 32);
-    const long long grid = std::min<long long>(2LL * ctx->prop.multiProcessorCount, units);
+    const long long grid = std::min(2LL * ctx->prop.multiProcessorCount, pass_blocks(p.tokens, p.top + p.shared, p.dim, p.inner));
     if (m->format == QX_FORMAT_Q4_0) {
       QX_TRY(p.digits == 2 ? (launch_experts<QX_FORMAT_Q4_0, 2>(p, grid, stream)) : (launch_experts<QX_FORMAT_Q4_0, 3>(p, grid, stream)));
     } else {
