@@ -25,6 +25,8 @@ std::atomic<int> g_threads{1};
 void set_last_error(const char* where, cudaError_t code) {
   tl_error = std::string(where) + ": " + cudaGetErrorName(code) + " (" +
              cudaGetErrorString(code) + ")";
+  // It is reported: the runtime would hand it to the next launch's check again. (What has broken the context stays.)
+  (void)cudaGetLastError();
 }
 void set_last_error_text(const char* text) { tl_error = text; }
 
