@@ -133,7 +133,7 @@ qx_status take_device_error(DeviceContext* ctx) {
   if (code == 0) return QX_STATUS_OK;
   *static_cast<volatile int*>(ctx->error_host) = 0;
   if (code < sm100::kErrorFirstBatch && ctx->workspace.base != nullptr) {
-    (void)cudaMemset(ctx->workspace.base, 0, kWorkspaceCounterBytes);
+    (void)zero_now(ctx->workspace.base, kWorkspaceCounterBytes);
   }
   char text[128];
   if (code == kv::kErrorSequence) {

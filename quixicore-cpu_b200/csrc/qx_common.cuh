@@ -97,6 +97,13 @@ bool format_info(int format, size_t* block_bytes);
 qx_status validate_nk(int format, long long n, long long k);
 qx_status packed_bytes(int format, long long n, long long k, size_t* size);
 
+// Device memory that is zero when this returns. cudaMemset does not wait for the default stream that it works on, and streams
+// made without ties to that one do not either: their kernels could count on what was there before.
+inline cudaError_t zero_now(void* data, size_t bytes) {
+  const cudaError_t state = cudaMemset(data, 0, bytes);
+  return state == cudaSuccess ? cudaStreamSynchronize(nullptr) : state;
+}
+
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // cudaFuncAttributeMaxDynamicSharedMemorySize is a per-device attribute of a kernel: every

@@ -86,7 +86,7 @@ qx_status current_context(DeviceContext** out) {
     }
     QX_CUDA_TRY(cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking));
     QX_CUDA_TRY(cudaMalloc(&ctx->flag, 256));
-    QX_CUDA_TRY(cudaMemset(ctx->flag, 0, 256));
+    QX_CUDA_TRY(zero_now(ctx->flag, 256));
     QX_CUDA_TRY(cudaHostAlloc(reinterpret_cast<void**>(&ctx->error_host), 64, cudaHostAllocMapped));
     ctx->error_host[0] = 0;
     QX_CUDA_TRY(cudaHostGetDevicePointer(reinterpret_cast<void**>(&ctx->error_dev), ctx->error_host, 0));
@@ -157,7 +157,7 @@ qx_status qx_workspace::reserve(size_t bytes) {
   const size_t want = qx::align_up(bytes + bytes / 8, 1 << 20);
   QX_CUDA_TRY(cudaMalloc(&base, want));
   capacity = want;
-  QX_CUDA_TRY(cudaMemset(base, 0, qx::kWorkspaceCounterBytes));
+  QX_CUDA_TRY(qx::zero_now(base, qx::kWorkspaceCounterBytes));
   return QX_STATUS_OK;
 }
 

@@ -548,7 +548,7 @@ qx_status stream_k_scratch(int device, StreamKScratch* out) {
       set_last_error("cudaMalloc(stream-K scratch)", err);
       return err == cudaErrorMemoryAllocation ? QX_STATUS_OUT_OF_MEMORY : QX_STATUS_DEVICE_ERROR;
     }
-    err = cudaMemset(static_cast<uint8_t*>(block) + partial_bytes, 0, counter_bytes);
+    err = zero_now(static_cast<uint8_t*>(block) + partial_bytes, counter_bytes);
     if (err != cudaSuccess) {
       set_last_error("cudaMemset(stream-K counters)", err);
       (void)cudaFree(block);

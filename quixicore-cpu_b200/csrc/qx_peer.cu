@@ -120,7 +120,7 @@ qx_status qx_peer_alloc(size_t bytes, void** dev_ptr, unsigned char handle[64]) 
     return err == cudaErrorMemoryAllocation ? QX_STATUS_OUT_OF_MEMORY : QX_STATUS_DEVICE_ERROR;
   }
   cudaIpcMemHandle_t ipc;
-  if ((err = cudaMemset(ptr, 0, align_up(bytes, 256))) != cudaSuccess ||
+  if ((err = zero_now(ptr, align_up(bytes, 256))) != cudaSuccess ||
       (err = cudaIpcGetMemHandle(&ipc, ptr)) != cudaSuccess) {
     set_last_error("cudaIpcGetMemHandle", err);
     (void)cudaFree(ptr);
