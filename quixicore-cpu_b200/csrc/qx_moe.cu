@@ -186,7 +186,7 @@ __device__ __forceinline__ T warp_sum(T v) {
   return v;
 }
 
-// The weight of a lane's expert where scores run out of f32 (sigmoids, or such as a bias has lifted past far larger logits):
+// The weight of a lane's expert where scores run out of f32 (sigmoids, or logits far below the largest):
 // quotients by logarithms, in 64 bits, where no score is too small. `most`, `all`: of a softmax, the largest of all logits and the
 // sum of all e^(l - most). (Rare, so not inline: what every token runs stays together.)
 __device__ __noinline__ float far_weight(double logit, bool sigmoid, double most, double all, bool takes, bool normalise, float scale) {
@@ -204,7 +204,7 @@ __device__ __noinline__ float far_weight(double logit, bool sigmoid, double most
 // A warp chooses a token's experts by their keys: logits, or scores and biases (`scores`, `logits`: without the biases).
 __device__ __forceinline__ void choose(const Params& p, unsigned long long* keys, double* logits, float* scores, int token) {
   const int lane = threadIdx.x & 31, places = p.top + p.shared, each = (p.experts + 31) / 32;
-  double most = -INFINITY, all = 0.0;  // softmax with biases: the largest of all logits, the sum of all e^(l - most)
+  double most = -INFINITY, all = 1.0;  // softmax: the largest of all logits, the sum of all e^(l - most) where the weights need it
   if (p.bias != nullptr && p.score == QX_MOE_SOFTMAX) {  // (scores need all logits)
     for (int e = lane; e < p.experts; e += 32) {
       logits[e] = from_ordered(keys[e]);
@@ -212,6 +212,7 @@ __device__ __forceinline__ void choose(const Params& p, unsigned long long* keys
     }
 #pragma unroll
     for (int h = 16; h > 0; h >>= 1) most = fmax(most, __shfl_xor_sync(0xFFFFFFFFu, most, h));
+    all = 0.0;
     for (int pass = 0; pass < 2; ++pass) {
       for (int e = lane; e < p.experts; e += 32) {
         const double score = exp(logits[e] - most);
@@ -267,7 +268,9 @@ __device__ __forceinline__ void choose(const Params& p, unsigned long long* keys
       total = 0.0f;
       for (int e = lane; e < p.experts; e += 32) total += expf(static_cast<float>(from_ordered(keys[e]) - largest));
       total = warp_sum(total);
+      all = total;
     }
+    most = largest;
   }
   if (p.normalise) total = warp_sum(score);
   if (takes) {
@@ -281,9 +284,9 @@ __device__ __forceinline__ void choose(const Params& p, unsigned long long* keys
     p.picks[token * places + p.top + lane] = p.experts + lane;
     p.weights[token * places + p.top + lane] = 1.0f;
   }
-  // Once more where scores ran out of f32. (A softmax without a bias stands against its largest, which is chosen. Behind all else,
-  // which costs the others 0.1 us; as a choice of the weight in front of the stores 0.3.)
-  if ((p.bias != nullptr || p.score == QX_MOE_SIGMOID) && __any_sync(0xFFFFFFFFu, takes && score < kLeastScore)) {
+  // Once more where scores ran out of f32. (Behind all else, which costs the others 0.1 us; as a choice of the weight in front of the
+  // stores 0.3.)
+  if (__any_sync(0xFFFFFFFFu, takes && score < kLeastScore)) {
     const double logit = p.bias != nullptr && takes ? logits[expert] : key;
     const float weight = far_weight(logit, p.score == QX_MOE_SIGMOID, most, all, takes, p.normalise != 0, p.scale);
     if (takes) {

@@ -94,6 +94,15 @@ def test_sigmoids_without_a_bias(qx, first, last, top, normalise):
     check(qx, m, x, top, True, False, normalise)
 
 
+@pytest.mark.parametrize("normalise", [False, True])
+@pytest.mark.parametrize("scale", [1.0, 1e30])
+def test_softmax_without_a_bias(qx, scale, normalise):
+    """Experts far below the largest, with a scale that makes plain numbers of their weights."""
+    m, x = far_layer([5.0, -60.0, -75.0, -90.0, -98.0, -120.0], [])
+    m.raw[2].reshape(-1, 18)[:, :2] = 0  # (down projections of zeros: outputs that fit)
+    check(qx, m, x, 6, False, False, normalise, scale)
+
+
 @pytest.mark.parametrize("sigmoid", [False, True])
 @pytest.mark.parametrize("biased", [False, True])
 def test_one_expert_takes_the_whole_weight(qx, sigmoid, biased):
