@@ -731,7 +731,10 @@ QX_API qx_status qx_kv_attention_dev(const qx_kv_cache* cache, const qx_kv_batch
  * itself. Bits of rows that the sequence does not have count for nothing. `window` is 0 or 64 and more: a row that sees d drafts stands
  * at position (tokens in front) + d - 1, and keys in front of the drafts at that position - window and before are hidden.
  * `seen` has an entry for every row of the views. All else is as for qx_kv_attention. Tokens that are accepted
- * in the end are appended again, in their order, as the last tokens of a sequence of that length. */
+ * in the end are appended again, in their order, as the last tokens of a sequence of that length. Drafts that are rejected
+ * leave a trace: where they began inside a block, its scales stay at least as large as theirs were, and its older codes
+ * have been rounded to that (see qx_kv_append). A program that wants none copies that block's codes and scales before it appends
+ * the drafts, and puts them back before it appends the accepted ones; blocks that an append begins start afresh. */
 QX_API qx_status qx_kv_tree_attention(const qx_kv_cache* cache, const qx_kv_batch* batch, const qx_heads* q,
                                       const qx_heads* out, float* lse, float scale, long long window,
                                       const uint64_t* seen);
@@ -799,14 +802,17 @@ typedef struct qx_moe_router {
   float scale;
 } qx_moe_router;
 /* x and out: [tokens][dim], each with a type of its own; out is x itself, the same view of it, or lies elsewhere.
- * `chosen` and `weights` (either may be NULL) receive the experts and their w, [tokens][top], largest first.
+ * `chosen` and `weights` (either may be NULL) receive the experts and their w, [tokens][top], in the order of the choice: the
+ * largest l, or s + bias, first.
  * `activation` is QX_ACTIVATION_*. Any number of tokens is served, in passes of up to 128; the kernels are made for few,
  * whose experts' weights are read once per eight tokens of theirs (f32: four).
- * Precision. Logits are summed up in 64 bits from f32 sums of 32 exact products, weights are f32 (choices by score and
- * bias: 64 bits). Codes are used as they are; x and the products of gate and up are rounded to 2^-15 of the largest of
- * their 32 neighbours (a block's columns) for 16-bit x, to 2^-23 of it for f32 x, and to 2^-103 where that is more. Sums
- * of a block are exact, sums of blocks f32, out is rounded once. A token's bits do not depend on the other tokens. A
- * token that holds a NaN or an infinity, or whose product of gate and up overflows, spoils its own output only.
+ * Precision. Logits are summed up in 64 bits from f32 sums of 32 exact products: they are off by 36 * 2^-24 of the sum of
+ * |x W| at most, and experts closer than that may change places. Choices by score and bias are taken in 64 bits; weights are
+ * f32, of scores however small those are. Codes are used as they are; x and the products of gate and up are rounded to 2^-15
+ * of the largest of their 32 neighbours (a block's columns) for 16-bit x, to 2^-23 of it for f32 x, and to 2^-103 where that
+ * is more. Sums of a block are exact and rounded once to f32, sums of blocks are f32, out is rounded once. A token's bits do
+ * not depend on the other tokens. A token that holds a NaN or an infinity, or whose product of gate and up overflows, spoils
+ * its own output only.
  * What lies between the kernels is in `workspace`, one of the current device (NULL: the library's default one); calls
  * that may run at the same time need one each. */
 QX_API qx_status qx_moe_apply(const qx_moe* moe, const qx_moe_router* router, const qx_rows* x, const qx_rows* out,
