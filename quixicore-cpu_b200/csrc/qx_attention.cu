@@ -20,7 +20,9 @@ constexpr long long kPromptFromTree = 17, kPromptFromTreeKeys = 1024;
 // two tiles the last would have one to itself. One tile | two tiles a CTA, us, bf16 unless it says f16: 16 sequences of 64 rows, up
 // to 8192 keys 107 | 149; 384 rows, 131072 keys 273 | 306; 4 of 320 rows, 8192 keys 109 | 117; 8 of 384 rows, up to 4096 keys
 // 57 | 73; one of 384 f16 rows of 64 elements, 16384 keys 45 | 52. An even number: 6 of 189 f16 rows of 64 elements, 4096 keys
-// 58 | 44; 4 of 192 rows, 4096 keys 47 | 44. (Five and more tiles would convert each code five times.)
+// 58 | 44; 4 of 192 rows, 4096 keys 47 | 44. Five tiles, each of which would convert every code: one session of 16384 keys 90 | 84, of
+// 131072 537 | 452, 8 of 4096 121 | 106, 16 of 2000 130 | 109, f16 rows of 64 elements 79 | 73; the other way round where CTAs of two
+// tiles leave much of the card empty, as 96 of them do (4 of 8192 116 | 177).
 constexpr long long kSpreadTiles = 3;
 
 // Joins the chunks of one row, in an order that their number fixes: the threads are cut into parts, a thread of part i

@@ -7,8 +7,9 @@
 // arranged around keeping those loads under way from the first to the last.
 //
 // Router (moe_router_kernel). Both operands are cut into bf16 terms that add up to them (one for bf16, two for f16, three for
-// f32), so that every product on bf16 MMAs is exact; sums over 32 columns are the MMA's, those over the rest 64-bit: two experts
-// on both sides of the choice are told apart as far as the inputs' own products are. A CTA takes 16 experts and eight tokens, its
+// f32), so that every product on bf16 MMAs is exact; sums over 32 columns are the MMAs', f32, in 2 .. 18 steps, those over the rest
+// 64-bit: a logit is off by no more than 36 * 2^-24 of the sum of |x w|, and two experts closer than that may change places
+// at the border of the choice. A CTA takes 16 experts and eight tokens, its
 // 16 warps 32 columns each in turn; the CTAs of eight tokens are a cluster, whose first gets all their logits in shared
 // memory and chooses the experts, a warp per token. Beside them, other CTAs turn the activations into digits. What it costs
 // is latency, a good part of it that of instructions which are fetched once, so loops stay loops here.
@@ -26,17 +27,19 @@
 // nibbles, laid out as the signed n - 8, as 16 times that in the upper halves of bytes (q4_0), against the activations as
 // balanced base-256 digits under a power of two per 32 columns: two digits for 16-bit inputs (2^-15 of a block's largest), three
 // for f32 ones (2^-23). An MMA takes a block and gives exact sums. A token's digits are neighbouring columns: a lane joins two
-// of them, and multiplies with the block's d and the activations' scale. Four tokens (f32: two) cost no more than one.
+// of them, exactly (up to 2^28), rounds that to f32 and multiplies with the block's d and the activations' scale. Four tokens
+// (f32: two) cost no more than one.
 // (As f16 pairs on f16 MMAs the conversion of the codes took three quarters of the instructions, and the layer twice the
 // time; sums that start at the bits of 1.5 * 2^23, to be f32 numbers after a subtraction, cost four moves an MMA.) The
 // products of gate and up get digits in the same way.
 //
 // A row's bits do not depend on the other tokens: columns are independent, and every sum has a fixed order.
 //
-// Measured, whole calls: 64 bf16 tokens, 8 of 128 q4_0 experts (4096 x 1536): 267 us, 5.0 TB/s, 0.76 of the copy bandwidth (63 % of
-// the issue slots: most of it block sums made f32 and scaled); 8 f16 tokens, 6 of 64 and 2 shared q8_0 experts (2048 x 1408): 63.5
-// us, 0.81; one bf16 token, 8 of 64 q4_0 experts (2048 x 1024): 18.6 us, of which 4.4 are its bytes: router 5.5, sorting
-// 0.5, up 6.6, down 3.5, combining 1.5, a chain; 5 f32 tokens, 2 of 8 and 1 shared q8_0 experts (1120 x 2016): 26.3.
+// Measured, whole calls on weights that have left L2: 64 bf16 tokens, 8 of 128 q4_0 experts (4096 x 1536): 265 us, under lasting
+// load 296 (the clock falls), 5.0 to 4.5 TB/s, 0.77 to 0.69 of the copy bandwidth (63 % of the issue slots: most of it block sums
+// made f32 and scaled); 8 f16 tokens, 6 of 64 and 2 shared q8_0 experts (2048 x 1408): 66 us, 0.78; one bf16 token, 8 of 64 q4_0
+// experts (2048 x 1024): 19.5 us, of which 4.4 are its bytes: router 5.5, sorting 0.5, up 6.6, down 3.5, combining 1.5, a chain; 5
+// f32 tokens, 2 of 8 and 1 shared q8_0 experts (1120 x 2016): 26 to 27.
 //
 // Every wait is bounded (two seconds); one that runs out raises the CTA's abort flag, is reported, and the copies in flight are
 // waited for (bounded).
@@ -631,7 +634,7 @@ __device__ __forceinline__ void multiply(const uint8_t* records, int tiles_there
       for (int n = 0; n < kN; ++n) {
         int sum[4];
         mma_block(sum, a, x[n]);
-        // (below 2^28)
+        // (below 2^28: rounded once, to f32)
         total[i][n][0] = fmaf(static_cast<float>(sum[1] * join + sum[0]), scale[n] * d.x, total[i][n][0]);
         total[i][n][1] = fmaf(static_cast<float>(sum[3] * join + sum[2]), scale[n] * d.y, total[i][n][1]);
       }

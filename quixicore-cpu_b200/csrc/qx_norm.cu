@@ -46,7 +46,8 @@ struct JoinParams {
 
 // How a thread's 8 * kVectors elements of a row lie, and how they are read and written. Vectors: runs of eight, whose
 // type the kernel knows. Elements: each on its own, neighbouring threads side by side, of types that the launch knows;
-// for rows that are no whole number of vectors or start off a 16-byte boundary, and rare mixtures of types.
+// for rows that are no whole number of vectors or start off a 16-byte boundary, and all other mixtures of types (2048 f32 rows of 4096
+// with f32 weights 26.5 us, with bf16 ones or a bf16 normed 36; 8192 bf16 rows of 4096 48, of 4098 390).
 template <int kType>
 struct InVectors {
   static constexpr bool kEach = false;
